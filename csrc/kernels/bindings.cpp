@@ -853,6 +853,211 @@ void sample_rows(const Tensor& logits, int64_t vocab, int64_t rows, const Tensor
   rc(zs_sample(&a, stream()), "zs_sample");
 }
 
+namespace {
+
+void token_probs(const Tensor& logits, const Tensor& temperature, const OptT& top_k, const OptT& top_p,
+                 const Tensor& out) {
+  for (const Tensor* t : {&logits, &out})
+    TORCH_CHECK(t->is_cuda() && t->dim() == 2 && t->scalar_type() == at::kFloat && t->stride(1) == 1,
+                "logits and out must be f32 CUDA matrices with contiguous rows");
+  TORCH_CHECK(logits.sizes() == out.sizes(), "out must have the shape of logits");
+  const int64_t rows = logits.size(0);
+  check_cuda(temperature, "temperature");
+  check_opt(top_k, "top_k");
+  check_opt(top_p, "top_p");
+  TORCH_CHECK(temperature.scalar_type() == at::kFloat && temperature.numel() == rows, "temperature: f32 [rows]");
+  TORCH_CHECK(!top_k.has_value() || (top_k->scalar_type() == at::kInt && top_k->numel() == rows), "top_k: int32 [rows]");
+  TORCH_CHECK(!top_p.has_value() || (top_p->scalar_type() == at::kFloat && top_p->numel() == rows), "top_p: f32 [rows]");
+  if (rows == 0) return;
+  TokenProbsArgs a{};
+  a.logits = ptr<const float>(logits);
+  a.ld = rows > 1 ? logits.stride(0) : logits.size(1);
+  a.rows = (int)rows;
+  a.vocab = (int)logits.size(1);
+  a.temperature = ptr<const float>(temperature);
+  a.top_k = optptr<const int>(top_k);
+  a.top_p = optptr<const float>(top_p);
+  a.out = ptr<float>(out);
+  a.ld_out = rows > 1 ? out.stride(0) : out.size(1);
+  rc(zs_token_probs(&a, stream()), "zs_token_probs");
+}
+
+void draft_verify(const Tensor& target, const OptT& draft_probs, const Tensor& drafts, const OptT& counts,
+                  const Tensor& uniform, const Tensor& record, const OptT& err) {
+  TORCH_CHECK(target.is_cuda() && target.dim() == 3 && target.scalar_type() == at::kFloat && target.stride(2) == 1,
+              "target must be f32 CUDA [n, k + 1, vocab] with contiguous rows");
+  const int64_t n = target.size(0), k = target.size(1) - 1, vocab = target.size(2);
+  check_cuda(drafts, "drafts");
+  check_cuda(uniform, "uniform");
+  check_cuda(record, "record");
+  check_opt(counts, "counts");
+  check_opt(err, "err");
+  TORCH_CHECK(drafts.scalar_type() == at::kInt && drafts.dim() == 2 && drafts.size(0) == n && drafts.size(1) == k,
+              "drafts: int32 [n, k]");
+  TORCH_CHECK(uniform.scalar_type() == at::kFloat && uniform.dim() == 2 && uniform.size(0) == n && uniform.size(1) == k + 1,
+              "uniform: f32 [n, k + 1]");
+  TORCH_CHECK(record.scalar_type() == at::kInt && record.numel() >= n * (k + 2), "record: int32 [n, k + 2]");
+  TORCH_CHECK(!counts.has_value() || (counts->scalar_type() == at::kInt && counts->numel() == n), "counts: int32 [n]");
+  TORCH_CHECK(!err.has_value() || err->scalar_type() == at::kInt, "err: int32");
+  DraftVerifyArgs a{};
+  if (draft_probs.has_value()) {
+    TORCH_CHECK(draft_probs->is_cuda() && draft_probs->dim() == 3 && draft_probs->scalar_type() == at::kFloat &&
+                    draft_probs->size(0) == n && draft_probs->size(1) == k && draft_probs->size(2) == vocab &&
+                    draft_probs->stride(2) == 1,
+                "draft_probs must be f32 CUDA [n, k, vocab] with contiguous rows");
+    a.draft_probs = ptr<const float>(*draft_probs);
+    a.draft_seq = draft_probs->stride(0);
+    a.draft_row = draft_probs->stride(1);
+  }
+  a.n = (int)n;
+  a.k = (int)k;
+  a.vocab = (int)vocab;
+  a.target = ptr<const float>(target);
+  a.target_seq = target.stride(0);
+  a.target_row = target.stride(1);
+  a.drafts = ptr<const int>(drafts);
+  a.counts = optptr<const int>(counts);
+  a.uniform = ptr<const float>(uniform);
+  a.record = ptr<int>(record);
+  a.err = optptr<int>(err);
+  rc(zs_draft_verify(&a, stream()), "zs_draft_verify");
+}
+
+void shared_attn(const Tensor& q, const OptT& gate, int64_t num_kv_heads, const Tensor& k_cache, const Tensor& v_cache,
+                 const Tensor& page_table, const Tensor& row_slot, const Tensor& seq_lens, int64_t levels,
+                 const Tensor& seg_start, const Tensor& seg_rows, const Tensor& seg_page0, const Tensor& seg_page1,
+                 const Tensor& entry_seg, const Tensor& row_entry, const Tensor& partial, double sm_scale,
+                 const OptT& out_bf16, const OptT& out_q, const OptT& out_sf, const OptT& err) {
+  check_cuda(q, "q");
+  TORCH_CHECK(q.dim() == 3 && q.scalar_type() == at::kBFloat16 && q.size(2) == 256, "q must be bf16 [rows, heads, 256]");
+  const int64_t rows = q.size(0), hq = q.size(1);
+  check_opt(gate, "gate");
+  TORCH_CHECK(!gate.has_value() || (gate->sizes() == q.sizes() && gate->scalar_type() == at::kBFloat16),
+              "gate must have the shape and type of q");
+  for (const Tensor* t : {&k_cache, &v_cache}) {
+    check_cuda(*t, "cache");
+    TORCH_CHECK(t->dim() == 4 && t->scalar_type() == at::kBFloat16 && t->size(1) == num_kv_heads && t->size(2) == 16 &&
+                    t->size(3) == 256,
+                "caches must be bf16 [pages, kv_heads, 16, 256]");
+  }
+  TORCH_CHECK(k_cache.sizes() == v_cache.sizes(), "k_cache and v_cache must have one shape");
+  for (const Tensor* t : {&page_table, &row_slot, &seq_lens, &seg_start, &seg_rows, &seg_page0, &seg_page1, &entry_seg,
+                          &row_entry}) {
+    check_cuda(*t, "index tensor");
+    TORCH_CHECK(t->scalar_type() == at::kInt, "index tensors must be int32");
+  }
+  check_cuda(partial, "partial");
+  TORCH_CHECK(page_table.dim() == 2, "page_table must be [slots, max_pages]");
+  TORCH_CHECK(row_slot.numel() == rows && seq_lens.numel() >= rows && row_entry.numel() == rows * levels,
+              "row_slot, seq_lens and row_entry must cover the rows");
+  TORCH_CHECK(partial.scalar_type() == at::kFloat && partial.numel() >= seg_rows.numel() * hq * 260, "partial too small");
+  SharedAttnArgs a{};
+  a.q = ptr(q);
+  a.gate = optptr(gate);
+  a.rows = (int)rows;
+  a.num_q_heads = (int)hq;
+  a.num_kv_heads = (int)num_kv_heads;
+  a.head_dim = 256;
+  a.page_size = 16;
+  a.k_cache = ptr(k_cache);
+  a.v_cache = ptr(v_cache);
+  a.num_pages = (int)k_cache.size(0);
+  a.page_table = ptr<const int>(page_table);
+  a.max_pages = (int)page_table.size(1);
+  a.row_slot = ptr<const int>(row_slot);
+  a.seq_lens = ptr<const int>(seq_lens);
+  a.num_segs = (int)seg_page0.numel();
+  a.entries = (int)seg_rows.numel();
+  a.levels = (int)levels;
+  a.seg_start = ptr<const int>(seg_start);
+  a.seg_rows = ptr<const int>(seg_rows);
+  a.seg_page0 = ptr<const int>(seg_page0);
+  a.seg_page1 = ptr<const int>(seg_page1);
+  a.entry_seg = ptr<const int>(entry_seg);
+  a.row_entry = ptr<const int>(row_entry);
+  a.partial = ptr<float>(partial);
+  a.sm_scale = (float)sm_scale;
+  check_opt(out_bf16, "out");
+  TORCH_CHECK(!out_bf16.has_value() || (out_bf16->scalar_type() == at::kBFloat16 && out_bf16->numel() >= rows * hq * 256),
+              "out must be bf16 [rows, heads * 256]");
+  TORCH_CHECK(out_q.has_value() == out_sf.has_value(), "the MXFP8 output needs out_q and out_sf");
+  if (out_q.has_value()) {
+    check_cuda(*out_q, "out_q");
+    check_cuda(*out_sf, "out_sf");
+    TORCH_CHECK(out_q->numel() >= rows * hq * 256 && out_sf->numel() >= (rows + 127) / 128 * (hq * 2) * 512,
+                "MXFP8 output too small");
+  }
+  a.out_bf16 = optptr(out_bf16);
+  a.out_q = optptr<uint8_t>(out_q);
+  a.out_sf = optptr<uint8_t>(out_sf);
+  a.err = optptr<int>(err);
+  rc(zs_shared_attn(&a, stream()), "zs_shared_attn");
+}
+
+// Page pool: `which` = 0 fork, 1 extend, 2 truncate, 3 compact, 4 copy.
+void pool_call(int64_t which, const Tensor& refcount, const Tensor& free_bits, const Tensor& seq_len,
+               const Tensor& page_table, int64_t page_size, const std::vector<Tensor>& caches, const OptT& slots,
+               const OptT& parents, const OptT& lens, const Tensor& scratch, const Tensor& err) {
+  for (const Tensor* t : {&refcount, &free_bits, &seq_len, &page_table, &scratch, &err}) {
+    check_cuda(*t, "pool state");
+    TORCH_CHECK(t->scalar_type() == at::kInt, "pool state: int32 tensors");
+  }
+  const int64_t pages = refcount.numel(), num_slots = seq_len.numel();
+  TORCH_CHECK(page_table.dim() == 2 && page_table.size(0) == num_slots, "page_table must be [slots, max_pages]");
+  TORCH_CHECK(free_bits.numel() >= (pages + 31) / 32, "free_bits too small");
+  TORCH_CHECK(scratch.numel() >= zs_pool_scratch_ints((int)pages, (int)num_slots), "pool scratch too small");
+  TORCH_CHECK(caches.size() <= ZS_POOL_MAX_CACHES, "at most ", ZS_POOL_MAX_CACHES, " caches");
+  PagePoolArgs a{};
+  a.refcount = ptr<int>(refcount);
+  a.free_bits = ptr<uint32_t>(free_bits);
+  a.seq_len = ptr<int>(seq_len);
+  a.page_table = ptr<int>(page_table);
+  a.num_pages = (int)pages;
+  a.num_slots = (int)num_slots;
+  a.max_pages = (int)page_table.size(1);
+  a.page_size = (int)page_size;
+  a.num_caches = (int)caches.size();
+  for (size_t c = 0; c < caches.size(); ++c) {
+    check_cuda(caches[c], "cache");
+    TORCH_CHECK(caches[c].dim() >= 2 && caches[c].size(1) == pages && caches[c].size(0) >= 1,
+                "cache must be [layers, pages, ...]");
+    a.cache[c] = ptr(caches[c]);
+    a.cache_layers[c] = (int)caches[c].size(0);
+    a.cache_page_bytes[c] = caches[c].numel() / (caches[c].size(0) * pages) * caches[c].element_size();
+    TORCH_CHECK(a.cache_page_bytes[c] % 16 == 0 && a.cache_page_bytes[c] > 0, "a cache page must be a multiple of 16 bytes");
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(a.cache[c]) % 16 == 0, "caches must be 16-byte aligned");
+  }
+  int64_t n = -1;
+  for (const OptT* t : {&slots, &parents, &lens}) {
+    if (!t->has_value()) continue;
+    check_cuda(**t, "pool request");
+    TORCH_CHECK((*t)->scalar_type() == at::kInt && (*t)->dim() == 1, "pool requests: int32 vectors");
+    TORCH_CHECK(n < 0 || (*t)->numel() == n, "pool requests must have one length");
+    n = (*t)->numel();
+  }
+  a.n = n < 0 ? 0 : (int)n;
+  TORCH_CHECK(which > 1 || a.n <= num_slots, "more requests than slots");
+  a.slots = optptr<const int>(slots);
+  a.parents = optptr<const int>(parents);
+  a.lens = optptr<const int>(lens);
+  a.scratch = ptr<int>(scratch);
+  a.err = ptr<int>(err);
+  switch (which) {
+    case 0: rc(zs_pool_fork(&a, stream()), "zs_pool_fork"); break;
+    case 1: rc(zs_pool_extend(&a, stream()), "zs_pool_extend"); break;
+    case 2: rc(zs_pool_truncate(&a, stream()), "zs_pool_truncate"); break;
+    case 3: rc(zs_pool_compact(&a, stream()), "zs_pool_compact"); break;
+    case 4:
+      a.copy_src = optptr<const int>(slots);
+      a.copy_dst = optptr<const int>(parents);
+      rc(zs_pool_copy(&a, stream()), "zs_pool_copy");
+      break;
+    default: TORCH_CHECK(false, "unknown pool call ", which);
+  }
+}
+
+}  // namespace
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sample", &sample_rows, py::arg("logits"), py::arg("vocab"), py::arg("rows"), py::arg("temperature"),
         py::arg("top_k"), py::arg("top_p"), py::arg("presence"), py::arg("frequency"), py::arg("repetition"),
@@ -923,6 +1128,19 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("push_mode") = 1, py::arg("last_m0") = 0, py::arg("last_mt") = 0);
   m.def("quant_mxf8", &quant_mxf8);
   m.def("spec_verify", &spec_verify);
+  m.def("token_probs", &token_probs, py::arg("logits"), py::arg("temperature"), py::arg("top_k"), py::arg("top_p"),
+        py::arg("out"));
+  m.def("draft_verify", &draft_verify, py::arg("target"), py::arg("draft_probs"), py::arg("drafts"), py::arg("counts"),
+        py::arg("uniform"), py::arg("record"), py::arg("err"));
+  m.def("shared_attn", &shared_attn, py::arg("q"), py::arg("gate"), py::arg("num_kv_heads"), py::arg("k_cache"),
+        py::arg("v_cache"), py::arg("page_table"), py::arg("row_slot"), py::arg("seq_lens"), py::arg("levels"),
+        py::arg("seg_start"), py::arg("seg_rows"), py::arg("seg_page0"), py::arg("seg_page1"), py::arg("entry_seg"),
+        py::arg("row_entry"), py::arg("partial"), py::arg("sm_scale"), py::arg("out_bf16") = py::none(),
+        py::arg("out_q") = py::none(), py::arg("out_sf") = py::none(), py::arg("err") = py::none());
+  m.def("pool_call", &pool_call, py::arg("which"), py::arg("refcount"), py::arg("free_bits"), py::arg("seq_len"),
+        py::arg("page_table"), py::arg("page_size"), py::arg("caches"), py::arg("slots") = py::none(),
+        py::arg("parents") = py::none(), py::arg("lens") = py::none(), py::arg("scratch"), py::arg("err"));
+  m.def("pool_scratch_ints", [](int64_t pages, int64_t slots) { return zs_pool_scratch_ints((int)pages, (int)slots); });
   m.def("add_rmsnorm_quant", &add_rmsnorm_quant, py::arg("residual"), py::arg("delta"), py::arg("n_terms"),
         py::arg("d_row_stride"), py::arg("d_term_stride"), py::arg("weight"), py::arg("w_offset"), py::arg("eps"),
         py::arg("rows"), py::arg("normed"), py::arg("q"), py::arg("sf"), py::arg("term_index") = py::none(),

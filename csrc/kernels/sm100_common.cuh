@@ -30,6 +30,7 @@ enum ErrorCode : int {
   kErrBadShape = 3,        // a kernel saw an argument outside its contract
   kErrDrainTimeout = 4,    // teardown could not drain in-flight copies in time
   kErrAbort = 5,           // host-set abort word observed
+  kErrNoPages = 6,         // a page pool had fewer free pages than a call needed
 };
 
 ZS_DEVICE void report_error(int* err, int code) {

@@ -593,6 +593,108 @@ typedef struct SpecVerifyArgs {
 
 int zs_spec_verify(const SpecVerifyArgs* args, cudaStream_t stream);
 
+// ----------------------------------------------------------------------------------
+// Page pool of a paged cache, on the device (pages.cu)
+// ----------------------------------------------------------------------------------
+#define ZS_POOL_MAX_CACHES 8
+
+typedef struct PagePoolArgs {
+  int* refcount;             // [num_pages] references per page (page 0, the padding page, keeps one)
+  uint32_t* free_bits;       // [ceil(num_pages / 32)] bit = 1: the page is free
+  int* seq_len;              // [num_slots] tokens of each slot (0: the slot is empty)
+  int* page_table;           // [num_slots, max_pages]; entries past a slot's pages are 0
+  int num_pages, num_slots, max_pages, page_size;
+  int num_caches;            // caches [layers, num_pages, page bytes], 16-byte aligned, contiguous
+  void* cache[ZS_POOL_MAX_CACHES];
+  int cache_layers[ZS_POOL_MAX_CACHES];
+  long long cache_page_bytes[ZS_POOL_MAX_CACHES];  // of one layer, a multiple of 16
+  int n;                     // requests of this call
+  const int* slots;          // [n] slots to fill / grow / cut (distinct for fork and extend)
+  const int* parents;        // [n] fork: where the tokens come from
+  const int* lens;           // [n] fork: tokens to share at most (NULL: all); extend, truncate: new length
+                             // (truncate: NULL = 0)
+  const int* copy_src;       // [n] zs_pool_copy
+  const int* copy_dst;
+  int* scratch;              // zs_pool_scratch_ints ints, zeroed once at allocation
+  int* err;                  // kErrBadShape: a bad request; kErrNoPages: too few free pages.  A fork or
+                             // extend with either changes nothing
+} PagePoolArgs;
+
+long long zs_pool_scratch_ints(int num_pages, int num_slots);
+int zs_pool_fork(const PagePoolArgs* args, cudaStream_t stream);
+int zs_pool_extend(const PagePoolArgs* args, cudaStream_t stream);
+int zs_pool_truncate(const PagePoolArgs* args, cudaStream_t stream);
+int zs_pool_compact(const PagePoolArgs* args, cudaStream_t stream);
+int zs_pool_copy(const PagePoolArgs* args, cudaStream_t stream);
+
+// ----------------------------------------------------------------------------------
+// Token probabilities and verification of drafted tokens (spec_sampling.cu)
+// ----------------------------------------------------------------------------------
+typedef struct TokenProbsArgs {
+  const float* logits;       // [rows, ld]; -inf and NaN: masked
+  long long ld;
+  int rows, vocab;
+  const float* temperature;  // [rows]; <= 0: all mass on the largest logit (lowest id on ties)
+  const int* top_k;          // [rows] (may be NULL); 0: off
+  const float* top_p;        // [rows] (may be NULL); >= 1: off
+  float* out;                // [rows, ld_out]; a row whose logits are all masked gives zeros
+  long long ld_out;
+} TokenProbsArgs;
+
+int zs_token_probs(const TokenProbsArgs* args, cudaStream_t stream);
+
+#define ZS_VERIFY_MAX_DRAFTS 64
+
+typedef struct DraftVerifyArgs {
+  int n, k, vocab;
+  const float* target;       // probabilities after row j of sequence s: target + s * target_seq + j * target_row, j <= k
+  long long target_seq, target_row;
+  const float* draft_probs;  // what draft j was drawn from (may be NULL: the drafts were certain)
+  long long draft_seq, draft_row;
+  const int* drafts;         // [n, k]
+  const int* counts;         // [n] drafts of each sequence, clamped to [0, k] (may be NULL: k)
+  const float* uniform;      // [n, k + 1] in [0, 1): one per draft, and one for the drawn token
+  int* record;               // [n, k + 2]: accepted drafts + 1, then those tokens and the drawn one, -1 after
+  int* err;                  // kErrBadShape: a row to draw from had no mass (token 0 stands there)
+} DraftVerifyArgs;
+
+int zs_draft_verify(const DraftVerifyArgs* args, cudaStream_t stream);
+
+// ----------------------------------------------------------------------------------
+// Gated GQA attention of rows that share leading pages (shared_attn.cu)
+// ----------------------------------------------------------------------------------
+#define ZS_SHARED_MAX_GROUP 64  // q heads per kv head
+
+typedef struct SharedAttnArgs {
+  const void* q;             // bf16 [rows, num_q_heads, 256] (normed + roped)
+  const void* gate;          // bf16 [rows, num_q_heads, 256] (may be NULL: no gate)
+  int rows, num_q_heads, num_kv_heads, head_dim, page_size;
+  const void* k_cache;       // bf16 [num_pages, kv_heads, 16 x 256] pre-swizzled blocks
+  const void* v_cache;
+  int num_pages;
+  const int* page_table;     // [slots, max_pages]
+  int max_pages;
+  const int* row_slot;       // [rows]
+  const int* seq_lens;       // [rows] keys visible to each row (0: none)
+  // Segments: rows and the page positions [page0, page1) that they share (-1: to the end of the
+  // longest row).  A row is in at most `levels` segments, of disjoint ranges.
+  int num_segs, entries, levels;
+  const int* seg_start;      // [num_segs + 1] entry ranges
+  const int* seg_rows;       // [entries]
+  const int* seg_page0;      // [num_segs]
+  const int* seg_page1;
+  const int* entry_seg;      // [entries]
+  const int* row_entry;      // [rows, levels] entry of each row's segments, -1: none
+  float* partial;            // scratch
+  float sm_scale;
+  void* out_bf16;            // optional [rows, num_q_heads * 256]
+  uint8_t* out_q;            // optional MXFP8 output + scale atoms
+  uint8_t* out_sf;
+  int* err;
+} SharedAttnArgs;
+
+int zs_shared_attn(const SharedAttnArgs* args, cudaStream_t stream);
+
 // Programmatic dependent launch of the compute kernels (on by default).
 void zs_set_pdl(int on);
 int zs_pdl_enabled();

@@ -1,0 +1,114 @@
+"""Attention of rows whose sequences share leading pages of the paged cache.
+
+A ``SharedPrefixPlan`` holds which rows share which page positions.  It changes only with the
+batch: while sequences grow, ``update(seq_lens)`` (once a step) and ``attend`` (once a layer)
+run on the device alone, so a step can be captured in a CUDA graph.  The pages of a segment are
+read once for all its rows instead of once per row.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _ext
+
+MAX_GROUP = 64   # q heads per kv head
+RECORD = 260     # floats of a partial record
+
+
+class SharedPrefixPlan:
+    def __init__(self, slots: list[int], segments: list[tuple[list[int], int, int | None]], num_q_heads: int,
+                 num_kv_heads: int, device="cuda"):
+        """``slots``: page-table row of each query row.  ``segments``: (rows, first page position,
+        end page position); the pages [first, end) of those rows' tables are the same, and an end
+        of None means up to each row's own length.  The segments of a row must follow one another
+        from position 0 to None."""
+        rows = len(slots)
+        if num_kv_heads < 1 or num_q_heads < 1 or num_q_heads % num_kv_heads or num_q_heads // num_kv_heads > MAX_GROUP:
+            raise ValueError(f"need 1..{MAX_GROUP} q heads per kv head, got {num_q_heads} / {num_kv_heads}")
+        if any(s < 0 for s in slots):
+            raise ValueError("slots must not be negative")
+        order = sorted(range(len(segments)), key=lambda i: segments[i][1])  # a row's segments by position
+        row_entry: list[list[int]] = [[] for _ in range(rows)]
+        reach: list[int | None] = [0] * rows
+        starts, seg_rows, entry_seg = [0], [], []
+        for s, i in enumerate(order):
+            members, first, end = segments[i]
+            if not members:
+                raise ValueError("a segment needs rows")
+            if end is not None and end <= first:
+                raise ValueError(f"segment [{first}, {end}) is empty")
+            for r in members:
+                if not 0 <= r < rows:
+                    raise ValueError(f"row {r} outside the {rows} rows")
+                if reach[r] is None or reach[r] != first:
+                    raise ValueError(f"the segments of row {r} must follow one another from position 0")
+                reach[r] = end
+                row_entry[r].append(len(seg_rows))
+                seg_rows.append(r)
+                entry_seg.append(s)
+            starts.append(len(seg_rows))
+        if any(x is not None for x in reach):
+            raise ValueError("the last segment of every row must end at None")
+        self.C = _ext.load()
+        self.rows, self.num_q_heads, self.num_kv_heads = rows, num_q_heads, num_kv_heads
+        self.device = torch.device(device)
+        self.max_slot = max(slots, default=0)
+        self.levels = max((len(e) for e in row_entry), default=1)
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+        self.slots = i32(slots)
+        self.seg_start, self.seg_rows, self.entry_seg = i32(starts), i32(seg_rows), i32(entry_seg)
+        self.seg_page0 = i32([segments[i][1] for i in order])
+        self.seg_page1 = i32([-1 if segments[i][2] is None else segments[i][2] for i in order])
+        self.row_entry = i32([x for e in row_entry for x in e + [-1] * (self.levels - len(e))])
+        self.err = torch.zeros(1, dtype=torch.int32, device=device)
+        self.partial = torch.empty(len(seg_rows) * num_q_heads * RECORD, dtype=torch.float32, device=device)
+
+    @classmethod
+    def from_prefixes(cls, slots: list[int], prefixes: list[tuple[list[int], int]], num_q_heads: int, num_kv_heads: int,
+                      device="cuda") -> "SharedPrefixPlan":
+        """Plan of rows in groups with a common prompt: (rows, whole pages that they share).  Behind
+        its prefix every sequence (rows of one slot) has pages of its own; rows in no group share
+        nothing."""
+        first = {}
+        segments: list[tuple[list[int], int, int | None]] = []
+        for members, pages in prefixes:
+            for r in members:
+                if r in first:
+                    raise ValueError(f"row {r} is in two groups")
+                first[r] = pages
+            if pages > 0 and members:
+                segments.append((list(members), 0, pages))
+        own: dict[tuple[int, int], list[int]] = {}
+        for r, s in enumerate(slots):
+            own.setdefault((s, first.get(r, 0)), []).append(r)
+        segments += [(members, pages, None) for (_, pages), members in own.items()]
+        return cls(slots, segments, num_q_heads, num_kv_heads, device)
+
+    def update(self, seq_lens: torch.Tensor) -> None:
+        """Divide the step's keys over the GPU: ``seq_lens`` [rows] int32, the keys each row sees."""
+
+    def attend(self, q: torch.Tensor, gate: torch.Tensor | None, k_cache: torch.Tensor, v_cache: torch.Tensor,
+               page_table: torch.Tensor, seq_lens: torch.Tensor, sm_scale: float, out: torch.Tensor | None = None,
+               out_q: torch.Tensor | None = None, out_sf: torch.Tensor | None = None) -> torch.Tensor | None:
+        """sigmoid(gate) * attention of ``q`` [rows, heads, 256] (bf16) over its sequences' pages;
+        ``gate`` None: no gate.  The result goes to ``out`` (bf16 [rows, heads * 256], allocated
+        unless the MXFP8 pair ``out_q``, ``out_sf`` is given alone).  ``seq_lens`` must be what the
+        last ``update`` got; a row of length 0 gives 0."""
+        if q.dim() != 3 or q.shape[0] != self.rows or q.shape[1] != self.num_q_heads:
+            raise ValueError(f"q must be [{self.rows}, {self.num_q_heads}, 256], got {tuple(q.shape)}")
+        if page_table.dim() != 2 or page_table.shape[0] <= self.max_slot:
+            raise ValueError(f"page_table must have more than {self.max_slot} rows")
+        if out is None and out_q is None:
+            out = torch.empty(self.rows, self.num_q_heads * 256, dtype=torch.bfloat16, device=q.device)
+        self.C.shared_attn(q, gate, self.num_kv_heads, k_cache, v_cache, page_table, self.slots, seq_lens, self.levels,
+                           self.seg_start, self.seg_rows, self.seg_page0, self.seg_page1, self.entry_seg,
+                           self.row_entry, self.partial, sm_scale, out, out_q, out_sf, self.err)
+        return out
+
+    def check(self) -> None:
+        """Raise if a call since the last check met a page or length outside the cache (reads the error word)."""
+        code = int(self.err.item())
+        if code:
+            self.err.zero_()
+            raise RuntimeError(f"shared-prefix attention: kernel error status {code}")
