@@ -923,11 +923,55 @@ void draft_verify(const Tensor& target, const OptT& draft_probs, const Tensor& d
   rc(zs_draft_verify(&a, stream()), "zs_draft_verify");
 }
 
+// The plan's side of the shared-prefix attention arguments.
+SharedAttnArgs shared_plan_args(int64_t rows, int64_t num_q_heads, int64_t num_kv_heads, int64_t max_pages,
+                                const Tensor& row_slot, const Tensor& seq_lens, int64_t levels,
+                                const std::vector<Tensor>& segs, const Tensor& work, const Tensor& err) {
+  TORCH_CHECK(segs.size() == 6, "segments: seg_start, seg_rows, seg_page0, seg_page1, entry_seg, row_entry");
+  for (const Tensor* t : {&row_slot, &seq_lens, &segs[0], &segs[1], &segs[2], &segs[3], &segs[4], &segs[5], &work, &err}) {
+    check_cuda(*t, "index tensor");
+    TORCH_CHECK(t->scalar_type() == at::kInt, "index tensors must be int32");
+  }
+  TORCH_CHECK(row_slot.numel() == rows && seq_lens.numel() == rows && segs[5].numel() == rows * levels,
+              "row_slot, seq_lens and row_entry must have one entry per row");
+  const int64_t num_segs = segs[2].numel();
+  TORCH_CHECK(segs[0].numel() == num_segs + 1 && segs[3].numel() == num_segs && segs[4].numel() == segs[1].numel(),
+              "segment tensors do not fit together");
+  TORCH_CHECK(work.numel() >= ZS_SHARED_WORK_INTS(num_segs), "work too small");
+  SharedAttnArgs a{};
+  a.rows = (int)rows;
+  a.num_q_heads = (int)num_q_heads;
+  a.num_kv_heads = (int)num_kv_heads;
+  a.head_dim = 256;
+  a.page_size = 16;
+  a.max_pages = (int)max_pages;
+  a.row_slot = ptr<const int>(row_slot);
+  a.seq_lens = ptr<const int>(seq_lens);
+  a.num_segs = (int)num_segs;
+  a.entries = (int)segs[1].numel();
+  a.levels = (int)levels;
+  a.seg_start = ptr<const int>(segs[0]);
+  a.seg_rows = ptr<const int>(segs[1]);
+  a.seg_page0 = ptr<const int>(segs[2]);
+  a.seg_page1 = ptr<const int>(segs[3]);
+  a.entry_seg = ptr<const int>(segs[4]);
+  a.row_entry = ptr<const int>(segs[5]);
+  a.work = ptr<int>(work);
+  a.err = ptr<int>(err);
+  return a;
+}
+
+void shared_attn_plan(int64_t num_q_heads, int64_t num_kv_heads, const Tensor& row_slot, const Tensor& seq_lens,
+                      int64_t levels, const std::vector<Tensor>& segs, const Tensor& work, const Tensor& err) {
+  SharedAttnArgs a = shared_plan_args(row_slot.numel(), num_q_heads, num_kv_heads, 1, row_slot, seq_lens, levels, segs,
+                                      work, err);
+  rc(zs_shared_attn_plan(&a, stream()), "zs_shared_attn_plan");
+}
+
 void shared_attn(const Tensor& q, const OptT& gate, int64_t num_kv_heads, const Tensor& k_cache, const Tensor& v_cache,
                  const Tensor& page_table, const Tensor& row_slot, const Tensor& seq_lens, int64_t levels,
-                 const Tensor& seg_start, const Tensor& seg_rows, const Tensor& seg_page0, const Tensor& seg_page1,
-                 const Tensor& entry_seg, const Tensor& row_entry, const Tensor& partial, double sm_scale,
-                 const OptT& out_bf16, const OptT& out_q, const OptT& out_sf, const OptT& err) {
+                 const std::vector<Tensor>& segs, const Tensor& work, const Tensor& partial, double sm_scale,
+                 const OptT& out_bf16, const OptT& out_q, const OptT& out_sf, const Tensor& err) {
   check_cuda(q, "q");
   TORCH_CHECK(q.dim() == 3 && q.scalar_type() == at::kBFloat16 && q.size(2) == 256, "q must be bf16 [rows, heads, 256]");
   const int64_t rows = q.size(0), hq = q.size(1);
@@ -939,42 +983,23 @@ void shared_attn(const Tensor& q, const OptT& gate, int64_t num_kv_heads, const 
     TORCH_CHECK(t->dim() == 4 && t->scalar_type() == at::kBFloat16 && t->size(1) == num_kv_heads && t->size(2) == 16 &&
                     t->size(3) == 256,
                 "caches must be bf16 [pages, kv_heads, 16, 256]");
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, "caches must be 16-byte aligned");
   }
   TORCH_CHECK(k_cache.sizes() == v_cache.sizes(), "k_cache and v_cache must have one shape");
-  for (const Tensor* t : {&page_table, &row_slot, &seq_lens, &seg_start, &seg_rows, &seg_page0, &seg_page1, &entry_seg,
-                          &row_entry}) {
-    check_cuda(*t, "index tensor");
-    TORCH_CHECK(t->scalar_type() == at::kInt, "index tensors must be int32");
-  }
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0, "q must be 16-byte aligned");
+  check_cuda(page_table, "page_table");
+  TORCH_CHECK(page_table.dim() == 2 && page_table.scalar_type() == at::kInt, "page_table must be int32 [slots, max_pages]");
+  SharedAttnArgs a = shared_plan_args(rows, hq, num_kv_heads, page_table.size(1), row_slot, seq_lens, levels, segs, work, err);
   check_cuda(partial, "partial");
-  TORCH_CHECK(page_table.dim() == 2, "page_table must be [slots, max_pages]");
-  TORCH_CHECK(row_slot.numel() == rows && seq_lens.numel() >= rows && row_entry.numel() == rows * levels,
-              "row_slot, seq_lens and row_entry must cover the rows");
-  TORCH_CHECK(partial.scalar_type() == at::kFloat && partial.numel() >= seg_rows.numel() * hq * 260, "partial too small");
-  SharedAttnArgs a{};
+  TORCH_CHECK(partial.scalar_type() == at::kFloat &&
+                  partial.numel() >= (segs[1].numel() * hq + ZS_SHARED_CTAS * ZS_SHARED_SLOTS) * 260,
+              "partial too small");
   a.q = ptr(q);
   a.gate = optptr(gate);
-  a.rows = (int)rows;
-  a.num_q_heads = (int)hq;
-  a.num_kv_heads = (int)num_kv_heads;
-  a.head_dim = 256;
-  a.page_size = 16;
   a.k_cache = ptr(k_cache);
   a.v_cache = ptr(v_cache);
   a.num_pages = (int)k_cache.size(0);
   a.page_table = ptr<const int>(page_table);
-  a.max_pages = (int)page_table.size(1);
-  a.row_slot = ptr<const int>(row_slot);
-  a.seq_lens = ptr<const int>(seq_lens);
-  a.num_segs = (int)seg_page0.numel();
-  a.entries = (int)seg_rows.numel();
-  a.levels = (int)levels;
-  a.seg_start = ptr<const int>(seg_start);
-  a.seg_rows = ptr<const int>(seg_rows);
-  a.seg_page0 = ptr<const int>(seg_page0);
-  a.seg_page1 = ptr<const int>(seg_page1);
-  a.entry_seg = ptr<const int>(entry_seg);
-  a.row_entry = ptr<const int>(row_entry);
   a.partial = ptr<float>(partial);
   a.sm_scale = (float)sm_scale;
   check_opt(out_bf16, "out");
@@ -984,13 +1009,13 @@ void shared_attn(const Tensor& q, const OptT& gate, int64_t num_kv_heads, const 
   if (out_q.has_value()) {
     check_cuda(*out_q, "out_q");
     check_cuda(*out_sf, "out_sf");
-    TORCH_CHECK(out_q->numel() >= rows * hq * 256 && out_sf->numel() >= (rows + 127) / 128 * (hq * 2) * 512,
+    TORCH_CHECK(out_q->element_size() == 1 && out_sf->element_size() == 1 && out_q->numel() >= rows * hq * 256 &&
+                    out_sf->numel() >= (rows + 127) / 128 * (hq * 2) * 512,
                 "MXFP8 output too small");
   }
   a.out_bf16 = optptr(out_bf16);
   a.out_q = optptr<uint8_t>(out_q);
   a.out_sf = optptr<uint8_t>(out_sf);
-  a.err = optptr<int>(err);
   rc(zs_shared_attn(&a, stream()), "zs_shared_attn");
 }
 
@@ -1132,11 +1157,17 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("out"));
   m.def("draft_verify", &draft_verify, py::arg("target"), py::arg("draft_probs"), py::arg("drafts"), py::arg("counts"),
         py::arg("uniform"), py::arg("record"), py::arg("err"));
+  m.attr("SHARED_MAX_GROUP") = ZS_SHARED_MAX_GROUP;
+  m.attr("SHARED_MAX_SEGS") = ZS_SHARED_MAX_SEGS;
+  m.def("shared_attn_sizes", [](int64_t segs, int64_t entries, int64_t heads) {
+    return std::make_pair((int64_t)ZS_SHARED_WORK_INTS(segs), (entries * heads + ZS_SHARED_CTAS * ZS_SHARED_SLOTS) * 260);
+  });
+  m.def("shared_attn_plan", &shared_attn_plan, py::arg("num_q_heads"), py::arg("num_kv_heads"), py::arg("row_slot"),
+        py::arg("seq_lens"), py::arg("levels"), py::arg("segs"), py::arg("work"), py::arg("err"));
   m.def("shared_attn", &shared_attn, py::arg("q"), py::arg("gate"), py::arg("num_kv_heads"), py::arg("k_cache"),
         py::arg("v_cache"), py::arg("page_table"), py::arg("row_slot"), py::arg("seq_lens"), py::arg("levels"),
-        py::arg("seg_start"), py::arg("seg_rows"), py::arg("seg_page0"), py::arg("seg_page1"), py::arg("entry_seg"),
-        py::arg("row_entry"), py::arg("partial"), py::arg("sm_scale"), py::arg("out_bf16") = py::none(),
-        py::arg("out_q") = py::none(), py::arg("out_sf") = py::none(), py::arg("err") = py::none());
+        py::arg("segs"), py::arg("work"), py::arg("partial"), py::arg("sm_scale"), py::arg("out_bf16"), py::arg("out_q"),
+        py::arg("out_sf"), py::arg("err"));
   m.def("pool_call", &pool_call, py::arg("which"), py::arg("refcount"), py::arg("free_bits"), py::arg("seq_len"),
         py::arg("page_table"), py::arg("page_size"), py::arg("caches"), py::arg("slots") = py::none(),
         py::arg("parents") = py::none(), py::arg("lens") = py::none(), py::arg("scratch"), py::arg("err"));

@@ -663,7 +663,10 @@ int zs_draft_verify(const DraftVerifyArgs* args, cudaStream_t stream);
 // ----------------------------------------------------------------------------------
 // Gated GQA attention of rows that share leading pages (shared_attn.cu)
 // ----------------------------------------------------------------------------------
-#define ZS_SHARED_MAX_GROUP 64  // q heads per kv head
+#define ZS_SHARED_MAX_GROUP 64    // q heads per kv head
+#define ZS_SHARED_MAX_SEGS 2048   // segments of a plan
+#define ZS_SHARED_SLOTS 128       // query slots (row x head of a GQA group) of a work unit
+#define ZS_SHARED_CTAS 148
 
 typedef struct SharedAttnArgs {
   const void* q;             // bf16 [rows, num_q_heads, 256] (normed + roped)
@@ -685,14 +688,20 @@ typedef struct SharedAttnArgs {
   const int* seg_page1;
   const int* entry_seg;      // [entries]
   const int* row_entry;      // [rows, levels] entry of each row's segments, -1: none
-  float* partial;            // scratch
-  float sm_scale;
+  int* work;                 // [ZS_SHARED_WORK_INTS(num_segs)] written by the plan
+  float* partial;            // scratch: 260 floats x (entries * num_q_heads + ZS_SHARED_CTAS * ZS_SHARED_SLOTS)
+  float sm_scale;            // > 0
   void* out_bf16;            // optional [rows, num_q_heads * 256]
   uint8_t* out_q;            // optional MXFP8 output + scale atoms
   uint8_t* out_sf;
   int* err;
 } SharedAttnArgs;
 
+#define ZS_SHARED_WORK_INTS(num_segs) (4 + 5 * (num_segs) + 1 + ZS_SHARED_CTAS)
+
+// Divide the step's keys over the GPU (from seq_lens, row_slot, the segments and the head counts;
+// q, caches and outputs are not read): once a step.  Then one zs_shared_attn per layer.
+int zs_shared_attn_plan(const SharedAttnArgs* args, cudaStream_t stream);
 int zs_shared_attn(const SharedAttnArgs* args, cudaStream_t stream);
 
 // Programmatic dependent launch of the compute kernels (on by default).

@@ -12,8 +12,8 @@ import torch
 
 from . import _ext
 
-MAX_GROUP = 64   # q heads per kv head
-RECORD = 260     # floats of a partial record
+MAX_GROUP = 64     # q heads per kv head
+MAX_SEGS = 2048    # segments of a plan
 
 
 class SharedPrefixPlan:
@@ -28,6 +28,8 @@ class SharedPrefixPlan:
             raise ValueError(f"need 1..{MAX_GROUP} q heads per kv head, got {num_q_heads} / {num_kv_heads}")
         if any(s < 0 for s in slots):
             raise ValueError("slots must not be negative")
+        if len(segments) > MAX_SEGS:
+            raise ValueError(f"at most {MAX_SEGS} segments, got {len(segments)}")
         order = sorted(range(len(segments)), key=lambda i: segments[i][1])  # a row's segments by position
         row_entry: list[list[int]] = [[] for _ in range(rows)]
         reach: list[int | None] = [0] * rows
@@ -57,12 +59,14 @@ class SharedPrefixPlan:
         self.levels = max((len(e) for e in row_entry), default=1)
         i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
         self.slots = i32(slots)
-        self.seg_start, self.seg_rows, self.entry_seg = i32(starts), i32(seg_rows), i32(entry_seg)
-        self.seg_page0 = i32([segments[i][1] for i in order])
-        self.seg_page1 = i32([-1 if segments[i][2] is None else segments[i][2] for i in order])
-        self.row_entry = i32([x for e in row_entry for x in e + [-1] * (self.levels - len(e))])
+        self._segs = [i32(starts), i32(seg_rows), i32([segments[i][1] for i in order]),
+                      i32([-1 if segments[i][2] is None else segments[i][2] for i in order]), i32(entry_seg),
+                      i32([x for e in row_entry for x in e + [-1] * (self.levels - len(e))])]
         self.err = torch.zeros(1, dtype=torch.int32, device=device)
-        self.partial = torch.empty(len(seg_rows) * num_q_heads * RECORD, dtype=torch.float32, device=device)
+        ints, floats = self.C.shared_attn_sizes(len(order), len(seg_rows), num_q_heads)
+        self._work = torch.zeros(ints, dtype=torch.int32, device=device)
+        self._partial = torch.empty(floats, dtype=torch.float32, device=device)
+        self._planned = False
 
     @classmethod
     def from_prefixes(cls, slots: list[int], prefixes: list[tuple[list[int], int]], num_q_heads: int, num_kv_heads: int,
@@ -86,7 +90,10 @@ class SharedPrefixPlan:
         return cls(slots, segments, num_q_heads, num_kv_heads, device)
 
     def update(self, seq_lens: torch.Tensor) -> None:
-        """Divide the step's keys over the GPU: ``seq_lens`` [rows] int32, the keys each row sees."""
+        """Divide a step's keys over the GPU: ``seq_lens`` [rows] int32, the keys each row sees."""
+        self.C.shared_attn_plan(self.num_q_heads, self.num_kv_heads, self.slots, seq_lens, self.levels, self._segs,
+                                self._work, self.err)
+        self._planned = True
 
     def attend(self, q: torch.Tensor, gate: torch.Tensor | None, k_cache: torch.Tensor, v_cache: torch.Tensor,
                page_table: torch.Tensor, seq_lens: torch.Tensor, sm_scale: float, out: torch.Tensor | None = None,
@@ -97,13 +104,14 @@ class SharedPrefixPlan:
         last ``update`` got; a row of length 0 gives 0."""
         if q.dim() != 3 or q.shape[0] != self.rows or q.shape[1] != self.num_q_heads:
             raise ValueError(f"q must be [{self.rows}, {self.num_q_heads}, 256], got {tuple(q.shape)}")
+        if not self._planned:
+            raise RuntimeError("attend needs an update first")
         if page_table.dim() != 2 or page_table.shape[0] <= self.max_slot:
             raise ValueError(f"page_table must have more than {self.max_slot} rows")
         if out is None and out_q is None:
             out = torch.empty(self.rows, self.num_q_heads * 256, dtype=torch.bfloat16, device=q.device)
         self.C.shared_attn(q, gate, self.num_kv_heads, k_cache, v_cache, page_table, self.slots, seq_lens, self.levels,
-                           self.seg_start, self.seg_rows, self.seg_page0, self.seg_page1, self.entry_seg,
-                           self.row_entry, self.partial, sm_scale, out, out_q, out_sf, self.err)
+                           self._segs, self._work, self._partial, sm_scale, out, out_q, out_sf, self.err)
         return out
 
     def check(self) -> None:
