@@ -937,7 +937,7 @@ SharedAttnArgs shared_plan_args(int64_t rows, int64_t num_q_heads, int64_t num_k
   const int64_t num_segs = segs[2].numel();
   TORCH_CHECK(segs[0].numel() == num_segs + 1 && segs[3].numel() == num_segs && segs[4].numel() == segs[1].numel(),
               "segment tensors do not fit together");
-  TORCH_CHECK(work.numel() >= ZS_SHARED_WORK_INTS(num_segs), "work too small");
+  TORCH_CHECK(work.numel() >= ZS_SHARED_WORK_INTS(num_segs, segs[1].numel()) && reinterpret_cast<uintptr_t>(work.data_ptr()) % 16 == 0, "work too small or not 16-byte aligned");
   SharedAttnArgs a{};
   a.rows = (int)rows;
   a.num_q_heads = (int)num_q_heads;
@@ -987,6 +987,7 @@ void shared_attn(const Tensor& q, const OptT& gate, int64_t num_kv_heads, const 
   }
   TORCH_CHECK(k_cache.sizes() == v_cache.sizes(), "k_cache and v_cache must have one shape");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0, "q must be 16-byte aligned");
+  TORCH_CHECK(!gate.has_value() || reinterpret_cast<uintptr_t>(gate->data_ptr()) % 8 == 0, "gate must be 8-byte aligned");
   check_cuda(page_table, "page_table");
   TORCH_CHECK(page_table.dim() == 2 && page_table.scalar_type() == at::kInt, "page_table must be int32 [slots, max_pages]");
   SharedAttnArgs a = shared_plan_args(rows, hq, num_kv_heads, page_table.size(1), row_slot, seq_lens, levels, segs, work, err);
@@ -1003,6 +1004,7 @@ void shared_attn(const Tensor& q, const OptT& gate, int64_t num_kv_heads, const 
   a.partial = ptr<float>(partial);
   a.sm_scale = (float)sm_scale;
   check_opt(out_bf16, "out");
+  TORCH_CHECK(!out_bf16.has_value() || reinterpret_cast<uintptr_t>(out_bf16->data_ptr()) % 8 == 0, "out must be 8-byte aligned");
   TORCH_CHECK(!out_bf16.has_value() || (out_bf16->scalar_type() == at::kBFloat16 && out_bf16->numel() >= rows * hq * 256),
               "out must be bf16 [rows, heads * 256]");
   TORCH_CHECK(out_q.has_value() == out_sf.has_value(), "the MXFP8 output needs out_q and out_sf");
@@ -1012,6 +1014,7 @@ void shared_attn(const Tensor& q, const OptT& gate, int64_t num_kv_heads, const 
     TORCH_CHECK(out_q->element_size() == 1 && out_sf->element_size() == 1 && out_q->numel() >= rows * hq * 256 &&
                     out_sf->numel() >= (rows + 127) / 128 * (hq * 2) * 512,
                 "MXFP8 output too small");
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(out_q->data_ptr()) % 4 == 0, "out_q must be 4-byte aligned");
   }
   a.out_bf16 = optptr(out_bf16);
   a.out_q = optptr<uint8_t>(out_q);
@@ -1160,7 +1163,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.attr("SHARED_MAX_GROUP") = ZS_SHARED_MAX_GROUP;
   m.attr("SHARED_MAX_SEGS") = ZS_SHARED_MAX_SEGS;
   m.def("shared_attn_sizes", [](int64_t segs, int64_t entries, int64_t heads) {
-    return std::make_pair((int64_t)ZS_SHARED_WORK_INTS(segs), (entries * heads + ZS_SHARED_CTAS * ZS_SHARED_SLOTS) * 260);
+    return std::make_pair((int64_t)ZS_SHARED_WORK_INTS(segs, entries), (entries * heads + ZS_SHARED_CTAS * ZS_SHARED_SLOTS) * 260);
   });
   m.def("shared_attn_plan", &shared_attn_plan, py::arg("num_q_heads"), py::arg("num_kv_heads"), py::arg("row_slot"),
         py::arg("seq_lens"), py::arg("levels"), py::arg("segs"), py::arg("work"), py::arg("err"));

@@ -29,20 +29,23 @@ constexpr int TILE = 64;                 // keys of a tile
 constexpr int TPAGES = TILE / PAGE;
 constexpr int STAGE = TPAGES * BLOCK;    // one tile of K or V: 32 KiB
 constexpr int STAGES = 4;
-constexpr int COMPUTE = 128;             // softmax threads (warps 0-3), then a copy and an MMA warp
+constexpr int COMPUTE = 256;             // softmax threads (warps 0-7), then a copy and an MMA warp
 constexpr int THREADS = COMPUTE + 64;
 constexpr int CTAS = ZS_SHARED_CTAS;
 constexpr int MAX_SEGS = ZS_SHARED_MAX_SEGS;
 
 // The plan (ints): header, then per segment its end page, tiles per unit, page-table row and
-// longest row, the first tile of every segment, and the first segment of every CTA.
+// longest row, the first tile of every segment, the first segment of every CTA, and per entry
+// (kv head 0) its unit's first tile, tiles, distance to the next kv head's unit and first slot.
 struct Work {
   int *total, *pend, *nt, *slot, *len, *tile0, *cta_seg;
+  int4* entry;
 };
 __host__ __device__ inline Work work_of(const SharedAttnArgs& a) {
   Work w;
   w.total = a.work;
-  w.pend = a.work + 4;
+  w.entry = reinterpret_cast<int4*>(a.work + 4);
+  w.pend = a.work + 4 + 4 * a.entries;
   w.nt = w.pend + a.num_segs;
   w.slot = w.nt + a.num_segs;
   w.len = w.slot + a.num_segs;
@@ -117,9 +120,15 @@ __global__ void __launch_bounds__(1024) plan_kernel(const SharedAttnArgs a) {
   }
   if (!fits) {
     for (int s = tid; s < a.num_segs; s += 1024) w.nt[s] = w.tile0[s] = 0;
+    for (int e = tid; e < a.entries; e += 1024) w.entry[e] = make_int4(0, 0, 0, 0);
     return;
   }
   __syncthreads();
+  for (int e = tid; e < a.entries; e += 1024) {
+    const int s = a.entry_seg[e], e0 = a.seg_start[s], at = e - e0, nt = w.nt[s];
+    const int nq = (a.seg_start[s + 1] - e0 + rpu - 1) / rpu;
+    w.entry[e] = make_int4(tile0[s] + at / rpu * nt, nt, nq * nt, at % rpu * group_of(a));
+  }
   const int total = (int)carry, n = active_ctas(total);
   for (int c = tid; c < n; c += 1024) {
     const int t = first_tile(total, n, c);
@@ -164,16 +173,16 @@ struct Walk {
 };
 
 struct Smem {
-  uint8_t q[D / 64][SLOTS * 128];   // Q: 128 slots, K-major, 4 chunks of 64 dims (128-byte swizzle)
   uint8_t ring[STAGES][STAGE];      // tiles as page images: K, V, K, V, ...
-  uint8_t p[2][SLOTS * 128];        // P: 128 slots x 64 keys bf16, K-major
-  float factor[SLOTS];
-  int vote[2][4];
-  int again[2];                     // the P in this buffer is followed by its rounding errors
+  float stage[8][32][68];           // a warp's 32 slots x 64 dims of O on their way out
+  float top[2][2][SLOTS];           // per half of a tile's keys, the largest score of every slot
+  int vote[2][8];
+  int again[2];                     // the P of this tile is followed by its rounding errors
+  float odd[SLOTS], sum[SLOTS];
   int least;                        // shortest visible length among a fragment's rows
   volatile int abort;
   uint32_t tmem;
-  uint64_t full[STAGES], empty[STAGES], s_full[2], s_empty[2], p_full[2], p_empty[2], q_full;
+  uint64_t full[STAGES], empty[STAGES], s_full[2], p_full[2], o_full[2], q_full;
 };
 
 // Waits give up when one of them in the CTA has run out (the error word is set then).
@@ -188,13 +197,13 @@ ZS_DEVICE bool wait_for(Smem& s, uint64_t* bar, uint32_t phase, int* err) {
   return false;
 }
 
-ZS_DEVICE void compute_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+ZS_DEVICE void compute_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 ZS_DEVICE bool compute_any(bool x) {
   int r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %1, 0;\n\t"
-      "bar.red.or.pred q, 1, 128, p;\n\t"
+      "bar.red.or.pred q, 1, 256, p;\n\t"
       "selp.b32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
       : "r"((int)x)
@@ -212,10 +221,35 @@ ZS_DEVICE uint32_t pack_bf16(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-ZS_DEVICE void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// c ? x : y, opaque: a chain of them over an array is not turned into an indexed load, which
+// would move the whole array from registers to local memory.
+ZS_DEVICE float pick(bool c, float x, float y) {
+  float r;
+  asm("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\tselp.f32 %0, %1, %2, p;\n\t}" : "=f"(r) : "f"(x), "f"(y), "r"((int)c));
+  return r;
 }
-ZS_DEVICE void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// A thread's own row in shared memory to global memory (16-byte aligned, a multiple of 16 bytes).
+ZS_DEVICE void bulk_store(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes) : "memory");
+}
+ZS_DEVICE void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+ZS_DEVICE void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+ZS_DEVICE void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+// One tcgen05.mma with A in TMEM.  The B descriptors of a product differ in their low words alone
+// (start address, leading offset): the high word (stride, version, 128-byte swizzle) is a constant.
+constexpr uint32_t desc_hi(uint32_t stride) { return (stride >> 4) | (1u << 14) | (2u << 29); }
+ZS_DEVICE uint32_t desc_lo(const void* p, uint32_t lead) { return (smem_u32(p) >> 4) | ((lead >> 4) << 16); }
+template <uint32_t HI_B>
+ZS_DEVICE void mma_step(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"((int)add), "n"(HI_B)
+      : "memory");
+}
 
 // Byte offset of (key k, 16-byte piece pc of its 512-byte row) in a tile's page images.
 ZS_DEVICE int tile_offset(int k, int pc) {
@@ -225,13 +259,16 @@ ZS_DEVICE bool not_finite(uint32_t two) {  // either of two bf16 is an infinity 
   return (two & 0x7F80u) == 0x7F80u || (two & 0x7F800000u) == 0x7F800000u;
 }
 
-constexpr uint32_t kTmemO = 128;     // TMEM columns: S of two tiles, then O^T (2 x 128 dims, a column per slot)
-constexpr uint32_t kTmemCols = 512;
+// TMEM columns: two S buffers of 64 (P as bf16 pairs takes their place: 32 columns, then 32 for its
+// rounding errors), Q as bf16 pairs, O.
+constexpr uint32_t kTmemQ = 128, kTmemO = 256, kTmemCols = 512;
 constexpr float kGrow = 8.f;         // O is rescaled when a maximum grows by more than 2^8
 
-// One CTA per SM; S = Q K^T (M = 128 slots, N = 64 keys) and O^T += V^T P^T (M = 128 dims twice,
-// N = slots in use) on tcgen05.  Thread s of the softmax warps owns query slot s: a row of S is
-// one TMEM lane, so maximum and sum need no exchange between threads.
+// One CTA per SM; S = Q K^T (M = 128 slots, N = 64 keys, K-major) and O += P V (M = 128 slots,
+// N = 256 dims, V read MN-major) on tcgen05, with Q and P as the TMEM operand: shared memory
+// then carries only the copies in and one read of K and V per tile (with Q and P^T there the
+// kernel was bound by shared-memory bandwidth).  A row of S, P and O is one TMEM lane; thread
+// (half, slot) of the softmax warps owns half of the keys of a tile, and of the dims of O.
 //  * copy warp: page ids, then one bulk copy per (page, kv head) block into a ring of four 32 KiB
 //    stages, running ahead across tiles and fragments;
 //  * MMA warp: S of the next tile is issued before O of this one, so it runs under the softmax;
@@ -239,14 +276,14 @@ constexpr float kGrow = 8.f;         // O is rescaled when a maximum grows by mo
 //    that grows by more than 2^8 (P stays below 2^8, O and l in fp32), so O in TMEM is rescaled
 //    rarely; the next fragment's Q is fetched during the last tile.
 // P is rounded to bf16 for the tensor cores, 2^-8 of a weight; over many keys those errors
-// average out, and where a weight is more than a quarter of the sum before its tile (first
-// tiles, few keys, peaked rows) a second product adds what the rounding lost.  l sums the
+// average out, and where a weight is more than a quarter of its half's sum before its tile
+// (first tiles, few keys, peaked rows) a second product adds what the rounding lost.  l sums the
 // weights before they are rounded.
 __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs a) {
   extern __shared__ __align__(1024) uint8_t raw[];
   Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (warp == 5) {
+  if (warp == 9) {
     tmem_alloc(&s.tmem, kTmemCols);
     tmem_relinquish();
   }
@@ -257,9 +294,8 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.s_full[i], 1);
-      mbar_init(&s.s_empty[i], COMPUTE);
       mbar_init(&s.p_full[i], COMPUTE);
-      mbar_init(&s.p_empty[i], 1);
+      mbar_init(&s.o_full[i], 1);
     }
     mbar_init(&s.q_full, COMPUTE);
     s.abort = 0;
@@ -281,7 +317,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
   }
   Fragment f;
 
-  if (warp == 4) {
+  if (warp == 8) {
     // ------------------------------------------------------------------ copies
     // Lane j holds the page id of the tile's page j and issues its K and V blocks.
     const char* kc = static_cast<const char*>(a.k_cache);
@@ -320,77 +356,103 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
     // Copies in flight land before the CTA gives its shared memory back.
     if (lane == 0)
       for (int m = max(0, issued - STAGES); m < issued; ++m) mbar_wait(&s.full[m & (STAGES - 1)], (m / STAGES) & 1, nullptr);
-  } else if (warp == 5) {
+  } else if (warp == 9) {
     // -------------------------------------------------------------------- MMA
-    if (lane == 0) {
-      const uint32_t idesc_s = make_idesc_bf16(SLOTS, TILE, 0, 0);
-      int ns = 0, no = 0;  // issued products: S of a tile, O of a round of P
-      auto scores = [&](int i) {  // S of tile i
-        const int st = (2 * i) & (STAGES - 1), b = i & 1;
-        if (!wait_for(s, &s.full[st], (i >> 1) & 1, a.err)) return false;
-        if (i >= 2 && !wait_for(s, &s.s_empty[b], ((i >> 1) - 1) & 1, a.err)) return false;
-        tc_fence_after();
+    // The warp stays together; one elected lane issues.
+    const bool leader = elect_one();
+    const uint32_t idesc_s = make_idesc_bf16(SLOTS, TILE, 0, 0), idesc_o = make_idesc_bf16(SLOTS, D, 0, 1);
+    const uint32_t k_lo = desc_lo(s.ring, 16), v_lo = desc_lo(s.ring, 1024);
+    int ns = 0, no = 0;  // issued products
+    auto scores = [&](int i) {  // S of tile i
+      const int st = (2 * i) & (STAGES - 1);
+      if (!wait_for(s, &s.full[st], (i >> 1) & 1, a.err)) return false;
+      // It takes the place of the P two tiles before: products with different accumulators have
+      // no order of their own.
+      if (i >= 2 && !wait_for(s, &s.o_full[i & 1], ((i >> 1) - 1) & 1, a.err)) return false;
+      tc_fence_after();
+      const uint32_t k_at = k_lo + st * (STAGE / 16), d = tmem + (i & 1) * TILE;
+      if (leader) {
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma_bf16(tmem + b * TILE, make_smem_desc(smem_u32(s.q[c]) + k * 32, 16, 1024, 2),
-                     make_smem_desc(smem_u32(s.ring[st] + c * 1024) + k * 32, 16, 4096, 2), idesc_s, (c | k) ? 1u : 0u);
+        for (int x = 0; x < D / 16; ++x)  // 16 dims each: 4 in a 64-dim chunk, 8 columns of Q
+          mma_step<desc_hi(4096)>(d, tmem + kTmemQ + x * 8, k_at + (x >> 2) * (1024 / 16) + (x & 3) * 2, idesc_s, x > 0);
         tc_commit(&s.empty[st]);
-        tc_commit(&s.s_full[b]);
-        ++ns;
-        return true;
-      };
-      auto output = [&](int i, bool fresh, uint32_t idesc) {  // O^T of tile i: one or two rounds of P
-        const int st = (2 * i + 1) & (STAGES - 1);
-        if (!wait_for(s, &s.full[st], (i >> 1) & 1, a.err)) return false;
-        for (bool again = true; again; fresh = false, ++no) {
-          const int b = no & 1;
-          if (!wait_for(s, &s.p_full[b], (no >> 1) & 1, a.err)) return false;
-          tc_fence_after();
-          again = s.again[b] != 0;
-#pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-            for (int k = 0; k < TPAGES; ++k)
-              mma_bf16(tmem + kTmemO + mt * SLOTS, make_smem_desc(smem_u32(s.ring[st] + 2 * mt * 1024) + k * BLOCK, 1024, 4096, 2),
-                       make_smem_desc(smem_u32(s.p[b]) + k * 32, 16, 1024, 2), idesc, (!fresh || k > 0) ? 1u : 0u);
-          if (!again) tc_commit(&s.empty[st]);
-          tc_commit(&s.p_empty[b]);
-        }
-        return true;
-      };
-      int i = 0, nf = 0;
-      bool ok = true;
-      for (; ok && walk.next(a, w, f); ++nf) {
-        const uint32_t idesc_o = make_idesc_bf16(128, (f.slots + 15) & ~15, 1, 0);
-        ok = wait_for(s, &s.q_full, nf & 1, a.err) && scores(i);
-        for (int t = f.t0; ok && t < f.t1; ++t, ++i) {
-          if (t + 1 < f.t1) ok = scores(i + 1);
-          ok = ok && output(i, t == f.t0, idesc_o);
-        }
+        tc_commit(&s.s_full[i & 1]);
       }
-      // The issued products end before TMEM is released.
-      if (ns > 0) mbar_wait(&s.s_full[(ns - 1) & 1], ((ns - 1) >> 1) & 1, nullptr);
-      if (no > 0) mbar_wait(&s.p_empty[(no - 1) & 1], ((no - 1) >> 1) & 1, nullptr);
+      ++ns;
+      return true;
+    };
+    // O of tile i.
+    auto output = [&](int i, bool fresh) {
+      const int st = (2 * i + 1) & (STAGES - 1), b = i & 1;
+      if (!wait_for(s, &s.full[st], (i >> 1) & 1, a.err)) return false;
+      if (!wait_for(s, &s.p_full[b], (i >> 1) & 1, a.err)) return false;
+      tc_fence_after();
+      const uint32_t v_at = v_lo + st * (STAGE / 16), p_at = tmem + b * TILE;
+      const bool again = s.again[b] != 0;
+      if (leader) {
+#pragma unroll
+        for (int k = 0; k < TPAGES; ++k)  // a page each: 16 keys
+          mma_step<desc_hi(4096)>(tmem + kTmemO, p_at + k * 8, v_at + k * (BLOCK / 16), idesc_o, !fresh || k > 0);
+        if (again) {
+#pragma unroll
+          for (int k = 0; k < TPAGES; ++k)
+            mma_step<desc_hi(4096)>(tmem + kTmemO, p_at + 32 + k * 8, v_at + k * (BLOCK / 16), idesc_o, true);
+        }
+        tc_commit(&s.empty[st]);
+        tc_commit(&s.o_full[b]);
+      }
+      ++no;
+      return true;
+    };
+    int i = 0, nf = 0;
+    bool ok = true;
+    for (; ok && walk.next(a, w, f); ++nf) {
+      ok = wait_for(s, &s.q_full, nf & 1, a.err) && scores(i);
+      ok = __all_sync(0xffffffff, ok);
+      for (int t = f.t0; ok && t < f.t1; ++t, ++i) {
+        if (t + 1 < f.t1) ok = scores(i + 1);
+        ok = ok && output(i, t == f.t0);
+        ok = __all_sync(0xffffffff, ok);
+      }
     }
+    // The issued products end before TMEM is released.
+    if (ns > 0) mbar_wait(&s.s_full[(ns - 1) & 1], ((ns - 1) >> 1) & 1, nullptr);
+    if (no > 0) mbar_wait(&s.o_full[(no - 1) & 1], ((no - 1) >> 1) & 1, nullptr);
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- softmax
-    const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
-    const float qscale = a.sm_scale * 1.4426950408889634f;  // exp2 domain
+    const int half = warp >> 2, slot = (warp & 3) * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);  // this warp's quarter of TMEM
+    const float qscale = a.sm_scale * 1.4426950408889634f;             // exp2 domain
     const int group = walk.group;
-    // Q of a fragment, 512 bytes a slot: slot = warp, warp + 4, ..
+    // This thread's half of its slot's query: 128 dims.
+    uint4 qv[16];
     auto fetch_q = [&](const Fragment& g) {
-      for (int sl = warp; sl < g.slots; sl += 4) {
-        const int row = a.seg_rows[g.e0 + sl / group];
-        const char* src = static_cast<const char*>(a.q) + (((size_t)row * a.num_q_heads + g.kvh * group + sl % group) * D + lane * 8) * 2;
-        cp_async16(smem_u32(s.q[lane >> 3]) + sl * 128 + (((lane & 7) ^ (sl & 7)) << 4), src);
+      if (slot < g.slots) {
+        const int row = a.seg_rows[g.e0 + slot / group];
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) +
+                                                          ((size_t)row * a.num_q_heads + g.kvh * group + slot % group) * D) + half * 16;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) qv[j] = __ldg(src + j);
       }
     };
-    auto q_ready = [&]() {
-      cp_async_wait();
-      fence_proxy_async_shared();
+    auto store_q = [&](const Fragment& g) {
+      if ((warp & 3) * 32 < g.slots) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t r[16];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            r[4 * k] = qv[4 * j + k].x;
+            r[4 * k + 1] = qv[4 * j + k].y;
+            r[4 * k + 2] = qv[4 * j + k].z;
+            r[4 * k + 3] = qv[4 * j + k].w;
+          }
+          tmem_st_32x32b_x16(lanes + kTmemQ + half * 64 + j * 16, r);
+        }
+        tmem_st_wait();
+      }
+      tc_fence_before();
       mbar_arrive(&s.q_full);
     };
     // After a wait that gave up these warps go on to the end with whatever is there (the error word
@@ -398,13 +460,13 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
     bool more = walk.next(a, w, f);
     if (more) {
       fetch_q(f);
-      q_ready();
+      store_q(f);
     }
-    int i = 0, pr = 0;  // tiles, rounds of P
+    int i = 0;
     while (more) {
       Fragment g;
-      const bool used = tid < f.slots, busy = warp * 32 < f.slots;
-      const int limit = used ? min(a.seq_lens[a.seg_rows[f.e0 + tid / group]], f.len) : 0x7FFFFFFF;  // keys this slot sees
+      const bool used = slot < f.slots, busy = (warp & 3) * 32 < f.slots;
+      const int limit = used ? min(a.seq_lens[a.seg_rows[f.e0 + slot / group]], f.len) : 0x7FFFFFFF;  // keys this slot sees
       {
         const int least = __reduce_min_sync(0xffffffff, limit);
         if (tid == 0) s.least = 0x7FFFFFFF;
@@ -413,7 +475,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
         compute_sync();
       }
       const int least = s.least;
-      float m = -INFINITY, l = 0.f;  // reference maximum (raw scores) and sum of this slot
+      float m = -INFINITY, l = 0.f;  // reference maximum (raw scores) of the slot, sum of this half's weights
       for (int t = f.t0; t < f.t1; ++t, ++i) {
         const int b = i & 1, key0 = (f.p0 + t * TPAGES) * PAGE;
         wait_for(s, &s.s_full[b], (i >> 1) & 1, a.err);
@@ -423,89 +485,88 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
           more = walk.next(a, w, g);
           if (more) fetch_q(g);
         }
-        uint32_t r[2][32];
+        uint32_t r[32];
         float mt = -INFINITY;
-        const int valid = limit - key0;
+        const int valid = limit - key0 - half * 32;
         if (busy) {
-          tmem_ld_32x32b_x32(tmem + b * TILE + lane_off, r[0]);
-          tmem_ld_32x32b_x32(tmem + b * TILE + 32 + lane_off, r[1]);
+          tmem_ld_32x32b_x32(lanes + b * TILE + half * 32, r);
           tmem_ld_wait();
-          if (valid < TILE) {
+          if (valid < 32) {
 #pragma unroll
-            for (int j = 0; j < TILE; ++j)
-              if (j >= valid) r[j >> 5][j & 31] = 0xFF800000u;  // -inf
+            for (int j = 0; j < 32; ++j)
+              if (j >= valid) r[j] = 0xFF800000u;  // -inf
           }
           float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int j = 0; j < TILE; ++j) x[j & 3] = fmaxf(x[j & 3], __uint_as_float(r[j >> 5][j & 31]));
+          for (int j = 0; j < 32; ++j) x[j & 3] = fmaxf(x[j & 3], __uint_as_float(r[j]));
           mt = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-        }
-        tc_fence_before();
-        mbar_arrive(&s.s_empty[b]);
-        // The reference follows the maximum when that outgrew it (and at first).
-        const bool grow = used && (m == -INFINITY ? mt > -INFINITY : (mt - m) * qscale > kGrow);
-        float fac = 1.f;
-        if (grow) {
-          fac = m == -INFINITY ? 0.f : ex2((m - mt) * qscale);
-          l *= fac;
-          m = mt;
+          s.top[b][half][slot] = mt;
         }
         // A weight above a quarter of the sum so far: its bf16 rounding (2^-8) would show.
-        const bool sharp = used && mt > -INFINITY && ex2((mt - m) * qscale) * 4.f > l;
+        const bool sharp = used && mt > -INFINITY && (m == -INFINITY || ex2((mt - m) * qscale) * 4.f > l);
         {
-          const int any = (__any_sync(0xffffffff, grow) ? 1 : 0) | (__any_sync(0xffffffff, sharp) ? 2 : 0);
+          const int any = __any_sync(0xffffffff, sharp);
           if (lane == 0) s.vote[b][warp] = any;
           compute_sync();
         }
-        const int votes = s.vote[b][0] | s.vote[b][1] | s.vote[b][2] | s.vote[b][3];
-        const bool fine = (votes & 2) != 0;
-        if ((votes & 1) && t > f.t0) {
-          s.factor[tid] = fac;
-          wait_for(s, &s.p_empty[(pr - 1) & 1], ((pr - 1) >> 1) & 1, a.err);  // O holds every tile before this one
-          compute_sync();
-          tc_fence_after();
-          for (int c0 = 0; c0 < f.slots; c0 += 16)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t o[16];
-              const uint32_t at = tmem + kTmemO + h * SLOTS + c0 + lane_off;
-              tmem_ld_32x32b_x16(at, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * s.factor[c0 + j]);
-              tmem_st_32x32b_x16(at, o);
-            }
-          tmem_st_wait();
-          compute_sync();
+        const int4 v0 = *reinterpret_cast<const int4*>(&s.vote[b][0]), v1 = *reinterpret_cast<const int4*>(&s.vote[b][4]);
+        const bool fine = (v0.x | v0.y | v0.z | v0.w | v1.x | v1.y | v1.z | v1.w) != 0;
+        float fac = 1.f;
+        bool grow = false;
+        if (busy) {
+          // The reference follows the maximum when that outgrew it (and at first); both halves agree.
+          mt = fmaxf(mt, s.top[b][half ^ 1][slot]);
+          grow = used && (m == -INFINITY ? mt > -INFINITY : (mt - m) * qscale > kGrow);
+          if (grow) {
+            fac = m == -INFINITY ? 0.f : ex2((m - mt) * qscale);
+            l *= fac;
+            m = mt;
+          }
         }
-        int pb = pr & 1;
-        if (pr >= 2) wait_for(s, &s.p_empty[pb], ((pr >> 1) - 1) & 1, a.err);  // the buffer's last P is read
+        if (__any_sync(0xffffffff, grow) && t > f.t0) {
+          wait_for(s, &s.o_full[(i - 1) & 1], ((i - 1) >> 1) & 1, a.err);  // O holds every tile before this one
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < 128; c += 16) {
+            uint32_t o[16];
+            const uint32_t at = lanes + kTmemO + half * 128 + c;
+            tmem_ld_32x32b_x16(at, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * fac);
+            tmem_st_32x32b_x16(at, o);
+          }
+        }
         if (busy) {
           const float off = m == -INFINITY ? 0.f : m * qscale;
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          uint32_t pk[16];
 #pragma unroll
-          for (int c = 0; c < TILE / 8; ++c) {
-            uint32_t pk[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int k = c * 8 + j * 2;
-              const float lo = ex2(fmaf(__uint_as_float(r[k >> 5][k & 31]), qscale, -off));
-              const float hi = ex2(fmaf(__uint_as_float(r[k >> 5][(k & 31) + 1]), qscale, -off));
-              sum[j] += lo + hi;
-              pk[j] = pack_bf16(lo, hi);
-              r[k >> 5][k & 31] = __float_as_uint(lo);
-              r[k >> 5][(k & 31) + 1] = __float_as_uint(hi);
-            }
-            *reinterpret_cast<uint4*>(s.p[pb] + tid * 128 + ((c ^ (tid & 7)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+          for (int j = 0; j < 16; ++j) {
+            const float lo = ex2(fmaf(__uint_as_float(r[2 * j]), qscale, -off));
+            const float hi = ex2(fmaf(__uint_as_float(r[2 * j + 1]), qscale, -off));
+            sum[j & 3] += lo + hi;
+            pk[j] = pack_bf16(lo, hi);
+            r[2 * j] = __float_as_uint(lo);
+            r[2 * j + 1] = __float_as_uint(hi);
           }
+          tmem_st_32x32b_x16(lanes + b * TILE + half * 16, pk);
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          if (fine) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              pk[j] = pack_bf16(__uint_as_float(r[2 * j]) - __uint_as_float(pk[j] << 16),
+                                __uint_as_float(r[2 * j + 1]) - __uint_as_float(pk[j] & 0xFFFF0000u));
+            tmem_st_32x32b_x16(lanes + b * TILE + 32 + half * 16, pk);
+          }
+          tmem_st_wait();
         }
-        if (tid == 0) s.again[pb] = fine;
+        if (tid == 0) s.again[b] = fine;
         // Values that a row does not see must not meet its zero weights as NaN or infinity.  Rows
         // of the tile that nobody sees are zeroed.  Rows that only some see are looked at: those
         // with such a value are zeroed too, and added by hand to the slots that see them.
         const int end = f.len - key0;  // keys of the tile that some row sees
-        uint64_t odd = 0;
+        unsigned long long odd = 0;
         if (end < TILE || least < key0 + TILE) {
           const int st = (2 * i + 1) & (STAGES - 1);
           wait_for(s, &s.full[st], (i >> 1) & 1, a.err);
@@ -516,8 +577,8 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
             found |= not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w);
           }
           if (from < stop && compute_any(found)) {
-            for (int k = from; k < stop; ++k) {  // 512 bytes a key, 4 a thread
-              uint32_t* at = reinterpret_cast<uint32_t*>(s.ring[st] + tile_offset(k, tid >> 2)) + (tid & 3);
+            for (int k = from; k < stop; ++k) {  // 512 bytes a key: 4 for each of 128 threads
+              uint32_t* at = reinterpret_cast<uint32_t*>(s.ring[st] + tile_offset(k, (tid & 127) >> 2)) + (tid & 3);
               if (compute_any(not_finite(*at))) {
                 odd |= 1ull << k;
                 *at = 0;
@@ -526,135 +587,163 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
           }
           for (int x = max(end, 0) * 32 + tid; x < TILE * 32; x += COMPUTE)
             *reinterpret_cast<uint4*>(s.ring[st] + tile_offset(x >> 5, x & 31)) = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_shared();
-        tc_fence_before();
-        mbar_arrive(&s.p_full[pb]);
-        ++pr;
-        if (fine) {  // a second round: what the first one's rounding lost
-          pb = pr & 1;
-          if (pr >= 2) wait_for(s, &s.p_empty[pb], ((pr >> 1) - 1) & 1, a.err);
-          if (busy) {
-#pragma unroll
-            for (int c = 0; c < TILE / 8; ++c) {
-              uint32_t pk[4];
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const int k = c * 8 + j * 2;
-                const float lo = __uint_as_float(r[k >> 5][k & 31]), hi = __uint_as_float(r[k >> 5][(k & 31) + 1]);
-                const uint32_t x = pack_bf16(lo, hi);
-                pk[j] = pack_bf16(lo - __uint_as_float(x << 16), hi - __uint_as_float(x & 0xFFFF0000u));
-              }
-              *reinterpret_cast<uint4*>(s.p[pb] + tid * 128 + ((c ^ (tid & 7)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-            }
-          }
-          if (tid == 0) s.again[pb] = 0;
           fence_proxy_async_shared();
-          mbar_arrive(&s.p_full[pb]);
-          ++pr;
         }
+        tc_fence_before();
+        mbar_arrive(&s.p_full[b]);
         if (odd != 0) {
-          wait_for(s, &s.p_empty[pb], ((pr - 1) >> 1) & 1, a.err);
+          wait_for(s, &s.o_full[b], (i >> 1) & 1, a.err);
           tc_fence_after();
-          for (int c0 = 0; c0 < f.slots; c0 += 16)
-            for (int h = 0; h < 2; ++h) {
+          for (int k = 0; k < TILE; ++k) {
+            if (!(odd >> k & 1)) continue;
+            compute_sync();
+            if (busy && (k >> 5) == half) {
+              float p = 0.f;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) p = pick(j == (k & 31), __uint_as_float(r[j]), p);
+              s.odd[slot] = p;
+            }
+            compute_sync();
+            const int at_page = (key0 + k) / PAGE, page = at_page < a.max_pages ? f.pt[at_page] : -1;
+            if (!busy || page < 0 || page >= a.num_pages) continue;
+            const uint8_t* blk = static_cast<const uint8_t*>(a.v_cache) + ((size_t)page * a.num_kv_heads + f.kvh) * BLOCK;
+            const float p = s.odd[slot];
+            for (int c = 0; c < 128; c += 16) {
               uint32_t o[16];
-              const uint32_t at = tmem + kTmemO + h * SLOTS + c0 + lane_off;
+              const uint32_t at = lanes + kTmemO + half * 128 + c;
               tmem_ld_32x32b_x16(at, o);
               tmem_ld_wait();
-              for (int k = 0; k < TILE; ++k) {
-                if (!(odd >> k & 1)) continue;
-                const int at_page = (key0 + k) / PAGE, d = h * 128 + tid;
-                const int page = at_page < a.max_pages ? f.pt[at_page] : -1;
-                if (page < 0 || page >= a.num_pages) continue;
-                const uint8_t* blk = static_cast<const uint8_t*>(a.v_cache) + ((size_t)page * a.num_kv_heads + f.kvh) * BLOCK;
-                const float v = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(blk + tile_offset(k & 15, d >> 3) + (d & 7) * 2));
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                  const int sl = c0 + j;
-                  const int pat = sl * 128 + (((k >> 3) ^ (sl & 7)) << 4) + (k & 7) * 2;
-                  float p = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(s.p[pb] + pat));
-                  if (fine) p += __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(s.p[pb ^ 1] + pat));
-                  if (p != 0.f) o[j] = __float_as_uint(__uint_as_float(o[j]) + p * v);
-                }
+              for (int j = 0; j < 16; ++j) {
+                const int d = half * 128 + c + j;
+                const float v = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(blk + tile_offset(k & 15, d >> 3) + (d & 7) * 2));
+                if (p != 0.f) o[j] = __float_as_uint(__uint_as_float(o[j]) + p * v);
               }
               tmem_st_32x32b_x16(at, o);
+              tmem_st_wait();
             }
-          tmem_st_wait();
+          }
           tc_fence_before();
-          compute_sync();  // all have read P before anyone writes the next
         }
       }
-      if (more) q_ready();
-      // ---- the fragment's records
-      wait_for(s, &s.p_empty[(pr - 1) & 1], ((pr - 1) >> 1) & 1, a.err);
+      if (more) store_q(g);
+      // ---- the fragment's records: those of the unit's first fragment lie by (entry, head), those of
+      // a later one by CTA and slot
+      if (half == 1) s.sum[slot] = l;
+      compute_sync();
+      wait_for(s, &s.o_full[(i - 1) & 1], ((i - 1) >> 1) & 1, a.err);
       tc_fence_after();
-      float* rec = a.partial + (f.first ? ((size_t)f.e0 * a.num_q_heads + f.kvh * group) * PREC
-                                        : ((size_t)a.entries * a.num_q_heads + (size_t)cta * SLOTS) * PREC);
-      // Records of the unit's first fragment lie by (entry, head), those of a later one by slot.
-      auto at = [&](int sl) { return rec + (f.first ? ((size_t)(sl / group) * a.num_q_heads + sl % group) : (size_t)sl) * PREC; };
-      for (int c0 = 0; c0 < f.slots; c0 += 16)
+      if (busy) {
+        const size_t at = f.first ? (size_t)(f.e0 + slot / group) * a.num_q_heads + f.kvh * group + slot % group
+                                  : (size_t)a.entries * a.num_q_heads + (size_t)cta * SLOTS + slot;
+        float* rec = a.partial + at * PREC;
+        float* row = s.stage[warp][lane];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t o[16];
-          tmem_ld_32x32b_x16(tmem + kTmemO + h * SLOTS + c0 + lane_off, o);
-          tmem_ld_wait();
+        for (int c = 0; c < 128; c += 64) {
+          bulk_wait_read();
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (c0 + j < f.slots) at(c0 + j)[h * 128 + tid] = __uint_as_float(o[j]);
+          for (int q = 0; q < 64; q += 32) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(lanes + kTmemO + half * 128 + c + q, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(row + q + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+          }
+          fence_proxy_async_shared();
+          if (used) bulk_store(rec + half * 128 + c, row, 256);
+          bulk_commit();
         }
-      if (used) {
-        at(tid)[D] = m * qscale;
-        at(tid)[D + 1] = l;
+        if (used && half == 0) *reinterpret_cast<float2*>(rec + D) = make_float2(m * qscale, l + s.sum[slot]);
       }
       tc_fence_before();
       f = g;
     }
+    bulk_wait();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 5) tmem_dealloc(tmem, kTmemCols);
+  if (warp == 9) tmem_dealloc(tmem, kTmemCols);
 }
 
-// One CTA per (row, q head), thread = dim.
-__global__ void __launch_bounds__(D) merge_kernel(const SharedAttnArgs a) {
+constexpr int MERGE_WARPS = 8;
+
+// One warp per (row, q head); a lane owns dims 4 lane .. + 3 and 128 + 4 lane .. + 3.  Records are
+// found and weighed 32 at a time (one a lane), then added in order.
+__global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const SharedAttnArgs a) {
   pdl_wait();
   pdl_trigger();
   const Work w = work_of(a);
-  const int row = blockIdx.x, h = blockIdx.y, d = threadIdx.x, group = group_of(a), rpu = SLOTS / group;
+  const int item = blockIdx.x * MERGE_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (item >= a.rows * a.num_q_heads) return;
+  const int row = item / a.num_q_heads, h = item % a.num_q_heads, group = group_of(a);
   const int total = *w.total, n = active_ctas(total);
-  float m = -INFINITY, l = 0.f, o = 0.f;
+  float m = -INFINITY, l = 0.f, o[8] = {};
   for (int j = 0; j < a.levels; ++j) {
     const int e = a.row_entry[row * a.levels + j];
     if (e < 0) break;
-    const int seg = a.entry_seg[e], nt = w.nt[seg];
-    if (nt == 0) continue;
-    const int at = e - a.seg_start[seg], nq = (a.seg_start[seg + 1] - a.seg_start[seg] + rpu - 1) / rpu;
-    const int first = w.tile0[seg] + ((h / group) * nq + at / rpu) * nt;
-    const int c0 = cta_of(total, n, first), c1 = cta_of(total, n, first + nt - 1);
-    const float* rec = a.partial + ((size_t)e * a.num_q_heads + h) * PREC;
-    const float* more = a.partial + ((size_t)a.entries * a.num_q_heads + (at % rpu) * group + h % group) * PREC;
-    for (int c = c0; c <= c1; ++c) {
-      if (c > c0) rec = more + (size_t)c * SLOTS * PREC;
-      const float mr = rec[D];
-      if (mr == -INFINITY) continue;
-      const float mn = fmaxf(m, mr), s0 = m == -INFINITY ? 0.f : exp2f(m - mn), s1 = exp2f(mr - mn);
-      l = l * s0 + rec[D + 1] * s1;
-      o = o * s0 + rec[d] * s1;
+    const int4 u = w.entry[e];
+    if (u.y == 0) continue;
+    const int first = u.x + h / group * u.z;
+    const int c0 = cta_of(total, n, first), c1 = cta_of(total, n, first + u.y - 1);
+    for (int c = c0; c <= c1; c += 32) {
+      const size_t at = c + lane == c0 ? (size_t)e * a.num_q_heads + h
+                                       : (size_t)a.entries * a.num_q_heads + (size_t)(c + lane) * SLOTS + u.w + h % group;
+      const float2 ml = c + lane <= c1 ? *reinterpret_cast<const float2*>(a.partial + at * PREC + D) : make_float2(-INFINITY, 0.f);
+      const float mn = fmaxf(m, warp_max(ml.x)), s0 = m == -INFINITY ? 0.f : exp2f(m - mn);
+      const float wt = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mn);
+      l = l * s0 + warp_sum(ml.x == -INFINITY ? 0.f : wt * ml.y);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) o[k] *= s0;
       m = mn;
+      const int cnt = min(32, c1 - c + 1);
+#pragma unroll 4
+      for (int x = 0; x < cnt; ++x) {
+        const float wx = __shfl_sync(0xffffffff, wt, x);
+        const float4* rec = reinterpret_cast<const float4*>(a.partial + __shfl_sync(0xffffffff, at, x) * PREC);
+        const float4 p = rec[lane], q = rec[32 + lane];
+        if (wx == 0.f) continue;
+        o[0] += wx * p.x;
+        o[1] += wx * p.y;
+        o[2] += wx * p.z;
+        o[3] += wx * p.w;
+        o[4] += wx * q.x;
+        o[5] += wx * q.y;
+        o[6] += wx * q.z;
+        o[7] += wx * q.w;
+      }
     }
   }
-  float y = m == -INFINITY ? 0.f : o / l;
-  const size_t at = ((size_t)row * a.num_q_heads + h) * D + d;
-  if (a.gate != nullptr) y *= sigmoidf_(__bfloat162float(static_cast<const __nv_bfloat16*>(a.gate)[at]));
-  if (a.out_bf16 != nullptr) static_cast<__nv_bfloat16*>(a.out_bf16)[at] = __float2bfloat16_rn(y);
-  if (a.out_q != nullptr) {
-    const uint8_t code = mx_scale_e8m0(warp_max(fabsf(y)));
-    a.out_q[at] = f32_to_e4m3(y * mx_inv_scale(code));
-    if ((d & 31) == 0) {
-      const int kb = h * (D / 32) + (d >> 5);
-      a.out_sf[((size_t)(row >> 7) * (a.num_q_heads * D >> 7) + (kb >> 2)) * 512 + sf_atom_offset(row & 127, kb & 3)] = code;
+  const float inv = m == -INFINITY ? 0.f : 1.f / l;
+  const size_t at = (size_t)item * D;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int d = k * 128 + lane * 4;
+    float* y = o + 4 * k;
+    float g[4] = {1.f, 1.f, 1.f, 1.f};
+    if (a.gate != nullptr) {
+      const uint2 gv = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(a.gate) + at + d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) g[j] = sigmoidf_(__bfloat162float(reinterpret_cast<const __nv_bfloat16*>(&gv)[j]));
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = m == -INFINITY ? 0.f : y[j] * inv * g[j];
+    if (a.out_bf16 != nullptr)
+      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out_bf16) + at + d) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+    if (a.out_q != nullptr) {  // a block of 32 dims is 8 lanes
+      float amax = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
+#pragma unroll
+      for (int x = 1; x < 8; x <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffff, amax, x));
+      const uint8_t code = mx_scale_e8m0(amax);
+      const float si = mx_inv_scale(code);
+      uint32_t four = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) four |= (uint32_t)f32_to_e4m3(y[j] * si) << (8 * j);
+      *reinterpret_cast<uint32_t*>(a.out_q + at + d) = four;
+      if ((lane & 7) == 0) {
+        const int kb = h * (D / 32) + (d >> 5);
+        a.out_sf[((size_t)(row >> 7) * (a.num_q_heads * D >> 7) + (kb >> 2)) * 512 + sf_atom_offset(row & 127, kb & 3)] = code;
+      }
     }
   }
 }
@@ -685,6 +774,8 @@ extern "C" int zs_shared_attn(const SharedAttnArgs* args, cudaStream_t stream) {
   const size_t smem = sizeof(zs::sattn::Smem) + 1024;
   cudaFuncSetAttribute(zs::sattn::tiles_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   zs_launch(zs::sattn::tiles_kernel, zs::sattn::CTAS, zs::sattn::THREADS, smem, stream, a);
-  zs_launch(zs::sattn::merge_kernel, dim3(a.rows, a.num_q_heads), zs::sattn::D, 0, stream, a);
+  const int items = a.rows * a.num_q_heads;
+  zs_launch(zs::sattn::merge_kernel, (items + zs::sattn::MERGE_WARPS - 1) / zs::sattn::MERGE_WARPS, zs::sattn::MERGE_WARPS * 32, 0,
+            stream, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }

@@ -688,7 +688,7 @@ typedef struct SharedAttnArgs {
   const int* seg_page1;
   const int* entry_seg;      // [entries]
   const int* row_entry;      // [rows, levels] entry of each row's segments, -1: none
-  int* work;                 // [ZS_SHARED_WORK_INTS(num_segs)] written by the plan
+  int* work;                 // [ZS_SHARED_WORK_INTS(num_segs, entries)], 16-byte aligned, written by the plan
   float* partial;            // scratch: 260 floats x (entries * num_q_heads + ZS_SHARED_CTAS * ZS_SHARED_SLOTS)
   float sm_scale;            // > 0
   void* out_bf16;            // optional [rows, num_q_heads * 256]
@@ -697,7 +697,7 @@ typedef struct SharedAttnArgs {
   int* err;
 } SharedAttnArgs;
 
-#define ZS_SHARED_WORK_INTS(num_segs) (4 + 5 * (num_segs) + 1 + ZS_SHARED_CTAS)
+#define ZS_SHARED_WORK_INTS(num_segs, entries) (4 + 4 * (entries) + 5 * (num_segs) + 1 + ZS_SHARED_CTAS)
 
 // Divide the step's keys over the GPU (from seq_lens, row_slot, the segments and the head counts;
 // q, caches and outputs are not read): once a step.  Then one zs_shared_attn per layer.

@@ -123,6 +123,8 @@ CASES = {
     "group_16": (16, 1, [8], [seq(0, 128, 30 + i) for i in range(9)]),
     "group_64": (64, 1, [8], [seq(0, 128, 5 + i) for i in range(5)]),
     "long": (16, 2, [300], [seq(0, 4800, 1 + 50 * i) for i in range(6)]),
+    "more_units_than_sms": (16, 2, [9, 30], [seq(i % 2, [144, 480][i % 2], 1 + (37 * i) % 230) for i in range(150)]),
+    "many_fragments_of_128_slots": (16, 2, [30] * 24, [seq(i % 24, 480, 1 + (7 * i) % 90, 1 + i % 3) for i in range(250)]),
     "long_alone": (16, 2, [], [seq(None, 0, 5000)]),
 }
 
