@@ -22,80 +22,87 @@ namespace sattn {
 
 constexpr int D = 256;
 constexpr int PAGE = 16;
-constexpr int PREC = D + 4;              // record: o[256], m, l, padding to 16 bytes
+constexpr int PREC = D + 4;              // record: o[256], m, l of either half of the keys, padding to 16 bytes
 constexpr int BLOCK = PAGE * D * 2;      // bytes of a (page, kv head) block
 constexpr int SLOTS = ZS_SHARED_SLOTS;   // query slots of a unit
 constexpr int TILE = 64;                 // keys of a tile
 constexpr int TPAGES = TILE / PAGE;
 constexpr int STAGE = TPAGES * BLOCK;    // one tile of K or V: 32 KiB
-constexpr int STAGES = 4;
+constexpr int STAGES = 5;
 constexpr int COMPUTE = 256;             // softmax threads (warps 0-7), then a copy and an MMA warp
 constexpr int THREADS = COMPUTE + 64;
 constexpr int CTAS = ZS_SHARED_CTAS;
 constexpr int MAX_SEGS = ZS_SHARED_MAX_SEGS;
 
-// The plan (ints): header, then per segment its end page, tiles per unit, page-table row and
-// longest row, the first tile of every segment, the first segment of every CTA, and per entry
-// (kv head 0) its unit's first tile, tiles, distance to the next kv head's unit and first slot.
+// A unit costs its tiles and UNIT_COST tiles more (its Q, its record, a pipeline that starts anew).
+constexpr int UNIT_COST = 2;
+
+// The plan (ints): the cost of everything, a Segment for each segment and one behind the last
+// (its cost0 alone), per entry (kv head 0) its unit's first cost, its tiles, the distance to the
+// next kv head's unit and its first slot, and the first segment of every CTA.
+struct Segment {
+  int cost0, nt, e0, rows;   // cost before it, tiles of a unit, first entry, rows
+  int p0, pend, len, slot;   // pages [p0, pend), its longest row's length (at most their end) and table row
+};
 struct Work {
-  int *total, *pend, *nt, *slot, *len, *tile0, *cta_seg;
+  int* total;
+  Segment* seg;
   int4* entry;
+  int* cta_seg;
 };
 __host__ __device__ inline Work work_of(const SharedAttnArgs& a) {
   Work w;
   w.total = a.work;
-  w.entry = reinterpret_cast<int4*>(a.work + 4);
-  w.pend = a.work + 4 + 4 * a.entries;
-  w.nt = w.pend + a.num_segs;
-  w.slot = w.nt + a.num_segs;
-  w.len = w.slot + a.num_segs;
-  w.tile0 = w.len + a.num_segs;
-  w.cta_seg = w.tile0 + a.num_segs + 1;
+  w.seg = reinterpret_cast<Segment*>(a.work + 4);
+  w.entry = reinterpret_cast<int4*>(w.seg + a.num_segs + 1);
+  w.cta_seg = reinterpret_cast<int*>(w.entry + a.entries);
   return w;
 }
 
 ZS_DEVICE int group_of(const SharedAttnArgs& a) { return a.num_q_heads / a.num_kv_heads; }
-// First tile of CTA c when `total` tiles are divided over n CTAs, and the CTA of a tile.
-ZS_DEVICE int first_tile(int total, int n, int c) { return (int)((long long)total * c / n); }
-ZS_DEVICE int cta_of(int total, int n, int tile) { return (int)(((long long)(tile + 1) * n - 1) / total); }
+// First cost of CTA c when `total` is divided over n CTAs, and the CTA of a cost.
+ZS_DEVICE int first_cost(int total, int n, int c) { return (int)((long long)total * c / n); }
+ZS_DEVICE int cta_of(int total, int n, int cost) { return (int)(((long long)(cost + 1) * n - 1) / total); }
 ZS_DEVICE int active_ctas(int total) { return min(CTAS, total); }
 
-// One CTA: the longest row of every segment decides how many pages it has; tiles are counted and
+// One CTA: the longest row of every segment decides how many pages it has; costs are counted and
 // the CTAs' ranges laid over them.
 __global__ void __launch_bounds__(1024) plan_kernel(const SharedAttnArgs a) {
-  pdl_wait();
   pdl_trigger();
   __shared__ unsigned long long longest[MAX_SEGS];  // (length, ~row)
-  __shared__ int tile0[MAX_SEGS + 1];
+  __shared__ int cost0[MAX_SEGS + 1], tiles[MAX_SEGS];
   __shared__ long long red[32];
   const Work w = work_of(a);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   for (int s = tid; s < a.num_segs; s += 1024) longest[s] = 0;
   __syncthreads();
+  const int row0 = tid < a.entries ? a.seg_rows[tid] : 0, seg0 = tid < a.entries ? a.entry_seg[tid] : 0;  // the plan's own
+  pdl_wait();
   for (int e = tid; e < a.entries; e += 1024) {
-    const int row = a.seg_rows[e];
+    const int row = e == tid ? row0 : a.seg_rows[e], s = e == tid ? seg0 : a.entry_seg[e];
     const int len = max(a.seq_lens[row], 0);
-    atomicMax(&longest[a.entry_seg[e]], ((unsigned long long)len << 32) | (uint32_t)~row);
+    atomicMax(&longest[s], ((unsigned long long)len << 32) | (uint32_t)~row);
   }
   __syncthreads();
-  const int rpu = SLOTS / group_of(a);
+  const int group = group_of(a), rpu = SLOTS / group;
   long long carry = 0;
   for (int s0 = 0; s0 < a.num_segs; s0 += 1024) {
     const int s = s0 + tid;
-    long long tiles = 0;
+    long long cost = 0;
+    Segment g = {};
     if (s < a.num_segs) {
-      const int len = (int)(longest[s] >> 32), row = (int)~(uint32_t)longest[s], p0 = a.seg_page0[s], p1 = a.seg_page1[s];
-      int pend = (int)(((long long)len + PAGE - 1) / PAGE);
-      if (p1 >= 0) pend = min(pend, p1);
-      const int nt = (max(pend - p0, 0) + TPAGES - 1) / TPAGES;
-      const int rows = a.seg_start[s + 1] - a.seg_start[s];
-      tiles = (long long)nt * ((rows + rpu - 1) / rpu) * a.num_kv_heads;
-      w.pend[s] = pend;
-      w.nt[s] = nt;
-      w.slot[s] = a.row_slot[row];
-      w.len[s] = (int)min((long long)len, (long long)pend * PAGE);
+      const int len = (int)(longest[s] >> 32), row = (int)~(uint32_t)longest[s], p1 = a.seg_page1[s];
+      g.e0 = a.seg_start[s];
+      g.rows = a.seg_start[s + 1] - g.e0;
+      g.p0 = a.seg_page0[s];
+      g.slot = a.row_slot[row];
+      g.pend = (int)(((long long)len + PAGE - 1) / PAGE);
+      if (p1 >= 0) g.pend = min(g.pend, p1);
+      g.nt = (max(g.pend - g.p0, 0) + TPAGES - 1) / TPAGES;
+      g.len = (int)min((long long)len, (long long)g.pend * PAGE);
+      if (g.nt > 0) cost = (long long)(g.nt + UNIT_COST) * ((g.rows + rpu - 1) / rpu) * a.num_kv_heads;
     }
-    long long x = tiles;
+    long long x = cost;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long y = __shfl_up_sync(0xffffffff, x, o);
@@ -104,38 +111,39 @@ __global__ void __launch_bounds__(1024) plan_kernel(const SharedAttnArgs a) {
     __syncthreads();
     if (lane == 31) red[warp] = x;
     __syncthreads();
-    long long before = carry, sum = carry;
-    for (int j = 0; j < 32; ++j) {
-      if (j < warp) before += red[j];
-      sum += red[j];
+    long long before = warp > 0 && lane < warp ? red[lane] : 0, sum = red[lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      before += __shfl_xor_sync(0xffffffff, before, o);
+      sum += __shfl_xor_sync(0xffffffff, sum, o);
     }
-    if (s < a.num_segs) tile0[s] = w.tile0[s] = (int)(before + x - tiles);
-    carry = sum;
+    if (s < a.num_segs) {
+      g.cost0 = (int)(carry + before + x - cost);
+      cost0[s] = g.cost0;
+      tiles[s] = g.nt;
+      w.seg[s] = g;
+    }
+    carry += sum;
   }
   const bool fits = carry < (1ll << 30);  // lengths beyond any cache: nothing is read
+  const int total = fits ? (int)carry : 0, n = active_ctas(total);
   if (tid == 0) {
     if (!fits) report_error(a.err, kErrBadShape);
-    tile0[a.num_segs] = w.tile0[a.num_segs] = fits ? (int)carry : 0;
-    *w.total = fits ? (int)carry : 0;
-  }
-  if (!fits) {
-    for (int s = tid; s < a.num_segs; s += 1024) w.nt[s] = w.tile0[s] = 0;
-    for (int e = tid; e < a.entries; e += 1024) w.entry[e] = make_int4(0, 0, 0, 0);
-    return;
+    cost0[a.num_segs] = w.seg[a.num_segs].cost0 = total;
+    *w.total = total;
   }
   __syncthreads();
   for (int e = tid; e < a.entries; e += 1024) {
-    const int s = a.entry_seg[e], e0 = a.seg_start[s], at = e - e0, nt = w.nt[s];
-    const int nq = (a.seg_start[s + 1] - e0 + rpu - 1) / rpu;
-    w.entry[e] = make_int4(tile0[s] + at / rpu * nt, nt, nq * nt, at % rpu * group_of(a));
+    const int s = e == tid ? seg0 : a.entry_seg[e], e0 = a.seg_start[s];
+    const int at = e - e0, nq = (a.seg_start[s + 1] - e0 + rpu - 1) / rpu, each = tiles[s] + UNIT_COST;
+    w.entry[e] = make_int4(cost0[s] + at / rpu * each, fits ? tiles[s] : 0, nq * each, at % rpu * group);
   }
-  const int total = (int)carry, n = active_ctas(total);
   for (int c = tid; c < n; c += 1024) {
-    const int t = first_tile(total, n, c);
-    int lo = 0, hi = a.num_segs;  // the last segment with tile0 <= t (empty ones before it share its tile0)
+    const int t = first_cost(total, n, c);
+    int lo = 0, hi = a.num_segs;  // the last segment with cost0 <= t (empty ones before it share its cost0)
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (tile0[mid] <= t) lo = mid; else hi = mid;
+      if (cost0[mid] <= t) lo = mid; else hi = mid;
     }
     w.cta_seg[c] = lo;
   }
@@ -143,47 +151,64 @@ __global__ void __launch_bounds__(1024) plan_kernel(const SharedAttnArgs a) {
 
 // A CTA's part of one unit: tiles [t0, t1).
 struct Fragment {
-  int seg, kvh, e0, slots, t0, t1, p0, pend, len;
+  int kvh, e0, slots, t0, t1, p0, pend, len;
   const int* pt;
-  bool first;  // holds the unit's first tile
 };
 
 struct Walk {
   int pos, end, seg, rpu, group;
   ZS_DEVICE bool next(const SharedAttnArgs& a, const Work& w, Fragment& f) {
-    if (pos >= end) return false;
-    while (pos >= w.tile0[seg + 1]) ++seg;
-    const int nt = w.nt[seg], at = pos - w.tile0[seg], u = at / nt;
-    const int e0 = a.seg_start[seg], rows = a.seg_start[seg + 1] - e0, nq = (rows + rpu - 1) / rpu;
-    const int qt = u % nq;  // the units of one kv head follow one another: they read the same pages
-    f.seg = seg;
-    f.kvh = u / nq;
-    f.e0 = e0 + qt * rpu;
-    f.slots = min(rpu, rows - qt * rpu) * group;
-    f.t0 = at - u * nt;
-    f.t1 = min(nt, f.t0 + end - pos);
-    f.p0 = a.seg_page0[seg];
-    f.pend = w.pend[seg];
-    f.len = w.len[seg];
-    f.pt = a.page_table + (size_t)w.slot[seg] * a.max_pages;
-    f.first = f.t0 == 0;
-    pos += f.t1 - f.t0;
-    return true;
+    while (pos < end) {
+      const int4* at4 = reinterpret_cast<const int4*>(w.seg + seg);
+      const int4 x = __ldg(at4), y = __ldg(at4 + 1);
+      if (pos >= __ldg(&w.seg[seg + 1].cost0)) {
+        ++seg;
+        continue;
+      }
+      const int nt = x.y, each = nt + UNIT_COST, u = (pos - x.x) / each, at = pos - x.x - u * each;
+      f.t0 = max(0, at - UNIT_COST);
+      f.t1 = min(nt, at - UNIT_COST + end - pos);
+      pos += min(each - at, end - pos);
+      if (f.t1 <= f.t0) continue;
+      const int nq = (x.w + rpu - 1) / rpu, qt = u % nq;  // the units of one kv head follow one another: they read the same pages
+      f.kvh = u / nq;
+      f.e0 = x.z + qt * rpu;
+      f.slots = min(rpu, x.w - qt * rpu) * group;
+      f.p0 = y.x;
+      f.pend = y.y;
+      f.len = y.z;
+      f.pt = a.page_table + (size_t)y.w * a.max_pages;
+      return true;
+    }
+    return false;
+  }
+};
+
+// Position in the ring of stages and the parity of its barriers there.
+struct Ring {
+  int st = 0, ph = 0;
+  ZS_DEVICE void next(int n = 1) {
+    st += n;
+    if (st >= STAGES) {
+      st -= STAGES;
+      ph ^= 1;
+    }
   }
 };
 
 struct Smem {
   uint8_t ring[STAGES][STAGE];      // tiles as page images: K, V, K, V, ...
-  float stage[8][32][68];           // a warp's 32 slots x 64 dims of O on their way out
+  uint8_t way[SLOTS][512];          // Q on its way in and O on its way out: 256 bytes of a row for each half
   float top[2][2][SLOTS];           // per half of a tile's keys, the largest score of every slot
   int vote[2][8];
   int again[2];                     // the P of this tile is followed by its rounding errors
-  float odd[SLOTS], sum[SLOTS];
-  int least;                        // shortest visible length among a fragment's rows
+  int least[2];                     // shortest visible length among a fragment's rows
   volatile int abort;
   uint32_t tmem;
   uint64_t full[STAGES], empty[STAGES], s_full[2], p_full[2], o_full[2], q_full;
 };
+constexpr int SMEM = (int)sizeof(Smem);
+static_assert(SMEM <= 232448, "shared memory of one CTA");
 
 // Waits give up when one of them in the CTA has run out (the error word is set then).
 ZS_DEVICE bool wait_for(Smem& s, uint64_t* bar, uint32_t phase, int* err) {
@@ -228,13 +253,10 @@ ZS_DEVICE float pick(bool c, float x, float y) {
   asm("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\tselp.f32 %0, %1, %2, p;\n\t}" : "=f"(r) : "f"(x), "f"(y), "r"((int)c));
   return r;
 }
-// A thread's own row in shared memory to global memory (16-byte aligned, a multiple of 16 bytes).
-ZS_DEVICE void bulk_store(void* dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes) : "memory");
+ZS_DEVICE void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
-ZS_DEVICE void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-ZS_DEVICE void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-ZS_DEVICE void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+ZS_DEVICE void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // One tcgen05.mma with A in TMEM.  The B descriptors of a product differ in their low words alone
 // (start address, leading offset): the high word (stride, version, 128-byte swizzle) is a constant.
@@ -269,19 +291,23 @@ constexpr float kGrow = 8.f;         // O is rescaled when a maximum grows by mo
 // then carries only the copies in and one read of K and V per tile (with Q and P^T there the
 // kernel was bound by shared-memory bandwidth).  A row of S, P and O is one TMEM lane; thread
 // (half, slot) of the softmax warps owns half of the keys of a tile, and of the dims of O.
-//  * copy warp: page ids, then one bulk copy per (page, kv head) block into a ring of four 32 KiB
+//  * copy warp: page ids, then one bulk copy per (page, kv head) block into a ring of five 32 KiB
 //    stages, running ahead across tiles and fragments;
 //  * MMA warp: S of the next tile is issued before O of this one, so it runs under the softmax;
 //  * softmax warps: P = 2^(s - m) with a reference m that follows the running maximum only when
 //    that grows by more than 2^8 (P stays below 2^8, O and l in fp32), so O in TMEM is rescaled
-//    rarely; the next fragment's Q is fetched during the last tile.
+//    rarely; the next fragment's Q goes to TMEM before this one's record leaves it.
 // P is rounded to bf16 for the tensor cores, 2^-8 of a weight; over many keys those errors
 // average out, and where a weight is more than a quarter of its half's sum before its tile
 // (first tiles, few keys, peaked rows) a second product adds what the rounding lost.  l sums the
 // weights before they are rounded.
 __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs a) {
   extern __shared__ __align__(1024) uint8_t raw[];
-  Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  Smem& s = *reinterpret_cast<Smem*>(raw);
+  if ((smem_u32(raw) & 1023) != 0) {  // the swizzled images need it
+    report_error(a.err, kErrBadShape);
+    return;
+  }
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (warp == 9) {
     tmem_alloc(&s.tmem, kTmemCols);
@@ -311,8 +337,8 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
   const int total = *w.total, n = active_ctas(total), cta = blockIdx.x;
   Walk walk{0, 0, 0, SLOTS / group_of(a), group_of(a)};
   if (cta < n) {
-    walk.pos = first_tile(total, n, cta);
-    walk.end = first_tile(total, n, cta + 1);
+    walk.pos = first_cost(total, n, cta);
+    walk.end = first_cost(total, n, cta + 1);
     walk.seg = w.cta_seg[cta];
   }
   Fragment f;
@@ -322,7 +348,8 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
     // Lane j holds the page id of the tile's page j and issues its K and V blocks.
     const char* kc = static_cast<const char*>(a.k_cache);
     const char* vc = static_cast<const char*>(a.v_cache);
-    int i = 0, issued = 0;  // tiles, stage uses
+    Ring r;
+    int issued = 0;
     bool ok = true;
     while (ok && walk.next(a, w, f)) {
       auto page_of = [&](int t) {
@@ -331,7 +358,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
         return p < a.max_pages ? __ldg(f.pt + p) : -1;  // a length behind the table row: a bad page
       };
       int page = page_of(f.t0);
-      for (int t = f.t0; ok && t < f.t1; ++t, ++i) {
+      for (int t = f.t0; ok && t < f.t1; ++t) {
         const int after = t + 1 < f.t1 ? page_of(t + 1) : 0;
         const int np = min(TPAGES, f.pend - (f.p0 + t * TPAGES));
         if (page < 0 || page >= a.num_pages) {
@@ -341,13 +368,13 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
         const size_t at = ((size_t)page * a.num_kv_heads + f.kvh) * BLOCK;
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
-          const int st = (2 * i + kv) & (STAGES - 1);
-          if (i >= 2) ok = ok && wait_for(s, &s.empty[st], ((i >> 1) - 1) & 1, a.err);
+          ok = ok && wait_for(s, &s.empty[r.st], r.ph ^ 1, a.err);  // passes at once in the first round
           ok = __all_sync(0xffffffff, ok);
           if (!ok) break;
-          if (lane == 0) mbar_expect_tx(&s.full[st], np * BLOCK);
+          if (lane == 0) mbar_expect_tx(&s.full[r.st], np * BLOCK);
           __syncwarp();
-          if (lane < np) bulk_load(s.ring[st] + lane * BLOCK, (kv ? vc : kc) + at, BLOCK, &s.full[st]);
+          if (lane < np) bulk_load(s.ring[r.st] + lane * BLOCK, (kv ? vc : kc) + at, BLOCK, &s.full[r.st]);
+          r.next();
           ++issued;
         }
         page = after;
@@ -355,7 +382,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
     }
     // Copies in flight land before the CTA gives its shared memory back.
     if (lane == 0)
-      for (int m = max(0, issued - STAGES); m < issued; ++m) mbar_wait(&s.full[m & (STAGES - 1)], (m / STAGES) & 1, nullptr);
+      for (int m = max(0, issued - STAGES); m < issued; ++m) mbar_wait(&s.full[m % STAGES], (m / STAGES) & 1, nullptr);
   } else if (warp == 9) {
     // -------------------------------------------------------------------- MMA
     // The warp stays together; one elected lane issues.
@@ -363,9 +390,11 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
     const uint32_t idesc_s = make_idesc_bf16(SLOTS, TILE, 0, 0), idesc_o = make_idesc_bf16(SLOTS, D, 0, 1);
     const uint32_t k_lo = desc_lo(s.ring, 16), v_lo = desc_lo(s.ring, 1024);
     int ns = 0, no = 0;  // issued products
+    Ring kr, vr;
+    vr.next();
     auto scores = [&](int i) {  // S of tile i
-      const int st = (2 * i) & (STAGES - 1);
-      if (!wait_for(s, &s.full[st], (i >> 1) & 1, a.err)) return false;
+      const int st = kr.st;
+      if (!wait_for(s, &s.full[st], kr.ph, a.err)) return false;
       // It takes the place of the P two tiles before: products with different accumulators have
       // no order of their own.
       if (i >= 2 && !wait_for(s, &s.o_full[i & 1], ((i >> 1) - 1) & 1, a.err)) return false;
@@ -378,13 +407,14 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
         tc_commit(&s.empty[st]);
         tc_commit(&s.s_full[i & 1]);
       }
+      kr.next(2);
       ++ns;
       return true;
     };
     // O of tile i.
     auto output = [&](int i, bool fresh) {
-      const int st = (2 * i + 1) & (STAGES - 1), b = i & 1;
-      if (!wait_for(s, &s.full[st], (i >> 1) & 1, a.err)) return false;
+      const int st = vr.st, b = i & 1;
+      if (!wait_for(s, &s.full[st], vr.ph, a.err)) return false;
       if (!wait_for(s, &s.p_full[b], (i >> 1) & 1, a.err)) return false;
       tc_fence_after();
       const uint32_t v_at = v_lo + st * (STAGE / 16), p_at = tmem + b * TILE;
@@ -401,17 +431,20 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
         tc_commit(&s.empty[st]);
         tc_commit(&s.o_full[b]);
       }
+      vr.next(2);
       ++no;
       return true;
     };
-    int i = 0, nf = 0;
-    bool ok = true;
-    for (; ok && walk.next(a, w, f); ++nf) {
+    int i = 0;
+    bool ok = true, more = walk.next(a, w, f);
+    for (int nf = 0; ok && more; ++nf) {
       ok = wait_for(s, &s.q_full, nf & 1, a.err) && scores(i);
       ok = __all_sync(0xffffffff, ok);
-      for (int t = f.t0; ok && t < f.t1; ++t, ++i) {
-        if (t + 1 < f.t1) ok = scores(i + 1);
-        ok = ok && output(i, t == f.t0);
+      const int t0 = f.t0, t1 = f.t1;
+      more = walk.next(a, w, f);  // looked up while the first tile is worked on
+      for (int t = t0; ok && t < t1; ++t, ++i) {
+        if (t + 1 < t1) ok = scores(i + 1);
+        ok = ok && output(i, t == t0);
         ok = __all_sync(0xffffffff, ok);
       }
     }
@@ -425,66 +458,73 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);  // this warp's quarter of TMEM
     const float qscale = a.sm_scale * 1.4426950408889634f;             // exp2 domain
     const int group = walk.group;
-    // This thread's half of its slot's query: 128 dims.
-    uint4 qv[16];
-    auto fetch_q = [&](const Fragment& g) {
-      if (slot < g.slots) {
-        const int row = a.seg_rows[g.e0 + slot / group];
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) +
-                                                          ((size_t)row * a.num_q_heads + g.kvh * group + slot % group) * D) + half * 16;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) qv[j] = __ldg(src + j);
+    const int head = slot % group;
+    auto row_of = [&](const Fragment& g) { return slot < g.slots ? a.seg_rows[g.e0 + slot / group] : -1; };
+    auto limit_of = [&](const Fragment& g, int row) { return row >= 0 ? min(a.seq_lens[row], g.len) : 0x7FFFFFFF; };  // keys it sees
+    // A warp's rows and half of the way: 16-byte piece p of slot r lies at piece p ^ (r % 8).
+    auto way = [&](int r, int p) { return s.way[r] + (((half * 16 + p) ^ (r & 7)) << 4); };
+    // Half of the queries of the warp's slots, two rows an instruction.
+    auto fetch_q = [&](const Fragment& g, int row) {
+      for (int j = 0; j < 16; ++j) {
+        const int x = 2 * j + (lane >> 4), r = (warp & 3) * 32 + x;
+        const int rr = __shfl_sync(0xffffffff, row, x), hh = __shfl_sync(0xffffffff, head, x);
+        if (rr >= 0)
+          cp_async16(way(r, lane & 15), static_cast<const char*>(a.q) +
+                                            (((size_t)rr * a.num_q_heads + g.kvh * group + hh) * D + half * 128 + (lane & 15) * 8) * 2);
       }
     };
     auto store_q = [&](const Fragment& g) {
       if ((warp & 3) * 32 < g.slots) {
+        cp_async_wait();
+        __syncwarp();
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           uint32_t r[16];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            r[4 * k] = qv[4 * j + k].x;
-            r[4 * k + 1] = qv[4 * j + k].y;
-            r[4 * k + 2] = qv[4 * j + k].z;
-            r[4 * k + 3] = qv[4 * j + k].w;
-          }
+          for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(r + 4 * k) = *reinterpret_cast<const uint4*>(way(slot, 4 * j + k));
           tmem_st_32x32b_x16(lanes + kTmemQ + half * 64 + j * 16, r);
         }
         tmem_st_wait();
+        __syncwarp();
       }
       tc_fence_before();
       mbar_arrive(&s.q_full);
     };
+    auto note_least = [&](int limit, int b) {
+      const int least = __reduce_min_sync(0xffffffff, limit);
+      if (lane == 0 && least < 0x7FFFFFFF) atomicMin(&s.least[b], least);
+    };
     // After a wait that gave up these warps go on to the end with whatever is there (the error word
     // is set, every later wait gives up at once): their barriers always meet.
     bool more = walk.next(a, w, f);
+    int row = -1, limit = 0x7FFFFFFF;
+    if (tid == 0) s.least[0] = 0x7FFFFFFF;
+    compute_sync();
     if (more) {
-      fetch_q(f);
+      row = row_of(f);
+      fetch_q(f, row);
+      limit = limit_of(f, row);
+      note_least(limit, 0);
       store_q(f);
+      compute_sync();
     }
     int i = 0;
-    while (more) {
+    Ring vr;
+    vr.next();
+    for (int nf = 0; more; ++nf) {
+      const bool used = row >= 0, busy = (warp & 3) * 32 < f.slots;
+      const int least = s.least[nf & 1];
+      // The next fragment is looked up now, its queries and its rows' lengths after the first tile.
       Fragment g;
-      const bool used = slot < f.slots, busy = (warp & 3) * 32 < f.slots;
-      const int limit = used ? min(a.seq_lens[a.seg_rows[f.e0 + slot / group]], f.len) : 0x7FFFFFFF;  // keys this slot sees
-      {
-        const int least = __reduce_min_sync(0xffffffff, limit);
-        if (tid == 0) s.least = 0x7FFFFFFF;
-        compute_sync();
-        if (lane == 0) atomicMin(&s.least, least);
-        compute_sync();
-      }
-      const int least = s.least;
+      more = walk.next(a, w, g);
+      const int next_row = more ? row_of(g) : -1;
+      int next_limit = 0x7FFFFFFF;
+      if (tid == 0) s.least[(nf + 1) & 1] = 0x7FFFFFFF;
       float m = -INFINITY, l = 0.f;  // reference maximum (raw scores) of the slot, sum of this half's weights
-      for (int t = f.t0; t < f.t1; ++t, ++i) {
+      for (int t = f.t0; t < f.t1; ++t, ++i, vr.next(2)) {
         const int b = i & 1, key0 = (f.p0 + t * TPAGES) * PAGE;
         wait_for(s, &s.s_full[b], (i >> 1) & 1, a.err);
         tc_fence_after();
-        const bool last = t + 1 == f.t1;
-        if (last) {  // every product with Q is done: the next fragment's Q can come
-          more = walk.next(a, w, g);
-          if (more) fetch_q(g);
-        }
         uint32_t r[32];
         float mt = -INFINITY;
         const int valid = limit - key0 - half * 32;
@@ -568,8 +608,8 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
         const int end = f.len - key0;  // keys of the tile that some row sees
         unsigned long long odd = 0;
         if (end < TILE || least < key0 + TILE) {
-          const int st = (2 * i + 1) & (STAGES - 1);
-          wait_for(s, &s.full[st], (i >> 1) & 1, a.err);
+          const int st = vr.st;
+          wait_for(s, &s.full[st], vr.ph, a.err);
           const int from = max(0, min(least - key0, TILE)), stop = min(end, TILE);
           bool found = false;
           for (int x = from * 32 + tid; x < stop * 32; x += COMPUTE) {
@@ -601,13 +641,13 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
               float p = 0.f;
 #pragma unroll
               for (int j = 0; j < 32; ++j) p = pick(j == (k & 31), __uint_as_float(r[j]), p);
-              s.odd[slot] = p;
+              s.top[b][0][slot] = p;
             }
             compute_sync();
             const int at_page = (key0 + k) / PAGE, page = at_page < a.max_pages ? f.pt[at_page] : -1;
             if (!busy || page < 0 || page >= a.num_pages) continue;
             const uint8_t* blk = static_cast<const uint8_t*>(a.v_cache) + ((size_t)page * a.num_kv_heads + f.kvh) * BLOCK;
-            const float p = s.odd[slot];
+            const float p = s.top[b][0][slot];
             for (int c = 0; c < 128; c += 16) {
               uint32_t o[16];
               const uint32_t at = lanes + kTmemO + half * 128 + c;
@@ -625,40 +665,54 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
           }
           tc_fence_before();
         }
+        if (more && t == f.t0) {
+          fetch_q(g, next_row);
+          next_limit = limit_of(g, next_row);
+          note_least(next_limit, (nf + 1) & 1);
+        }
       }
-      if (more) store_q(g);
+      if (f.t1 - f.t0 == 1) compute_sync();  // the next shortest length is complete
+      if (more) store_q(g);                  // every product with the last Q is done
       // ---- the fragment's records: those of the unit's first fragment lie by (entry, head), those of
-      // a later one by CTA and slot
-      if (half == 1) s.sum[slot] = l;
-      compute_sync();
+      // a later one by CTA and slot.  They pass through shared memory so that the stores are whole lines.
       wait_for(s, &s.o_full[(i - 1) & 1], ((i - 1) >> 1) & 1, a.err);
       tc_fence_after();
       if (busy) {
-        const size_t at = f.first ? (size_t)(f.e0 + slot / group) * a.num_q_heads + f.kvh * group + slot % group
-                                  : (size_t)a.entries * a.num_q_heads + (size_t)cta * SLOTS + slot;
-        float* rec = a.partial + at * PREC;
-        float* row = s.stage[warp][lane];
+        const size_t at = f.t0 == 0 ? (size_t)(f.e0 + slot / group) * a.num_q_heads + f.kvh * group + head
+                                    : (size_t)a.entries * a.num_q_heads + (size_t)cta * SLOTS + slot;
+        const int rows = min(32, f.slots - (warp & 3) * 32);
 #pragma unroll
-        for (int c = 0; c < 128; c += 64) {
-          bulk_wait_read();
+        for (int c = 0; c < 2; ++c) {
 #pragma unroll
-          for (int q = 0; q < 64; q += 32) {
+          for (int q = 0; q < 2; ++q) {
             uint32_t o[32];
-            tmem_ld_32x32b_x32(lanes + kTmemO + half * 128 + c + q, o);
+            tmem_ld_32x32b_x32(lanes + kTmemO + half * 128 + c * 64 + q * 32, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(row + q + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+            for (int j = 0; j < 8; ++j)
+              *reinterpret_cast<uint4*>(way(slot, q * 8 + j)) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
           }
-          fence_proxy_async_shared();
-          if (used) bulk_store(rec + half * 128 + c, row, 256);
-          bulk_commit();
+          __syncwarp();
+          for (int j = 0; 2 * j < rows; ++j) {
+            const int x = 2 * j + (lane >> 4);
+            const size_t to = __shfl_sync(0xffffffff, at, x);
+            if (x < rows)
+              *reinterpret_cast<uint4*>(a.partial + to * PREC + half * 128 + c * 64 + (lane & 15) * 4) =
+                  *reinterpret_cast<const uint4*>(way((warp & 3) * 32 + x, lane & 15));
+          }
+          __syncwarp();
         }
-        if (used && half == 0) *reinterpret_cast<float2*>(rec + D) = make_float2(m * qscale, l + s.sum[slot]);
+        if (used) {
+          float* end = a.partial + at * PREC + D;
+          if (half == 0) *reinterpret_cast<float2*>(end) = make_float2(m * qscale, l);
+          else end[2] = l;
+        }
       }
       tc_fence_before();
       f = g;
+      row = next_row;
+      limit = next_limit;
     }
-    bulk_wait();
   }
   tc_fence_before();
   __syncthreads();
@@ -667,15 +721,23 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
 }
 
 constexpr int MERGE_WARPS = 8;
+// (row, q head) pairs up to which a whole CTA merges one of them, its warps sharing the records:
+// with few rows a long prefix leaves a record in every CTA.  Above, a warp each: 16 x 64 pairs of
+// two or three records take 4.6 us with a CTA each and 3.3 us with a warp each, 64 pairs of 33
+// records 4.3 and 8.9 us.
+constexpr int MERGE_WIDE = 512;
 
-// One warp per (row, q head); a lane owns dims 4 lane .. + 3 and 128 + 4 lane .. + 3.  Records are
-// found and weighed 32 at a time (one a lane), then added in order.
+// A lane owns dims 4 lane .. + 3 and 128 + 4 lane .. + 3.  Records are found and weighed 32 at a
+// time (one a lane), then added in order; with PARTS warps on a pair, warp p takes every PARTS-th
+// record and the parts are joined in order.
+template <int PARTS>
 __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const SharedAttnArgs a) {
   pdl_wait();
   pdl_trigger();
   const Work w = work_of(a);
-  const int item = blockIdx.x * MERGE_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (item >= a.rows * a.num_q_heads) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % PARTS;
+  const int item = blockIdx.x * (MERGE_WARPS / PARTS) + warp / PARTS;
+  if (item >= a.rows * a.num_q_heads) return;  // PARTS == 1 alone
   const int row = item / a.num_q_heads, h = item % a.num_q_heads, group = group_of(a);
   const int total = *w.total, n = active_ctas(total);
   float m = -INFINITY, l = 0.f, o[8] = {};
@@ -684,19 +746,20 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const SharedAtt
     if (e < 0) break;
     const int4 u = w.entry[e];
     if (u.y == 0) continue;
-    const int first = u.x + h / group * u.z;
+    const int first = u.x + h / group * u.z + UNIT_COST;
     const int c0 = cta_of(total, n, first), c1 = cta_of(total, n, first + u.y - 1);
-    for (int c = c0; c <= c1; c += 32) {
-      const size_t at = c + lane == c0 ? (size_t)e * a.num_q_heads + h
-                                       : (size_t)a.entries * a.num_q_heads + (size_t)(c + lane) * SLOTS + u.w + h % group;
-      const float2 ml = c + lane <= c1 ? *reinterpret_cast<const float2*>(a.partial + at * PREC + D) : make_float2(-INFINITY, 0.f);
+    for (int c = c0 + part; c <= c1; c += 32 * PARTS) {
+      const int mine = c + lane * PARTS;
+      const size_t at = mine == c0 ? (size_t)e * a.num_q_heads + h
+                                   : (size_t)a.entries * a.num_q_heads + (size_t)mine * SLOTS + u.w + h % group;
+      const float4 ml = mine <= c1 ? *reinterpret_cast<const float4*>(a.partial + at * PREC + D) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
       const float mn = fmaxf(m, warp_max(ml.x)), s0 = m == -INFINITY ? 0.f : exp2f(m - mn);
       const float wt = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mn);
-      l = l * s0 + warp_sum(ml.x == -INFINITY ? 0.f : wt * ml.y);
+      l = l * s0 + warp_sum(ml.x == -INFINITY ? 0.f : wt * (ml.y + ml.z));
 #pragma unroll
       for (int k = 0; k < 8; ++k) o[k] *= s0;
       m = mn;
-      const int cnt = min(32, c1 - c + 1);
+      const int cnt = min(32, (c1 - c) / PARTS + 1);
 #pragma unroll 4
       for (int x = 0; x < cnt; ++x) {
         const float wx = __shfl_sync(0xffffffff, wt, x);
@@ -712,6 +775,30 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const SharedAtt
         o[6] += wx * q.z;
         o[7] += wx * q.w;
       }
+    }
+  }
+  if (PARTS > 1) {
+    __shared__ float parts[PARTS][D + 2];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) parts[part][(k >> 2) * 128 + lane * 4 + (k & 3)] = o[k];
+    if (lane == 0) {
+      parts[part][D] = m;
+      parts[part][D + 1] = l;
+    }
+    __syncthreads();
+    if (part != 0) return;
+    const float mp = lane < PARTS ? parts[lane][D] : -INFINITY;
+    m = warp_max(mp);
+    const float wp = mp == -INFINITY ? 0.f : exp2f(mp - m);
+    l = warp_sum(mp == -INFINITY ? 0.f : wp * parts[lane][D + 1]);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o[k] = 0.f;
+#pragma unroll
+    for (int x = 0; x < PARTS; ++x) {
+      const float wx = __shfl_sync(0xffffffff, wp, x);
+      if (wx == 0.f) continue;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) o[k] += wx * parts[x][(k >> 2) * 128 + lane * 4 + (k & 3)];
     }
   }
   const float inv = m == -INFINITY ? 0.f : 1.f / l;
@@ -771,11 +858,11 @@ extern "C" int zs_shared_attn(const SharedAttnArgs* args, cudaStream_t stream) {
   if (int e = zs::sattn::check(a)) return e;
   if (a.partial == nullptr || !(a.sm_scale > 0.f) || a.num_pages < 1) return -1;
   if (a.rows == 0) return 0;
-  const size_t smem = sizeof(zs::sattn::Smem) + 1024;
-  cudaFuncSetAttribute(zs::sattn::tiles_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  zs_launch(zs::sattn::tiles_kernel, zs::sattn::CTAS, zs::sattn::THREADS, smem, stream, a);
+  using namespace zs::sattn;
+  cudaFuncSetAttribute(tiles_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+  zs_launch(tiles_kernel, CTAS, THREADS, SMEM, stream, a);
   const int items = a.rows * a.num_q_heads;
-  zs_launch(zs::sattn::merge_kernel, (items + zs::sattn::MERGE_WARPS - 1) / zs::sattn::MERGE_WARPS, zs::sattn::MERGE_WARPS * 32, 0,
-            stream, a);
+  if (items <= MERGE_WIDE) zs_launch(merge_kernel<MERGE_WARPS>, items, MERGE_WARPS * 32, 0, stream, a);
+  else zs_launch(merge_kernel<1>, (items + MERGE_WARPS - 1) / MERGE_WARPS, MERGE_WARPS * 32, 0, stream, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
