@@ -28,18 +28,19 @@ constexpr int SLOTS = ZS_SHARED_SLOTS;   // query slots of a unit
 constexpr int TILE = 64;                 // keys of a tile
 constexpr int TPAGES = TILE / PAGE;
 constexpr int STAGE = TPAGES * BLOCK;    // one tile of K or V: 32 KiB
-constexpr int STAGES = 5;
-constexpr int COMPUTE = 256;             // softmax threads (warps 0-7), then a copy and an MMA warp
-constexpr int THREADS = COMPUTE + 64;
+constexpr int STAGES = 4;
+constexpr int COMPUTE = 256;             // softmax threads (warps 0-7), then a copy, an MMA and a lookup warp
+constexpr int THREADS = COMPUTE + 96;
+constexpr int AHEAD = 3;                 // fragments known at a time
 constexpr int CTAS = ZS_SHARED_CTAS;
 constexpr int MAX_SEGS = ZS_SHARED_MAX_SEGS;
 
-// A unit costs its tiles and UNIT_COST tiles more (its Q, its record, a pipeline that starts anew).
-constexpr int UNIT_COST = 2;
+// A unit costs its tiles and a few tiles more: a pipeline that starts anew, its Q and its record.
+ZS_DEVICE int unit_cost(int rows, int rpu, int group) { return 2 + min(rows, rpu) * group / 64; }
 
 // The plan (ints): the cost of everything, a Segment for each segment and one behind the last
-// (its cost0 alone), per entry (kv head 0) its unit's first cost, its tiles, the distance to the
-// next kv head's unit and its first slot, and the first segment of every CTA.
+// (its cost0 alone), per entry (kv head 0) its unit's first tile (as a cost), its tiles, the distance to the
+// next kv head's unit and its first slot, and the range of costs and first segment of every CTA.
 struct Segment {
   int cost0, nt, e0, rows;   // cost before it, tiles of a unit, first entry, rows
   int p0, pend, len, slot;   // pages [p0, pend), its longest row's length (at most their end) and table row
@@ -47,15 +48,14 @@ struct Segment {
 struct Work {
   int* total;
   Segment* seg;
-  int4* entry;
-  int* cta_seg;
+  int4 *entry, *cta;
 };
 __host__ __device__ inline Work work_of(const SharedAttnArgs& a) {
   Work w;
   w.total = a.work;
   w.seg = reinterpret_cast<Segment*>(a.work + 4);
   w.entry = reinterpret_cast<int4*>(w.seg + a.num_segs + 1);
-  w.cta_seg = reinterpret_cast<int*>(w.entry + a.entries);
+  w.cta = w.entry + a.entries;
   return w;
 }
 
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const SharedAttnArgs a) {
       if (p1 >= 0) g.pend = min(g.pend, p1);
       g.nt = (max(g.pend - g.p0, 0) + TPAGES - 1) / TPAGES;
       g.len = (int)min((long long)len, (long long)g.pend * PAGE);
-      if (g.nt > 0) cost = (long long)(g.nt + UNIT_COST) * ((g.rows + rpu - 1) / rpu) * a.num_kv_heads;
+      if (g.nt > 0) cost = (long long)(g.nt + unit_cost(g.rows, rpu, group)) * ((g.rows + rpu - 1) / rpu) * a.num_kv_heads;
     }
     long long x = cost;
 #pragma unroll
@@ -135,24 +135,24 @@ __global__ void __launch_bounds__(1024) plan_kernel(const SharedAttnArgs a) {
   __syncthreads();
   for (int e = tid; e < a.entries; e += 1024) {
     const int s = e == tid ? seg0 : a.entry_seg[e], e0 = a.seg_start[s];
-    const int at = e - e0, nq = (a.seg_start[s + 1] - e0 + rpu - 1) / rpu, each = tiles[s] + UNIT_COST;
-    w.entry[e] = make_int4(cost0[s] + at / rpu * each, fits ? tiles[s] : 0, nq * each, at % rpu * group);
+    const int rows = a.seg_start[s + 1] - e0, more = unit_cost(rows, rpu, group);
+    const int at = e - e0, nq = (rows + rpu - 1) / rpu, each = tiles[s] + more;
+    w.entry[e] = make_int4(cost0[s] + at / rpu * each + more, fits ? tiles[s] : 0, nq * each, at % rpu * group);
   }
-  for (int c = tid; c < n; c += 1024) {
-    const int t = first_cost(total, n, c);
+  for (int c = tid; c < CTAS; c += 1024) {
+    const int t = c < n ? first_cost(total, n, c) : 0;
     int lo = 0, hi = a.num_segs;  // the last segment with cost0 <= t (empty ones before it share its cost0)
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (cost0[mid] <= t) lo = mid; else hi = mid;
     }
-    w.cta_seg[c] = lo;
+    w.cta[c] = make_int4(t, c < n ? first_cost(total, n, c + 1) : 0, lo, 0);
   }
 }
 
 // A CTA's part of one unit: tiles [t0, t1).
 struct Fragment {
-  int kvh, e0, slots, t0, t1, p0, pend, len;
-  const int* pt;
+  int kvh, e0, slots, t0, t1, p0, pend, len, table;
 };
 
 struct Walk {
@@ -165,9 +165,9 @@ struct Walk {
         ++seg;
         continue;
       }
-      const int nt = x.y, each = nt + UNIT_COST, u = (pos - x.x) / each, at = pos - x.x - u * each;
-      f.t0 = max(0, at - UNIT_COST);
-      f.t1 = min(nt, at - UNIT_COST + end - pos);
+      const int nt = x.y, cost = unit_cost(x.w, rpu, group), each = nt + cost, u = (pos - x.x) / each, at = pos - x.x - u * each;
+      f.t0 = max(0, at - cost);
+      f.t1 = min(nt, at - cost + end - pos);
       pos += min(each - at, end - pos);
       if (f.t1 <= f.t0) continue;
       const int nq = (x.w + rpu - 1) / rpu, qt = u % nq;  // the units of one kv head follow one another: they read the same pages
@@ -177,7 +177,7 @@ struct Walk {
       f.p0 = y.x;
       f.pend = y.y;
       f.len = y.z;
-      f.pt = a.page_table + (size_t)y.w * a.max_pages;
+      f.table = y.w;
       return true;
     }
     return false;
@@ -198,14 +198,16 @@ struct Ring {
 
 struct Smem {
   uint8_t ring[STAGES][STAGE];      // tiles as page images: K, V, K, V, ...
-  uint8_t way[SLOTS][512];          // Q on its way in and O on its way out: 256 bytes of a row for each half
+  uint8_t way[SLOTS][528];          // Q on its way in and O on its way out: 256 bytes of a row for each half
   float top[2][2][SLOTS];           // per half of a tile's keys, the largest score of every slot
   int vote[2][8];
   int again[2];                     // the P of this tile is followed by its rounding errors
-  int least[2];                     // shortest visible length among a fragment's rows
+  Fragment frag[AHEAD];             // t1 == 0: no more
+  int row[AHEAD][SLOTS], limit[AHEAD][SLOTS];  // row of each slot (-1: unused) and the keys it sees
+  int least[AHEAD];                 // the fewest of them
   volatile int abort;
   uint32_t tmem;
-  uint64_t full[STAGES], empty[STAGES], s_full[2], p_full[2], o_full[2], q_full;
+  uint64_t full[STAGES], empty[STAGES], s_full[2], p_full[2], o_full[2], q_full, f_full[AHEAD], f_empty[AHEAD], r_full[AHEAD], way_full, way_empty;
 };
 constexpr int SMEM = (int)sizeof(Smem);
 static_assert(SMEM <= 232448, "shared memory of one CTA");
@@ -253,11 +255,6 @@ ZS_DEVICE float pick(bool c, float x, float y) {
   asm("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\tselp.f32 %0, %1, %2, p;\n\t}" : "=f"(r) : "f"(x), "f"(y), "r"((int)c));
   return r;
 }
-ZS_DEVICE void cp_async16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-ZS_DEVICE void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-
 // One tcgen05.mma with A in TMEM.  The B descriptors of a product differ in their low words alone
 // (start address, leading offset): the high word (stride, version, 128-byte swizzle) is a constant.
 constexpr uint32_t desc_hi(uint32_t stride) { return (stride >> 4) | (1u << 14) | (2u << 29); }
@@ -291,12 +288,13 @@ constexpr float kGrow = 8.f;         // O is rescaled when a maximum grows by mo
 // then carries only the copies in and one read of K and V per tile (with Q and P^T there the
 // kernel was bound by shared-memory bandwidth).  A row of S, P and O is one TMEM lane; thread
 // (half, slot) of the softmax warps owns half of the keys of a tile, and of the dims of O.
-//  * copy warp: page ids, then one bulk copy per (page, kv head) block into a ring of five 32 KiB
+//  * copy warp: page ids, then one bulk copy per (page, kv head) block into a ring of four 32 KiB
 //    stages, running ahead across tiles and fragments;
 //  * MMA warp: S of the next tile is issued before O of this one, so it runs under the softmax;
+//  * lookup warp: the next fragments, their rows and lengths, and their Q into shared memory;
 //  * softmax warps: P = 2^(s - m) with a reference m that follows the running maximum only when
 //    that grows by more than 2^8 (P stays below 2^8, O and l in fp32), so O in TMEM is rescaled
-//    rarely; the next fragment's Q goes to TMEM before this one's record leaves it.
+//    rarely; the next fragment's Q goes to TMEM during this one's last tile.
 // P is rounded to bf16 for the tensor cores, 2^-8 of a weight; over many keys those errors
 // average out, and where a weight is more than a quarter of its half's sum before its tile
 // (first tiles, few keys, peaked rows) a second product adds what the rounding lost.  l sums the
@@ -324,6 +322,13 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
       mbar_init(&s.o_full[i], 1);
     }
     mbar_init(&s.q_full, COMPUTE);
+    for (int i = 0; i < AHEAD; ++i) {
+      mbar_init(&s.f_full[i], 1);
+      mbar_init(&s.r_full[i], 32);
+      mbar_init(&s.f_empty[i], COMPUTE / 32);
+    }
+    mbar_init(&s.way_full, 1);
+    mbar_init(&s.way_empty, COMPUTE);
     s.abort = 0;
     fence_barrier_init();
   }
@@ -333,14 +338,19 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
   const uint32_t tmem = s.tmem;
   pdl_wait();
   pdl_trigger();
-  const Work w = work_of(a);
-  const int total = *w.total, n = active_ctas(total), cta = blockIdx.x;
-  Walk walk{0, 0, 0, SLOTS / group_of(a), group_of(a)};
-  if (cta < n) {
-    walk.pos = first_cost(total, n, cta);
-    walk.end = first_cost(total, n, cta + 1);
-    walk.seg = w.cta_seg[cta];
-  }
+  const int cta = blockIdx.x, group = group_of(a);
+  // Fragment k of the CTA, once the lookup warp has it; false when there is none (or a wait gave up).
+  int fk = 0;
+  uint32_t fph = 0;
+  auto next_fragment = [&](Fragment& f) {
+    if (!wait_for(s, &s.f_full[fk], fph, a.err)) return false;
+    f = s.frag[fk];
+    if (++fk == AHEAD) {
+      fk = 0;
+      fph ^= 1;
+    }
+    return f.t1 > 0;
+  };
   Fragment f;
 
   if (warp == 8) {
@@ -351,11 +361,12 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
     Ring r;
     int issued = 0;
     bool ok = true;
-    while (ok && walk.next(a, w, f)) {
+    while (ok && __all_sync(0xffffffff, next_fragment(f))) {
+      const int* pt = a.page_table + (size_t)f.table * a.max_pages;
       auto page_of = [&](int t) {
         const int p = f.p0 + t * TPAGES + lane;
         if (lane >= TPAGES || p >= f.pend) return 0;
-        return p < a.max_pages ? __ldg(f.pt + p) : -1;  // a length behind the table row: a bad page
+        return p < a.max_pages ? __ldg(pt + p) : -1;  // a length behind the table row: a bad page
       };
       int page = page_of(f.t0);
       for (int t = f.t0; ok && t < f.t1; ++t) {
@@ -436,14 +447,18 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
       return true;
     };
     int i = 0;
-    bool ok = true, more = walk.next(a, w, f);
-    for (int nf = 0; ok && more; ++nf) {
-      ok = wait_for(s, &s.q_full, nf & 1, a.err) && scores(i);
-      ok = __all_sync(0xffffffff, ok);
+    bool more = __all_sync(0xffffffff, next_fragment(f));
+    bool ok = more && __all_sync(0xffffffff, wait_for(s, &s.q_full, 0, a.err) && scores(0));
+    for (int nf = 1; ok && more; ++nf) {
       const int t0 = f.t0, t1 = f.t1;
-      more = walk.next(a, w, f);  // looked up while the first tile is worked on
       for (int t = t0; ok && t < t1; ++t, ++i) {
-        if (t + 1 < t1) ok = scores(i + 1);
+        // S of the next tile, which may be the next fragment's first, goes before O of this one.
+        if (t + 1 < t1) {
+          ok = scores(i + 1);
+        } else {
+          more = __all_sync(0xffffffff, next_fragment(f));
+          if (more) ok = wait_for(s, &s.q_full, nf & 1, a.err) && scores(i + 1);
+        }
         ok = ok && output(i, t == t0);
         ok = __all_sync(0xffffffff, ok);
       }
@@ -452,79 +467,103 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
     if (ns > 0) mbar_wait(&s.s_full[(ns - 1) & 1], ((ns - 1) >> 1) & 1, nullptr);
     if (no > 0) mbar_wait(&s.o_full[(no - 1) & 1], ((no - 1) >> 1) & 1, nullptr);
     __syncwarp();
+  } else if (warp == 10) {
+    // ----------------------------------------------------------------- lookup
+    // What a fragment is, its rows and their lengths, AHEAD fragments before the others are done;
+    // and its Q into the way as soon as that is free.
+    const Work w = work_of(a);
+    const int4 mine = __ldg(w.cta + cta);
+    Walk walk{mine.x, mine.y, mine.z, SLOTS / group, group};
+    const char* qbase = static_cast<const char*>(a.q);
+    bool ok = true, more = true;
+    for (int k = 0, at = 0, ph = 0; ok && more; ++k) {
+      more = walk.next(a, w, f);
+      if (!more) f.t1 = 0;
+      ok = __all_sync(0xffffffff, wait_for(s, &s.f_empty[at], ph ^ 1, a.err));  // passes at once in the first round
+      if (lane == 0) {
+        s.frag[at] = f;
+        mbar_arrive(&s.f_full[at]);
+      }
+      if (!more) break;
+      int row[4], least = 0x7FFFFFFF;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) row[j] = j * 32 + lane < f.slots ? a.seg_rows[f.e0 + (j * 32 + lane) / group] : -1;
+      ok = ok && (k == 0 || wait_for(s, &s.way_empty, (k - 1) & 1, a.err));
+      ok = __all_sync(0xffffffff, ok);
+      if (!ok) break;
+      if (lane == 0) mbar_expect_tx(&s.way_full, f.slots * D * 2);
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (row[j] >= 0)
+          bulk_load(s.way[j * 32 + lane], qbase + ((size_t)row[j] * a.num_q_heads + f.kvh * group + (j * 32 + lane) % group) * (D * 2),
+                    D * 2, &s.way_full);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int limit = row[j] >= 0 ? min(a.seq_lens[row[j]], f.len) : 0x7FFFFFFF;
+        s.row[at][j * 32 + lane] = row[j];
+        s.limit[at][j * 32 + lane] = limit;
+        least = min(least, limit);
+      }
+      least = __reduce_min_sync(0xffffffff, least);
+      if (lane == 0) s.least[at] = least;
+      mbar_arrive(&s.r_full[at]);
+      if (++at == AHEAD) {
+        at = 0;
+        ph ^= 1;
+      }
+      ++fk;  // fragments whose Q was asked for
+    }
+    if (lane == 0 && fk > 0) mbar_wait(&s.way_full, (fk - 1) & 1, nullptr);  // no copy outlives the CTA
   } else {
     // ---------------------------------------------------------------- softmax
     const int half = warp >> 2, slot = (warp & 3) * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);  // this warp's quarter of TMEM
     const float qscale = a.sm_scale * 1.4426950408889634f;             // exp2 domain
-    const int group = walk.group;
     const int head = slot % group;
-    auto row_of = [&](const Fragment& g) { return slot < g.slots ? a.seg_rows[g.e0 + slot / group] : -1; };
-    auto limit_of = [&](const Fragment& g, int row) { return row >= 0 ? min(a.seq_lens[row], g.len) : 0x7FFFFFFF; };  // keys it sees
-    // A warp's rows and half of the way: 16-byte piece p of slot r lies at piece p ^ (r % 8).
-    auto way = [&](int r, int p) { return s.way[r] + (((half * 16 + p) ^ (r & 7)) << 4); };
-    // Half of the queries of the warp's slots, two rows an instruction.
-    auto fetch_q = [&](const Fragment& g, int row) {
-      for (int j = 0; j < 16; ++j) {
-        const int x = 2 * j + (lane >> 4), r = (warp & 3) * 32 + x;
-        const int rr = __shfl_sync(0xffffffff, row, x), hh = __shfl_sync(0xffffffff, head, x);
-        if (rr >= 0)
-          cp_async16(way(r, lane & 15), static_cast<const char*>(a.q) +
-                                            (((size_t)rr * a.num_q_heads + g.kvh * group + hh) * D + half * 128 + (lane & 15) * 8) * 2);
-      }
-    };
-    auto store_q = [&](const Fragment& g) {
-      if ((warp & 3) * 32 < g.slots) {
-        cp_async_wait();
-        __syncwarp();
+    auto way = [&](int r, int p) { return s.way[r] + ((half * 16 + p) << 4); };  // 16-byte piece p of the warp's half
+    auto store_q = [&](int slots, int k) {  // Q of fragment k from the way to TMEM
+      wait_for(s, &s.way_full, k & 1, a.err);
+      if ((warp & 3) * 32 < slots) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           uint32_t r[16];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(r + 4 * k) = *reinterpret_cast<const uint4*>(way(slot, 4 * j + k));
+          for (int x = 0; x < 4; ++x) *reinterpret_cast<uint4*>(r + 4 * x) = *reinterpret_cast<const uint4*>(way(slot, 4 * j + x));
           tmem_st_32x32b_x16(lanes + kTmemQ + half * 64 + j * 16, r);
         }
         tmem_st_wait();
-        __syncwarp();
       }
       tc_fence_before();
       mbar_arrive(&s.q_full);
     };
-    auto note_least = [&](int limit, int b) {
-      const int least = __reduce_min_sync(0xffffffff, limit);
-      if (lane == 0 && least < 0x7FFFFFFF) atomicMin(&s.least[b], least);
-    };
-    // After a wait that gave up these warps go on to the end with whatever is there (the error word
-    // is set, every later wait gives up at once): their barriers always meet.
-    bool more = walk.next(a, w, f);
-    int row = -1, limit = 0x7FFFFFFF;
-    if (tid == 0) s.least[0] = 0x7FFFFFFF;
-    compute_sync();
+    // After a wait that gave up these warps go on to the end of the fragment with whatever is there (the
+    // error word is set, every later wait gives up at once) and leave together: their barriers always meet.
+    bool more = !compute_any(!next_fragment(f));
+    int kf = 0;  // place of the fragment
+    uint32_t kph = 0;
     if (more) {
-      row = row_of(f);
-      fetch_q(f, row);
-      limit = limit_of(f, row);
-      note_least(limit, 0);
-      store_q(f);
-      compute_sync();
+      store_q(f.slots, 0);
+      fence_proxy_async_shared();
+      mbar_arrive(&s.way_empty);
     }
     int i = 0;
     Ring vr;
     vr.next();
     for (int nf = 0; more; ++nf) {
+      wait_for(s, &s.r_full[kf], kph, a.err);
+      const int row = s.row[kf][slot], limit = s.limit[kf][slot], least = s.least[kf];
       const bool used = row >= 0, busy = (warp & 3) * 32 < f.slots;
-      const int least = s.least[nf & 1];
-      // The next fragment is looked up now, its queries and its rows' lengths after the first tile.
       Fragment g;
-      more = walk.next(a, w, g);
-      const int next_row = more ? row_of(g) : -1;
-      int next_limit = 0x7FFFFFFF;
-      if (tid == 0) s.least[(nf + 1) & 1] = 0x7FFFFFFF;
       float m = -INFINITY, l = 0.f;  // reference maximum (raw scores) of the slot, sum of this half's weights
       for (int t = f.t0; t < f.t1; ++t, ++i, vr.next(2)) {
         const int b = i & 1, key0 = (f.p0 + t * TPAGES) * PAGE;
         wait_for(s, &s.s_full[b], (i >> 1) & 1, a.err);
         tc_fence_after();
+        if (t + 1 == f.t1) {  // every product with this Q is done: the next fragment's takes its place
+          more = !compute_any(!next_fragment(g));
+          if (more) store_q(g.slots, nf + 1);
+        }
         uint32_t r[32];
         float mt = -INFINITY;
         const int valid = limit - key0 - half * 32;
@@ -644,7 +683,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
               s.top[b][0][slot] = p;
             }
             compute_sync();
-            const int at_page = (key0 + k) / PAGE, page = at_page < a.max_pages ? f.pt[at_page] : -1;
+            const int at_page = (key0 + k) / PAGE, page = at_page < a.max_pages ? a.page_table[(size_t)f.table * a.max_pages + at_page] : -1;
             if (!busy || page < 0 || page >= a.num_pages) continue;
             const uint8_t* blk = static_cast<const uint8_t*>(a.v_cache) + ((size_t)page * a.num_kv_heads + f.kvh) * BLOCK;
             const float p = s.top[b][0][slot];
@@ -665,14 +704,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
           }
           tc_fence_before();
         }
-        if (more && t == f.t0) {
-          fetch_q(g, next_row);
-          next_limit = limit_of(g, next_row);
-          note_least(next_limit, (nf + 1) & 1);
-        }
       }
-      if (f.t1 - f.t0 == 1) compute_sync();  // the next shortest length is complete
-      if (more) store_q(g);                  // every product with the last Q is done
       // ---- the fragment's records: those of the unit's first fragment lie by (entry, head), those of
       // a later one by CTA and slot.  They pass through shared memory so that the stores are whole lines.
       wait_for(s, &s.o_full[(i - 1) & 1], ((i - 1) >> 1) & 1, a.err);
@@ -693,6 +725,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
               *reinterpret_cast<uint4*>(way(slot, q * 8 + j)) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
           }
           __syncwarp();
+#pragma unroll 4
           for (int j = 0; 2 * j < rows; ++j) {
             const int x = 2 * j + (lane >> 4);
             const size_t to = __shfl_sync(0xffffffff, at, x);
@@ -709,9 +742,15 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
         }
       }
       tc_fence_before();
+      fence_proxy_async_shared();
+      mbar_arrive(&s.way_empty);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.f_empty[kf]);
+      if (++kf == AHEAD) {
+        kf = 0;
+        kph ^= 1;
+      }
       f = g;
-      row = next_row;
-      limit = next_limit;
     }
   }
   tc_fence_before();
@@ -746,7 +785,7 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const SharedAtt
     if (e < 0) break;
     const int4 u = w.entry[e];
     if (u.y == 0) continue;
-    const int first = u.x + h / group * u.z + UNIT_COST;
+    const int first = u.x + h / group * u.z;
     const int c0 = cta_of(total, n, first), c1 = cta_of(total, n, first + u.y - 1);
     for (int c = c0 + part; c <= c1; c += 32 * PARTS) {
       const int mine = c + lane * PARTS;

@@ -697,7 +697,7 @@ typedef struct SharedAttnArgs {
   int* err;
 } SharedAttnArgs;
 
-#define ZS_SHARED_WORK_INTS(num_segs, entries) (4 + 8 * ((num_segs) + 1) + 4 * (entries) + ZS_SHARED_CTAS)
+#define ZS_SHARED_WORK_INTS(num_segs, entries) (4 + 8 * ((num_segs) + 1) + 4 * (entries) + 4 * ZS_SHARED_CTAS)
 
 // Divide the step's keys over the GPU (from seq_lens, row_slot, the segments and the head counts;
 // q, caches and outputs are not read): once a step.  Then one zs_shared_attn per layer.
