@@ -926,18 +926,20 @@ void draft_verify(const Tensor& target, const OptT& draft_probs, const Tensor& d
 // The plan's side of the shared-prefix attention arguments.
 SharedAttnArgs shared_plan_args(int64_t rows, int64_t num_q_heads, int64_t num_kv_heads, int64_t max_pages,
                                 const Tensor& row_slot, const Tensor& seq_lens, int64_t levels,
-                                const std::vector<Tensor>& segs, const Tensor& work, const Tensor& err) {
-  TORCH_CHECK(segs.size() == 6, "segments: seg_start, seg_rows, seg_page0, seg_page1, entry_seg, row_entry");
-  for (const Tensor* t : {&row_slot, &seq_lens, &segs[0], &segs[1], &segs[2], &segs[3], &segs[4], &segs[5], &work, &err}) {
+                                int64_t num_segs, const std::vector<Tensor>& segs, const Tensor& work, const Tensor& err) {
+  TORCH_CHECK(segs.size() == 5, "segments: seg_rows, entry_seg, entry_piece, row_entry, pieces");
+  for (const Tensor* t : {&row_slot, &seq_lens, &segs[0], &segs[1], &segs[2], &segs[3], &segs[4], &work, &err}) {
     check_cuda(*t, "index tensor");
     TORCH_CHECK(t->scalar_type() == at::kInt, "index tensors must be int32");
   }
-  TORCH_CHECK(row_slot.numel() == rows && seq_lens.numel() == rows && segs[5].numel() == rows * levels,
+  TORCH_CHECK(row_slot.numel() == rows && seq_lens.numel() == rows && segs[3].numel() == rows * levels,
               "row_slot, seq_lens and row_entry must have one entry per row");
-  const int64_t num_segs = segs[2].numel();
-  TORCH_CHECK(segs[0].numel() == num_segs + 1 && segs[3].numel() == num_segs && segs[4].numel() == segs[1].numel(),
+  const int64_t entries = segs[0].numel(), pieces = segs[4].numel() / 8;
+  TORCH_CHECK(segs[1].numel() == entries && segs[2].numel() == entries && segs[4].numel() % 8 == 0,
               "segment tensors do not fit together");
-  TORCH_CHECK(work.numel() >= ZS_SHARED_WORK_INTS(num_segs, segs[1].numel()) && reinterpret_cast<uintptr_t>(work.data_ptr()) % 16 == 0, "work too small or not 16-byte aligned");
+  TORCH_CHECK(work.numel() >= ZS_SHARED_WORK_INTS(pieces, entries) && reinterpret_cast<uintptr_t>(work.data_ptr()) % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(segs[4].data_ptr()) % 16 == 0,
+              "work too small, or work or pieces not 16-byte aligned");
   SharedAttnArgs a{};
   a.rows = (int)rows;
   a.num_q_heads = (int)num_q_heads;
@@ -948,29 +950,30 @@ SharedAttnArgs shared_plan_args(int64_t rows, int64_t num_q_heads, int64_t num_k
   a.row_slot = ptr<const int>(row_slot);
   a.seq_lens = ptr<const int>(seq_lens);
   a.num_segs = (int)num_segs;
-  a.entries = (int)segs[1].numel();
+  a.entries = (int)entries;
   a.levels = (int)levels;
-  a.seg_start = ptr<const int>(segs[0]);
-  a.seg_rows = ptr<const int>(segs[1]);
-  a.seg_page0 = ptr<const int>(segs[2]);
-  a.seg_page1 = ptr<const int>(segs[3]);
-  a.entry_seg = ptr<const int>(segs[4]);
-  a.row_entry = ptr<const int>(segs[5]);
+  a.num_pieces = (int)pieces;
+  a.seg_rows = ptr<const int>(segs[0]);
+  a.entry_seg = ptr<const int>(segs[1]);
+  a.entry_piece = ptr<const int>(segs[2]);
+  a.row_entry = ptr<const int>(segs[3]);
+  a.pieces = ptr<const int>(segs[4]);
   a.work = ptr<int>(work);
   a.err = ptr<int>(err);
   return a;
 }
 
 void shared_attn_plan(int64_t num_q_heads, int64_t num_kv_heads, const Tensor& row_slot, const Tensor& seq_lens,
-                      int64_t levels, const std::vector<Tensor>& segs, const Tensor& work, const Tensor& err) {
-  SharedAttnArgs a = shared_plan_args(row_slot.numel(), num_q_heads, num_kv_heads, 1, row_slot, seq_lens, levels, segs,
-                                      work, err);
+                      int64_t levels, int64_t num_segs, const std::vector<Tensor>& segs, const Tensor& work,
+                      const Tensor& err) {
+  SharedAttnArgs a = shared_plan_args(row_slot.numel(), num_q_heads, num_kv_heads, 1, row_slot, seq_lens, levels, num_segs,
+                                      segs, work, err);
   rc(zs_shared_attn_plan(&a, stream()), "zs_shared_attn_plan");
 }
 
 void shared_attn(const Tensor& q, const OptT& gate, int64_t num_kv_heads, const Tensor& k_cache, const Tensor& v_cache,
                  const Tensor& page_table, const Tensor& row_slot, const Tensor& seq_lens, int64_t levels,
-                 const std::vector<Tensor>& segs, const Tensor& work, const Tensor& partial, double sm_scale,
+                 int64_t num_segs, const std::vector<Tensor>& segs, const Tensor& work, const Tensor& partial, double sm_scale,
                  const OptT& out_bf16, const OptT& out_q, const OptT& out_sf, const Tensor& err) {
   check_cuda(q, "q");
   TORCH_CHECK(q.dim() == 3 && q.scalar_type() == at::kBFloat16 && q.size(2) == 256, "q must be bf16 [rows, heads, 256]");
@@ -990,10 +993,11 @@ void shared_attn(const Tensor& q, const OptT& gate, int64_t num_kv_heads, const 
   TORCH_CHECK(!gate.has_value() || reinterpret_cast<uintptr_t>(gate->data_ptr()) % 8 == 0, "gate must be 8-byte aligned");
   check_cuda(page_table, "page_table");
   TORCH_CHECK(page_table.dim() == 2 && page_table.scalar_type() == at::kInt, "page_table must be int32 [slots, max_pages]");
-  SharedAttnArgs a = shared_plan_args(rows, hq, num_kv_heads, page_table.size(1), row_slot, seq_lens, levels, segs, work, err);
+  SharedAttnArgs a = shared_plan_args(rows, hq, num_kv_heads, page_table.size(1), row_slot, seq_lens, levels, num_segs,
+                                      segs, work, err);
   check_cuda(partial, "partial");
   TORCH_CHECK(partial.scalar_type() == at::kFloat &&
-                  partial.numel() >= (segs[1].numel() * hq + ZS_SHARED_CTAS * ZS_SHARED_SLOTS) * 260,
+                  partial.numel() >= (segs[0].numel() * hq + ZS_SHARED_CTAS * ZS_SHARED_SLOTS) * 260,
               "partial too small");
   a.q = ptr(q);
   a.gate = optptr(gate);
@@ -1162,14 +1166,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("uniform"), py::arg("record"), py::arg("err"));
   m.attr("SHARED_MAX_GROUP") = ZS_SHARED_MAX_GROUP;
   m.attr("SHARED_MAX_SEGS") = ZS_SHARED_MAX_SEGS;
-  m.def("shared_attn_sizes", [](int64_t segs, int64_t entries, int64_t heads) {
-    return std::make_pair((int64_t)ZS_SHARED_WORK_INTS(segs, entries), (entries * heads + ZS_SHARED_CTAS * ZS_SHARED_SLOTS) * 260);
+  m.attr("SHARED_MAX_PIECES") = ZS_SHARED_MAX_PIECES;
+  m.attr("SHARED_SLOTS") = ZS_SHARED_SLOTS;
+  m.def("shared_attn_sizes", [](int64_t pieces, int64_t entries, int64_t heads) {
+    return std::make_pair((int64_t)ZS_SHARED_WORK_INTS(pieces, entries), (entries * heads + ZS_SHARED_CTAS * ZS_SHARED_SLOTS) * 260);
   });
   m.def("shared_attn_plan", &shared_attn_plan, py::arg("num_q_heads"), py::arg("num_kv_heads"), py::arg("row_slot"),
-        py::arg("seq_lens"), py::arg("levels"), py::arg("segs"), py::arg("work"), py::arg("err"));
+        py::arg("seq_lens"), py::arg("levels"), py::arg("num_segs"), py::arg("segs"), py::arg("work"), py::arg("err"));
   m.def("shared_attn", &shared_attn, py::arg("q"), py::arg("gate"), py::arg("num_kv_heads"), py::arg("k_cache"),
         py::arg("v_cache"), py::arg("page_table"), py::arg("row_slot"), py::arg("seq_lens"), py::arg("levels"),
-        py::arg("segs"), py::arg("work"), py::arg("partial"), py::arg("sm_scale"), py::arg("out_bf16"), py::arg("out_q"),
+        py::arg("num_segs"), py::arg("segs"), py::arg("work"), py::arg("partial"), py::arg("sm_scale"), py::arg("out_bf16"), py::arg("out_q"),
         py::arg("out_sf"), py::arg("err"));
   m.def("pool_call", &pool_call, py::arg("which"), py::arg("refcount"), py::arg("free_bits"), py::arg("seq_len"),
         py::arg("page_table"), py::arg("page_size"), py::arg("caches"), py::arg("slots") = py::none(),

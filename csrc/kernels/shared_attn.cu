@@ -8,12 +8,13 @@
 //   out = sigmoid(gate) * (sum_j exp(m_j - M) o_j) / (sum_j exp(m_j - M) l_j),  M = max m_j.
 // A row that sees no key gives 0.  Cache blocks are those of attention.cu.
 //
-// Work: a unit is (segment, kv head, up to 128 / G rows: 128 query slots = row x head of the
-// GQA group), its keys go through 64-key tiles.  The tiles of all units, one after the other,
-// are divided evenly over the CTAs (one per SM), so a CTA works on the end of one unit, some
-// whole ones and the start of another; each such fragment leaves one record per slot, and a
-// last kernel merges a row's records.  A prefix's pages are read once for 128 query slots
-// instead of once per row; tails and prefixes run in one launch without a tail of idle SMs.
+// Work: a unit is up to 128 / G rows (128 query slots = row x head of the GQA group) and a kv
+// head.  It goes through its pieces, the segments of those rows one after the other, in 64-key
+// tiles: a common prompt fills a unit or several, the own tokens of many sequences are pieces of
+// one.  The tiles of all units, one after the other, are divided evenly over the CTAs (one per
+// SM); a CTA's part of a unit leaves one record per slot that had tiles there, and a last kernel
+// merges a row's records.  A prefix's pages are read once for 128 query slots instead of once per
+// row, and tails and prefixes run in one launch without a tail of idle SMs.
 #include "sm100_common.cuh"
 #include "zs_kernels.h"
 
@@ -31,30 +32,29 @@ constexpr int STAGE = TPAGES * BLOCK;    // one tile of K or V: 32 KiB
 constexpr int STAGES = 4;
 constexpr int COMPUTE = 256;             // softmax threads (warps 0-7), then a copy, an MMA and a lookup warp
 constexpr int THREADS = COMPUTE + 96;
-constexpr int AHEAD = 3;                 // fragments known at a time
+constexpr int AHEAD = 3;                 // pieces known at a time
 constexpr int CTAS = ZS_SHARED_CTAS;
 constexpr int MAX_SEGS = ZS_SHARED_MAX_SEGS;
+constexpr int MAX_PIECES = ZS_SHARED_MAX_PIECES;
 
-// A unit costs its tiles and a few tiles more: a pipeline that starts anew, its Q and its record.
-ZS_DEVICE int unit_cost(int rows, int rpu, int group) { return 2 + min(rows, rpu) * group / 64; }
-
-// The plan (ints): the cost of everything, a Segment for each segment and one behind the last
-// (its cost0 alone), per entry (kv head 0) its unit's first tile (as a cost), its tiles, the distance to the
-// next kv head's unit and its first slot, and the range of costs and first segment of every CTA.
-struct Segment {
-  int cost0, nt, e0, rows;   // cost before it, tiles of a unit, first entry, rows
-  int p0, pend, len, slot;   // pages [p0, pend), its longest row's length (at most their end) and table row
+// The plan (ints): header (cost of everything, cost of one kv head), a Piece for each piece and one
+// behind the last (its cost0 alone), per entry (kv head 0) the place of its first tile among the
+// costs, its tiles and its first slot, and the range of costs and first piece of every CTA.
+struct Piece {
+  int cost0, nt, over, e0;    // cost before it, tiles, cost of the unit that it starts (or 0), the unit's first entry
+  int rows, r0, r1, p0;       // rows of the unit, the piece's rows in it, first page
+  int pend, len, table, pad;  // last page + 1, its longest row's length (at most that end) and page-table row
 };
 struct Work {
-  int* total;
-  Segment* seg;
+  int* head;
+  Piece* piece;
   int4 *entry, *cta;
 };
 __host__ __device__ inline Work work_of(const SharedAttnArgs& a) {
   Work w;
-  w.total = a.work;
-  w.seg = reinterpret_cast<Segment*>(a.work + 4);
-  w.entry = reinterpret_cast<int4*>(w.seg + a.num_segs + 1);
+  w.head = a.work;
+  w.piece = reinterpret_cast<Piece*>(a.work + 4);
+  w.entry = reinterpret_cast<int4*>(w.piece + a.num_pieces + 1);
   w.cta = w.entry + a.entries;
   return w;
 }
@@ -69,38 +69,56 @@ ZS_DEVICE int active_ctas(int total) { return min(CTAS, total); }
 // the CTAs' ranges laid over them.
 __global__ void __launch_bounds__(1024) plan_kernel(const SharedAttnArgs a) {
   pdl_trigger();
-  __shared__ unsigned long long longest[MAX_SEGS];  // (length, ~row)
-  __shared__ int cost0[MAX_SEGS + 1], tiles[MAX_SEGS];
+  __shared__ unsigned long long longest[MAX_SEGS];  // (length, ~entry)
+  __shared__ int table[MAX_SEGS];
+  __shared__ int cost0[MAX_PIECES + 1];
   __shared__ long long red[32];
   const Work w = work_of(a);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   for (int s = tid; s < a.num_segs; s += 1024) longest[s] = 0;
+  // The plan's own tensors do not change: what a thread needs of them first is read before the wait.
+  const bool e_in = tid < a.entries, p_in = tid < a.num_pieces;
+  const int row = e_in ? a.seg_rows[tid] : 0, seg = e_in ? a.entry_seg[tid] : 0, slot = e_in ? a.row_slot[row] : 0;
+  const int at_piece = e_in ? a.entry_piece[tid] : 0;
+  const int4 px = p_in ? reinterpret_cast<const int4*>(a.pieces)[2 * tid] : make_int4(0, 0, 0, 0);
+  const int4 py = p_in ? reinterpret_cast<const int4*>(a.pieces)[2 * tid + 1] : make_int4(0, 0, 0, 0);
   __syncthreads();
-  const int row0 = tid < a.entries ? a.seg_rows[tid] : 0, seg0 = tid < a.entries ? a.entry_seg[tid] : 0;  // the plan's own
   pdl_wait();
-  for (int e = tid; e < a.entries; e += 1024) {
-    const int row = e == tid ? row0 : a.seg_rows[e], s = e == tid ? seg0 : a.entry_seg[e];
-    const int len = max(a.seq_lens[row], 0);
-    atomicMax(&longest[s], ((unsigned long long)len << 32) | (uint32_t)~row);
+  auto key = [&](int e, int r) { return ((unsigned long long)max(a.seq_lens[r], 0) << 32) | (uint32_t)~e; };
+  const unsigned long long mine = e_in ? key(tid, row) : 0;
+  if (e_in) atomicMax(&longest[seg], mine);
+  for (int e = tid + 1024; e < a.entries; e += 1024) atomicMax(&longest[a.entry_seg[e]], key(e, a.seg_rows[e]));
+  __syncthreads();
+  if (e_in && longest[seg] == mine) table[seg] = slot;
+  for (int e = tid + 1024; e < a.entries; e += 1024) {
+    const int s = a.entry_seg[e];
+    if ((uint32_t)longest[s] == (uint32_t)~e) table[s] = a.row_slot[a.seg_rows[e]];
   }
   __syncthreads();
-  const int group = group_of(a), rpu = SLOTS / group;
+  const int group = group_of(a);
   long long carry = 0;
-  for (int s0 = 0; s0 < a.num_segs; s0 += 1024) {
-    const int s = s0 + tid;
+  for (int i0 = 0; i0 < a.num_pieces; i0 += 1024) {
+    const int i = i0 + tid;
     long long cost = 0;
-    Segment g = {};
-    if (s < a.num_segs) {
-      const int len = (int)(longest[s] >> 32), row = (int)~(uint32_t)longest[s], p1 = a.seg_page1[s];
-      g.e0 = a.seg_start[s];
-      g.rows = a.seg_start[s + 1] - g.e0;
-      g.p0 = a.seg_page0[s];
-      g.slot = a.row_slot[row];
+    Piece g = {};
+    if (i < a.num_pieces) {
+      // (segment, unit's first entry, unit's rows, starts a unit), (rows r0..r1 of it, pages p0..p1)
+      const int4 x = i0 == 0 ? px : reinterpret_cast<const int4*>(a.pieces)[2 * i];
+      const int4 y = i0 == 0 ? py : reinterpret_cast<const int4*>(a.pieces)[2 * i + 1];
+      const int len = (int)(longest[x.x] >> 32);
+      g.e0 = x.y;
+      g.rows = x.z;
+      // A unit costs a few tiles besides its own: a pipeline that starts anew, its Q, its records.
+      g.over = x.w != 0 ? 2 + x.z * group / 64 : 0;
+      g.r0 = y.x;
+      g.r1 = y.y;
+      g.p0 = y.z;
       g.pend = (int)(((long long)len + PAGE - 1) / PAGE);
-      if (p1 >= 0) g.pend = min(g.pend, p1);
+      if (y.w >= 0) g.pend = min(g.pend, y.w);
       g.nt = (max(g.pend - g.p0, 0) + TPAGES - 1) / TPAGES;
       g.len = (int)min((long long)len, (long long)g.pend * PAGE);
-      if (g.nt > 0) cost = (long long)(g.nt + unit_cost(g.rows, rpu, group)) * ((g.rows + rpu - 1) / rpu) * a.num_kv_heads;
+      g.table = table[x.x];
+      cost = g.nt + g.over;
     }
     long long x = cost;
 #pragma unroll
@@ -108,76 +126,82 @@ __global__ void __launch_bounds__(1024) plan_kernel(const SharedAttnArgs a) {
       const long long y = __shfl_up_sync(0xffffffff, x, o);
       if (lane >= o) x += y;
     }
-    __syncthreads();
     if (lane == 31) red[warp] = x;
     __syncthreads();
-    long long before = warp > 0 && lane < warp ? red[lane] : 0, sum = red[lane];
+    long long before = lane < warp ? red[lane] : 0, sum = red[lane];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       before += __shfl_xor_sync(0xffffffff, before, o);
       sum += __shfl_xor_sync(0xffffffff, sum, o);
     }
-    if (s < a.num_segs) {
+    if (i < a.num_pieces) {
       g.cost0 = (int)(carry + before + x - cost);
-      cost0[s] = g.cost0;
-      tiles[s] = g.nt;
-      w.seg[s] = g;
+      cost0[i] = g.cost0;
+      w.piece[i] = g;
     }
     carry += sum;
+    __syncthreads();
   }
-  const bool fits = carry < (1ll << 30);  // lengths beyond any cache: nothing is read
-  const int total = fits ? (int)carry : 0, n = active_ctas(total);
+  const bool fits = carry * a.num_kv_heads < (1ll << 30);  // lengths beyond any cache: nothing is read
+  const int each = fits ? (int)carry : 0, total = each * a.num_kv_heads, n = active_ctas(total);
   if (tid == 0) {
     if (!fits) report_error(a.err, kErrBadShape);
-    cost0[a.num_segs] = w.seg[a.num_segs].cost0 = total;
-    *w.total = total;
+    cost0[a.num_pieces] = w.piece[a.num_pieces].cost0 = each;
+    w.head[0] = total;
+    w.head[1] = each;
   }
   __syncthreads();
-  for (int e = tid; e < a.entries; e += 1024) {
-    const int s = e == tid ? seg0 : a.entry_seg[e], e0 = a.seg_start[s];
-    const int rows = a.seg_start[s + 1] - e0, more = unit_cost(rows, rpu, group);
-    const int at = e - e0, nq = (rows + rpu - 1) / rpu, each = tiles[s] + more;
-    w.entry[e] = make_int4(cost0[s] + at / rpu * each + more, fits ? tiles[s] : 0, nq * each, at % rpu * group);
-  }
   for (int c = tid; c < CTAS; c += 1024) {
-    const int t = c < n ? first_cost(total, n, c) : 0;
-    int lo = 0, hi = a.num_segs;  // the last segment with cost0 <= t (empty ones before it share its cost0)
+    const int t = c < n ? first_cost(total, n, c) : 0, rel = each > 0 ? t % each : 0;
+    int lo = 0, hi = a.num_pieces;  // the last piece with cost0 <= rel (empty ones before it share its cost0)
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (cost0[mid] <= t) lo = mid; else hi = mid;
+      if (cost0[mid] <= rel) lo = mid; else hi = mid;
     }
     w.cta[c] = make_int4(t, c < n ? first_cost(total, n, c + 1) : 0, lo, 0);
   }
+  for (int e = tid; e < a.entries; e += 1024) {
+    const int i = e == tid ? at_piece : a.entry_piece[e];
+    const int4 x = reinterpret_cast<const int4*>(a.pieces)[2 * i];
+    const int over = x.w != 0 ? 2 + x.z * group / 64 : 0;
+    w.entry[e] = make_int4(cost0[i] + over, fits ? cost0[i + 1] - cost0[i] - over : 0, (e - x.y) * group, 0);
+  }
 }
 
-// A CTA's part of one unit: tiles [t0, t1).
+// A CTA's part of a piece: tiles [t0, t1) for the slots [s0, s1) of its unit.
 struct Fragment {
-  int kvh, e0, slots, t0, t1, p0, pend, len, table;
+  int kvh, e0, slots, s0, s1, t0, t1, p0, pend, len, table;
+  int first;  // of the unit in this CTA: a new Q
 };
 
 struct Walk {
-  int pos, end, seg, rpu, group;
+  int pos, end, i, each, group;
+  int kvh, e0;
   ZS_DEVICE bool next(const SharedAttnArgs& a, const Work& w, Fragment& f) {
     while (pos < end) {
-      const int4* at4 = reinterpret_cast<const int4*>(w.seg + seg);
-      const int4 x = __ldg(at4), y = __ldg(at4 + 1);
-      if (pos >= __ldg(&w.seg[seg + 1].cost0)) {
-        ++seg;
+      const int4* at4 = reinterpret_cast<const int4*>(w.piece + i);
+      const int4 x = __ldg(at4), y = __ldg(at4 + 1), z = __ldg(at4 + 2);
+      const int head = pos / each, at = pos - head * each - x.x;
+      if (at >= __ldg(&w.piece[i + 1].cost0) - x.x) {  // behind this piece: the next one
+        ++i;
         continue;
       }
-      const int nt = x.y, cost = unit_cost(x.w, rpu, group), each = nt + cost, u = (pos - x.x) / each, at = pos - x.x - u * each;
-      f.t0 = max(0, at - cost);
-      f.t1 = min(nt, at - cost + end - pos);
-      pos += min(each - at, end - pos);
+      const int cost = x.y + x.z;
+      f.t0 = max(0, at - x.z);
+      f.t1 = min(x.y, at - x.z + end - pos);
+      pos += min(cost - at, end - pos);
+      if (pos == (head + 1) * each) i = 0;  // the next kv head
       if (f.t1 <= f.t0) continue;
-      const int nq = (x.w + rpu - 1) / rpu, qt = u % nq;  // the units of one kv head follow one another: they read the same pages
-      f.kvh = u / nq;
-      f.e0 = x.z + qt * rpu;
-      f.slots = min(rpu, x.w - qt * rpu) * group;
-      f.p0 = y.x;
-      f.pend = y.y;
-      f.len = y.z;
-      f.table = y.w;
+      f.first = head != kvh || x.w != e0;
+      f.kvh = kvh = head;
+      f.e0 = e0 = x.w;
+      f.slots = y.x * group;
+      f.s0 = y.y * group;
+      f.s1 = y.z * group;
+      f.p0 = y.w;
+      f.pend = z.x;
+      f.len = z.y;
+      f.table = z.z;
       return true;
     }
     return false;
@@ -203,8 +227,8 @@ struct Smem {
   int vote[2][8];
   int again[2];                     // the P of this tile is followed by its rounding errors
   Fragment frag[AHEAD];             // t1 == 0: no more
-  int row[AHEAD][SLOTS], limit[AHEAD][SLOTS];  // row of each slot (-1: unused) and the keys it sees
-  int least[AHEAD];                 // the fewest of them
+  int limit[AHEAD][SLOTS];          // keys that each slot sees (0: unused)
+  int least[AHEAD];                 // the fewest among the piece's slots
   volatile int abort;
   uint32_t tmem;
   uint64_t full[STAGES], empty[STAGES], s_full[2], p_full[2], o_full[2], q_full, f_full[AHEAD], f_empty[AHEAD], r_full[AHEAD], way_full, way_empty;
@@ -259,14 +283,24 @@ ZS_DEVICE float pick(bool c, float x, float y) {
 // (start address, leading offset): the high word (stride, version, 128-byte swizzle) is a constant.
 constexpr uint32_t desc_hi(uint32_t stride) { return (stride >> 4) | (1u << 14) | (2u << 29); }
 ZS_DEVICE uint32_t desc_lo(const void* p, uint32_t lead) { return (smem_u32(p) >> 4) | ((lead >> 4) << 16); }
-template <uint32_t HI_B>
+constexpr uint32_t kHiB = desc_hi(4096);  // 8-key groups of a tile are 4 KiB apart
 ZS_DEVICE void mma_step(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, bool add) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "mov.b64 b, {%2, %5};\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
-      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"((int)add), "n"(HI_B)
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"((int)add), "n"(kHiB)
+      : "memory");
+}
+// The same for some rows of D: lanes whose bit in `off` is set keep what they hold.
+ZS_DEVICE void mma_step_rows(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, const uint32_t (&off)[4], bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, {%6, %7, %8, %9}, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"((int)add), "n"(kHiB), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
       : "memory");
 }
 
@@ -414,7 +448,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
       if (leader) {
 #pragma unroll
         for (int x = 0; x < D / 16; ++x)  // 16 dims each: 4 in a 64-dim chunk, 8 columns of Q
-          mma_step<desc_hi(4096)>(d, tmem + kTmemQ + x * 8, k_at + (x >> 2) * (1024 / 16) + (x & 3) * 2, idesc_s, x > 0);
+          mma_step(d, tmem + kTmemQ + x * 8, k_at + (x >> 2) * (1024 / 16) + (x & 3) * 2, idesc_s, x > 0);
         tc_commit(&s.empty[st]);
         tc_commit(&s.s_full[i & 1]);
       }
@@ -422,7 +456,8 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
       ++ns;
       return true;
     };
-    // O of tile i.
+    // O of tile i, for the rows of its piece alone: the others' stay as they are, whatever the tile holds.
+    uint32_t off[4];
     auto output = [&](int i, bool fresh) {
       const int st = vr.st, b = i & 1;
       if (!wait_for(s, &s.full[st], vr.ph, a.err)) return false;
@@ -433,11 +468,11 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
       if (leader) {
 #pragma unroll
         for (int k = 0; k < TPAGES; ++k)  // a page each: 16 keys
-          mma_step<desc_hi(4096)>(tmem + kTmemO, p_at + k * 8, v_at + k * (BLOCK / 16), idesc_o, !fresh || k > 0);
+          mma_step_rows(tmem + kTmemO, p_at + k * 8, v_at + k * (BLOCK / 16), idesc_o, off, !fresh || k > 0);
         if (again) {
 #pragma unroll
           for (int k = 0; k < TPAGES; ++k)
-            mma_step<desc_hi(4096)>(tmem + kTmemO, p_at + 32 + k * 8, v_at + k * (BLOCK / 16), idesc_o, true);
+            mma_step_rows(tmem + kTmemO, p_at + 32 + k * 8, v_at + k * (BLOCK / 16), idesc_o, off, true);
         }
         tc_commit(&s.empty[st]);
         tc_commit(&s.o_full[b]);
@@ -446,20 +481,24 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
       ++no;
       return true;
     };
-    int i = 0;
+    int i = 0, nq = 1;
     bool more = __all_sync(0xffffffff, next_fragment(f));
     bool ok = more && __all_sync(0xffffffff, wait_for(s, &s.q_full, 0, a.err) && scores(0));
-    for (int nf = 1; ok && more; ++nf) {
+    while (ok && more) {
       const int t0 = f.t0, t1 = f.t1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int lo = min(max(f.s0 - 32 * j, 0), 32), hi = min(max(f.s1 - 32 * j, 0), 32);
+        off[j] = ~((uint32_t)((1ull << hi) - 1) & ~(uint32_t)((1ull << lo) - 1));
+      }
       for (int t = t0; ok && t < t1; ++t, ++i) {
-        // S of the next tile, which may be the next fragment's first, goes before O of this one.
-        if (t + 1 < t1) {
-          ok = scores(i + 1);
-        } else {
-          more = __all_sync(0xffffffff, next_fragment(f));
-          if (more) ok = wait_for(s, &s.q_full, nf & 1, a.err) && scores(i + 1);
+        // S of the next tile, which may be the next unit's first, goes before O of this one.
+        bool next = t + 1 < t1;
+        if (!next) {
+          next = more = __all_sync(0xffffffff, next_fragment(f));
+          if (more && f.first) ok = wait_for(s, &s.q_full, nq++ & 1, a.err);
         }
-        ok = ok && output(i, t == t0);
+        ok = ok && (!next || scores(i + 1)) && output(i, t == t0);
         ok = __all_sync(0xffffffff, ok);
       }
     }
@@ -473,10 +512,11 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
     // and its Q into the way as soon as that is free.
     const Work w = work_of(a);
     const int4 mine = __ldg(w.cta + cta);
-    Walk walk{mine.x, mine.y, mine.z, SLOTS / group, group};
+    Walk walk{mine.x, mine.y, mine.z, max(1, __ldg(w.head + 1)), group, -1, -1};
     const char* qbase = static_cast<const char*>(a.q);
     bool ok = true, more = true;
-    for (int k = 0, at = 0, ph = 0; ok && more; ++k) {
+    int row[4], len[4], units = 0;
+    for (int at = 0, ph = 0; ok && more;) {
       more = walk.next(a, w, f);
       if (!more) f.t1 = 0;
       ok = __all_sync(0xffffffff, wait_for(s, &s.f_empty[at], ph ^ 1, a.err));  // passes at once in the first round
@@ -484,26 +524,31 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
         s.frag[at] = f;
         mbar_arrive(&s.f_full[at]);
       }
-      if (!more) break;
-      int row[4], least = 0x7FFFFFFF;
+      if (!more || !ok) break;
+      if (f.first) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) row[j] = j * 32 + lane < f.slots ? a.seg_rows[f.e0 + (j * 32 + lane) / group] : -1;
-      ok = ok && (k == 0 || wait_for(s, &s.way_empty, (k - 1) & 1, a.err));
-      ok = __all_sync(0xffffffff, ok);
-      if (!ok) break;
-      if (lane == 0) mbar_expect_tx(&s.way_full, f.slots * D * 2);
-      __syncwarp();
+        for (int j = 0; j < 4; ++j) row[j] = j * 32 + lane < f.slots ? a.seg_rows[f.e0 + (j * 32 + lane) / group] : -1;
+        ok = units == 0 || wait_for(s, &s.way_empty, (units - 1) & 1, a.err);
+        ok = __all_sync(0xffffffff, ok);
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(&s.way_full, f.slots * D * 2);
+        __syncwarp();
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (row[j] >= 0)
-          bulk_load(s.way[j * 32 + lane], qbase + ((size_t)row[j] * a.num_q_heads + f.kvh * group + (j * 32 + lane) % group) * (D * 2),
-                    D * 2, &s.way_full);
+        for (int j = 0; j < 4; ++j)
+          if (row[j] >= 0)
+            bulk_load(s.way[j * 32 + lane], qbase + ((size_t)row[j] * a.num_q_heads + f.kvh * group + (j * 32 + lane) % group) * (D * 2),
+                      D * 2, &s.way_full);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) len[j] = row[j] >= 0 ? max(a.seq_lens[row[j]], 0) : 0;
+        ++units;
+      }
+      int least = 0x7FFFFFFF;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int limit = row[j] >= 0 ? min(a.seq_lens[row[j]], f.len) : 0x7FFFFFFF;
-        s.row[at][j * 32 + lane] = row[j];
-        s.limit[at][j * 32 + lane] = limit;
-        least = min(least, limit);
+        const int sl = j * 32 + lane;
+        const bool in = sl >= f.s0 && sl < f.s1;
+        s.limit[at][sl] = in ? min(len[j], f.len) : 0;
+        if (in) least = min(least, min(len[j], f.len));
       }
       least = __reduce_min_sync(0xffffffff, least);
       if (lane == 0) s.least[at] = least;
@@ -512,9 +557,8 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
         at = 0;
         ph ^= 1;
       }
-      ++fk;  // fragments whose Q was asked for
     }
-    if (lane == 0 && fk > 0) mbar_wait(&s.way_full, (fk - 1) & 1, nullptr);  // no copy outlives the CTA
+    if (lane == 0 && units > 0) mbar_wait(&s.way_full, (units - 1) & 1, nullptr);  // no copy outlives the CTA
   } else {
     // ---------------------------------------------------------------- softmax
     const int half = warp >> 2, slot = (warp & 3) * 32 + lane;
@@ -540,29 +584,37 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
     // After a wait that gave up these warps go on to the end of the fragment with whatever is there (the
     // error word is set, every later wait gives up at once) and leave together: their barriers always meet.
     bool more = !compute_any(!next_fragment(f));
-    int kf = 0;  // place of the fragment
+    int kf = 0;  // place of the piece
     uint32_t kph = 0;
     if (more) {
       store_q(f.slots, 0);
       fence_proxy_async_shared();
       mbar_arrive(&s.way_empty);
     }
-    int i = 0;
+    int i = 0, units = 1;
     Ring vr;
     vr.next();
-    for (int nf = 0; more; ++nf) {
+    float m = -INFINITY, l = 0.f;  // reference maximum (raw scores) of the slot, sum of this half's weights
+    int rec = -1;                  // record of the slot, once it had a tile
+    while (more) {
       wait_for(s, &s.r_full[kf], kph, a.err);
-      const int row = s.row[kf][slot], limit = s.limit[kf][slot], least = s.least[kf];
-      const bool used = row >= 0, busy = (warp & 3) * 32 < f.slots;
-      Fragment g;
-      float m = -INFINITY, l = 0.f;  // reference maximum (raw scores) of the slot, sum of this half's weights
+      const int limit = s.limit[kf][slot], least = s.least[kf];
+      const bool used = slot >= f.s0 && slot < f.s1, busy = (warp & 3) * 32 < f.s1 && (warp & 3) * 32 + 32 > f.s0;
+      if (used) {
+        // The CTA with a piece's first tile keeps the record by (entry, head), the others by CTA and slot.
+        rec = f.t0 == 0 ? (f.e0 + slot / group) * a.num_q_heads + f.kvh * group + head
+                        : a.entries * a.num_q_heads + cta * SLOTS + slot;
+        m = -INFINITY;
+        l = 0.f;
+      }
+      Fragment g = {};
       for (int t = f.t0; t < f.t1; ++t, ++i, vr.next(2)) {
         const int b = i & 1, key0 = (f.p0 + t * TPAGES) * PAGE;
         wait_for(s, &s.s_full[b], (i >> 1) & 1, a.err);
         tc_fence_after();
-        if (t + 1 == f.t1) {  // every product with this Q is done: the next fragment's takes its place
+        if (t + 1 == f.t1) {
           more = !compute_any(!next_fragment(g));
-          if (more) store_q(g.slots, nf + 1);
+          if (more && g.first) store_q(g.slots, units++);  // every product with this Q is done: the next takes its place
         }
         uint32_t r[32];
         float mt = -INFINITY;
@@ -705,45 +757,58 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
           tc_fence_before();
         }
       }
-      // ---- the fragment's records: those of the unit's first fragment lie by (entry, head), those of
-      // a later one by CTA and slot.  They pass through shared memory so that the stores are whole lines.
-      wait_for(s, &s.o_full[(i - 1) & 1], ((i - 1) >> 1) & 1, a.err);
-      tc_fence_after();
-      if (busy) {
-        const size_t at = f.t0 == 0 ? (size_t)(f.e0 + slot / group) * a.num_q_heads + f.kvh * group + head
-                                    : (size_t)a.entries * a.num_q_heads + (size_t)cta * SLOTS + slot;
-        const int rows = min(32, f.slots - (warp & 3) * 32);
+      if (!more || g.first) {
+        // ---- the unit's records.  A warp with more than a few passes them through shared memory so that
+        // the stores are whole lines (128 slots: 4.4 us directly, 3.2 us so; 8 slots: 0.7 and 1.3 us).
+        wait_for(s, &s.o_full[(i - 1) & 1], ((i - 1) >> 1) & 1, a.err);
+        tc_fence_after();
+        const uint32_t has = __ballot_sync(0xffffffff, rec >= 0);
+        float* to = a.partial + (size_t)max(rec, 0) * PREC;
+        if (has != 0 && __popc(has) <= 8) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
+          for (int c = 0; c < 128; c += 32) {
             uint32_t o[32];
-            tmem_ld_32x32b_x32(lanes + kTmemO + half * 128 + c * 64 + q * 32, o);
+            tmem_ld_32x32b_x32(lanes + kTmemO + half * 128 + c, o);
             tmem_ld_wait();
+            if (rec >= 0) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              *reinterpret_cast<uint4*>(way(slot, q * 8 + j)) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+              for (int j = 0; j < 32; j += 4)
+                *reinterpret_cast<uint4*>(to + half * 128 + c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+            }
           }
-          __syncwarp();
+        } else if (has != 0) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              uint32_t o[32];
+              tmem_ld_32x32b_x32(lanes + kTmemO + half * 128 + c * 64 + q * 32, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                *reinterpret_cast<uint4*>(way(slot, q * 8 + j)) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            }
+            __syncwarp();
 #pragma unroll 4
-          for (int j = 0; 2 * j < rows; ++j) {
-            const int x = 2 * j + (lane >> 4);
-            const size_t to = __shfl_sync(0xffffffff, at, x);
-            if (x < rows)
-              *reinterpret_cast<uint4*>(a.partial + to * PREC + half * 128 + c * 64 + (lane & 15) * 4) =
-                  *reinterpret_cast<const uint4*>(way((warp & 3) * 32 + x, lane & 15));
+            for (int j = 0; j < 16; ++j) {
+              const int x = 2 * j + (lane >> 4);
+              const int rx = __shfl_sync(0xffffffff, rec, x);
+              if (rx >= 0)
+                *reinterpret_cast<uint4*>(a.partial + (size_t)rx * PREC + half * 128 + c * 64 + (lane & 15) * 4) =
+                    *reinterpret_cast<const uint4*>(way((warp & 3) * 32 + x, lane & 15));
+            }
+            __syncwarp();
           }
-          __syncwarp();
+          fence_proxy_async_shared();
         }
-        if (used) {
-          float* end = a.partial + at * PREC + D;
-          if (half == 0) *reinterpret_cast<float2*>(end) = make_float2(m * qscale, l);
-          else end[2] = l;
+        if (rec >= 0) {
+          if (half == 0) *reinterpret_cast<float2*>(to + D) = make_float2(m * qscale, l);
+          else to[D + 2] = l;
         }
+        rec = -1;
+        tc_fence_before();
+        mbar_arrive(&s.way_empty);
       }
-      tc_fence_before();
-      fence_proxy_async_shared();
-      mbar_arrive(&s.way_empty);
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.f_empty[kf]);
       if (++kf == AHEAD) {
@@ -778,32 +843,55 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const SharedAtt
   const int item = blockIdx.x * (MERGE_WARPS / PARTS) + warp / PARTS;
   if (item >= a.rows * a.num_q_heads) return;  // PARTS == 1 alone
   const int row = item / a.num_q_heads, h = item % a.num_q_heads, group = group_of(a);
-  const int total = *w.total, n = active_ctas(total);
+  const int total = w.head[0], each = w.head[1], n = active_ctas(total);
   float m = -INFINITY, l = 0.f, o[8] = {};
-  for (int j = 0; j < a.levels; ++j) {
-    const int e = a.row_entry[row * a.levels + j];
-    if (e < 0) break;
-    const int4 u = w.entry[e];
-    if (u.y == 0) continue;
-    const int first = u.x + h / group * u.z;
-    const int c0 = cta_of(total, n, first), c1 = cta_of(total, n, first + u.y - 1);
-    for (int c = c0 + part; c <= c1; c += 32 * PARTS) {
-      const int mine = c + lane * PARTS;
-      const size_t at = mine == c0 ? (size_t)e * a.num_q_heads + h
-                                   : (size_t)a.entries * a.num_q_heads + (size_t)mine * SLOTS + u.w + h % group;
-      const float4 ml = mine <= c1 ? *reinterpret_cast<const float4*>(a.partial + at * PREC + D) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+  // A lane per segment of the row: where its records are.  first[j] = records before segment j.
+  const int own = a.row_entry[row * a.levels + min(lane, a.levels - 1)];
+  for (int j0 = 0; j0 < a.levels; j0 += 32) {
+    const int e = j0 == 0 ? (lane < a.levels ? own : -1) : (j0 + lane < a.levels ? a.row_entry[row * a.levels + j0 + lane] : -1);
+    int c0 = 0, cnt = 0, slot = 0;
+    if (e >= 0) {
+      const int4 u = w.entry[e];
+      const int first = u.x + h / group * each;
+      slot = u.z + h % group;
+      if (u.y > 0) {
+        c0 = cta_of(total, n, first);
+        cnt = cta_of(total, n, first + u.y - 1) - c0 + 1;
+      }
+    }
+    int before = cnt;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const int y = __shfl_up_sync(0xffffffff, before, x);
+      if (lane >= x) before += y;
+    }
+    const int records = __shfl_sync(0xffffffff, before, 31);
+    before -= cnt;
+    for (int r0 = part; r0 < records; r0 += 32 * PARTS) {
+      const int r = r0 + lane * PARTS;  // this lane's record
+      int j = 0;                        // its segment: the last with before <= r and records
+      for (int x = 1; x < 32; ++x) {
+        const int bx = __shfl_sync(0xffffffff, before, x), cx = __shfl_sync(0xffffffff, cnt, x);
+        if (cx > 0 && bx <= r) j = x;
+        if (j0 + x + 1 >= a.levels) break;
+      }
+      const int c = __shfl_sync(0xffffffff, c0, j) + r - __shfl_sync(0xffffffff, before, j);
+      const int sl = __shfl_sync(0xffffffff, slot, j), ej = __shfl_sync(0xffffffff, e, j);
+      const size_t at = r == __shfl_sync(0xffffffff, before, j) ? (size_t)ej * a.num_q_heads + h
+                                                               : (size_t)a.entries * a.num_q_heads + (size_t)c * SLOTS + sl;
+      const float4 ml = r < records ? *reinterpret_cast<const float4*>(a.partial + at * PREC + D) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
       const float mn = fmaxf(m, warp_max(ml.x)), s0 = m == -INFINITY ? 0.f : exp2f(m - mn);
       const float wt = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mn);
       l = l * s0 + warp_sum(ml.x == -INFINITY ? 0.f : wt * (ml.y + ml.z));
 #pragma unroll
       for (int k = 0; k < 8; ++k) o[k] *= s0;
       m = mn;
-      const int cnt = min(32, (c1 - c) / PARTS + 1);
+      const int cnt_here = min(32, (records - r0 + PARTS - 1) / PARTS);
 #pragma unroll 4
-      for (int x = 0; x < cnt; ++x) {
+      for (int x = 0; x < cnt_here; ++x) {
         const float wx = __shfl_sync(0xffffffff, wt, x);
-        const float4* rec = reinterpret_cast<const float4*>(a.partial + __shfl_sync(0xffffffff, at, x) * PREC);
-        const float4 p = rec[lane], q = rec[32 + lane];
+        const float4* from = reinterpret_cast<const float4*>(a.partial + __shfl_sync(0xffffffff, at, x) * PREC);
+        const float4 p = from[lane], q = from[32 + lane];
         if (wx == 0.f) continue;
         o[0] += wx * p.x;
         o[1] += wx * p.y;
@@ -877,6 +965,7 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const SharedAtt
 int check(const SharedAttnArgs& a) {
   if (a.num_kv_heads < 1 || a.num_q_heads % a.num_kv_heads != 0 || a.num_q_heads / a.num_kv_heads > ZS_SHARED_MAX_GROUP) return -1;
   if (a.head_dim != D || a.page_size != PAGE || a.levels < 1 || a.num_segs < 0 || a.num_segs > MAX_SEGS || a.rows < 0) return -1;
+  if (a.num_pieces < 0 || a.num_pieces > MAX_PIECES) return -1;
   if (a.work == nullptr || a.max_pages < 1 || a.max_pages > (1 << 26)) return -1;
   return 0;
 }

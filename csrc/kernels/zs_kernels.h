@@ -664,7 +664,8 @@ int zs_draft_verify(const DraftVerifyArgs* args, cudaStream_t stream);
 // Gated GQA attention of rows that share leading pages (shared_attn.cu)
 // ----------------------------------------------------------------------------------
 #define ZS_SHARED_MAX_GROUP 64    // q heads per kv head
-#define ZS_SHARED_MAX_SEGS 2048   // segments of a plan
+#define ZS_SHARED_MAX_SEGS 1024   // segments of a plan
+#define ZS_SHARED_MAX_PIECES 4096 // their pieces
 #define ZS_SHARED_SLOTS 128       // query slots (row x head of a GQA group) of a work unit
 #define ZS_SHARED_CTAS 148
 
@@ -679,16 +680,18 @@ typedef struct SharedAttnArgs {
   int max_pages;
   const int* row_slot;       // [rows]
   const int* seq_lens;       // [rows] keys visible to each row (0: none)
-  // Segments: rows and the page positions [page0, page1) that they share (-1: to the end of the
-  // longest row).  A row is in at most `levels` segments, of disjoint ranges.
-  int num_segs, entries, levels;
-  const int* seg_start;      // [num_segs + 1] entry ranges
-  const int* seg_rows;       // [entries]
-  const int* seg_page0;      // [num_segs]
-  const int* seg_page1;
+  // Segments: rows and the page positions [page0, page1) that they share (page1 -1: to the end of
+  // the longest row).  A row is in at most `levels` segments, of disjoint ranges.  An entry is a row
+  // of a segment; units are up to ZS_SHARED_SLOTS / (q heads per kv head) entries in a row, and a
+  // piece is the part of a segment in a unit.
+  int num_segs, entries, levels, num_pieces;
+  const int* seg_rows;       // [entries] row of each entry, segment by segment
   const int* entry_seg;      // [entries]
-  const int* row_entry;      // [rows, levels] entry of each row's segments, -1: none
-  int* work;                 // [ZS_SHARED_WORK_INTS(num_segs, entries)], 16-byte aligned, written by the plan
+  const int* entry_piece;    // [entries]
+  const int* row_entry;      // [rows, levels] entry of each row's segments, -1: none (at the end)
+  const int* pieces;         // [num_pieces, 8]: segment, first entry and rows of its unit, whether it is the
+                             // unit's first piece, its rows [r0, r1) in the unit, page0, page1; 16-byte aligned
+  int* work;                 // [ZS_SHARED_WORK_INTS(num_pieces, entries)], 16-byte aligned, written by the plan
   float* partial;            // scratch: 260 floats x (entries * num_q_heads + ZS_SHARED_CTAS * ZS_SHARED_SLOTS)
   float sm_scale;            // > 0
   void* out_bf16;            // optional [rows, num_q_heads * 256]
@@ -697,7 +700,7 @@ typedef struct SharedAttnArgs {
   int* err;
 } SharedAttnArgs;
 
-#define ZS_SHARED_WORK_INTS(num_segs, entries) (4 + 8 * ((num_segs) + 1) + 4 * (entries) + 4 * ZS_SHARED_CTAS)
+#define ZS_SHARED_WORK_INTS(num_pieces, entries) (4 + 12 * ((num_pieces) + 1) + 4 * (entries) + 4 * ZS_SHARED_CTAS)
 
 // Divide the step's keys over the GPU (from seq_lens, row_slot, the segments and the head counts;
 // q, caches and outputs are not read): once a step.  Then one zs_shared_attn per layer.

@@ -13,7 +13,9 @@ import torch
 from . import _ext
 
 MAX_GROUP = 64     # q heads per kv head
-MAX_SEGS = 2048    # segments of a plan
+MAX_SEGS = 1024    # segments of a plan
+MAX_PIECES = 4096  # their parts in work units
+SLOTS = 128        # query slots (row x head of a GQA group) of a work unit
 
 
 class SharedPrefixPlan:
@@ -33,7 +35,9 @@ class SharedPrefixPlan:
         order = sorted(range(len(segments)), key=lambda i: segments[i][1])  # a row's segments by position
         row_entry: list[list[int]] = [[] for _ in range(rows)]
         reach: list[int | None] = [0] * rows
-        starts, seg_rows, entry_seg = [0], [], []
+        seg_rows, entry_seg, entry_piece, pieces = [], [], [], []
+        room = SLOTS // (num_q_heads // num_kv_heads)   # rows of a work unit
+        unit = [0, 0]                                   # first entry and rows of the last one
         for s, i in enumerate(order):
             members, first, end = segments[i]
             if not members:
@@ -49,7 +53,20 @@ class SharedPrefixPlan:
                 row_entry[r].append(len(seg_rows))
                 seg_rows.append(r)
                 entry_seg.append(s)
-            starts.append(len(seg_rows))
+            # Units: a segment that does not fit behind the others of the last unit starts one.
+            done = len(seg_rows) - len(members)
+            while done < len(seg_rows):
+                left = len(seg_rows) - done
+                start = not pieces or unit[1] + min(left, room) > room
+                if start:
+                    unit = [done, 0]
+                take = min(left, room - unit[1])
+                pieces.append([s, unit, int(start), unit[1], unit[1] + take, first, -1 if end is None else end])
+                unit[1] += take
+                entry_piece += [len(pieces) - 1] * take
+                done += take
+        if len(pieces) > MAX_PIECES:
+            raise ValueError(f"at most {MAX_PIECES} pieces of segments, got {len(pieces)}")
         if any(x is not None for x in reach):
             raise ValueError("the last segment of every row must end at None")
         self.C = _ext.load()
@@ -59,11 +76,12 @@ class SharedPrefixPlan:
         self.levels = max((len(e) for e in row_entry), default=1)
         i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
         self.slots = i32(slots)
-        self._segs = [i32(starts), i32(seg_rows), i32([segments[i][1] for i in order]),
-                      i32([-1 if segments[i][2] is None else segments[i][2] for i in order]), i32(entry_seg),
-                      i32([x for e in row_entry for x in e + [-1] * (self.levels - len(e))])]
+        self._num_segs = len(order)
+        self._segs = [i32(seg_rows), i32(entry_seg), i32(entry_piece),
+                      i32([x for e in row_entry for x in e + [-1] * (self.levels - len(e))]),
+                      i32([x for s, u, start, r0, r1, p0, p1 in pieces for x in (s, u[0], u[1], start, r0, r1, p0, p1)])]
         self.err = torch.zeros(1, dtype=torch.int32, device=device)
-        ints, floats = self.C.shared_attn_sizes(len(order), len(seg_rows), num_q_heads)
+        ints, floats = self.C.shared_attn_sizes(len(pieces), len(seg_rows), num_q_heads)
         self._work = torch.zeros(ints, dtype=torch.int32, device=device)
         self._partial = torch.empty(floats, dtype=torch.float32, device=device)
         self._planned = False
@@ -91,7 +109,7 @@ class SharedPrefixPlan:
 
     def update(self, seq_lens: torch.Tensor) -> None:
         """Divide a step's keys over the GPU: ``seq_lens`` [rows] int32, the keys each row sees."""
-        self.C.shared_attn_plan(self.num_q_heads, self.num_kv_heads, self.slots, seq_lens, self.levels, self._segs,
+        self.C.shared_attn_plan(self.num_q_heads, self.num_kv_heads, self.slots, seq_lens, self.levels, self._num_segs, self._segs,
                                 self._work, self.err)
         self._planned = True
 
@@ -111,7 +129,7 @@ class SharedPrefixPlan:
         if out is None and out_q is None:
             out = torch.empty(self.rows, self.num_q_heads * 256, dtype=torch.bfloat16, device=q.device)
         self.C.shared_attn(q, gate, self.num_kv_heads, k_cache, v_cache, page_table, self.slots, seq_lens, self.levels,
-                           self._segs, self._work, self._partial, sm_scale, out, out_q, out_sf, self.err)
+                           self._num_segs, self._segs, self._work, self._partial, sm_scale, out, out_q, out_sf, self.err)
         return out
 
     def check(self) -> None:
