@@ -937,7 +937,7 @@ SharedAttnArgs shared_plan_args(int64_t rows, int64_t num_q_heads, int64_t num_k
   const int64_t entries = segs[0].numel(), pieces = segs[4].numel() / 8;
   TORCH_CHECK(segs[1].numel() == entries && segs[2].numel() == entries && segs[4].numel() % 8 == 0,
               "segment tensors do not fit together");
-  TORCH_CHECK(work.numel() >= ZS_SHARED_WORK_INTS(pieces, entries) && reinterpret_cast<uintptr_t>(work.data_ptr()) % 16 == 0 &&
+  TORCH_CHECK(work.numel() >= ZS_SHARED_WORK_INTS(pieces, entries * num_kv_heads) && reinterpret_cast<uintptr_t>(work.data_ptr()) % 16 == 0 &&
                   reinterpret_cast<uintptr_t>(segs[4].data_ptr()) % 16 == 0,
               "work too small, or work or pieces not 16-byte aligned");
   SharedAttnArgs a{};
@@ -1168,8 +1168,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.attr("SHARED_MAX_SEGS") = ZS_SHARED_MAX_SEGS;
   m.attr("SHARED_MAX_PIECES") = ZS_SHARED_MAX_PIECES;
   m.attr("SHARED_SLOTS") = ZS_SHARED_SLOTS;
-  m.def("shared_attn_sizes", [](int64_t pieces, int64_t entries, int64_t heads) {
-    return std::make_pair((int64_t)ZS_SHARED_WORK_INTS(pieces, entries), (entries * heads + ZS_SHARED_CTAS * ZS_SHARED_SLOTS) * 260);
+  m.def("shared_attn_sizes", [](int64_t pieces, int64_t entries, int64_t heads, int64_t kv_heads) {
+    return std::make_pair((int64_t)ZS_SHARED_WORK_INTS(pieces, entries * kv_heads), (entries * heads + ZS_SHARED_CTAS * ZS_SHARED_SLOTS) * 260);
   });
   m.def("shared_attn_plan", &shared_attn_plan, py::arg("num_q_heads"), py::arg("num_kv_heads"), py::arg("row_slot"),
         py::arg("seq_lens"), py::arg("levels"), py::arg("num_segs"), py::arg("segs"), py::arg("work"), py::arg("err"));

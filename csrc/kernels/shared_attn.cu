@@ -29,17 +29,17 @@ constexpr int SLOTS = ZS_SHARED_SLOTS;   // query slots of a unit
 constexpr int TILE = 64;                 // keys of a tile
 constexpr int TPAGES = TILE / PAGE;
 constexpr int STAGE = TPAGES * BLOCK;    // one tile of K or V: 32 KiB
-constexpr int STAGES = 4;
-constexpr int COMPUTE = 256;             // softmax threads (warps 0-7), then a copy, an MMA and a lookup warp
-constexpr int THREADS = COMPUTE + 96;
+constexpr int STAGES = 2;                // of K, and of V
+constexpr int COMPUTE = 256;             // softmax threads (warps 0-7), then K copy, MMA, lookup and V copy warps
+constexpr int THREADS = COMPUTE + 128;
 constexpr int AHEAD = 3;                 // pieces known at a time
 constexpr int CTAS = ZS_SHARED_CTAS;
 constexpr int MAX_SEGS = ZS_SHARED_MAX_SEGS;
 constexpr int MAX_PIECES = ZS_SHARED_MAX_PIECES;
 
-// The plan (ints): header (cost of everything, cost of one kv head), a Piece for each piece and one
-// behind the last (its cost0 alone), per entry (kv head 0) the place of its first tile among the
-// costs, its tiles and its first slot, and the range of costs and first piece of every CTA.
+// The plan (ints): header (cost of one kv head), a Piece for each piece and one behind the last (its
+// cost0 alone), per entry and kv head the first CTA and the number of CTAs that have tiles of it and
+// its first slot, and the range of costs and first piece of every CTA.
 struct Piece {
   int cost0, nt, over, e0;    // cost before it, tiles, cost of the unit that it starts (or 0), the unit's first entry
   int rows, r0, r1, p0;       // rows of the unit, the piece's rows in it, first page
@@ -55,15 +55,24 @@ __host__ __device__ inline Work work_of(const SharedAttnArgs& a) {
   w.head = a.work;
   w.piece = reinterpret_cast<Piece*>(a.work + 4);
   w.entry = reinterpret_cast<int4*>(w.piece + a.num_pieces + 1);
-  w.cta = w.entry + a.entries;
+  w.cta = w.entry + (size_t)a.entries * a.num_kv_heads;
   return w;
 }
 
 ZS_DEVICE int group_of(const SharedAttnArgs& a) { return a.num_q_heads / a.num_kv_heads; }
-// First cost of CTA c when `total` is divided over n CTAs, and the CTA of a cost.
-ZS_DEVICE int first_cost(int total, int n, int c) { return (int)((long long)total * c / n); }
-ZS_DEVICE int cta_of(int total, int n, int cost) { return (int)(((long long)(cost + 1) * n - 1) / total); }
-ZS_DEVICE int active_ctas(int total) { return min(CTAS, total); }
+// The last i in [0, n) with x[i] <= v (x ascending, x[0] <= v).
+ZS_DEVICE int last_at(const int* x, int n, int v) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (x[mid] <= v) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// What a piece costs besides its tiles, in tiles: another Q; for a unit's first one also a pipeline
+// that starts anew and the records.  x: the first half of the piece's static description.
+ZS_DEVICE int piece_over(const int4& x, int i, int group) { return x.w == i ? 2 + x.z * group / 64 : 1; }
 
 // One CTA: the longest row of every segment decides how many pages it has; costs are counted and
 // the CTAs' ranges laid over them.
@@ -71,7 +80,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const SharedAttnArgs a) {
   pdl_trigger();
   __shared__ unsigned long long longest[MAX_SEGS];  // (length, ~entry)
   __shared__ int table[MAX_SEGS];
-  __shared__ int cost0[MAX_PIECES + 1];
+  __shared__ int cost0[MAX_PIECES + 1], start[CTAS + 1];
   __shared__ long long red[32];
   const Work w = work_of(a);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -102,22 +111,23 @@ __global__ void __launch_bounds__(1024) plan_kernel(const SharedAttnArgs a) {
     long long cost = 0;
     Piece g = {};
     if (i < a.num_pieces) {
-      // (segment, unit's first entry, unit's rows, starts a unit), (rows r0..r1 of it, pages p0..p1)
+      // (segment, unit's first entry, unit's rows, unit's first piece), (the next unit's first piece, its
+      // rows r0 << 16 | r1 of the unit, pages p0..p1)
       const int4 x = i0 == 0 ? px : reinterpret_cast<const int4*>(a.pieces)[2 * i];
       const int4 y = i0 == 0 ? py : reinterpret_cast<const int4*>(a.pieces)[2 * i + 1];
       const int len = (int)(longest[x.x] >> 32);
       g.e0 = x.y;
       g.rows = x.z;
-      // A unit costs a few tiles besides its own: a pipeline that starts anew, its Q, its records.
-      g.over = x.w != 0 ? 2 + x.z * group / 64 : 0;
-      g.r0 = y.x;
-      g.r1 = y.y;
+      g.over = piece_over(x, i, group);
+      g.r0 = y.y >> 16;
+      g.r1 = y.y & 0xFFFF;
       g.p0 = y.z;
       g.pend = (int)(((long long)len + PAGE - 1) / PAGE);
       if (y.w >= 0) g.pend = min(g.pend, y.w);
       g.nt = (max(g.pend - g.p0, 0) + TPAGES - 1) / TPAGES;
       g.len = (int)min((long long)len, (long long)g.pend * PAGE);
       g.table = table[x.x];
+      if (g.nt == 0 && x.w != i) g.over = 0;
       cost = g.nt + g.over;
     }
     long long x = cost;
@@ -143,35 +153,43 @@ __global__ void __launch_bounds__(1024) plan_kernel(const SharedAttnArgs a) {
     __syncthreads();
   }
   const bool fits = carry * a.num_kv_heads < (1ll << 30);  // lengths beyond any cache: nothing is read
-  const int each = fits ? (int)carry : 0, total = each * a.num_kv_heads, n = active_ctas(total);
+  const int each = fits ? (int)carry : 0, total = each * a.num_kv_heads, n = min(CTAS, total);
   if (tid == 0) {
     if (!fits) report_error(a.err, kErrBadShape);
     cost0[a.num_pieces] = w.piece[a.num_pieces].cost0 = each;
-    w.head[0] = total;
-    w.head[1] = each;
+    w.head[0] = each;
   }
   __syncthreads();
-  for (int c = tid; c < CTAS; c += 1024) {
-    const int t = c < n ? first_cost(total, n, c) : 0, rel = each > 0 ? t % each : 0;
-    int lo = 0, hi = a.num_pieces;  // the last piece with cost0 <= rel (empty ones before it share its cost0)
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (cost0[mid] <= rel) lo = mid; else hi = mid;
+  const int4* pieces = reinterpret_cast<const int4*>(a.pieces);
+  // Equal shares; a border near an end of a unit moves there (a CTA that only ends or only starts a
+  // unit with a tile or two pays for another Q and other records).
+  for (int c = tid; c <= CTAS; c += 1024) {
+    int at = c < n ? (int)((long long)total * c / n) : total;
+    if (at > 0 && at < total) {
+      const int rel = at % each, i = last_at(cost0, a.num_pieces, rel), u0 = pieces[2 * i].w, u1 = pieces[2 * i + 1].x;
+      const int near = min(3, total / n / 4), over = 2 + pieces[2 * i].z * group / 64;
+      if (rel < cost0[u0] + over + near) at += cost0[u0] - rel;
+      else if (rel + near >= cost0[u1]) at += cost0[u1] - rel;
     }
-    w.cta[c] = make_int4(t, c < n ? first_cost(total, n, c + 1) : 0, lo, 0);
+    start[c] = at;
   }
-  for (int e = tid; e < a.entries; e += 1024) {
-    const int i = e == tid ? at_piece : a.entry_piece[e];
-    const int4 x = reinterpret_cast<const int4*>(a.pieces)[2 * i];
-    const int over = x.w != 0 ? 2 + x.z * group / 64 : 0;
-    w.entry[e] = make_int4(cost0[i] + over, fits ? cost0[i + 1] - cost0[i] - over : 0, (e - x.y) * group, 0);
+  __syncthreads();
+  for (int c = tid; c < CTAS; c += 1024)
+    w.cta[c] = make_int4(start[c], start[c + 1], each > 0 ? last_at(cost0, a.num_pieces, start[c] % each) : 0, 0);
+  for (int x = tid; x < a.entries * a.num_kv_heads; x += 1024) {
+    const int e = x / a.num_kv_heads, i = e == tid ? at_piece : a.entry_piece[e];
+    const int4 p = pieces[2 * i];
+    const int over = piece_over(p, i, group), first = (x % a.num_kv_heads) * each + cost0[i] + over;
+    const int nt = fits ? max(0, cost0[i + 1] - cost0[i] - over) : 0;
+    const int c0 = nt > 0 ? last_at(start, CTAS, first) : 0, c1 = nt > 0 ? last_at(start, CTAS, first + nt - 1) : -1;
+    w.entry[x] = make_int4(c0, c1 - c0 + 1, (e - p.y) * group, 0);
   }
 }
 
 // A CTA's part of a piece: tiles [t0, t1) for the slots [s0, s1) of its unit.
 struct Fragment {
   int kvh, e0, slots, s0, s1, t0, t1, p0, pend, len, table;
-  int first;  // of the unit in this CTA: a new Q
+  int first;  // of the unit in this CTA
 };
 
 struct Walk {
@@ -208,21 +226,10 @@ struct Walk {
   }
 };
 
-// Position in the ring of stages and the parity of its barriers there.
-struct Ring {
-  int st = 0, ph = 0;
-  ZS_DEVICE void next(int n = 1) {
-    st += n;
-    if (st >= STAGES) {
-      st -= STAGES;
-      ph ^= 1;
-    }
-  }
-};
-
 struct Smem {
-  uint8_t ring[STAGES][STAGE];      // tiles as page images: K, V, K, V, ...
-  uint8_t way[SLOTS][528];          // Q on its way in and O on its way out: 256 bytes of a row for each half
+  uint8_t ring[2][STAGES][STAGE];   // tiles of K, and of V, as page images
+  uint8_t way[SLOTS][528];          // Q on its way to TMEM, 512 bytes a slot
+  float stage[8][32][20];           // a warp's 32 slots x 16 dims of O on their way out
   float top[2][2][SLOTS];           // per half of a tile's keys, the largest score of every slot
   int vote[2][8];
   int again[2];                     // the P of this tile is followed by its rounding errors
@@ -231,7 +238,7 @@ struct Smem {
   int least[AHEAD];                 // the fewest among the piece's slots
   volatile int abort;
   uint32_t tmem;
-  uint64_t full[STAGES], empty[STAGES], s_full[2], p_full[2], o_full[2], q_full, f_full[AHEAD], f_empty[AHEAD], r_full[AHEAD], way_full, way_empty;
+  uint64_t full[2][STAGES], empty[2][STAGES], s_full[2], p_full[2], o_full[2], q_full, f_full[AHEAD], f_empty[AHEAD], r_full[AHEAD], way_full[2], way_empty[2];
 };
 constexpr int SMEM = (int)sizeof(Smem);
 static_assert(SMEM <= 232448, "shared memory of one CTA");
@@ -322,8 +329,8 @@ constexpr float kGrow = 8.f;         // O is rescaled when a maximum grows by mo
 // then carries only the copies in and one read of K and V per tile (with Q and P^T there the
 // kernel was bound by shared-memory bandwidth).  A row of S, P and O is one TMEM lane; thread
 // (half, slot) of the softmax warps owns half of the keys of a tile, and of the dims of O.
-//  * copy warp: page ids, then one bulk copy per (page, kv head) block into a ring of four 32 KiB
-//    stages, running ahead across tiles and fragments;
+//  * copy warps, K and V: page ids, then one bulk copy per (page, kv head) block into two 32 KiB
+//    stages each, running ahead across tiles and pieces;
 //  * MMA warp: S of the next tile is issued before O of this one, so it runs under the softmax;
 //  * lookup warp: the next fragments, their rows and lengths, and their Q into shared memory;
 //  * softmax warps: P = 2^(s - m) with a reference m that follows the running maximum only when
@@ -346,9 +353,9 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
     tmem_relinquish();
   }
   if (tid == 0) {
-    for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&s.full[i], 1);
-      mbar_init(&s.empty[i], 1);
+    for (int i = 0; i < 2 * STAGES; ++i) {
+      mbar_init(&s.full[0][0] + i, 1);
+      mbar_init(&s.empty[0][0] + i, 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.s_full[i], 1);
@@ -361,8 +368,10 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
       mbar_init(&s.r_full[i], 32);
       mbar_init(&s.f_empty[i], COMPUTE / 32);
     }
-    mbar_init(&s.way_full, 1);
-    mbar_init(&s.way_empty, COMPUTE);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.way_full[i], 1);
+      mbar_init(&s.way_empty[i], COMPUTE);
+    }
     s.abort = 0;
     fence_barrier_init();
   }
@@ -387,13 +396,12 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
   };
   Fragment f;
 
-  if (warp == 8) {
+  if (warp == 8 || warp == 11) {
     // ------------------------------------------------------------------ copies
-    // Lane j holds the page id of the tile's page j and issues its K and V blocks.
-    const char* kc = static_cast<const char*>(a.k_cache);
-    const char* vc = static_cast<const char*>(a.v_cache);
-    Ring r;
-    int issued = 0;
+    // Warp 8 brings K, warp 11 V.  Lane j holds the page id of the tile's page j and issues its block.
+    const int kv = warp == 8 ? 0 : 1;
+    const char* cache = static_cast<const char*>(kv ? a.v_cache : a.k_cache);
+    int i = 0;  // tiles asked for
     bool ok = true;
     while (ok && __all_sync(0xffffffff, next_fragment(f))) {
       const int* pt = a.page_table + (size_t)f.table * a.max_pages;
@@ -403,43 +411,36 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
         return p < a.max_pages ? __ldg(pt + p) : -1;  // a length behind the table row: a bad page
       };
       int page = page_of(f.t0);
-      for (int t = f.t0; ok && t < f.t1; ++t) {
+      for (int t = f.t0; t < f.t1; ++t, ++i) {
         const int after = t + 1 < f.t1 ? page_of(t + 1) : 0;
-        const int np = min(TPAGES, f.pend - (f.p0 + t * TPAGES));
+        const int np = min(TPAGES, f.pend - (f.p0 + t * TPAGES)), st = i & 1;
         if (page < 0 || page >= a.num_pages) {
           report_error(a.err, kErrBadShape);
           page = 0;
         }
-        const size_t at = ((size_t)page * a.num_kv_heads + f.kvh) * BLOCK;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          ok = ok && wait_for(s, &s.empty[r.st], r.ph ^ 1, a.err);  // passes at once in the first round
-          ok = __all_sync(0xffffffff, ok);
-          if (!ok) break;
-          if (lane == 0) mbar_expect_tx(&s.full[r.st], np * BLOCK);
-          __syncwarp();
-          if (lane < np) bulk_load(s.ring[r.st] + lane * BLOCK, (kv ? vc : kc) + at, BLOCK, &s.full[r.st]);
-          r.next();
-          ++issued;
-        }
+        if (i >= STAGES) ok = wait_for(s, &s.empty[kv][st], ((i >> 1) - 1) & 1, a.err);
+        ok = __all_sync(0xffffffff, ok);
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(&s.full[kv][st], np * BLOCK);
+        __syncwarp();
+        if (lane < np)
+          bulk_load(s.ring[kv][st] + lane * BLOCK, cache + ((size_t)page * a.num_kv_heads + f.kvh) * BLOCK, BLOCK, &s.full[kv][st]);
         page = after;
       }
     }
     // Copies in flight land before the CTA gives its shared memory back.
     if (lane == 0)
-      for (int m = max(0, issued - STAGES); m < issued; ++m) mbar_wait(&s.full[m % STAGES], (m / STAGES) & 1, nullptr);
+      for (int m = max(0, i - STAGES); m < i; ++m) mbar_wait(&s.full[kv][m & 1], (m >> 1) & 1, nullptr);
   } else if (warp == 9) {
     // -------------------------------------------------------------------- MMA
     // The warp stays together; one elected lane issues.
     const bool leader = elect_one();
     const uint32_t idesc_s = make_idesc_bf16(SLOTS, TILE, 0, 0), idesc_o = make_idesc_bf16(SLOTS, D, 0, 1);
-    const uint32_t k_lo = desc_lo(s.ring, 16), v_lo = desc_lo(s.ring, 1024);
+    const uint32_t k_lo = desc_lo(s.ring[0], 16), v_lo = desc_lo(s.ring[1], 1024);
     int ns = 0, no = 0;  // issued products
-    Ring kr, vr;
-    vr.next();
     auto scores = [&](int i) {  // S of tile i
-      const int st = kr.st;
-      if (!wait_for(s, &s.full[st], kr.ph, a.err)) return false;
+      const int st = i & 1;
+      if (!wait_for(s, &s.full[0][st], (i >> 1) & 1, a.err)) return false;
       // It takes the place of the P two tiles before: products with different accumulators have
       // no order of their own.
       if (i >= 2 && !wait_for(s, &s.o_full[i & 1], ((i >> 1) - 1) & 1, a.err)) return false;
@@ -449,18 +450,17 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
 #pragma unroll
         for (int x = 0; x < D / 16; ++x)  // 16 dims each: 4 in a 64-dim chunk, 8 columns of Q
           mma_step(d, tmem + kTmemQ + x * 8, k_at + (x >> 2) * (1024 / 16) + (x & 3) * 2, idesc_s, x > 0);
-        tc_commit(&s.empty[st]);
+        tc_commit(&s.empty[0][st]);
         tc_commit(&s.s_full[i & 1]);
       }
-      kr.next(2);
       ++ns;
       return true;
     };
     // O of tile i, for the rows of its piece alone: the others' stay as they are, whatever the tile holds.
     uint32_t off[4];
     auto output = [&](int i, bool fresh) {
-      const int st = vr.st, b = i & 1;
-      if (!wait_for(s, &s.full[st], vr.ph, a.err)) return false;
+      const int st = i & 1, b = i & 1;
+      if (!wait_for(s, &s.full[1][st], (i >> 1) & 1, a.err)) return false;
       if (!wait_for(s, &s.p_full[b], (i >> 1) & 1, a.err)) return false;
       tc_fence_after();
       const uint32_t v_at = v_lo + st * (STAGE / 16), p_at = tmem + b * TILE;
@@ -474,10 +474,9 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
           for (int k = 0; k < TPAGES; ++k)
             mma_step_rows(tmem + kTmemO, p_at + 32 + k * 8, v_at + k * (BLOCK / 16), idesc_o, off, true);
         }
-        tc_commit(&s.empty[st]);
+        tc_commit(&s.empty[1][st]);
         tc_commit(&s.o_full[b]);
       }
-      vr.next(2);
       ++no;
       return true;
     };
@@ -496,7 +495,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
         bool next = t + 1 < t1;
         if (!next) {
           next = more = __all_sync(0xffffffff, next_fragment(f));
-          if (more && f.first) ok = wait_for(s, &s.q_full, nq++ & 1, a.err);
+          if (more) ok = wait_for(s, &s.q_full, nq++ & 1, a.err);
         }
         ok = ok && (!next || scores(i + 1)) && output(i, t == t0);
         ok = __all_sync(0xffffffff, ok);
@@ -508,14 +507,13 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
     __syncwarp();
   } else if (warp == 10) {
     // ----------------------------------------------------------------- lookup
-    // What a fragment is, its rows and their lengths, AHEAD fragments before the others are done;
-    // and its Q into the way as soon as that is free.
+    // The pieces ahead, their slots' lengths, and their queries to shared memory.
     const Work w = work_of(a);
     const int4 mine = __ldg(w.cta + cta);
-    Walk walk{mine.x, mine.y, mine.z, max(1, __ldg(w.head + 1)), group, -1, -1};
+    Walk walk{mine.x, mine.y, mine.z, max(1, __ldg(w.head)), group, -1, -1};
     const char* qbase = static_cast<const char*>(a.q);
     bool ok = true, more = true;
-    int row[4], len[4], units = 0;
+    int row[4], len[4], parts = 0;  // pieces whose Q was asked for
     for (int at = 0, ph = 0; ok && more;) {
       more = walk.next(a, w, f);
       if (!more) f.t1 = 0;
@@ -528,19 +526,27 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
       if (f.first) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) row[j] = j * 32 + lane < f.slots ? a.seg_rows[f.e0 + (j * 32 + lane) / group] : -1;
-        ok = units == 0 || wait_for(s, &s.way_empty, (units - 1) & 1, a.err);
-        ok = __all_sync(0xffffffff, ok);
-        if (!ok) break;
-        if (lane == 0) mbar_expect_tx(&s.way_full, f.slots * D * 2);
-        __syncwarp();
+      }
+      // Queries of two pieces of a unit may be on their way (their slots differ); those of the next
+      // unit wait until all of the last one's have left.
+      if (parts >= 2) ok = wait_for(s, &s.way_empty[parts & 1], ((parts >> 1) - 1) & 1, a.err);
+      if (f.first && parts >= 1) ok = ok && wait_for(s, &s.way_empty[(parts - 1) & 1], ((parts - 1) >> 1) & 1, a.err);
+      ok = __all_sync(0xffffffff, ok);
+      if (!ok) break;
+      // The queries of the piece's slots, then the lengths of its rows.
+      if (lane == 0) mbar_expect_tx(&s.way_full[parts & 1], (f.s1 - f.s0) * D * 2);
+      __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (row[j] >= 0)
-            bulk_load(s.way[j * 32 + lane], qbase + ((size_t)row[j] * a.num_q_heads + f.kvh * group + (j * 32 + lane) % group) * (D * 2),
-                      D * 2, &s.way_full);
+      for (int j = 0; j < 4; ++j) {
+        const int sl = j * 32 + lane;
+        if (sl >= f.s0 && sl < f.s1)
+          bulk_load(s.way[sl], qbase + ((size_t)row[j] * a.num_q_heads + f.kvh * group + sl % group) * (D * 2), D * 2, &s.way_full[parts & 1]);
+      }
+      ++parts;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) len[j] = row[j] >= 0 ? max(a.seq_lens[row[j]], 0) : 0;
-        ++units;
+      for (int j = 0; j < 4; ++j) {
+        const int sl = j * 32 + lane;
+        len[j] = sl >= f.s0 && sl < f.s1 ? max(a.seq_lens[row[j]], 0) : 0;
       }
       int least = 0x7FFFFFFF;
 #pragma unroll
@@ -558,7 +564,8 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
         ph ^= 1;
       }
     }
-    if (lane == 0 && units > 0) mbar_wait(&s.way_full, (units - 1) & 1, nullptr);  // no copy outlives the CTA
+    if (lane == 0)  // no copy outlives the CTA
+      for (int k = max(0, parts - 2); k < parts; ++k) mbar_wait(&s.way_full[k & 1], (k >> 1) & 1, nullptr);
   } else {
     // ---------------------------------------------------------------- softmax
     const int half = warp >> 2, slot = (warp & 3) * 32 + lane;
@@ -566,9 +573,9 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
     const float qscale = a.sm_scale * 1.4426950408889634f;             // exp2 domain
     const int head = slot % group;
     auto way = [&](int r, int p) { return s.way[r] + ((half * 16 + p) << 4); };  // 16-byte piece p of the warp's half
-    auto store_q = [&](int slots, int k) {  // Q of fragment k from the way to TMEM
-      wait_for(s, &s.way_full, k & 1, a.err);
-      if ((warp & 3) * 32 < slots) {
+    auto store_q = [&](const Fragment& g, int k) {  // Q of piece k from the way to TMEM
+      wait_for(s, &s.way_full[k & 1], (k >> 1) & 1, a.err);
+      if ((warp & 3) * 32 < g.s1 && (warp & 3) * 32 + 32 > g.s0) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           uint32_t r[16];
@@ -580,20 +587,15 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
       }
       tc_fence_before();
       mbar_arrive(&s.q_full);
+      mbar_arrive(&s.way_empty[k & 1]);
     };
     // After a wait that gave up these warps go on to the end of the fragment with whatever is there (the
     // error word is set, every later wait gives up at once) and leave together: their barriers always meet.
     bool more = !compute_any(!next_fragment(f));
     int kf = 0;  // place of the piece
     uint32_t kph = 0;
-    if (more) {
-      store_q(f.slots, 0);
-      fence_proxy_async_shared();
-      mbar_arrive(&s.way_empty);
-    }
-    int i = 0, units = 1;
-    Ring vr;
-    vr.next();
+    if (more) store_q(f, 0);
+    int i = 0, parts = 1;
     float m = -INFINITY, l = 0.f;  // reference maximum (raw scores) of the slot, sum of this half's weights
     int rec = -1;                  // record of the slot, once it had a tile
     while (more) {
@@ -608,13 +610,13 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
         l = 0.f;
       }
       Fragment g = {};
-      for (int t = f.t0; t < f.t1; ++t, ++i, vr.next(2)) {
+      for (int t = f.t0; t < f.t1; ++t, ++i) {
         const int b = i & 1, key0 = (f.p0 + t * TPAGES) * PAGE;
         wait_for(s, &s.s_full[b], (i >> 1) & 1, a.err);
         tc_fence_after();
         if (t + 1 == f.t1) {
           more = !compute_any(!next_fragment(g));
-          if (more && g.first) store_q(g.slots, units++);  // every product with this Q is done: the next takes its place
+          if (more) store_q(g, parts++);  // every product with this Q is done: the next takes its place
         }
         uint32_t r[32];
         float mt = -INFINITY;
@@ -699,17 +701,17 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
         const int end = f.len - key0;  // keys of the tile that some row sees
         unsigned long long odd = 0;
         if (end < TILE || least < key0 + TILE) {
-          const int st = vr.st;
-          wait_for(s, &s.full[st], vr.ph, a.err);
+          uint8_t* const vt = s.ring[1][b];
+          wait_for(s, &s.full[1][b], (i >> 1) & 1, a.err);
           const int from = max(0, min(least - key0, TILE)), stop = min(end, TILE);
           bool found = false;
           for (int x = from * 32 + tid; x < stop * 32; x += COMPUTE) {
-            const uint4 v = *reinterpret_cast<const uint4*>(s.ring[st] + tile_offset(x >> 5, x & 31));
+            const uint4 v = *reinterpret_cast<const uint4*>(vt + tile_offset(x >> 5, x & 31));
             found |= not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w);
           }
           if (from < stop && compute_any(found)) {
             for (int k = from; k < stop; ++k) {  // 512 bytes a key: 4 for each of 128 threads
-              uint32_t* at = reinterpret_cast<uint32_t*>(s.ring[st] + tile_offset(k, (tid & 127) >> 2)) + (tid & 3);
+              uint32_t* at = reinterpret_cast<uint32_t*>(vt + tile_offset(k, (tid & 127) >> 2)) + (tid & 3);
               if (compute_any(not_finite(*at))) {
                 odd |= 1ull << k;
                 *at = 0;
@@ -717,7 +719,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
             }
           }
           for (int x = max(end, 0) * 32 + tid; x < TILE * 32; x += COMPUTE)
-            *reinterpret_cast<uint4*>(s.ring[st] + tile_offset(x >> 5, x & 31)) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(vt + tile_offset(x >> 5, x & 31)) = make_uint4(0, 0, 0, 0);
           fence_proxy_async_shared();
         }
         tc_fence_before();
@@ -778,28 +780,27 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
           }
         } else if (has != 0) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < 128; c += 32) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(lanes + kTmemO + half * 128 + c, o);
+            tmem_ld_wait();
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-              uint32_t o[32];
-              tmem_ld_32x32b_x32(lanes + kTmemO + half * 128 + c * 64 + q * 32, o);
-              tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
-                *reinterpret_cast<uint4*>(way(slot, q * 8 + j)) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+              for (int j = 0; j < 16; j += 4)
+                *reinterpret_cast<uint4*>(&s.stage[warp][lane][j]) =
+                    make_uint4(o[q * 16 + j], o[q * 16 + j + 1], o[q * 16 + j + 2], o[q * 16 + j + 3]);
+              __syncwarp();
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {  // 8 rows of 64 bytes an instruction
+                const int x = 8 * j + (lane >> 2), rx = __shfl_sync(0xffffffff, rec, x);
+                if (rx >= 0)
+                  *reinterpret_cast<uint4*>(a.partial + (size_t)rx * PREC + half * 128 + c + q * 16 + (lane & 3) * 4) =
+                      *reinterpret_cast<const uint4*>(&s.stage[warp][x][(lane & 3) * 4]);
+              }
+              __syncwarp();
             }
-            __syncwarp();
-#pragma unroll 4
-            for (int j = 0; j < 16; ++j) {
-              const int x = 2 * j + (lane >> 4);
-              const int rx = __shfl_sync(0xffffffff, rec, x);
-              if (rx >= 0)
-                *reinterpret_cast<uint4*>(a.partial + (size_t)rx * PREC + half * 128 + c * 64 + (lane & 15) * 4) =
-                    *reinterpret_cast<const uint4*>(way((warp & 3) * 32 + x, lane & 15));
-            }
-            __syncwarp();
           }
-          fence_proxy_async_shared();
         }
         if (rec >= 0) {
           if (half == 0) *reinterpret_cast<float2*>(to + D) = make_float2(m * qscale, l);
@@ -807,7 +808,6 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
         }
         rec = -1;
         tc_fence_before();
-        mbar_arrive(&s.way_empty);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.f_empty[kf]);
@@ -843,7 +843,6 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const SharedAtt
   const int item = blockIdx.x * (MERGE_WARPS / PARTS) + warp / PARTS;
   if (item >= a.rows * a.num_q_heads) return;  // PARTS == 1 alone
   const int row = item / a.num_q_heads, h = item % a.num_q_heads, group = group_of(a);
-  const int total = w.head[0], each = w.head[1], n = active_ctas(total);
   float m = -INFINITY, l = 0.f, o[8] = {};
   // A lane per segment of the row: where its records are.  first[j] = records before segment j.
   const int own = a.row_entry[row * a.levels + min(lane, a.levels - 1)];
@@ -851,13 +850,10 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const SharedAtt
     const int e = j0 == 0 ? (lane < a.levels ? own : -1) : (j0 + lane < a.levels ? a.row_entry[row * a.levels + j0 + lane] : -1);
     int c0 = 0, cnt = 0, slot = 0;
     if (e >= 0) {
-      const int4 u = w.entry[e];
-      const int first = u.x + h / group * each;
+      const int4 u = w.entry[(size_t)e * a.num_kv_heads + h / group];
+      c0 = u.x;
+      cnt = u.y;
       slot = u.z + h % group;
-      if (u.y > 0) {
-        c0 = cta_of(total, n, first);
-        cnt = cta_of(total, n, first + u.y - 1) - c0 + 1;
-      }
     }
     int before = cnt;
 #pragma unroll

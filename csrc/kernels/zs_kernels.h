@@ -689,9 +689,9 @@ typedef struct SharedAttnArgs {
   const int* entry_seg;      // [entries]
   const int* entry_piece;    // [entries]
   const int* row_entry;      // [rows, levels] entry of each row's segments, -1: none (at the end)
-  const int* pieces;         // [num_pieces, 8]: segment, first entry and rows of its unit, whether it is the
-                             // unit's first piece, its rows [r0, r1) in the unit, page0, page1; 16-byte aligned
-  int* work;                 // [ZS_SHARED_WORK_INTS(num_pieces, entries)], 16-byte aligned, written by the plan
+  const int* pieces;         // [num_pieces, 8]: segment, first entry and rows of its unit, first piece of the unit
+                             // and of the next, its rows r0 << 16 | r1 in the unit, page0, page1; 16-byte aligned
+  int* work;                 // [ZS_SHARED_WORK_INTS(num_pieces, entries * num_kv_heads)], 16-byte aligned, written by the plan
   float* partial;            // scratch: 260 floats x (entries * num_q_heads + ZS_SHARED_CTAS * ZS_SHARED_SLOTS)
   float sm_scale;            // > 0
   void* out_bf16;            // optional [rows, num_q_heads * 256]
@@ -700,7 +700,7 @@ typedef struct SharedAttnArgs {
   int* err;
 } SharedAttnArgs;
 
-#define ZS_SHARED_WORK_INTS(num_pieces, entries) (4 + 12 * ((num_pieces) + 1) + 4 * (entries) + 4 * ZS_SHARED_CTAS)
+#define ZS_SHARED_WORK_INTS(num_pieces, heads) (4 + 12 * ((num_pieces) + 1) + 4 * (heads) + 4 * ZS_SHARED_CTAS)
 
 // Divide the step's keys over the GPU (from seq_lens, row_slot, the segments and the head counts;
 // q, caches and outputs are not read): once a step.  Then one zs_shared_attn per layer.

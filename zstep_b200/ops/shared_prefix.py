@@ -38,6 +38,7 @@ class SharedPrefixPlan:
         seg_rows, entry_seg, entry_piece, pieces = [], [], [], []
         room = SLOTS // (num_q_heads // num_kv_heads)   # rows of a work unit
         unit = [0, 0]                                   # first entry and rows of the last one
+        units: list[int] = []                           # first piece of each
         for s, i in enumerate(order):
             members, first, end = segments[i]
             if not members:
@@ -61,7 +62,9 @@ class SharedPrefixPlan:
                 if start:
                     unit = [done, 0]
                 take = min(left, room - unit[1])
-                pieces.append([s, unit, int(start), unit[1], unit[1] + take, first, -1 if end is None else end])
+                if start:
+                    units.append(len(pieces))
+                pieces.append((s, unit, len(units) - 1, unit[1] << 16 | unit[1] + take, first, -1 if end is None else end))
                 unit[1] += take
                 entry_piece += [len(pieces) - 1] * take
                 done += take
@@ -77,11 +80,12 @@ class SharedPrefixPlan:
         i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
         self.slots = i32(slots)
         self._num_segs = len(order)
+        ends = units + [len(pieces)]
         self._segs = [i32(seg_rows), i32(entry_seg), i32(entry_piece),
                       i32([x for e in row_entry for x in e + [-1] * (self.levels - len(e))]),
-                      i32([x for s, u, start, r0, r1, p0, p1 in pieces for x in (s, u[0], u[1], start, r0, r1, p0, p1)])]
+                      i32([x for s, u, k, r, p0, p1 in pieces for x in (s, u[0], u[1], ends[k], ends[k + 1], r, p0, p1)])]
         self.err = torch.zeros(1, dtype=torch.int32, device=device)
-        ints, floats = self.C.shared_attn_sizes(len(pieces), len(seg_rows), num_q_heads)
+        ints, floats = self.C.shared_attn_sizes(len(pieces), len(seg_rows), num_q_heads, num_kv_heads)
         self._work = torch.zeros(ints, dtype=torch.int32, device=device)
         self._partial = torch.empty(floats, dtype=torch.float32, device=device)
         self._planned = False
