@@ -286,6 +286,15 @@ ZS_DEVICE float pick(bool c, float x, float y) {
   asm("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\tselp.f32 %0, %1, %2, p;\n\t}" : "=f"(r) : "f"(x), "f"(y), "r"((int)c));
   return r;
 }
+ZS_DEVICE void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+// Arrives on the barrier when the thread's copies so far have landed.
+ZS_DEVICE void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+ZS_DEVICE void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // One tcgen05.mma with A in TMEM.  The B descriptors of a product differ in their low words alone
 // (start address, leading offset): the high word (stride, version, 128-byte swizzle) is a constant.
 constexpr uint32_t desc_hi(uint32_t stride) { return (stride >> 4) | (1u << 14) | (2u << 29); }
@@ -369,7 +378,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
       mbar_init(&s.f_empty[i], COMPUTE / 32);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s.way_full[i], 1);
+      mbar_init(&s.way_full[i], 32);
       mbar_init(&s.way_empty[i], COMPUTE);
     }
     s.abort = 0;
@@ -513,7 +522,9 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
     Walk walk{mine.x, mine.y, mine.z, max(1, __ldg(w.head)), group, -1, -1};
     const char* qbase = static_cast<const char*>(a.q);
     bool ok = true, more = true;
-    int row[4], len[4], parts = 0;  // pieces whose Q was asked for
+    int row[4], len[4], head[4], parts = 0;  // pieces whose Q was asked for
+#pragma unroll
+    for (int j = 0; j < 4; ++j) head[j] = (j * 32 + lane) % group;
     for (int at = 0, ph = 0; ok && more;) {
       more = walk.next(a, w, f);
       if (!more) f.t1 = 0;
@@ -534,14 +545,16 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
       ok = __all_sync(0xffffffff, ok);
       if (!ok) break;
       // The queries of the piece's slots, then the lengths of its rows.
-      if (lane == 0) mbar_expect_tx(&s.way_full[parts & 1], (f.s1 - f.s0) * D * 2);
-      __syncwarp();
+      // (Not bulk copies: those would wait behind the tiles that the copy warps asked for.)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int sl = j * 32 + lane;
-        if (sl >= f.s0 && sl < f.s1)
-          bulk_load(s.way[sl], qbase + ((size_t)row[j] * a.num_q_heads + f.kvh * group + sl % group) * (D * 2), D * 2, &s.way_full[parts & 1]);
+        const int index = row[j] * a.num_q_heads + f.kvh * group + head[j];
+        const int lo = max(f.s0, j * 32), hi = min(f.s1, j * 32 + 32);
+#pragma unroll 8
+        for (int x = lo; x < hi; ++x)
+          cp_async16(s.way[x] + lane * 16, qbase + (size_t)__shfl_sync(0xffffffff, index, x & 31) * (D * 2) + lane * 16);
       }
+      cp_async_arrive(&s.way_full[parts & 1]);
       ++parts;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -564,8 +577,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
         ph ^= 1;
       }
     }
-    if (lane == 0)  // no copy outlives the CTA
-      for (int k = max(0, parts - 2); k < parts; ++k) mbar_wait(&s.way_full[k & 1], (k >> 1) & 1, nullptr);
+    cp_async_wait();
   } else {
     // ---------------------------------------------------------------- softmax
     const int half = warp >> 2, slot = (warp & 3) * 32 + lane;
