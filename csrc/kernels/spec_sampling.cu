@@ -14,14 +14,19 @@
 //
 // A probability below 2^-38 (4e-12) counts as 0: the mass that can lose is below 1e-6 of a row
 // of 2^18 tokens, the rounding of a 32-bit softmax over it.
+#include <cooperative_groups.h>
+
 #include "sm100_common.cuh"
 #include "zs_kernels.h"
 
 namespace zs {
 namespace spec {
 
-constexpr int T = 1024;
+namespace cg = cooperative_groups;
+
 constexpr float kFix = 274877906944.0f;  // 2^38
+constexpr float kMax = 3.4028234663852886e38f;
+constexpr int kCluster = 16;             // CTAs on a row at most
 typedef unsigned long long u64;
 
 ZS_DEVICE uint32_t okey(float f) {
@@ -31,25 +36,350 @@ ZS_DEVICE uint32_t okey(float f) {
 ZS_DEVICE float from_okey(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k); }
 
 // NaN counts as masked, +inf as the largest number (two of them share the mass).
-ZS_DEVICE float clean(float x) { return x != x ? -INFINITY : fminf(x, 3.4028234663852886e38f); }
+ZS_DEVICE float clean(float x) { return x != x ? -INFINITY : fminf(x, kMax); }
+
+ZS_DEVICE float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 template <typename V, typename F>
-ZS_DEVICE V block_all(V v, V* red, F op) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffff, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[threadIdx.x & 31];
+ZS_DEVICE V warp_all(V v, F op) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffff, v, o));
   return v;
 }
+// Over all threads of the block; red: a value per warp.
+template <int WARPS, typename V, typename F>
+ZS_DEVICE V block_all(V v, V* red, F op, V none) {
+  v = warp_all(v, op);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return warp_all((threadIdx.x & 31) < WARPS ? red[threadIdx.x & 31] : none, op);
+}
 
-// Probabilities of one row (a CTA each): max, top-k threshold (radix select over the ordered
-// image of the logit, ties with the k-th kept), top-p threshold (the same over fixed-point
-// masses, whose histogram sums have one value; ties kept), sum of the kept, quotients.
-__global__ void __launch_bounds__(T) probs_kernel(const TokenProbsArgs a) {
+// The other CTAs of a cluster may be written to once they run: announced at the start, waited for
+// before the first access.
+ZS_DEVICE void cluster_started() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+ZS_DEVICE void cluster_wait_started() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
+// ---------------------------------------------------------------------------------------
+// Token probabilities.  A cluster of up to 16 CTAs holds a row in shared memory (64 KiB each, two
+// CTAs to an SM, so that one loads while the other computes): the row is read once and written
+// once whatever it asks for.  What the CTAs have to know of one another goes through distributed
+// shared memory.
+//   plain     e = 2^((x - m) c) against the CTA's own maximum and its sum; (m, sum) of all CTAs;
+//             one exchange.
+//   greedy    the row's maximum, then its lowest id.
+//   top-k     up to 256: the k-th largest of the warps' maxima (at least k logits are as large)
+//             leaves little more than k candidates, which every CTA ranks for itself: exact
+//             threshold, nucleus and sum from the sorted list.  Two exchanges.
+//   otherwise (a nucleus of the whole vocabulary, k above 256, many ties): radix select by 8 bits
+//             of the ordered image of the logit over histograms of counts or of fixed-point masses,
+//             whose sums have one value in any order.
+constexpr int PT = 512, PW = PT / 32;
+constexpr int kChunk = 16384;            // logits of a CTA at most
+constexpr int kSmallK = 256;             // as many as a full row has warps
+constexpr int kList = 256, kCand = 1024; // candidates of a CTA, of a row
+
+struct ProbsSmem {
+  float x[kChunk];
+  union {
+    struct {
+      float list[kCluster][kList];
+      float cand[kCand], sorted[kCand];
+    };
+    u64 hist[PW][256];                   // a histogram per warp; [0] is the CTA's
+  };
+  u64 total[256];
+  uint32_t warp_max[kCluster][PW];
+  float2 part[kCluster];                 // (maximum, sum) of every CTA
+  uint32_t first[kCluster];              // greedy: lowest id of the maximum
+  int count[kCluster];                   // candidates of every CTA
+  u64 red[32], left;
+  float bound;
+  uint32_t pick;
+  int mine;
+};
+static_assert(2 * (sizeof(ProbsSmem) + 1024) <= 228 * 1024, "two CTAs on an SM");
+
+ZS_DEVICE void cp_async(void* dst, const void* src, bool wide) {
+  const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+  if (wide) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(d), "l"(src) : "memory");
+}
+
+template <int VEC>
+__global__ void __launch_bounds__(PT, 2) probs_kernel(const TokenProbsArgs a) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  ProbsSmem& s = *reinterpret_cast<ProbsSmem*>(raw);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int n = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), row = blockIdx.x / n;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, V = a.vocab;
+  cluster_started();
+  pdl_wait();
+  pdl_trigger();
+  const int chunk = ((V + n - 1) / n + 3) & ~3, base = rank * chunk, len = max(0, min(V - base, chunk));
+  const float* in = a.logits + row * a.ld + base;
+  float* out = a.out + row * a.ld_out + base;
+  // A thread reads what it brought itself: groups of VEC logits, PT groups apart.
+  for (int i = tid * VEC; i < len; i += PT * VEC) {
+    if (VEC == 4 && i + 3 < len) {
+      cp_async(s.x + i, in + i, true);
+    } else {
+      for (int k = 0; k < VEC; ++k) {
+        if (i + k < len) cp_async(s.x + i + k, in + i + k, false);
+        else s.x[i + k] = -INFINITY;
+      }
+    }
+  }
+  const float temp = a.temperature[row];
+  const int K = a.top_k != nullptr ? a.top_k[row] : 0;
+  const float P = a.top_p != nullptr ? a.top_p[row] : 1.f;
+  const bool greedy = !(temp > 0.f), by_k = !greedy && K > 0 && K < V, by_p = !greedy && P < 1.f;
+  const float c = greedy ? 0.f : fminf(1.4426950408889634f / temp, kMax);  // exponents in the exp2 domain
+  // f(place in the chunk, logit) for this thread's logits; the last group may pass len (masked there).
+  auto each = [&](auto f) {
+#pragma unroll 2
+    for (int i = tid * VEC; i < len; i += PT * VEC) {
+      if (VEC == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(s.x + i);
+        f(i, clean(v.x));
+        f(i + 1, clean(v.y));
+        f(i + 2, clean(v.z));
+        f(i + 3, clean(v.w));
+      } else {
+        f(i, clean(s.x[i]));
+      }
+    }
+  };
+  // out = value(place, logit).
+  auto store = [&](auto value) {
+#pragma unroll 2
+    for (int i = tid * VEC; i < len; i += PT * VEC) {
+      if (VEC == 4 && i + 3 < len) {
+        const float4 v = *reinterpret_cast<const float4*>(s.x + i);
+        __stcs(reinterpret_cast<float4*>(out + i),
+               make_float4(value(i, clean(v.x)), value(i + 1, clean(v.y)), value(i + 2, clean(v.z)), value(i + 3, clean(v.w))));
+      } else {
+        for (int k = 0; k < VEC; ++k)
+          if (i + k < len) __stcs(out + i + k, value(i + k, clean(s.x[i + k])));
+      }
+    }
+  };
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  float top = -INFINITY;
+  each([&](int, float x) { top = fmaxf(top, x); });
+  cluster_wait_started();
+
+  if (!greedy && !by_k && !by_p) {
+    top = block_all<PW>(top, reinterpret_cast<float*>(s.red), [](float p, float q) { return fmaxf(p, q); }, -INFINITY);
+    const float off = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    each([&](int, float x) { sum += ex2((x - off) * c); });
+    sum = block_all<PW>(sum, reinterpret_cast<float*>(s.red), [](float p, float q) { return p + q; }, 0.f);
+    if (tid < n) cluster.map_shared_rank(s.part, tid)[rank] = make_float2(top, sum);
+    cluster.sync();
+    const float2 p = lane < n ? s.part[lane] : make_float2(-INFINITY, 0.f);
+    const float all = warp_max(p.x);
+    const float z = warp_sum(p.x == -INFINITY ? 0.f : p.y * ex2((p.x - all) * c));
+    const float scale = top == -INFINITY ? 0.f : ex2((top - all) * c) / z;
+    store([&](int, float x) { return ex2((x - off) * c) * scale; });
+    return;
+  }
+
+  // The row's maximum, and every warp's.
+  {
+    const uint32_t k = __reduce_max_sync(0xffffffff, okey(top));
+    if (lane < n) cluster.map_shared_rank(&s.warp_max[0][0], lane)[rank * PW + warp] = k;
+  }
+  if (tid == 0) s.mine = 0;
+  cluster.sync();
+  uint32_t top_key = 0;
+  for (int i = lane; i < n * PW; i += 32) top_key = max(top_key, s.warp_max[0][i]);
+  top = from_okey(__reduce_max_sync(0xffffffff, top_key));
+
+  if (greedy || top == -INFINITY) {  // all mass on the best token, none where every token is masked
+    uint32_t first = 0xFFFFFFFFu;
+    if (top > -INFINITY)
+      each([&](int i, float x) {
+        if (x == top) first = min(first, (uint32_t)(base + i));
+      });
+    first = block_all<PW>(first, reinterpret_cast<uint32_t*>(s.red), [](uint32_t p, uint32_t q) { return min(p, q); }, 0xFFFFFFFFu);
+    if (tid < n) cluster.map_shared_rank(s.first, tid)[rank] = first;
+    cluster.sync();
+    first = __reduce_min_sync(0xffffffff, lane < n ? s.first[lane] : 0xFFFFFFFFu);
+    store([&](int i, float) { return (uint32_t)(base + i) == first ? 1.f : 0.f; });
+    return;
+  }
+
+  auto mass = [&](float v) { return ex2((v - top) * c); };
+  float thr = -INFINITY, inv = 0.f;  // keep x >= thr
+  bool done = false;
+  if (by_k && K <= min(kSmallK, n * PW)) {
+    // K-th largest of the warp maxima (equal ones in any order).
+    if (tid < n * PW) {
+      const uint32_t k = s.warp_max[0][tid];
+      int above = 0;
+      for (int i = 0; i < n * PW; ++i) above += s.warp_max[0][i] > k || (s.warp_max[0][i] == k && i < tid);
+      if (above == K - 1) s.bound = from_okey(k);
+    }
+    __syncthreads();
+    const float bound = s.bound;
+    if (bound > -INFINITY) {
+      each([&](int, float x) {
+        if (x >= bound) {
+          const int at = atomicAdd(&s.mine, 1);
+          if (at < kList)
+            for (int r = 0; r < n; ++r) cluster.map_shared_rank(&s.list[0][0], r)[rank * kList + at] = x;
+        }
+      });
+    }
+    __syncthreads();
+    // No bound (fewer than K warps have an unmasked logit), too many candidates: the general way.
+    if (tid < n) cluster.map_shared_rank(s.count, tid)[rank] = bound > -INFINITY ? s.mine : kList + 1;
+    cluster.sync();
+    int cnt = lane < n ? s.count[lane] : 0;
+    const int total = (int)__reduce_add_sync(0xffffffff, (unsigned)min(cnt, kList + 1));
+    done = __all_sync(0xffffffff, cnt <= kList) && total <= kCand;
+    if (done) {
+      // One list, ranked: larger values first.
+      int before = cnt;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffff, before, o);
+        if (lane >= o) before += y;
+      }
+      before -= cnt;
+      for (int r = warp; r < n; r += PW) {
+        const int at = __shfl_sync(0xffffffff, before, r), m = __shfl_sync(0xffffffff, cnt, r);
+        for (int i = lane; i < m; i += 32) s.cand[at + i] = s.list[r][i];
+      }
+      __syncthreads();
+      for (int i = tid; i < total; i += PT) {
+        const float v = s.cand[i];
+        int above = 0;
+        for (int y = 0; y < total; ++y) above += s.cand[y] > v || (s.cand[y] == v && y < i);
+        s.sorted[above] = v;
+      }
+      __syncthreads();
+      // Threshold, nucleus and sum by the first warp, in sorted order.
+      if (warp == 0) {
+        thr = s.sorted[K - 1];
+        float z = 0.f;
+        int kept = 0;
+        for (int i = lane; i < total; i += 32) {
+          const float v = s.sorted[i];
+          if (v >= thr) z += mass(v), ++kept;
+        }
+        z = warp_sum(z);
+        kept = (int)__reduce_add_sync(0xffffffff, (unsigned)kept);
+        if (by_p) {  // tokens in descending order while the mass before them is below P
+          const float goal = fmaxf(P, 0.f) * z;
+          float run = 0.f, keep_z = 0.f, last = s.sorted[0];
+          for (int i0 = 0; i0 < kept; i0 += 32) {
+            const float v = i0 + lane < kept ? s.sorted[i0 + lane] : -INFINITY, mv = v == -INFINITY ? 0.f : mass(v);
+            float inc = mv;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const float y = __shfl_up_sync(0xffffffff, inc, o);
+              if (lane >= o) inc += y;
+            }
+            const uint32_t in = __ballot_sync(0xffffffff, v > -INFINITY && (run + inc - mv < goal || i0 + lane == 0));
+            if (in != 0) last = __shfl_sync(0xffffffff, v, 31 - __clz(in));
+            run += __shfl_sync(0xffffffff, inc, 31);
+            if (in != 0xffffffffu) break;
+          }
+          thr = last;
+          for (int i = lane; i < kept; i += 32)
+            if (s.sorted[i] >= thr) keep_z += mass(s.sorted[i]);
+          z = warp_sum(keep_z);
+        }
+        if (lane == 0) s.part[0] = make_float2(thr, z);
+      }
+      __syncthreads();
+      thr = s.part[0].x;
+      inv = 1.f / s.part[0].y;
+    }
+  }
+
+  if (!done) {
+    uint32_t key_thr = 0;
+    for (int phase = 0; phase < 2; ++phase) {
+      const bool by_mass = phase == 1;
+      if (by_mass ? !by_p : !by_k) continue;
+      u64 need = (u64)K;
+      uint32_t prefix = 0;
+      for (int shift = 24; shift >= 0; shift -= 8) {
+        for (int i = tid; i < PW * 256; i += PT) (&s.hist[0][0])[i] = 0;
+        __syncthreads();
+        each([&](int, float x) {
+          const uint32_t k = okey(x);
+          const bool counts = x > -INFINITY && k >= key_thr && (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)));
+          if (counts) atomicAdd(&s.hist[warp][(k >> shift) & 255], by_mass ? (u64)(mass(x) * kFix) : 1ull);
+        });
+        __syncthreads();
+        if (tid < 256) {
+          u64 sum = 0;
+          for (int i = 0; i < PW; ++i) sum += s.hist[i][tid];
+          s.hist[0][tid] = sum;
+        }
+        cluster.sync();
+        if (tid < 256) {
+          u64 sum = 0;
+          for (int r = 0; r < n; ++r) sum += cluster.map_shared_rank(&s.hist[0][0], r)[tid];
+          s.total[tid] = sum;
+        }
+        cluster.sync();  // the others have read this CTA's
+        __syncthreads();
+        if (warp == 0) {  // lane l: bins 255 - 8 l and the 7 below
+          u64 sum = 0;
+          for (int d = 0; d < 8; ++d) sum += s.total[255 - 8 * lane - d];
+          u64 upto = sum;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const u64 y = __shfl_up_sync(0xffffffff, upto, o);
+            if (lane >= o) upto += y;
+          }
+          if (by_mass && shift == 24) {
+            need = (u64)((double)fmaxf(P, 0.f) * (double)__shfl_sync(0xffffffff, upto, 31));
+            if (need == 0) need = 1;
+          }
+          const uint32_t enough = __ballot_sync(0xffffffff, upto >= need);
+          if (lane == (enough != 0 ? __ffs(enough) - 1 : 31)) {
+            u64 left = need - (upto - sum);
+            int d = 255 - 8 * lane;
+            const int low = d - 7;
+            for (; d > low && s.total[d] < left; --d) left -= s.total[d];
+            s.pick = prefix | ((uint32_t)d << shift);
+            s.left = left;
+          }
+        }
+        __syncthreads();
+        prefix = s.pick;
+        need = s.left;
+      }
+      key_thr = max(key_thr, prefix);
+    }
+    thr = key_thr == 0 ? -INFINITY : from_okey(key_thr);
+    float sum = 0.f;
+    each([&](int, float x) {
+      if (x >= thr) sum += mass(x);
+    });
+    sum = block_all<PW>(sum, reinterpret_cast<float*>(s.red), [](float p, float q) { return p + q; }, 0.f);
+    if (tid < n) cluster.map_shared_rank(s.part, tid)[rank] = make_float2(0.f, sum);
+    cluster.sync();
+    inv = 1.f / warp_sum(lane < n ? s.part[lane].y : 0.f);
+  }
+  store([&](int, float x) { return x >= thr ? mass(x) * inv : 0.f; });
+}
+
+// Vocabularies that 16 CTAs do not hold: a CTA per row reads it once per step.
+constexpr int T = 1024;
+
+__global__ void __launch_bounds__(T) probs_wide_kernel(const TokenProbsArgs a) {
   pdl_wait();
   pdl_trigger();
   const int tid = threadIdx.x, V = a.vocab;
@@ -65,7 +395,7 @@ __global__ void __launch_bounds__(T) probs_kernel(const TokenProbsArgs a) {
     const u64 k = ((u64)okey(clean(x[i])) << 32) | (uint32_t)~i;
     best = k > best ? k : best;
   }
-  best = block_all(best, red, [](u64 p, u64 q) { return p > q ? p : q; });
+  best = block_all<32>(best, red, [](u64 p, u64 q) { return p > q ? p : q; }, (u64)0);
   const float top = from_okey((uint32_t)(best >> 32));
   const float temp = a.temperature[blockIdx.x];
   if (top == -INFINITY || !(temp > 0.f)) {  // nothing left, or greedy: all mass on the best token
@@ -73,7 +403,7 @@ __global__ void __launch_bounds__(T) probs_kernel(const TokenProbsArgs a) {
     for (int i = tid; i < V; i += T) out[i] = i == id ? 1.f : 0.f;
     return;
   }
-  const float inv_t = fminf(1.f / temp, 3.4028234663852886e38f);
+  const float inv_t = fminf(1.f / temp, kMax);
   auto mass = [&](float v) { return exp2f((v - top) * inv_t * 1.4426950408889634f); };
   uint32_t thr = 0;  // keep keys >= thr
   const int K = a.top_k != nullptr ? a.top_k[blockIdx.x] : 0;
@@ -88,7 +418,7 @@ __global__ void __launch_bounds__(T) probs_kernel(const TokenProbsArgs a) {
         const float v = clean(x[i]);
         if (okey(v) >= thr) sum += (u64)(mass(v) * kFix);
       }
-      sum = block_all(sum, red, [](u64 p, u64 q) { return p + q; });
+      sum = block_all<32>(sum, red, [](u64 p, u64 q) { return p + q; }, (u64)0);
       need = (u64)((double)fmaxf(P, 0.f) * (double)sum);
       if (need == 0) need = 1;
     }
@@ -121,7 +451,7 @@ __global__ void __launch_bounds__(T) probs_kernel(const TokenProbsArgs a) {
     const float v = clean(x[i]);
     if (okey(v) >= thr) sum += mass(v);
   }
-  sum = block_all(sum, reinterpret_cast<float*>(red), [](float p, float q) { return p + q; });
+  sum = block_all<32>(sum, reinterpret_cast<float*>(red), [](float p, float q) { return p + q; }, 0.f);
   const float inv = 1.f / sum;
   for (int i = tid; i < V; i += T) {
     const float v = clean(x[i]);
@@ -132,111 +462,173 @@ __global__ void __launch_bounds__(T) probs_kernel(const TokenProbsArgs a) {
 ZS_DEVICE u64 fixed(float p) { return (u64)(fminf(fmaxf(p, 0.f), 1.f) * kFix); }
 ZS_DEVICE u64 ubits(float u) { return (u64)(fminf(fmaxf(u, 0.f), 0.99999994f) * 16777216.f); }
 
+// ---------------------------------------------------------------------------------------
+// Verification: a cluster per sequence; CTA r and warp w own contiguous parts of the vocabulary.
+// The row to draw from is read once for the parts' sums, which every CTA gets through
+// distributed shared memory; the warp whose part holds the drawn mass reads that part again.
+constexpr int VT = 512, VW = VT / 32;
+
 struct Weights {
   const float *p, *q;  // q: draft probabilities, or null
   int less;            // without q: the rejected draft, -1 for none
-  ZS_DEVICE u64 operator()(int i) const {
-    const u64 w = fixed(p[i]);
+  ZS_DEVICE u64 of(float x, float y, int i) const {
+    const u64 w = fixed(x);
     if (q != nullptr) {
-      const u64 v = fixed(q[i]);
+      const u64 v = fixed(y);
       return w > v ? w - v : 0;
     }
     return i == less ? 0 : w;
   }
+  ZS_DEVICE u64 operator()(int i) const { return of(p[i], q != nullptr ? q[i] : 0.f, i); }
 };
 
-// One CTA per sequence; each warp owns a contiguous part of the vocabulary.
-__global__ void __launch_bounds__(T) verify_kernel(const DraftVerifyArgs a) {
+template <int VEC>
+__global__ void __launch_bounds__(VT) verify_kernel(const DraftVerifyArgs a) {
+  __shared__ u64 part[kCluster][VW];  // sums of every warp of the row's CTAs
+  cg::cluster_group cluster = cg::this_cluster();
+  const int n = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), s = blockIdx.x / n;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.vocab;
+  cluster_started();
   pdl_wait();
   pdl_trigger();
-  const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.vocab;
-  __shared__ u64 part[33];
-  __shared__ int taken_s;
   const int m = a.counts != nullptr ? min(max(a.counts[s], 0), a.k) : a.k;
   const int* drafts = a.drafts + (size_t)s * a.k;
   const float* u = a.uniform + (size_t)s * (a.k + 1);
-  if (tid == 0) {
-    int j = 0;
-    for (; j < m; ++j) {
-      const int d = drafts[j];
-      if (d < 0 || d >= V) break;
-      const u64 p = fixed(a.target[s * a.target_seq + j * a.target_row + d]);
-      const u64 q = a.draft_probs != nullptr ? fixed(a.draft_probs[s * a.draft_seq + j * a.draft_row + d]) : (1ull << 38);
-      if (!(ubits(u[j]) * q < (p << 24))) break;
+  int taken = m;  // every warp finds it for itself: a lane per draft
+  for (int j0 = 0; j0 < m; j0 += 32) {
+    bool ok = true;
+    if (j0 + lane < m) {
+      const int j = j0 + lane, d = drafts[j];
+      ok = d >= 0 && d < V;
+      if (ok) {
+        const u64 p = fixed(a.target[s * a.target_seq + j * a.target_row + d]);
+        const u64 q = a.draft_probs != nullptr ? fixed(a.draft_probs[s * a.draft_seq + j * a.draft_row + d]) : (1ull << 38);
+        ok = ubits(u[j]) * q < (p << 24);
+      }
     }
-    taken_s = j;
+    const uint32_t no = __ballot_sync(0xffffffff, !ok);
+    if (no != 0) {
+      taken = j0 + __ffs(no) - 1;
+      break;
+    }
   }
-  __syncthreads();
-  const int taken = taken_s;
   const bool rejected = taken < m;
   Weights w{a.target + s * a.target_seq + taken * a.target_row, nullptr, -1};
   if (rejected) {
     if (a.draft_probs != nullptr) w.q = a.draft_probs + s * a.draft_seq + taken * a.draft_row;
     else w.less = drafts[taken];
   }
-  const int per = ((V + 31) / 32 + 31) / 32 * 32, i0 = min(V, warp * per), i1 = min(V, i0 + per);
+  const int per = ((V + n * VW - 1) / (n * VW) + 127) / 128 * 128, i0 = min(V, (rank * VW + warp) * per), i1 = min(V, i0 + per);
   u64 total = 0;
   for (int round = 0; round < 2; ++round) {
     u64 sum = 0;
-    for (int i = i0 + lane; i < i1; i += 32) sum += w(i);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffff, sum, o);
-    __syncthreads();
-    if (lane == 0) part[warp] = sum;
-    __syncthreads();
+    if (VEC == 4) {
+#pragma unroll 4
+      for (int i = i0 + lane * 4; i < i1; i += 128) {  // V and so i1 - i are multiples of 4
+        const float4 x = __ldg(reinterpret_cast<const float4*>(w.p + i));
+        const float4 y = w.q != nullptr ? __ldg(reinterpret_cast<const float4*>(w.q + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        sum += w.of(x.x, y.x, i) + w.of(x.y, y.y, i + 1) + w.of(x.z, y.z, i + 2) + w.of(x.w, y.w, i + 3);
+      }
+    } else {
+#pragma unroll 4
+      for (int i = i0 + lane; i < i1; i += 32) sum += w(i);
+    }
+    sum = warp_all(sum, [](u64 p, u64 q) { return p + q; });
+    if (round == 0) cluster_wait_started();
+    else cluster.sync();  // the first round's sums are read
+    if (lane < n) cluster.map_shared_rank(&part[0][0], lane)[rank * VW + warp] = sum;
+    cluster.sync();
     total = 0;
-    for (int j = 0; j < 32; ++j) total += part[j];
+    for (int j = lane; j < n * VW; j += 32) total += (&part[0][0])[j];
+    total = warp_all(total, [](u64 p, u64 q) { return p + q; });
     if (total != 0 || !rejected) break;
     w.q = nullptr;  // p <= q everywhere: the target itself
     w.less = -1;
   }
   const u64 un = ubits(u[a.k]);
   const u64 goal = un * (total >> 24) + ((un * (total & 0xFFFFFFull)) >> 24);
-  u64 before = 0;
-  for (int j = 0; j < warp; ++j) before += part[j];
   int* rec = a.record + (size_t)s * (a.k + 2);
-  if (tid == 0) {
-    rec[0] = taken + 1;
-    for (int j = 0; j <= a.k; ++j)
-      if (j != taken) rec[1 + j] = j < taken ? drafts[j] : -1;
-    if (total == 0) {
-      rec[1 + taken] = 0;
+  if (rank == 0 && tid <= a.k) {
+    if (tid == 0) rec[0] = taken + 1;
+    if (tid != taken) rec[1 + tid] = tid < taken ? drafts[tid] : -1;
+    else if (total == 0) {
+      rec[1 + tid] = 0;
       report_error(a.err, kErrBadShape);
     }
   }
-  if (total != 0 && goal >= before && goal < before + part[warp]) {
-    for (int i = i0; i < i1; i += 32) {
-      u64 x = i + lane < i1 ? w(i + lane) : 0;
+  if (total == 0) return;
+  u64 before = 0;
+  for (int j = lane; j < rank * VW + warp; j += 32) before += (&part[0][0])[j];
+  before = warp_all(before, [](u64 p, u64 q) { return p + q; });
+  if (goal < before || goal >= before + part[rank][warp]) return;
+  for (int i = i0; i < i1; i += 32) {
+    u64 x = i + lane < i1 ? w(i + lane) : 0;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const u64 y = __shfl_up_sync(0xffffffff, x, o);
-        if (lane >= o) x += y;
-      }
-      const uint32_t over = __ballot_sync(0xffffffff, before + x > goal);
-      if (over != 0) {
-        if (lane == 0) rec[1 + taken] = i + __ffs(over) - 1;
-        break;
-      }
-      before += __shfl_sync(0xffffffff, x, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 y = __shfl_up_sync(0xffffffff, x, o);
+      if (lane >= o) x += y;
     }
+    const uint32_t over = __ballot_sync(0xffffffff, before + x > goal);
+    if (over != 0) {
+      if (lane == 0) rec[1 + taken] = i + __ffs(over) - 1;
+      break;
+    }
+    before += __shfl_sync(0xffffffff, x, 31);
   }
 }
+
+// `kernel` on `rows` clusters of n CTAs.
+template <typename Args>
+int launch_clusters(void (*kernel)(Args), int rows, int n, int threads, size_t smem, cudaStream_t stream, const Args& a) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)rows * n);
+  cfg.blockDim = threads;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = n;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = zs_pdl_enabled() ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  if (n > 8) cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaLaunchKernelEx(&cfg, kernel, a);
+  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+}
+
+bool aligned16(const void* p, long long stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 4 == 0; }
 
 }  // namespace spec
 }  // namespace zs
 
 extern "C" int zs_token_probs(const TokenProbsArgs* args, cudaStream_t stream) {
+  using namespace zs::spec;
   const TokenProbsArgs& a = *args;
   if (a.vocab < 1 || a.rows < 0 || a.ld < a.vocab || a.ld_out < a.vocab || a.temperature == nullptr) return -1;
   if (a.rows == 0) return 0;
-  zs_launch(zs::spec::probs_kernel, a.rows, zs::spec::T, 0, stream, a);
-  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+  int n = 1;
+  while (n < kCluster && (long long)n * kChunk < a.vocab) n *= 2;
+  if ((long long)n * kChunk < a.vocab || (long long)a.rows * n > 0x7FFFFFFF) {
+    zs_launch(probs_wide_kernel, a.rows, T, 0, stream, a);
+    return cudaGetLastError() == cudaSuccess ? 0 : -2;
+  }
+  const bool vec = aligned16(a.logits, a.rows > 1 ? a.ld : 0) && aligned16(a.out, a.rows > 1 ? a.ld_out : 0);
+  return launch_clusters(vec ? probs_kernel<4> : probs_kernel<1>, a.rows, n, PT, sizeof(ProbsSmem), stream, a);
 }
 
 extern "C" int zs_draft_verify(const DraftVerifyArgs* args, cudaStream_t stream) {
+  using namespace zs::spec;
   const DraftVerifyArgs& a = *args;
   if (a.n < 0 || a.k < 1 || a.k > ZS_VERIFY_MAX_DRAFTS || a.vocab < 1 || a.vocab > (1 << 24)) return -1;
   if (a.n == 0) return 0;
-  zs_launch(zs::spec::verify_kernel, a.n, zs::spec::T, 0, stream, a);
-  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+  // 16 CTAs of 512 threads bring a row of 2^18 tokens in one go; small vocabularies need fewer.
+  int n = 1;
+  while (n < kCluster && (long long)n * VT * 16 < a.vocab) n *= 2;
+  if ((long long)a.n * n > 0x7FFFFFFF) return -1;
+  const bool vec = a.vocab % 4 == 0 && aligned16(a.target, a.target_row) && a.target_seq % 4 == 0 &&
+                   (a.draft_probs == nullptr || (aligned16(a.draft_probs, a.draft_row) && a.draft_seq % 4 == 0));
+  return launch_clusters(vec ? verify_kernel<4> : verify_kernel<1>, a.n, n, VT, 0, stream, a);
 }

@@ -69,6 +69,30 @@ def test_probs_temperature_and_top_k(vocab):
 
 
 @gpu
+@pytest.mark.parametrize("vocab", [16384, 16385, 65537, 262144, 262145, 300001])
+def test_probs_sizes_around_the_clusters(vocab):
+    """Vocabularies that fill a CTA, a cluster, or neither; k on either side of the candidate lists."""
+    g = torch.Generator().manual_seed(vocab)
+    x = torch.randn(6, vocab, generator=g) * 4
+    check_probs(x, [1.0, 0.8, 0.0, 1.2, 1.0, 0.6], [0, 256, 0, 257, 3000, 40], [1.0, 1.0, 1.0, 1.0, 0.9, 0.7])
+
+
+@gpu
+def test_probs_candidates_in_one_place():
+    """The largest logits side by side (all in one CTA's part), equal in hundreds, or rarer than k."""
+    x = torch.full((6, 100000), -5.0)
+    x[0] = torch.arange(100000).float() / 3000       # ascending: the last CTA holds the top
+    x[1, 70000:70400] = 2.0                          # 400 tie for the first place
+    x[2, 40000:43000] = 1.0                          # 3000 do
+    x[3] = -math.inf
+    x[3, [5, 90000, 50000]] = torch.tensor([1.0, 2.0, 3.0])   # fewer than k tokens
+    x[4, ::2] = math.nan
+    x[5, 10:200] = torch.arange(190) / 10.0
+    got = check_probs(x, [1.0, 1.0, 1.0, 1.0, 1.0, 1.0], [200, 50, 50, 50, 50, 256], [1.0, 1.0, 0.5, 1.0, 1.0, 0.95])
+    assert int((got[1] > 0).sum()) == 400 and int((got[2] > 0).sum()) == 3000 and int((got[3] > 0).sum()) == 3
+
+
+@gpu
 def test_probs_ties_and_masks():
     x = torch.zeros(9, 777)
     x[0, 300:] = -math.inf
