@@ -362,10 +362,11 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
     tmem_relinquish();
   }
   if (tid == 0) {
-    for (int i = 0; i < 2 * STAGES; ++i) {
-      mbar_init(&s.full[0][0] + i, 1);
-      mbar_init(&s.empty[0][0] + i, 1);
-    }
+    for (int kv = 0; kv < 2; ++kv)
+      for (int i = 0; i < STAGES; ++i) {
+        mbar_init(&s.full[kv][i], 1);
+        mbar_init(&s.empty[kv][i], 1);
+      }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.s_full[i], 1);
       mbar_init(&s.p_full[i], COMPUTE);

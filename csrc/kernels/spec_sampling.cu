@@ -88,13 +88,13 @@ struct ProbsSmem {
   float x[kChunk];
   union {
     struct {
-      float list[kCluster][kList];
+      float list[kCluster * kList];      // kList of every CTA
       float cand[kCand], sorted[kCand];
     };
-    u64 hist[PW][256];                   // a histogram per warp; [0] is the CTA's
+    u64 hist[PW * 256];                  // a histogram per warp; the first becomes the CTA's
   };
   u64 total[256];
-  uint32_t warp_max[kCluster][PW];
+  uint32_t warp_max[kCluster * PW];
   float2 part[kCluster];                 // (maximum, sum) of every CTA
   uint32_t first[kCluster];              // greedy: lowest id of the maximum
   int count[kCluster];                   // candidates of every CTA
@@ -136,9 +136,9 @@ __global__ void __launch_bounds__(PT, 2) probs_kernel(const TokenProbsArgs a) {
     }
   }
   const float temp = a.temperature[row];
-  const int K = a.top_k != nullptr ? a.top_k[row] : 0;
-  const float P = a.top_p != nullptr ? a.top_p[row] : 1.f;
-  const bool greedy = !(temp > 0.f), by_k = !greedy && K > 0 && K < V, by_p = !greedy && P < 1.f;
+  const bool greedy = !(temp > 0.f);
+  const int K = a.top_k != nullptr && a.top_k[row] < V ? a.top_k[row] : 0;                // <= 0: all
+  const float P = a.top_p != nullptr && a.top_p[row] < 1.f ? fmaxf(a.top_p[row], 0.f) : 1.f;  // 1: all
   const float c = greedy ? 0.f : fminf(1.4426950408889634f / temp, kMax);  // exponents in the exp2 domain
   // f(place in the chunk, logit) for this thread's logits; the last group may pass len (masked there).
   auto each = [&](auto f) {
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(PT, 2) probs_kernel(const TokenProbsArgs a) {
   each([&](int, float x) { top = fmaxf(top, x); });
   cluster_wait_started();
 
-  if (!greedy && !by_k && !by_p) {
+  if (!greedy && K <= 0 && P == 1.f) {
     top = block_all<PW>(top, reinterpret_cast<float*>(s.red), [](float p, float q) { return fmaxf(p, q); }, -INFINITY);
     const float off = top == -INFINITY ? 0.f : top;
     float sum = 0.f;
@@ -193,12 +193,12 @@ __global__ void __launch_bounds__(PT, 2) probs_kernel(const TokenProbsArgs a) {
   // The row's maximum, and every warp's.
   {
     const uint32_t k = __reduce_max_sync(0xffffffff, okey(top));
-    if (lane < n) cluster.map_shared_rank(&s.warp_max[0][0], lane)[rank * PW + warp] = k;
+    if (lane < n) cluster.map_shared_rank(s.warp_max, lane)[rank * PW + warp] = k;
   }
   if (tid == 0) s.mine = 0;
   cluster.sync();
   uint32_t top_key = 0;
-  for (int i = lane; i < n * PW; i += 32) top_key = max(top_key, s.warp_max[0][i]);
+  for (int i = lane; i < n * PW; i += 32) top_key = max(top_key, s.warp_max[i]);
   top = from_okey(__reduce_max_sync(0xffffffff, top_key));
 
   if (greedy || top == -INFINITY) {  // all mass on the best token, none where every token is masked
@@ -218,12 +218,12 @@ __global__ void __launch_bounds__(PT, 2) probs_kernel(const TokenProbsArgs a) {
   auto mass = [&](float v) { return ex2((v - top) * c); };
   float thr = -INFINITY, inv = 0.f;  // keep x >= thr
   bool done = false;
-  if (by_k && K <= min(kSmallK, n * PW)) {
+  if (K > 0 && K <= min(kSmallK, n * PW)) {
     // K-th largest of the warp maxima (equal ones in any order).
     if (tid < n * PW) {
-      const uint32_t k = s.warp_max[0][tid];
+      const uint32_t k = s.warp_max[tid];
       int above = 0;
-      for (int i = 0; i < n * PW; ++i) above += s.warp_max[0][i] > k || (s.warp_max[0][i] == k && i < tid);
+      for (int i = 0; i < n * PW; ++i) above += s.warp_max[i] > k || (s.warp_max[i] == k && i < tid);
       if (above == K - 1) s.bound = from_okey(k);
     }
     __syncthreads();
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(PT, 2) probs_kernel(const TokenProbsArgs a) {
         if (x >= bound) {
           const int at = atomicAdd(&s.mine, 1);
           if (at < kList)
-            for (int r = 0; r < n; ++r) cluster.map_shared_rank(&s.list[0][0], r)[rank * kList + at] = x;
+            for (int r = 0; r < n; ++r) cluster.map_shared_rank(s.list, r)[rank * kList + at] = x;
         }
       });
     }
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(PT, 2) probs_kernel(const TokenProbsArgs a) {
       before -= cnt;
       for (int r = warp; r < n; r += PW) {
         const int at = __shfl_sync(0xffffffff, before, r), m = __shfl_sync(0xffffffff, cnt, r);
-        for (int i = lane; i < m; i += 32) s.cand[at + i] = s.list[r][i];
+        for (int i = lane; i < m; i += 32) s.cand[at + i] = s.list[r * kList + i];
       }
       __syncthreads();
       for (int i = tid; i < total; i += PT) {
@@ -276,8 +276,8 @@ __global__ void __launch_bounds__(PT, 2) probs_kernel(const TokenProbsArgs a) {
         }
         z = warp_sum(z);
         kept = (int)__reduce_add_sync(0xffffffff, (unsigned)kept);
-        if (by_p) {  // tokens in descending order while the mass before them is below P
-          const float goal = fmaxf(P, 0.f) * z;
+        if (P < 1.f) {  // tokens in descending order while the mass before them is below P
+          const float goal = P * z;
           float run = 0.f, keep_z = 0.f, last = s.sorted[0];
           for (int i0 = 0; i0 < kept; i0 += 32) {
             const float v = i0 + lane < kept ? s.sorted[i0 + lane] : -INFINITY, mv = v == -INFINITY ? 0.f : mass(v);
@@ -309,27 +309,27 @@ __global__ void __launch_bounds__(PT, 2) probs_kernel(const TokenProbsArgs a) {
     uint32_t key_thr = 0;
     for (int phase = 0; phase < 2; ++phase) {
       const bool by_mass = phase == 1;
-      if (by_mass ? !by_p : !by_k) continue;
+      if (by_mass ? P == 1.f : K <= 0) continue;
       u64 need = (u64)K;
       uint32_t prefix = 0;
       for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < PW * 256; i += PT) (&s.hist[0][0])[i] = 0;
+        for (int i = tid; i < PW * 256; i += PT) s.hist[i] = 0;
         __syncthreads();
         each([&](int, float x) {
           const uint32_t k = okey(x);
           const bool counts = x > -INFINITY && k >= key_thr && (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)));
-          if (counts) atomicAdd(&s.hist[warp][(k >> shift) & 255], by_mass ? (u64)(mass(x) * kFix) : 1ull);
+          if (counts) atomicAdd(&s.hist[warp * 256 + ((k >> shift) & 255)], by_mass ? (u64)(mass(x) * kFix) : 1ull);
         });
         __syncthreads();
         if (tid < 256) {
           u64 sum = 0;
-          for (int i = 0; i < PW; ++i) sum += s.hist[i][tid];
-          s.hist[0][tid] = sum;
+          for (int i = 0; i < PW; ++i) sum += s.hist[i * 256 + tid];
+          s.hist[tid] = sum;
         }
         cluster.sync();
         if (tid < 256) {
           u64 sum = 0;
-          for (int r = 0; r < n; ++r) sum += cluster.map_shared_rank(&s.hist[0][0], r)[tid];
+          for (int r = 0; r < n; ++r) sum += cluster.map_shared_rank(s.hist, r)[tid];
           s.total[tid] = sum;
         }
         cluster.sync();  // the others have read this CTA's
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(PT, 2) probs_kernel(const TokenProbsArgs a) {
             if (lane >= o) upto += y;
           }
           if (by_mass && shift == 24) {
-            need = (u64)((double)fmaxf(P, 0.f) * (double)__shfl_sync(0xffffffff, upto, 31));
+            need = (u64)((double)P * (double)__shfl_sync(0xffffffff, upto, 31));
             if (need == 0) need = 1;
           }
           const uint32_t enough = __ballot_sync(0xffffffff, upto >= need);
@@ -484,7 +484,7 @@ struct Weights {
 
 template <int VEC>
 __global__ void __launch_bounds__(VT) verify_kernel(const DraftVerifyArgs a) {
-  __shared__ u64 part[kCluster][VW];  // sums of every warp of the row's CTAs
+  __shared__ u64 part[kCluster * VW];  // sums of every warp of the row's CTAs
   cg::cluster_group cluster = cg::this_cluster();
   const int n = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), s = blockIdx.x / n;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.vocab;
@@ -536,10 +536,10 @@ __global__ void __launch_bounds__(VT) verify_kernel(const DraftVerifyArgs a) {
     sum = warp_all(sum, [](u64 p, u64 q) { return p + q; });
     if (round == 0) cluster_wait_started();
     else cluster.sync();  // the first round's sums are read
-    if (lane < n) cluster.map_shared_rank(&part[0][0], lane)[rank * VW + warp] = sum;
+    if (lane < n) cluster.map_shared_rank(part, lane)[rank * VW + warp] = sum;
     cluster.sync();
     total = 0;
-    for (int j = lane; j < n * VW; j += 32) total += (&part[0][0])[j];
+    for (int j = lane; j < n * VW; j += 32) total += part[j];
     total = warp_all(total, [](u64 p, u64 q) { return p + q; });
     if (total != 0 || !rejected) break;
     w.q = nullptr;  // p <= q everywhere: the target itself
@@ -558,9 +558,9 @@ __global__ void __launch_bounds__(VT) verify_kernel(const DraftVerifyArgs a) {
   }
   if (total == 0) return;
   u64 before = 0;
-  for (int j = lane; j < rank * VW + warp; j += 32) before += (&part[0][0])[j];
+  for (int j = lane; j < rank * VW + warp; j += 32) before += part[j];
   before = warp_all(before, [](u64 p, u64 q) { return p + q; });
-  if (goal < before || goal >= before + part[rank][warp]) return;
+  if (goal < before || goal >= before + part[rank * VW + warp]) return;
   for (int i = i0; i < i1; i += 32) {
     u64 x = i + lane < i1 ? w(i + lane) : 0;
 #pragma unroll
