@@ -716,10 +716,11 @@ extern "C" int zs_draft_verify(const DraftVerifyArgs* args, cudaStream_t stream)
   const DraftVerifyArgs& a = *args;
   if (a.n < 0 || a.k < 1 || a.k > ZS_VERIFY_MAX_DRAFTS || a.vocab < 1 || a.vocab > (1 << 24)) return -1;
   if (a.n == 0) return 0;
-  // 16 CTAs of 512 threads bring a row of 2^18 tokens in one go; small vocabularies need fewer, and many
-  // sequences too: four CTAs an SM run at once (128 sequences: 103 us with 16 CTAs each, 48 us with 4).
+  // CTAs of a sequence: a part of some 8000 tokens keeps one busy, and two fit on an SM; further waves
+  // only repeat the latencies (128 sequences of 248320 tokens: 70 us with 2 CTAs each, 74 with 4, 83
+  // with 8; 64 sequences: 43 us with 4, 61 with 8).
   int n = 1;
-  while (n < kCluster && (long long)n * VT * 16 < a.vocab && 2ll * n * a.n <= 148 * 4) n *= 2;
+  while (n < kCluster && (long long)n * VT * 16 < a.vocab && 2ll * n * a.n <= 148 * 2) n *= 2;
   if ((long long)a.n * n > 0x7FFFFFFF) return -1;
   const bool vec = a.vocab % 4 == 0 && aligned16(a.target, a.target_row) && a.target_seq % 4 == 0 &&
                    (a.draft_probs == nullptr || (aligned16(a.draft_probs, a.draft_row) && a.draft_seq % 4 == 0));
