@@ -1,0 +1,168 @@
+"""Many samples of shared prompts through the runner: attention of the shared-prefix path against
+the per-row path, right drafts accepted and wrong ones taken back, pages returned."""
+
+import pytest
+import torch
+
+from zstep_b200.config import Qwen35Config, qwen35_small_gpu
+from zstep_b200.ops import mx
+from zstep_b200.models.parallel_sampling import ParallelSampler, prompt_lookup
+
+
+def test_prompt_lookup():
+    assert prompt_lookup([1, 2, 3, 9, 1, 2, 3], 2) == [9, 1]
+    assert prompt_lookup([5, 6, 5], 3) == [6, 5]
+    assert prompt_lookup([1, 2, 3], 3) == []
+    assert prompt_lookup([7], 3) == []
+
+
+@pytest.fixture(scope="module")
+def runner():
+    from zstep_b200.models.qwen35 import Qwen35Runner
+    from zstep_b200.models.weights import RandomWeights
+
+    cfg = Qwen35Config(vocab_size=4096, num_hidden_layers=2, layer_types=("full_attention",) * 2, num_experts=16,
+                       mtp_num_hidden_layers=0, name="attention-only")
+    return Qwen35Runner(cfg, weights=RandomWeights(cfg, seed=4), max_seqs=16, max_prefill_tokens=256, num_pages=120,
+                        max_model_len=256)
+
+
+def _start(runner, lens=(70, 33), samples=5, k=3):
+    g = torch.Generator().manual_seed(9)
+    s = ParallelSampler(runner, k)
+    prompts = [torch.randint(0, 4096, (n,), generator=g).tolist() for n in lens]
+    return s, s.start(prompts, samples)
+
+
+def _first_attention(s, slots, drafts, shared):
+    """The first layer's attention output as its projection gets it (MXFP8), in 32 bits."""
+    r, calls = s.r, []
+    real = r._proj_out
+
+    def spy(w, xq, xsf, rows, *a, **kw):
+        if not calls:
+            calls.append(mx.dequantize(xq[:rows].clone(), mx.codes_from_atoms(xsf.clone(), rows, xq.shape[1])))
+        return real(w, xq, xsf, rows, *a, **kw)
+
+    r._proj_out = spy
+    try:
+        s.logits(slots, drafts, shared)
+    finally:
+        r._proj_out = real
+    return calls[0].double()
+
+
+def _same_attention(s, slots, drafts):
+    """Both paths get the same q, K and V in the first layer.  Each output is within 2^-8 (A + 2 |y|) of
+    the true one (bf16 weights and outputs; A <= max |v|, the gate is below 1), then within 2^-4 of itself
+    or half the smallest step of e4m3 under its block's scale (2^-10 * 2 amax / 448)."""
+    a, b = (_first_attention(s, slots, drafts, x) for x in (True, False))
+    vmax = float(s.r.v_cache[0].abs().max())
+    amax = b.abs().view(b.shape[0], -1, 32).amax(-1, keepdim=True).expand(-1, -1, 32).reshape(b.shape)
+    tol = 2 * (2.0 ** -8 * (vmax + 2 * b.abs()) + 2.0 ** -4 * b.abs() + 2.0 ** -10 * 2 * amax / 448)
+    assert b.abs().max() > 0 and ((a - b).abs() <= tol).all()
+    # and on the whole far nearer than that
+    assert float((a - b).norm() / b.norm()) < 2.0 ** -4
+
+
+@pytest.mark.gpu
+def test_attention_equals_the_unshared_path(runner):
+    s, slots = _start(runner)
+    g = torch.Generator().manual_seed(1)
+    for _ in range(3):
+        drafts = [torch.randint(0, 4096, (3,), generator=g).tolist() for _ in slots]
+        _same_attention(s, slots, drafts)
+        s.step(slots, 0.9, top_k=40, top_p=0.9, drafts=drafts)
+    assert runner.check_error() == 0
+    s.finish(slots)
+
+
+@pytest.mark.gpu
+def test_right_drafts_are_accepted_and_wrong_ones_taken_back(runner):
+    """Greedy: drafting what the model itself said is accepted whole; a wrong draft ends the row there."""
+    s, slots = _start(runner)
+    said = {x: [] for x in slots}
+    for _ in range(8):   # no drafts: one token a step
+        for x, t in zip(slots, s.step(slots, 0.0, drafts=[[] for _ in slots])):
+            assert len(t) == 1
+            said[x] += t
+    by_prompt = {}
+    for x in slots:      # samples of one prompt say the same
+        assert by_prompt.setdefault(s.prompt_of[x], said[x]) == said[x]
+    s.finish(slots)
+    s, slots = _start(runner)
+    new = s.step(slots, 0.0, drafts=[said[x][:3] for x in slots])
+    assert new == [said[x][:4] for x in slots]
+    wrong = [[said[x][4], (said[x][5] + 1) % 4096, said[x][6]] for x in slots]
+    new = s.step(slots, 0.0, drafts=wrong)
+    assert new == [said[x][4:6] for x in slots]
+    assert s.pool.seq_len[slots].tolist() == [len(s.tokens[x]) - 1 for x in slots]
+    s.finish(slots)
+
+
+@pytest.mark.gpu
+def test_ends_free_what_only_they_used(runner):
+    s, slots = _start(runner, samples=4)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    for _ in range(5):
+        s.step(slots, 1.1, generator=gen)
+    half = slots[::2]
+    left = [x for x in slots if x not in half]
+    done = s.finish(half)
+    assert all(len(t) >= 33 + 5 for t in done)
+    for _ in range(3):   # the others go on over moved pages
+        _same_attention(s, left, [[1, 2, 3] for _ in left])
+        s.step(left, 1.1, generator=gen)
+    s.finish(left)
+    live = s.pool.refcount > 0   # packed: what the prompts hold
+    assert bool(live[:int(live.sum())].all()) and int(live.sum()) == 1 + 5 + 2
+    s.pool.free(torch.tensor([0, 1], dtype=torch.int32, device="cuda"))
+    s.pool.check()
+    assert s.pool.refcount.tolist() == [1] + [0] * (s.pool.num_pages - 1)
+
+
+@pytest.mark.gpu
+def test_refusals(runner):
+    from zstep_b200.models.qwen35 import Qwen35Runner
+
+    hybrid = Qwen35Runner(qwen35_small_gpu(4, 1024, 8), max_seqs=2, max_prefill_tokens=16, num_pages=8, max_model_len=32)
+    with pytest.raises(ValueError, match="attention layers"):
+        ParallelSampler(hybrid)
+    with pytest.raises(ValueError, match="num_drafts"):
+        ParallelSampler(runner, 0)
+    with pytest.raises(ValueError, match="slots"):
+        _start(runner, samples=8)
+
+
+@pytest.mark.gpu
+def test_decode_graph_with_a_prefix_plan():
+    """A decode step captured with a plan replays while the sequences grow."""
+    from zstep_b200.models.qwen35 import Qwen35Runner
+    from zstep_b200.ops.shared_prefix import SharedPrefixPlan
+
+    cfg = qwen35_small_gpu(num_layers=4, vocab=4096, experts=16)
+    r = Qwen35Runner(cfg, max_seqs=4, max_prefill_tokens=160, num_pages=64, max_model_len=160)
+    prompt = torch.randint(0, 4096, (64,), generator=torch.Generator().manual_seed(2)).tolist()
+    for s in range(4):   # the prompt's four pages once, then own pages; every slot runs its own recurrent state
+        r.set_pages(s, [1, 2, 3, 4] + list(range(5 + 6 * s, 11 + 6 * s)))
+    for s in range(4):
+        r.stage(prompt, list(range(64)), [s] * 64, seq_start=[0, 64])
+        r.prefill_forward(64, 1)
+    k, v, conv, ssm = (t.clone() for t in (r.k_cache, r.v_cache, r.conv_state, r.ssm_state))
+    outs = []
+    for plan in (None, SharedPrefixPlan.from_prefixes(list(range(4)), [(list(range(4)), 4)], r.hq, r.hkv)):
+        for t, c in zip((r.k_cache, r.v_cache, r.conv_state, r.ssm_state), (k, v, conv, ssm)):
+            t.copy_(c)
+        r.prefix_plan = plan
+        r.graphs.clear()
+        hidden = []
+        for i in range(3):
+            r.stage([11 + s + 7 * i for s in range(4)], [64 + i] * 4, list(range(4)))
+            r.decode_step(4)
+            torch.cuda.synchronize()   # the next step's inputs go through the same pinned block
+            hidden.append(r.buf["hidden"][:4].float().clone())
+        outs.append(hidden)
+    assert r.check_error() == 0
+    plan.check()
+    for a, b in zip(*outs):
+        torch.testing.assert_close(a, b, rtol=5e-2, atol=5e-2)

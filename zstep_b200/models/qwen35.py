@@ -136,6 +136,9 @@ class Qwen35Runner:
         self._alloc_state()
         self._alloc_buffers()
         self.graphs: dict[int, torch.cuda.CUDAGraph] = {}
+        # Rows that share leading pages (ops.shared_prefix.SharedPrefixPlan over the rows of the
+        # coming steps): full attention then reads shared pages once.  None: every row reads its own.
+        self.prefix_plan = None
         self.spec = None
         if self.num_spec:
             from .qwen35_spec import SpecDecoder
@@ -467,6 +470,9 @@ class Qwen35Runner:
         cfg, C, b = self.cfg, self.C, self.buf
         H = cfg.hidden_size
         pos, slot, lens = b["in_pos"][:rows], b["in_slot"][:rows], b["in_len"][:rows]
+        plan = self.prefix_plan
+        if plan is not None:
+            plan.update(lens)
         C.embed_rmsnorm_quant(b["in_ids"][:rows], self.embed, b["hidden"], self.layers[0]["input_norm"], 1.0,
                               self.eps, rows, None, b["xq"], b["xsf"])
         for li, L in enumerate(self.layers):
@@ -495,16 +501,20 @@ class Qwen35Runner:
                                 self.eps, self.k_cache[ai], self.v_cache[ai], self.page_size, self.page_table, slot,
                                 pos, rows, b["q_out"], b["gate_out"])
                 midq = self._mid(self.hq * cfg.head_dim)
-                splits = self._attn_splits(rows, decode)
-                # Varlen steps pass their sequence boundaries: the tensor-core kernel then
-                # serves several query rows of a sequence from each K/V tile it loads.
-                grouped = not decode and num_seqs > 0
-                C.attn_decode(b["q_out"], b["gate_out"], self.hq, self.hkv, self.k_cache[ai], self.v_cache[ai],
-                              self.page_size, self.page_table, slot, lens, rows, b["partial"], splits,
-                              1.0 / math.sqrt(cfg.head_dim), None, midq, b["midsf"],
-                              impl=0 if decode else self.prefill_attn_impl,
-                              seq_start=b["seq_start"][:num_seqs + 1] if grouped else None,
-                              num_seqs=num_seqs if grouped else 0)
+                if plan is not None:
+                    plan.attend(b["q_out"][:rows], b["gate_out"][:rows], self.k_cache[ai], self.v_cache[ai],
+                                self.page_table, lens, 1.0 / math.sqrt(cfg.head_dim), out_q=midq, out_sf=b["midsf"])
+                else:
+                    splits = self._attn_splits(rows, decode)
+                    # Varlen steps pass their sequence boundaries: the tensor-core kernel then
+                    # serves several query rows of a sequence from each K/V tile it loads.
+                    grouped = not decode and num_seqs > 0
+                    C.attn_decode(b["q_out"], b["gate_out"], self.hq, self.hkv, self.k_cache[ai], self.v_cache[ai],
+                                  self.page_size, self.page_table, slot, lens, rows, b["partial"], splits,
+                                  1.0 / math.sqrt(cfg.head_dim), None, midq, b["midsf"],
+                                  impl=0 if decode else self.prefill_attn_impl,
+                                  seq_start=b["seq_start"][:num_seqs + 1] if grouped else None,
+                                  num_seqs=num_seqs if grouped else 0)
                 self._proj_out(L["o_proj"], midq, b["midsf"], rows, L["post_norm"])
             self._moe(L, rows)
             next_w = self.layers[li + 1]["input_norm"] if li + 1 < len(self.layers) else self.final_norm
