@@ -43,19 +43,8 @@ ZS_DEVICE float ex2(float x) {
   return y;
 }
 
-// floor(clamp(p, 0, 1) * 2^38).  A sum with 16 rounded towards zero holds 19 bits behind the point:
-// two of them, of p and of what the first left, cost a sixth of a conversion to 64 bits.
-ZS_DEVICE void fixed_parts(float p, uint32_t& high, uint32_t& low) {
-  p = fminf(fmaxf(p, 0.f), 1.f);
-  const float t = __fadd_rz(p, 16.f);
-  high = __float_as_uint(t) - 0x41800000u;
-  low = __float_as_uint(__fadd_rz((p - (t - 16.f)) * 524288.f, 16.f)) - 0x41800000u;
-}
-ZS_DEVICE u64 fixed(float p) {
-  uint32_t high, low;
-  fixed_parts(p, high, low);
-  return ((u64)high << 19) + low;
-}
+// floor(clamp(p, 0, 1) * 2^38).
+ZS_DEVICE u64 fixed(float p) { return (u64)(fminf(fmaxf(p, 0.f), 1.f) * 274877906944.f); }
 
 template <typename V, typename F>
 ZS_DEVICE V warp_all(V v, F op) {
@@ -357,10 +346,9 @@ __global__ void __launch_bounds__(PT, 2) probs_kernel(const TokenProbsArgs a) {
           if (!counts) return;
           const int bin = warp * 256 + ((k >> shift) & 255);
           if (by_mass) {
-            uint32_t high, low;
-            fixed_parts(mass(x), high, low);
-            atomicAdd(&s.low[bin], low);
-            atomicAdd(&s.high[bin], high);
+            const u64 v = fixed(mass(x));
+            atomicAdd(&s.low[bin], (uint32_t)v & 0x7FFFF);
+            atomicAdd(&s.high[bin], (uint32_t)(v >> 19));
           } else {
             atomicAdd(&s.low[bin], 1u);
           }
@@ -717,8 +705,8 @@ extern "C" int zs_draft_verify(const DraftVerifyArgs* args, cudaStream_t stream)
   if (a.n < 0 || a.k < 1 || a.k > ZS_VERIFY_MAX_DRAFTS || a.vocab < 1 || a.vocab > (1 << 24)) return -1;
   if (a.n == 0) return 0;
   // CTAs of a sequence: a part of some 8000 tokens keeps one busy, and two fit on an SM; further waves
-  // only repeat the latencies (128 sequences of 248320 tokens: 70 us with 2 CTAs each, 74 with 4, 83
-  // with 8; 64 sequences: 43 us with 4, 61 with 8).
+  // only repeat the latencies (128 sequences of 248320 tokens: 54 us with 2 CTAs each, 67 with 1, 59
+  // with 4; 64 sequences: 33 us with 4, 40 with 2, 37 with 8; 32 sequences: 19 us with 8, 22 with 4).
   int n = 1;
   while (n < kCluster && (long long)n * VT * 16 < a.vocab && 2ll * n * a.n <= 148 * 2) n *= 2;
   if ((long long)a.n * n > 0x7FFFFFFF) return -1;
