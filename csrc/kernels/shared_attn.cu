@@ -773,25 +773,12 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
         }
       }
       if (!more || g.first) {
-        // ---- the unit's records.  A warp with more than a few passes them through shared memory so that
-        // the stores are whole lines (128 slots: 4.4 us directly, 3.2 us so; 8 slots: 0.7 and 1.3 us).
+        // ---- the unit's records, through shared memory so that the stores are whole lines.
         wait_for(s, &s.o_full[(i - 1) & 1], ((i - 1) >> 1) & 1, a.err);
         tc_fence_after();
         const uint32_t has = __ballot_sync(0xffffffff, rec >= 0);
         float* to = a.partial + (size_t)max(rec, 0) * PREC;
-        if (has != 0 && __popc(has) <= 8) {
-#pragma unroll
-          for (int c = 0; c < 128; c += 32) {
-            uint32_t o[32];
-            tmem_ld_32x32b_x32(lanes + kTmemO + half * 128 + c, o);
-            tmem_ld_wait();
-            if (rec >= 0) {
-#pragma unroll
-              for (int j = 0; j < 32; j += 4)
-                *reinterpret_cast<uint4*>(to + half * 128 + c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-            }
-          }
-        } else if (has != 0) {
+        if (has != 0) {
 #pragma unroll
           for (int c = 0; c < 128; c += 32) {
             uint32_t o[32];
@@ -838,12 +825,6 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
 }
 
 constexpr int MERGE_WARPS = 8;
-// (row, q head) pairs up to which a whole CTA merges one of them, its warps sharing the records:
-// with few rows a long prefix leaves a record in every CTA.  Above, a warp each: 16 x 64 pairs of
-// two or three records take 4.6 us with a CTA each and 3.3 us with a warp each, 64 pairs of 33
-// records 4.3 and 8.9 us.
-constexpr int MERGE_WIDE = 512;
-
 // A lane owns dims 4 lane .. + 3 and 128 + 4 lane .. + 3.  Records are found and weighed 32 at a
 // time (one a lane), then added in order; with PARTS warps on a pair, warp p takes every PARTS-th
 // record and the parts are joined in order.
@@ -853,8 +834,7 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const SharedAtt
   pdl_trigger();
   const Work w = work_of(a);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % PARTS;
-  const int item = blockIdx.x * (MERGE_WARPS / PARTS) + warp / PARTS;
-  if (item >= a.rows * a.num_q_heads) return;  // PARTS == 1 alone
+  const int at_item = blockIdx.x * (MERGE_WARPS / PARTS) + warp / PARTS, item = min(at_item, a.rows * a.num_q_heads - 1);
   const int row = item / a.num_q_heads, h = item % a.num_q_heads, group = group_of(a);
   float m = -INFINITY, l = 0.f, o[8] = {};
   // A lane per segment of the row: where its records are.  first[j] = records before segment j.
@@ -914,7 +894,8 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const SharedAtt
     }
   }
   if (PARTS > 1) {
-    __shared__ float parts[PARTS][D + 2];
+    __shared__ float all[MERGE_WARPS][D + 2];
+    float(*parts)[D + 2] = all + warp / PARTS * PARTS;
 #pragma unroll
     for (int k = 0; k < 8; ++k) parts[part][(k >> 2) * 128 + lane * 4 + (k & 3)] = o[k];
     if (lane == 0) {
@@ -937,6 +918,7 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const SharedAtt
       for (int k = 0; k < 8; ++k) o[k] += wx * parts[x][(k >> 2) * 128 + lane * 4 + (k & 3)];
     }
   }
+  if (at_item != item) return;
   const float inv = m == -INFINITY ? 0.f : 1.f / l;
   const size_t at = (size_t)item * D;
 #pragma unroll
@@ -999,7 +981,13 @@ extern "C" int zs_shared_attn(const SharedAttnArgs* args, cudaStream_t stream) {
   cudaFuncSetAttribute(tiles_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
   zs_launch(tiles_kernel, CTAS, THREADS, SMEM, stream, a);
   const int items = a.rows * a.num_q_heads;
-  if (items <= MERGE_WIDE) zs_launch(merge_kernel<MERGE_WARPS>, items, MERGE_WARPS * 32, 0, stream, a);
-  else zs_launch(merge_kernel<1>, (items + MERGE_WARPS - 1) / MERGE_WARPS, MERGE_WARPS * 32, 0, stream, a);
+  // Warps that share the records of a (row, q head) pair: with few pairs a long prefix leaves a record
+  // in every CTA, with many there are a few each and the device is full without.  The whole call in us
+  // with 1, 2, 4 and 8: 64 pairs 27.1, 21.5, 19.9, 19.2; 768 pairs 70.6, 61.0, 58.1, 62.1; 2048 pairs
+  // 43.2, 42.4, 46.7, 53.7; 8192 pairs 62.2, 70.5, 81.7, 105.5.
+  int parts = MERGE_WARPS;
+  while (parts > 1 && (long long)items * parts > 4096) parts /= 2;
+  const auto merge = parts == 8 ? merge_kernel<8> : parts == 4 ? merge_kernel<4> : parts == 2 ? merge_kernel<2> : merge_kernel<1>;
+  zs_launch(merge, (int)(((long long)items * parts + MERGE_WARPS - 1) / MERGE_WARPS), MERGE_WARPS * 32, 0, stream, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
