@@ -128,6 +128,33 @@ def test_probs_top_p_keeps_ties():
 
 
 @gpu
+@pytest.mark.parametrize("vocab", [90, 248320, 262150])
+def test_probs_infinite_temperature_leaves_the_unmasked_alike(vocab):
+    x = torch.randn(2, vocab, generator=torch.Generator().manual_seed(2))
+    x[:, ::3] = -math.inf
+    x[:, 1::7] = math.nan
+    kept = x > -math.inf
+    for k, p in ((0, 1.0), (0, 0.999999)):
+        got = token_probs(x.cuda(), torch.tensor([math.inf, math.inf], device="cuda"),
+                          top_k=torch.tensor([k, k], dtype=torch.int32, device="cuda"),
+                          top_p=torch.tensor([p, p], device="cuda")).cpu()
+        assert not got[~kept].any()
+        if p == 1.0:
+            # a sum of n ones is within n 2^-24 of it, the quotient within 2^-23
+            torch.testing.assert_close(got[kept].double(), (1.0 / kept.sum(1, keepdim=True).double()).expand(-1, vocab)[kept],
+                                       rtol=vocab * 2.0 ** -24 + 2.0 ** -22, atol=0)
+
+
+@gpu
+@pytest.mark.parametrize("vocab", [16384, 248320, 262144])
+def test_probs_one_value_everywhere_fills_one_bin(vocab):
+    x = torch.full((2, vocab), 1.5)
+    got = token_probs(x.cuda(), torch.tensor([1.0, 0.5], device="cuda"), top_k=torch.tensor([0, 400], dtype=torch.int32, device="cuda"),
+                      top_p=torch.tensor([0.5, 0.9], device="cuda")).cpu().double()
+    torch.testing.assert_close(got, torch.full_like(got, 1.0 / vocab), rtol=vocab * 2.0 ** -24 + 2.0 ** -22, atol=0)
+
+
+@gpu
 def test_probs_strided_rows_and_repeats():
     g = torch.Generator(device="cuda").manual_seed(3)
     x = torch.randn(5, 1003, generator=g, device="cuda")[:, 1:999]   # rows that start off 16-byte boundaries
