@@ -70,10 +70,6 @@ ZS_DEVICE int last_at(const int* x, int n, int v) {
   return lo;
 }
 
-// What a piece costs besides its tiles, in tiles: another Q; for a unit's first one also a pipeline
-// that starts anew and the records.  x: the first half of the piece's static description.
-ZS_DEVICE int piece_over(const int4& x, int i, int group) { return x.w == i ? 2 + x.z * group / 64 : 1; }
-
 // One CTA: the longest row of every segment decides how many pages it has; costs are counted and
 // the CTAs' ranges laid over them.
 __global__ void __launch_bounds__(1024) plan_kernel(const SharedAttnArgs a) {
@@ -81,6 +77,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const SharedAttnArgs a) {
   __shared__ unsigned long long longest[MAX_SEGS];  // (length, ~entry)
   __shared__ int table[MAX_SEGS];
   __shared__ int cost0[MAX_PIECES + 1], start[CTAS + 1];
+  __shared__ uint8_t over[MAX_PIECES];
   __shared__ long long red[32];
   const Work w = work_of(a);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -88,7 +85,8 @@ __global__ void __launch_bounds__(1024) plan_kernel(const SharedAttnArgs a) {
   // The plan's own tensors do not change: what a thread needs of them first is read before the wait.
   const bool e_in = tid < a.entries, p_in = tid < a.num_pieces;
   const int row = e_in ? a.seg_rows[tid] : 0, seg = e_in ? a.entry_seg[tid] : 0, slot = e_in ? a.row_slot[row] : 0;
-  const int at_piece = e_in ? a.entry_piece[tid] : 0;
+  // (entry, kv head) pair `tid`
+  const int of = tid / a.num_kv_heads, of_piece = of < a.entries ? a.entry_piece[of] : 0, of_unit = of < a.entries ? a.pieces[8 * of_piece + 1] : 0;
   const int4 px = p_in ? reinterpret_cast<const int4*>(a.pieces)[2 * tid] : make_int4(0, 0, 0, 0);
   const int4 py = p_in ? reinterpret_cast<const int4*>(a.pieces)[2 * tid + 1] : make_int4(0, 0, 0, 0);
   __syncthreads();
@@ -118,7 +116,9 @@ __global__ void __launch_bounds__(1024) plan_kernel(const SharedAttnArgs a) {
       const int len = (int)(longest[x.x] >> 32);
       g.e0 = x.y;
       g.rows = x.z;
-      g.over = piece_over(x, i, group);
+      // What a piece costs besides its tiles, in tiles of 1.1 us: another Q, 0.9 us; for a unit's first
+      // one also a pipeline that starts anew and the last unit's records, 3.4 us with 128 slots.
+      g.over = x.w == i ? 3 + x.z * group / 128 : 1;
       g.r0 = y.y >> 16;
       g.r1 = y.y & 0xFFFF;
       g.p0 = y.z;
@@ -147,6 +147,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const SharedAttnArgs a) {
     if (i < a.num_pieces) {
       g.cost0 = (int)(carry + before + x - cost);
       cost0[i] = g.cost0;
+      over[i] = (uint8_t)g.over;
       w.piece[i] = g;
     }
     carry += sum;
@@ -160,29 +161,23 @@ __global__ void __launch_bounds__(1024) plan_kernel(const SharedAttnArgs a) {
     w.head[0] = each;
   }
   __syncthreads();
-  const int4* pieces = reinterpret_cast<const int4*>(a.pieces);
-  // Equal shares; a border near an end of a unit moves there (a CTA that only ends or only starts a
-  // unit with a tile or two pays for another Q and other records).
-  for (int c = tid; c <= CTAS; c += 1024) {
-    int at = c < n ? (int)((long long)total * c / n) : total;
-    if (at > 0 && at < total) {
-      const int rel = at % each, i = last_at(cost0, a.num_pieces, rel), u0 = pieces[2 * i].w, u1 = pieces[2 * i + 1].x;
-      const int near = min(3, total / n / 4), over = 2 + pieces[2 * i].z * group / 64;
-      if (rel < cost0[u0] + over + near) at += cost0[u0] - rel;
-      else if (rel + near >= cost0[u1]) at += cost0[u1] - rel;
-    }
-    start[c] = at;
+  // Equal shares; a border within what a unit's start costs moves to the start, which then costs
+  // nobody anything.
+  int at = total, in = 0;
+  if (tid < n) {
+    at = total / n * tid + total % n * tid / n;
+    const int rel = at % each;
+    in = last_at(cost0, a.num_pieces, rel);
+    if (over[in] > 1 && rel < cost0[in] + over[in]) at += cost0[in] - rel;
   }
+  if (tid <= CTAS) start[tid] = at;
   __syncthreads();
-  for (int c = tid; c < CTAS; c += 1024)
-    w.cta[c] = make_int4(start[c], start[c + 1], each > 0 ? last_at(cost0, a.num_pieces, start[c] % each) : 0, 0);
+  if (tid < CTAS) w.cta[tid] = make_int4(at, start[tid + 1], in, 0);
   for (int x = tid; x < a.entries * a.num_kv_heads; x += 1024) {
-    const int e = x / a.num_kv_heads, i = e == tid ? at_piece : a.entry_piece[e];
-    const int4 p = pieces[2 * i];
-    const int over = piece_over(p, i, group), first = (x % a.num_kv_heads) * each + cost0[i] + over;
-    const int nt = fits ? max(0, cost0[i + 1] - cost0[i] - over) : 0;
+    const int e = x == tid ? of : x / a.num_kv_heads, i = x == tid ? of_piece : a.entry_piece[e];
+    const int first = (x - e * a.num_kv_heads) * each + cost0[i] + over[i], nt = fits ? max(0, cost0[i + 1] - cost0[i] - over[i]) : 0;
     const int c0 = nt > 0 ? last_at(start, CTAS, first) : 0, c1 = nt > 0 ? last_at(start, CTAS, first + nt - 1) : -1;
-    w.entry[x] = make_int4(c0, c1 - c0 + 1, (e - p.y) * group, 0);
+    w.entry[x] = make_int4(c0, c1 - c0 + 1, (e - (x == tid ? of_unit : a.pieces[8 * i + 1])) * group, 0);
   }
 }
 
@@ -349,6 +344,11 @@ constexpr float kGrow = 8.f;         // O is rescaled when a maximum grows by mo
 // average out, and where a weight is more than a quarter of its half's sum before its tile
 // (first tiles, few keys, peaked rows) a second product adds what the rounding lost.  l sums the
 // weights before they are rounded.
+// Long pieces run at 1.0 to 1.1 us a tile and CTA, 9 TB/s over the device with the cache in L2; the two
+// products take 0.53 us of it (1024 clocks at 4096 multiply-adds a clock).  S and P in places of their own, so
+// that the next S need not wait for O, gave 1.15 us: the copies set the pace.  What short calls pay
+// for is the way to the first tile (5 us from the plan's end: range, piece, rows, Q) and a unit's
+// records (3.6 us for 128 slots, as fast as L2 takes them from all SMs at once).
 __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs a) {
   extern __shared__ __align__(1024) uint8_t raw[];
   Smem& s = *reinterpret_cast<Smem*>(raw);
@@ -389,8 +389,10 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s.tmem;
-  pdl_wait();
-  pdl_trigger();
+  if (warp >= COMPUTE / 32) {  // the softmax warps have something to do first
+    pdl_wait();
+    pdl_trigger();
+  }
   const int cta = blockIdx.x, group = group_of(a);
   // Fragment k of the CTA, once the lookup warp has it; false when there is none (or a wait gave up).
   int fk = 0;
@@ -545,10 +547,11 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
       if (f.first && parts >= 1) ok = ok && wait_for(s, &s.way_empty[(parts - 1) & 1], ((parts - 1) >> 1) & 1, a.err);
       ok = __all_sync(0xffffffff, ok);
       if (!ok) break;
-      // The queries of the piece's slots, then the lengths of its rows.
+      // The queries of the piece's slots (the softmax warps fetch the first piece's themselves), then
+      // the lengths of its rows.
       // (Not bulk copies: those would wait behind the tiles that the copy warps asked for.)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 4 && parts > 0; ++j) {
         const int index = row[j] * a.num_q_heads + f.kvh * group + head[j];
         const int lo = max(f.s0, j * 32), hi = min(f.s1, j * 32 + 32);
 #pragma unroll 8
@@ -586,6 +589,18 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
     const float qscale = a.sm_scale * 1.4426950408889634f;             // exp2 domain
     const int head = slot % group;
     auto way = [&](int r, int p) { return s.way[r] + ((half * 16 + p) << 4); };  // 16-byte piece p of the warp's half
+    // The first piece's Q: every warp fetches what it will store, two slots' halves at a time, in a
+    // quarter of the time that one warp takes for 128 slots while tiles arrive (4.1 us).
+    auto fetch_q = [&](const Fragment& g) {
+      const int index = (slot >= g.s0 && slot < g.s1 ? a.seg_rows[g.e0 + slot / group] : 0) * a.num_q_heads + g.kvh * group + head;
+#pragma unroll
+      for (int x = 0; x < 32; x += 2) {
+        const int at = x + (lane >> 4), from = __shfl_sync(0xffffffff, index, at), to = (warp & 3) * 32 + at, c = half * 256 + (lane & 15) * 16;
+        if (to >= g.s0 && to < g.s1) cp_async16(s.way[to] + c, static_cast<const char*>(a.q) + (size_t)from * (D * 2) + c);
+      }
+      cp_async_wait();
+      __syncwarp();
+    };
     auto store_q = [&](const Fragment& g, int k) {  // Q of piece k from the way to TMEM
       wait_for(s, &s.way_full[k & 1], (k >> 1) & 1, a.err);
       if ((warp & 3) * 32 < g.s1 && (warp & 3) * 32 + 32 > g.s0) {
@@ -604,20 +619,25 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
     };
     // After a wait that gave up these warps go on to the end of the fragment with whatever is there (the
     // error word is set, every later wait gives up at once) and leave together: their barriers always meet.
-    bool more = !compute_any(!next_fragment(f));
+    // Before the plan is there, one tile is computed from whatever TMEM holds and nothing is kept of
+    // it: the first real tile then finds its instructions in the cache (without: 3.4 us from its S to its P, with: 1.3 us).
+    int dry;
+    asm volatile("mov.u32 %0, 1;" : "=r"(dry));
+    f = Fragment{0, 0, SLOTS, 0, SLOTS, 0, 1, 0, TPAGES, TILE, 0, 1};
+    bool more = true;
     int kf = 0;  // place of the piece
     uint32_t kph = 0;
-    if (more) store_q(f, 0);
     int i = 0, parts = 1;
     float m = -INFINITY, l = 0.f;  // reference maximum (raw scores) of the slot, sum of this half's weights
     int rec = -1;                  // record of the slot, once it had a tile
     while (more) {
-      wait_for(s, &s.r_full[kf], kph, a.err);
-      const int limit = s.limit[kf][slot], least = s.least[kf];
+      if (!dry) wait_for(s, &s.r_full[kf], kph, a.err);
+      const int limit = dry ? TILE : s.limit[kf][slot], least = dry ? TILE : s.least[kf];
       const bool used = slot >= f.s0 && slot < f.s1, busy = (warp & 3) * 32 < f.s1 && (warp & 3) * 32 + 32 > f.s0;
       if (used) {
         // The CTA with a piece's first tile keeps the record by (entry, head), the others by CTA and slot.
-        rec = f.t0 == 0 ? (f.e0 + slot / group) * a.num_q_heads + f.kvh * group + head
+        rec = dry       ? -1
+              : f.t0 == 0 ? (f.e0 + slot / group) * a.num_q_heads + f.kvh * group + head
                         : a.entries * a.num_q_heads + cta * SLOTS + slot;
         m = -INFINITY;
         l = 0.f;
@@ -625,9 +645,9 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
       Fragment g = {};
       for (int t = f.t0; t < f.t1; ++t, ++i) {
         const int b = i & 1, key0 = (f.p0 + t * TPAGES) * PAGE;
-        wait_for(s, &s.s_full[b], (i >> 1) & 1, a.err);
+        if (!dry) wait_for(s, &s.s_full[b], (i >> 1) & 1, a.err);
         tc_fence_after();
-        if (t + 1 == f.t1) {
+        if (t + 1 == f.t1 && !dry) {
           more = !compute_any(!next_fragment(g));
           if (more) store_q(g, parts++);  // every product with this Q is done: the next takes its place
         }
@@ -649,7 +669,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
           s.top[b][half][slot] = mt;
         }
         // A weight above a quarter of the sum so far: its bf16 rounding (2^-8) would show.
-        const bool sharp = used && mt > -INFINITY && (m == -INFINITY || ex2((mt - m) * qscale) * 4.f > l);
+        const bool sharp = dry || (used && mt > -INFINITY && (m == -INFINITY || ex2((mt - m) * qscale) * 4.f > l));
         {
           const int any = __any_sync(0xffffffff, sharp);
           if (lane == 0) s.vote[b][warp] = any;
@@ -736,7 +756,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
           fence_proxy_async_shared();
         }
         tc_fence_before();
-        mbar_arrive(&s.p_full[b]);
+        if (!dry) mbar_arrive(&s.p_full[b]);
         if (odd != 0) {
           wait_for(s, &s.o_full[b], (i >> 1) & 1, a.err);
           tc_fence_after();
@@ -772,13 +792,13 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
           tc_fence_before();
         }
       }
-      if (!more || g.first) {
+      if (!more || g.first || dry) {
         // ---- the unit's records, through shared memory so that the stores are whole lines.
-        wait_for(s, &s.o_full[(i - 1) & 1], ((i - 1) >> 1) & 1, a.err);
+        if (!dry) wait_for(s, &s.o_full[(i - 1) & 1], ((i - 1) >> 1) & 1, a.err);
         tc_fence_after();
         const uint32_t has = __ballot_sync(0xffffffff, rec >= 0);
         float* to = a.partial + (size_t)max(rec, 0) * PREC;
-        if (has != 0) {
+        if (has != 0 || dry) {
 #pragma unroll
           for (int c = 0; c < 128; c += 32) {
             uint32_t o[32];
@@ -810,6 +830,17 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
         tc_fence_before();
       }
       __syncwarp();
+      if (dry) {
+        pdl_wait();
+        pdl_trigger();
+        dry = i = 0;
+        more = !compute_any(!next_fragment(f));
+        if (more) {
+          fetch_q(f);
+          store_q(f, 0);
+        }
+        continue;
+      }
       if (lane == 0) mbar_arrive(&s.f_empty[kf]);
       if (++kf == AHEAD) {
         kf = 0;
@@ -824,26 +855,27 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
   if (warp == 9) tmem_dealloc(tmem, kTmemCols);
 }
 
-constexpr int MERGE_WARPS = 8;
-// A lane owns dims 4 lane .. + 3 and 128 + 4 lane .. + 3.  Records are found and weighed 32 at a
-// time (one a lane), then added in order; with PARTS warps on a pair, warp p takes every PARTS-th
-// record and the parts are joined in order.
+constexpr int MERGE_WARPS = 8, AT_ONCE = 2;
+// The join of a (row, q head) pair's records, read once from L2 (4.2 us for 2048 pairs' 20 MB after
+// the tiles' end; latencies bound it).  A lane owns dims 4 lane .. + 3 and 128 + 4 lane .. + 3.  Records
+// are found and weighed 32 at a time (one a lane), then added in order, AT_ONCE on their way together;
+// with PARTS warps on a pair, warp p takes every PARTS-th record and the parts are joined in order.
+// 64 registers, so that four CTAs share an SM, are worth more than more loads in flight (2048 pairs:
+// 40.5 us the whole call with 2, 40.9 with 3; with 4 and 80 registers 45.4).
 template <int PARTS>
-__global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const SharedAttnArgs a) {
-  pdl_wait();
-  pdl_trigger();
+__global__ void __launch_bounds__(MERGE_WARPS * 32, 4) merge_kernel(const SharedAttnArgs a) {
   const Work w = work_of(a);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % PARTS;
   const int at_item = blockIdx.x * (MERGE_WARPS / PARTS) + warp / PARTS, item = min(at_item, a.rows * a.num_q_heads - 1);
   const int row = item / a.num_q_heads, h = item % a.num_q_heads, group = group_of(a);
   float m = -INFINITY, l = 0.f, o[8] = {};
-  // A lane per segment of the row: where its records are.  first[j] = records before segment j.
-  const int own = a.row_entry[row * a.levels + min(lane, a.levels - 1)];
+  uint2 gate[2] = {};
   for (int j0 = 0; j0 < a.levels; j0 += 32) {
-    const int e = j0 == 0 ? (lane < a.levels ? own : -1) : (j0 + lane < a.levels ? a.row_entry[row * a.levels + j0 + lane] : -1);
+    // A lane per segment of the row: where its records are.  before = records of the segments before.
+    const int e = j0 + lane < a.levels ? __ldg(a.row_entry + row * a.levels + j0 + lane) : -1;
     int c0 = 0, cnt = 0, slot = 0;
     if (e >= 0) {
-      const int4 u = w.entry[(size_t)e * a.num_kv_heads + h / group];
+      const int4 u = __ldcg(w.entry + (size_t)e * a.num_kv_heads + h / group);
       c0 = u.x;
       cnt = u.y;
       slot = u.z + h % group;
@@ -856,9 +888,9 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const SharedAtt
     }
     const int records = __shfl_sync(0xffffffff, before, 31);
     before -= cnt;
-    for (int r0 = part; r0 < records; r0 += 32 * PARTS) {
-      const int r = r0 + lane * PARTS;  // this lane's record
-      int j = 0;                        // its segment: the last with before <= r and records
+    // Where record r is, counted over this group of segments.
+    auto place = [&](int r) {
+      int j = 0;  // its segment: the last with before <= r and records
       for (int x = 1; x < 32; ++x) {
         const int bx = __shfl_sync(0xffffffff, before, x), cx = __shfl_sync(0xffffffff, cnt, x);
         if (cx > 0 && bx <= r) j = x;
@@ -866,30 +898,56 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const SharedAtt
       }
       const int c = __shfl_sync(0xffffffff, c0, j) + r - __shfl_sync(0xffffffff, before, j);
       const int sl = __shfl_sync(0xffffffff, slot, j), ej = __shfl_sync(0xffffffff, e, j);
-      const size_t at = r == __shfl_sync(0xffffffff, before, j) ? (size_t)ej * a.num_q_heads + h
-                                                               : (size_t)a.entries * a.num_q_heads + (size_t)c * SLOTS + sl;
-      const float4 ml = r < records ? *reinterpret_cast<const float4*>(a.partial + at * PREC + D) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+      return r == __shfl_sync(0xffffffff, before, j) ? ej * a.num_q_heads + h
+                                                    : a.entries * a.num_q_heads + c * SLOTS + sl;
+    };
+    int at = place(part + lane * PARTS);  // this lane's record
+    if (j0 == 0) {
+      // What came so far is from kernels that had ended when the tiles began (their CTAs let this
+      // kernel start after their own wait); the records are not.
+      if (a.gate != nullptr) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          gate[k] = __ldcg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(a.gate) + (size_t)item * D + k * 128 + lane * 4));
+      }
+      pdl_wait();
+      pdl_trigger();
+    }
+    for (int r0 = part; r0 < records; r0 += 32 * PARTS) {
+      const int r = r0 + lane * PARTS;
+      if (r0 > part) at = place(r);
+      const float4 ml = r < records ? *reinterpret_cast<const float4*>(a.partial + (size_t)at * PREC + D) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+      const int here = min(32, (records - r0 + PARTS - 1) / PARTS);
+      float4 p[AT_ONCE], q[AT_ONCE];  // the first records, on their way together with the weights
+      auto load = [&](int x0) {
+#pragma unroll
+        for (int x = 0; x < AT_ONCE; ++x) {
+          const float4* from = reinterpret_cast<const float4*>(a.partial + (size_t)__shfl_sync(0xffffffff, at, x0 + x) * PREC);
+          if (x0 + x < here) p[x] = from[lane], q[x] = from[32 + lane];
+        }
+      };
+      load(0);
       const float mn = fmaxf(m, warp_max(ml.x)), s0 = m == -INFINITY ? 0.f : exp2f(m - mn);
       const float wt = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mn);
       l = l * s0 + warp_sum(ml.x == -INFINITY ? 0.f : wt * (ml.y + ml.z));
 #pragma unroll
       for (int k = 0; k < 8; ++k) o[k] *= s0;
       m = mn;
-      const int cnt_here = min(32, (records - r0 + PARTS - 1) / PARTS);
-#pragma unroll 4
-      for (int x = 0; x < cnt_here; ++x) {
-        const float wx = __shfl_sync(0xffffffff, wt, x);
-        const float4* from = reinterpret_cast<const float4*>(a.partial + __shfl_sync(0xffffffff, at, x) * PREC);
-        const float4 p = from[lane], q = from[32 + lane];
-        if (wx == 0.f) continue;
-        o[0] += wx * p.x;
-        o[1] += wx * p.y;
-        o[2] += wx * p.z;
-        o[3] += wx * p.w;
-        o[4] += wx * q.x;
-        o[5] += wx * q.y;
-        o[6] += wx * q.z;
-        o[7] += wx * q.w;
+      for (int x0 = 0; x0 < here; x0 += AT_ONCE) {
+        if (x0 > 0) load(x0);
+#pragma unroll
+        for (int x = 0; x < AT_ONCE; ++x) {
+          const float wx = __shfl_sync(0xffffffff, wt, x0 + x);
+          if (x0 + x >= here || wx == 0.f) continue;
+          o[0] += wx * p[x].x;
+          o[1] += wx * p[x].y;
+          o[2] += wx * p[x].z;
+          o[3] += wx * p[x].w;
+          o[4] += wx * q[x].x;
+          o[5] += wx * q[x].y;
+          o[6] += wx * q[x].z;
+          o[7] += wx * q[x].w;
+        }
       }
     }
   }
@@ -920,21 +978,19 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const SharedAtt
   }
   if (at_item != item) return;
   const float inv = m == -INFINITY ? 0.f : 1.f / l;
-  const size_t at = (size_t)item * D;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int d = k * 128 + lane * 4;
     float* y = o + 4 * k;
     float g[4] = {1.f, 1.f, 1.f, 1.f};
     if (a.gate != nullptr) {
-      const uint2 gv = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(a.gate) + at + d);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) g[j] = sigmoidf_(__bfloat162float(reinterpret_cast<const __nv_bfloat16*>(&gv)[j]));
+      for (int j = 0; j < 4; ++j) g[j] = sigmoidf_(__bfloat162float(reinterpret_cast<const __nv_bfloat16*>(&gate[k])[j]));
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) y[j] = m == -INFINITY ? 0.f : y[j] * inv * g[j];
     if (a.out_bf16 != nullptr)
-      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out_bf16) + at + d) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out_bf16) + (size_t)item * D + d) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
     if (a.out_q != nullptr) {  // a block of 32 dims is 8 lanes
       float amax = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
 #pragma unroll
@@ -944,7 +1000,7 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) merge_kernel(const SharedAtt
       uint32_t four = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) four |= (uint32_t)f32_to_e4m3(y[j] * si) << (8 * j);
-      *reinterpret_cast<uint32_t*>(a.out_q + at + d) = four;
+      *reinterpret_cast<uint32_t*>(a.out_q + (size_t)item * D + d) = four;
       if ((lane & 7) == 0) {
         const int kb = h * (D / 32) + (d >> 5);
         a.out_sf[((size_t)(row >> 7) * (a.num_q_heads * D >> 7) + (kb >> 2)) * 512 + sf_atom_offset(row & 127, kb & 3)] = code;
@@ -983,8 +1039,8 @@ extern "C" int zs_shared_attn(const SharedAttnArgs* args, cudaStream_t stream) {
   const int items = a.rows * a.num_q_heads;
   // Warps that share the records of a (row, q head) pair: with few pairs a long prefix leaves a record
   // in every CTA, with many there are a few each and the device is full without.  The whole call in us
-  // with 1, 2, 4 and 8: 64 pairs 27.1, 21.5, 19.9, 19.2; 768 pairs 70.6, 61.0, 58.1, 62.1; 2048 pairs
-  // 43.2, 42.4, 46.7, 53.7; 8192 pairs 62.2, 70.5, 81.7, 105.5.
+  // with 1, 2, 4 and 8: 64 pairs 21.7, 18.8, 17.0, 16.2; 768 pairs 61.6, 55.6, 52.4, 56.7; 2048 pairs
+  // 39.6, 39.7, 43.6, 49.4; 8192 pairs 57.1, 65.3, 75.3, 96.5.
   int parts = MERGE_WARPS;
   while (parts > 1 && (long long)items * parts > 4096) parts /= 2;
   const auto merge = parts == 8 ? merge_kernel<8> : parts == 4 ? merge_kernel<4> : parts == 2 ? merge_kernel<2> : merge_kernel<1>;
