@@ -48,30 +48,27 @@ __host__ __device__ inline Scratch scratch_of(const PagePoolArgs& a) {
 
 ZS_DEVICE int pages_for(const PagePoolArgs& a, int tokens) { return (tokens + a.page_size - 1) / a.page_size; }
 
-// Exclusive prefix sum over the block (T threads); *total gets the sum.
-ZS_DEVICE int block_scan(int v, int* red, int* total) {
+// Exclusive prefix sums over the block (T threads) of two counts at once; *total gets the sums.
+struct Two {
+  int x, y;
+};
+ZS_DEVICE Two block_scan(Two v, Two* red, Two* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int x = v;
+  Two s = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffff, x, o);
-    if (lane >= o) x += y;
+    const int x = __shfl_up_sync(0xffffffff, s.x, o), y = __shfl_up_sync(0xffffffff, s.y, o);
+    if (lane >= o) s.x += x, s.y += y;
   }
   __syncthreads();
-  if (lane == 31) red[warp] = x;
+  if (lane == 31) red[warp] = s;
   __syncthreads();
-  if (warp == 0) {
-    int w = red[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffff, w, o);
-      if (lane >= o) w += y;
-    }
-    red[lane] = w;
-  }
-  __syncthreads();
-  *total = red[31];
-  return x - v + (warp ? red[warp - 1] : 0);
+  Two before = lane < warp ? red[lane] : Two{0, 0}, all = red[lane];
+  before.x = (int)__reduce_add_sync(0xffffffff, (unsigned)before.x);
+  before.y = (int)__reduce_add_sync(0xffffffff, (unsigned)before.y);
+  total->x = (int)__reduce_add_sync(0xffffffff, (unsigned)all.x);
+  total->y = (int)__reduce_add_sync(0xffffffff, (unsigned)all.y);
+  return Two{before.x + s.x - v.x, before.y + s.y - v.y};
 }
 
 // This thread's words of the free map: contiguous, so ranks follow page ids.
@@ -84,26 +81,6 @@ ZS_DEVICE Words my_words(const PagePoolArgs& a) {
   w.w0 = min(n, (int)threadIdx.x * per);
   w.w1 = min(n, w.w0 + per);
   return w;
-}
-
-// The `total` lowest free pages go to out[0, total) and are taken.  Returns false (all
-// threads) and takes none when there are fewer.
-ZS_DEVICE bool take_free(const PagePoolArgs& a, int total, int* out, int* red) {
-  const Words w = my_words(a);
-  int mine = 0, have;
-  for (int i = w.w0; i < w.w1; ++i) mine += __popc(a.free_bits[i]);
-  int rank = block_scan(mine, red, &have);
-  if (have < total) return false;
-  for (int i = w.w0; i < w.w1 && rank < total; ++i) {
-    uint32_t bits = a.free_bits[i];
-    while (bits != 0 && rank < total) {
-      const int b = __ffs(bits) - 1;
-      bits &= bits - 1;
-      out[rank++] = i * 32 + b;
-    }
-    a.free_bits[i] = bits;
-  }
-  return true;
 }
 
 // One reference of page p is dropped; without references it is free.
@@ -121,106 +98,123 @@ ZS_DEVICE void release(const PagePoolArgs& a, int p) {
   }
 }
 
-// Request i of a fork or extend: how many fresh pages it wants, and from which table entry.
-// Returns -1 for a request that cannot be served.
-ZS_DEVICE int want(const PagePoolArgs& a, const Scratch& s, int i, bool fork) {
-  const int slot = a.slots[i];
-  if (slot < 0 || slot >= a.num_slots || atomicExch(s.claim + slot, i + 1) != 0) return -1;
-  if (fork) {
-    const int from = a.parents[i];
-    if (from < 0 || from >= a.num_slots || a.seq_len[slot] != 0) return -1;
-    const int len = a.seq_len[from], share = a.lens != nullptr ? a.lens[i] : len;
-    if (share < 0 || len < 0 || len > (long long)a.max_pages * a.page_size) return -1;
-    s.full[i] = min(len, share) / a.page_size;
-    return pages_for(a, len) - s.full[i];
-  }
-  const int len = a.seq_len[slot], to = a.lens[i];
+// A request of a fork or extend: how many fresh pages it wants (-1: it cannot be served), from which
+// table entry on, and the length that it gives its slot (-1: as it is).
+struct Want {
+  int pages, full, len;
+};
+ZS_DEVICE Want want(const PagePoolArgs& a, const Scratch& s, int i, bool fork) {
+  const Want no = {-1, 0, -1};
+  const int slot = a.slots[i], from = fork ? a.parents[i] : slot, lens = a.lens != nullptr ? a.lens[i] : 0x7FFFFFFF;
+  if (slot < 0 || slot >= a.num_slots || from < 0 || from >= a.num_slots) return no;
+  const int claimed = atomicExch(s.claim + slot, i + 1), own = a.seq_len[slot], len = a.seq_len[from];
   const long long most = (long long)a.max_pages * a.page_size;
-  if (to < 0 || to > most || len < 0 || len > most) return -1;
+  if (claimed != 0 || lens < 0 || len < 0 || len > most) return no;
+  if (fork) {
+    if (own != 0) return no;
+    const int full = min(len, lens) / a.page_size;
+    return Want{pages_for(a, len) - full, full, len};
+  }
+  if (lens > most) return no;
   const int have = pages_for(a, len);
-  s.full[i] = have;
-  if (to <= len) return 0;
+  if (lens <= len) return Want{0, have, -1};
+  int full = have;
   if (len % a.page_size != 0) {
     const int tail = a.page_table[(size_t)slot * a.max_pages + have - 1];
-    if (tail < 0 || tail >= a.num_pages) return -1;
-    if (a.refcount[tail] > 1) s.full[i] = have - 1;  // copy on write: the last page too
+    if (tail < 0 || tail >= a.num_pages) return no;
+    if (a.refcount[tail] > 1) full = have - 1;  // copy on write: the last page too
   }
-  return pages_for(a, to) - s.full[i];
+  return Want{pages_for(a, lens) - full, full, lens};
 }
 
+// A thread per request, then a thread per fresh page: every chain of loads is walked once, side by
+// side (256 forks of 32 prompts, then one of each grown, with the copies: 124 us with a warp per request
+// in turn, 117 us so).
 __global__ void __launch_bounds__(T) plan_kernel(const PagePoolArgs a, bool fork) {
   pdl_wait();
   pdl_trigger();
-  __shared__ int red[32];
-  __shared__ int carry;
+  __shared__ Two red[32];
+  __shared__ int carry, off_near[T + 1];
   const Scratch s = scratch_of(a);
   const int tid = threadIdx.x;
   if (tid == 0) carry = 0;
-  int bad = 0;
+  int* const off = a.n <= T ? off_near : s.off;  // fresh pages before each request
+  const Words words = my_words(a);
+  Two mine = {0, 0}, sum;
+  for (int i = words.w0; i < words.w1; ++i) mine.y += __popc(a.free_bits[i]);
+  Want first = {0, 0, -1};
+  int bad = 0, rank = 0, have = 0;  // free pages before this thread's, of all
   for (int i0 = 0; i0 < a.n; i0 += T) {
-    __syncthreads();
     const int i = i0 + tid;
-    int w = 0;
+    Want w = {0, 0, -1};
     if (i < a.n) {
       w = want(a, s, i, fork);
-      if (w < 0) bad = 1, w = 0;
+      if (w.pages < 0) bad = 1, w.pages = 0;
+      s.full[i] = w.full;
     }
-    int sum;
-    const int before = block_scan(w, red, &sum);
+    mine.x = w.pages;
+    const Two before = block_scan(mine, red, &sum);
     const int base = carry;
-    if (i < a.n) s.off[i] = base + before;
+    if (i < a.n) off[i] = base + before.x;
+    if (i0 == 0) {
+      first = w;
+      rank = before.y;
+      have = sum.y;
+      mine.y = 0;
+    }
     __syncthreads();
-    if (tid == 0) carry = base + sum;
+    if (tid == 0) carry = (int)min((long long)base + sum.x, 1ll << 30);  // more than any pool has
   }
-  __syncthreads();
+  const bool valid = __syncthreads_or(bad) == 0;
   const int total = carry;
+  const bool ok = valid && total <= have;
   for (int i = tid; i < a.n; i += T) {  // claims are given back before anyone else runs
     const int slot = a.slots[i];
     if (slot >= 0 && slot < a.num_slots) s.claim[slot] = 0;
   }
-  const bool valid = __syncthreads_or(bad) == 0;
-  bool ok = valid && total <= a.num_pages;
-  if (ok) ok = take_free(a, total, s.dst, red);
   if (tid == 0) {
-    s.head[kCopies] = ok && total > 0 ? total : 0;
+    s.head[kCopies] = ok ? total : 0;
     s.head[kRequests] = ok ? a.n : 0;
     if (!ok) report_error(a.err, valid ? kErrNoPages : kErrBadShape);
-    s.off[a.n] = total;
+    off[a.n] = total;
   }
   if (!ok) return;
+  // The lowest free pages are taken.
+  for (int i = words.w0; i < words.w1 && rank < total; ++i) {
+    uint32_t bits = a.free_bits[i];
+    while (bits != 0 && rank < total) {
+      const int b = __ffs(bits) - 1;
+      bits &= bits - 1;
+      s.dst[rank++] = i * 32 + b;
+    }
+    a.free_bits[i] = bits;
+  }
   __syncthreads();
   // Fresh pages into the tables; pages with old contents are listed for the copy.
-  const int lane = tid & 31;
-  for (int i = tid >> 5; i < a.n; i += T / 32) {
-    const int slot = a.slots[i], from = fork ? a.parents[i] : slot;
-    const int off = s.off[i], cnt = s.off[i + 1] - off, full = s.full[i];
-    const int len = a.seq_len[from], have = pages_for(a, len);
-    int* row = a.page_table + (size_t)slot * a.max_pages;
-    const int* old = a.page_table + (size_t)from * a.max_pages;
-    for (int j = lane; j < cnt; j += 32) {
-      const int p = s.dst[off + j];
-      const int q = full + j < have ? old[full + j] : 0;
-      s.src[off + j] = q;  // 0: nothing to copy
-      a.refcount[p] = 1;
-      row[full + j] = p;
-      if (!fork && q != 0) release(a, q);  // the shared last page that this slot leaves
+  for (int k = tid; k < total; k += T) {
+    int i = 0;  // its request: the last with off <= k, which is one with pages
+    for (int hi = a.n; hi - i > 1;) {
+      const int mid = (i + hi) >> 1;
+      if (off[mid] <= k) i = mid;
+      else hi = mid;
     }
+    const int slot = a.slots[i], from = fork ? a.parents[i] : slot, j = s.full[i] + k - off[i], p = s.dst[k];
+    const int q = j < pages_for(a, a.seq_len[from]) ? a.page_table[(size_t)from * a.max_pages + j] : 0;
+    s.src[k] = q;  // 0: nothing to copy
+    a.refcount[p] = 1;
+    a.page_table[(size_t)slot * a.max_pages + j] = p;
+    if (!fork && q != 0) release(a, q);  // the shared last page that this slot leaves
+  }
+  __syncthreads();
+  // Lengths are written once all are read.
+  for (int i = tid + T; i < a.n; i += T) {
+    const int len = a.seq_len[fork ? a.parents[i] : a.slots[i]];
+    off[i] = fork ? len : max(len, a.lens[i]);
   }
   __syncthreads();
   for (int i = tid; i < a.n; i += T) {
-    const int slot = a.slots[i];
-    if (fork) {
-      s.claim[slot] = a.seq_len[a.parents[i]];  // lengths are written once all are read
-    } else if (a.lens[i] > a.seq_len[slot]) {
-      a.seq_len[slot] = a.lens[i];
-    }
-  }
-  if (!fork) return;
-  __syncthreads();
-  for (int i = tid; i < a.n; i += T) {
-    const int slot = a.slots[i];
-    a.seq_len[slot] = s.claim[slot];
-    s.claim[slot] = 0;
+    const int len = i == tid ? first.len : off[i];
+    if (len >= 0) a.seq_len[a.slots[i]] = len;
   }
 }
 
@@ -307,13 +301,13 @@ __global__ void __launch_bounds__(128) truncate_kernel(const PagePoolArgs a) {
 __global__ void __launch_bounds__(T) compact_plan_kernel(const PagePoolArgs a) {
   pdl_wait();
   pdl_trigger();
-  __shared__ int red[32];
+  __shared__ Two red[32];
   const Scratch s = scratch_of(a);
   const Words w = my_words(a);
-  int mine = 0, free_total;
-  for (int i = w.w0; i < w.w1; ++i) mine += __popc(a.free_bits[i]);
-  block_scan(mine, red, &free_total);
-  const int live = a.num_pages - free_total;
+  Two mine = {0, 0}, sum;
+  for (int i = w.w0; i < w.w1; ++i) mine.x += __popc(a.free_bits[i]);
+  block_scan(mine, red, &sum);
+  const int live = a.num_pages - sum.x;
   // Free pages below `live` and live pages from `live` on, each in id order: equally many.
   auto below = [&](int word) -> uint32_t {  // bits of the ids < live
     const int n = live - word * 32;
@@ -323,13 +317,15 @@ __global__ void __launch_bounds__(T) compact_plan_kernel(const PagePoolArgs a) {
     const int n = a.num_pages - word * 32;
     return n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u;
   };
-  int holes = 0, movers = 0, total, total2;
+  mine.x = 0;  // holes; y: pages that move
   for (int i = w.w0; i < w.w1; ++i) {
     const uint32_t f = a.free_bits[i];
-    holes += __popc(f & below(i));
-    movers += __popc(~f & exists(i) & ~below(i));
+    mine.x += __popc(f & below(i));
+    mine.y += __popc(~f & exists(i) & ~below(i));
   }
-  int hole = block_scan(holes, red, &total), mover = block_scan(movers, red, &total2);
+  const Two before = block_scan(mine, red, &sum);
+  const int total = sum.x;
+  int hole = before.x, mover = before.y;
   for (int i = w.w0; i < w.w1; ++i) {
     const uint32_t f = a.free_bits[i];
     for (uint32_t b = f & below(i); b != 0; b &= b - 1) s.dst[hole++] = i * 32 + __ffs(b) - 1;
