@@ -71,9 +71,11 @@ ZS_DEVICE void cluster_wait_started() { asm volatile("barrier.cluster.wait.align
 
 // ---------------------------------------------------------------------------------------
 // Token probabilities.  A cluster of up to 16 CTAs holds a row in shared memory (64 KiB each, three
-// CTAs to an SM, so that some load while others compute; 256 rows of 248320 tokens with two and with
-// three: 141 and 110 us plain, 257 and 211 us with top-k 50): the row is read once and written once
-// whatever it asks for.  What the CTAs have to know of one another goes through distributed
+// CTAs to an SM, so that some load while others compute; with two, 256 rows of 248320 tokens took 141
+// us plain instead of 110): the row is read once and written once whatever it asks for.  Those rows'
+// 509 MB take 78 us to copy; they take 110 us plain, 123 greedy, 173 with k = 50, 282 with k = 200 and
+// 780 with a nucleus of half the vocabulary: 21 clusters fit on the device, and a cluster's steps
+// wait for one another.  What the CTAs have to know of one another goes through distributed
 // shared memory.
 //   plain     e = 2^((x - m) c) against the CTA's own maximum and its sum; (m, sum) of all CTAs;
 //             one exchange.
@@ -96,7 +98,7 @@ struct ProbsSmem {
   union {
     struct {
       uint32_t warp_max[kCluster * PW];
-      float list[kList], cand[kCand];    // the CTA's candidates, the row's
+      float list[kList], cand[kCand + 4];    // the CTA's candidates, the row's
     };
     struct {
       uint32_t low[kHist * 256], high[kHist * 256];  // 19 bits of a mass each
@@ -108,9 +110,9 @@ struct ProbsSmem {
   uint32_t first[kCluster];              // greedy: lowest id of the maximum
   int count[kCluster];                   // candidates of every CTA
   u64 red[PW], left;
-  float bound;
   uint32_t pick;
   int mine;
+  uint8_t vote[2][PW];
 };
 static_assert(3 * (sizeof(ProbsSmem) + 1024) <= 228 * 1024, "three CTAs on an SM");
 static_assert((u64)kChunk / kHist << 19 < 1ull << 32, "a histogram's sums in 32 bits");
@@ -243,22 +245,26 @@ __global__ void __launch_bounds__(PT, 3) probs_kernel(const TokenProbsArgs a) {
   // A nucleus without top-k: is it within the candidates of 128 maxima?
   const int k_bound = K > 0 ? K : min(128, n * PW);
   if (k_bound <= min(kSmallK, n * PW)) {
-    // k-th largest of the warp maxima (equal ones in any order).
-    {  // two threads a maximum, each against half of them
-      const int i = tid >> 1, h = n * PW / 2 * (tid & 1);
-      const uint32_t k = i < n * PW ? s.warp_max[i] : 0;
-      int above = 0;
-#pragma unroll 4
-      for (int y = h; y < h + n * PW / 2; y += 4) {
-        const uint4 v = *reinterpret_cast<const uint4*>(s.warp_max + y);
-        above += (v.x > k || (v.x == k && y < i)) + (v.y > k || (v.y == k && y + 1 < i)) + (v.z > k || (v.z == k && y + 2 < i)) +
-                 (v.w > k || (v.w == k && y + 3 < i));
+    // A lower bound of the k-th largest of the warp maxima, the upper 16 bits of its image, by digits of
+    // 4 bits: every warp counts for one digit.  (Ranking the maxima read shared memory for 3 us.)
+    uint32_t bound_key = 0;
+    {
+      uint32_t key[kCluster * PW / 32];
+#pragma unroll
+      for (int x = 0; x < kCluster * PW / 32; ++x) key[x] = x * 32 + lane < n * PW ? s.warp_max[x * 32 + lane] : 0;
+#pragma unroll 1
+      for (int shift = 28; shift >= 16; shift -= 4) {
+        const uint32_t t = bound_key | (uint32_t)warp << shift;
+        uint32_t c = 0;
+#pragma unroll
+        for (int x = 0; x < kCluster * PW / 32; ++x) c += key[x] >= t;
+        c = __reduce_add_sync(0xffffffff, c);
+        if (lane == 0) s.vote[shift >> 2 & 1][warp] = warp == 0 || c >= (uint32_t)k_bound;
+        __syncthreads();
+        bound_key |= (uint32_t)(31 - __clz(__ballot_sync(0xffffffff, lane < PW && s.vote[shift >> 2 & 1][lane & (PW - 1)]))) << shift;
       }
-      above += __shfl_xor_sync(0xffffffff, above, 1);
-      if (i < n * PW && above == k_bound - 1) s.bound = from_okey(k);
     }
-    __syncthreads();
-    const float bound = s.bound;
+    const float bound = from_okey(bound_key);  // a NaN where fewer than k warps have an unmasked logit
     if (bound > -INFINITY) {
       each([&](int, float x) {
         if (x >= bound) {
@@ -283,7 +289,8 @@ __global__ void __launch_bounds__(PT, 3) probs_kernel(const TokenProbsArgs a) {
     const int total = (int)__reduce_add_sync(0xffffffff, (unsigned)min(cnt, kList + 1));
     done = __all_sync(0xffffffff, cnt <= kList) && total <= kCand;
     if (done) {
-      // One list, ranked: larger values first.
+      // One list, ranked: larger values first.  (Compared four at a time, by one comparison each: k = 200
+      // took 389 us with two comparisons a value, 318 so.)
       int before = cnt;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -296,17 +303,30 @@ __global__ void __launch_bounds__(PT, 3) probs_kernel(const TokenProbsArgs a) {
         const float* list = cluster.map_shared_rank(s.list, r);
         for (int i = lane; i < m; i += 32) s.cand[at + i] = list[i];
       }
+      if (tid < 3) s.cand[total + tid] = -INFINITY;  // the last group of 4
       __syncthreads();
       cluster_arrive();  // the others' lists are read
       float v[kCand / PT];
       int above[kCand / PT];
 #pragma unroll
       for (int q = 0; q < kCand / PT; ++q) {
-        const int i = tid + q * PT;
+        // Equal values stay in the list's order: before this warp's own 32 `>=` counts, behind them `>`.
+        const int i = tid + q * PT, own = i & ~31;
         v[q] = i < total ? s.cand[i] : 0.f;
         above[q] = 0;
-        if (i < total)
-          for (int y = 0; y < total; ++y) above[q] += s.cand[y] > v[q] || (s.cand[y] == v[q] && y < i);
+        if (own >= total) break;
+        const float4* list = reinterpret_cast<const float4*>(s.cand);
+#pragma unroll 2
+        for (int y = 0; y < own / 4; ++y) {
+          const float4 o = list[y];
+          above[q] += (o.x >= v[q]) + (o.y >= v[q]) + (o.z >= v[q]) + (o.w >= v[q]);
+        }
+        for (int y = own; y < min(own + 32, total); ++y) above[q] += s.cand[y] > v[q] || (s.cand[y] == v[q] && y < i);
+#pragma unroll 2
+        for (int y = own / 4 + 8; y < (total + 3) / 4; ++y) {
+          const float4 o = list[y];
+          above[q] += (o.x > v[q]) + (o.y > v[q]) + (o.z > v[q]) + (o.w > v[q]);
+        }
       }
       __syncthreads();
 #pragma unroll
