@@ -74,7 +74,7 @@ ZS_DEVICE void cluster_wait_started() { asm volatile("barrier.cluster.wait.align
 // CTAs to an SM, so that some load while others compute; with two, 256 rows of 248320 tokens took 141
 // us plain instead of 110): the row is read once and written once whatever it asks for.  Those rows'
 // 509 MB take 78 us to copy; they take 110 us plain, 123 greedy, 173 with k = 50, 282 with k = 200 and
-// 780 with a nucleus of half the vocabulary: 21 clusters fit on the device, and a cluster's steps
+// 780 with a nucleus of 500 tokens (the radix select): 21 clusters fit on the device, and a cluster's steps
 // wait for one another.  What the CTAs have to know of one another goes through distributed
 // shared memory.
 //   plain     e = 2^((x - m) c) against the CTA's own maximum and its sum; (m, sum) of all CTAs;
