@@ -856,11 +856,11 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
 }
 
 constexpr int MERGE_WARPS = 8, AT_ONCE = 2;
-// The join of a (row, q head) pair's records, read once from L2 (4.2 us for 2048 pairs' 20 MB after
+// The join of a (row, q head) pair's records, read once from L2 (4.2 us for 1824 pairs' 20 MB after
 // the tiles' end; latencies bound it).  A lane owns dims 4 lane .. + 3 and 128 + 4 lane .. + 3.  Records
 // are found and weighed 32 at a time (one a lane), then added in order, AT_ONCE on their way together;
 // with PARTS warps on a pair, warp p takes every PARTS-th record and the parts are joined in order.
-// 64 registers, so that four CTAs share an SM, are worth more than more loads in flight (2048 pairs:
+// 64 registers, so that four CTAs share an SM, are worth more than more loads in flight (1824 pairs:
 // 40.5 us the whole call with 2, 40.9 with 3; with 4 and 80 registers 45.4).
 template <int PARTS>
 __global__ void __launch_bounds__(MERGE_WARPS * 32, 4) merge_kernel(const SharedAttnArgs a) {
@@ -1039,8 +1039,8 @@ extern "C" int zs_shared_attn(const SharedAttnArgs* args, cudaStream_t stream) {
   const int items = a.rows * a.num_q_heads;
   // Warps that share the records of a (row, q head) pair: with few pairs a long prefix leaves a record
   // in every CTA, with many there are a few each and the device is full without.  The whole call in us
-  // with 1, 2, 4 and 8: 64 pairs 21.7, 18.8, 17.0, 16.2; 768 pairs 61.6, 55.6, 52.4, 56.7; 2048 pairs
-  // 39.6, 39.7, 43.6, 49.4; 8192 pairs 57.1, 65.3, 75.3, 96.5.
+  // with 1, 2, 4 and 8: 64 pairs 21.7, 18.8, 17.0, 16.2; 768 pairs 61.6, 55.6, 52.4, 56.7; 1824 pairs
+  // 39.6, 39.7, 43.6, 49.4; 7296 pairs 57.1, 65.3, 75.3, 96.5.
   int parts = MERGE_WARPS;
   while (parts > 1 && (long long)items * parts > 4096) parts /= 2;
   const auto merge = parts == 8 ? merge_kernel<8> : parts == 4 ? merge_kernel<4> : parts == 2 ? merge_kernel<2> : merge_kernel<1>;
