@@ -74,7 +74,7 @@ ZS_DEVICE void cluster_wait_started() { asm volatile("barrier.cluster.wait.align
 // CTAs to an SM, so that some load while others compute; with two, 256 rows of 248320 tokens took 141
 // us plain instead of 110): the row is read once and written once whatever it asks for.  Those rows'
 // 509 MB take 78 us to copy; they take 110 us plain, 123 greedy, 173 with k = 50, 282 with k = 200 and
-// 780 with a nucleus of 500 tokens (the radix select): 21 clusters fit on the device, and a cluster's steps
+// 541 with a nucleus of 500 tokens (the radix select): 21 clusters fit on the device, and a cluster's steps
 // wait for one another.  What the CTAs have to know of one another goes through distributed
 // shared memory.
 //   plain     e = 2^((x - m) c) against the CTA's own maximum and its sum; (m, sum) of all CTAs;
@@ -84,8 +84,8 @@ ZS_DEVICE void cluster_wait_started() { asm volatile("barrier.cluster.wait.align
 //             leaves little more than k candidates, which every CTA ranks for itself: exact
 //             threshold, nucleus and sum from the sorted list.  Two exchanges.
 //   top-p     the same with the candidates of k = 128, where the nucleus lies within them.
-//   otherwise (a wide nucleus, k above 256, many ties): radix select by 8 bits of the ordered image
-//             of the logit over histograms of counts or of fixed-point masses, whose sums have
+//   otherwise (a wide nucleus, k above 256, many ties): radix select by 8 bits of the distance of
+//             ordered images from the top's over histograms of counts or of fixed-point masses, whose sums have
 //             one value in any order.
 constexpr int PT = 512, PW = PT / 32;
 constexpr int kChunk = 16384;            // logits of a CTA at most
@@ -102,9 +102,9 @@ struct ProbsSmem {
     };
     struct {
       uint32_t low[kHist * 256], high[kHist * 256];  // 19 bits of a mass each
-      u64 mine_hist[256];                // the CTA's
+      u64 mine_hist[257];                // the CTA's, and what is outside
     };
-    u64 total[256];                      // the row's
+    u64 total[257];                      // the row's
   };
   float2 part[kCluster];                 // (maximum, sum) of every CTA
   uint32_t first[kCluster];              // greedy: lowest id of the maximum
@@ -112,7 +112,7 @@ struct ProbsSmem {
   u64 red[PW], left;
   uint32_t pick;
   int mine;
-  uint8_t vote[2][PW];
+  uint8_t vote[2][PW], found;
 };
 static_assert(3 * (sizeof(ProbsSmem) + 1024) <= 228 * 1024, "three CTAs on an SM");
 static_assert((u64)kChunk / kHist << 19 < 1ull << 32, "a histogram's sums in 32 bits");
@@ -377,72 +377,93 @@ __global__ void __launch_bounds__(PT, 3) probs_kernel(const TokenProbsArgs a) {
   }
 
   if (!done) {
-    uint32_t key_thr = 0;
+    // A logit's place: how far its ordered image is below the top's, in digits of 8 bits.  Most of what
+    // counts is within 2^24 of the top, so the first digit is taken for 0, and looked at only if that is
+    // wrong (256 rows with a nucleus of 500 tokens: 788 us with that digit first, when most logits fall
+    // into few bins, 582 so; 541 with every CTA adding up its share of the bins, not all of them, and
+    // masses only where they are asked for).
+    const uint32_t top_image = okey(top);
+    uint32_t far = 0xFFFFFFFFu;  // places up to here are kept
     for (int phase = 0; phase < 2; ++phase) {
       const bool by_mass = phase == 1;
       if (by_mass ? P == 1.f : K <= 0) continue;
       u64 need = (u64)K;
       uint32_t prefix = 0;
-      for (int shift = 24; shift >= 0; shift -= 8) {
+      bool first = true;
+      for (int shift = 16; shift >= 0;) {
         for (int i = tid; i < kHist * 256; i += PT) s.low[i] = s.high[i] = 0;
         __syncthreads();
+        u64 outside = 0;
         each([&](int, float x) {
-          const uint32_t k = okey(x);
-          const bool counts = x > -INFINITY && k >= key_thr && (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)));
-          if (!counts) return;
-          const int bin = warp % kHist * 256 + ((k >> shift) & 255);
-          if (by_mass) {
-            const u64 v = fixed(mass(x));
-            atomicAdd(&s.low[bin], (uint32_t)v & 0x7FFFF);
-            atomicAdd(&s.high[bin], (uint32_t)(v >> 19));
-          } else {
-            atomicAdd(&s.low[bin], 1u);
+          const uint32_t k = top_image - okey(x);
+          if (!(x > -INFINITY) || k > far) return;
+          const bool in = shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8));
+          if (!in && !(by_mass && first)) return;
+          const u64 v = by_mass ? fixed(mass(x)) : 1;
+          if (!in) {
+            outside += v;
+            return;
           }
+          const int bin = warp % kHist * 256 + ((k >> shift) & 255);
+          atomicAdd(&s.low[bin], (uint32_t)v & 0x7FFFF);
+          if (by_mass) atomicAdd(&s.high[bin], (uint32_t)(v >> 19));
         });
+        if (by_mass && first) outside = block_all<PW>(outside, s.red, [](u64 p, u64 q) { return p + q; }, (u64)0);
         __syncthreads();
         if (tid < 256) {
           u64 sum = 0;
           for (int i = 0; i < kHist; ++i) sum += s.low[i * 256 + tid] + ((u64)s.high[i * 256 + tid] << 19);
           s.mine_hist[tid] = sum;
+        } else if (tid == 256) {
+          s.mine_hist[256] = outside;
         }
         cluster.sync();
-        if (tid < 256) {
-          u64 sum = 0;
-          for (int r = 0; r < n; ++r) sum += cluster.map_shared_rank(s.mine_hist, r)[tid];
-          s.total[tid] = sum;
+        // Every CTA adds up its share of the bins and tells all: a thread per bin and CTA, n of them side
+        // by side.  (The first one's ninth warp does the same with what is outside.)
+        if (tid < 256 || (rank == 0 && warp == 8)) {
+          const int r = tid & (n - 1), bin = tid < 256 ? (rank * 256 + tid) / n : 256;
+          u64 sum = cluster.map_shared_rank(s.mine_hist, r)[bin];
+          for (int o = 1; o < n; o <<= 1) sum += __shfl_xor_sync(0xffffffff, sum, o);
+          cluster.map_shared_rank(s.total, r)[bin] = sum;
         }
-        cluster.sync();  // the others have read this CTA's
-        __syncthreads();
-        if (warp == 0) {  // lane l: bins 255 - 8 l and the 7 below
+        cluster.sync();
+        if (warp == 0) {  // lane l: bins 8 l and the 7 behind
           u64 sum = 0;
-          for (int d = 0; d < 8; ++d) sum += s.total[255 - 8 * lane - d];
+          for (int d = 0; d < 8; ++d) sum += s.total[8 * lane + d];
           u64 upto = sum;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
             const u64 y = __shfl_up_sync(0xffffffff, upto, o);
             if (lane >= o) upto += y;
           }
-          if (by_mass && shift == 24) {
-            need = (u64)((double)P * (double)__shfl_sync(0xffffffff, upto, 31));
+          if (by_mass && first) {
+            need = (u64)((double)P * (double)(__shfl_sync(0xffffffff, upto, 31) + s.total[256]));
             if (need == 0) need = 1;
           }
           const uint32_t enough = __ballot_sync(0xffffffff, upto >= need);
           if (lane == (enough != 0 ? __ffs(enough) - 1 : 31)) {
             u64 left = need - (upto - sum);
-            int d = 255 - 8 * lane;
-            const int low = d - 7;
-            for (; d > low && s.total[d] < left; --d) left -= s.total[d];
+            int d = 8 * lane;
+            const int high = d + 7;
+            for (; d < high && s.total[d] < left; ++d) left -= s.total[d];
+            s.found = enough != 0 || !(first && shift == 16);
             s.pick = prefix | ((uint32_t)d << shift);
-            s.left = left;
+            s.left = s.found ? left : need;
           }
         }
         __syncthreads();
-        prefix = s.pick;
         need = s.left;
+        if (s.found) {
+          prefix = s.pick;
+          shift -= 8;
+        } else {
+          shift = 24;
+        }
+        first = false;
       }
-      key_thr = max(key_thr, prefix);
+      far = min(far, prefix);
     }
-    thr = key_thr == 0 ? -INFINITY : from_okey(key_thr);
+    thr = far > top_image ? -INFINITY : from_okey(top_image - far);
     float sum = 0.f;
     each([&](int, float x) {
       if (x >= thr) sum += mass(x);

@@ -119,6 +119,18 @@ def test_probs_top_p(vocab):
 
 
 @gpu
+@pytest.mark.parametrize("vocab", [700, 30000, 248320])
+def test_probs_wide_nuclei_and_large_k(vocab):
+    # From peaked rows to flat ones whose nucleus reaches across zero and far below the top's image.
+    x = torch.randn(8, vocab, generator=torch.Generator().manual_seed(vocab)) * 4
+    x[6] = x[6].abs() * 1e-3
+    x[7] -= 200.0
+    x[:, 5::11] = -math.inf
+    check_probs(x, [1.0, 8.0, 50.0, 1.0, 8.0, 50.0, 2.0, 3.0], [0, 0, 0, 300, 600, 257, 0, 400],
+                [0.95, 0.5, 0.999, 1.0, 0.9, 0.3, 0.7, 0.99])
+
+
+@gpu
 def test_probs_top_p_keeps_ties():
     x = torch.zeros(2, 100)
     x[0, :10] = 5.0
