@@ -117,8 +117,10 @@ __global__ void __launch_bounds__(1024) plan_kernel(const SharedAttnArgs a) {
       g.e0 = x.y;
       g.rows = x.z;
       // What a piece costs besides its tiles, in tiles of 1.1 us: another Q, 0.9 us; for a unit's first
-      // one also a pipeline that starts anew and the last unit's records, 3.4 us with 128 slots.
-      g.over = x.w == i ? 3 + x.z * group / 128 : 1;
+      // one also the last unit's records and a pipeline that starts anew, 6 to 7 us with 128 slots
+      // (eight prompts: 36.9 us the call with 6 tiles for it, 39.8 with 4, 36.7 with 7; four rows a
+      // sequence: 57.3, 57.3, 58.2).
+      g.over = x.w == i ? 4 + x.z * group / 64 : 1;
       g.r0 = y.y >> 16;
       g.r1 = y.y & 0xFFFF;
       g.p0 = y.z;
