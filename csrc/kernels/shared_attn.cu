@@ -838,6 +838,8 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
         pdl_wait();
         pdl_trigger();
         dry = i = 0;
+        m = -INFINITY;
+        l = 0.f;
         more = !compute_any(!next_fragment(f));
         if (more) {
           fetch_q(f);
