@@ -374,6 +374,8 @@ __global__ void __launch_bounds__(PT, 3) probs_kernel(const TokenProbsArgs a) {
       done = s.part[0].y > 0.f;
       cluster_wait();  // nobody reads this CTA's list any more
     }
+  } else {
+    __syncthreads();  // every warp has read warp_max: the histograms take its place
   }
 
   if (!done) {

@@ -178,6 +178,24 @@ def test_probs_strided_rows_and_repeats():
 
 
 @gpu
+@pytest.mark.parametrize("vocab,k", [(248320, 257), (248320, 300), (62081, 257), (16384, 17), (8192, 50), (2000, 33)])
+def test_probs_of_many_rows_repeat_beyond_the_candidate_path(vocab, k):
+    """k above 256, or above the warps of a row's CTAs: no candidates, the radix select comes right behind the
+    row's maximum.  Every row is the same one and has to give the same bits, launch after launch."""
+    x = torch.randn(1, vocab, generator=torch.Generator().manual_seed(k)) * 4
+    check_probs(x, [0.9], [k], [0.95])
+    rows = 256
+    wide = x.cuda().expand(rows, vocab).contiguous()
+    t, p = torch.full((rows,), 0.9, device="cuda"), torch.full((rows,), 0.95, device="cuda")
+    ks = torch.full((rows,), k, dtype=torch.int32, device="cuda")
+    first, out = token_probs(wide, t, ks, p)[0].clone(), torch.empty_like(wide)
+    wrong = torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(40):
+        wrong += (token_probs(wide, t, ks, p, out=out) != first).sum()
+    assert int(wrong) == 0
+
+
+@gpu
 def test_probs_refusals():
     x, t = torch.zeros(3, 10, device="cuda"), torch.ones(3, device="cuda")
     for args in ((x.half(), t), (x.t(), t), (x, t[:2]), (x, t, t), (x, t, None, t.int()), (x[0], t), (x.cpu(), t)):
