@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
     for (int i = 0; i < AHEAD; ++i) {
       mbar_init(&s.f_full[i], 1);
       mbar_init(&s.r_full[i], 32);
-      mbar_init(&s.f_empty[i], COMPUTE / 32);
+      mbar_init(&s.f_empty[i], COMPUTE / 32 + 3);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.way_full[i], 32);
@@ -400,8 +400,18 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
   int fk = 0;
   uint32_t fph = 0;
   auto next_fragment = [&](Fragment& f) {
-    if (!wait_for(s, &s.f_full[fk], fph, a.err)) return false;
+    // The softmax warps give its place back when they are through with the piece (they also read the
+    // limits there), the copy and MMA warps as soon as they have read it: none of them may be so far
+    // behind that the lookup warp writes the next piece over one that it has yet to read.
+    const bool reader = warp >= COMPUTE / 32;
+    bool ok = wait_for(s, &s.f_full[fk], fph, a.err);
+    if (reader) ok = __all_sync(0xffffffff, ok);
+    if (!ok) return false;
     f = s.frag[fk];
+    if (reader) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.f_empty[fk]);
+    }
     if (++fk == AHEAD) {
       fk = 0;
       fph ^= 1;

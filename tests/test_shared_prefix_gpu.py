@@ -271,6 +271,21 @@ def test_two_calls_give_the_same_bits():
 
 
 @gpu
+def test_many_pieces_of_one_tile():
+    """Hundreds of sequences within one tile: every warp gets a new piece with every tile."""
+    b = Batch(16, 2, [], [seq(None, 0, 1 + (7 * i) % 64) for i in range(700)], seed=17)
+    plan, d = b.plan(), b.device()
+    out = run(b, plan)
+    near(out, b.want())
+    again = torch.empty_like(out)
+    for _ in range(50):
+        plan.update(d["seq_lens"])
+        plan.attend(d["q"], d["gate"], d["k_cache"], d["v_cache"], d["page_table"], d["seq_lens"], 1 / 16, out=again)
+        assert torch.equal(out, again)
+    plan.check()
+
+
+@gpu
 def test_page_beyond_four_gigabytes_of_elements():
     """A page whose element offset passes 2^32 (and byte offset 2^33)."""
     hq, hkv = 2, 1
