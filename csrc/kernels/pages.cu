@@ -46,7 +46,7 @@ __host__ __device__ inline Scratch scratch_of(const PagePoolArgs& a) {
   return s;
 }
 
-ZS_DEVICE int pages_for(const PagePoolArgs& a, int tokens) { return (tokens + a.page_size - 1) / a.page_size; }
+ZS_DEVICE int pages_for(const PagePoolArgs& a, int tokens) { return tokens / a.page_size + (tokens % a.page_size > 0); }
 
 // Exclusive prefix sums over the block (T threads) of two counts at once; *total gets the sums.
 struct Two {

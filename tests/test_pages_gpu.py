@@ -238,6 +238,23 @@ def test_a_slot_cut_twice_in_one_call_ends_at_the_shorter_length():
     same(pool, m)
 
 
+@pytest.mark.parametrize("huge", [2 ** 31 - 1, 2 ** 31 - PAGE, 2 ** 31 - PAGE + 1])
+def test_lengths_whose_pages_pass_32_bits(huge):
+    """A cut to more than a slot holds has no effect, however much more; growth to that is refused."""
+    pool, m = make(40, 4, 8)
+    both(pool, m, "extend", [1, 3], [100, 128])
+    pool.truncate(ints([1, 3, 0]), ints([huge] * 3))
+    pool.check()
+    same(pool, m)
+    pool.extend(ints([1]), ints([huge]))
+    with pytest.raises(RuntimeError):
+        pool.check()
+    same(pool, m)
+    both(pool, m, "fork", [1], [0], [huge])
+    pool.check()
+    same(pool, m)
+
+
 def test_copy_and_adopt():
     pool, m = make(50, 4, 6, ((2, 1, PAGE, 256), (3, PAGE, 40)))
     table = [[7, 9, 0], [7, 30, 49], [0, 0, 0], [12, 0, 0]]
