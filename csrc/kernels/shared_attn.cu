@@ -945,7 +945,7 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32, 4) merge_kernel(const Shared
       load(0);
       const float mn = fmaxf(m, warp_max(ml.x)), s0 = m == -INFINITY ? 0.f : exp2f(m - mn);
       const float wt = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mn);
-      l = l * s0 + warp_sum(ml.x == -INFINITY ? 0.f : wt * (ml.y + ml.z));
+      l = l * s0 + warp_sum(wt * (ml.y + ml.z));  // a sum without a maximum is 0, or NaN where every score was
 #pragma unroll
       for (int k = 0; k < 8; ++k) o[k] *= s0;
       m = mn;
@@ -981,7 +981,7 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32, 4) merge_kernel(const Shared
     const float mp = lane < PARTS ? parts[lane][D] : -INFINITY;
     m = warp_max(mp);
     const float wp = mp == -INFINITY ? 0.f : exp2f(mp - m);
-    l = warp_sum(mp == -INFINITY ? 0.f : wp * parts[lane][D + 1]);
+    l = warp_sum(lane < PARTS ? wp * parts[lane][D + 1] : 0.f);
 #pragma unroll
     for (int k = 0; k < 8; ++k) o[k] = 0.f;
 #pragma unroll
@@ -993,7 +993,9 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32, 4) merge_kernel(const Shared
     }
   }
   if (at_item != item) return;
-  const float inv = m == -INFINITY ? 0.f : 1.f / l;
+  // A row without keys gives 0.  Any other whose sum is 0 or NaN (its scores all -inf, or one NaN) gives NaN.
+  const bool empty = a.seq_lens[row] <= 0;
+  const float inv = 1.f / l;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int d = k * 128 + lane * 4;
@@ -1004,7 +1006,7 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32, 4) merge_kernel(const Shared
       for (int j = 0; j < 4; ++j) g[j] = sigmoidf_(__bfloat162float(reinterpret_cast<const __nv_bfloat16*>(&gate[k])[j]));
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = m == -INFINITY ? 0.f : y[j] * inv * g[j];
+    for (int j = 0; j < 4; ++j) y[j] = empty ? 0.f : y[j] * inv * g[j];
     if (a.out_bf16 != nullptr)
       *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out_bf16) + (size_t)item * D + d) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
     if (a.out_q != nullptr) {  // a block of 32 dims is 8 lanes

@@ -160,6 +160,45 @@ def test_a_value_that_only_another_row_sees_does_not_count(bad):
     assert not torch.isfinite(out[[r for r in range(len(b.lens)) if r not in seen]]).all()
 
 
+def near_where_finite(out, want):
+    y, a = want
+    out = out.cpu().double()
+    assert torch.equal(out.isnan(), y.isnan())
+    tol = 2.0 ** -9 * (a + 2 * y.abs()) + 1e-4 * a + 1e-30
+    assert ((out - y).abs() <= tol)[~y.isnan()].all()
+
+
+@gpu
+@pytest.mark.parametrize("prefix", [3, 200])
+def test_scores_that_are_all_nan_are_not_taken_for_no_keys(prefix):
+    """A query row of NaN; a NaN key that is the only one of its record, beside records of finite ones."""
+    n = prefix * PAGE
+    b = Batch(16, 2, [prefix], [seq(0, n, 5), seq(0, n, 1), seq(0, n, 40), (0, n + 7, [0, n + 7])], seed=18)
+    b.q[2] = float("nan")
+    b.q[0, 3] = float("nan")
+    b.k[b.table[1, prefix], 1, 0] = float("nan")
+    y, a = b.want()
+    nan = y.view(5, 16, D).isnan().all(-1)
+    assert nan[0].tolist() == [h == 3 for h in range(16)] and nan[1].tolist() == [h >= 8 for h in range(16)]
+    assert nan[2].all() and not nan[3:].any()
+    near_where_finite(run(b), (y, a))
+
+
+@gpu
+def test_scores_that_are_all_minus_infinity():
+    """Keys that a row sees, all with a score of -inf, are no empty mask: 0 / 0.  Beside finite ones they weigh nothing."""
+    b = Batch(16, 2, [2], [(None, 33, [33]), (0, 40, [0, 40])], seed=19)
+    b.q[:, :, 0] = 1.0
+    for t in range(33):
+        b.k[b.table[0, t // PAGE], 0, t % PAGE, 0] = float("-inf")
+    b.k[b.table[1, 2], :, 3, 0] = float("-inf")
+    y, a = b.want()
+    assert y.view(3, 16, D)[0, :8].isnan().all() and not y.view(3, 16, D)[0, 8:].isnan().any() and not y[1:].isnan().any()
+    out = run(b)
+    near_where_finite(out, (y, a))
+    assert not out[1].any()
+
+
 @gpu
 def test_rows_without_keys_and_rows_inside_the_prefix():
     """Length 0 gives 0; a row shorter than its group's prefix sees that much of it."""
