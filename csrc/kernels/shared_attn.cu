@@ -228,8 +228,6 @@ struct Smem {
   uint8_t way[SLOTS][528];          // Q on its way to TMEM, 512 bytes a slot
   float stage[8][32][20];           // a warp's 32 slots x 16 dims of O on their way out
   float top[2][2][SLOTS];           // per half of a tile's keys, the largest score of every slot
-  int vote[2][8];
-  int again[2];                     // the P of this tile is followed by its rounding errors
   Fragment frag[AHEAD];             // t1 == 0: no more
   int limit[AHEAD][SLOTS];          // keys that each slot sees (0: unused)
   int least[AHEAD];                 // the fewest among the piece's slots
@@ -342,15 +340,18 @@ constexpr float kGrow = 8.f;         // O is rescaled when a maximum grows by mo
 //  * softmax warps: P = 2^(s - m) with a reference m that follows the running maximum only when
 //    that grows by more than 2^8 (P stays below 2^8, O and l in fp32), so O in TMEM is rescaled
 //    rarely; the next fragment's Q goes to TMEM during this one's last tile.
-// P is rounded to bf16 for the tensor cores, 2^-8 of a weight; over many keys those errors
-// average out, and where a weight is more than a quarter of its half's sum before its tile
-// (first tiles, few keys, peaked rows) a second product adds what the rounding lost.  l sums the
-// weights before they are rounded.
-// Long pieces run at 1.0 to 1.1 us a tile and CTA, 9 TB/s over the device with the cache in L2; the two
-// products take 0.53 us of it (1024 clocks at 4096 multiply-adds a clock).  S and P in places of their own, so
-// that the next S need not wait for O, gave 1.15 us: the copies set the pace.  What short calls pay
-// for is the way to the first tile (5 us from the plan's end: range, piece, rows, Q) and a unit's
-// records (3.6 us for 128 slots, 5.5 TB/s over all SMs).
+// The tensor cores take P as bf16, so it goes through them twice: rounded, and what the rounding left
+// (2^-18 of a weight is lost then).  A single product loses 2^-9 of every weight, and as values of
+// either sign cancel in the output as much as those errors do, that is 2^-9 of the output too, as much
+// again as its own rounding (0.0021 of the result's norm at 2000 and 33000 keys, 0.0017 so).  Left out
+// where no weight is above a quarter of the sum so far, the second product saved 0, 3 and 2 % of a call
+// (eight prompts, the same with four rows a sequence, a long document).  l sums the weights before
+// they are rounded.  A value that is infinite where a row sees it gives NaN, not an infinity.
+// Long pieces run at 1.0 to 1.1 us a tile and CTA; the three products take 0.8 us of it (1536
+// clocks at 4096 multiply-adds a clock).  A copy takes 2 us from its issue to its S, and two of K are on
+// their way at a time; S and P in places of their own, so that the next S need not wait for O, gave
+// 1.15 us.  What short calls pay for is the way to the first tile (5 us from the plan's end: range,
+// piece, rows, Q) and a unit's records (3.6 us for 128 slots, 5.5 TB/s over all SMs).
 __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs a) {
   extern __shared__ __align__(1024) uint8_t raw[];
   Smem& s = *reinterpret_cast<Smem*>(raw);
@@ -488,16 +489,13 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
       if (!wait_for(s, &s.p_full[b], (i >> 1) & 1, a.err)) return false;
       tc_fence_after();
       const uint32_t v_at = v_lo + st * (STAGE / 16), p_at = tmem + b * TILE;
-      const bool again = s.again[b] != 0;
       if (leader) {
 #pragma unroll
         for (int k = 0; k < TPAGES; ++k)  // a page each: 16 keys
           mma_step_rows(tmem + kTmemO, p_at + k * 8, v_at + k * (BLOCK / 16), idesc_o, off, !fresh || k > 0);
-        if (again) {
 #pragma unroll
-          for (int k = 0; k < TPAGES; ++k)
-            mma_step_rows(tmem + kTmemO, p_at + 32 + k * 8, v_at + k * (BLOCK / 16), idesc_o, off, true);
-        }
+        for (int k = 0; k < TPAGES; ++k)  // what the rounding of P to bf16 left
+          mma_step_rows(tmem + kTmemO, p_at + 32 + k * 8, v_at + k * (BLOCK / 16), idesc_o, off, true);
         tc_commit(&s.empty[1][st]);
         tc_commit(&s.o_full[b]);
       }
@@ -682,15 +680,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
           mt = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
           s.top[b][half][slot] = mt;
         }
-        // A weight above a quarter of the sum so far: its bf16 rounding (2^-8) would show.
-        const bool sharp = dry || (used && mt > -INFINITY && (m == -INFINITY || ex2((mt - m) * qscale) * 4.f > l));
-        {
-          const int any = __any_sync(0xffffffff, sharp);
-          if (lane == 0) s.vote[b][warp] = any;
-          compute_sync();
-        }
-        const int4 v0 = *reinterpret_cast<const int4*>(&s.vote[b][0]), v1 = *reinterpret_cast<const int4*>(&s.vote[b][4]);
-        const bool fine = (v0.x | v0.y | v0.z | v0.w | v1.x | v1.y | v1.z | v1.w) != 0;
+        compute_sync();  // both halves' maxima are there, and S is read: P takes its place
         float fac = 1.f;
         bool grow = false;
         if (busy) {
@@ -732,16 +722,13 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
           }
           tmem_st_32x32b_x16(lanes + b * TILE + half * 16, pk);
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          if (fine) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              pk[j] = pack_bf16(__uint_as_float(r[2 * j]) - __uint_as_float(pk[j] << 16),
-                                __uint_as_float(r[2 * j + 1]) - __uint_as_float(pk[j] & 0xFFFF0000u));
-            tmem_st_32x32b_x16(lanes + b * TILE + 32 + half * 16, pk);
-          }
+          for (int j = 0; j < 16; ++j)
+            pk[j] = pack_bf16(__uint_as_float(r[2 * j]) - __uint_as_float(pk[j] << 16),
+                              __uint_as_float(r[2 * j + 1]) - __uint_as_float(pk[j] & 0xFFFF0000u));
+          tmem_st_32x32b_x16(lanes + b * TILE + 32 + half * 16, pk);
           tmem_st_wait();
         }
-        if (tid == 0) s.again[b] = fine;
         // Values that a row does not see must not meet its zero weights as NaN or infinity.  Rows
         // of the tile that nobody sees are zeroed.  Rows that only some see are looked at: those
         // with such a value are zeroed too, and added by hand to the slots that see them.
