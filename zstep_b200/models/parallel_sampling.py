@@ -68,7 +68,8 @@ class ParallelSampler:
             starts.append(starts[-1] + len(p) - 1)
         if ids:
             r.stage(ids, pos, slots, seq_start=starts)
-            r._layers(len(ids), decode=False, num_seqs=n)
+            with r.eager_plan(None):
+                r._layers(len(ids), decode=False, num_seqs=n)
         kids = list(range(n, n + n * samples))
         parent = [s for s in range(n) for _ in range(samples)]
         self.pool.fork(self._ints(parent), self._ints(kids))
@@ -104,11 +105,8 @@ class ParallelSampler:
             rows += [s] * k1
         self.pool.extend(self._ints(slots), self._ints([len(self.tokens[s]) + self.k for s in slots]))
         r.stage(ids, pos, rows, seq_start=[i * k1 for i in range(n + 1)])
-        r.prefix_plan = self._plan(slots) if shared else None
-        try:
+        with r.eager_plan(self._plan(slots) if shared else None):
             r._layers(n * k1, decode=False, num_seqs=n)
-        finally:
-            r.prefix_plan = None
         out = torch.empty(n * k1, r.vocab_local, dtype=torch.float32, device=r.dev)
         r._gemm(r.lm_head, r.buf["xq"], r.buf["xsf"], n * k1, out, r.vocab_local, EPI_F32)
         return out.view(n, k1, r.vocab_local)

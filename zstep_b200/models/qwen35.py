@@ -28,6 +28,7 @@ forward, 1236 varlen prefill, 1404 graph capture, 484-524 state allocation).
 
 from __future__ import annotations
 
+import contextlib
 import math
 from dataclasses import dataclass
 
@@ -133,13 +134,11 @@ class Qwen35Runner:
         self.dummy_slot = self.num_slots - 1
         src = weights or RandomWeights(cfg, seed=seed)
         self._load_weights(src)
+        self.graphs: dict[int, torch.cuda.CUDAGraph] = {}
+        self.spec = None
+        self.prefix_plan = None
         self._alloc_state()
         self._alloc_buffers()
-        self.graphs: dict[int, torch.cuda.CUDAGraph] = {}
-        # Rows that share leading pages (ops.shared_prefix.SharedPrefixPlan over the rows of the
-        # coming steps): full attention then reads shared pages once.  None: every row reads its own.
-        self.prefix_plan = None
-        self.spec = None
         if self.num_spec:
             from .qwen35_spec import SpecDecoder
 
@@ -558,6 +557,46 @@ class Qwen35Runner:
         else:
             self.C.argmax_reduce(b["lm_keys"], rows, self.vocab_tiles, b["out_ids"], b["out_vals"], b["out_keys"])
 
+    # ------------------------------------------------------------------ what graphs depend on
+    # A captured graph holds the addresses of the page table and of the plan's tensors, and
+    # launches one kind of attention: where either is replaced, the graphs go.
+    @property
+    def page_table(self) -> torch.Tensor:
+        return self._page_table
+
+    @page_table.setter
+    def page_table(self, table: torch.Tensor) -> None:
+        self._drop_graphs()
+        self._page_table = table
+
+    @property
+    def prefix_plan(self):
+        """Rows that share leading pages (ops.shared_prefix.SharedPrefixPlan over the rows of the
+        coming steps): full attention then reads shared pages once.  None: every row reads its own."""
+        return self._prefix_plan
+
+    @prefix_plan.setter
+    def prefix_plan(self, plan) -> None:
+        if plan is not getattr(self, "_prefix_plan", None):
+            self._drop_graphs()
+        self._prefix_plan = plan
+
+    @contextlib.contextmanager
+    def eager_plan(self, plan):
+        """`plan` in the place of `prefix_plan` for the steps inside, which replay no graph."""
+        held, self._prefix_plan = self._prefix_plan, plan
+        try:
+            yield
+        finally:
+            self._prefix_plan = held
+
+    def _drop_graphs(self) -> None:
+        held = [g for g in (self.graphs, getattr(self.spec, "g_graphs", None)) if g]
+        if held:
+            torch.cuda.synchronize(self.dev)  # none of them is running any more
+        for g in held:
+            g.clear()
+
     # ------------------------------------------------------------------ public step API
     def decode_forward(self, rows: int) -> torch.Tensor:
         """Run one decode step over the first `rows` staged inputs; returns out_ids[:rows]."""
@@ -715,4 +754,7 @@ class Qwen35Runner:
         err = int(self.buf["err"].item())
         if not err and self.coll is not None and hasattr(self.coll, "check_error"):
             err = self.coll.check_error()
+        plan = getattr(self, "prefix_plan", None)
+        if not err and plan is not None:
+            err = int(plan.err.item())
         return err
