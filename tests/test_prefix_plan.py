@@ -58,6 +58,21 @@ def test_a_failed_plan_shows_in_the_runners_error(host):
     assert host.check_error() == 1
 
 
+def test_rows_that_are_not_the_plans_are_refused(host):
+    host.host_inputs, host._staged_rows = torch.zeros(4, 4, dtype=torch.int32), 3
+    host.host_inputs[2] = torch.tensor([5, 0, 1, 9])
+    host.check_plan_rows(4)
+    host.prefix_plan = plan_of([5, 0, 1, 2])
+    host.check_plan_rows(4)              # the fourth row is not staged: padding
+    host.check_plan_rows(2)
+    for slots in ([0, 5, 1, 2], [5, 0], [5, 0, 2, 1]):
+        host.prefix_plan = plan_of(slots)
+        with pytest.raises(ValueError, match="staged"):
+            host.check_plan_rows(4)
+    host.host_inputs[2, 2] = 2           # checked with every step
+    host.check_plan_rows(4)
+
+
 @pytest.fixture(scope="module")
 def four():
     """Four sequences behind one 64-token prompt, each with its own pages, and their state."""
@@ -102,6 +117,24 @@ def test_each_plan_is_the_one_that_runs(four):
         for a, b in zip(first, decode(four)):
             torch.testing.assert_close(a, b, rtol=5e-2, atol=5e-2)
         assert [bool(p._partial.isnan().all()) for p in plans] == [p is not plan for p in plans]
+    r.prefix_plan = None
+
+
+@gpu
+def test_a_batch_in_another_order_is_refused(four):
+    """Before a graph of the plan is there, and when it is; the runner goes on with the right order."""
+    r = four[0]
+    first = decode(four)
+    r.prefix_plan = SharedPrefixPlan.from_prefixes(list(range(4)), [([0, 1, 2, 3], 4)], r.hq, r.hkv)
+    for _ in range(2):
+        r.stage([11, 12, 13, 14], [64] * 4, [1, 0, 2, 3])
+        with pytest.raises(ValueError, match="staged"):
+            r.decode_step(4)
+        for a, b in zip(first, decode(four)):
+            torch.testing.assert_close(a, b, rtol=5e-2, atol=5e-2)
+    r.stage([1], [66], [1], seq_start=[0, 1])
+    with pytest.raises(ValueError, match="staged"):
+        r.prefill_forward(1, 1)
     r.prefix_plan = None
 
 

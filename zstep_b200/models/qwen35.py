@@ -471,6 +471,7 @@ class Qwen35Runner:
         pos, slot, lens = b["in_pos"][:rows], b["in_slot"][:rows], b["in_len"][:rows]
         plan = self.prefix_plan
         if plan is not None:
+            self.check_plan_rows(rows)
             plan.update(lens)
         C.embed_rmsnorm_quant(b["in_ids"][:rows], self.embed, b["hidden"], self.layers[0]["input_norm"], 1.0,
                               self.eps, rows, None, b["xq"], b["xsf"])
@@ -589,6 +590,12 @@ class Qwen35Runner:
             yield
         finally:
             self._prefix_plan = held
+
+    def check_plan_rows(self, rows: int) -> None:
+        """A plan is for rows in one order: those staged have to be the plan's first ones."""
+        plan, n = self.prefix_plan, min(rows, getattr(self, "_staged_rows", 0))
+        if plan is not None and self.host_inputs[2, :n].tolist() != plan.slot_list[:n]:
+            raise ValueError("the staged rows are not the sequences, in their order, that the prefix plan was made for")
 
     def _drop_graphs(self) -> None:
         held = [g for g in (self.graphs, getattr(self.spec, "g_graphs", None)) if g]
@@ -726,7 +733,8 @@ class Qwen35Runner:
     def capture_decode_graph(self, bucket: int) -> None:
         """Capture one decode step over `bucket` rows into a CUDA graph."""
         b = self.buf
-        saved = b["inputs"].clone()
+        saved, staged = b["inputs"].clone(), getattr(self, "_staged_rows", 0)
+        self._staged_rows = 0
         self.pad_decode_inputs(0, bucket)
         s = torch.cuda.Stream(self.dev)
         s.wait_stream(torch.cuda.current_stream(self.dev))
@@ -739,6 +747,7 @@ class Qwen35Runner:
             self.decode_forward(bucket)
         self.graphs[bucket] = g
         b["inputs"].copy_(saved)  # capture ran on dummy rows; restore the staged step
+        self._staged_rows = staged
 
     def decode_step(self, n: int) -> torch.Tensor:
         """Replay the graph of the bucket that fits n staged rows (captured on demand)."""
@@ -747,6 +756,8 @@ class Qwen35Runner:
         if bucket not in self.graphs:
             self.capture_decode_graph(bucket)
             self.pad_decode_inputs(n, bucket)
+        if getattr(self, "prefix_plan", None) is not None:
+            self.check_plan_rows(n)
         self.graphs[bucket].replay()
         return self.buf["out_ids"][:n]
 

@@ -217,6 +217,7 @@ class SpecDecoder:
             b["inputs"].copy_(saved[0])
             b["seq_start"].copy_(saved[1])
             self.out_slots.copy_(saved[2])
+        self.r.check_plan_rows(nb * (self.K + 1))
         self.g_graphs[nb].replay()
 
     # ------------------------------------------------------------------ MTP head

@@ -75,6 +75,7 @@ class SharedPrefixPlan:
         self.C = _ext.load()
         self.rows, self.num_q_heads, self.num_kv_heads = rows, num_q_heads, num_kv_heads
         self.device = torch.device(device)
+        self.slot_list = list(slots)
         self.max_slot = max(slots, default=0)
         self.levels = max((len(e) for e in row_entry), default=1)
         i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
