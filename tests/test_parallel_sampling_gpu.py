@@ -8,6 +8,8 @@ from zstep_b200.config import Qwen35Config, qwen35_small_gpu
 from zstep_b200.ops import mx
 from zstep_b200.models.parallel_sampling import ParallelSampler, prompt_lookup
 
+PAGE = 16
+
 
 def test_prompt_lookup():
     assert prompt_lookup([1, 2, 3, 9, 1, 2, 3], 2) == [9, 1]
@@ -119,6 +121,71 @@ def test_ends_free_what_only_they_used(runner):
     s.pool.free(torch.tensor([0, 1], dtype=torch.int32, device="cuda"))
     s.pool.check()
     assert s.pool.refcount.tolist() == [1] + [0] * (s.pool.num_pages - 1)
+
+
+def _prompts(lens, seed):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randint(0, 4096, (n,), generator=g).tolist() for n in lens]
+
+
+def _own_pages(s, slots):
+    """What every sample writes to next is its own page."""
+    table, lens, ref = s.pool.page_table.tolist(), s.pool.seq_len.tolist(), s.pool.refcount.tolist()
+    for x in slots:
+        assert lens[x] == len(s.tokens[x]) - 1
+        if lens[x] % PAGE:
+            assert ref[table[x][lens[x] // PAGE]] == 1
+
+
+@pytest.mark.gpu
+def test_a_sampler_starts_again(runner):
+    """Shorter, longer and regrouped prompts in the slots of earlier ones say what a new sampler says."""
+    s, slots = _start(runner, lens=(150, 40), samples=3)
+    s.step(slots, 0.0)
+    s.finish(slots)
+    for seed, (lens, samples) in enumerate([((60, 40), 3), ((60, 90), 3), ((33, 20, 47), 2)]):
+        prompts = _prompts(lens, seed)
+        slots = s.start(prompts, samples)
+        assert s.pool.seq_len[slots].tolist() == [n - 1 for n in lens for _ in range(samples)]
+        drafts = [[1, 2, 3] for _ in slots]
+        _same_attention(s, slots, drafts)
+        said = {x: [] for x in slots}
+        for _ in range(4):
+            for x, t in zip(slots, s.step(slots, 0.0)):
+                said[x] += t
+            _own_pages(s, slots)
+        new = ParallelSampler(runner, 3)
+        again = new.start(prompts, samples)
+        for _ in range(4):
+            new.step(again, 0.0)
+        assert [said[x] for x in slots] == [new.tokens[x][n:] for x, n in zip(again, (n for n in lens for _ in range(samples)))]
+        new.finish(again)
+        runner.page_table = s.pool.page_table
+        s.finish(slots)
+    assert s.start([], 1) == []          # nothing but what ended is given back
+    assert s.pool.refcount.tolist() == [1] + [0] * (s.pool.num_pages - 1)
+
+
+@pytest.mark.gpu
+def test_samples_go_on_while_others_start(runner):
+    s, first = _start(runner, lens=(70,), samples=4)
+    for _ in range(2):
+        s.step(first, 0.0)
+    second = s.start(_prompts((33, 50), 4), 2)
+    assert not set(first) & set(second) and len(set(second)) == 4
+    with pytest.raises(ValueError, match="slots"):
+        s.start(_prompts((10,), 5), 5)   # 11 of 16 slots are taken
+    both = first + second
+    _same_attention(s, both, [[4, 5, 6] for _ in both])
+    for _ in range(3):
+        s.step(both, 0.0)
+        _own_pages(s, both)
+    assert all(s.tokens[x] == s.tokens[first[0]] for x in first)
+    s.finish(first)
+    third = s.start(_prompts((20,), 6), 4)
+    assert not set(third) & set(second)
+    s.step(third + second, 0.0)
+    s.finish(third + second)
 
 
 @pytest.mark.gpu

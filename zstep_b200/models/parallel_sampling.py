@@ -46,23 +46,34 @@ class ParallelSampler:
         self.pool = PagePool(runner.paged_caches(), runner.num_slots, runner.max_pages, runner.page_size)
         runner.page_table = self.pool.page_table
         # Padding rows of a step point at the dummy slot, whose table row stays at the padding page.
-        self.tokens: dict[int, list[int]] = {}   # slot -> prompt and generated tokens
-        self.prompt_of: dict[int, int] = {}      # sample slot -> pages that it shares with its prompt, by prompt
+        self.tokens: dict[int, list[int]] = {}   # sample slot -> prompt and generated tokens
+        self.prompt_of: dict[int, int] = {}      # sample slot -> its prompt's slot
+        self.prompt_pages: dict[int, int] = {}   # prompt slot -> pages that its samples share
         self._plan_key = None
 
     def _ints(self, x) -> torch.Tensor:
         return torch.tensor(x, dtype=torch.int32, device=self.r.dev)
 
     def start(self, prompts: list[list[int]], samples: int) -> list[int]:
-        """Prefill each prompt into a slot and fork it into ``samples`` sample slots; returns those slots."""
+        """Prefill each prompt into a slot and fork it into ``samples`` sample slots; returns those slots.
+        Samples of earlier calls go on.  A prompt's slot and pages are kept until the first call
+        after its last sample has ended."""
         r, n = self.r, len(prompts)
-        if n * (samples + 1) > r.max_seqs:
-            raise ValueError(f"{n} prompts x {samples} samples need {n * (samples + 1)} of {r.max_seqs} slots")
+        living = {self.prompt_of[s] for s in self.tokens}
+        taken = living | set(self.tokens)
+        free = [s for s in range(r.max_seqs) if s not in taken]
+        if n * (samples + 1) > len(free):
+            raise ValueError(f"{n} prompts x {samples} samples need {n * (samples + 1)} of {len(free)} slots")
+        ended = [p for p in self.prompt_pages if p not in living]
+        self.pool.free(self._ints(ended))
+        for p in ended:
+            del self.prompt_pages[p]
+        parents, kids = free[:n], free[n:n * (samples + 1)]
         # The last prompt token is the first step's input: its row comes with the drafts.
         ids = [t for p in prompts for t in p[:-1]]
         pos = [i for p in prompts for i in range(len(p) - 1)]
-        slots = [s for s, p in enumerate(prompts) for _ in p[:-1]]
-        self.pool.extend(self._ints(list(range(n))), self._ints([len(p) - 1 for p in prompts]))
+        slots = [s for s, p in zip(parents, prompts) for _ in p[:-1]]
+        self.pool.extend(self._ints(parents), self._ints([len(p) - 1 for p in prompts]))
         starts = [0]
         for p in prompts:
             starts.append(starts[-1] + len(p) - 1)
@@ -70,19 +81,20 @@ class ParallelSampler:
             r.stage(ids, pos, slots, seq_start=starts)
             with r.eager_plan(None):
                 r._layers(len(ids), decode=False, num_seqs=n)
-        kids = list(range(n, n + n * samples))
-        parent = [s for s in range(n) for _ in range(samples)]
+        parent = [s for s in parents for _ in range(samples)]
         self.pool.fork(self._ints(parent), self._ints(kids))
         self.pool.check()
-        for s, p in zip(kids, parent):
-            self.tokens[s] = list(prompts[p])
+        for s, p in zip(parents, prompts):
+            self.prompt_pages[s] = (len(p) - 1) // r.page_size
+        for i, (s, p) in enumerate(zip(kids, parent)):
+            self.tokens[s] = list(prompts[i // samples])
             self.prompt_of[s] = p
-        self.prompt_pages = {s: (len(prompts[s]) - 1) // r.page_size for s in range(n)}
         return kids
 
     def _plan(self, slots: list[int]) -> SharedPrefixPlan:
-        """Who shares what: changes only when samples end."""
-        if self._plan_key != tuple(slots):
+        """Who shares what: changes only when samples end or start."""
+        key = tuple((s, self.prompt_of[s], self.prompt_pages[self.prompt_of[s]]) for s in slots)
+        if self._plan_key != key:
             rows = [s for s in slots for _ in range(self.k + 1)]
             groups: dict[int, list[int]] = {}
             for i, s in enumerate(rows):
@@ -90,7 +102,7 @@ class ParallelSampler:
             prefixes = [(members, self.prompt_pages[p]) for p, members in groups.items()]
             self.plan = SharedPrefixPlan.from_prefixes(rows, prefixes, self.r.hq, self.r.hkv, device=self.r.dev)
             self.verifier = DraftVerifier(len(slots), self.k, self.r.cfg.vocab_size, device=self.r.dev)
-            self._plan_key = tuple(slots)
+            self._plan_key = key
         return self.plan
 
     def logits(self, slots: list[int], drafts: list[list[int]], shared: bool = True) -> torch.Tensor:
@@ -140,6 +152,8 @@ class ParallelSampler:
         self.pool.check()
         self.verifier.check()
         self.plan.check()
+        for s in slots:
+            del self.prompt_of[s]
         return [self.tokens.pop(s) for s in slots]
 
 
