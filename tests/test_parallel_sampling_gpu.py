@@ -189,6 +189,46 @@ def test_samples_go_on_while_others_start(runner):
 
 
 @pytest.mark.gpu
+def test_a_step_that_pages_run_short_for_adds_nothing():
+    """39 pages: prompts of 8 each, 12 samples that need a page each with the first step."""
+    from zstep_b200.models.qwen35 import Qwen35Runner
+
+    cfg = Qwen35Config(vocab_size=4096, num_hidden_layers=2, layer_types=("full_attention",) * 2, num_experts=16,
+                       mtp_num_hidden_layers=0, name="attention-only")
+    s = ParallelSampler(Qwen35Runner(cfg, max_seqs=16, max_prefill_tokens=256, num_pages=40, max_model_len=256), 3)
+    prompts = _prompts((129, 129), 7)
+
+    def steps(slots, n):
+        for _ in range(n):
+            s.step(slots, 0.0, drafts=[[] for _ in slots])
+
+    slots = s.start(prompts, 6)
+    steps(slots, 6)
+    want = [s.tokens[x] for x in slots]
+    s.finish(slots)
+    slots = s.start(prompts, 6)
+    hog = torch.tensor([s.pool.num_slots - 1], dtype=torch.int32, device="cuda")   # no request's slot takes 16 of 23
+    s.pool.extend(hog, torch.full_like(hog, 256))
+    s.pool.check()
+    state = s.pool.state.clone()
+    short = pytest.raises(RuntimeError, match="few free pages")
+    for _ in range(2):
+        with short:
+            steps(slots, 1)
+        assert [s.tokens[x] for x in slots] == [p for p in prompts for _ in range(6)]
+        assert torch.equal(state, s.pool.state)
+    for n in (130, 98):   # 9 pages; the last 7, and then a copy of the last one
+        with short:
+            s.start(_prompts((n,), 8), 1)
+        assert torch.equal(state, s.pool.state) and len(s.prompt_pages) == 2
+    s.finish(slots[:3] + slots[6:9])
+    left = slots[3:6] + slots[9:]
+    steps(left, 6)        # six pages: enough for these, as if nothing had been
+    assert [s.tokens[x] for x in left] == want[3:6] + want[9:]
+    s.finish(left)
+
+
+@pytest.mark.gpu
 def test_refusals(runner):
     from zstep_b200.models.qwen35 import Qwen35Runner
 

@@ -74,6 +74,7 @@ class ParallelSampler:
         pos = [i for p in prompts for i in range(len(p) - 1)]
         slots = [s for s, p in zip(parents, prompts) for _ in p[:-1]]
         self.pool.extend(self._ints(parents), self._ints([len(p) - 1 for p in prompts]))
+        self.pool.check()   # short of pages, no slot has grown
         starts = [0]
         for p in prompts:
             starts.append(starts[-1] + len(p) - 1)
@@ -83,7 +84,11 @@ class ParallelSampler:
                 r._layers(len(ids), decode=False, num_seqs=n)
         parent = [s for s in parents for _ in range(samples)]
         self.pool.fork(self._ints(parent), self._ints(kids))
-        self.pool.check()
+        try:
+            self.pool.check()
+        except RuntimeError:
+            self.pool.free(self._ints(parents))
+            raise
         for s, p in zip(parents, prompts):
             self.prompt_pages[s] = (len(p) - 1) // r.page_size
         for i, (s, p) in enumerate(zip(kids, parent)):
@@ -116,6 +121,7 @@ class ParallelSampler:
             pos += list(range(have, have + k1))
             rows += [s] * k1
         self.pool.extend(self._ints(slots), self._ints([len(self.tokens[s]) + self.k for s in slots]))
+        self.pool.check()   # short of pages, no slot has grown, and rows would have nowhere to go
         r.stage(ids, pos, rows, seq_start=[i * k1 for i in range(n + 1)])
         with r.eager_plan(self._plan(slots) if shared else None):
             r._layers(n * k1, decode=False, num_seqs=n)
@@ -125,7 +131,8 @@ class ParallelSampler:
 
     def step(self, slots: list[int], temperature: float, top_k: int = 0, top_p: float = 1.0,
              generator: torch.Generator | None = None, drafts: list[list[int]] | None = None) -> list[list[int]]:
-        """One verify step; appends to and returns the new tokens of each sample."""
+        """One verify step; appends to and returns the new tokens of each sample.  A step that fails (short
+        of pages) adds nothing: it can be tried again when samples have ended."""
         n, k1 = len(slots), self.k + 1
         if drafts is None:
             drafts = [prompt_lookup(self.tokens[s], self.k) for s in slots]
@@ -138,6 +145,8 @@ class ParallelSampler:
         record = self.verifier.verify(probs.view(n, k1, -1), self._ints([d + [0] * (self.k - len(d)) for d in drafts]),
                                       torch.rand(n, k1, generator=generator, device=dev),
                                       counts=self._ints([len(d) for d in drafts])).tolist()
+        self.verifier.check()
+        self.plan.check()
         new = [rec[1:1 + rec[0]] for rec in record]
         for s, t in zip(slots, new):
             self.tokens[s] += t
