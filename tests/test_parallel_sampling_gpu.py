@@ -229,6 +229,40 @@ def test_a_step_that_pages_run_short_for_adds_nothing():
 
 
 @pytest.mark.gpu
+def test_a_sample_ends_at_its_table_rows_end(runner):
+    s = ParallelSampler(runner, 3)
+    slots = s.start(_prompts((252,), 9), 2) + s.start(_prompts((20,), 10), 2)   # 256 tokens a sequence
+    for _ in range(2):                   # the second one's last draft row is the last of all
+        s.step(slots, 0.0, drafts=[[] for _ in slots])
+    table = s.pool.page_table.clone()
+    with pytest.raises(ValueError, match="256 tokens"):
+        s.step(slots, 0.0, drafts=[[] for _ in slots])
+    with pytest.raises(ValueError, match="256 tokens"):
+        s.logits(slots[:1], [[]])
+    assert torch.equal(table, s.pool.page_table) and len(s.tokens[slots[0]]) == 254
+    s.finish(slots[:2])
+    s.step(slots[2:], 0.0)
+    s.finish(slots[2:])
+
+
+@pytest.mark.gpu
+def test_what_a_step_cannot_take_is_refused(runner):
+    s, slots = _start(runner)
+    state = s.pool.state.clone()
+    for drafts in ([[1]], [[1, 2, 3, 4]] * len(slots), [[4096]] * len(slots), [[-1]] * len(slots)):
+        with pytest.raises(ValueError):
+            s.step(slots, 0.0, drafts=drafts)
+    for prompts in ([[]], [[1, 4096]], [[-1, 2]], [[1] * 257], [[1] * 200, [2] * 200]):
+        with pytest.raises(ValueError):
+            s.start(prompts, 1)
+    with pytest.raises(RuntimeError, match="cannot serve"):   # one sample twice
+        s.step(slots[:1] * 2, 0.0)
+    assert torch.equal(state, s.pool.state)
+    s.step(slots, 0.0)
+    s.finish(slots)
+
+
+@pytest.mark.gpu
 def test_refusals(runner):
     from zstep_b200.models.qwen35 import Qwen35Runner
 

@@ -54,6 +54,11 @@ class ParallelSampler:
     def _ints(self, x) -> torch.Tensor:
         return torch.tensor(x, dtype=torch.int32, device=self.r.dev)
 
+    def _known(self, tokens: list[list[int]]) -> None:
+        vocab = self.r.cfg.vocab_size
+        if any(not 0 <= t < vocab for x in tokens for t in x):
+            raise ValueError(f"a token outside the vocabulary of {vocab}")
+
     def start(self, prompts: list[list[int]], samples: int) -> list[int]:
         """Prefill each prompt into a slot and fork it into ``samples`` sample slots; returns those slots.
         Samples of earlier calls go on.  A prompt's slot and pages are kept until the first call
@@ -64,6 +69,13 @@ class ParallelSampler:
         free = [s for s in range(r.max_seqs) if s not in taken]
         if n * (samples + 1) > len(free):
             raise ValueError(f"{n} prompts x {samples} samples need {n * (samples + 1)} of {len(free)} slots")
+        if any(not p for p in prompts):
+            raise ValueError("a prompt needs at least one token")
+        if max(map(len, prompts), default=0) > r.max_pages * r.page_size:
+            raise ValueError(f"a prompt passes the {r.max_pages * r.page_size} tokens of a sequence")
+        if sum(len(p) - 1 for p in prompts) > r.R:
+            raise ValueError(f"the prompts pass the {r.R} rows of a step")
+        self._known(prompts)
         ended = [p for p in self.prompt_pages if p not in living]
         self.pool.free(self._ints(ended))
         for p in ended:
@@ -114,6 +126,13 @@ class ParallelSampler:
         """f32 logits [len(slots), k + 1, vocab] after the newest token of each sample and after each of its
         drafts (missing drafts are padded with token 0)."""
         r, k1, n = self.r, self.k + 1, len(slots)
+        if len(drafts) != n or any(len(d) > self.k for d in drafts):
+            raise ValueError(f"drafts must be one list of up to {self.k} tokens for each sample")
+        if n * k1 > r.R:
+            raise ValueError(f"{n} samples x {k1} rows pass the {r.R} rows of a step")
+        if max((len(self.tokens[s]) for s in slots), default=0) + self.k > r.max_pages * r.page_size:
+            raise ValueError(f"a sample and its drafts pass the {r.max_pages * r.page_size} tokens of a sequence")
+        self._known(drafts)
         ids, pos, rows = [], [], []
         for s, d in zip(slots, drafts):
             have = len(self.tokens[s]) - 1   # cached tokens
@@ -132,7 +151,7 @@ class ParallelSampler:
     def step(self, slots: list[int], temperature: float, top_k: int = 0, top_p: float = 1.0,
              generator: torch.Generator | None = None, drafts: list[list[int]] | None = None) -> list[list[int]]:
         """One verify step; appends to and returns the new tokens of each sample.  A step that fails (short
-        of pages) adds nothing: it can be tried again when samples have ended."""
+        of pages, past a sequence's end) adds nothing: it can be tried again when samples have ended."""
         n, k1 = len(slots), self.k + 1
         if drafts is None:
             drafts = [prompt_lookup(self.tokens[s], self.k) for s in slots]
