@@ -263,6 +263,18 @@ def test_what_a_step_cannot_take_is_refused(runner):
 
 
 @pytest.mark.gpu
+def test_samples_end_before_any_step(runner):
+    s, slots = _start(runner)
+    state = s.pool.state.clone()
+    for wrong in ([0], [slots[0]] * 2, [slots[0], 15]):   # a prompt's slot, one twice, none
+        with pytest.raises(ValueError, match="samples"):
+            s.finish(wrong)
+    assert torch.equal(state, s.pool.state)
+    assert [len(t) for t in s.finish(slots)] == [70] * 5 + [33] * 5
+    assert not s.tokens and s.finish([]) == []
+
+
+@pytest.mark.gpu
 def test_refusals(runner):
     from zstep_b200.models.qwen35 import Qwen35Runner
 

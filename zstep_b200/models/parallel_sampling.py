@@ -49,7 +49,7 @@ class ParallelSampler:
         self.tokens: dict[int, list[int]] = {}   # sample slot -> prompt and generated tokens
         self.prompt_of: dict[int, int] = {}      # sample slot -> its prompt's slot
         self.prompt_pages: dict[int, int] = {}   # prompt slot -> pages that its samples share
-        self._plan_key = None
+        self.plan = self.verifier = self._plan_key = None   # of the first step on
 
     def _ints(self, x) -> torch.Tensor:
         return torch.tensor(x, dtype=torch.int32, device=self.r.dev)
@@ -175,11 +175,14 @@ class ParallelSampler:
 
     def finish(self, slots: list[int]) -> list[list[int]]:
         """End samples: their pages go back and the live ones move together.  Returns their tokens."""
+        if len(set(slots)) != len(slots) or any(s not in self.tokens for s in slots):
+            raise ValueError(f"not all of {slots} are samples, each once")
+        for x in (self.plan, self.verifier):
+            if x is not None:
+                x.check()
         self.pool.free(self._ints(slots))
         self.pool.compact()
         self.pool.check()
-        self.verifier.check()
-        self.plan.check()
         for s in slots:
             del self.prompt_of[s]
         return [self.tokens.pop(s) for s in slots]
