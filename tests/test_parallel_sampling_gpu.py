@@ -1,12 +1,14 @@
 """Many samples of shared prompts through the runner: attention of the shared-prefix path against
 the per-row path, right drafts accepted and wrong ones taken back, pages returned."""
 
+import json
+
 import pytest
 import torch
 
 from zstep_b200.config import Qwen35Config, qwen35_small_gpu
 from zstep_b200.ops import mx
-from zstep_b200.models.parallel_sampling import ParallelSampler, prompt_lookup
+from zstep_b200.models.parallel_sampling import ParallelSampler, main, prompt_lookup
 
 PAGE = 16
 
@@ -272,6 +274,23 @@ def test_samples_end_before_any_step(runner):
     assert torch.equal(state, s.pool.state)
     assert [len(t) for t in s.finish(slots)] == [70] * 5 + [33] * 5
     assert not s.tokens and s.finish([]) == []
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,temperature", [(1, 0.8), (3, 0.0), (40, 0.0)])
+def test_the_command_ends_every_sample_at_its_length(tokens, temperature, capsys):
+    """Fewer tokens than drafts, and greedy samples of which some run ahead by accepted drafts."""
+    main(["--prompts", "2", "--samples", "2", "--prompt-len", "40", "--tokens", str(tokens), "--layers", "1",
+          "--temperature", str(temperature)])
+    said = json.loads(capsys.readouterr().out.strip().splitlines()[-1])
+    assert said["samples"] == 4 and 1 <= said["steps"] <= tokens
+    assert 4 * tokens <= said["tokens"] <= 4 * (tokens + 3)
+
+
+def test_the_command_refuses_sizes(capsys):
+    for name in ("prompts", "samples", "prompt-len", "tokens", "drafts", "layers"):
+        with pytest.raises(SystemExit):
+            main([f"--{name}", "0"])
 
 
 @pytest.mark.gpu

@@ -188,7 +188,7 @@ class ParallelSampler:
         return [self.tokens.pop(s) for s in slots]
 
 
-def main() -> None:
+def main(argv: list[str] | None = None) -> None:
     from ..config import Qwen35Config
 
     ap = argparse.ArgumentParser()
@@ -201,7 +201,9 @@ def main() -> None:
     ap.add_argument("--temperature", type=float, default=0.8)
     ap.add_argument("--top-k", type=int, default=50)
     ap.add_argument("--top-p", type=float, default=0.95)
-    a = ap.parse_args()
+    a = ap.parse_args(argv)
+    if min(a.prompts, a.samples, a.prompt_len, a.tokens, a.drafts, a.layers) < 1:
+        ap.error("prompts, samples, prompt-len, tokens, drafts and layers must be at least 1")
     cfg = Qwen35Config(vocab_size=8192, num_hidden_layers=a.layers, layer_types=("full_attention",) * a.layers,
                        num_experts=32, name="attention-only")
     seqs = a.prompts * (a.samples + 1)
@@ -213,15 +215,17 @@ def main() -> None:
     prompts = torch.randint(0, cfg.vocab_size, (a.prompts, a.prompt_len), generator=gen, device=runner.dev).tolist()
     sampler = ParallelSampler(runner, a.drafts)
     slots = sampler.start(prompts, a.samples)
-    steps = 0
-    while min(len(sampler.tokens[s]) for s in slots) < a.prompt_len + a.tokens - a.drafts:
+    steps = made = pages = 0
+    while slots:
         sampler.step(slots, a.temperature, a.top_k, a.top_p, gen)
         steps += 1
-    made = sum(len(sampler.tokens[s]) - a.prompt_len for s in slots)
-    pages = int((sampler.pool.refcount > 0).sum())
-    sampler.finish(slots)
-    print(json.dumps({"samples": len(slots), "steps": steps, "tokens": made, "tokens_per_step": round(made / steps, 2),
-                      "pages_in_use": pages, "pages_without_sharing": len(slots) * -(-length // 16)}))
+        done = [s for s in slots if len(sampler.tokens[s]) >= a.prompt_len + a.tokens]
+        if done:
+            pages = max(pages, int((sampler.pool.refcount > 0).sum()))
+            made += sum(len(t) - a.prompt_len for t in sampler.finish(done))
+            slots = [s for s in slots if s in sampler.tokens]
+    print(json.dumps({"samples": a.prompts * a.samples, "steps": steps, "tokens": made, "tokens_per_step": round(made / steps, 2),
+                      "pages_in_use": pages, "pages_without_sharing": a.prompts * a.samples * -(-length // 16)}))
 
 
 if __name__ == "__main__":
