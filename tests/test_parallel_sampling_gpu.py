@@ -277,6 +277,17 @@ def test_samples_end_before_any_step(runner):
 
 
 @pytest.mark.gpu
+def test_a_sampler_whose_runner_has_another_is_refused(runner):
+    s, slots = _start(runner)
+    new, others = _start(runner)
+    for call in (lambda: s.step(slots, 0.0), lambda: s.logits(slots, [[] for _ in slots]), lambda: s.start([[1, 2]], 1)):
+        with pytest.raises(RuntimeError, match="one sampler"):
+            call()
+    new.step(others, 0.0)
+    new.finish(others)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("tokens,temperature", [(1, 0.8), (3, 0.0), (40, 0.0)])
 def test_the_command_ends_every_sample_at_its_length(tokens, temperature, capsys):
     """Fewer tokens than drafts, and greedy samples of which some run ahead by accepted drafts."""

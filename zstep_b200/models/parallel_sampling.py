@@ -54,6 +54,10 @@ class ParallelSampler:
     def _ints(self, x) -> torch.Tensor:
         return torch.tensor(x, dtype=torch.int32, device=self.r.dev)
 
+    def _current(self) -> None:
+        if self.r.page_table is not self.pool.page_table:
+            raise RuntimeError("the runner's page table is no longer this sampler's: one sampler at a time")
+
     def _known(self, tokens: list[list[int]]) -> None:
         vocab = self.r.cfg.vocab_size
         if any(not 0 <= t < vocab for x in tokens for t in x):
@@ -64,6 +68,7 @@ class ParallelSampler:
         Samples of earlier calls go on.  A prompt's slot and pages are kept until the first call
         after its last sample has ended."""
         r, n = self.r, len(prompts)
+        self._current()
         living = {self.prompt_of[s] for s in self.tokens}
         taken = living | set(self.tokens)
         free = [s for s in range(r.max_seqs) if s not in taken]
@@ -126,6 +131,7 @@ class ParallelSampler:
         """f32 logits [len(slots), k + 1, vocab] after the newest token of each sample and after each of its
         drafts (missing drafts are padded with token 0)."""
         r, k1, n = self.r, self.k + 1, len(slots)
+        self._current()
         if len(drafts) != n or any(len(d) > self.k for d in drafts):
             raise ValueError(f"drafts must be one list of up to {self.k} tokens for each sample")
         if n * k1 > r.R:
