@@ -265,6 +265,20 @@ def test_what_a_step_cannot_take_is_refused(runner):
 
 
 @pytest.mark.gpu
+def test_steps_that_cannot_be_planned_change_nothing(runner, monkeypatch):
+    with pytest.raises(ValueError, match="64"):
+        ParallelSampler(runner, 65)
+    s, slots = _start(runner, k=64, samples=2)
+    assert len(s.step(slots[2:3], 0.0, drafts=[[1] * 64])) == 1   # 64 drafts
+    monkeypatch.setattr("zstep_b200.ops.shared_prefix.MAX_SEGS", 2)
+    state = s.pool.state.clone()
+    with pytest.raises(ValueError, match="at most 2 segments"):
+        s.step(slots[:3], 0.0)
+    assert torch.equal(state, s.pool.state)
+    s.finish(slots)
+
+
+@pytest.mark.gpu
 def test_samples_end_before_any_step(runner):
     s, slots = _start(runner)
     state = s.pool.state.clone()

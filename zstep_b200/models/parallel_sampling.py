@@ -20,7 +20,7 @@ import torch
 
 from ..ops.pages import PagePool
 from ..ops.shared_prefix import SharedPrefixPlan
-from ..ops.spec_sampling import DraftVerifier, token_probs
+from ..ops.spec_sampling import MAX_DRAFTS, DraftVerifier, token_probs
 from .qwen35 import EPI_F32, Qwen35Runner
 
 
@@ -40,8 +40,8 @@ class ParallelSampler:
             raise ValueError("forks copy pages, not recurrent state: the model must have attention layers only")
         if runner.tp != 1:
             raise ValueError("one rank only")
-        if num_drafts < 1:
-            raise ValueError("num_drafts must be at least 1")
+        if not 1 <= num_drafts <= MAX_DRAFTS:
+            raise ValueError(f"num_drafts must be at least 1 and at most {MAX_DRAFTS}")
         self.r, self.k = runner, num_drafts
         self.pool = PagePool(runner.paged_caches(), runner.num_slots, runner.max_pages, runner.page_size)
         runner.page_table = self.pool.page_table
@@ -145,10 +145,11 @@ class ParallelSampler:
             ids += [self.tokens[s][-1]] + d + [0] * (self.k - len(d))
             pos += list(range(have, have + k1))
             rows += [s] * k1
+        plan = self._plan(slots) if shared else None
         self.pool.extend(self._ints(slots), self._ints([len(self.tokens[s]) + self.k for s in slots]))
         self.pool.check()   # short of pages, no slot has grown, and rows would have nowhere to go
         r.stage(ids, pos, rows, seq_start=[i * k1 for i in range(n + 1)])
-        with r.eager_plan(self._plan(slots) if shared else None):
+        with r.eager_plan(plan):
             r._layers(n * k1, decode=False, num_seqs=n)
         out = torch.empty(n * k1, r.vocab_local, dtype=torch.float32, device=r.dev)
         r._gemm(r.lm_head, r.buf["xq"], r.buf["xsf"], n * k1, out, r.vocab_local, EPI_F32)
