@@ -756,7 +756,7 @@ bool aligned16(const void* p, long long stride) { return reinterpret_cast<uintpt
 extern "C" int zs_token_probs(const TokenProbsArgs* args, cudaStream_t stream) {
   using namespace zs::spec;
   const TokenProbsArgs& a = *args;
-  if (a.vocab < 1 || a.rows < 0 || a.ld < a.vocab || a.ld_out < a.vocab || a.temperature == nullptr) return -1;
+  if (a.vocab < 1 || a.rows < 0 || a.ld < 0 || a.ld_out < a.vocab || a.temperature == nullptr) return -1;
   if (a.rows == 0) return 0;
   int n = 1;
   while (n < kCluster && (long long)n * kChunk < a.vocab) n *= 2;

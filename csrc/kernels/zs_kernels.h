@@ -632,7 +632,7 @@ int zs_pool_copy(const PagePoolArgs* args, cudaStream_t stream);
 // ----------------------------------------------------------------------------------
 typedef struct TokenProbsArgs {
   const float* logits;       // [rows, ld]; -inf and NaN: masked
-  long long ld;
+  long long ld;              // >= 0: rows may overlap or be the same
   int rows, vocab;
   const float* temperature;  // [rows]; <= 0: all mass on the largest logit (lowest id on ties)
   const int* top_k;          // [rows] (may be NULL); 0: off

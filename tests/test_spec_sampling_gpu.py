@@ -196,6 +196,16 @@ def test_probs_of_many_rows_repeat_beyond_the_candidate_path(vocab, k):
 
 
 @gpu
+@pytest.mark.parametrize("vocab", [1000, 62081])
+def test_probs_of_one_row_under_several_settings(vocab):
+    """Rows that are one row in memory (a stride of 0), and rows that overlap."""
+    x = torch.randn(vocab + 9, generator=torch.Generator().manual_seed(vocab)).cuda() * 4
+    temp, k, p = [0.0, 0.5, 1.0, 2.0], [0, 0, 7, 300], [1.0, 0.9, 1.0, 1.0]
+    for rows in (x[:vocab].expand(4, vocab), x.as_strided((4, vocab), (3, 1))):
+        check_probs(rows, temp, k, p, out=torch.empty(4, vocab, device="cuda"))
+
+
+@gpu
 def test_probs_refusals():
     x, t = torch.zeros(3, 10, device="cuda"), torch.ones(3, device="cuda")
     for args in ((x.half(), t), (x.t(), t), (x, t[:2]), (x, t, t), (x, t, None, t.int()), (x[0], t), (x.cpu(), t)):
