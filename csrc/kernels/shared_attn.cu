@@ -344,7 +344,7 @@ constexpr float kGrow = 8.f;         // O is rescaled when a maximum grows by mo
 // (2^-18 of a weight is lost then).  A single product loses 2^-9 of every weight, and as values of
 // either sign cancel in the output as much as those errors do, that is 2^-9 of the output too, as much
 // again as its own rounding (0.0021 of the result's norm at 2000 and 33000 keys, 0.0017 so).  Left out
-// where no weight is above a quarter of the sum so far, the second product saved 0, 3 and 2 % of a call
+// where no weight is above a quarter of the sum so far, the second product saved 0, 3 and 4 % of a call
 // (eight prompts, the same with four rows a sequence, a long document).  l sums the weights before
 // they are rounded.  A value that is infinite where a row sees it gives NaN, not an infinity.
 // Long pieces run at 1.0 to 1.1 us a tile and CTA; the three products take 0.8 us of it (1536
