@@ -274,6 +274,12 @@ ZS_DEVICE uint32_t pack_bf16(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+// Towards zero, so that what is left of a positive number is not negative.
+ZS_DEVICE uint32_t pack_bf16_down(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
 // c ? x : y, opaque: a chain of them over an array is not turned into an indexed load, which
 // would move the whole array from registers to local memory.
 ZS_DEVICE float pick(bool c, float x, float y) {
@@ -340,13 +346,13 @@ constexpr float kGrow = 8.f;         // O is rescaled when a maximum grows by mo
 //  * softmax warps: P = 2^(s - m) with a reference m that follows the running maximum only when
 //    that grows by more than 2^8 (P stays below 2^8, O and l in fp32), so O in TMEM is rescaled
 //    rarely; the next fragment's Q goes to TMEM during this one's last tile.
-// The tensor cores take P as bf16, so it goes through them twice: rounded, and what the rounding left
-// (2^-18 of a weight is lost then).  A single product loses 2^-9 of every weight, and as values of
+// The tensor cores take P as bf16, so it goes through them twice: cut to bf16, and what the cut left
+// (2^-17 of a weight is lost then).  A single product loses 2^-9 of every weight, and as values of
 // either sign cancel in the output as much as those errors do, that is 2^-9 of the output too, as much
 // again as its own rounding (0.0021 of the result's norm at 2000 and 33000 keys, 0.0017 so).  Left out
 // where no weight is above a quarter of the sum so far, the second product saved 0, 3 and 4 % of a call
 // (eight prompts, the same with four rows a sequence, a long document).  l sums the weights before
-// they are rounded.  A value that is infinite where a row sees it gives NaN, not an infinity.
+// they are cut.  Both parts are positive, so that an infinite value that a row sees stays that infinity.
 // Long pieces run at 1.0 to 1.1 us a tile and CTA; the three products take 0.8 us of it (1536
 // clocks at 4096 multiply-adds a clock).  A copy takes 2 us from its issue to its S, and two of K are on
 // their way at a time; S and P in places of their own, so that the next S need not wait for O, gave
@@ -716,16 +722,16 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const SharedAttnArgs 
             const float lo = ex2(fmaf(__uint_as_float(r[2 * j]), qscale, -off));
             const float hi = ex2(fmaf(__uint_as_float(r[2 * j + 1]), qscale, -off));
             sum[j & 3] += lo + hi;
-            pk[j] = pack_bf16(lo, hi);
+            pk[j] = pack_bf16_down(lo, hi);
             r[2 * j] = __float_as_uint(lo);
             r[2 * j + 1] = __float_as_uint(hi);
           }
           tmem_st_32x32b_x16(lanes + b * TILE + half * 16, pk);
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
+          for (int j = 0; j < 16; ++j)  // above 0 by the smallest step at least: an infinite value times 0 would be NaN
             pk[j] = pack_bf16(__uint_as_float(r[2 * j]) - __uint_as_float(pk[j] << 16),
-                              __uint_as_float(r[2 * j + 1]) - __uint_as_float(pk[j] & 0xFFFF0000u));
+                              __uint_as_float(r[2 * j + 1]) - __uint_as_float(pk[j] & 0xFFFF0000u)) | 0x00010001u;
           tmem_st_32x32b_x16(lanes + b * TILE + 32 + half * 16, pk);
           tmem_st_wait();
         }

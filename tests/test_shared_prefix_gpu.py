@@ -204,6 +204,25 @@ def test_scores_that_are_all_nan_are_not_taken_for_no_keys(prefix):
 
 
 @gpu
+@pytest.mark.parametrize("keys", [(5,), (40, 200), (527,), (900, 1033)])
+def test_infinite_values_that_rows_see_stay_infinite(keys):
+    """In the prefix's first tiles, in later ones, and among own tokens that not every row sees."""
+    b = Batch(16, 2, [64], [seq(0, 1024, 30, 4), seq(0, 1024, 9), seq(0, 1024, 70)], seed=21)
+    for i, t in enumerate(keys):
+        b.v[b.table[0, t // PAGE], :, t % PAGE, 10 + i] = float("inf")
+        b.v[b.table[0, t // PAGE], 1, t % PAGE, 20 + i] = float("-inf")
+    y, a = b.want()
+    y, n = y.view(-1, 16, D), len(keys)
+    assert y[3, :, 10:10 + n].isinf().all() and y[3, 8:, 20:20 + n].isinf().all()
+    assert not y.isnan().any()
+    out = run(b).cpu().double().view_as(y)
+    inf = y.isinf()
+    assert torch.equal(out[inf], y[inf])
+    tol = (2.0 ** -9 * (a.view_as(y) + 2 * y.abs()) + 1e-4 * a.view_as(y) + 1e-30)
+    assert ((out - y).abs() <= tol)[~inf].all()
+
+
+@gpu
 def test_scores_that_are_all_minus_infinity():
     """Keys that a row sees, all with a score of -inf, are no empty mask: 0 / 0.  Beside finite ones they weigh nothing."""
     b = Batch(16, 2, [2], [(None, 33, [33]), (0, 40, [0, 40])], seed=19)
