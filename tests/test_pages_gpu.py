@@ -307,6 +307,19 @@ def test_calls_in_a_graph_and_on_another_stream():
     same(pool, m)
 
 
+def test_adopt_refuses_lengths_below_zero():
+    """Such a slot could neither be filled nor cut nor freed."""
+    pool, m = make(20, 3, 4)
+    both(pool, m, "extend", [1], [20])
+    with pytest.raises(ValueError, match="negative"):
+        pool.adopt(ints([0, -1, 5]), ints([[0], [0], [3]]))
+    same(pool, m)
+    for call in (lambda: pool.free(None), lambda: pool.fork(None, None), lambda: pool.copy(ints([1]), None)):
+        with pytest.raises(ValueError):   # not taken for a call without requests
+            call()
+    same(pool, m)
+
+
 def test_large_caches():
     """Page offsets that pass 2^31 elements and 2^32 bytes."""
     pages = (1 << 32) // (PAGE * 256 * 2) + 70

@@ -76,6 +76,8 @@ class PagePool:
             raise ValueError("adopt: a page id outside the pool")
         if int(seq_len.max()) > width * self.page_size:
             raise ValueError("adopt: a sequence is longer than its table row")
+        if int(seq_len.min()) < 0:
+            raise ValueError("adopt: a negative length")
         self.page_table.zero_()
         self.page_table[:, :width].copy_(torch.where(used, page_table.to(self.state.device), 0))
         self.seq_len.copy_(seq_len)
@@ -84,6 +86,8 @@ class PagePool:
         self._count_free()
 
     def _call(self, which: int, slots=None, parents=None, lens=None) -> None:
+        if which != COMPACT and (slots is None or which in (FORK, COPY) and parents is None):
+            raise ValueError("a page pool call needs its slots (or pages)")
         self.C.pool_call(which, self.refcount, self.free_bits, self.seq_len, self.page_table, self.page_size,
                          self.caches, slots, parents, lens, self._scratch, self.err)
 
