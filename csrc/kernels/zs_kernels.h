@@ -717,6 +717,67 @@ int zs_ipc_handle(void* ptr, void* handle_out);
 int zs_ipc_open(const void* handle, void** ptr);
 int zs_ipc_close(void* ptr);
 
+// ----------------------------------------------------------------------------------
+// K/V cache held in 4 or 8 bits (quant_cache.cu).  One layer: [pages][kv_heads][page / 16 blocks].
+// ----------------------------------------------------------------------------------
+#define ZS_QUANT_CTAS 296   // most CTAs of zs_quant_attn
+
+typedef struct QuantRowsArgs {
+  uint8_t* data;            // the layer
+  int num_pages, num_kv_heads, head_dim, bits;
+  int page_shift;           // log2 of the tokens of a page, 4..8
+  int rows;
+  const int* slots;         // [rows] page-table row
+  const int* positions;     // [rows]; negative: no place (nothing is stored, zeros are read)
+  const int* page_table;    // [num_slots, max_pages]
+  int num_slots, max_pages;
+  const void* k;            // store: rows read; load: rows written (dims contiguous, 16-byte aligned)
+  const void* v;
+  long long k_row, k_head, v_row, v_head;   // strides in elements
+  int half;                 // f16 instead of bf16
+  int f32;                  // load: f32
+  int* err;
+} QuantRowsArgs;
+
+int zs_quant_block_bytes(int head_dim, int bits);   // of 16 tokens of a kv head
+int zs_quant_store(const QuantRowsArgs* args, cudaStream_t stream);
+int zs_quant_load(const QuantRowsArgs* args, cudaStream_t stream);
+
+typedef struct QuantAttnArgs {
+  const uint8_t* data;
+  int num_pages, num_kv_heads, head_dim, bits, page_shift;
+  int num_q_heads;
+  int rows, max_rows;       // of this step; of the workspace
+  int num_seqs;
+  int max_seq_rows;         // most rows of a sequence
+  const int* slots;         // [rows]
+  const int* seq_lens;      // [rows] keys that the row sees
+  const int* seq_start;     // [num_seqs + 1] rows of the sequences; NULL: a row each
+  const int* page_table;    // [num_slots, max_pages]
+  int num_slots, max_pages;
+  const void* q;            // [rows, heads, dim], strides in elements
+  long long q_row, q_head;
+  const void* gate;         // like q, or NULL
+  long long gate_row, gate_head;
+  int half;                 // f16 instead of bf16
+  float sm_scale;
+  int tiles, slot_warps;    // zs_quant_attn_shape
+  int chunk;                // slots of a unit: 8 * tiles * slot_warps
+  int max_chunks;
+  void* work;               // zs_quant_attn_work bytes, 32-byte aligned
+  float* partial;           // (max_chunks * kv_heads + ZS_QUANT_CTAS) * chunk * (dim + 2)
+  void* out;                // [rows, heads * dim] like q, or NULL
+  uint8_t* out_q;           // MXFP8 of the same, or NULL
+  uint8_t* out_sf;
+  int ring, ring_offset, grid;   // set by the launcher
+  int* err;
+} QuantAttnArgs;
+
+void zs_quant_attn_shape(int head_dim, int slots, int* tiles, int* slot_warps);
+long long zs_quant_attn_work(int max_chunks, int max_rows, int max_seqs);
+int zs_quant_attn_plan(const QuantAttnArgs* args, cudaStream_t stream);   // once a step
+int zs_quant_attn(const QuantAttnArgs* args, cudaStream_t stream);        // once a layer
+
 #ifdef __cplusplus
 }
 #endif

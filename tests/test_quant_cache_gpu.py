@@ -1,0 +1,492 @@
+"""The K/V cache held in 4 or 8 bits: rows written and read back, and attention over it."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from zstep_b200.ops.pages import PagePool
+from zstep_b200.ops.quant_cache import QuantAttention, QuantCache
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def _bf16_beside(x, up):
+    """The nearest bf16 not below (up) or not above 64-bit numbers; exact down to 2^-126."""
+    m, e = np.frexp(x)
+    return np.ldexp((np.ceil if up else np.floor)(np.ldexp(m, 8)), e - 8)
+
+
+def quantised(x, bits):
+    """What a cache holds of rows [n, heads, dim], in 64 bits: values and their scales and offsets."""
+    f = x.double().cpu().numpy().reshape(*x.shape[:2], -1, 64)
+    z = _bf16_beside(f.min(-1, keepdims=True), False)
+    s = _bf16_beside((f.max(-1, keepdims=True) - z) / (2 ** bits - 1), True)
+    with np.errstate(divide="ignore", invalid="ignore"):
+        n = np.where(s > 0, np.rint((f - z) / s), 0.0)
+    n = np.minimum(n, 2 ** bits - 1)
+    return (n * s + z).reshape(x.shape), s, z
+
+
+def rows_of(n, heads, dim, dtype, seed, scale=1.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    size = torch.exp(torch.randn(heads, dim, generator=g, device=DEV) * 0.5)
+    return (scale * size * (torch.randn(n, heads, dim, generator=g, device=DEV) + torch.randn(heads, dim, generator=g, device=DEV))).to(dtype)
+
+
+def table_of(lens, page, seed=0, spare=1):
+    """Shuffled pages (from 1) for sequences of these lengths; (page_table, pages in all)."""
+    need = [max(1, -(-n // page)) for n in lens]
+    ids = np.random.default_rng(seed).permutation(sum(need)) + 1
+    t = np.zeros((len(lens), max(need) + spare), dtype=np.int32)
+    at = 0
+    for i, k in enumerate(need):
+        t[i, :k] = ids[at:at + k]
+        at += k
+    return torch.from_numpy(t).to(DEV), sum(need) + 1
+
+
+def places_of(lens):
+    return _i32(np.repeat(np.arange(len(lens)), lens)), _i32(np.concatenate([np.arange(n) for n in lens] + [np.zeros(0)]).astype(int))
+
+
+# ------------------------------------------------------------------------------ write, read
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_rows_read_back(bits, dim, page, dtype):
+    lens, heads = [1, 17, 130], 3
+    table, pages = table_of(lens, page)
+    slots, pos = places_of(lens)
+    k, v = rows_of(len(slots), heads, dim, dtype, 1), rows_of(len(slots), heads, dim, dtype, 2, 0.01)
+    cache = QuantCache(2, pages, heads, dim, bits=bits, page_size=page)
+    cache.write(1, k, v, table, slots, pos)
+    got = cache.read(1, table, slots, pos, dtype=torch.float32)
+    cache.check()
+    for x, y in zip((k, v), got):
+        want, s, z = quantised(x, bits)
+        # The 32-bit sum s n + z is rounded once.
+        assert np.all(np.abs(y.double().cpu().numpy() - want) <= 2.0 ** -24 * np.abs(want))
+        # And what is held is within half a step and a rounding of what was written.
+        step = np.repeat(s, 64, -1).reshape(x.shape)
+        assert np.all(np.abs(x.double().cpu().numpy() - want) <= step * (0.5 + 2.0 ** -20))
+    for t in (torch.bfloat16, torch.float16):
+        for a, b in zip(cache.read(1, table, slots, pos, dtype=t), got):
+            assert torch.equal(a, b.to(t))
+    assert not cache.data[0].any()   # the other layer is as it was
+
+
+def test_strided_rows_and_given_outputs():
+    heads, dim, n = 2, 128, 21
+    table, pages = table_of([n], 16)
+    slots, pos = places_of([n])
+    whole = rows_of(n, 3 * heads + 1, dim, torch.bfloat16, 3)
+    k, v = whole[:, 1:1 + heads], whole[:, 2:2 + 2 * heads:2]
+    a, b = QuantCache(1, pages, heads, dim), QuantCache(1, pages, heads, dim)
+    a.write(0, k, v, table, slots, pos)
+    b.write(0, k.contiguous(), v.contiguous(), table, slots, pos)
+    assert torch.equal(a.data, b.data)
+    out = torch.full((n, 2 * heads + 1, dim), 7.0, dtype=torch.float16, device=DEV)
+    a.read(0, table, slots, pos, k=out[:, :heads], v=out[:, heads + 1:])
+    want = b.read(0, table, slots, pos, dtype=torch.float16)
+    assert torch.equal(out[:, :heads], want[0]) and torch.equal(out[:, heads + 1:], want[1])
+    assert bool((out[:, heads] == 7).all())
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_special_groups(bits):
+    """Constant, tiny, huge and non-finite groups; each spoils only itself."""
+    dim, heads = 256, 1
+    x = rows_of(8, heads, dim, torch.bfloat16, 4)
+    x[0, 0, :64] = 0.0
+    x[0, 0, 64:128] = -3.25
+    x[1, 0, 5] = float("nan")
+    x[2, 0, 70] = float("inf")
+    x[3, 0, 200] = float("-inf")
+    x[4, 0, 64:128] *= 2.0 ** -100
+    x[5, 0, :64] *= 2.0 ** 100
+    x[6, 0, 128:192] = 0.0
+    x[6, 0, 130] = 2.0 ** -133           # the smallest bf16: N steps do not fit under it
+    x[7, 0, 3] = 2.0 ** 127
+    table, pages = table_of([8], 16)
+    slots, pos = places_of([8])
+    cache = QuantCache(1, pages, heads, dim, bits=bits)
+    cache.write(0, x, x.flip(0), table, slots, pos)
+    k, v = (t.double().cpu().numpy() for t in cache.read(0, table, slots, pos, dtype=torch.float32))
+    bad = np.zeros((8, 1, 4), dtype=bool)
+    bad[1, 0, 0] = bad[2, 0, 1] = bad[3, 0, 3] = bad[7, 0, 0] = True
+    bad = np.repeat(bad, 64, -1)
+    want, s, _ = quantised(x, bits)
+    step = np.repeat(s, 64, -1).reshape(x.shape)
+    raw = x.double().cpu().numpy()
+    for got, flip in ((k, False), (v, True)):
+        got = got[::-1] if flip else got
+        assert np.isnan(got[bad]).all() and np.isfinite(got[~bad]).all()
+        ok = ~bad
+        ok[6, 0, 128:192] = False        # s is a subnormal there: looked at below
+        assert np.all(np.abs(got - want)[ok] <= 2.0 ** -24 * np.abs(want)[ok])
+        assert np.all(np.abs(got - raw)[ok] <= step[ok] * (0.5 + 2.0 ** -20))
+        assert np.abs(got[6, 0, 128:192]).max() <= 2.0 ** -132
+    assert np.all(k[0, 0, :64] == 0) and np.all(k[0, 0, 64:128] == -3.25)
+
+
+def test_rows_without_a_place():
+    heads, dim = 2, 64
+    table, pages = table_of([16], 16)
+    cache = QuantCache(1, pages, heads, dim)
+    x = rows_of(4, heads, dim, torch.bfloat16, 5)
+    cache.write(0, x, x, table, _i32([0, 0, 0, 0]), _i32([3, -1, -7, 4]))
+    k, _ = cache.read(0, table, _i32([0, 0, 0, 0, 0]), _i32([3, 4, -1, 5, 0]), dtype=torch.float32)
+    cache.check()
+    want = quantised(x, 4)[0]
+    assert np.allclose(k[:2].double().cpu().numpy(), want[[0, 3]], rtol=2.0 ** -23, atol=0) and not k[2:].any()
+    before = cache.data.clone()
+    for slots, pos, tab in (([1], [0], table), ([-1], [0], table), ([0], [32], table), ([0], [0], torch.full_like(table, pages)),
+                            ([0], [0], torch.full_like(table, -1))):
+        cache.write(0, x[:1], x[:1], tab, _i32(slots), _i32(pos))
+        with pytest.raises(RuntimeError, match="outside the cache"):
+            cache.check()
+        k, v = cache.read(0, tab, _i32(slots), _i32(pos))
+        assert not k.any() and not v.any()
+        with pytest.raises(RuntimeError, match="outside the cache"):
+            cache.check()
+    cache.check()
+    assert torch.equal(cache.data, before)
+    cache.write(0, x[:0], x[:0], table, _i32([]), _i32([]))
+    assert cache.read(0, table, _i32([]), _i32([]))[0].shape == (0, heads, dim)
+
+
+# -------------------------------------------------------------------------------- attention
+def filled(lens, heads, dim, bits, page=16, dtype=torch.bfloat16, seed=0, v_scale=1.0):
+    """A cache of sequences of these lengths whose other tokens hold poison."""
+    table, pages = table_of(lens, page, seed)
+    cache = QuantCache(1, pages, heads, dim, bits=bits, page_size=page)
+    every = torch.arange(pages, dtype=torch.int32, device=DEV)[None]
+    all_pos = torch.arange(pages * page, dtype=torch.int32, device=DEV)
+    nan = torch.full((pages * page, heads, dim), float("nan"), dtype=dtype, device=DEV)
+    cache.write(0, nan, nan, every, torch.zeros_like(all_pos), all_pos)
+    slots, pos = places_of(lens)
+    if len(slots):
+        cache.write(0, rows_of(len(slots), heads, dim, dtype, seed + 10), rows_of(len(slots), heads, dim, dtype, seed + 11, v_scale),
+                    table, slots, pos)
+    cache.check()
+    return cache, table
+
+
+def reference(cache, table, q, slots, lens, scale, gate=None):
+    """Attention over what the cache holds in 64 bits, and a bound of what the kernel may be off by.
+
+    A weight is off by: its f16 rounding (2^-11 relative, 2^-26 of the largest where it is a subnormal), and its
+    score's error, which is at most 2^-19 of the sum of the magnitudes that go into it (each of some 2^4 32-bit
+    additions cuts 2^-23 of them).  The output is then rounded to its type."""
+    rows, hq, dim = q.shape
+    kvh = cache.num_kv_heads
+    out = np.zeros((rows, hq, dim))
+    tol = np.zeros((rows, hq, dim))
+    half_step = torch.finfo(q.dtype).eps / 2
+    qn = q.double().cpu().numpy()
+    for r in range(rows):
+        n = int(lens[r])
+        if n <= 0:
+            continue
+        pos = torch.arange(n, dtype=torch.int32, device=DEV)
+        k, v = (t.double().cpu().numpy() for t in cache.read(0, table, torch.full_like(pos, int(slots[r])), pos, dtype=torch.float32))
+        for h in range(hq):
+            kk, vv = k[:, h * kvh // hq], v[:, h * kvh // hq]
+            x = kk @ qn[r, h] * scale
+            w = np.exp(x - x.max())
+            w /= w.sum()
+            o = w @ vv
+            spread = np.abs(vv).max(0) + np.abs(vv).max()   # |V - z| is at most the span of its group
+            # The offsets may be far larger than the values: |s n| + |z| <= 2 (max - min) + |x| of the group, at most 5 max |k|.
+            delta = 2.0 ** -19 * np.abs(scale) * (np.abs(qn[r, h]).sum() * 5 * np.abs(kk).max())
+            arithmetic = (2.0 ** -11 + n * 2.0 ** -26 + 2 * delta + 2.0 ** -18) * spread
+            g = 1.0
+            if gate is not None:
+                g = 1 / (1 + np.exp(-gate[r, h].double().cpu().numpy()))
+            out[r, h] = o * g
+            # The gate's sigmoid: 2^-20 relative.
+            tol[r, h] = arithmetic * g + (half_step + 2.0 ** -20) * np.abs(out[r, h]) + 2.0 ** -25
+    return out.reshape(rows, -1), tol.reshape(rows, -1)
+
+
+def check_attention(cache, table, hq, slots, lens, starts=None, dtype=torch.bfloat16, gate=False, seed=0, scale=None, plan=None):
+    rows = len(slots)
+    g = torch.Generator(device=DEV).manual_seed(seed + 100)
+    q = torch.randn(rows, hq, cache.head_dim, generator=g, device=DEV).to(dtype)
+    gt = torch.randn(rows, hq, cache.head_dim, generator=g, device=DEV).to(dtype) if gate else None
+    scale = cache.head_dim ** -0.5 if scale is None else scale
+    if plan is None:
+        most = 1 if starts is None else max([b - a for a, b in zip(starts, starts[1:])] + [1])
+        plan = QuantAttention(cache, hq, max_rows=max(rows, 1), max_seqs=max(1, rows if starts is None else len(starts) - 1), max_seq_rows=most)
+    plan.update(_i32(slots), _i32(lens), None if starts is None else _i32(starts))
+    got = plan.attend(0, q, table, scale, gate=gt)
+    plan.check()
+    want, tol = reference(cache, table, q, slots, lens, scale, gt)
+    err = np.abs(got.double().cpu().numpy() - want)
+    assert np.all(err <= tol), (float(np.nanmax(err / np.maximum(tol, 1e-300))), np.isnan(err).sum(), np.argwhere(~(err <= tol))[:4].tolist())
+    return got
+
+
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (8, 1), (6, 2), (16, 2), (16, 1), (12, 12)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_decode_rows(bits, dim, hq, hkv):
+    lens = [1, 15, 16, 17, 33, 300, 0, 700]
+    cache, table = filled(lens, hkv, dim, bits, seed=dim + hq)
+    check_attention(cache, table, hq, list(range(len(lens))), lens, gate=hq == 16, seed=hq)
+
+
+@pytest.mark.parametrize("page", [32, 128])
+def test_larger_pages(page):
+    lens = [5, 129, 260]
+    cache, table = filled(lens, 2, 128, 4, page=page, seed=9)
+    check_attention(cache, table, 8, [2, 0, 1], [260, 5, 129])
+
+
+@pytest.mark.parametrize("dim,bits", [(64, 4), (128, 4), (256, 4), (64, 8), (128, 8), (256, 8)])
+@pytest.mark.parametrize("per", [2, 4, 9, 40])
+def test_rows_of_a_sequence(dim, bits, per):
+    """Verify rows and chunks: rows of one sequence, each up to its own length, in ragged numbers."""
+    lens = [per + 3, 200, 67]
+    cache, table = filled(lens, 2, dim, bits, seed=per)
+    counts = [per, max(1, per - 1), per]
+    starts = [0, per, per + counts[1], sum(counts)]
+    slots = [s for s, c in enumerate(counts) for _ in range(c)]
+    seen = [lens[s] - c + 1 + i for s, c in enumerate(counts) for i in range(c)]
+    check_attention(cache, table, 8, slots, seen, starts, gate=True, seed=per)
+
+
+def test_many_heads_of_one_kv_head():
+    """More q heads than one work unit holds, and rows whose heads are in two units."""
+    cache, table = filled([90, 41], 1, 256, 4, seed=3)
+    check_attention(cache, table, 160, [0, 0, 0, 1], [88, 89, 90, 41], [0, 3, 4])
+
+
+def test_lengths_in_any_order_and_rows_of_no_sequence():
+    cache, table = filled([100, 50, 40], 2, 128, 4, seed=5)
+    starts = [0, 3, 3, 5]   # the second sequence has no rows; row 5 belongs to none
+    plan = QuantAttention(cache, 4, max_rows=6, max_seqs=4, max_seq_rows=3)
+    slots, seen = [0, 0, 0, 2, 2, 1], [100, 0, 7, 40, 39, 50]
+    g = torch.Generator(device=DEV).manual_seed(1)
+    q = torch.randn(6, 4, 128, generator=g, device=DEV).to(torch.bfloat16)
+    plan.update(_i32(slots), _i32(seen), _i32(starts))
+    got = plan.attend(0, q, table, 0.1)
+    plan.check()
+    want, tol = reference(cache, table, q[:5], slots[:5], seen[:5], 0.1)
+    assert np.all(np.abs(got[:5].double().cpu().numpy() - want) <= tol) and not got[5].any() and not got[1].any()
+
+
+def test_f16_and_extreme_sizes():
+    cache, table = filled([130, 77], 2, 128, 4, dtype=torch.float16, seed=6)
+    check_attention(cache, table, 8, [0, 1], [130, 77], dtype=torch.float16, gate=True)
+    for v_scale in (2.0 ** -40, 2.0 ** 60):
+        cache, table = filled([130, 77], 2, 128, 4, seed=7, v_scale=v_scale)
+        q = torch.randn(2, 8, 128, device=DEV).to(torch.bfloat16)
+        plan = QuantAttention(cache, 8, 2)
+        plan.update(_i32([0, 1]), _i32([130, 77]))
+        got = plan.attend(0, q, table, 0.09).double().cpu().numpy()
+        want, tol = reference(cache, table, q, [0, 1], [130, 77], 0.09)
+        assert np.all(np.abs(got - want) <= tol - 2.0 ** -25)
+    # Queries of any size: the scores of the small ones are all alike, those of the large ones pick a key.
+    cache, table = filled([130], 2, 128, 4, seed=8)
+    for size in (2.0 ** -90, 2.0 ** 40):
+        q = (size * torch.randn(1, 8, 128, device=DEV)).to(torch.bfloat16)
+        plan = QuantAttention(cache, 8, 1)
+        plan.update(_i32([0]), _i32([130]))
+        got = plan.attend(0, q, table, 0.09).double().cpu().numpy()
+        want, tol = reference(cache, table, q, [0], [130], 0.09)
+        if size < 1:
+            assert np.all(np.abs(got - want) <= tol)
+        else:   # the winner leads by far more than its score's error
+            assert np.all(np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -11 * np.abs(want).max() * 4)
+
+
+def test_large_and_uneven_scores():
+    """One key far above the others, early or late, and V groups of very different sizes."""
+    lens, dim = [400], 128
+    table, pages = table_of(lens, 16)
+    cache = QuantCache(1, pages, 1, dim)
+    slots, pos = places_of(lens)
+    k, v = rows_of(400, 1, dim, torch.bfloat16, 1), rows_of(400, 1, dim, torch.bfloat16, 2)
+    v[:, :, 64:] *= 2.0 ** -12
+    for hot in (0, 399, 170):
+        k2 = k.clone()
+        k2[hot] *= 12
+        cache.write(0, k2, v, table, slots, pos)
+        check_attention(cache, table, 8, [0], lens, seed=hot)
+
+
+def test_poison_and_masks():
+    """NaN in K that a row sees makes the row NaN; in V only the dims of its group; behind the length nothing."""
+    dim, n = 128, 50
+    table, pages = table_of([n], 16)
+    slots, pos = places_of([n])
+    k, v = rows_of(n, 1, dim, torch.bfloat16, 1), rows_of(n, 1, dim, torch.bfloat16, 2)
+    q = torch.randn(3, 4, dim, device=DEV).to(torch.bfloat16)
+    plan, seen, starts = None, [39, 40, 41], [0, 3]
+    for which in ("k", "v"):
+        a, b = k.clone(), v.clone()
+        (a if which == "k" else b)[40, 0, 70] = float("nan")   # seen by the last row alone
+        cache = QuantCache(1, pages, 1, dim)
+        cache.write(0, a, b, table, slots, pos)
+        plan = QuantAttention(cache, 4, 3, 1, 3)
+        plan.update(_i32([0, 0, 0]), _i32(seen), _i32(starts))
+        got = plan.attend(0, q, table, 0.1).view(3, 4, dim)
+        want, tol = reference(cache, table, q[:2], [0, 0], seen[:2], 0.1)
+        assert np.all(np.abs(got[:2].double().cpu().numpy().reshape(2, -1) - want) <= tol)
+        if which == "k":
+            assert bool(got[2].isnan().all())
+        else:
+            assert bool(got[2, :, 64:].isnan().all()) and bool(got[2, :, :64].isfinite().all())
+    # A query that is not finite spoils its own head only.
+    cache = QuantCache(1, pages, 1, dim)
+    cache.write(0, k, v, table, slots, pos)
+    q[1, 2, 5] = float("inf")
+    plan.cache = cache
+    plan.update(_i32([0, 0, 0]), _i32(seen), _i32(starts))
+    got = plan.attend(0, q, table, 0.1).view(3, 4, dim)
+    assert bool(got[1, 2].isnan().all())
+    got[1, 2] = 0
+    assert bool(got.isfinite().all())
+
+
+def test_strided_queries_and_mxfp8():
+    from zstep_b200.ops import mx
+
+    lens, hq, dim = [130, 77, 200], 8, 256
+    cache, table = filled(lens, 2, dim, 4, seed=12)
+    wide = torch.randn(3, 2 * hq + 1, dim, device=DEV).to(torch.bfloat16)
+    q, gate = wide[:, 0:2 * hq:2], wide[:, 1:2 * hq:2]
+    plan = QuantAttention(cache, hq, 3)
+    plan.update(_i32([0, 1, 2]), _i32(lens))
+    out = torch.empty(3, hq * dim, dtype=torch.bfloat16, device=DEV)
+    out_q = torch.empty(128, hq * dim, dtype=torch.uint8, device=DEV)
+    out_sf = torch.zeros(mx.atoms_bytes(3, hq * dim), dtype=torch.uint8, device=DEV)
+    plan.attend(0, q, table, 0.0625, gate=gate, out=out, out_q=out_q, out_sf=out_sf)
+    same = plan.attend(0, q.contiguous(), table, 0.0625, gate=gate.contiguous())
+    assert torch.equal(out, same)
+    got = mx.dequantize(out_q[:3], mx.codes_from_atoms(out_sf, 3, hq * dim))
+    # e4m3: half a step is 2^-4 of the value, or 2^-10 of the block's scale where it is a subnormal; bf16's rounding.
+    block = out.float().abs().view(3, -1, 32).amax(-1, keepdim=True).expand(-1, -1, 32).reshape(3, -1)
+    assert bool(((got - out.float()).abs() <= out.float().abs() * (2.0 ** -4 + 2.0 ** -8) + block * 2.0 ** -10).all())
+
+
+def test_long_sequence_is_split_and_repeats_exactly():
+    """A lone long sequence takes every SM; the result does not depend on the order they finish in."""
+    n, dim = 20000, 64
+    table, pages = table_of([n], 16)
+    cache = QuantCache(1, pages, 1, dim)
+    slots, pos = places_of([n])
+    cache.write(0, rows_of(n, 1, dim, torch.bfloat16, 1), rows_of(n, 1, dim, torch.bfloat16, 2), table, slots, pos)
+    first = check_attention(cache, table, 2, [0], [n - 3], seed=3)
+    for _ in range(3):
+        assert torch.equal(check_attention(cache, table, 2, [0], [n - 3], seed=3), first)
+
+
+def test_many_short_sequences():
+    rng = np.random.default_rng(3)
+    lens = rng.integers(0, 60, 700).tolist()
+    cache, table = filled(lens, 1, 64, 4, seed=2)
+    check_attention(cache, table, 2, list(range(700)), lens)
+
+
+def test_places_outside_are_reported():
+    cache, table = filled([40], 1, 64, 4)
+    q = torch.randn(1, 2, 64, device=DEV).to(torch.bfloat16)
+    plan = QuantAttention(cache, 2, 4, 2, 2)
+    for slots, lens, starts, tab in (([1], [40], None, table), ([-1], [40], None, table), ([0], [65], None, table),
+                                     ([0], [40], None, torch.full_like(table, cache.num_pages)), ([0], [40], [0, 2], table),
+                                     ([0], [40], [1, 0], table), ([0], [40], [-1, 1], table)):
+        plan.update(_i32(slots), _i32(lens), None if starts is None else _i32(starts))
+        plan.attend(0, q, tab, 0.1)
+        with pytest.raises(RuntimeError, match="error status"):
+            plan.check()
+    check_attention(cache, table, 2, [0], [40], plan=plan)
+    plan.update(_i32([0, 0, 0]), _i32([1, 2, 3]), _i32([0, 3]))   # more rows of a sequence than the plan takes
+    with pytest.raises(RuntimeError, match="error status"):
+        plan.check()
+    plan.update(_i32([0] * 4), _i32([9] * 4), _i32([0, 2, 4]))
+    plan.check()
+
+
+# --------------------------------------------------------------------------------- together
+def test_generation_loop_in_a_graph_over_a_page_pool():
+    """Prompt rows written and attended as a chunk, sequences forked, then single tokens written and attended by one
+    captured graph, replayed."""
+    hkv, hq, dim = 2, 8, 128
+    cache = QuantCache(1, 64, hkv, dim)
+    pool = PagePool([cache.data], num_slots=4, max_pages=8)
+    g = torch.Generator(device=DEV).manual_seed(0)
+    rnd = lambda n, h: torch.randn(n, h, dim, generator=g, device=DEV).to(torch.bfloat16)  # noqa: E731
+    prompt = 37
+    pool.extend(_i32([0]), _i32([prompt]))
+    slots, pos = places_of([prompt])
+    k, v, q = rnd(prompt, hkv), rnd(prompt, hkv), rnd(prompt, hq)
+    cache.write(0, k, v, pool.page_table, slots, pos)
+    chunk = QuantAttention(cache, hq, prompt, 1, prompt)
+    chunk.update(slots, pos + 1, _i32([0, prompt]))
+    got = chunk.attend(0, q, pool.page_table, 0.1)
+    want, tol = reference(cache, pool.page_table, q, [0] * prompt, (pos + 1).tolist(), 0.1)
+    assert np.all(np.abs(got.double().cpu().numpy() - want) <= tol)
+    pool.fork(_i32([0, 0]), _i32([2, 3]))
+    live = _i32([0, 2, 3])
+    step = QuantAttention(cache, hq, 3)
+    k, v, q = rnd(3, hkv), rnd(3, hkv), rnd(3, hq)
+    out = torch.empty(3, hq * dim, dtype=torch.bfloat16, device=DEV)
+    at = torch.full((3,), prompt, dtype=torch.int32, device=DEV)
+
+    def one():
+        pool.extend(live, at + 1)
+        cache.write(0, k, v, pool.page_table, live, at)
+        step.update(live, at + 1)
+        step.attend(0, q, pool.page_table, 0.1, out=out)
+        at.add_(1)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        one()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        one()
+    for i in range(1, 30):
+        k.copy_(rnd(3, hkv))
+        v.copy_(rnd(3, hkv))
+        q.copy_(rnd(3, hq))
+        graph.replay()
+        n = prompt + i + 1
+        want, tol = reference(cache, pool.page_table, q, [0, 2, 3], [n] * 3, 0.1)
+        assert np.all(np.abs(out.double().cpu().numpy() - want) <= tol), i
+        held = cache.read(0, pool.page_table, live, at - 1, dtype=torch.float32)[0].double().cpu().numpy()
+        assert np.allclose(held, quantised(k, 4)[0], rtol=2.0 ** -23, atol=0)
+    for x in (pool, cache, step, chunk):
+        x.check()
+
+
+def test_plan_is_shared_by_layers_and_its_workspace_is_reused():
+    lens, dim = [90, 33], 128
+    table, pages = table_of(lens, 16)
+    cache = QuantCache(3, pages, 2, dim)
+    slots, pos = places_of(lens)
+    for layer in range(3):
+        cache.write(layer, rows_of(len(slots), 2, dim, torch.bfloat16, layer), rows_of(len(slots), 2, dim, torch.bfloat16, 9 + layer),
+                    table, slots, pos)
+    plan = QuantAttention(cache, 4, 2)
+    q = torch.randn(2, 4, dim, device=DEV).to(torch.bfloat16)
+    plan.update(_i32([0, 1]), _i32(lens))
+    got = [plan.attend(layer, q, table, 0.1).clone() for layer in range(3)]
+    for layer in range(3):
+        one = QuantCache(1, pages, 2, dim)
+        one.data[0].copy_(cache.data[layer])
+        want, tol = reference(one, table, q, [0, 1], lens, 0.1)
+        assert np.all(np.abs(got[layer].double().cpu().numpy() - want) <= tol)
+    assert math.isfinite(float(got[0].float().sum()))
