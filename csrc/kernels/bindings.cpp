@@ -1089,32 +1089,43 @@ void pool_call(int64_t which, const Tensor& refcount, const Tensor& free_bits, c
   }
 }
 
-// Quantised K/V cache.  A layer is uint8 [pages, bytes of a page].
-void check_quant_layer(const Tensor& data, int64_t num_kv_heads, int64_t head_dim, int64_t bits, int64_t page_size) {
-  check_cuda(data, "cache layer");
-  TORCH_CHECK(head_dim == 64 || head_dim == 128 || head_dim == 256, "head_dim must be 64, 128 or 256, got ", head_dim);
-  TORCH_CHECK(bits == 4 || bits == 8, "bits must be 4 or 8, got ", bits);
-  TORCH_CHECK(page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0,
-              "page_size must be a power of two from 16 to 256, got ", page_size);
-  TORCH_CHECK(num_kv_heads >= 1, "num_kv_heads must be positive");
-  TORCH_CHECK(data.dim() == 2 && data.scalar_type() == at::kByte && data.size(0) >= 1 && data.size(0) < (1ll << 31) &&
-                  data.size(1) == num_kv_heads * (page_size / 16) * zs_quant_block_bytes((int)head_dim, (int)bits),
-              "a cache layer must be uint8 [pages, bytes of a page]");
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(data.data_ptr()) % 16 == 0, "the cache must be 16-byte aligned");
-}
-int page_shift(int64_t page_size) {
-  int s = 0;
-  while ((int64_t)1 << s < page_size) ++s;
-  return s;
-}
-void check_index(const Tensor& t, const Tensor& like, const char* name) {
-  check_cuda(t, name);
-  TORCH_CHECK(t.scalar_type() == at::kInt, name, " must be int32");
+// Quantised K/V cache: what does not change from call to call is checked once, here.
+struct QuantCacheState {
+  Tensor data, err;   // uint8 [layers, pages, bytes of a page]; int32 [1]
+  int heads, dim, bits, page_shift;
+
+  QuantCacheState(const Tensor& data_, int64_t heads_, int64_t dim_, int64_t bits_, int64_t page, const Tensor& err_)
+      : data(data_), err(err_), heads((int)heads_), dim((int)dim_), bits((int)bits_), page_shift(0) {
+    TORCH_CHECK(dim == 64 || dim == 128 || dim == 256, "head_dim must be 64, 128 or 256, got ", dim_);
+    TORCH_CHECK(bits == 4 || bits == 8, "bits must be 4 or 8, got ", bits_);
+    TORCH_CHECK(page >= 16 && page <= 256 && (page & (page - 1)) == 0, "page_size must be a power of two from 16 to 256, got ", page);
+    while ((int64_t)1 << page_shift < page) ++page_shift;
+    TORCH_CHECK(heads_ >= 1 && data.dim() == 3 && data.is_contiguous() && data.scalar_type() == at::kByte && data.size(0) >= 1 &&
+                    data.size(1) >= 1 && data.size(2) == heads_ * (page / 16) * zs_quant_block_bytes(dim, bits),
+                "a quantised cache must be uint8 [layers, pages, bytes of a page]");
+    TORCH_CHECK(data.size(1) * heads_ * (page / 16) < (1ll << 31), "too many blocks in a layer");
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(data.data_ptr()) % 16 == 0, "the cache must be 16-byte aligned");
+    TORCH_CHECK(err.scalar_type() == at::kInt && err.numel() == 1 && err.device() == data.device(), "err: int32 [1]");
+  }
+  uint8_t* layer(int64_t i) const {
+    TORCH_CHECK_VALUE(i >= 0 && i < data.size(0), "layer ", i, " outside the ", data.size(0), " layers");
+    TORCH_CHECK(data.is_cuda(), "the cache must be on a CUDA device");
+    return ptr<uint8_t>(data) + i * data.stride(0);
+  }
+};
+
+void check_index(const Tensor& t, const Tensor& like, int64_t dim, const char* name) {
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == dim && t.is_contiguous(), name, " must be a contiguous int32 tensor of ", dim,
+              dim == 1 ? " dimension" : " dimensions");
   TORCH_CHECK(t.device() == like.device(), name, " must be on ", like.device(), ", got ", t.device());
+}
+void check_table(const Tensor& t, const Tensor& like, int64_t rows) {
+  check_index(t, like, 2, "page_table");
+  TORCH_CHECK(t.size(0) < (1ll << 31) && t.size(1) < (1ll << 27) && (rows == 0 || t.numel() > 0), "page_table must be [slots, max_pages]");
 }
 // [rows, heads, dim] whose dims are contiguous and whose rows and heads start on 16-byte boundaries.
 void check_heads(const Tensor& t, const Tensor& like, int64_t rows, int64_t heads, int64_t dim, const char* name) {
-  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be a tensor on ", like.device());
+  TORCH_CHECK(t.device() == like.device(), name, " must be on ", like.device(), ", got ", t.device());
   TORCH_CHECK(t.dim() == 3 && t.size(0) == rows && t.size(1) == heads && t.size(2) == dim, name, " must be [", rows, ", ",
               heads, ", ", dim, "], got ", t.sizes());
   const int64_t e = t.element_size();
@@ -1123,33 +1134,27 @@ void check_heads(const Tensor& t, const Tensor& like, int64_t rows, int64_t head
               name, " must have contiguous dims, and rows and heads on 16-byte boundaries");
 }
 
-// `store` true: k and v into the cache; false: the cache into k and v.
-void quant_rows(bool store, const Tensor& data, int64_t num_kv_heads, int64_t head_dim, int64_t bits, int64_t page_size,
-                const Tensor& page_table, const Tensor& slots, const Tensor& positions, const Tensor& k, const Tensor& v,
-                const Tensor& err) {
-  check_quant_layer(data, num_kv_heads, head_dim, bits, page_size);
-  check_index(page_table, data, "page_table");
-  check_index(slots, data, "slots");
-  check_index(positions, data, "positions");
-  check_index(err, data, "err");
+void quant_rows(bool store, const QuantCacheState& c, int64_t layer, const Tensor& page_table, const Tensor& slots,
+                const Tensor& positions, const Tensor& k, const Tensor& v) {
+  QuantRowsArgs a{};
+  a.data = c.layer(layer);
   const int64_t rows = slots.numel();
-  TORCH_CHECK(slots.dim() == 1 && positions.dim() == 1 && positions.numel() == rows, "slots and positions must have one entry per row");
-  TORCH_CHECK(rows < (1ll << 31), "too many rows");
-  TORCH_CHECK(page_table.dim() == 2 && (rows == 0 || page_table.numel() > 0), "page_table must be int32 [slots, max_pages]");
-  check_heads(k, data, rows, num_kv_heads, head_dim, "k");
-  check_heads(v, data, rows, num_kv_heads, head_dim, "v");
+  check_index(slots, c.data, 1, "slots");
+  check_index(positions, c.data, 1, "positions");
+  TORCH_CHECK(positions.numel() == rows && rows < (1ll << 31), "slots and positions must have one entry per row");
+  check_table(page_table, c.data, rows);
+  check_heads(k, c.data, rows, c.heads, c.dim, "k");
+  check_heads(v, c.data, rows, c.heads, c.dim, "v");
   const auto type = k.scalar_type();
   TORCH_CHECK(type == v.scalar_type() && (type == at::kBFloat16 || type == at::kHalf || (!store && type == at::kFloat)),
               "k and v must both be bf16 or both f16", store ? "" : " or both f32");
   if (rows == 0) return;
-  const at::cuda::CUDAGuard guard(data.device());
-  QuantRowsArgs a{};
-  a.data = ptr<uint8_t>(data);
-  a.num_pages = (int)data.size(0);
-  a.num_kv_heads = (int)num_kv_heads;
-  a.head_dim = (int)head_dim;
-  a.bits = (int)bits;
-  a.page_shift = page_shift(page_size);
+  const at::cuda::CUDAGuard guard(c.data.device());
+  a.num_pages = (int)c.data.size(1);
+  a.num_kv_heads = c.heads;
+  a.head_dim = c.dim;
+  a.bits = c.bits;
+  a.page_shift = c.page_shift;
   a.rows = (int)rows;
   a.slots = ptr<const int>(slots);
   a.positions = ptr<const int>(positions);
@@ -1164,129 +1169,133 @@ void quant_rows(bool store, const Tensor& data, int64_t num_kv_heads, int64_t he
   a.v_head = v.stride(1);
   a.half = type == at::kHalf;
   a.f32 = type == at::kFloat;
-  a.err = ptr<int>(err);
+  a.err = ptr<int>(c.err);
   rc(store ? zs_quant_store(&a, stream()) : zs_quant_load(&a, stream()), store ? "zs_quant_store" : "zs_quant_load");
 }
 
-// Sizes of an attention workspace: bytes of `work`, floats of `partial`, slots of a unit, chunks.
-std::vector<int64_t> quant_attn_sizes(int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t max_rows,
-                                      int64_t max_seqs, int64_t max_seq_rows) {
-  int tiles, slot_warps;
-  const int64_t group = num_q_heads / num_kv_heads;
-  zs_quant_attn_shape((int)head_dim, (int)std::min<int64_t>(group * max_seq_rows, 1 << 20), &tiles, &slot_warps);
-  const int64_t chunk = 8 * tiles * slot_warps, chunks = max_seqs + max_rows * group / chunk;
-  return {zs_quant_attn_work((int)chunks, (int)max_rows, (int)max_seqs),
-          (chunks * num_kv_heads + ZS_QUANT_CTAS) * chunk * (head_dim + 2), tiles, slot_warps, chunks};
+std::pair<Tensor, Tensor> quant_read(const QuantCacheState& c, int64_t layer, const Tensor& page_table, const Tensor& slots,
+                                     const Tensor& positions, at::ScalarType dtype, const OptT& k, const OptT& v) {
+  const std::vector<int64_t> shape{slots.numel(), c.heads, c.dim};
+  const auto options = c.data.options().dtype(k.has_value() ? k->scalar_type() : v.has_value() ? v->scalar_type() : dtype);
+  std::pair<Tensor, Tensor> out(k.has_value() ? *k : at::empty(shape, options), v.has_value() ? *v : at::empty(shape, options));
+  quant_rows(false, c, layer, page_table, slots, positions, out.first, out.second);
+  return out;
 }
 
-QuantAttnArgs quant_attn_args(int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t bits, int64_t rows,
-                              int64_t max_rows, int64_t num_seqs, int64_t max_seqs, int64_t max_seq_rows, const Tensor& work,
-                              const Tensor& partial, const Tensor& err) {
-  TORCH_CHECK(num_kv_heads >= 1 && num_q_heads >= 1 && num_q_heads % num_kv_heads == 0, "q heads must be a multiple of kv heads");
-  TORCH_CHECK(rows >= 0 && rows <= max_rows && num_seqs >= 0 && num_seqs <= max_seqs && max_seq_rows >= 1, "a step of ", rows,
-              " rows and ", num_seqs, " sequences does not fit a plan of ", max_rows, " rows and ", max_seqs, " sequences");
-  const auto sizes = quant_attn_sizes(num_q_heads, num_kv_heads, head_dim, max_rows, max_seqs, max_seq_rows);
-  check_cuda(work, "work");
-  check_cuda(partial, "partial");
-  check_index(err, work, "err");
-  TORCH_CHECK(work.device() == partial.device() && work.element_size() == 1 && work.numel() >= sizes[0] &&
-                  partial.scalar_type() == at::kFloat && partial.numel() >= sizes[1] &&
-                  reinterpret_cast<uintptr_t>(work.data_ptr()) % 32 == 0 && reinterpret_cast<uintptr_t>(partial.data_ptr()) % 16 == 0,
-              "workspace too small, misaligned or on two devices");
-  QuantAttnArgs a{};
-  a.num_q_heads = (int)num_q_heads;
-  a.num_kv_heads = (int)num_kv_heads;
-  a.head_dim = (int)head_dim;
-  a.bits = (int)bits;
-  a.rows = (int)rows;
-  a.max_rows = (int)max_rows;
-  a.num_seqs = (int)num_seqs;
-  a.max_seq_rows = (int)max_seq_rows;
-  a.tiles = (int)sizes[2];
-  a.slot_warps = (int)sizes[3];
-  a.chunk = 8 * a.tiles * a.slot_warps;
-  a.max_chunks = (int)sizes[4];
-  a.work = ptr(work);
-  a.partial = ptr<float>(partial);
-  a.err = ptr<int>(err);
-  return a;
-}
+// A plan of QuantAttention: its sizes, its workspace and the step it holds.
+struct QuantPlanState {
+  QuantAttnArgs base{};
+  Tensor work, partial, err;
+  int64_t max_seqs = 0, rows = -1;
+  int64_t dim = 0, bits = 0;
 
-void quant_attn_plan(int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t bits, int64_t max_rows,
-                     int64_t max_seqs, int64_t max_seq_rows, const Tensor& slots, const Tensor& seq_lens, const OptT& seq_start,
-                     const Tensor& work, const Tensor& partial, const Tensor& err) {
-  check_index(slots, work, "slots");
-  check_index(seq_lens, work, "seq_lens");
-  const int64_t rows = slots.numel();
-  TORCH_CHECK(slots.dim() == 1 && seq_lens.dim() == 1 && seq_lens.numel() == rows, "slots and seq_lens must have one entry per row");
-  if (seq_start.has_value()) {
-    check_index(*seq_start, work, "seq_start");
-    TORCH_CHECK(seq_start->dim() == 1 && seq_start->numel() >= 1, "seq_start must be int32 [sequences + 1]");
+  QuantPlanState(const QuantCacheState& c, int64_t q_heads, int64_t max_rows, int64_t max_seqs_, int64_t max_seq_rows, const Tensor& err_)
+      : err(err_), max_seqs(max_seqs_), dim(c.dim), bits(c.bits) {
+    TORCH_CHECK_VALUE(q_heads >= 1 && q_heads % c.heads == 0, q_heads, " q heads are not a multiple of ", c.heads, " kv heads");
+    TORCH_CHECK_VALUE(max_rows >= 1 && max_seqs >= 1 && max_seq_rows >= 1, "max_rows, max_seqs and max_seq_rows must be positive");
+    const int64_t group = q_heads / c.heads;
+    TORCH_CHECK_VALUE(max_rows * q_heads < (1ll << 28) && max_seqs < (1ll << 24), "too many rows or sequences for a plan");
+    QuantAttnArgs& a = base;
+    zs_quant_attn_shape(c.dim, c.bits, (int)std::min<int64_t>(group * max_seq_rows, 1 << 20), &a.tiles, &a.slot_warps, &a.stage);
+    a.chunk = 8 * a.tiles * a.slot_warps;
+    a.max_chunks = (int)(max_seqs + max_rows * group / a.chunk);
+    a.num_q_heads = (int)q_heads;
+    a.num_kv_heads = c.heads;
+    a.head_dim = c.dim;
+    a.bits = c.bits;
+    a.max_rows = (int)max_rows;
+    a.max_seq_rows = (int)std::min<int64_t>(max_seq_rows, 1 << 30);
+    const auto bytes = c.data.options();
+    work = at::zeros({zs_quant_attn_work(a.max_chunks, a.max_rows, (int)max_seqs)}, bytes);
+    partial = at::empty({((int64_t)a.max_chunks * c.heads + ZS_QUANT_CTAS) * a.chunk * (c.dim + 2)}, bytes.dtype(at::kFloat));
+    TORCH_CHECK(err.scalar_type() == at::kInt && err.numel() == 1 && err.device() == c.data.device(), "err: int32 [1]");
+    a.work = ptr(work);
+    a.partial = ptr<float>(partial);
+    a.err = ptr<int>(err);
   }
-  const at::cuda::CUDAGuard guard(work.device());
-  QuantAttnArgs a = quant_attn_args(num_q_heads, num_kv_heads, head_dim, bits, rows, max_rows,
-                                    seq_start.has_value() ? seq_start->numel() - 1 : rows, max_seqs, max_seq_rows, work, partial, err);
-  a.slots = ptr<const int>(slots);
-  a.seq_lens = ptr<const int>(seq_lens);
-  a.seq_start = optptr<const int>(seq_start);
-  rc(zs_quant_attn_plan(&a, stream()), "zs_quant_attn_plan");
-}
 
-void quant_attn(const Tensor& data, int64_t num_kv_heads, int64_t head_dim, int64_t bits, int64_t page_size, int64_t num_seqs,
-                int64_t max_rows, int64_t max_seqs, int64_t max_seq_rows, const Tensor& q, const OptT& gate,
-                const Tensor& page_table, double sm_scale, const OptT& out, const OptT& out_q, const OptT& out_sf,
-                const Tensor& work, const Tensor& partial, const Tensor& err) {
-  check_quant_layer(data, num_kv_heads, head_dim, bits, page_size);
-  TORCH_CHECK(q.dim() == 3, "q must be [rows, heads, ", head_dim, "]");
-  const int64_t rows = q.size(0), heads = q.size(1);
-  TORCH_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf, "q must be bf16 or f16");
-  check_heads(q, data, rows, heads, head_dim, "q");
-  check_index(page_table, data, "page_table");
-  TORCH_CHECK(page_table.dim() == 2 && (rows == 0 || page_table.numel() > 0), "page_table must be int32 [slots, max_pages]");
-  TORCH_CHECK(work.device() == data.device(), "the plan must be on the cache's device");
-  const at::cuda::CUDAGuard guard(data.device());
-  QuantAttnArgs a = quant_attn_args(heads, num_kv_heads, head_dim, bits, rows, max_rows, num_seqs, max_seqs, max_seq_rows, work, partial, err);
-  a.data = ptr<const uint8_t>(data);
-  a.num_pages = (int)data.size(0);
-  a.page_shift = page_shift(page_size);
-  a.page_table = ptr<const int>(page_table);
-  a.num_slots = (int)page_table.size(0);
-  a.max_pages = (int)page_table.size(1);
-  a.q = ptr(q);
-  a.q_row = q.stride(0);
-  a.q_head = q.stride(1);
-  if (gate.has_value()) {
-    check_heads(*gate, data, rows, heads, head_dim, "gate");
-    TORCH_CHECK(gate->scalar_type() == q.scalar_type(), "gate must have the type of q");
-    a.gate = ptr(*gate);
-    a.gate_row = gate->stride(0);
-    a.gate_head = gate->stride(1);
+  void update(const Tensor& slots, const Tensor& seq_lens, const OptT& seq_start) {
+    rows = -1;
+    TORCH_CHECK(work.is_cuda(), "the cache must be on a CUDA device");
+    check_index(slots, work, 1, "slots");
+    check_index(seq_lens, work, 1, "seq_lens");
+    const int64_t n = slots.numel();
+    TORCH_CHECK(seq_lens.numel() == n, "slots and seq_lens must have one entry per row");
+    int64_t seqs = n;
+    if (seq_start.has_value()) {
+      check_index(*seq_start, work, 1, "seq_start");
+      seqs = seq_start->numel() - 1;
+      TORCH_CHECK(seqs >= 0, "seq_start must be int32 [sequences + 1]");
+    }
+    TORCH_CHECK_VALUE(n <= base.max_rows && seqs <= max_seqs, "a step of ", n, " rows and ", seqs, " sequences does not fit a plan of ",
+                      base.max_rows, " rows and ", max_seqs, " sequences");
+    const at::cuda::CUDAGuard guard(work.device());
+    QuantAttnArgs a = base;
+    a.rows = (int)n;
+    a.num_seqs = (int)seqs;
+    a.slots = ptr<const int>(slots);
+    a.seq_lens = ptr<const int>(seq_lens);
+    a.seq_start = optptr<const int>(seq_start);
+    rc(zs_quant_attn_plan(&a, stream()), "zs_quant_attn_plan");
+    rows = n;
   }
-  a.half = q.scalar_type() == at::kHalf;
-  a.sm_scale = (float)sm_scale;
-  TORCH_CHECK(out.has_value() || out_q.has_value(), "attention needs an output");
-  if (out.has_value()) {
-    check_cuda(*out, "out");
-    TORCH_CHECK(out->device() == data.device() && out->scalar_type() == q.scalar_type() && out->numel() == rows * heads * head_dim &&
-                    reinterpret_cast<uintptr_t>(out->data_ptr()) % 16 == 0,
-                "out must be [rows, heads * ", head_dim, "] of q's type, 16-byte aligned");
-    a.out = ptr(*out);
+
+  Tensor attend(const QuantCacheState& c, int64_t layer, const Tensor& q, const Tensor& page_table, double sm_scale, const OptT& gate,
+                const OptT& out, const OptT& out_q, const OptT& out_sf) {
+    QuantAttnArgs a = base;
+    a.data = c.layer(layer);
+    TORCH_CHECK(rows >= 0, "attend needs an update first");
+    TORCH_CHECK(c.dim == dim && c.bits == bits && c.heads == a.num_kv_heads && c.data.device() == work.device(),
+                "the plan was made for a cache of another form or device");
+    TORCH_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf, "q must be bf16 or f16");
+    check_heads(q, c.data, rows, a.num_q_heads, dim, "q");
+    check_table(page_table, c.data, rows);
+    const at::cuda::CUDAGuard guard(c.data.device());
+    const int64_t width = a.num_q_heads * dim;
+    a.num_pages = (int)c.data.size(1);
+    a.page_shift = c.page_shift;
+    a.rows = (int)rows;
+    a.page_table = ptr<const int>(page_table);
+    a.num_slots = (int)page_table.size(0);
+    a.max_pages = (int)page_table.size(1);
+    a.q = ptr(q);
+    a.q_row = q.stride(0);
+    a.q_head = q.stride(1);
+    if (gate.has_value()) {
+      check_heads(*gate, c.data, rows, a.num_q_heads, dim, "gate");
+      TORCH_CHECK(gate->scalar_type() == q.scalar_type(), "gate must have the type of q");
+      a.gate = ptr(*gate);
+      a.gate_row = gate->stride(0);
+      a.gate_head = gate->stride(1);
+    }
+    a.half = q.scalar_type() == at::kHalf;
+    a.sm_scale = (float)sm_scale;
+    Tensor o;
+    if (out.has_value()) {
+      o = *out;
+      TORCH_CHECK(o.is_contiguous() && o.device() == c.data.device() && o.scalar_type() == q.scalar_type() && o.numel() == rows * width &&
+                      reinterpret_cast<uintptr_t>(o.data_ptr()) % 16 == 0,
+                  "out must be a contiguous [rows, heads * dim] of q's type, 16-byte aligned");
+    } else if (!out_q.has_value()) {
+      o = at::empty({rows, width}, q.options());
+    }
+    if (o.defined()) a.out = ptr(o);
+    TORCH_CHECK(out_q.has_value() == out_sf.has_value(), "the MXFP8 output needs out_q and out_sf");
+    if (out_q.has_value()) {
+      check_cuda(*out_q, "out_q");
+      check_cuda(*out_sf, "out_sf");
+      TORCH_CHECK(width % 128 == 0, "the MXFP8 output needs rows of a multiple of 128");
+      TORCH_CHECK(out_q->device() == c.data.device() && out_sf->device() == c.data.device() && out_q->element_size() == 1 &&
+                      out_sf->element_size() == 1 && out_q->numel() >= rows * width &&
+                      out_sf->numel() >= (rows + 127) / 128 * (width / 128) * 512 && reinterpret_cast<uintptr_t>(out_q->data_ptr()) % 16 == 0,
+                  "MXFP8 output too small or misaligned");
+      a.out_q = ptr<uint8_t>(*out_q);
+      a.out_sf = ptr<uint8_t>(*out_sf);
+    }
+    rc(zs_quant_attn(&a, stream()), "zs_quant_attn");
+    return o;
   }
-  TORCH_CHECK(out_q.has_value() == out_sf.has_value(), "the MXFP8 output needs out_q and out_sf");
-  if (out_q.has_value()) {
-    check_cuda(*out_q, "out_q");
-    check_cuda(*out_sf, "out_sf");
-    TORCH_CHECK(heads * head_dim % 128 == 0, "the MXFP8 output needs rows of a multiple of 128");
-    TORCH_CHECK(out_q->device() == data.device() && out_sf->device() == data.device() && out_q->element_size() == 1 &&
-                    out_sf->element_size() == 1 && out_q->numel() >= rows * heads * head_dim &&
-                    out_sf->numel() >= (rows + 127) / 128 * (heads * head_dim / 128) * 512 &&
-                    reinterpret_cast<uintptr_t>(out_q->data_ptr()) % 16 == 0,
-                "MXFP8 output too small or misaligned");
-    a.out_q = ptr<uint8_t>(*out_q);
-    a.out_sf = ptr<uint8_t>(*out_sf);
-  }
-  rc(zs_quant_attn(&a, stream()), "zs_quant_attn");
-}
+};
 
 }  // namespace
 
@@ -1378,16 +1387,21 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("num_segs"), py::arg("segs"), py::arg("work"), py::arg("partial"), py::arg("sm_scale"), py::arg("out_bf16"), py::arg("out_q"),
         py::arg("out_sf"), py::arg("err"));
   m.def("quant_block_bytes", [](int64_t d, int64_t bits) { return zs_quant_block_bytes((int)d, (int)bits); });
-  m.def("quant_rows", &quant_rows, py::arg("store"), py::arg("data"), py::arg("num_kv_heads"), py::arg("head_dim"), py::arg("bits"),
-        py::arg("page_size"), py::arg("page_table"), py::arg("slots"), py::arg("positions"), py::arg("k"), py::arg("v"), py::arg("err"));
-  m.def("quant_attn_sizes", &quant_attn_sizes);
-  m.def("quant_attn_plan", &quant_attn_plan, py::arg("num_q_heads"), py::arg("num_kv_heads"), py::arg("head_dim"), py::arg("bits"),
-        py::arg("max_rows"), py::arg("max_seqs"), py::arg("max_seq_rows"), py::arg("slots"), py::arg("seq_lens"),
-        py::arg("seq_start"), py::arg("work"), py::arg("partial"), py::arg("err"));
-  m.def("quant_attn", &quant_attn, py::arg("data"), py::arg("num_kv_heads"), py::arg("head_dim"), py::arg("bits"),
-        py::arg("page_size"), py::arg("num_seqs"), py::arg("max_rows"), py::arg("max_seqs"), py::arg("max_seq_rows"), py::arg("q"),
-        py::arg("gate"), py::arg("page_table"), py::arg("sm_scale"), py::arg("out"), py::arg("out_q"), py::arg("out_sf"),
-        py::arg("work"), py::arg("partial"), py::arg("err"));
+  py::class_<QuantCacheState>(m, "QuantCacheState")
+      .def(py::init<const Tensor&, int64_t, int64_t, int64_t, int64_t, const Tensor&>(), py::arg("data"), py::arg("num_kv_heads"),
+           py::arg("head_dim"), py::arg("bits"), py::arg("page_size"), py::arg("err"))
+      .def("write", [](const QuantCacheState& c, int64_t layer, const Tensor& k, const Tensor& v, const Tensor& page_table, const Tensor& slots,
+                       const Tensor& positions) { quant_rows(true, c, layer, page_table, slots, positions, k, v); })
+      .def("read", &quant_read);
+  py::class_<QuantPlanState>(m, "QuantPlanState")
+      .def(py::init<const QuantCacheState&, int64_t, int64_t, int64_t, int64_t, const Tensor&>(), py::arg("cache"), py::arg("num_q_heads"),
+           py::arg("max_rows"), py::arg("max_seqs"), py::arg("max_seq_rows"), py::arg("err"))
+      .def("update", &QuantPlanState::update)
+      .def("attend", [](QuantPlanState& p, const QuantCacheState& c, int64_t layer, const Tensor& q, const Tensor& page_table, double sm_scale,
+                        const OptT& gate, const OptT& out, const OptT& out_q, const OptT& out_sf) -> OptT {
+        const Tensor o = p.attend(c, layer, q, page_table, sm_scale, gate, out, out_q, out_sf);
+        return o.defined() ? OptT(o) : OptT();
+      });
   m.def("pool_call", &pool_call, py::arg("which"), py::arg("refcount"), py::arg("free_bits"), py::arg("seq_len"),
         py::arg("page_table"), py::arg("page_size"), py::arg("caches"), py::arg("slots") = py::none(),
         py::arg("parents") = py::none(), py::arg("lens") = py::none(), py::arg("scratch"), py::arg("err"));

@@ -202,12 +202,11 @@ __global__ void __launch_bounds__(ROW_THREADS) load_kernel(const QuantRowsArgs a
 
 // ------------------------------------------------------------------------------------ plan
 // A query slot is one (row, q head of the kv head's group) of a sequence; up to `a.chunk` slots of one
-// sequence and kv head are a unit, and its keys are walked in stages of 32.  The chunks (units of all
+// sequence and kv head are a unit, and its keys are walked in stages of 16 or 32.  The chunks (units of all
 // kv heads at once) stand in a table with the number of stages before them; CTA b of the attention
 // takes the stages [b T / B, (b + 1) T / B) of all T, so that every CTA has the same work whatever the
 // lengths.  One CTA of 1024 threads plans; a step's layers share the plan.
 constexpr int PLAN_THREADS = 1024;
-constexpr int STAGE = 32;   // keys
 
 struct Chunk {          // 32 bytes
   long long before;     // stages of the chunks before, all kv heads
@@ -218,10 +217,10 @@ struct Chunk {          // 32 bytes
 
 struct Plan {           // the workspace's integers
   long long* total;     // stages of all chunks, all kv heads
-  int* chunks;          // number of chunks
   Chunk* table;         // [max_chunks]
   int2* rows;           // [max_rows] first chunk and first row of the row's sequence (-1: none)
   int* lens;            // [max_rows] keys of the row
+  int* start;           // [ZS_QUANT_CTAS] chunk of a CTA's first stage
   int* offset;          // [max_seqs] chunks before the sequence
 };
 
@@ -229,12 +228,17 @@ __host__ __device__ inline Plan plan_of(const QuantAttnArgs& a) {
   Plan p;
   uint8_t* w = reinterpret_cast<uint8_t*>(a.work);
   p.total = reinterpret_cast<long long*>(w);
-  p.chunks = reinterpret_cast<int*>(w + 8);
   p.table = reinterpret_cast<Chunk*>(w + 32);
   p.rows = reinterpret_cast<int2*>(p.table + a.max_chunks);
   p.lens = reinterpret_cast<int*>(p.rows + a.max_rows);
-  p.offset = p.lens + a.max_rows;
+  p.start = p.lens + a.max_rows;
+  p.offset = p.start + ZS_QUANT_CTAS;
   return p;
+}
+
+// Number of CTAs that share T stages.
+__device__ __forceinline__ int ctas_of(long long total, int grid, int least) {
+  return (int)max(1ll, min((long long)grid, total / least));
 }
 
 // Exclusive sum over the CTA's threads; *all gets the sum of all.
@@ -321,26 +325,29 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const QuantAttnArgs 
         // A row whose slots are in two chunks is entered by both, with the same numbers.
         p.rows[r] = make_int2(p.offset[lo], r0);
       }
-      e.stages = (e.len + STAGE - 1) / STAGE;
+      e.stages = (e.len + a.stage - 1) / a.stage;
     }
     const long long cost = (long long)e.stages * a.num_kv_heads;
     e.before = base + block_scan(cost, warps, &all);
     if (c < chunks) p.table[c] = e;
     base += all;
   }
-  if (threadIdx.x == 0) {
-    *p.total = base;
-    *p.chunks = chunks;
+  __syncthreads();
+  const int ctas = base > 0 ? ctas_of(base, a.grid, a.least) : 0;
+  for (int b = threadIdx.x; b < ctas; b += PLAN_THREADS) {
+    const long long first = base * b / ctas;
+    int lo = 0, hi = chunks;   // the last chunk that starts at or before it
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (p.table[mid].before <= first) lo = mid;
+      else hi = mid;
+    }
+    p.start[b] = lo;
   }
-}
-
-// Number of CTAs that share T stages.
-__device__ __forceinline__ int ctas_of(long long total, int grid, int least) {
-  return (int)max(1ll, min((long long)grid, total / least));
+  if (threadIdx.x == 0) *p.total = base;
 }
 
 // ------------------------------------------------------------------------------- attention
-constexpr int WARPS = 8;
 constexpr int MAX_RING = 8;
 constexpr float LIFT = 11.f;    // log2 of what a weight times its scale is held at: below 2^(11 + 1 + SLACK)
 constexpr float SLACK = 3.f;    // the reference moves when a score goes this far above it
@@ -386,17 +393,26 @@ __device__ __forceinline__ void lds(uint32_t (&r)[N], const uint8_t* p) {
   }
 }
 
-// Shared memory of a CTA with `lanes` key lanes (KW) of `sw` warps.
-template <int D, int BITS, int NT>
+// A variant: head dim, bits, tiles of 8 slots of a warp, warps of a CTA, blocks of 16 keys of a stage,
+// CTAs of an SM, and whether the weights keep what f16 cuts off (f16 outputs).
+template <int D_, int BITS_, int NT_, int WARPS_, int KB_, int CTAS_, bool FINE_>
 struct Shape {
+  static constexpr int D = D_, BITS = BITS_, NT = NT_, WARPS = WARPS_, KB = KB_, CTAS = CTAS_;
+  static constexpr bool FINE = FINE_;
   static constexpr int KS = D / 16;                 // k16 steps of a score
   static constexpr int NG = D / GROUP;
   static constexpr int CODES = code_bytes(D, BITS);
   static constexpr int BLOCK = block_bytes(D, BITS);
-  static constexpr int STAGE_BYTES = 2 * BLOCK;
+  static constexpr int KEYS = KB * TOK;             // of a stage
+  static constexpr int STAGE_BYTES = KB * BLOCK;
   static constexpr int MERGE_REGS = KS * NT * 4 + NG * NT * 2 + 4 * NT;   // O, its offset part, l and reference
   static constexpr int MERGE = WARPS / 2 * MERGE_REGS * 128;
   static constexpr int HEAD = 2 * WARPS * MAX_RING * 8;
+  // A row of 16 dims a lane is stored as slabs: 16 bytes a lane and token, 8 bytes where the whole row is 32.
+  static constexpr bool SMALL = BITS == 4 && D == 64;
+  static constexpr int SLABS = SMALL ? 1 : D * BITS / 512;
+  static constexpr int SLAB_GROUPS = BITS == 4 && !SMALL ? 2 : 1;
+  static constexpr int SLAB_WORDS = SMALL ? 2 : 4;
   __host__ __device__ static constexpr int slots(int sw) { return 8 * NT * sw; }
   __host__ __device__ static constexpr int fixed(int sw) {
     return HEAD + slots(sw) * (NG + 2) * 4 + KS * NT * sw * 256 + (sw < WARPS ? MERGE : 0);
@@ -408,17 +424,233 @@ struct Piece {
   int row, slot, slot0, count, len;
 };
 
-template <int D, int BITS, int NT, int MIN_CTAS>
-__global__ void __launch_bounds__(WARPS * 32, MIN_CTAS) attend_kernel(const QuantAttnArgs a) {
-  using S = Shape<D, BITS, NT>;
-  constexpr int KS = S::KS, NG = S::NG, BLOCK = S::BLOCK;
+// What a warp holds of its slots: column j of tile n is slot 8 n + 2 t + j, and register r of a sum is
+// one of its dims (g's).
+template <class S>
+struct State {
+  float o[S::KS][S::NT][4], oz[S::NG][S::NT][2], l[S::NT][2], ref[S::NT][2];
+  float fac[S::NT][2];
+  int lens[S::NT][2];
+};
+
+// One stage: the scores of its keys, their weights, and what they add to the sums.  With MASK a key at or
+// behind a slot's length is left out whatever the cache holds there.
+template <class S, bool MASK>
+__device__ __forceinline__ void stage_step(State<S>& st, const uint8_t* in, const uint8_t* qf, int q_step, const float* qsum,
+                                           int slots, int key0, int g, int t) {
+  constexpr int NT = S::NT, NG = S::NG, KS = S::KS, KB = S::KB, BITS = S::BITS;
+  float sc[KB][NT][4];
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sc[kb][n][j] = 0.f;
+  uint32_t sz[KB][2][NG];
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) lds(sz[kb][r], in + kb * S::BLOCK + 2 * S::CODES + (g + 8 * r) * NG * 4);
+#pragma unroll
+  for (int sl = 0; sl < S::SLABS; ++sl) {
+    uint32_t w[KB][2][S::SLAB_WORDS];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        lds(w[kb][r], in + kb * S::BLOCK + (S::SMALL ? (g + 8 * r) * 32 + t * 8 : sl * 1024 + (g + 8 * r) * 64 + t * 16));
+#pragma unroll
+    for (int sg = 0; sg < S::SLAB_GROUPS; ++sg) {
+      const int gi = sl * S::SLAB_GROUPS + sg;
+      float acc[KB][NT][4];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[kb][n][j] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t bq[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) lds(bq[n], qf + (gi * 4 + k) * q_step + n * 256);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          uint32_t f[2][2];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            if (BITS == 4) {
+              const uint32_t x = w[kb][r][(sg * 2 + (k >> 1)) % S::SLAB_WORDS] >> (8 * (k & 1));
+              f[r][0] = x & 0x000F000Fu;
+              f[r][1] = x & 0x00F000F0u;
+            } else {
+              const uint32_t x = w[kb][r][k % S::SLAB_WORDS];
+              f[r][0] = x & 0x00FF00FFu;
+              f[r][1] = (x >> 8) & 0x00FF00FFu;
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816(acc[kb][n], f[0][0], f[1][0], f[0][1], f[1][1], bq[n][0], bq[n][1]);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float2 qs = *reinterpret_cast<const float2*>(qsum + gi * slots + n * 8 + 2 * t);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t x = sz[kb][j >> 1][gi];
+            sc[kb][n][j] = fmaf(scale_of(x), acc[kb][n][j], fmaf(offset_of(x), j & 1 ? qs.y : qs.x, sc[kb][n][j]));
+          }
+      }
+    }
+  }
+  // V's scales: the largest exponent among this lane's keys bounds them all.  The bits of a scale grow with it;
+  // a poisoned one is negative.
+  int top = 0x1F800000;   // 2^-64
+  int longest = 0;
+  if (MASK) {   // what stands behind the sequence may be anything
+#pragma unroll
+    for (int n = 0; n < NT; ++n) longest = max(longest, max(st.lens[n][0], st.lens[n][1]));
+  }
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      lds(sz[kb][r], in + kb * S::BLOCK + 2 * S::CODES + TOK * NG * 4 + (g + 8 * r) * NG * 4);
+#pragma unroll
+      for (int gi = 0; gi < NG; ++gi)
+        if (!MASK || key0 + kb * 16 + r * 8 + g < longest) top = max(top, (int)(sz[kb][r][gi] << 16));
+    }
+  const float ex = __uint_as_float(0x4B000000u | (uint32_t)(top >> 23)) - (8388608.f + 127.f);
+  float most[NT][2];
+  bool move = false;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float m = -INFINITY;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float x = sc[kb][n][2 * r + j] * st.fac[n][j];
+          if (MASK && key0 + kb * 16 + r * 8 + g >= st.lens[n][j]) x = -INFINITY;
+          sc[kb][n][2 * r + j] = x;
+          m = fmaxf(m, x);
+        }
+      most[n][j] = m + ex;
+      move = move || most[n][j] > st.ref[n][j] + SLACK;
+    }
+  if (__any_sync(0xffffffff, move)) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float m = most[n][j];
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, x));
+        m = fmaxf(m, st.ref[n][j]);
+        const float f = m == st.ref[n][j] ? 1.f : ex2(st.ref[n][j] - m);
+        st.ref[n][j] = m;
+        st.l[n][j] *= f;
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi) st.oz[gi][n][j] *= f;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          st.o[i][n][j] *= f;
+          st.o[i][n][2 + j] *= f;
+        }
+      }
+  }
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // A masked score is -inf; where the reference still is too, the difference would be NaN.
+        float p = ex2(sc[kb][n][j] + (LIFT - st.ref[n][j & 1]));
+        if (MASK && key0 + kb * 16 + (j >> 1) * 8 + g >= st.lens[n][j & 1]) p = 0.f;
+        sc[kb][n][j] = p;
+        st.l[n][j & 1] += p;
+      }
+#pragma unroll
+    for (int sl = 0; sl < S::SLABS; ++sl) {
+      // V's numbers of tokens 2t, 2t + 1 and 2t + 8, 2t + 9 for this lane's 8 dims of each group.
+      uint32_t u[2][S::SLAB_WORDS];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        lds(u[h], in + kb * S::BLOCK + S::CODES +
+                      (S::SMALL ? g * 64 + (h ^ ((g >> 1) & 1)) * 32 + t * 8 : sl * 1024 + g * 128 + (h ^ (g & 1)) * 64 + t * 16));
+#pragma unroll
+      for (int sg = 0; sg < S::SLAB_GROUPS; ++sg) {
+        const int gi = sl * S::SLAB_GROUPS + sg;
+        uint32_t bp[NT][2], bl[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float ps[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t x = sz[kb][j >> 1][gi];
+            ps[j] = sc[kb][n][j] * scale_of(x);
+            float& oz = st.oz[gi][n][j & 1];
+            if (MASK) {   // nothing of a masked key, NaN among it, is taken
+              const bool out = key0 + kb * 16 + (j >> 1) * 8 + g >= st.lens[n][j & 1];
+              ps[j] = out ? 0.f : ps[j];
+              oz = out ? oz : fmaf(sc[kb][n][j], offset_of(x), oz);
+            } else {
+              oz = fmaf(sc[kb][n][j], offset_of(x), oz);
+            }
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t hi = pack_f16(ps[2 * h], ps[2 * h + 1]);
+            bp[n][h] = transpose8x8(hi);
+            if (S::FINE) {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+              bl[n][h] = transpose8x8(pack_f16(ps[2 * h] - f.x, ps[2 * h + 1] - f.y));
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t f[2][2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (BITS == 4) {   // words of the two tokens: SLAB_WORDS / 2 apart
+              const uint32_t x = __byte_perm(u[h][sg], u[h][S::SLAB_WORDS / 2 + sg], i < 2 ? 0x5410 : 0x7632) >> (8 * (i & 1));
+              f[h][0] = x & 0x000F000Fu;
+              f[h][1] = x & 0x00F000F0u;
+            } else {
+              const uint32_t x = __byte_perm(u[h][i >> 1], u[h][(S::SLAB_WORDS / 2 + (i >> 1)) % S::SLAB_WORDS], i & 1 ? 0x7632 : 0x5410);
+              f[h][0] = x & 0x00FF00FFu;
+              f[h][1] = (x >> 8) & 0x00FF00FFu;
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma16816(st.o[gi * 4 + i][n], f[0][0], f[0][1], f[1][0], f[1][1], bp[n][0], bp[n][1]);
+            if (S::FINE) mma16816(st.o[gi * 4 + i][n], f[0][0], f[0][1], f[1][0], f[1][1], bl[n][0], bl[n][1]);
+          }
+        }
+      }
+    }
+  }
+}
+
+template <class S>
+__global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const QuantAttnArgs a) {
+  constexpr int KS = S::KS, NG = S::NG, NT = S::NT, D = S::D, BITS = S::BITS, BLOCK = S::BLOCK, WARPS = S::WARPS, KB = S::KB;
   extern __shared__ __align__(128) uint8_t smem[];
   pdl_wait();
   pdl_trigger();
   const Plan plan = plan_of(a);
   const long long total = *plan.total;
+  const int first_chunk = plan.start[blockIdx.x];
   const int sw_n = a.slot_warps, kw = WARPS / sw_n, ring = a.ring;
-  const int B = ctas_of(total, gridDim.x, kw);
+  const int B = ctas_of(total, gridDim.x, a.least);
   const int b = blockIdx.x;
   if (b >= B || total == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -447,19 +679,7 @@ __global__ void __launch_bounds__(WARPS * 32, MIN_CTAS) attend_kernel(const Quan
 
   // This CTA's stages, and the chunk that the first is in.
   const long long lo = total * b / B, hi = total * (b + 1) / B;
-  const int chunks = *plan.chunks;
-  int c = 0;
-  {
-    int n = chunks;   // the last chunk with before <= lo, 32 candidates at a time
-    while (n > 1) {
-      const int step = (n + 31) / 32;
-      const int at = c + lane * step;
-      const bool below = lane * step < n && plan.table[at].before <= lo;
-      const int k = 31 - __clz(__ballot_sync(0xffffffff, below));   // lane 0 is always below
-      c += k * step;
-      n = min(step, n - k * step);
-    }
-  }
+  int c = first_chunk;
   __syncthreads();
 
   auto piece_at = [&](long long pos) {   // c: a chunk at or before pos
@@ -479,56 +699,51 @@ __global__ void __launch_bounds__(WARPS * 32, MIN_CTAS) attend_kernel(const Quan
     return p;
   };
 
-  // The producer of a key lane: its first warp.  Lane j of it holds the page of block j % 2 of stage j / 2 of 16.
-  int ids = 0, ids_next = 0, issued = 0, fill = 0, fill_phase = 1;   // stages of the piece issued; ring place
+  // The producer of a key lane is its first warp.  Lane j of it holds where block j % KB of stage j / KB is.
+  constexpr int AHEAD = 32 / KB;
+  int at_block = 0, at_next = 0, issued = 0, fill = 0, fill_phase = 1;   // stages of the piece issued; ring place
   Piece src = {};      // the piece that is being loaded
   int src_n = 0;
   const int bshift = a.page_shift - 4;
-  auto page_ids = [&](int i0) {
-    const int stage = src.first + kl + (i0 + (lane >> 1)) * kw;
-    const int blk = stage * 2 + (lane & 1);
-    int page = 0;
-    if (i0 + (lane >> 1) < src_n && blk * TOK < src.len) {
-      const int index = blk >> bshift;
-      const bool ok = src.slot >= 0 && src.slot < a.num_slots && index < a.max_pages;
-      page = ok ? a.page_table[(size_t)src.slot * a.max_pages + index] : -1;
-      if (page < 0 || page >= a.num_pages) {
-        report_error(a.err, kErrBadShape);
-        page = 0;
-      }
+  auto blocks_from = [&](int i0) {
+    const int i = i0 + lane / KB;
+    const int blk = (src.first + kl + i * kw) * KB + lane % KB;
+    if (i >= src_n || blk * TOK >= src.len) return -1;
+    const int index = blk >> bshift;
+    const bool ok = src.slot >= 0 && src.slot < a.num_slots && index < a.max_pages;
+    int page = ok ? a.page_table[(size_t)src.slot * a.max_pages + index] : -1;
+    if (page < 0 || page >= a.num_pages) {
+      report_error(a.err, kErrBadShape);
+      page = 0;
     }
-    return page;
+    return ((page * a.num_kv_heads + src.head) << bshift) + (blk & ((1 << bshift) - 1));
   };
   auto start_loads = [&](const Piece& p) {
     src = p;
-    src_n = (p.n - kl + kw - 1) / kw;
-    if (p.n <= kl) src_n = 0;
+    src_n = p.n > kl ? (p.n - kl + kw - 1) / kw : 0;
     issued = 0;
-    ids = page_ids(0);
-    ids_next = page_ids(16);
+    at_block = blocks_from(0);
+    at_next = blocks_from(AHEAD);
   };
   auto issue = [&]() {   // the next stage of the source piece into the ring
     if (issued >= src_n) return;
     mbar_wait(&empty[fill], fill_phase, a.err);
-    const int stage = src.first + kl + issued * kw;
-    const int k = issued & 15;
-    const int p0 = __shfl_sync(0xffffffff, ids, 2 * k), p1 = __shfl_sync(0xffffffff, ids, 2 * k + 1);
+    const int k = issued % AHEAD * KB;
+    const int b0 = __shfl_sync(0xffffffff, at_block, k);
+    const int b1 = KB == 2 ? __shfl_sync(0xffffffff, at_block, (k + 1) & 31) : -1;
     if (lane == 0) {
-      uint8_t* to = stage0 + (size_t)fill * S::STAGE_BYTES;
-      const int blk = stage * 2, mask = (1 << bshift) - 1;
-      const bool two = (blk + 1) * TOK < src.len;
-      mbar_expect_tx(&full[fill], two ? 2 * BLOCK : BLOCK);
-      bulk_load(to, a.data + (((((size_t)p0 * a.num_kv_heads + src.head) << bshift) + (blk & mask)) * BLOCK), BLOCK, &full[fill]);
-      if (two)
-        bulk_load(to + BLOCK, a.data + (((((size_t)p1 * a.num_kv_heads + src.head) << bshift) + ((blk + 1) & mask)) * BLOCK), BLOCK, &full[fill]);
+      uint8_t* to = stage0 + fill * S::STAGE_BYTES;
+      mbar_expect_tx(&full[fill], b1 >= 0 ? 2 * BLOCK : BLOCK);
+      bulk_load(to, a.data + (size_t)(unsigned)b0 * BLOCK, BLOCK, &full[fill]);
+      if (b1 >= 0) bulk_load(to + BLOCK, a.data + (size_t)(unsigned)b1 * BLOCK, BLOCK, &full[fill]);
     }
     if (++fill == ring) {
       fill = 0;
       fill_phase ^= 1;
     }
-    if ((++issued & 15) == 0) {
-      ids = ids_next;
-      ids_next = page_ids(issued + 16);
+    if (++issued % AHEAD == 0) {
+      at_block = at_next;
+      at_next = blocks_from(issued + AHEAD);
     }
   };
 
@@ -618,32 +833,23 @@ __global__ void __launch_bounds__(WARPS * 32, MIN_CTAS) attend_kernel(const Quan
 
     // A part of the slots that the chunk does not reach has nothing to do (but it releases the stages).
     const bool busy = sw * NT * 8 < slot_end;
-    float o[KS][NT][4], oz[NG][NT][2], l[NT][2], ref[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int i = 0; i < KS; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[i][n][j] = 0.f;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int i = 0; i < NG; ++i) oz[i][n][j] = 0.f;
-        l[n][j] = 0.f;
-        ref[n][j] = -INFINITY;
-      }
-    }
-    int lens[NT][2], shortest = INT_MAX;
-    float fac[NT][2];
+    State<S> st;
+    int shortest = INT_MAX;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int i = 0; i < KS; ++i) st.o[i][n][j] = st.o[i][n][2 + j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) st.oz[i][n][j] = 0.f;
+        st.l[n][j] = 0.f;
+        st.ref[n][j] = -INFINITY;
         const int s = (sw * NT + n) * 8 + 2 * t + j;
         const bool there = s < slot_end;
-        lens[n][j] = there ? qlen[s] : cur.len;
-        fac[n][j] = there ? qfac[s] : 0.f;
-        shortest = min(shortest, lens[n][j]);
+        st.lens[n][j] = there ? qlen[s] : cur.len;
+        st.fac[n][j] = there ? qfac[s] : 0.f;
+        shortest = min(shortest, st.lens[n][j]);
       }
     shortest = __reduce_min_sync(0xffffffff, shortest);
 
@@ -651,202 +857,11 @@ __global__ void __launch_bounds__(WARPS * 32, MIN_CTAS) attend_kernel(const Quan
     for (int it = 0; it < n_mine; ++it) {
       mbar_wait(&full[use], use_phase, a.err);
       if (busy) {
-        const uint8_t* st = stage0 + (size_t)use * S::STAGE_BYTES;
-        const int key0 = (cur.first + kl + it * kw) * STAGE;
-        // Scores.
-        float sc[2][NT][4];
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) sc[kb][n][j] = 0.f;
-        uint32_t ksz[2][2][NG];
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int r = 0; r < 2; ++r) lds(ksz[kb][r], st + kb * BLOCK + 2 * S::CODES + (g + 8 * r) * NG * 4);
-#pragma unroll
-        for (int gi = 0; gi < NG; ++gi) {
-          constexpr int WG = BITS / 2;   // words of a lane in a group
-          uint32_t w[2][2][WG];
-          constexpr bool SMALL = BITS == 4 && D == 64;
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const int row = g + 8 * r;
-              const uint8_t* p = st + kb * BLOCK +
-                                 (SMALL ? row * 32 + t * 8 : BITS == 8 ? gi * 1024 + row * 64 + t * 16 : (gi >> 1) * 1024 + row * 64 + t * 16 + (gi & 1) * 8);
-              lds(w[kb][r], p);
-            }
-          float acc[2][NT][4];
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) acc[kb][n][j] = 0.f;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t bq[NT][2];
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-              lds(bq[n], qfrag + (((gi * 4 + k) * NT * sw_n + sw * NT + n) * 32 + lane) * 8);
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-              uint32_t f[2][2];
-#pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                if (BITS == 4) {
-                  const uint32_t x = w[kb][r][k >> 1] >> (8 * (k & 1));
-                  f[r][0] = x & 0x000F000Fu;
-                  f[r][1] = x & 0x00F000F0u;
-                } else {
-                  f[r][0] = w[kb][r][k % WG] & 0x00FF00FFu;
-                  f[r][1] = (w[kb][r][k % WG] >> 8) & 0x00FF00FFu;
-                }
-              }
-#pragma unroll
-              for (int n = 0; n < NT; ++n) mma16816(acc[kb][n], f[0][0], f[1][0], f[0][1], f[1][1], bq[n][0], bq[n][1]);
-            }
-          }
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const float2 qs = *reinterpret_cast<const float2*>(qsum + gi * slots + (sw * NT + n) * 8 + 2 * t);
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const uint32_t sz = ksz[kb][j >> 1][gi];
-                sc[kb][n][j] = fmaf(scale_of(sz), acc[kb][n][j], fmaf(offset_of(sz), j & 1 ? qs.y : qs.x, sc[kb][n][j]));
-              }
-          }
-        }
-        // Weights.
-        const bool whole = key0 + STAGE <= shortest;
-        uint32_t vsz[2][2][NG];
-        float most[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) most[n][0] = most[n][1] = -INFINITY;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            lds(vsz[kb][r], st + kb * BLOCK + 2 * S::CODES + TOK * NG * 4 + (g + 8 * r) * NG * 4);
-            int top = 0x1F80;   // at least 2^-64; a poisoned scale is negative
-#pragma unroll
-            for (int gi = 0; gi < NG; ++gi) top = max(top, (int)(short)(vsz[kb][r][gi] & 0xFFFFu));
-            const float ex = __uint_as_float(0x4B000000u | (uint32_t)(top >> 7)) - (8388608.f + 127.f);
-            const int key = key0 + kb * 16 + r * 8 + g;
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                float x = sc[kb][n][2 * r + j] * fac[n][j];
-                if (!whole && key >= lens[n][j]) x = -INFINITY;
-                sc[kb][n][2 * r + j] = x;
-                most[n][j] = fmaxf(most[n][j], x + ex);
-              }
-          }
-        bool move = false;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) move = move || most[n][0] > ref[n][0] + SLACK || most[n][1] > ref[n][1] + SLACK;
-        if (__any_sync(0xffffffff, move)) {
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              float m = most[n][j];
-#pragma unroll
-              for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, x));
-              m = fmaxf(m, ref[n][j]);
-              const float f = m == ref[n][j] ? 1.f : ex2(ref[n][j] - m);
-              ref[n][j] = m;
-              l[n][j] *= f;
-#pragma unroll
-              for (int gi = 0; gi < NG; ++gi) oz[gi][n][j] *= f;
-#pragma unroll
-              for (int i = 0; i < KS; ++i) {
-                o[i][n][j] *= f;
-                o[i][n][2 + j] *= f;
-              }
-            }
-        }
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          bool seen[NT][4];
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              seen[n][j] = whole || key0 + kb * 16 + (j >> 1) * 8 + g < lens[n][j & 1];
-              const float p = seen[n][j] ? ex2(sc[kb][n][j] - ref[n][j & 1] + LIFT) : 0.f;
-              sc[kb][n][j] = p;
-              l[n][j & 1] += p;
-            }
-#pragma unroll
-          for (int gi = 0; gi < NG; ++gi) {
-            uint32_t bp[NT][2];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              float ps[4];
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const uint32_t sz = vsz[kb][j >> 1][gi];
-                ps[j] = sc[kb][n][j] * scale_of(sz);
-                float pz = sc[kb][n][j] * offset_of(sz);
-                if (!seen[n][j]) ps[j] = pz = 0.f;   // nothing of a masked key, NaN among it, is taken
-                oz[gi][n][j & 1] += pz;
-              }
-              bp[n][0] = transpose8x8(pack_f16(ps[0], ps[1]));
-              bp[n][1] = transpose8x8(pack_f16(ps[2], ps[3]));
-            }
-            // V's numbers of tokens 2t, 2t + 1 and 2t + 8, 2t + 9 for this lane's 8 dims of the group.
-            constexpr int WV = BITS / 4;   // words of 8 dims
-            uint32_t va[2][2][WV];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint8_t* vp = st + kb * BLOCK + S::CODES;
-              if constexpr (BITS == 4 && D == 64) {
-                uint32_t u[2];
-                lds(u, vp + g * 64 + (h ^ ((g >> 1) & 1)) * 32 + t * 8);
-                va[h][0][0] = u[0];
-                va[h][1][0] = u[1];
-              } else {
-                uint32_t u[4];
-                lds(u, vp + (BITS == 8 ? gi : gi >> 1) * 1024 + g * 128 + (h ^ (g & 1)) * 64 + t * 16);
-                if constexpr (BITS == 4) {
-                  va[h][0][0] = u[gi & 1];
-                  va[h][1][0] = u[2 + (gi & 1)];
-                } else {
-                  va[h][0][0] = u[0];
-                  va[h][0][WV - 1] = u[1];
-                  va[h][1][0] = u[2];
-                  va[h][1][WV - 1] = u[3];
-                }
-              }
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t f[2][2];
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                if (BITS == 4) {
-                  const uint32_t x = __byte_perm(va[h][0][0], va[h][1][0], i < 2 ? 0x5410 : 0x7632) >> (8 * (i & 1));
-                  f[h][0] = x & 0x000F000Fu;
-                  f[h][1] = x & 0x00F000F0u;
-                } else {
-                  const uint32_t x = __byte_perm(va[h][0][(i >> 1) % WV], va[h][1][(i >> 1) % WV], i & 1 ? 0x7632 : 0x5410);
-                  f[h][0] = x & 0x00FF00FFu;
-                  f[h][1] = (x >> 8) & 0x00FF00FFu;
-                }
-              }
-#pragma unroll
-              for (int n = 0; n < NT; ++n) mma16816(o[gi * 4 + i][n], f[0][0], f[0][1], f[1][0], f[1][1], bp[n][0], bp[n][1]);
-            }
-          }
-        }
+        const uint8_t* in = stage0 + use * S::STAGE_BYTES;
+        const uint8_t* qf = qfrag + (sw * NT * 32 + lane) * 8;
+        const int key0 = (cur.first + kl + it * kw) * S::KEYS;
+        if (key0 + S::KEYS <= shortest) stage_step<S, false>(st, in, qf, NT * sw_n * 256, qsum + sw * NT * 8, slots, key0, g, t);
+        else stage_step<S, true>(st, in, qf, NT * sw_n * 256, qsum + sw * NT * 8, slots, key0, g, t);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[use]);
@@ -877,14 +892,14 @@ __global__ void __launch_bounds__(WARPS * 32, MIN_CTAS) attend_kernel(const Quan
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            place[32 * r++] = ref[n][j];
-            place[32 * r++] = l[n][j];
+            place[32 * r++] = st.ref[n][j];
+            place[32 * r++] = st.l[n][j];
 #pragma unroll
-            for (int gi = 0; gi < NG; ++gi) place[32 * r++] = oz[gi][n][j];
+            for (int gi = 0; gi < NG; ++gi) place[32 * r++] = st.oz[gi][n][j];
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
-              place[32 * r++] = o[i][n][j];
-              place[32 * r++] = o[i][n][2 + j];
+              place[32 * r++] = st.o[i][n][j];
+              place[32 * r++] = st.o[i][n][2 + j];
             }
           }
         }
@@ -897,16 +912,16 @@ __global__ void __launch_bounds__(WARPS * 32, MIN_CTAS) attend_kernel(const Quan
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const float other = place[32 * r++];
-            const float m = fmaxf(ref[n][j], other);
-            const float f0 = ref[n][j] == m ? 1.f : ex2(ref[n][j] - m), f1 = other == m ? 1.f : ex2(other - m);
-            ref[n][j] = m;
-            l[n][j] = l[n][j] * f0 + place[32 * r++] * f1;
+            const float m = fmaxf(st.ref[n][j], other);
+            const float f0 = st.ref[n][j] == m ? 1.f : ex2(st.ref[n][j] - m), f1 = other == m ? 1.f : ex2(other - m);
+            st.ref[n][j] = m;
+            st.l[n][j] = st.l[n][j] * f0 + place[32 * r++] * f1;
 #pragma unroll
-            for (int gi = 0; gi < NG; ++gi) oz[gi][n][j] = oz[gi][n][j] * f0 + place[32 * r++] * f1;
+            for (int gi = 0; gi < NG; ++gi) st.oz[gi][n][j] = st.oz[gi][n][j] * f0 + place[32 * r++] * f1;
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
-              o[i][n][j] = o[i][n][j] * f0 + place[32 * r++] * f1;
-              o[i][n][2 + j] = o[i][n][2 + j] * f0 + place[32 * r++] * f1;
+              st.o[i][n][j] = st.o[i][n][j] * f0 + place[32 * r++] * f1;
+              st.o[i][n][2 + j] = st.o[i][n][2 + j] * f0 + place[32 * r++] * f1;
             }
           }
         }
@@ -923,20 +938,20 @@ __global__ void __launch_bounds__(WARPS * 32, MIN_CTAS) attend_kernel(const Quan
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int s = (sw * NT + n) * 8 + 2 * t + j;
-          float sum = l[n][j];
+          float sum = st.l[n][j];
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffff, sum, x);
-          if (g == 0 && s < done.count) *reinterpret_cast<float2*>(to + slots * D + 2 * s) = make_float2(ref[n][j], sum);
+          if (g == 0 && s < done.count) *reinterpret_cast<float2*>(to + slots * D + 2 * s) = make_float2(st.ref[n][j], sum);
 #pragma unroll
           for (int gi = 0; gi < NG; ++gi) {
-            float zz = oz[gi][n][j];
+            float zz = st.oz[gi][n][j];
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) zz += __shfl_xor_sync(0xffffffff, zz, x);
             float v[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              v[2 * i] = fmaf(o[gi * 4 + i][n][j], 0x1p24f, zz);
-              v[2 * i + 1] = fmaf(o[gi * 4 + i][n][2 + j], BITS == 4 ? 0x1p20f : 0x1p24f, zz);
+              v[2 * i] = fmaf(st.o[gi * 4 + i][n][j], 0x1p24f, zz);
+              v[2 * i + 1] = fmaf(st.o[gi * 4 + i][n][2 + j], BITS == 4 ? 0x1p20f : 0x1p24f, zz);
             }
             if (s < done.count) {
               float4* to4 = reinterpret_cast<float4*>(to + s * D + gi * GROUP + g * 8);
@@ -950,113 +965,144 @@ __global__ void __launch_bounds__(WARPS * 32, MIN_CTAS) attend_kernel(const Quan
   }
 }
 
-// Joins the records of a (row, kv head): a CTA of 8 warps.  With few records a warp takes a head; with
-// many the warps share a head's records.
-template <int D>
-__global__ void __launch_bounds__(256) join_kernel(const QuantAttnArgs a) {
+// Joins the records of a (row, q head): PARTS warps, which take every PARTS-th record, one of 32 a lane
+// first for its weight, then four at a time.
+constexpr int JOIN_WARPS = 8;
+
+template <int D, int PARTS>
+__global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const QuantAttnArgs a) {
   constexpr int PER = D / 32;
-  __shared__ float part[8][D + 2];
   pdl_wait();
   pdl_trigger();
   const Plan plan = plan_of(a);
-  const int row = blockIdx.x, kvh = blockIdx.y;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = a.num_q_heads / a.num_kv_heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % PARTS;
+  const int items = a.rows * a.num_q_heads;
+  const int at_item = blockIdx.x * (JOIN_WARPS / PARTS) + warp / PARTS;
+  const int item = min(at_item, items - 1);
+  const int row = item / a.num_q_heads, head = item % a.num_q_heads;
+  const int group = a.num_q_heads / a.num_kv_heads, kvh = head / group;
   const long long total = *plan.total;
-  const int B = ctas_of(total, a.grid, 8 / a.slot_warps);
   const int2 where = plan.rows[row];
   const int len = plan.lens[row];
-  for (int h0 = 0; h0 < group; ++h0) {
-    const int s = (row - where.y) * group + h0;
-    Chunk e = {};
-    int chunk = 0, n = 0, first = 0;
-    if (where.x >= 0) {
-      chunk = where.x + s / a.chunk;
-      e = plan.table[chunk];
-      if (e.stages > 0) {
-        const long long p0 = e.before + (long long)kvh * e.stages, p1 = p0 + e.stages - 1;
-        first = (int)(((p0 + 1) * B - 1) / total);
-        n = (int)(((p1 + 1) * B - 1) / total) - first + 1;
+  uint32_t gate[PER / 2];
+  if (a.gate != nullptr) {
+    const uint16_t* gp = static_cast<const uint16_t*>(a.gate) + (size_t)row * a.gate_row + (size_t)head * a.gate_head + lane * PER;
+#pragma unroll
+    for (int j = 0; j < PER / 2; ++j) gate[j] = reinterpret_cast<const uint32_t*>(gp)[j];
+  }
+  int n = 0, at = 0;
+  const float* rec = a.partial;
+  if (where.x >= 0) {
+    const int s = (row - where.y) * group + head % group;
+    const int chunk = where.x + s / a.chunk;
+    at = s % a.chunk;
+    const Chunk e = plan.table[chunk];
+    if (e.stages > 0) {
+      // CTA b has the stages from floor(b T / B): stage x is of CTA floor(((x + 1) B - 1) / T).
+      const int B = ctas_of(total, a.grid, a.least);
+      const long long p0 = e.before + (long long)kvh * e.stages, p1 = p0 + e.stages - 1;
+      const int first = (int)(((p0 + 1) * B - 1) / total);
+      n = (int)(((p1 + 1) * B - 1) / total) - first + 1;
+      rec += ((size_t)chunk * a.num_kv_heads + kvh + first) * a.chunk * (D + 2);
+    }
+  }
+  const size_t step = (size_t)PARTS * a.chunk * (D + 2);
+  rec += part * (size_t)a.chunk * (D + 2);
+  const int mine = n > part ? (n - part + PARTS - 1) / PARTS : 0;
+  float m = -INFINITY, l = 0.f, o[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) o[j] = 0.f;
+  for (int i0 = 0; i0 < mine; i0 += 32) {
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (i0 + lane < mine) ml = *reinterpret_cast<const float2*>(rec + (i0 + lane) * step + a.chunk * D + 2 * at);
+    const float top = fmaxf(m, warp_max(ml.x));
+    const float f = m == top ? 1.f : ex2(m - top);
+    const float w = ml.x == top ? 1.f : ex2(ml.x - top);
+    m = top;
+    l = l * f + warp_sum(i0 + lane < mine ? w * ml.y : 0.f);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) o[j] *= f;
+    const int cnt = min(32, mine - i0);
+    const float* from = rec + i0 * step + at * D + lane * PER;
+    for (int i = 0; i < cnt; i += 4) {
+      float x[4][PER];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (i + k < cnt) {
+#pragma unroll
+          for (int j = 0; j < PER; j += 2) {
+            const float2 y = *reinterpret_cast<const float2*>(from + (i + k) * step + j);
+            x[k][j] = y.x;
+            x[k][j + 1] = y.y;
+          }
+        }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float wk = __shfl_sync(0xffffffff, w, (i + k) & 31);
+        if (i + k < cnt) {
+#pragma unroll
+          for (int j = 0; j < PER; ++j) o[j] = fmaf(wk, x[k][j], o[j]);
+        }
       }
     }
-    const bool shared = n > 4;   // the same in all warps
-    if (!shared && warp != (h0 & 7)) continue;
-    const int at = s % a.chunk;
-    const float* rec = a.partial + ((size_t)chunk * a.num_kv_heads + kvh + first) * a.chunk * (D + 2);
-    float m = -INFINITY, l = 0.f, o[PER];
+  }
+  if (PARTS > 1) {
+    __shared__ float all[JOIN_WARPS][D + 2];
+    float(*parts)[D + 2] = all + warp / PARTS * PARTS;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) parts[part][j * 32 + lane] = o[j];
+    if (lane == 0) {
+      parts[part][D] = m;
+      parts[part][D + 1] = l;
+    }
+    __syncthreads();
+    if (part != 0) return;
+    m = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < PARTS; ++x) m = fmaxf(m, parts[x][D]);
+    l = 0.f;
 #pragma unroll
     for (int j = 0; j < PER; ++j) o[j] = 0.f;
-    for (int i = shared ? warp : 0; i < n; i += shared ? 8 : 1) {
-      const float* from = rec + (size_t)i * a.chunk * (D + 2);
-      const float2 ml = *reinterpret_cast<const float2*>(from + a.chunk * D + 2 * at);
-      const float mm = fmaxf(m, ml.x);
-      const float f0 = m == mm ? 1.f : ex2(m - mm), f1 = ml.x == mm ? 1.f : ex2(ml.x - mm);
-      m = mm;
-      l = l * f0 + ml.y * f1;
 #pragma unroll
-      for (int j = 0; j < PER; j += 2) {
-        const float2 x = *reinterpret_cast<const float2*>(from + at * D + lane * PER + j);
-        o[j] = o[j] * f0 + x.x * f1;
-        o[j + 1] = o[j + 1] * f0 + x.y * f1;
-      }
+    for (int x = 0; x < PARTS; ++x) {
+      const float w = parts[x][D] == m ? 1.f : ex2(parts[x][D] - m);
+      l += w * parts[x][D + 1];
+#pragma unroll
+      for (int j = 0; j < PER; ++j) o[j] = fmaf(w, parts[x][j * 32 + lane], o[j]);
     }
-    if (shared) {
-      __syncthreads();
+  }
+  if (at_item != item) return;
+  // A row without keys gives 0; one whose weights are all 0 (scores of -inf) or NaN gives NaN.
+  const float inv = 1.f / l;
+  float y[PER];
 #pragma unroll
-      for (int j = 0; j < PER; ++j) part[warp][lane * PER + j] = o[j];
-      if (lane == 0) {
-        part[warp][D] = m;
-        part[warp][D + 1] = l;
-      }
-      __syncthreads();
-      if (warp != (h0 & 7)) continue;
-      m = -INFINITY;
-      for (int i = 0; i < 8; ++i) m = fmaxf(m, part[i][D]);
-      l = 0.f;
+  for (int j = 0; j < PER; ++j) y[j] = n > 0 && len > 0 ? o[j] * inv : 0.f;
+  if (a.gate != nullptr) {
 #pragma unroll
-      for (int j = 0; j < PER; ++j) o[j] = 0.f;
-      for (int i = 0; i < 8; ++i) {
-        const float f = part[i][D] == m ? 1.f : ex2(part[i][D] - m);
-        l += part[i][D + 1] * f;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) o[j] += part[i][lane * PER + j] * f;
-      }
+    for (int j = 0; j < PER / 2; ++j) {
+      const float2 f = two_floats(gate[j], a.half);
+      y[2 * j] *= sigmoidf_(f.x);
+      y[2 * j + 1] *= sigmoidf_(f.y);
     }
-    // A row without keys gives 0; one whose weights are all 0 (scores of -inf) or NaN gives NaN.
-    const int head = kvh * group + h0;
-    const float inv = 1.f / l;
-    float y[PER];
+  }
+  if (a.out != nullptr) {
+    uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + (size_t)item * D + lane * PER);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) y[j] = len > 0 && where.x >= 0 ? o[j] * inv : 0.f;
-    if (a.gate != nullptr) {
-      const uint16_t* gp = static_cast<const uint16_t*>(a.gate) + (size_t)row * a.gate_row + (size_t)head * a.gate_head + lane * PER;
+    for (int j = 0; j < PER / 2; ++j) to[j] = two_halves(y[2 * j], y[2 * j + 1], a.half);
+  }
+  if (a.out_q != nullptr) {
+    float big = 0.f;
 #pragma unroll
-      for (int j = 0; j < PER; j += 2) {
-        const float2 f = two_floats(*reinterpret_cast<const uint32_t*>(gp + j), a.half);
-        y[j] *= sigmoidf_(f.x);
-        y[j + 1] *= sigmoidf_(f.y);
-      }
-    }
-    const size_t item = (size_t)row * a.num_q_heads + head;
-    if (a.out != nullptr) {
-      uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + item * D + lane * PER);
+    for (int j = 0; j < PER; ++j) big = fmaxf(big, fabsf(y[j]));
 #pragma unroll
-      for (int j = 0; j < PER; j += 2) to[j / 2] = two_halves(y[j], y[j + 1], a.half);
-    }
-    if (a.out_q != nullptr) {
-      float big = 0.f;
+    for (int x = 1; x < 32 / PER; x <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffff, big, x));
+    const uint8_t code = mx_scale_e8m0(big);
+    const float si = mx_inv_scale(code);
 #pragma unroll
-      for (int j = 0; j < PER; ++j) big = fmaxf(big, fabsf(y[j]));
-#pragma unroll
-      for (int x = 1; x < 32 / PER; x <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffff, big, x));
-      const uint8_t code = mx_scale_e8m0(big);
-      const float si = mx_inv_scale(code);
-#pragma unroll
-      for (int j = 0; j < PER; ++j) a.out_q[item * D + lane * PER + j] = f32_to_e4m3(y[j] * si);
-      if (lane % (32 / PER) == 0) {
-        const int kb = (head * D + lane * PER) >> 5;
-        a.out_sf[((size_t)(row >> 7) * (a.num_q_heads * D >> 7) + (kb >> 2)) * 512 + sf_atom_offset(row & 127, kb & 3)] = code;
-      }
+    for (int j = 0; j < PER; ++j) a.out_q[(size_t)item * D + lane * PER + j] = f32_to_e4m3(y[j] * si);
+    if (lane % (32 / PER) == 0) {
+      const int kb = (head * D + lane * PER) >> 5;
+      a.out_sf[((size_t)(row >> 7) * (a.num_q_heads * D >> 7) + (kb >> 2)) * 512 + sf_atom_offset(row & 127, kb & 3)] = code;
     }
   }
 }
@@ -1073,23 +1119,63 @@ int row_blocks(const QuantRowsArgs& a) {
   return (int)((items + ROW_THREADS - 1) / ROW_THREADS);
 }
 
-template <int D, int BITS, int NT, int MIN_CTAS>
+// The variant for sequences of so many query slots.
+struct Variant {
+  int tiles, warps, blocks, ctas;   // tiles of 8 slots of a warp; warps of a CTA; blocks of a stage; CTAs of an SM
+};
+constexpr Variant variant_of(int d, int bits, int slots) {
+  if (d == 256) return slots <= 8 ? Variant{1, 4, 1, bits == 4 ? 3 : 2} : Variant{2, 8, 1, 1};
+  if (slots <= 8) return {1, 8, d == 128 && bits == 8 ? 1 : 2, 2};
+  if (slots <= 16) return {2, 8, 2, d == 64 ? 2 : 1};
+  return {4, 8, d == 64 ? 2 : 1, 1};
+}
+
+template <class S>
 int launch_attend(QuantAttnArgs a, cudaStream_t stream) {
-  using S = Shape<D, BITS, NT>;
-  const int kw = WARPS / a.slot_warps;
-  const int room = (227 * 1024 / MIN_CTAS - 1024 * (MIN_CTAS > 1)) & ~127;
+  const int kw = S::WARPS / a.slot_warps;
+  const int room = (227 * 1024 / S::CTAS - 1024 * (S::CTAS > 1)) & ~127;
   a.ring_offset = (S::fixed(a.slot_warps) + 127) & ~127;
   a.ring = (room - a.ring_offset) / (kw * S::STAGE_BYTES);
   if (a.ring > MAX_RING) a.ring = MAX_RING;
-  if (a.ring < 1 || a.chunk != S::slots(a.slot_warps)) return -1;
+  if (a.ring < 1 || a.chunk != S::slots(a.slot_warps) || a.stage != S::KEYS) return -1;
   const int bytes = a.ring_offset + kw * a.ring * S::STAGE_BYTES;
-  a.grid = 148 * MIN_CTAS;
-  if (a.grid > ZS_QUANT_CTAS) return -1;
-  const auto kernel = attend_kernel<D, BITS, NT, MIN_CTAS>;
+  const auto kernel = attend_kernel<S>;
   cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  zs_launch(kernel, a.grid, WARPS * 32, bytes, stream, a);
-  zs_launch(join_kernel<D>, dim3(a.rows, a.num_kv_heads), 256, 0, stream, a);
+  zs_launch(kernel, a.grid, S::WARPS * 32, bytes, stream, a);
+  // Warps that share a pair's records: with few pairs a long sequence leaves a record in every CTA.
+  const long long items = (long long)a.rows * a.num_q_heads;
+  int parts = JOIN_WARPS;
+  while (parts > 1 && items * parts > 4096) parts /= 2;
+  const auto join = parts == 8 ? join_kernel<S::D, 8> : parts == 4 ? join_kernel<S::D, 4> : parts == 2 ? join_kernel<S::D, 2> : join_kernel<S::D, 1>;
+  zs_launch(join, (int)((items * parts + JOIN_WARPS - 1) / JOIN_WARPS), JOIN_WARPS * 32, 0, stream, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
+}
+
+template <int D, int BITS, int SLOTS, bool FINE>
+int launch_variant(const QuantAttnArgs& a, cudaStream_t stream) {
+  constexpr Variant v = variant_of(D, BITS, SLOTS);
+  return launch_attend<Shape<D, BITS, v.tiles, v.warps, v.blocks, v.ctas, FINE>>(a, stream);
+}
+
+template <int D, int BITS, bool FINE>
+int launch_tiles(const QuantAttnArgs& a, cudaStream_t stream) {
+  if (a.tiles == 1) return launch_variant<D, BITS, 8, FINE>(a, stream);
+  if (a.tiles == 2) return launch_variant<D, BITS, 16, FINE>(a, stream);
+  if constexpr (D < 256) return launch_variant<D, BITS, 32, FINE>(a, stream);
+  return -1;
+}
+
+template <int D>
+int launch_bits(const QuantAttnArgs& a, cudaStream_t stream) {
+  if (a.bits == 4) return a.half ? launch_tiles<D, 4, true>(a, stream) : launch_tiles<D, 4, false>(a, stream);
+  return a.half ? launch_tiles<D, 8, true>(a, stream) : launch_tiles<D, 8, false>(a, stream);
+}
+
+// CTAs of the attention, and the fewest stages that are worth one (a stage a key lane).
+void set_grid(QuantAttnArgs& a) {
+  const Variant v = variant_of(a.head_dim, a.bits, 8 * a.tiles);
+  a.grid = 148 * v.ctas;
+  a.least = v.warps / a.slot_warps;
 }
 
 int check_attn(const QuantAttnArgs& a) {
@@ -1119,49 +1205,36 @@ extern "C" int zs_quant_load(const QuantRowsArgs* args, cudaStream_t stream) {
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
-// Tiles of 8 slots a warp holds (its sums are D / 4 registers a tile), and the warps that share a key lane.
-extern "C" void zs_quant_attn_shape(int head_dim, int slots, int* tiles, int* slot_warps) {
-  const int most = head_dim == 256 ? 2 : 4;
-  *tiles = 1;
-  while (*tiles < most && 8 * *tiles < slots) *tiles *= 2;
+// The variant for sequences of `slots` query slots: tiles of 8 slots of a warp, warps that share a key lane, keys
+// of a stage.
+extern "C" void zs_quant_attn_shape(int head_dim, int bits, int slots, int* tiles, int* slot_warps, int* stage) {
+  const zs::qc::Variant v = zs::qc::variant_of(head_dim, bits, slots);
+  *tiles = v.tiles;
+  *stage = v.blocks * zs::qc::TOK;
   *slot_warps = 1;
-  while (*slot_warps < zs::qc::WARPS && 8 * *tiles * *slot_warps < slots) *slot_warps *= 2;
+  while (*slot_warps < v.warps && 8 * v.tiles * *slot_warps < slots) *slot_warps *= 2;
 }
 
 extern "C" long long zs_quant_attn_work(int max_chunks, int max_rows, int max_seqs) {
-  return 32 + (long long)max_chunks * 32 + (long long)max_rows * 12 + (long long)max_seqs * 4;
+  return 32 + (long long)max_chunks * 32 + (long long)max_rows * 12 + (long long)(ZS_QUANT_CTAS + max_seqs) * 4;
 }
 
 extern "C" int zs_quant_attn_plan(const QuantAttnArgs* args, cudaStream_t stream) {
   if (int e = zs::qc::check_attn(*args)) return e;
-  zs_launch(zs::qc::plan_kernel, 1, zs::qc::PLAN_THREADS, 0, stream, *args);
+  QuantAttnArgs a = *args;
+  zs::qc::set_grid(a);
+  zs_launch(zs::qc::plan_kernel, 1, zs::qc::PLAN_THREADS, 0, stream, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
 extern "C" int zs_quant_attn(const QuantAttnArgs* args, cudaStream_t stream) {
   using namespace zs::qc;
-  const QuantAttnArgs& a = *args;
+  QuantAttnArgs a = *args;
   if (int e = check_attn(a)) return e;
+  set_grid(a);
   if (a.num_pages < 1 || a.num_slots < 1 || a.max_pages < 1 || a.page_shift < 4 || a.page_shift > 8 || a.partial == nullptr) return -1;
   if (a.rows == 0) return 0;
-#define ZS_QUANT_CASE(d, bits_, nt, ctas) \
-  if (a.head_dim == d && a.bits == bits_ && a.tiles == nt) return launch_attend<d, bits_, nt, ctas>(a, stream);
-  ZS_QUANT_CASE(64, 4, 1, 2)
-  ZS_QUANT_CASE(64, 4, 2, 2)
-  ZS_QUANT_CASE(64, 4, 4, 1)
-  ZS_QUANT_CASE(64, 8, 1, 2)
-  ZS_QUANT_CASE(64, 8, 2, 2)
-  ZS_QUANT_CASE(64, 8, 4, 1)
-  ZS_QUANT_CASE(128, 4, 1, 2)
-  ZS_QUANT_CASE(128, 4, 2, 1)
-  ZS_QUANT_CASE(128, 4, 4, 1)
-  ZS_QUANT_CASE(128, 8, 1, 2)
-  ZS_QUANT_CASE(128, 8, 2, 1)
-  ZS_QUANT_CASE(128, 8, 4, 1)
-  ZS_QUANT_CASE(256, 4, 1, 1)
-  ZS_QUANT_CASE(256, 4, 2, 1)
-  ZS_QUANT_CASE(256, 8, 1, 1)
-  ZS_QUANT_CASE(256, 8, 2, 1)
-#undef ZS_QUANT_CASE
-  return -1;
+  if (a.head_dim == 64) return launch_bits<64>(a, stream);
+  if (a.head_dim == 128) return launch_bits<128>(a, stream);
+  return launch_bits<256>(a, stream);
 }

@@ -720,7 +720,7 @@ int zs_ipc_close(void* ptr);
 // ----------------------------------------------------------------------------------
 // K/V cache held in 4 or 8 bits (quant_cache.cu).  One layer: [pages][kv_heads][page / 16 blocks].
 // ----------------------------------------------------------------------------------
-#define ZS_QUANT_CTAS 296   // most CTAs of zs_quant_attn
+#define ZS_QUANT_CTAS 592   // most CTAs of zs_quant_attn
 
 typedef struct QuantRowsArgs {
   uint8_t* data;            // the layer
@@ -761,7 +761,7 @@ typedef struct QuantAttnArgs {
   long long gate_row, gate_head;
   int half;                 // f16 instead of bf16
   float sm_scale;
-  int tiles, slot_warps;    // zs_quant_attn_shape
+  int tiles, slot_warps, stage;   // zs_quant_attn_shape
   int chunk;                // slots of a unit: 8 * tiles * slot_warps
   int max_chunks;
   void* work;               // zs_quant_attn_work bytes, 32-byte aligned
@@ -769,11 +769,11 @@ typedef struct QuantAttnArgs {
   void* out;                // [rows, heads * dim] like q, or NULL
   uint8_t* out_q;           // MXFP8 of the same, or NULL
   uint8_t* out_sf;
-  int ring, ring_offset, grid;   // set by the launcher
+  int ring, ring_offset, grid, least;   // set by the launcher
   int* err;
 } QuantAttnArgs;
 
-void zs_quant_attn_shape(int head_dim, int slots, int* tiles, int* slot_warps);
+void zs_quant_attn_shape(int head_dim, int bits, int slots, int* tiles, int* slot_warps, int* stage);
 long long zs_quant_attn_work(int max_chunks, int max_rows, int max_seqs);
 int zs_quant_attn_plan(const QuantAttnArgs* args, cudaStream_t stream);   // once a step
 int zs_quant_attn(const QuantAttnArgs* args, cudaStream_t stream);        // once a layer

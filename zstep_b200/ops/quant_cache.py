@@ -39,38 +39,28 @@ class QuantCache:
             raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
         if layers < 1 or num_pages < 1 or num_kv_heads < 1:
             raise ValueError("layers, num_pages and num_kv_heads must be positive")
-        self.C = _ext.load()
+        C = _ext.load()
         self.layers, self.num_pages, self.num_kv_heads = layers, num_pages, num_kv_heads
         self.head_dim, self.bits, self.page_size = head_dim, bits, page_size
-        self.page_bytes = num_kv_heads * (page_size // BLOCK) * self.C.quant_block_bytes(head_dim, bits)
+        self.page_bytes = num_kv_heads * (page_size // BLOCK) * C.quant_block_bytes(head_dim, bits)
         self.data = torch.zeros(layers, num_pages, self.page_bytes, dtype=torch.uint8, device=device)
         self.err = torch.zeros(1, dtype=torch.int32, device=device)
-
-    def _layer(self, layer: int) -> torch.Tensor:
-        if not 0 <= layer < self.layers:
-            raise ValueError(f"layer {layer} outside the {self.layers} layers")
-        return self.data[layer]
+        self.state = C.QuantCacheState(self.data, num_kv_heads, head_dim, bits, page_size, self.err)
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, slots: torch.Tensor,
               positions: torch.Tensor) -> None:
         """Quantise the rows ``k`` and ``v`` [rows, kv heads, dim] (bf16 or f16; rows and heads may be strided)
         into token ``positions`` [rows] (int32) of the sequences ``slots`` [rows] (int32; rows of ``page_table``).
         A row with a negative position is not written.  Two rows must not name one place."""
-        self.C.quant_rows(True, self._layer(layer), self.num_kv_heads, self.head_dim, self.bits, self.page_size, page_table,
-                          slots, positions, k, v, self.err)
+        self.state.write(layer, k, v, page_table, slots, positions)
 
     def read(self, layer: int, page_table: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor,
              dtype: torch.dtype = torch.bfloat16, k: torch.Tensor | None = None,
              v: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """The values held at ``positions`` of ``slots``: two tensors [rows, kv heads, dim] of ``dtype`` (bf16, f16 or
-        f32), or ``k`` and ``v`` (rows and heads may be strided) where they are given.  A row with a negative
-        position is 0."""
-        shape = (slots.numel(), self.num_kv_heads, self.head_dim)
-        k = torch.empty(shape, dtype=dtype, device=self.data.device) if k is None else k
-        v = torch.empty(shape, dtype=dtype if k is None else k.dtype, device=self.data.device) if v is None else v
-        self.C.quant_rows(False, self._layer(layer), self.num_kv_heads, self.head_dim, self.bits, self.page_size, page_table,
-                          slots, positions, k, v, self.err)
-        return k, v
+        f32), or ``k`` and ``v`` (of one such type; rows and heads may be strided) where they are given.  A row with
+        a negative position is 0."""
+        return self.state.read(layer, page_table, slots, positions, dtype, k, v)
 
     def check(self) -> None:
         """Raise if a write or read since the last check named a place outside the cache (reads the error word)."""
@@ -87,28 +77,16 @@ class QuantAttention:
     workspace holds one step: calls of one object follow one another on a stream."""
 
     def __init__(self, cache: QuantCache, num_q_heads: int, max_rows: int, max_seqs: int | None = None, max_seq_rows: int = 1):
-        max_seqs = max_rows if max_seqs is None else max_seqs
-        if num_q_heads < 1 or num_q_heads % cache.num_kv_heads:
-            raise ValueError(f"{num_q_heads} q heads are not a multiple of {cache.num_kv_heads} kv heads")
-        if max_rows < 1 or max_seqs < 1 or max_seq_rows < 1:
-            raise ValueError("max_rows, max_seqs and max_seq_rows must be positive")
-        self.C, self.cache = cache.C, cache
-        self.num_q_heads, self.max_rows, self.max_seqs, self.max_seq_rows = num_q_heads, max_rows, max_seqs, max_seq_rows
-        work, partial, *_ = self.C.quant_attn_sizes(num_q_heads, cache.num_kv_heads, cache.head_dim, max_rows, max_seqs, max_seq_rows)
-        dev = cache.data.device
-        self._work = torch.zeros(work, dtype=torch.uint8, device=dev)
-        self._partial = torch.empty(partial, dtype=torch.float32, device=dev)
-        self.err = torch.zeros(1, dtype=torch.int32, device=dev)
-        self._planned: tuple[int, int] | None = None   # rows and sequences of the last update
+        self.cache, self.num_q_heads = cache, num_q_heads
+        self.max_rows, self.max_seqs, self.max_seq_rows = max_rows, max_rows if max_seqs is None else max_seqs, max_seq_rows
+        self.err = torch.zeros(1, dtype=torch.int32, device=cache.data.device)
+        self.state = _ext.load().QuantPlanState(cache.state, num_q_heads, max_rows, self.max_seqs, max_seq_rows, self.err)
 
     def update(self, slots: torch.Tensor, seq_lens: torch.Tensor, seq_start: torch.Tensor | None = None) -> None:
         """Divide a step's keys over the GPU.  ``slots`` [rows] and ``seq_lens`` [rows] (int32): the sequence of each
         row and the keys it sees (0: none).  ``seq_start`` [sequences + 1] (int32): rows seq_start[i] to
         seq_start[i+1] are of one sequence and read its keys together; None: every row reads its own."""
-        self._planned = None
-        self.C.quant_attn_plan(self.num_q_heads, self.cache.num_kv_heads, self.cache.head_dim, self.cache.bits, self.max_rows,
-                               self.max_seqs, self.max_seq_rows, slots, seq_lens, seq_start, self._work, self._partial, self.err)
-        self._planned = (slots.numel(), slots.numel() if seq_start is None else seq_start.numel() - 1)
+        self.state.update(slots, seq_lens, seq_start)
 
     def attend(self, layer: int, q: torch.Tensor, page_table: torch.Tensor, sm_scale: float, gate: torch.Tensor | None = None,
                out: torch.Tensor | None = None, out_q: torch.Tensor | None = None,
@@ -117,17 +95,7 @@ class QuantAttention:
         the rows of the last ``update``; ``gate`` None: no gate.  The result goes to ``out`` ([rows, heads * dim]
         of q's type, allocated unless the MXFP8 pair ``out_q``, ``out_sf`` is given alone).  A row without keys, or
         of no sequence, gives 0."""
-        if self._planned is None:
-            raise RuntimeError("attend needs an update first")
-        rows, seqs = self._planned
-        if q.dim() != 3 or q.shape[0] != rows or q.shape[1] != self.num_q_heads:
-            raise ValueError(f"q must be [{rows}, {self.num_q_heads}, {self.cache.head_dim}], got {tuple(q.shape)}")
-        if out is None and out_q is None:
-            out = torch.empty(rows, self.num_q_heads * self.cache.head_dim, dtype=q.dtype, device=q.device)
-        c = self.cache
-        self.C.quant_attn(c._layer(layer), c.num_kv_heads, c.head_dim, c.bits, c.page_size, seqs, self.max_rows, self.max_seqs,
-                          self.max_seq_rows, q, gate, page_table, sm_scale, out, out_q, out_sf, self._work, self._partial, self.err)
-        return out
+        return self.state.attend(self.cache.state, layer, q, page_table, sm_scale, gate, out, out_q, out_sf)
 
     def check(self) -> None:
         """Raise if a call since the last check met a slot, page or sequence that does not fit (reads the error word)."""
