@@ -10,16 +10,18 @@
 // Storage.  16 tokens of one kv head are one block: the numbers of K, those of V, then a 32-bit
 // (s | z << 16) per token and group, of K and of V.  The order of the numbers is the one in which
 // the attention's matrix fragments want them (k_offset, v_offset): a lane reads 16 bytes that are
-// its own, the eight lanes of a phase touch 32 different banks, and a block is one bulk copy.
+// its own, a warp 512 in a row, and a block is one bulk copy.
 //
 // Attention.  With q . K_j = sum over groups of s (q . n) + z (sum of q), and the same for
 // sum_j p_j V_j = sum_j (p_j s) n_j + p_j z, the whole numbers themselves are the matrix operand:
-// (w & 0x000F000F) of a 32-bit word of eight numbers is two f16 subnormals n 2^-24, exact, and
-// (w & 0x00F000F0) the next two times 16.  So a pair costs one or two integer instructions and no
-// multiplication; scales go to the 32-bit scores and to the weights.  The scaled weights are
-// rounded to f16 (2^-11): the running reference of a row is the maximum of score + log2(scale), so
-// that they stay below 2^15 whatever the size of V.
+// (w & 0x000F000F) of a word of eight is two f16 subnormals n 2^-24, exact, and (w & 0x00F000F0) the next two
+// times 16.  A pair costs one integer instruction and a part of a shift, and no multiplication; scales go to the
+// 32-bit scores and to the weights.  The scaled weights are rounded to f16 (2^-11; for f16 outputs a second
+// product takes what that cuts off): the running reference of a row bounds score + log2(scale), so that
+// they stay below 2^15 whatever the size of V.
 #include <cuda_fp16.h>
+
+#include <climits>
 
 #include "sm100_common.cuh"
 #include "zs_kernels.h"
@@ -35,21 +37,17 @@ constexpr uint32_t POISON = 0x7FFFFFFFu;  // z = NaN, s = NaN with its sign set 
 __host__ __device__ constexpr int code_bytes(int d, int bits) { return TOK * d * bits / 8; }
 __host__ __device__ constexpr int block_bytes(int d, int bits) { return 2 * code_bytes(d, bits) + 2 * TOK * (d / GROUP) * 4; }
 
-// Where the 8 numbers of dims d..d+7 (d a multiple of 8) of K's token t are in the block: bits bytes.
-__device__ __forceinline__ int k_offset(int dim, int bits, int t, int d) {
-  const int lane = (d & 63) >> 4, half = (d >> 3) & 1;   // of the four lanes of a row, 16 dims each
-  if (bits == 8) return (d >> 6) * 1024 + t * 64 + lane * 16 + half * 8;
-  if (dim == 64) return t * 32 + lane * 8 + half * 4;
-  return (d >> 7) * 1024 + t * 64 + lane * 16 + ((d >> 6) & 1) * 8 + half * 4;
+// Where the 8 numbers of dims d..d+7 (d a multiple of 8) of K's token t are in the block: `bits` bytes.  Rows
+// g and g + 8 of a fragment are the tokens 2g and 2g + 1, and four lanes have 16 dims of a group each.
+__device__ __forceinline__ int k_offset(int bits, int t, int d) {
+  const int lane = (d & 63) >> 4, half = (d >> 3) & 1;
+  if (bits == 8) return (d >> 6) * 1024 + (t & 1) * 512 + (t >> 1) * 64 + lane * 16 + half * 8;
+  return (d >> 6) * 512 + (t >> 1) * 64 + lane * 16 + (t & 1) * 8 + half * 4;
 }
-
-// The same of V's: eight lanes have 8 dims of a group each, for all 16 tokens.  The two halves of the
-// tokens are exchanged in every second of them, which spreads a phase over all banks.
-__device__ __forceinline__ int v_offset(int dim, int bits, int t, int d) {
-  const int lane = (d & 63) >> 3;
-  if (bits == 4 && dim == 64) return lane * 64 + ((t >> 3) ^ ((lane >> 1) & 1)) * 32 + (t & 7) * 4;
-  const int at = lane * 128 + ((t >> 3) ^ (lane & 1)) * 64 + (t & 7) * 8;
-  return bits == 8 ? (d >> 6) * 1024 + at : (d >> 7) * 1024 + at + ((d >> 6) & 1) * 4;
+// V is held by fours of tokens: byte t & 3 of a word is token t's.  With 4 bits the 8 dims d..d+7 are a byte
+// each two in 4 words in a row, with 8 bits a byte each in 4 words and 4 more 512 bytes on.
+__device__ __forceinline__ int v_offset(int bits, int t, int d) {
+  return (d >> 6) * (bits * 128) + ((d & 63) >> 3) * 64 + (t >> 2) * 16;
 }
 
 __device__ __forceinline__ float bf16_up(float x) {   // x >= 0
@@ -92,111 +90,165 @@ __device__ __forceinline__ uint8_t* block_at(const QuantRowsArgs& a, int row, in
   return a.data + (((size_t)page * a.num_kv_heads << (a.page_shift - 4)) + sub) * block_bytes(a.head_dim, a.bits);
 }
 
-// Eight dims a thread, eight threads a group.
-constexpr int ROW_THREADS = 256;
+// Rows go by fours: a warp has one group of 64 dims of four rows, eight dims a lane, and walks `a.share`-th
+// parts of the groups of K and V of all heads.
+constexpr int ROW_WARPS = 8;
 
-__global__ void __launch_bounds__(ROW_THREADS) store_kernel(const QuantRowsArgs a) {
+struct RowLane {
+  uint8_t* block;   // of the lane's row for kv head 0, or null
+  int row, token;
+};
+__device__ __forceinline__ RowLane row_lane(const QuantRowsArgs& a, int quad) {
+  RowLane r;
+  r.row = quad * 4 + ((threadIdx.x & 31) >> 3);
+  r.token = 0;
+  r.block = r.row < a.rows ? block_at(a, r.row, &r.token) : nullptr;
+  return r;
+}
+
+template <int BITS>
+__global__ void __launch_bounds__(ROW_WARPS * 32) store_kernel(const QuantRowsArgs a) {
   pdl_wait();
   pdl_trigger();
-  const int octets = a.head_dim / 8;
-  const long long item = (long long)blockIdx.x * ROW_THREADS + threadIdx.x;
-  const int d = (int)(item % octets) * 8;
-  const long long rest = item / octets;
-  const int head = (int)(rest % a.num_kv_heads);
-  const bool is_v = (rest / a.num_kv_heads) & 1;
-  const long long row = rest / a.num_kv_heads / 2;
-  if (row >= a.rows) return;   // whole groups of eight threads
-  const unsigned mates = 0xFFu << (threadIdx.x & 24);
-  const long long from = is_v ? row * a.v_row + head * a.v_head : row * a.k_row + head * a.k_head;
-  const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(is_v ? a.v : a.k) + from + d);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-  float x[8];
+  const int lane = threadIdx.x & 31;
+  const int w = blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
+  const int quad = w / a.share;
+  if (quad * 4 >= a.rows) return;
+  const RowLane r = row_lane(a, quad);
+  const int groups = a.head_dim / GROUP, items = 2 * a.num_kv_heads * groups, octet = lane & 7;
+  const int codes = code_bytes(a.head_dim, BITS), head_bytes = block_bytes(a.head_dim, BITS) << (a.page_shift - 4);
+  constexpr int TOP = (1 << BITS) - 1;
+  // Four rows that are the four tokens of one word of V's are written as words.
+  const long long first = __shfl_sync(0xffffffff, (long long)r.block, 0);
+  const int token = __shfl_sync(0xffffffff, r.token, 0);
+  const bool whole = __all_sync(0xffffffff, r.block != nullptr && (long long)r.block == first && (token & 3) == 0 && r.token == token + (lane >> 3));
+  for (int i = w % a.share; i < items; i += a.share) {
+    const int gi = i % groups, head = i / groups % a.num_kv_heads;
+    const bool is_v = i >= items / 2;
+    const int d = gi * GROUP + octet * 8;
+    float x[8];
+    if (r.row < a.rows) {
+      const long long from = is_v ? r.row * a.v_row + head * a.v_head : r.row * a.k_row + head * a.k_head;
+      const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(is_v ? a.v : a.k) + from + d);
+      const uint32_t word[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 f = two_floats(w[j], a.half);
-    x[2 * j] = f.x;
-    x[2 * j + 1] = f.y;
-  }
-  float lo = x[0], hi = x[0];
-  bool fine = true;
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = two_floats(word[j], a.half);
+        x[2 * j] = f.x;
+        x[2 * j + 1] = f.y;
+      }
+    } else {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    lo = fminf(lo, x[j]);
-    hi = fmaxf(hi, x[j]);
-    fine = fine && fabsf(x[j]) <= 0x1p126f;
-  }
+      for (int j = 0; j < 8; ++j) x[j] = 0.f;
+    }
+    float lo = x[0], hi = x[0];
+    bool fine = true;
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(mates, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(mates, hi, o));
-  }
-  fine = (__ballot_sync(mates, fine) & mates) == mates;
-  const int top = (1 << a.bits) - 1;
-  const float z = bf16_down(lo);
-  const float s = bf16_up(__fdiv_rn(hi - z, (float)top));
-  uint32_t n[2] = {0, 0};
+    for (int j = 0; j < 8; ++j) {
+      lo = fminf(lo, x[j]);
+      hi = fmaxf(hi, x[j]);
+      fine = fine && fabsf(x[j]) <= 0x1p126f;
+    }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    float q = s > 0.f ? rintf(__fdiv_rn(x[j] - z, s)) : 0.f;
-    q = fine ? fminf(fmaxf(q, 0.f), (float)top) : 0.f;
-    if (a.bits == 4) n[0] |= (uint32_t)q << (4 * j);
-    else n[j >> 2] |= (uint32_t)q << (8 * (j & 3));
-  }
-  int t = 0;
-  uint8_t* block = block_at(a, (int)row, &t);
-  if (block == nullptr) return;
-  block += ((size_t)head << (a.page_shift - 4)) * block_bytes(a.head_dim, a.bits);
-  const int codes = code_bytes(a.head_dim, a.bits), groups = a.head_dim / GROUP;
-  uint8_t* to = is_v ? block + codes + v_offset(a.head_dim, a.bits, t, d) : block + k_offset(a.head_dim, a.bits, t, d);
-  if (a.bits == 4) *reinterpret_cast<uint32_t*>(to) = n[0];
-  else *reinterpret_cast<uint2*>(to) = make_uint2(n[0], n[1]);
-  if ((d & 63) == 0) {
-    uint32_t* sz = reinterpret_cast<uint32_t*>(block + 2 * codes) + (is_v ? TOK * groups : 0) + t * groups + d / GROUP;
-    *sz = fine ? __float_as_uint(s) >> 16 | __float_as_uint(z) : POISON;
+    for (int o = 1; o < 8; o <<= 1) {
+      lo = fminf(lo, __shfl_xor_sync(0xffffffff, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffff, hi, o));
+    }
+    const uint32_t mates = 0xFFu << (lane & 24);
+    fine = (__ballot_sync(0xffffffff, fine) & mates) == mates;
+    const float z = bf16_down(lo);
+    const float s = bf16_up(__fdiv_rn(hi - z, (float)TOP));
+    uint32_t n[BITS / 4] = {};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float q = s > 0.f ? rintf(__fdiv_rn(x[j] - z, s)) : 0.f;
+      q = fine ? fminf(fmaxf(q, 0.f), (float)TOP) : 0.f;
+      n[j * BITS / 32] |= (uint32_t)q << (BITS * j & 31);
+    }
+    uint8_t* block = r.block + (size_t)head * head_bytes;
+    if (!is_v) {
+      if (r.block != nullptr) {
+        uint8_t* to = block + k_offset(BITS, r.token, d);
+        if constexpr (BITS == 4) *reinterpret_cast<uint32_t*>(to) = n[0];
+        else *reinterpret_cast<uint2*>(to) = make_uint2(n[0], n[1]);
+      }
+    } else if (whole) {
+      // Lane r of a four gets bytes r of all four rows: word r (and r + 4).
+      const int mine = lane >> 3;
+#pragma unroll
+      for (int h = 0; h < BITS / 4; ++h) {
+        uint32_t word = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t other = __shfl_sync(0xffffffff, n[h], k * 8 + octet);
+          word |= (other >> (8 * mine) & 255u) << (8 * k);
+        }
+        *reinterpret_cast<uint32_t*>(block + codes + v_offset(BITS, r.token, d) + h * 512 + mine * 4) = word;
+      }
+    } else if (r.block != nullptr) {
+      uint8_t* to = block + codes + v_offset(BITS, r.token, d) + (r.token & 3);
+#pragma unroll
+      for (int j = 0; j < BITS; ++j) to[(j >> 2) * 512 + (j & 3) * 4] = (uint8_t)(n[j >> 2] >> (8 * (j & 3)));
+    }
+    if (octet == 0 && r.block != nullptr) {
+      uint32_t* sz = reinterpret_cast<uint32_t*>(block + 2 * codes) + (is_v ? TOK * groups : 0) + r.token * groups + gi;
+      *sz = fine ? __float_as_uint(s) >> 16 | __float_as_uint(z) : POISON;
+    }
   }
 }
 
-__global__ void __launch_bounds__(ROW_THREADS) load_kernel(const QuantRowsArgs a) {
+template <int BITS>
+__global__ void __launch_bounds__(ROW_WARPS * 32) load_kernel(const QuantRowsArgs a) {
   pdl_wait();
   pdl_trigger();
-  const int octets = a.head_dim / 8;
-  const long long item = (long long)blockIdx.x * ROW_THREADS + threadIdx.x;
-  const int d = (int)(item % octets) * 8;
-  const long long rest = item / octets;
-  const int head = (int)(rest % a.num_kv_heads);
-  const bool is_v = (rest / a.num_kv_heads) & 1;
-  const long long row = rest / a.num_kv_heads / 2;
-  if (row >= a.rows) return;
-  int t = 0;
-  const uint8_t* block = block_at(a, (int)row, &t);
-  float x[8];
+  const int lane = threadIdx.x & 31;
+  const int w = blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
+  const int quad = w / a.share;
+  if (quad * 4 >= a.rows) return;
+  const RowLane r = row_lane(a, quad);
+  if (r.row >= a.rows) return;
+  const int groups = a.head_dim / GROUP, items = 2 * a.num_kv_heads * groups, octet = lane & 7;
+  const int codes = code_bytes(a.head_dim, BITS), head_bytes = block_bytes(a.head_dim, BITS) << (a.page_shift - 4);
+#pragma unroll 4
+  for (int i = w % a.share; i < items; i += a.share) {
+    const int gi = i % groups, head = i / groups % a.num_kv_heads;
+    const bool is_v = i >= items / 2;
+    const int d = gi * GROUP + octet * 8;
+    float x[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) x[j] = 0.f;
-  if (block != nullptr) {
-    block += ((size_t)head << (a.page_shift - 4)) * block_bytes(a.head_dim, a.bits);
-    const int codes = code_bytes(a.head_dim, a.bits), groups = a.head_dim / GROUP;
-    const uint8_t* from = is_v ? block + codes + v_offset(a.head_dim, a.bits, t, d) : block + k_offset(a.head_dim, a.bits, t, d);
-    const uint32_t sz = *(reinterpret_cast<const uint32_t*>(block + 2 * codes) + (is_v ? TOK * groups : 0) + t * groups + d / GROUP);
-    const float s = scale_of(sz), z = offset_of(sz);
-    if (a.bits == 4) {
-      const uint32_t n = *reinterpret_cast<const uint32_t*>(from);
+    for (int j = 0; j < 8; ++j) x[j] = 0.f;
+    if (r.block != nullptr) {
+      const uint8_t* block = r.block + (size_t)head * head_bytes;
+      const uint32_t sz = *(reinterpret_cast<const uint32_t*>(block + 2 * codes) + (is_v ? TOK * groups : 0) + r.token * groups + gi);
+      uint32_t n[BITS / 4];
+      if (is_v) {
+        const uint32_t pick = (r.token & 3) * 0x11 + 0x40;   // this token's byte of two words
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = fmaf((float)(n >> (4 * j) & 15), s, z);
-    } else {
-      const uint2 n = *reinterpret_cast<const uint2*>(from);
+        for (int h = 0; h < BITS / 4; ++h) {
+          const uint4 u = *reinterpret_cast<const uint4*>(block + codes + v_offset(BITS, r.token, d) + h * 512);
+          n[h] = __byte_perm(__byte_perm(u.x, u.y, pick), __byte_perm(u.z, u.w, pick), 0x5410);
+        }
+      } else if constexpr (BITS == 4) {
+        n[0] = *reinterpret_cast<const uint32_t*>(block + k_offset(4, r.token, d));
+      } else {
+        const uint2 u = *reinterpret_cast<const uint2*>(block + k_offset(8, r.token, d));
+        n[0] = u.x;
+        n[BITS / 4 - 1] = u.y;
+      }
+      const float s = scale_of(sz), z = offset_of(sz);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = fmaf((float)((j < 4 ? n.x : n.y) >> (8 * (j & 3)) & 255), s, z);
+      for (int j = 0; j < 8; ++j) x[j] = fmaf((float)(n[j * BITS / 32] >> (BITS * j & 31) & ((1 << BITS) - 1)), s, z);
     }
-  }
-  const long long to = is_v ? row * a.v_row + head * a.v_head : row * a.k_row + head * a.k_head;
-  void* out = const_cast<void*>(is_v ? a.v : a.k);
-  if (a.f32) {
-    float4* o = reinterpret_cast<float4*>(static_cast<float*>(out) + to + d);
-    o[0] = make_float4(x[0], x[1], x[2], x[3]);
-    o[1] = make_float4(x[4], x[5], x[6], x[7]);
-  } else {
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + to + d) =
-        make_uint4(two_halves(x[0], x[1], a.half), two_halves(x[2], x[3], a.half), two_halves(x[4], x[5], a.half), two_halves(x[6], x[7], a.half));
+    const long long to = (is_v ? r.row * a.v_row + head * a.v_head : r.row * a.k_row + head * a.k_head) + d;
+    void* out = const_cast<void*>(is_v ? a.v : a.k);
+    if (a.f32) {
+      float4* o = reinterpret_cast<float4*>(static_cast<float*>(out) + to);
+      o[0] = make_float4(x[0], x[1], x[2], x[3]);
+      o[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + to) =
+          make_uint4(two_halves(x[0], x[1], a.half), two_halves(x[2], x[3], a.half), two_halves(x[4], x[5], a.half), two_halves(x[6], x[7], a.half));
+    }
   }
 }
 
@@ -358,6 +410,12 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma16816_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ float ex2(float x) {   // 2^x, results below 2^-126 as 0
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -399,7 +457,7 @@ template <int D_, int BITS_, int NT_, int WARPS_, int KB_, int CTAS_, bool FINE_
 struct Shape {
   static constexpr int D = D_, BITS = BITS_, NT = NT_, WARPS = WARPS_, KB = KB_, CTAS = CTAS_;
   static constexpr bool FINE = FINE_;
-  static constexpr int KS = D / 16;                 // k16 steps of a score
+  static constexpr int KS = D / 16;                 // tiles of 16 dims of V
   static constexpr int NG = D / GROUP;
   static constexpr int CODES = code_bytes(D, BITS);
   static constexpr int BLOCK = block_bytes(D, BITS);
@@ -408,11 +466,6 @@ struct Shape {
   static constexpr int MERGE_REGS = KS * NT * 4 + NG * NT * 2 + 4 * NT;   // O, its offset part, l and reference
   static constexpr int MERGE = WARPS / 2 * MERGE_REGS * 128;
   static constexpr int HEAD = 2 * WARPS * MAX_RING * 8;
-  // A row of 16 dims a lane is stored as slabs: 16 bytes a lane and token, 8 bytes where the whole row is 32.
-  static constexpr bool SMALL = BITS == 4 && D == 64;
-  static constexpr int SLABS = SMALL ? 1 : D * BITS / 512;
-  static constexpr int SLAB_GROUPS = BITS == 4 && !SMALL ? 2 : 1;
-  static constexpr int SLAB_WORDS = SMALL ? 2 : 4;
   __host__ __device__ static constexpr int slots(int sw) { return 8 * NT * sw; }
   __host__ __device__ static constexpr int fixed(int sw) {
     return HEAD + slots(sw) * (NG + 2) * 4 + KS * NT * sw * 256 + (sw < WARPS ? MERGE : 0);
@@ -440,71 +493,70 @@ __device__ __forceinline__ void stage_step(State<S>& st, const uint8_t* in, cons
                                            int slots, int key0, int g, int t) {
   constexpr int NT = S::NT, NG = S::NG, KS = S::KS, KB = S::KB, BITS = S::BITS;
   float sc[KB][NT][4];
+  uint32_t sz[KB][2 * NG];   // of tokens 2g and 2g + 1, which are rows g and g + 8 of a fragment
 #pragma unroll
-  for (int kb = 0; kb < KB; ++kb)
+  for (int kb = 0; kb < KB; ++kb) lds(sz[kb], in + kb * S::BLOCK + 2 * S::CODES + g * NG * 8);
+  // Groups are walked side by side (GB at a time): every chain of four products then has others between its links.
+  constexpr int GB = NG * KB * NT <= 4 ? NG : NG * KB * NT <= 8 ? (NG + 1) / 2 : 1;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+  for (int g0 = 0; g0 < NG; g0 += GB) {
+    uint32_t w[GB][KB][BITS];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sc[kb][n][j] = 0.f;
-  uint32_t sz[KB][2][NG];
-#pragma unroll
-  for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-    for (int r = 0; r < 2; ++r) lds(sz[kb][r], in + kb * S::BLOCK + 2 * S::CODES + (g + 8 * r) * NG * 4);
-#pragma unroll
-  for (int sl = 0; sl < S::SLABS; ++sl) {
-    uint32_t w[KB][2][S::SLAB_WORDS];
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-        lds(w[kb][r], in + kb * S::BLOCK + (S::SMALL ? (g + 8 * r) * 32 + t * 8 : sl * 1024 + (g + 8 * r) * 64 + t * 16));
-#pragma unroll
-    for (int sg = 0; sg < S::SLAB_GROUPS; ++sg) {
-      const int gi = sl * S::SLAB_GROUPS + sg;
-      float acc[KB][NT][4];
+    for (int gi = 0; gi < GB; ++gi)
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int r = 0; r < BITS / 4; ++r) {
+          uint32_t u[4];
+          lds(u, in + kb * S::BLOCK + (g0 + gi) * (BITS * 128) + r * 512 + (g * 4 + t) * 16);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[kb][n][j] = 0.f;
+          for (int j = 0; j < 4; ++j) w[gi][kb][4 * r + j] = u[j];
+        }
+    float acc[GB][KB][NT][4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int gi = 0; gi < GB; ++gi) {
         uint32_t bq[NT][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) lds(bq[n], qf + (gi * 4 + k) * q_step + n * 256);
+        for (int n = 0; n < NT; ++n) lds(bq[n], qf + ((g0 + gi) * 4 + k) * q_step + n * 256);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
-          uint32_t f[2][2];
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            if (BITS == 4) {
-              const uint32_t x = w[kb][r][(sg * 2 + (k >> 1)) % S::SLAB_WORDS] >> (8 * (k & 1));
-              f[r][0] = x & 0x000F000Fu;
-              f[r][1] = x & 0x00F000F0u;
-            } else {
-              const uint32_t x = w[kb][r][k % S::SLAB_WORDS];
-              f[r][0] = x & 0x00FF00FFu;
-              f[r][1] = (x >> 8) & 0x00FF00FFu;
-            }
+          uint32_t a0, a1, a2, a3;   // rows g and g + 8
+          if (BITS == 4) {
+            const uint32_t x = w[gi][kb][k >> 1] >> (8 * (k & 1)), y = w[gi][kb][2 + (k >> 1)] >> (8 * (k & 1));
+            a0 = x & 0x000F000Fu;
+            a1 = y & 0x000F000Fu;
+            a2 = x & 0x00F000F0u;
+            a3 = y & 0x00F000F0u;
+          } else {
+            const uint32_t x = w[gi][kb][k], y = w[gi][kb][(4 + k) % BITS];
+            a0 = x & 0x00FF00FFu;
+            a1 = y & 0x00FF00FFu;
+            a2 = (x >> 8) & 0x00FF00FFu;
+            a3 = (y >> 8) & 0x00FF00FFu;
           }
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma16816(acc[kb][n], f[0][0], f[1][0], f[0][1], f[1][1], bq[n][0], bq[n][1]);
+          for (int n = 0; n < NT; ++n) {
+            if (k == 0) mma16816_first(acc[gi][kb][n], a0, a1, a2, a3, bq[n][0], bq[n][1]);
+            else mma16816(acc[gi][kb][n], a0, a1, a2, a3, bq[n][0], bq[n][1]);
+          }
         }
       }
 #pragma unroll
+    for (int gi = 0; gi < GB; ++gi)
+#pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const float2 qs = *reinterpret_cast<const float2*>(qsum + gi * slots + n * 8 + 2 * t);
+        const float2 qs = *reinterpret_cast<const float2*>(qsum + (g0 + gi) * slots + n * 8 + 2 * t);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const uint32_t x = sz[kb][j >> 1][gi];
-            sc[kb][n][j] = fmaf(scale_of(x), acc[kb][n][j], fmaf(offset_of(x), j & 1 ? qs.y : qs.x, sc[kb][n][j]));
+            const uint32_t x = sz[kb][(j >> 1) * NG + g0 + gi];
+            const float y = j & 1 ? qs.y : qs.x;
+            sc[kb][n][j] = fmaf(scale_of(x), acc[gi][kb][n][j], g0 + gi == 0 ? offset_of(x) * y : fmaf(offset_of(x), y, sc[kb][n][j]));
           }
       }
-    }
   }
   // V's scales: the largest exponent among this lane's keys bounds them all.  The bits of a scale grow with it;
   // a poisoned one is negative.
@@ -515,14 +567,14 @@ __device__ __forceinline__ void stage_step(State<S>& st, const uint8_t* in, cons
     for (int n = 0; n < NT; ++n) longest = max(longest, max(st.lens[n][0], st.lens[n][1]));
   }
 #pragma unroll
-  for (int kb = 0; kb < KB; ++kb)
+  for (int kb = 0; kb < KB; ++kb) {
+    lds(sz[kb], in + kb * S::BLOCK + 2 * S::CODES + TOK * NG * 4 + g * NG * 8);
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      lds(sz[kb][r], in + kb * S::BLOCK + 2 * S::CODES + TOK * NG * 4 + (g + 8 * r) * NG * 4);
+    for (int r = 0; r < 2; ++r)
 #pragma unroll
       for (int gi = 0; gi < NG; ++gi)
-        if (!MASK || key0 + kb * 16 + r * 8 + g < longest) top = max(top, (int)(sz[kb][r][gi] << 16));
-    }
+        if (!MASK || key0 + kb * 16 + 2 * g + r < longest) top = max(top, (int)(sz[kb][r * NG + gi] << 16));
+  }
   const float ex = __uint_as_float(0x4B000000u | (uint32_t)(top >> 23)) - (8388608.f + 127.f);
   float most[NT][2];
   bool move = false;
@@ -536,7 +588,7 @@ __device__ __forceinline__ void stage_step(State<S>& st, const uint8_t* in, cons
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           float x = sc[kb][n][2 * r + j] * st.fac[n][j];
-          if (MASK && key0 + kb * 16 + r * 8 + g >= st.lens[n][j]) x = -INFINITY;
+          if (MASK && key0 + kb * 16 + 2 * g + r >= st.lens[n][j]) x = -INFINITY;
           sc[kb][n][2 * r + j] = x;
           m = fmaxf(m, x);
         }
@@ -572,68 +624,80 @@ __device__ __forceinline__ void stage_step(State<S>& st, const uint8_t* in, cons
       for (int j = 0; j < 4; ++j) {
         // A masked score is -inf; where the reference still is too, the difference would be NaN.
         float p = ex2(sc[kb][n][j] + (LIFT - st.ref[n][j & 1]));
-        if (MASK && key0 + kb * 16 + (j >> 1) * 8 + g >= st.lens[n][j & 1]) p = 0.f;
+        if (MASK && key0 + kb * 16 + 2 * g + (j >> 1) >= st.lens[n][j & 1]) p = 0.f;
         sc[kb][n][j] = p;
         st.l[n][j & 1] += p;
       }
 #pragma unroll
-    for (int sl = 0; sl < S::SLABS; ++sl) {
-      // V's numbers of tokens 2t, 2t + 1 and 2t + 8, 2t + 9 for this lane's 8 dims of each group.
-      uint32_t u[2][S::SLAB_WORDS];
+    for (int gi = 0; gi < NG; ++gi) {
+      // V's numbers of the tokens 4t..4t+3 (columns 2t, 2t + 8, 2t + 1 and 2t + 9 of a fragment) for this lane's
+      // 8 dims of the group, which are rows g and g + 8 of four tiles.
+      uint32_t u[BITS];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        lds(u[h], in + kb * S::BLOCK + S::CODES +
-                      (S::SMALL ? g * 64 + (h ^ ((g >> 1) & 1)) * 32 + t * 8 : sl * 1024 + g * 128 + (h ^ (g & 1)) * 64 + t * 16));
+      for (int h = 0; h < BITS / 4; ++h) {
+        uint32_t x[4];
+        lds(x, in + kb * S::BLOCK + S::CODES + gi * (BITS * 128) + h * 512 + (g * 4 + t) * 16);
 #pragma unroll
-      for (int sg = 0; sg < S::SLAB_GROUPS; ++sg) {
-        const int gi = sl * S::SLAB_GROUPS + sg;
-        uint32_t bp[NT][2], bl[NT][2];
+        for (int j = 0; j < 4; ++j) u[4 * h + j] = x[j];
+      }
+      uint32_t bp[NT][2], bl[NT][2], f[4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float ps[4];
+      for (int n = 0; n < NT; ++n) {
+        float ps[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t x = sz[kb][j >> 1][gi];
-            ps[j] = sc[kb][n][j] * scale_of(x);
-            float& oz = st.oz[gi][n][j & 1];
-            if (MASK) {   // nothing of a masked key, NaN among it, is taken
-              const bool out = key0 + kb * 16 + (j >> 1) * 8 + g >= st.lens[n][j & 1];
-              ps[j] = out ? 0.f : ps[j];
-              oz = out ? oz : fmaf(sc[kb][n][j], offset_of(x), oz);
-            } else {
-              oz = fmaf(sc[kb][n][j], offset_of(x), oz);
-            }
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t hi = pack_f16(ps[2 * h], ps[2 * h + 1]);
-            bp[n][h] = transpose8x8(hi);
-            if (S::FINE) {
-              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-              bl[n][h] = transpose8x8(pack_f16(ps[2 * h] - f.x, ps[2 * h + 1] - f.y));
-            }
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t x = sz[kb][(j >> 1) * NG + gi];
+          ps[j] = sc[kb][n][j] * scale_of(x);
+          float& oz = st.oz[gi][n][j & 1];
+          if (MASK) {   // nothing of a masked key, NaN among it, is taken
+            const bool out = key0 + kb * 16 + 2 * g + (j >> 1) >= st.lens[n][j & 1];
+            ps[j] = out ? 0.f : ps[j];
+            oz = out ? oz : fmaf(sc[kb][n][j], offset_of(x), oz);
+          } else {
+            oz = fmaf(sc[kb][n][j], offset_of(x), oz);
           }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t f[2][2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (BITS == 4) {   // words of the two tokens: SLAB_WORDS / 2 apart
-              const uint32_t x = __byte_perm(u[h][sg], u[h][S::SLAB_WORDS / 2 + sg], i < 2 ? 0x5410 : 0x7632) >> (8 * (i & 1));
-              f[h][0] = x & 0x000F000Fu;
-              f[h][1] = x & 0x00F000F0u;
-            } else {
-              const uint32_t x = __byte_perm(u[h][i >> 1], u[h][(S::SLAB_WORDS / 2 + (i >> 1)) % S::SLAB_WORDS], i & 1 ? 0x7632 : 0x5410);
-              f[h][0] = x & 0x00FF00FFu;
-              f[h][1] = (x >> 8) & 0x00FF00FFu;
-            }
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t hi = pack_f16(ps[2 * h], ps[2 * h + 1]);
+          bp[n][h] = transpose8x8(hi);
+          if (S::FINE) {
+            const float2 cut = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+            bl[n][h] = transpose8x8(pack_f16(ps[2 * h] - cut.x, ps[2 * h + 1] - cut.y));
           }
+        }
+      }
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma16816(st.o[gi * 4 + i][n], f[0][0], f[0][1], f[1][0], f[1][1], bp[n][0], bp[n][1]);
-            if (S::FINE) mma16816(st.o[gi * 4 + i][n], f[0][0], f[0][1], f[1][0], f[1][1], bl[n][0], bl[n][1]);
+      for (int i = 0; i < 4; ++i) {
+        uint32_t a0, a1, a2, a3;
+        if (BITS == 4) {
+          const uint32_t x = u[i], y = u[i] >> 8;
+          a0 = x & 0x000F000Fu;
+          a1 = x & 0x00F000F0u;
+          a2 = y & 0x000F000Fu;
+          a3 = y & 0x00F000F0u;
+        } else {
+          const uint32_t x = u[(2 * i) % BITS], y = u[(2 * i + 1) % BITS];
+          a0 = x & 0x00FF00FFu;
+          a1 = y & 0x00FF00FFu;
+          a2 = (x >> 8) & 0x00FF00FFu;
+          a3 = (y >> 8) & 0x00FF00FFu;
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma16816(st.o[gi * 4 + i][n], a0, a1, a2, a3, bp[n][0], bp[n][1]);
+        if (S::FINE) {   // a tile behind, so that its sum's last product has left the pipe
+          if (i > 0) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma16816(st.o[gi * 4 + i - 1][n], f[0], f[1], f[2], f[3], bl[n][0], bl[n][1]);
           }
+          if (i == 3) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma16816(st.o[gi * 4 + 3][n], a0, a1, a2, a3, bl[n][0], bl[n][1]);
+          }
+          f[0] = a0;
+          f[1] = a1;
+          f[2] = a2;
+          f[3] = a3;
         }
       }
     }
@@ -705,29 +769,35 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
   Piece src = {};      // the piece that is being loaded
   int src_n = 0;
   const int bshift = a.page_shift - 4;
-  auto blocks_from = [&](int i0) {
+  auto page_ids = [&](int i0) {   // raw, so that nothing waits for it here
     const int i = i0 + lane / KB;
     const int blk = (src.first + kl + i * kw) * KB + lane % KB;
-    if (i >= src_n || blk * TOK >= src.len) return -1;
+    if (i >= src_n || blk * TOK >= src.len) return INT_MIN;
     const int index = blk >> bshift;
-    const bool ok = src.slot >= 0 && src.slot < a.num_slots && index < a.max_pages;
-    int page = ok ? a.page_table[(size_t)src.slot * a.max_pages + index] : -1;
+    if (src.slot < 0 || src.slot >= a.num_slots || index >= a.max_pages) return -1;
+    return a.page_table[(size_t)src.slot * a.max_pages + index];
+  };
+  auto blocks_of = [&](int page, int i0) {   // -1: behind the sequence's end
+    if (page == INT_MIN) return -1;
     if (page < 0 || page >= a.num_pages) {
       report_error(a.err, kErrBadShape);
       page = 0;
     }
+    const int blk = (src.first + kl + (i0 + lane / KB) * kw) * KB + lane % KB;
     return ((page * a.num_kv_heads + src.head) << bshift) + (blk & ((1 << bshift) - 1));
   };
   auto start_loads = [&](const Piece& p) {
     src = p;
     src_n = p.n > kl ? (p.n - kl + kw - 1) / kw : 0;
     issued = 0;
-    at_block = blocks_from(0);
-    at_next = blocks_from(AHEAD);
+    const int now = page_ids(0);
+    at_next = src_n > AHEAD ? page_ids(AHEAD) : INT_MIN;
+    at_block = blocks_of(now, 0);
   };
   auto issue = [&]() {   // the next stage of the source piece into the ring
     if (issued >= src_n) return;
-    mbar_wait(&empty[fill], fill_phase, a.err);
+    // A warp that is alone on its key lane has read the place itself.
+    if (sw_n > 1) mbar_wait(&empty[fill], fill_phase, a.err);
     const int k = issued % AHEAD * KB;
     const int b0 = __shfl_sync(0xffffffff, at_block, k);
     const int b1 = KB == 2 ? __shfl_sync(0xffffffff, at_block, (k + 1) & 31) : -1;
@@ -741,9 +811,9 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
       fill = 0;
       fill_phase ^= 1;
     }
-    if (++issued % AHEAD == 0) {
-      at_block = at_next;
-      at_next = blocks_from(issued + AHEAD);
+    if (++issued % AHEAD == 0 && issued < src_n) {
+      at_block = blocks_of(at_next, issued);
+      at_next = page_ids(issued + AHEAD);
     }
   };
 
@@ -755,9 +825,8 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
     for (int i = 0; i < ring; ++i) issue();
   }
   while (true) {
-    // Queries: a warp a slot.  A slot's numbers are brought to [2^13, 2^14) by a power of two, where f16
-    // holds a bf16 or f16 exactly down to 2^-27 of the largest; the numbers that meet w & 0x00F000F0 are
-    // divided by 16.
+    // Queries: a warp a slot.  A power of two brings a slot's numbers to [2^13, 2^14), where f16 is exact down to
+    // 2^-27 of the largest; the numbers that meet w & 0x00F000F0 are divided by 16.
     const int slot_end = min(slots, (cur.count + 7) / 8 * 8);
     for (int s = warp; s < slot_end; s += WARPS) {
       constexpr int PER = D / 32;
@@ -810,12 +879,11 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
         qfac[s] = a.sm_scale * 1.4426950408889634f * __uint_as_float((uint32_t)(24 - e + 127) << 23);
         qlen[s] = real ? plan.lens[row] : cur.len;
       }
-      __half* q16 = reinterpret_cast<__half*>(qfrag);
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        const int d = lane * PER + j, in = d & 15;
+        const int d = lane * PER + j, in = d & 15, ln = (s & 7) * 4 + ((d & 63) >> 4);
         int ks, reg, part;
-        if (BITS == 4) {
+        if (BITS == 4) {   // number in & 7 of word in / 8: bits 8 .. 15 are shifted down for the second step
           ks = (d >> 6) * 4 + (in >> 3) * 2 + ((in >> 1) & 1);
           reg = in & 1;
           part = (in >> 2) & 1;
@@ -825,8 +893,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
           reg = in & 1;
           part = (in >> 1) & 1;
         }
-        const int ln = (s & 7) * 4 + ((d & 63) >> 4);
-        q16[(((ks * NT * sw_n + (s >> 3)) * 32 + ln) * 2 + reg) * 2 + part] = __float2half_rn(x[j]);
+        reinterpret_cast<__half*>(qfrag)[(((ks * NT * sw_n + (s >> 3)) * 32 + ln) * 2 + reg) * 2 + part] = __float2half_rn(x[j]);
       }
     }
     __syncthreads();
@@ -864,7 +931,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
         else stage_step<S, true>(st, in, qf, NT * sw_n * 256, qsum + sw * NT * 8, slots, key0, g, t);
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[use]);
+      if (sw_n > 1 && lane == 0) mbar_arrive(&empty[use]);
       if (++use == ring) {
         use = 0;
         use_phase ^= 1;
@@ -1114,9 +1181,13 @@ int check_rows(const QuantRowsArgs& a) {
   return 0;
 }
 
-int row_blocks(const QuantRowsArgs& a) {
-  const long long items = (long long)a.rows * a.num_kv_heads * 2 * (a.head_dim / 8);
-  return (int)((items + ROW_THREADS - 1) / ROW_THREADS);
+// Warps that share four rows: all their groups where rows are few, so that the device fills up.
+int row_blocks(QuantRowsArgs& a) {
+  const long long quads = ((long long)a.rows + 3) / 4;
+  const int items = 2 * a.num_kv_heads * (a.head_dim / GROUP);
+  a.share = (int)((148 * 64 + quads - 1) / quads);
+  a.share = a.share > items ? items : a.share < 1 ? 1 : a.share;
+  return (int)((quads * a.share + ROW_WARPS - 1) / ROW_WARPS);
 }
 
 // The variant for sequences of so many query slots.
@@ -1194,14 +1265,18 @@ extern "C" int zs_quant_block_bytes(int head_dim, int bits) { return zs::qc::blo
 extern "C" int zs_quant_store(const QuantRowsArgs* args, cudaStream_t stream) {
   if (int e = zs::qc::check_rows(*args)) return e;
   if (args->rows == 0) return 0;
-  zs_launch(zs::qc::store_kernel, zs::qc::row_blocks(*args), zs::qc::ROW_THREADS, 0, stream, *args);
+  QuantRowsArgs a = *args;
+  const int blocks = zs::qc::row_blocks(a);
+  zs_launch(a.bits == 4 ? zs::qc::store_kernel<4> : zs::qc::store_kernel<8>, blocks, zs::qc::ROW_WARPS * 32, 0, stream, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
 extern "C" int zs_quant_load(const QuantRowsArgs* args, cudaStream_t stream) {
   if (int e = zs::qc::check_rows(*args)) return e;
   if (args->rows == 0) return 0;
-  zs_launch(zs::qc::load_kernel, zs::qc::row_blocks(*args), zs::qc::ROW_THREADS, 0, stream, *args);
+  QuantRowsArgs a = *args;
+  const int blocks = zs::qc::row_blocks(a);
+  zs_launch(a.bits == 4 ? zs::qc::load_kernel<4> : zs::qc::load_kernel<8>, blocks, zs::qc::ROW_WARPS * 32, 0, stream, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 

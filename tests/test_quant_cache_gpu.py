@@ -358,6 +358,40 @@ def test_poison_and_masks():
     assert bool(got.isfinite().all())
 
 
+@pytest.mark.parametrize("dim,bits,hq", [(64, 4, 16), (128, 4, 8), (256, 4, 8), (64, 8, 16), (128, 8, 32), (256, 8, 16)])
+def test_what_stands_behind_a_sequence_does_not_matter(dim, bits, hq):
+    """Values of any size in the places behind a length, and other sequences' in the blocks read before."""
+    lens = [1, 17, 300, 33, 5]
+    table, pages = table_of(lens, 16)
+    cache = QuantCache(1, pages, 1, dim, bits=bits)
+    every = torch.arange(pages, dtype=torch.int32, device=DEV)[None]
+    at = torch.arange(pages * 16, dtype=torch.int32, device=DEV)
+    huge = rows_of(pages * 16, 1, dim, torch.bfloat16, 1, 2.0 ** 100)
+    cache.write(0, huge, huge, every, torch.zeros_like(at), at)
+    slots, pos = places_of(lens)
+    cache.write(0, rows_of(len(slots), 1, dim, torch.bfloat16, 2), rows_of(len(slots), 1, dim, torch.bfloat16, 3), table, slots, pos)
+    check_attention(cache, table, hq, list(range(5)) * 40, lens * 40)
+
+
+def test_tokens_in_any_order():
+    """Rows whose tokens are scattered, alone and by fours, hold what rows in order do."""
+    n, dim = 64, 128
+    table, pages = table_of([n], 16)
+    for bits in (4, 8):
+        a, b = QuantCache(1, pages, 2, dim, bits=bits), QuantCache(1, pages, 2, dim, bits=bits)
+        slots, pos = places_of([n])
+        k, v = rows_of(n, 2, dim, torch.bfloat16, 1), rows_of(n, 2, dim, torch.bfloat16, 2)
+        a.write(0, k, v, table, slots, pos)
+        for order in (torch.randperm(n, device=DEV), torch.arange(n, device=DEV).view(4, 4, 4).transpose(1, 2).reshape(-1),
+                      (torch.arange(n, device=DEV) + 3) % n, torch.arange(n, device=DEV).flip(0)):
+            b.data.zero_()
+            for part in order.split(23):
+                b.write(0, k[part], v[part], table, slots[part], pos[part])
+            assert torch.equal(a.data, b.data)
+            for x, y in zip(b.read(0, table, slots[order], pos[order]), a.read(0, table, slots, pos)):
+                assert torch.equal(x, y[order])
+
+
 def test_strided_queries_and_mxfp8():
     from zstep_b200.ops import mx
 
