@@ -22,6 +22,7 @@
 #include <cuda_fp16.h>
 
 #include <climits>
+#include <type_traits>
 
 #include "sm100_common.cuh"
 #include "zs_kernels.h"
@@ -90,110 +91,127 @@ __device__ __forceinline__ uint8_t* block_at(const QuantRowsArgs& a, int row, in
   return a.data + (((size_t)page * a.num_kv_heads << (a.page_shift - 4)) + sub) * block_bytes(a.head_dim, a.bits);
 }
 
-// Rows go by fours: a warp has one group of 64 dims of four rows, eight dims a lane, and walks `a.share`-th
-// parts of the groups of K and V of all heads.
+// Rows go by fours: a warp has one group of 64 dims of four rows, eight dims a lane, and walks every `a.step`-th
+// head of K and V.
 constexpr int ROW_WARPS = 8;
 
 struct RowLane {
-  uint8_t* block;   // of the lane's row for kv head 0, or null
-  int row, token;
+  int row;         // of the lane
+  int gi, first;   // group, first head
 };
-__device__ __forceinline__ RowLane row_lane(const QuantRowsArgs& a, int quad) {
-  RowLane r;
-  r.row = quad * 4 + ((threadIdx.x & 31) >> 3);
-  r.token = 0;
-  r.block = r.row < a.rows ? block_at(a, r.row, &r.token) : nullptr;
-  return r;
+__device__ __forceinline__ bool row_lane(const QuantRowsArgs& a, int groups, RowLane* r) {
+  const int w = blockIdx.x * ROW_WARPS + (threadIdx.x >> 5), share = a.step * groups;
+  const int quad = w / share, in = w - quad * share;
+  r->first = in / groups;
+  r->gi = in - r->first * groups;
+  r->row = quad * 4 + ((threadIdx.x & 31) >> 3);
+  return quad * 4 < a.rows;
 }
 
 template <int BITS>
 __global__ void __launch_bounds__(ROW_WARPS * 32) store_kernel(const QuantRowsArgs a) {
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31;
-  const int w = blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
-  const int quad = w / a.share;
-  if (quad * 4 >= a.rows) return;
-  const RowLane r = row_lane(a, quad);
-  const int groups = a.head_dim / GROUP, items = 2 * a.num_kv_heads * groups, octet = lane & 7;
+  const int lane = threadIdx.x & 31, octet = lane & 7, mine = lane >> 3;
+  const int groups = a.head_dim / GROUP, heads = a.num_kv_heads;
+  RowLane r;
+  if (!row_lane(a, groups, &r)) return;
   const int codes = code_bytes(a.head_dim, BITS), head_bytes = block_bytes(a.head_dim, BITS) << (a.page_shift - 4);
-  constexpr int TOP = (1 << BITS) - 1;
+  const int d = r.gi * GROUP + octet * 8;
+  constexpr float TOP = (1 << BITS) - 1;
+  // The first head's numbers are on their way while the rows' places are looked up.
+  const uint16_t* k_from = static_cast<const uint16_t*>(a.k) + r.row * a.k_row + d;
+  const uint16_t* v_from = static_cast<const uint16_t*>(a.v) + r.row * a.v_row + d;
+  auto load = [&](const uint16_t* from, long long stride, int h) {
+    return h < heads && r.row < a.rows ? *reinterpret_cast<const uint4*>(from + h * stride) : make_uint4(0, 0, 0, 0);
+  };
+  uint4 k_next = load(k_from, a.k_head, r.first), v_next = load(v_from, a.v_head, r.first);
+  int my_token = 0;
+  uint8_t* my_block = r.row < a.rows ? block_at(a, r.row, &my_token) : nullptr;
+  const bool there = my_block != nullptr;
   // Four rows that are the four tokens of one word of V's are written as words.
-  const long long first = __shfl_sync(0xffffffff, (long long)r.block, 0);
-  const int token = __shfl_sync(0xffffffff, r.token, 0);
-  const bool whole = __all_sync(0xffffffff, r.block != nullptr && (long long)r.block == first && (token & 3) == 0 && r.token == token + (lane >> 3));
-  for (int i = w % a.share; i < items; i += a.share) {
-    const int gi = i % groups, head = i / groups % a.num_kv_heads;
-    const bool is_v = i >= items / 2;
-    const int d = gi * GROUP + octet * 8;
+  const long long first = __shfl_sync(0xffffffff, (long long)my_block, 0);
+  const int token = __shfl_sync(0xffffffff, my_token, 0);
+  const bool whole = __all_sync(0xffffffff, there && (long long)my_block == first && (token & 3) == 0 && my_token == token + mine);
+  auto put = [&](auto is_v, const uint4& u, int h) {
+    constexpr bool V = decltype(is_v)::value;
+    uint8_t* block = my_block + (V ? codes + v_offset(BITS, my_token, d) : k_offset(BITS, my_token, d));
+    uint8_t* scales = my_block + 2 * codes + (V ? TOK * groups * 4 : 0) + (my_token * groups + r.gi) * 4;
+    const uint32_t word[4] = {u.x, u.y, u.z, u.w};
     float x[8];
-    if (r.row < a.rows) {
-      const long long from = is_v ? r.row * a.v_row + head * a.v_head : r.row * a.k_row + head * a.k_head;
-      const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(is_v ? a.v : a.k) + from + d);
-      const uint32_t word[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = two_floats(word[j], a.half);
-        x[2 * j] = f.x;
-        x[2 * j + 1] = f.y;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = 0.f;
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = two_floats(word[j], a.half);
+      x[2 * j] = f.x;
+      x[2 * j + 1] = f.y;
     }
-    float lo = x[0], hi = x[0];
-    bool fine = true;
+    float lo = x[0], hi = x[0], nan = 0.f;   // NaN once a NaN or an infinity has come
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       lo = fminf(lo, x[j]);
       hi = fmaxf(hi, x[j]);
-      fine = fine && fabsf(x[j]) <= 0x1p126f;
+      nan = fmaf(x[j], 0.f, nan);
     }
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) {
       lo = fminf(lo, __shfl_xor_sync(0xffffffff, lo, o));
       hi = fmaxf(hi, __shfl_xor_sync(0xffffffff, hi, o));
+      nan += __shfl_xor_sync(0xffffffff, nan, o);
     }
-    const uint32_t mates = 0xFFu << (lane & 24);
-    fine = (__ballot_sync(0xffffffff, fine) & mates) == mates;
+    const bool fine = nan == 0.f && fmaxf(fabsf(lo), fabsf(hi)) <= 0x1p126f;
     const float z = bf16_down(lo);
-    const float s = bf16_up(__fdiv_rn(hi - z, (float)TOP));
+    const float s = bf16_up(__fdiv_rn(hi - z, TOP));
+    // (x - z) / s rounded as a division rounds, by Markstein's correction of x' times the rounded 1 / s; a power
+    // of two keeps 1 / s and the remainder in range.  The sum with 1.5 2^23 rounds it to a whole number, ties to
+    // even.  Horner's scheme puts numbers together while they are floats (exact below 2^24).
+    const float up = s < 0x1p-64f ? 0x1p100f : 1.f;
+    const float su = s * up, inv = s > 0.f ? __frcp_rn(su) : 0.f;
+    constexpr int PER = 16 / BITS;   // numbers of 16 bits
     uint32_t n[BITS / 4] = {};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float q = s > 0.f ? rintf(__fdiv_rn(x[j] - z, s)) : 0.f;
-      q = fine ? fminf(fmaxf(q, 0.f), (float)TOP) : 0.f;
-      n[j * BITS / 32] |= (uint32_t)q << (BITS * j & 31);
+    for (int c = 0; c < 8 / PER; ++c) {
+      float both = 0.f;
+#pragma unroll
+      for (int j = PER - 1; j >= 0; --j) {
+        const float y = (x[c * PER + j] - z) * up, q0 = y * inv;
+        const float q = fminf(fmaf(fmaf(-q0, su, y), inv, q0), TOP);
+        both = fmaf(both, TOP + 1.f, (q + 12582912.f) - 12582912.f);
+      }
+      n[c / 2] |= (__float_as_uint(both + 12582912.f) & 0xFFFFu) << (16 * (c & 1));
     }
-    uint8_t* block = r.block + (size_t)head * head_bytes;
-    if (!is_v) {
-      if (r.block != nullptr) {
-        uint8_t* to = block + k_offset(BITS, r.token, d);
-        if constexpr (BITS == 4) *reinterpret_cast<uint32_t*>(to) = n[0];
-        else *reinterpret_cast<uint2*>(to) = make_uint2(n[0], n[1]);
+    if (!fine) {
+#pragma unroll
+      for (int i = 0; i < BITS / 4; ++i) n[i] = 0;
+    }
+    const long long at = (long long)h * head_bytes;
+    if (!V) {
+      if (there) {
+        if constexpr (BITS == 4) *reinterpret_cast<uint32_t*>(block + at) = n[0];
+        else *reinterpret_cast<uint2*>(block + at) = make_uint2(n[0], n[1]);
       }
     } else if (whole) {
-      // Lane r of a four gets bytes r of all four rows: word r (and r + 4).
-      const int mine = lane >> 3;
+      // A four by four exchange of bytes: lane `mine` of a four gets byte `mine` of all four rows.
 #pragma unroll
-      for (int h = 0; h < BITS / 4; ++h) {
-        uint32_t word = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t other = __shfl_sync(0xffffffff, n[h], k * 8 + octet);
-          word |= (other >> (8 * mine) & 255u) << (8 * k);
-        }
-        *reinterpret_cast<uint32_t*>(block + codes + v_offset(BITS, r.token, d) + h * 512 + mine * 4) = word;
+      for (int i = 0; i < BITS / 4; ++i) {
+        const uint32_t x1 = __shfl_xor_sync(0xffffffff, n[i], 8);
+        const uint32_t y = mine & 1 ? __byte_perm(x1, n[i], 0x7351) : __byte_perm(n[i], x1, 0x6240);   // bytes b, b + 2 of two rows
+        const uint32_t x2 = __shfl_xor_sync(0xffffffff, y, 16);
+        const uint32_t all = mine & 2 ? __byte_perm(x2, y, 0x7632) : __byte_perm(y, x2, 0x5410);
+        *reinterpret_cast<uint32_t*>(block + at + i * 512 + mine * 4) = all;
       }
-    } else if (r.block != nullptr) {
-      uint8_t* to = block + codes + v_offset(BITS, r.token, d) + (r.token & 3);
+    } else if (there) {
+      uint8_t* to = block + at + (my_token & 3);
 #pragma unroll
       for (int j = 0; j < BITS; ++j) to[(j >> 2) * 512 + (j & 3) * 4] = (uint8_t)(n[j >> 2] >> (8 * (j & 3)));
     }
-    if (octet == 0 && r.block != nullptr) {
-      uint32_t* sz = reinterpret_cast<uint32_t*>(block + 2 * codes) + (is_v ? TOK * groups : 0) + r.token * groups + gi;
-      *sz = fine ? __float_as_uint(s) >> 16 | __float_as_uint(z) : POISON;
-    }
+    if (octet == 0 && there) *reinterpret_cast<uint32_t*>(scales + at) = fine ? __float_as_uint(s) >> 16 | __float_as_uint(z) : POISON;
+  };
+  for (int h = r.first; h < heads; h += a.step) {
+    const uint4 k = k_next, v = v_next;
+    k_next = load(k_from, a.k_head, h + a.step);
+    v_next = load(v_from, a.v_head, h + a.step);
+    put(std::false_type(), k, h);
+    put(std::true_type(), v, h);
   }
 }
 
@@ -201,46 +219,30 @@ template <int BITS>
 __global__ void __launch_bounds__(ROW_WARPS * 32) load_kernel(const QuantRowsArgs a) {
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31;
-  const int w = blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
-  const int quad = w / a.share;
-  if (quad * 4 >= a.rows) return;
-  const RowLane r = row_lane(a, quad);
+  const int lane = threadIdx.x & 31, octet = lane & 7;
+  const int groups = a.head_dim / GROUP, heads = a.num_kv_heads;
+  RowLane r;
+  if (!row_lane(a, groups, &r)) return;
   if (r.row >= a.rows) return;
-  const int groups = a.head_dim / GROUP, items = 2 * a.num_kv_heads * groups, octet = lane & 7;
   const int codes = code_bytes(a.head_dim, BITS), head_bytes = block_bytes(a.head_dim, BITS) << (a.page_shift - 4);
-#pragma unroll 4
-  for (int i = w % a.share; i < items; i += a.share) {
-    const int gi = i % groups, head = i / groups % a.num_kv_heads;
-    const bool is_v = i >= items / 2;
-    const int d = gi * GROUP + octet * 8;
+  const int d = r.gi * GROUP + octet * 8;
+  int token = 0;
+  const uint8_t* block = block_at(a, r.row, &token);
+  const bool there = block != nullptr;
+  const uint32_t pick = (token & 3) * 0x11 + 0x40;   // this token's byte of two words
+  const uint8_t* k_from = block + k_offset(BITS, token, d);
+  const uint8_t* v_from = block + codes + v_offset(BITS, token, d);
+  const uint8_t* scales = block + 2 * codes + (token * groups + r.gi) * 4;
+  const long long k_to = r.row * a.k_row + d, v_to = r.row * a.v_row + d;
+  auto put = [&](void* out, long long to, const uint32_t (&n)[BITS / 4], uint32_t sz) {
+    const float s = scale_of(sz), z = offset_of(sz);
     float x[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = 0.f;
-    if (r.block != nullptr) {
-      const uint8_t* block = r.block + (size_t)head * head_bytes;
-      const uint32_t sz = *(reinterpret_cast<const uint32_t*>(block + 2 * codes) + (is_v ? TOK * groups : 0) + r.token * groups + gi);
-      uint32_t n[BITS / 4];
-      if (is_v) {
-        const uint32_t pick = (r.token & 3) * 0x11 + 0x40;   // this token's byte of two words
-#pragma unroll
-        for (int h = 0; h < BITS / 4; ++h) {
-          const uint4 u = *reinterpret_cast<const uint4*>(block + codes + v_offset(BITS, r.token, d) + h * 512);
-          n[h] = __byte_perm(__byte_perm(u.x, u.y, pick), __byte_perm(u.z, u.w, pick), 0x5410);
-        }
-      } else if constexpr (BITS == 4) {
-        n[0] = *reinterpret_cast<const uint32_t*>(block + k_offset(4, r.token, d));
-      } else {
-        const uint2 u = *reinterpret_cast<const uint2*>(block + k_offset(8, r.token, d));
-        n[0] = u.x;
-        n[BITS / 4 - 1] = u.y;
-      }
-      const float s = scale_of(sz), z = offset_of(sz);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = fmaf((float)(n[j * BITS / 32] >> (BITS * j & 31) & ((1 << BITS) - 1)), s, z);
+    for (int j = 0; j < 8; ++j) {   // a byte below 0x4B0000 is 2^23 + n
+      const uint32_t bytes = BITS == 8 ? n[(j >> 2) % (BITS / 4)] : j & 1 ? (n[0] >> 4) & 0x0F0F0F0Fu : n[0] & 0x0F0F0F0Fu;
+      const int at = BITS == 8 ? j & 3 : j >> 1;
+      x[j] = fmaf(__uint_as_float(__byte_perm(bytes, 0x4B000000u, 0x7440 + at)) - 8388608.f, s, z);
     }
-    const long long to = (is_v ? r.row * a.v_row + head * a.v_head : r.row * a.k_row + head * a.k_head) + d;
-    void* out = const_cast<void*>(is_v ? a.v : a.k);
     if (a.f32) {
       float4* o = reinterpret_cast<float4*>(static_cast<float*>(out) + to);
       o[0] = make_float4(x[0], x[1], x[2], x[3]);
@@ -248,6 +250,38 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) load_kernel(const QuantRowsArg
     } else {
       *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + to) =
           make_uint4(two_halves(x[0], x[1], a.half), two_halves(x[2], x[3], a.half), two_halves(x[4], x[5], a.half), two_halves(x[6], x[7], a.half));
+    }
+  };
+  constexpr int AT_ONCE = 4;   // heads whose loads are on their way together
+  for (int h0 = r.first; h0 < heads; h0 += AT_ONCE * a.step) {
+    uint32_t n[AT_ONCE][BITS / 4] = {}, k_sz[AT_ONCE] = {}, v_sz[AT_ONCE] = {};
+    uint4 u[AT_ONCE][BITS / 4] = {};
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const int h = h0 + i * a.step;
+      if (h >= heads || !there) continue;
+      const long long at = (long long)h * head_bytes;
+      k_sz[i] = *reinterpret_cast<const uint32_t*>(scales + at);
+      v_sz[i] = *reinterpret_cast<const uint32_t*>(scales + at + TOK * groups * 4);
+      if constexpr (BITS == 4) {
+        n[i][0] = *reinterpret_cast<const uint32_t*>(k_from + at);
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(k_from + at);
+        n[i][0] = x.x;
+        n[i][BITS / 4 - 1] = x.y;
+      }
+#pragma unroll
+      for (int k = 0; k < BITS / 4; ++k) u[i][k] = *reinterpret_cast<const uint4*>(v_from + at + k * 512);
+    }
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const int h = h0 + i * a.step;
+      if (h >= heads) break;
+      put(const_cast<void*>(a.k), k_to + h * a.k_head, n[i], k_sz[i]);
+      uint32_t v[BITS / 4];
+#pragma unroll
+      for (int k = 0; k < BITS / 4; ++k) v[k] = __byte_perm(__byte_perm(u[i][k].x, u[i][k].y, pick), __byte_perm(u[i][k].z, u[i][k].w, pick), 0x5410);
+      put(const_cast<void*>(a.v), v_to + h * a.v_head, v, v_sz[i]);
     }
   }
 }
@@ -1181,13 +1215,12 @@ int check_rows(const QuantRowsArgs& a) {
   return 0;
 }
 
-// Warps that share four rows: all their groups where rows are few, so that the device fills up.
+// Warps that share four rows and a group: a head each where rows are few, so that the device fills up.
 int row_blocks(QuantRowsArgs& a) {
-  const long long quads = ((long long)a.rows + 3) / 4;
-  const int items = 2 * a.num_kv_heads * (a.head_dim / GROUP);
-  a.share = (int)((148 * 64 + quads - 1) / quads);
-  a.share = a.share > items ? items : a.share < 1 ? 1 : a.share;
-  return (int)((quads * a.share + ROW_WARPS - 1) / ROW_WARPS);
+  const long long some = ((long long)a.rows + 3) / 4 * (a.head_dim / GROUP);
+  const long long want = (148 * 48 + some - 1) / some;
+  a.step = (int)(want > a.num_kv_heads ? a.num_kv_heads : want);
+  return (int)((some * a.step + ROW_WARPS - 1) / ROW_WARPS);
 }
 
 // The variant for sequences of so many query slots.

@@ -736,7 +736,7 @@ typedef struct QuantRowsArgs {
   long long k_row, k_head, v_row, v_head;   // strides in elements
   int half;                 // f16 instead of bf16
   int f32;                  // load: f32
-  int share;                // warps of four rows (set by the launcher)
+  int step;                 // warps of four rows and a group (set by the launcher)
   int* err;
 } QuantRowsArgs;
 
