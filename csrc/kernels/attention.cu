@@ -50,7 +50,8 @@ __device__ __forceinline__ int swz(int r, int d) {
 }
 
 // One CTA per row; one warp per head (q heads then k heads then v heads); lane owns 8 dims.
-__global__ void prologue_kernel(const AttnArgs a) {
+// k_out: K's rows, instead of the write of K and V into the cache.
+__global__ void prologue_kernel(const AttnArgs a, __nv_bfloat16* k_out) {
   pdl_wait();  // predecessor kernel done: its outputs are visible
   pdl_trigger();
   const int row = blockIdx.x;
@@ -59,9 +60,9 @@ __global__ void prologue_kernel(const AttnArgs a) {
   const int pos = a.positions[row];
   const int half = a.rotary_dim / 2;
   const __nv_bfloat16* qkv = static_cast<const __nv_bfloat16*>(a.qkv) + (size_t)row * a.ld_qkv;
-  const int slot = a.slots[row];
-  const int page = a.page_table[(size_t)slot * a.max_pages + pos / a.page_size];
-  for (int h = warp; h < nh + a.num_kv_heads; h += blockDim.x >> 5) {
+  const bool cached = k_out == nullptr;
+  const int page = cached ? a.page_table[(size_t)a.slots[row] * a.max_pages + pos / a.page_size] : 0;
+  for (int h = warp; h < (cached ? nh + a.num_kv_heads : nh); h += blockDim.x >> 5) {
     if (h >= nh) {
       // V head: straight copy into the cache.
       const int kvh = h - nh;
@@ -129,6 +130,8 @@ __global__ void prologue_kernel(const AttnArgs a) {
       reinterpret_cast<uint4*>(qo)[lane] = pv;
       __nv_bfloat16* go = static_cast<__nv_bfloat16*>(a.gate_out) + ((size_t)row * a.num_q_heads + h) * D;
       reinterpret_cast<uint4*>(go)[lane] = reinterpret_cast<const uint4*>(src + D)[lane];
+    } else if (!cached) {
+      reinterpret_cast<uint4*>(k_out + ((size_t)row * a.num_kv_heads + h - a.num_q_heads) * D)[lane] = pv;
     } else {
       const int kvh = h - a.num_q_heads;
       *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.k_cache) + kv_offset(a, page, kvh) +
@@ -1079,7 +1082,15 @@ extern "C" int zs_attn_prologue(const AttnArgs* args, cudaStream_t stream) {
   const AttnArgs& a = *args;
   if (a.head_dim != zs::attn::D || a.rotary_dim % 16 != 0 || a.rotary_dim > a.head_dim) return -1;
   if (a.rows == 0) return 0;
-  zs_launch(zs::attn::prologue_kernel, a.rows, 256, 0, stream, a);
+  zs_launch(zs::attn::prologue_kernel, a.rows, 256, 0, stream, a, static_cast<__nv_bfloat16*>(nullptr));
+  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+}
+
+extern "C" int zs_attn_prologue_rows(const AttnArgs* args, void* k_out, cudaStream_t stream) {
+  const AttnArgs& a = *args;
+  if (a.head_dim != zs::attn::D || a.rotary_dim % 16 != 0 || a.rotary_dim > a.head_dim || k_out == nullptr) return -1;
+  if (a.rows == 0) return 0;
+  zs_launch(zs::attn::prologue_kernel, a.rows, 256, 0, stream, a, static_cast<__nv_bfloat16*>(k_out));
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 

@@ -274,6 +274,32 @@ void attn_prologue(const Tensor& qkv, int64_t num_q_heads, int64_t num_kv_heads,
   rc(zs_attn_prologue(&a, stream()), "zs_attn_prologue");
 }
 
+// The prologue of a model whose K/V cache is written apart: K's normed and rotated rows to k_out.
+void attn_prologue_rows(const Tensor& qkv, int64_t num_q_heads, int64_t num_kv_heads, int64_t rotary_dim, double rope_theta,
+                        const Tensor& q_norm_w, const Tensor& k_norm_w, double eps, const Tensor& positions, int64_t rows,
+                        const Tensor& q_out, const Tensor& gate_out, const Tensor& k_out) {
+  for (const Tensor* t : {&qkv, &positions, &q_out, &gate_out, &k_out}) check_cuda(*t, "prologue operand");
+  TORCH_CHECK(positions.scalar_type() == at::kInt && positions.numel() >= rows, "positions must be int32 [rows]");
+  TORCH_CHECK(k_out.scalar_type() == at::kBFloat16 && k_out.numel() >= rows * num_kv_heads * 256, "k_out must be bf16 [rows, kv heads, 256]");
+  AttnArgs a{};
+  a.qkv = ptr(qkv);
+  a.ld_qkv = (int)qkv.size(-1);
+  a.num_q_heads = (int)num_q_heads;
+  a.num_kv_heads = (int)num_kv_heads;
+  a.head_dim = 256;
+  a.rotary_dim = (int)rotary_dim;
+  a.rope_theta = (float)rope_theta;
+  a.q_norm_w = ptr(q_norm_w);
+  a.k_norm_w = ptr(k_norm_w);
+  a.eps = (float)eps;
+  a.page_size = 16;
+  a.positions = ptr<const int>(positions);
+  a.rows = (int)rows;
+  a.q_out = ptr(q_out);
+  a.gate_out = ptr(gate_out);
+  rc(zs_attn_prologue_rows(&a, ptr(k_out), stream()), "zs_attn_prologue_rows");
+}
+
 void attn_decode(const Tensor& q_out, const Tensor& gate_out, int64_t num_q_heads,
                  int64_t num_kv_heads, const Tensor& k_cache, const Tensor& v_cache,
                  int64_t page_size, const Tensor& page_table, const Tensor& slots,
@@ -1198,7 +1224,8 @@ struct QuantPlanState {
     QuantAttnArgs& a = base;
     zs_quant_attn_shape(c.dim, c.bits, (int)std::min<int64_t>(group * max_seq_rows, 1 << 20), &a.tiles, &a.slot_warps, &a.stage);
     a.chunk = 8 * a.tiles * a.slot_warps;
-    a.max_chunks = (int)(max_seqs + max_rows * group / a.chunk);
+    const int64_t of_seq = (group * std::min(max_seq_rows, max_rows) + a.chunk - 1) / a.chunk;
+    a.max_chunks = (int)std::min(max_seqs + max_rows * group / a.chunk, max_seqs * of_seq);
     a.num_q_heads = (int)q_heads;
     a.num_kv_heads = c.heads;
     a.head_dim = c.dim;
@@ -1439,6 +1466,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
      py::arg("num_seqs"), py::arg("ckpt_rows"), py::arg("ckpt_slots"), py::arg("max_ckpt"), py::arg("err"),
      py::arg("out_slots") = py::none(), py::arg("impl") = 0, py::arg("max_seq_rows") = 0);
   m.def("attn_prologue", &attn_prologue);
+  m.def("attn_prologue_rows", &attn_prologue_rows);
   m.def("attn_decode", &attn_decode, py::arg("q_out"), py::arg("gate_out"), py::arg("num_q_heads"),
         py::arg("num_kv_heads"), py::arg("k_cache"), py::arg("v_cache"), py::arg("page_size"), py::arg("page_table"),
         py::arg("slots"), py::arg("seq_lens"), py::arg("rows"), py::arg("partial"), py::arg("num_splits"),

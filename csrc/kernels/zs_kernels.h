@@ -201,6 +201,8 @@ typedef struct AttnArgs {
 } AttnArgs;
 
 int zs_attn_prologue(const AttnArgs* args, cudaStream_t stream);
+// The prologue without the K/V write: K's normed and rotated rows go to k_out (bf16 [rows, Hkv, head_dim]), V stays in qkv.
+int zs_attn_prologue_rows(const AttnArgs* args, void* k_out, cudaStream_t stream);
 int zs_attn_decode(const AttnArgs* args, cudaStream_t stream);
 int zs_attn_prefill(const AttnArgs* args, cudaStream_t stream);
 

@@ -64,7 +64,8 @@ const char* kServeUsage =
     "  --page-block-tokens N        KV page size (default 16)\n"
     "  --num-kv-pages N             KV pages per GPU (default: --gpu-memory-utilization x 32768 / 0.95)\n"
     "  --gpu-memory-utilization F   KV page calibration factor in (0, 1] (default 0.95)\n"
-    "  --kv-cache-dtype auto|bf16   KV cache dtype (the caches are bf16; fp8 is rejected)\n"
+    "  --kv-cache-dtype T           K/V of the attention layers: auto or bf16, or int8 / int4 with a scale and an\n"
+    "                               offset per 64 numbers (CUDA, Qwen3.5 models); fp8 is rejected\n"
     "  --tokenizer-mode auto|chatml|deepseek|deepseek_v41\n"
     "  --enable-prefix-caching | --no-enable-prefix-caching   (default on)\n"
     "  --apc-node-pages N           Pages per prefix-cache node (default 8)\n"
@@ -316,8 +317,13 @@ bool build_engine(const Args& a, Built* b, std::string* err) {
   // fit beside the weights on one 180 GB GPU at 0.95).
   c.num_pages = (uint32_t)a.num("num-kv-pages", std::max<long>(128, std::lround(util / 0.95 * 32768.0)));
   const std::string kv_dtype = a.get("kv-cache-dtype", "auto");
-  if (kv_dtype != "auto" && kv_dtype != "bf16" && kv_dtype != "bfloat16") {
-    *err = "--kv-cache-dtype `" + kv_dtype + "` is not supported: the KV caches are bf16 (pass auto or bf16)";
+  const bool kv_quant = kv_dtype == "int8" || kv_dtype == "int4";
+  if (!kv_quant && kv_dtype != "auto" && kv_dtype != "bf16" && kv_dtype != "bfloat16") {
+    *err = "--kv-cache-dtype `" + kv_dtype + "` is not supported (pass auto, bf16, int8 or int4)";
+    return false;
+  }
+  if (kv_quant && a.get("device", "cuda") != "cuda") {
+    *err = "--kv-cache-dtype " + kv_dtype + " needs --device cuda";
     return false;
   }
   c.max_model_len = (uint32_t)a.num("max-model-len", 32768);
@@ -446,6 +452,8 @@ bool build_engine(const Args& a, Built* b, std::string* err) {
                       std::to_string(c.max_model_len),
                       "--num-ckpt-slots",
                       std::to_string(c.num_ckpt_slots),
+                      "--kv-cache-dtype",
+                      kv_quant ? kv_dtype : std::string("bf16"),
                       "--spec-method",
                       c.spec_method,
                       "--num-spec-tokens",

@@ -9,6 +9,7 @@ CUDA graph per batch bucket.  Per layer (decode or varlen prefill):
               -> out_proj GEMM -> residual add + RMSNorm + MXFP8 quant
   GQA layer : qkv GEMM -> q/k norm + partial RoPE + paged KV write -> split-KV gated
               attention (MXFP8 out) -> o_proj GEMM -> residual add + RMSNorm + quant
+              (K and V in 4 or 8 bits: the write and the attention of ops/quant_cache.py)
   MoE       : router GEMM (f32 logits) -> top-k + grouped scatter -> grouped gate/up
               GEMM with SiLU*up + MXFP8 epilogue -> grouped down GEMM scattering
               weight-scaled rows -> combine of the 9 pair rows + residual + RMSNorm
@@ -38,6 +39,7 @@ from ..config import Qwen35Config
 from ..ops import _ext
 from ..utils.env import runtime_config
 from ..ops import mx
+from ..ops.quant_cache import QuantAttention, QuantCache
 from .weights import RandomWeights
 
 EPI_BF16, EPI_F32, EPI_SILU, EPI_SCATTER, EPI_ARGMAX, EPI_PUSH = 0, 1, 2, 3, 4, 5
@@ -94,7 +96,12 @@ class Qwen35Runner:
     def __init__(self, cfg: Qwen35Config, *, device="cuda", weights=None, max_seqs: int = 256,
                  max_prefill_tokens: int = 4096, num_pages: int = 4096, page_size: int = 16,
                  max_model_len: int = 4096, num_ckpt_slots: int = 0, tp_rank: int = 0, tp_size: int = 1,
-                 collectives=None, seed: int = 0, num_spec_tokens: int = 0):
+                 collectives=None, seed: int = 0, num_spec_tokens: int = 0, kv_bits: int = 16):
+        """``kv_bits`` 4 or 8: the attention layers' K and V are held in a ``QuantCache`` (``self.quant``)
+        instead of bf16 (16)."""
+        if kv_bits not in (4, 8, 16):
+            raise ValueError(f"kv_bits must be 4, 8 or 16, got {kv_bits}")
+        self.kv_bits = kv_bits
         self.cfg = cfg
         self.dev = torch.device(device)
         self.C = _ext.load()
@@ -247,8 +254,13 @@ class Qwen35Runner:
         self.conv_state = torch.zeros(nG, self.num_slots, 2, conv_dim, 3, dtype=torch.bfloat16, device=dev)
         self.ssm_state = torch.zeros(nG, self.num_slots, self.hv, 128, 128, dtype=torch.float32, device=dev)
         kv_shape = (nA, self.num_pages, self.hkv, self.page_size, cfg.head_dim)  # head-major pages
-        self.k_cache = torch.zeros(kv_shape, dtype=torch.bfloat16, device=dev)
-        self.v_cache = torch.zeros(kv_shape, dtype=torch.bfloat16, device=dev)
+        self.quant = None
+        if self.kv_bits == 16:
+            self.k_cache = torch.zeros(kv_shape, dtype=torch.bfloat16, device=dev)
+            self.v_cache = torch.zeros(kv_shape, dtype=torch.bfloat16, device=dev)
+        else:
+            self.quant = QuantCache(nA, self.num_pages, self.hkv, cfg.head_dim, bits=self.kv_bits, page_size=self.page_size,
+                                    device=dev)
         # Page table: one row per request slot (+ dummy row).  Page 0 is the dummy page.
         self.page_table = torch.zeros(self.num_slots, self.max_pages, dtype=torch.int32, device=dev)
 
@@ -291,9 +303,19 @@ class Qwen35Runner:
                                      device=dev)
         b["q_out"] = torch.zeros(R, self.hq, cfg.head_dim, dtype=torch.bfloat16, device=dev)
         b["gate_out"] = torch.zeros(R, self.hq, cfg.head_dim, dtype=torch.bfloat16, device=dev)
+        if self.quant is not None:
+            b["k_rows"] = torch.zeros(R, self.hkv, cfg.head_dim, dtype=torch.bfloat16, device=dev)
+            # By the most rows of a sequence: decode steps, verify steps, everything else.
+            kinds = {1: (self.max_seqs, self.max_seqs)}
+            if self.num_spec:
+                kinds[self.num_spec + 1] = (R, self.max_seqs)
+            kinds[max(R, self.num_spec + 2)] = (R, self.max_seqs)
+            self.quant_plans = {most: QuantAttention(self.quant, self.hq, max_rows=rows, max_seqs=seqs, max_seq_rows=most)
+                                for most, (rows, seqs) in kinds.items()}
         self.max_splits = 16
-        b["partial"] = torch.zeros(max(R * self.hq, self.max_seqs * self.hq * self.max_splits) * 260,
-                                   dtype=torch.float32, device=dev)
+        if self.quant is None or self.num_spec:   # (a draft head's own cache is bf16)
+            b["partial"] = torch.zeros(max(R * self.hq, self.max_seqs * self.hq * self.max_splits) * 260,
+                                       dtype=torch.float32, device=dev)
         nr = self.layers[0]["router"].n_pad
         b["logits"] = torch.zeros(max(R * nr, self.max_ksplit * self.max_seqs * nr), dtype=torch.float32, device=dev)
         G = self.groups
@@ -473,6 +495,9 @@ class Qwen35Runner:
         if plan is not None:
             self.check_plan_rows(rows)
             plan.update(lens)
+        quant = self._quant_plan(rows, decode, num_seqs, max_seq_rows) if self.quant is not None else None
+        if quant is not None:
+            quant.update(slot, lens, None if decode else b["seq_start"][:num_seqs + 1])
         C.embed_rmsnorm_quant(b["in_ids"][:rows], self.embed, b["hidden"], self.layers[0]["input_norm"], 1.0,
                               self.eps, rows, None, b["xq"], b["xsf"])
         for li, L in enumerate(self.layers):
@@ -497,10 +522,20 @@ class Qwen35Runner:
                 ai = self.attn_index[li]
                 qkv = b["proj"][:rows * self.qkv_w].view(rows, self.qkv_w)
                 self._gemm(L["qkv"], b["xq"], b["xsf"], rows, qkv, self.qkv_w)
+                midq = self._mid(self.hq * cfg.head_dim)
+                if quant is not None:
+                    C.attn_prologue_rows(qkv, self.hq, self.hkv, cfg.rotary_dim, cfg.rope_theta, L["q_norm"], L["k_norm"],
+                                         self.eps, pos, rows, b["q_out"], b["gate_out"], b["k_rows"])
+                    v_rows = qkv[:, self.qkv_w - self.hkv * cfg.head_dim:].unflatten(1, (self.hkv, cfg.head_dim))
+                    self.quant.write(ai, b["k_rows"][:rows], v_rows, self.page_table, slot, pos)
+                    quant.attend(ai, b["q_out"][:rows], self.page_table, 1.0 / math.sqrt(cfg.head_dim),
+                                 gate=b["gate_out"][:rows], out_q=midq, out_sf=b["midsf"])
+                    self._proj_out(L["o_proj"], midq, b["midsf"], rows, L["post_norm"])
+                    self._moe_and_next(li, L, rows)
+                    continue
                 C.attn_prologue(qkv, self.hq, self.hkv, cfg.rotary_dim, cfg.rope_theta, L["q_norm"], L["k_norm"],
                                 self.eps, self.k_cache[ai], self.v_cache[ai], self.page_size, self.page_table, slot,
                                 pos, rows, b["q_out"], b["gate_out"])
-                midq = self._mid(self.hq * cfg.head_dim)
                 if plan is not None:
                     plan.attend(b["q_out"][:rows], b["gate_out"][:rows], self.k_cache[ai], self.v_cache[ai],
                                 self.page_table, lens, 1.0 / math.sqrt(cfg.head_dim), out_q=midq, out_sf=b["midsf"])
@@ -516,10 +551,22 @@ class Qwen35Runner:
                                   seq_start=b["seq_start"][:num_seqs + 1] if grouped else None,
                                   num_seqs=num_seqs if grouped else 0)
                 self._proj_out(L["o_proj"], midq, b["midsf"], rows, L["post_norm"])
-            self._moe(L, rows)
-            next_w = self.layers[li + 1]["input_norm"] if li + 1 < len(self.layers) else self.final_norm
-            self._row_parallel_reduce(b["moe_y"], rows, self.k1, next_w, 0, H, term_index=b["pair_src"],
-                                      term_scale=b["pair_w"])
+            self._moe_and_next(li, L, rows)
+
+    def _quant_plan(self, rows: int, decode: bool, num_seqs: int, max_seq_rows: int) -> QuantAttention:
+        """The quantised cache's attention plan of a step: the one for the fewest rows of a sequence that holds it."""
+        if not decode and num_seqs < 1:
+            raise ValueError("varlen steps over a quantised cache need their sequence boundaries")
+        most = 1 if decode else max_seq_rows or rows
+        return self.quant_plans[min(k for k in self.quant_plans if k >= most)]
+
+    def _moe_and_next(self, li: int, L, rows: int) -> None:
+        """The layer's MoE, then the residual sum and the norm that the next layer (or the head) starts from."""
+        b = self.buf
+        self._moe(L, rows)
+        next_w = self.layers[li + 1]["input_norm"] if li + 1 < len(self.layers) else self.final_norm
+        self._row_parallel_reduce(b["moe_y"], rows, self.k1, next_w, 0, self.cfg.hidden_size, term_index=b["pair_src"],
+                                  term_scale=b["pair_w"])
 
     def _moe(self, L, rows: int) -> None:
         cfg, C, b = self.cfg, self.C, self.buf
@@ -578,6 +625,8 @@ class Qwen35Runner:
 
     @prefix_plan.setter
     def prefix_plan(self, plan) -> None:
+        if plan is not None and self.kv_bits != 16:
+            raise ValueError("shared-prefix attention reads a bf16 cache, not a quantised one")
         if plan is not getattr(self, "_prefix_plan", None):
             self._drop_graphs()
         self._prefix_plan = plan
@@ -585,6 +634,8 @@ class Qwen35Runner:
     @contextlib.contextmanager
     def eager_plan(self, plan):
         """`plan` in the place of `prefix_plan` for the steps inside, which replay no graph."""
+        if plan is not None and self.kv_bits != 16:
+            raise ValueError("shared-prefix attention reads a bf16 cache, not a quantised one")
         held, self._prefix_plan = self._prefix_plan, plan
         try:
             yield
@@ -683,7 +734,7 @@ class Qwen35Runner:
 
     def paged_caches(self) -> list[torch.Tensor]:
         """Device tensors indexed [layer, page, ...] (the attention layers' K and V)."""
-        return [self.k_cache, self.v_cache]
+        return [self.k_cache, self.v_cache] if self.quant is None else [self.quant.data]
 
     def copy_recurrent_state(self, src_slot: int, dst_slot: int) -> None:
         """Restore a checkpoint: GDN state and both conv-window buffers of every layer."""
@@ -768,4 +819,7 @@ class Qwen35Runner:
         plan = getattr(self, "prefix_plan", None)
         if not err and plan is not None:
             err = int(plan.err.item())
+        if not err and getattr(self, "quant", None) is not None:
+            for part in (self.quant, *self.quant_plans.values()):
+                err = err or int(part.err.item())
         return err

@@ -362,11 +362,15 @@ class GpuRunner:
             raise ValueError(f"--speculative-method {args.spec_method} does not fit this model (use {want})")
         num_spec = args.num_spec_tokens if args.spec_method == want else 0
         runner_cls = DeepSeekRunner if _is_deepseek(self.cfg) else Qwen35Runner
+        kv_dtype = getattr(args, "kv_cache_dtype", "bf16")
+        if kv_dtype != "bf16" and runner_cls is not Qwen35Runner:
+            raise ValueError(f"--kv-cache-dtype {kv_dtype}: this model's latent and index caches are bf16")
+        kv = {} if kv_dtype == "bf16" else {"kv_bits": {"int8": 8, "int4": 4}[kv_dtype]}
         self.r = runner_cls(self.cfg, device=self.dev, weights=_weights(self.cfg, args.model, args.seed),
                               max_seqs=geo.max_seqs, max_prefill_tokens=geo.max_step_tokens,
                               num_pages=args.num_pages, page_size=geo.page_size, max_model_len=args.max_model_len,
                               num_ckpt_slots=args.num_ckpt_slots, tp_rank=rank, tp_size=world, collectives=coll,
-                              seed=args.seed, num_spec_tokens=num_spec)
+                              seed=args.seed, num_spec_tokens=num_spec, **kv)
         self.rank = rank
         self.head = None  # full-distribution sampling head, created on first use
         self.dram = None

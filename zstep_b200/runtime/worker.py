@@ -160,6 +160,7 @@ def parse_args(argv=None):
     ap.add_argument("--num-pages", type=int, default=4096)
     ap.add_argument("--max-model-len", type=int, default=4096)
     ap.add_argument("--num-ckpt-slots", type=int, default=0)
+    ap.add_argument("--kv-cache-dtype", default="bf16", choices=["bf16", "int8", "int4"], help="K/V of the attention layers")
     ap.add_argument("--spec-method", default="none")
     ap.add_argument("--num-spec-tokens", type=int, default=0)
     ap.add_argument("--dram-kv-blocks", type=int, default=0, help="host DRAM tier blocks (pinned page arena)")
