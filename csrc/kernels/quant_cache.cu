@@ -19,24 +19,13 @@
 // 32-bit scores and to the weights.  The scaled weights are rounded to f16 (2^-11; for f16 outputs a second
 // product takes what that cuts off): the running reference of a row bounds score + log2(scale), so that
 // they stay below 2^15 whatever the size of V.
-#include <cuda_fp16.h>
-
-#include <climits>
+#include <cstdlib>
 #include <type_traits>
 
-#include "sm100_common.cuh"
-#include "zs_kernels.h"
+#include "quant_cache.cuh"
 
 namespace zs {
 namespace qc {
-
-constexpr int TOK = 16;      // tokens of a block
-constexpr int GROUP = 64;    // dims that share a scale and an offset
-constexpr uint32_t POISON = 0x7FFFFFFFu;  // z = NaN, s = NaN with its sign set (a negative 16-bit number)
-
-// Bytes of the block of 16 tokens of one kv head.
-__host__ __device__ constexpr int code_bytes(int d, int bits) { return TOK * d * bits / 8; }
-__host__ __device__ constexpr int block_bytes(int d, int bits) { return 2 * code_bytes(d, bits) + 2 * TOK * (d / GROUP) * 4; }
 
 // Where the 8 numbers of dims d..d+7 (d a multiple of 8) of K's token t are in the block: `bits` bytes.  Rows
 // g and g + 8 of a fragment are the tokens 2g and 2g + 1, and four lanes have 16 dims of a group each.
@@ -58,21 +47,6 @@ __device__ __forceinline__ float bf16_down(float x) {
   const uint32_t u = __float_as_uint(x);
   return __uint_as_float((u >> 31 ? u + 0xFFFFu : u) & 0xFFFF0000u);
 }
-__device__ __forceinline__ float scale_of(uint32_t sz) { return __uint_as_float(sz << 16); }
-__device__ __forceinline__ float offset_of(uint32_t sz) { return __uint_as_float(sz & 0xFFFF0000u); }
-
-__device__ __forceinline__ float2 two_floats(uint32_t u, bool half) {
-  return half ? __half22float2(*reinterpret_cast<const __half2*>(&u)) : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u));
-}
-__device__ __forceinline__ uint32_t two_halves(float a, float b, bool half) {
-  if (half) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 // The block of (slot, position) for kv head 0, or null where there is none.  Heads are `stride` bytes apart.
 __device__ __forceinline__ uint8_t* block_at(const QuantRowsArgs& a, int row, int* token) {
   const int pos = a.positions[row], slot = a.slots[row];
@@ -294,39 +268,6 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) load_kernel(const QuantRowsArg
 // lengths.  One CTA of 1024 threads plans; a step's layers share the plan.
 constexpr int PLAN_THREADS = 1024;
 
-struct Chunk {          // 32 bytes
-  long long before;     // stages of the chunks before, all kv heads
-  int row, slot;        // first row of the sequence, its page-table row
-  int first, count;     // slots [first, first + count) of the sequence
-  int len, stages;      // keys of the longest row among them, stages of one kv head
-};
-
-struct Plan {           // the workspace's integers
-  long long* total;     // stages of all chunks, all kv heads
-  Chunk* table;         // [max_chunks]
-  int2* rows;           // [max_rows] first chunk and first row of the row's sequence (-1: none)
-  int* lens;            // [max_rows] keys of the row
-  int* start;           // [ZS_QUANT_CTAS] chunk of a CTA's first stage
-  int* offset;          // [max_seqs] chunks before the sequence
-};
-
-__host__ __device__ inline Plan plan_of(const QuantAttnArgs& a) {
-  Plan p;
-  uint8_t* w = reinterpret_cast<uint8_t*>(a.work);
-  p.total = reinterpret_cast<long long*>(w);
-  p.table = reinterpret_cast<Chunk*>(w + 32);
-  p.rows = reinterpret_cast<int2*>(p.table + a.max_chunks);
-  p.lens = reinterpret_cast<int*>(p.rows + a.max_rows);
-  p.start = p.lens + a.max_rows;
-  p.offset = p.start + ZS_QUANT_CTAS;
-  return p;
-}
-
-// Number of CTAs that share T stages.
-__device__ __forceinline__ int ctas_of(long long total, int grid, int least) {
-  return (int)max(1ll, min((long long)grid, total / least));
-}
-
 // Exclusive sum over the CTA's threads; *all gets the sum of all.
 __device__ __forceinline__ long long block_scan(long long x, long long* warps, long long* all) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -435,9 +376,6 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const QuantAttnArgs 
 
 // ------------------------------------------------------------------------------- attention
 constexpr int MAX_RING = 8;
-constexpr float LIFT = 11.f;    // log2 of what a weight times its scale is held at: below 2^(11 + 1 + SLACK)
-constexpr float SLACK = 3.f;    // the reference moves when a score goes this far above it
-
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -449,11 +387,6 @@ __device__ __forceinline__ void mma16816_first(float (&c)[4], uint32_t a0, uint3
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
-}
-__device__ __forceinline__ float ex2(float x) {   // 2^x, results below 2^-126 as 0
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -1223,6 +1156,9 @@ int row_blocks(QuantRowsArgs& a) {
   return (int)((some * a.step + ROW_WARPS - 1) / ROW_WARPS);
 }
 
+// More slots of a sequence than this go to quant_wide.cu.
+int most_narrow(int d) { static const int n = getenv("QW") ? atoi(getenv("QW")) : (d == 256 ? 16 : 32); return n; }
+
 // The variant for sequences of so many query slots.
 struct Variant {
   int tiles, warps, blocks, ctas;   // tiles of 8 slots of a warp; warps of a CTA; blocks of a stage; CTAs of an SM
@@ -1232,6 +1168,17 @@ constexpr Variant variant_of(int d, int bits, int slots) {
   if (slots <= 8) return {1, 8, d == 128 && bits == 8 ? 1 : 2, 2};
   if (slots <= 16) return {2, 8, 2, d == 64 ? 2 : 1};
   return {4, 8, d == 64 ? 2 : 1, 1};
+}
+
+template <int D>
+int launch_join(const QuantAttnArgs& a, cudaStream_t stream) {
+  // Warps that share a pair's records: with few pairs a long sequence leaves a record in every CTA.
+  const long long items = (long long)a.rows * a.num_q_heads;
+  int parts = JOIN_WARPS;
+  while (parts > 1 && items * parts > 4096) parts /= 2;
+  const auto join = parts == 8 ? join_kernel<D, 8> : parts == 4 ? join_kernel<D, 4> : parts == 2 ? join_kernel<D, 2> : join_kernel<D, 1>;
+  zs_launch(join, (int)((items * parts + JOIN_WARPS - 1) / JOIN_WARPS), JOIN_WARPS * 32, 0, stream, a);
+  return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
 template <class S>
@@ -1246,13 +1193,7 @@ int launch_attend(QuantAttnArgs a, cudaStream_t stream) {
   const auto kernel = attend_kernel<S>;
   cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   zs_launch(kernel, a.grid, S::WARPS * 32, bytes, stream, a);
-  // Warps that share a pair's records: with few pairs a long sequence leaves a record in every CTA.
-  const long long items = (long long)a.rows * a.num_q_heads;
-  int parts = JOIN_WARPS;
-  while (parts > 1 && items * parts > 4096) parts /= 2;
-  const auto join = parts == 8 ? join_kernel<S::D, 8> : parts == 4 ? join_kernel<S::D, 4> : parts == 2 ? join_kernel<S::D, 2> : join_kernel<S::D, 1>;
-  zs_launch(join, (int)((items * parts + JOIN_WARPS - 1) / JOIN_WARPS), JOIN_WARPS * 32, 0, stream, a);
-  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+  return launch_join<S::D>(a, stream);
 }
 
 template <int D, int BITS, int SLOTS, bool FINE>
@@ -1271,12 +1212,21 @@ int launch_tiles(const QuantAttnArgs& a, cudaStream_t stream) {
 
 template <int D>
 int launch_bits(const QuantAttnArgs& a, cudaStream_t stream) {
+  if (a.chunk == WIDE_SLOTS) {
+    const int e = launch_wide(a, stream);
+    return e ? e : launch_join<D>(a, stream);
+  }
   if (a.bits == 4) return a.half ? launch_tiles<D, 4, true>(a, stream) : launch_tiles<D, 4, false>(a, stream);
   return a.half ? launch_tiles<D, 8, true>(a, stream) : launch_tiles<D, 8, false>(a, stream);
 }
 
 // CTAs of the attention, and the fewest stages that are worth one (a stage a key lane).
 void set_grid(QuantAttnArgs& a) {
+  if (a.chunk == WIDE_SLOTS) {
+    a.grid = 148;
+    a.least = 1;
+    return;
+  }
   const Variant v = variant_of(a.head_dim, a.bits, 8 * a.tiles);
   a.grid = 148 * v.ctas;
   a.least = v.warps / a.slot_warps;
@@ -1316,6 +1266,12 @@ extern "C" int zs_quant_load(const QuantRowsArgs* args, cudaStream_t stream) {
 // The variant for sequences of `slots` query slots: tiles of 8 slots of a warp, warps that share a key lane, keys
 // of a stage.
 extern "C" void zs_quant_attn_shape(int head_dim, int bits, int slots, int* tiles, int* slot_warps, int* stage) {
+  if (slots > zs::qc::most_narrow(head_dim)) {
+    *tiles = zs::qc::WIDE_SLOTS / 8;
+    *slot_warps = 1;
+    *stage = zs::qc::WIDE_KEYS;
+    return;
+  }
   const zs::qc::Variant v = zs::qc::variant_of(head_dim, bits, slots);
   *tiles = v.tiles;
   *stage = v.blocks * zs::qc::TOK;

@@ -1,0 +1,651 @@
+// Attention over the quantised K/V cache for sequences with many query slots (slot = row x head of a
+// kv head's group): the rows of a verify step, chunks of prompts, wide groups.
+//
+// A unit is up to 128 slots of one sequence and kv head; a CTA (one an SM) takes its share of all units'
+// 64-key tiles as in quant_cache.cu, and its records are joined there.  S = Q K^T (M = 128 slots, N = 64
+// keys) and O += P V (N = the dims) run on tcgen05 with Q and P in TMEM, so that a tile is turned into f16
+// once for all slots and shared memory is read once for it:
+//  * copy warp: page ids, then one bulk copy per 16-token block into a ring of tiles;
+//  * 8 converter warps, one for K or V of a block: s n + z as one f16 fused multiply-add of two numbers,
+//    rounded once (2^-12 of a value).  (w & 0x000F000F) is two subnormals n 2^-24 and the factor s 2^24, so a
+//    pair costs an integer instruction, a part of a shift and the multiply-add.  A power of two per block
+//    brings its largest value to [2^-8, 2^-7), which keeps s 2^24 and every value in f16's range whatever
+//    their size; the scores and the weights take it back.  K goes to a swizzled image of keys x dims, V to one
+//    of dims x keys (as it is stored), both K-major operands;
+//  * MMA warp: S of the next tile goes before O of this one;
+//  * softmax warps: a thread has half of a tile's keys for a slot.  The weights 2^(x - reference) are held
+//    below 2^14 times the block's power of two, as f16 (2^-11; for f16 outputs the rest goes through a second
+//    product); the reference follows the largest score only when that outgrew it by 2^3, and O in TMEM is
+//    rescaled then.
+// A poisoned group of V (NaN) is 0 in the image; the slots that see its key note it, and their dims of the
+// group become NaN in the record.  So nothing of a masked key reaches a slot.
+#include "quant_cache.cuh"
+
+namespace zs {
+namespace qc {
+namespace {
+
+constexpr int SOFT = 256, CONV = 256;               // threads; then the MMA and the copy warp
+constexpr int THREADS = SOFT + CONV + 64;
+constexpr int MMA_WARP = (SOFT + CONV) / 32, COPY_WARP = MMA_WARP + 1;
+constexpr int TBLOCKS = WIDE_KEYS / TOK;
+constexpr uint32_t TMEM_Q = 128, TMEM_O = 256, TMEM_COLS = 512;   // two S of 64 columns, Q as pairs, O
+constexpr int MAX_RAW = 4;
+
+struct Smem {
+  uint64_t raw_full[MAX_RAW], raw_empty[MAX_RAW];
+  uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], o_full[2], q_full, unit_full[4];
+  uint32_t tmem;
+  int abort;
+  float k_unit[4][TBLOCKS];          // what the blocks of K of a tile are multiples of
+  float v_log[4][TBLOCKS];           // log2 of the same of V
+  uint32_t v_bad[4][TBLOCKS][2];     // poisoned (token, group) pairs: pair x is bit x / n of word x % n (n words are used)
+  alignas(16) uint32_t pairs[CONV / 32][16 * 4];   // of a converter's block: per group and token, scale and offset in f16
+  float top[2][WIDE_SLOTS];
+};
+
+template <int D_, int BITS_>
+struct Wide {
+  static constexpr int D = D_, BITS = BITS_, NG = D / GROUP;
+  static constexpr int CODES = code_bytes(D, BITS), BLOCK = block_bytes(D, BITS);
+  static constexpr int K_IMAGE = WIDE_KEYS * D * 2, V_IMAGE = D * WIDE_KEYS * 2;
+  static constexpr int IMAGES = 2 * (K_IMAGE + V_IMAGE);
+  static constexpr int RAW = TBLOCKS * BLOCK;
+  static constexpr int RING = (227 * 1024 - IMAGES - (int)sizeof(Smem) - 1024) / RAW < MAX_RAW
+                                  ? (227 * 1024 - IMAGES - (int)sizeof(Smem) - 1024) / RAW : MAX_RAW;
+  static constexpr int BYTES = IMAGES + RING * RAW + (int)sizeof(Smem);
+  static_assert(RING >= 2, "");
+};
+
+struct Piece {
+  int chunk, head, first, n;   // tiles [first, first + n) of the unit
+  int row, slot, slot0, count, len;
+};
+
+// A wait that gave up makes all later ones that would wait give up at once.
+__device__ __forceinline__ bool wait_for(Smem& s, uint64_t* bar, uint32_t phase, int* err) {
+  if (mbar_try_wait(bar, phase)) return true;
+  for (uint32_t i = 0; i < kMbarSpinLimit; ++i) {
+    if (mbar_try_wait(bar, phase)) return true;
+    if (*reinterpret_cast<volatile int*>(&s.abort)) return false;
+    if (i > 64) __nanosleep(64);
+  }
+  report_error(err, kErrMbarTimeout);
+  *reinterpret_cast<volatile int*>(&s.abort) = 1;
+  return false;
+}
+__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ bool soft_any(bool x) {
+  int r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %1, 0;\n\t"
+      "bar.red.or.pred q, 1, 256, p;\n\t"
+      "selp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((int)x)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t sixteenth(uint32_t a) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(0x2C002C00u));
+  return d;
+}
+template <int N>
+__device__ __forceinline__ void lds(uint32_t (&r)[N], const uint8_t* p) {
+  if constexpr (N == 2) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    r[0] = u.x;
+    r[1] = u.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 u = reinterpret_cast<const uint4*>(p)[i];
+      r[4 * i] = u.x;
+      r[4 * i + 1] = u.y;
+      r[4 * i + 2] = u.z;
+      r[4 * i + 3] = u.w;
+    }
+  }
+}
+__device__ __forceinline__ uint4 lds128(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
+
+// A in TMEM, B K-major with a 128-byte swizzle, 8-row groups 1024 bytes apart.
+__device__ __forceinline__ void mma_step(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"((int)add), "n"((1024 >> 4) | (1 << 14) | (2 << 29))
+      : "memory");
+}
+__device__ __forceinline__ uint32_t desc_lo(const void* p) { return (smem_u32(p) >> 4) | ((16 >> 4) << 16); }
+constexpr uint32_t idesc_f16(uint32_t m, uint32_t n) { return 1u << 4 | (n >> 3) << 17 | (m >> 4) << 24; }
+
+// floor(log2 x) of the largest of a warp's numbers, at least -72 (and then the unit at least 2^-64).
+__device__ __forceinline__ int warp_exponent(float x) {
+  const uint32_t u = __reduce_max_sync(0xffffffff, __float_as_uint(x));
+  return min(max((int)(u >> 23) - 127, -72), 118);
+}
+
+template <class W>
+__global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a) {
+  constexpr int D = W::D, BITS = W::BITS, NG = W::NG, BLOCK = W::BLOCK, RING = W::RING;
+  extern __shared__ __align__(1024) uint8_t raw_smem[];
+  uint8_t* k_image = raw_smem;
+  uint8_t* v_image = raw_smem + 2 * W::K_IMAGE;
+  uint8_t* ring = raw_smem + W::IMAGES;
+  Smem& s = *reinterpret_cast<Smem*>(ring + RING * W::RAW);
+  if ((smem_u32(raw_smem) & 1023) != 0) {   // the swizzled images need it
+    report_error(a.err, kErrBadShape);
+    return;
+  }
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (warp == MMA_WARP) {
+    tmem_alloc(&s.tmem, TMEM_COLS);
+    tmem_relinquish();
+  }
+  if (tid == 0) {
+    for (int i = 0; i < RING; ++i) {
+      mbar_init(&s.raw_full[i], 1);
+      mbar_init(&s.raw_empty[i], CONV / 32);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.k_full[i], TBLOCKS);
+      mbar_init(&s.v_full[i], TBLOCKS);
+      mbar_init(&s.k_empty[i], 1);
+      mbar_init(&s.v_empty[i], 1);
+      mbar_init(&s.s_full[i], 1);
+      mbar_init(&s.p_full[i], SOFT);
+      mbar_init(&s.o_full[i], 1);
+    }
+    mbar_init(&s.q_full, SOFT);
+    for (int i = 0; i < 4; ++i) mbar_init(&s.unit_full[i], TBLOCKS);
+    s.abort = 0;
+    fence_barrier_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s.tmem;
+  pdl_wait();
+  pdl_trigger();
+  const Plan plan = plan_of(a);
+  const long long total = *plan.total;
+  const int B = ctas_of(total, gridDim.x, a.least), cta = blockIdx.x;
+  const bool work = cta < B && total > 0;
+  const int group = a.num_q_heads / a.num_kv_heads;
+  // Every role walks the CTA's pieces by itself.
+  long long pos = work ? total * cta / B : 0;
+  const long long hi = work ? total * (cta + 1) / B : 0;
+  int chunk = work ? plan.start[cta] : 0;
+  auto next_piece = [&](Piece& p) {
+    if (pos >= hi) return false;
+    Chunk e = plan.table[chunk];
+    while (e.before + (long long)e.stages * a.num_kv_heads <= pos) e = plan.table[++chunk];
+    const int r = (int)(pos - e.before);
+    p.chunk = chunk;
+    p.head = r / e.stages;
+    p.first = r % e.stages;
+    p.n = (int)min((long long)(e.stages - p.first), hi - pos);
+    p.row = e.row;
+    p.slot = e.slot;
+    p.slot0 = e.first;
+    p.count = e.count;
+    p.len = e.len;
+    pos += p.n;
+    return true;
+  };
+  Piece p;
+
+  if (warp == COPY_WARP) {
+    // ------------------------------------------------------------------ copies
+    const int bshift = a.page_shift - 4;
+    int i = 0, st = 0;
+    uint32_t phase = 1;   // of raw_empty: passes at once in the first round
+    bool ok = true;
+    while (ok && next_piece(p)) {
+      const bool known = p.slot >= 0 && p.slot < a.num_slots;
+      auto page_of = [&](int t) {   // -1: a place that does not exist; raw, so that nothing waits for it here
+        const int blk = (p.first + t) * TBLOCKS + lane;
+        if (lane >= TBLOCKS || t >= p.n || blk * TOK >= p.len) return 0;
+        return known && (blk >> bshift) < a.max_pages ? a.page_table[(size_t)p.slot * a.max_pages + (blk >> bshift)] : -1;
+      };
+      int page = page_of(0);
+      for (int t = 0; ok && t < p.n; ++t, ++i) {
+        const int after = page_of(t + 1);
+        const int blk = (p.first + t) * TBLOCKS + lane, count = min(TBLOCKS, (p.len + TOK - 1) / TOK - (p.first + t) * TBLOCKS);
+        if (page < 0 || page >= a.num_pages) {
+          report_error(a.err, kErrBadShape);
+          page = 0;
+        }
+        ok = __all_sync(0xffffffff, wait_for(s, &s.raw_empty[st], phase, a.err));
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(&s.raw_full[st], count * BLOCK);
+        __syncwarp();
+        if (lane < count)
+          bulk_load(ring + st * W::RAW + lane * BLOCK,
+                    a.data + ((((size_t)page * a.num_kv_heads + p.head) << bshift) + (blk & ((1 << bshift) - 1))) * BLOCK, BLOCK, &s.raw_full[st]);
+        page = after;
+        if (++st == RING) {
+          st = 0;
+          phase ^= 1;
+        }
+      }
+    }
+    // Copies in flight land before the CTA gives its shared memory back.
+    if (lane == 0)
+      for (int m = max(0, i - RING); m < i; ++m) mbar_wait(&s.raw_full[m % RING], (m / RING) & 1, nullptr);
+  } else if (warp == MMA_WARP) {
+    // -------------------------------------------------------------------- MMA
+    const bool leader = elect_one();
+    const uint32_t idesc_s = idesc_f16(WIDE_SLOTS, WIDE_KEYS), idesc_o = idesc_f16(WIDE_SLOTS, D);
+    const uint32_t k_lo = desc_lo(k_image), v_lo = desc_lo(v_image);
+    int ns = 0, no = 0, nq = 0;   // issued products, queries met
+    auto scores = [&](int i) {
+      const int b = i & 1;
+      if (!wait_for(s, &s.k_full[b], (i >> 1) & 1, a.err)) return false;
+      // It takes the place of the P two tiles before.
+      if (i >= 2 && !wait_for(s, &s.o_full[b], ((i >> 1) - 1) & 1, a.err)) return false;
+      tc_fence_after();
+      if (leader) {
+#pragma unroll
+        for (int x = 0; x < D / 16; ++x)
+          mma_step(tmem + b * 64, tmem + TMEM_Q + x * 8, k_lo + (b * W::K_IMAGE + (x >> 2) * WIDE_KEYS * 128) / 16 + (x & 3) * 2, idesc_s, x > 0);
+        tc_commit(&s.k_empty[b]);
+        tc_commit(&s.s_full[b]);
+      }
+      ++ns;
+      return true;
+    };
+    auto output = [&](int i, bool fresh) {
+      const int b = i & 1;
+      if (!wait_for(s, &s.v_full[b], (i >> 1) & 1, a.err)) return false;
+      if (!wait_for(s, &s.p_full[b], (i >> 1) & 1, a.err)) return false;
+      tc_fence_after();
+      if (leader) {
+#pragma unroll
+        for (int k = 0; k < WIDE_KEYS / 16; ++k)
+          mma_step(tmem + TMEM_O, tmem + b * 64 + k * 8, v_lo + b * W::V_IMAGE / 16 + k * 2, idesc_o, !fresh || k > 0);
+        if (a.half) {
+#pragma unroll
+          for (int k = 0; k < WIDE_KEYS / 16; ++k)   // what the rounding of P left
+            mma_step(tmem + TMEM_O, tmem + b * 64 + 32 + k * 8, v_lo + b * W::V_IMAGE / 16 + k * 2, idesc_o, true);
+        }
+        tc_commit(&s.v_empty[b]);
+        tc_commit(&s.o_full[b]);
+      }
+      ++no;
+      return true;
+    };
+    int i = 0;
+    bool ok = true;
+    while (ok && next_piece(p)) {
+      ok = __all_sync(0xffffffff, wait_for(s, &s.q_full, nq++ & 1, a.err) && scores(i));
+      for (int t = 0; ok && t < p.n; ++t, ++i) {
+        // S of the piece's next tile goes before O of this one; the next piece's waits for its queries.
+        const bool good = (t + 1 >= p.n || scores(i + 1)) && output(i, t == 0);
+        ok = __all_sync(0xffffffff, good);
+      }
+    }
+    // The issued products end before TMEM is released.
+    if (ns > 0) mbar_wait(&s.s_full[(ns - 1) & 1], ((ns - 1) >> 1) & 1, nullptr);
+    if (no > 0) mbar_wait(&s.o_full[(no - 1) & 1], ((no - 1) >> 1) & 1, nullptr);
+    __syncwarp();
+  } else if (warp >= SOFT / 32) {
+    // -------------------------------------------------------------- converters
+    const int w = warp - SOFT / 32, kb = w & (TBLOCKS - 1), g = lane >> 2, t4 = lane & 3;
+    const bool is_v = w >= TBLOCKS;
+    constexpr float TOP = (1 << BITS) - 1;
+    constexpr int PAIRS = (TOK * NG + 31) / 32;
+    int i = 0, st = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    while (ok && next_piece(p)) {
+      for (int t = 0; ok && t < p.n; ++t, ++i) {
+        const int b = i & 1, left = p.len - (p.first + t) * WIDE_KEYS - kb * TOK;   // keys of the block from here on
+        const uint8_t* in = ring + st * W::RAW + kb * BLOCK;
+        ok = __all_sync(0xffffffff, wait_for(s, &s.raw_full[st], phase, a.err));
+        if (!ok) break;
+        // The block's unit from its scales and offsets (a lane has one or two of the 16 NG pairs), and those as multiples
+        // of it: s 2^24 and z.  What is behind the sequence does not count, and is 0 in V, as poisoned groups are.
+        {
+          const uint32_t* sz = reinterpret_cast<const uint32_t*>(in + 2 * W::CODES + (is_v ? TOK * NG * 4 : 0));
+          float sf[PAIRS], zf[PAIRS], top = 0.f;
+          uint32_t bad[PAIRS];
+#pragma unroll
+          for (int c = 0; c < PAIRS; ++c) {
+            const int x = lane * PAIRS + c, token = x / NG;
+            const uint32_t u = x < TOK * NG ? sz[x] : 0;
+            const bool nan = (u & 0x7FFFu) > 0x7F80u, out = token >= left;
+            sf[c] = scale_of(u);
+            zf[c] = offset_of(u);
+            bad[c] = __ballot_sync(0xffffffff, nan && !out);
+            if (nan || out) {
+              if (is_v) sf[c] = zf[c] = 0.f;
+            } else {
+              top = fmaxf(top, fmaf(TOP, sf[c], fabsf(zf[c])));
+            }
+          }
+          const int e = warp_exponent(top) + 8;
+          const float f1 = __uint_as_float((uint32_t)(127 - (e >> 1)) << 23), f2 = __uint_as_float((uint32_t)(127 - (e - (e >> 1))) << 23);
+#pragma unroll
+          for (int c = 0; c < PAIRS; ++c) {
+            const int x = lane * PAIRS + c;
+            if (x < TOK * NG) s.pairs[w][x % NG * TOK + x / NG] = pack_f16(sf[c] * f1 * f2 * 0x1p24f, zf[c] * f1 * f2);
+          }
+          if (lane == 0) {
+            if (is_v) {
+              s.v_log[i & 3][kb] = (float)e;
+              s.v_bad[i & 3][kb][0] = bad[0];
+              s.v_bad[i & 3][kb][1] = PAIRS > 1 ? bad[PAIRS - 1] : 0;
+            } else {
+              s.k_unit[i & 3][kb] = __uint_as_float((uint32_t)min(e + 127, 254) << 23);
+            }
+          }
+          __syncwarp();
+          if (is_v && lane == 0) mbar_arrive(&s.unit_full[i & 3]);   // the softmax need not wait for the image
+        }
+        if (i >= 2) ok = __all_sync(0xffffffff, wait_for(s, is_v ? &s.v_empty[b] : &s.k_empty[b], ((i >> 1) - 1) & 1, a.err));
+        if (!ok) break;
+        if (!is_v) {
+          const int r0 = kb * 16 + 2 * g;
+          uint8_t* out = k_image + b * W::K_IMAGE + r0 * 128;
+          // Every second row the other way round: the lanes of a phase then touch 32 banks.
+          const int flip = g & 1, at0 = ((t4 * 2 + flip) ^ (r0 & 7)) << 4, at1 = at0 ^ 16;
+#pragma unroll 1
+          for (int gi = 0; gi < NG; ++gi) {
+            const uint2 sz = *reinterpret_cast<const uint2*>(&s.pairs[w][gi * TOK + 2 * g]);
+#pragma unroll
+            for (int tk = 0; tk < 2; ++tk) {
+              const uint32_t pair = tk ? sz.y : sz.x, S = __byte_perm(pair, pair, 0x1010), Z = __byte_perm(pair, pair, 0x3232);
+              uint8_t* row = out + gi * (WIDE_KEYS * 128) + tk * 128;   // an odd row: pieces and their neighbours change places
+              if constexpr (BITS == 4) {
+                const uint2 u = *reinterpret_cast<const uint2*>(in + gi * 512 + lane * 16 + tk * 8);
+                const uint32_t n0 = flip ? u.y : u.x, n1 = flip ? u.x : u.y, m0 = n0 >> 8, m1 = n1 >> 8, T = sixteenth(S);
+                *reinterpret_cast<uint4*>(row + (at0 ^ (tk * 16))) =
+                    make_uint4(fma2(n0 & 0x000F000Fu, S, Z), fma2(n0 & 0x00F000F0u, T, Z), fma2(m0 & 0x000F000Fu, S, Z), fma2(m0 & 0x00F000F0u, T, Z));
+                *reinterpret_cast<uint4*>(row + (at1 ^ (tk * 16))) =
+                    make_uint4(fma2(n1 & 0x000F000Fu, S, Z), fma2(n1 & 0x00F000F0u, T, Z), fma2(m1 & 0x000F000Fu, S, Z), fma2(m1 & 0x00F000F0u, T, Z));
+              } else {
+                const uint4 u = lds128(in + gi * 1024 + tk * 512 + lane * 16);
+                const uint32_t n0 = flip ? u.z : u.x, m0 = flip ? u.w : u.y, n1 = flip ? u.x : u.z, m1 = flip ? u.y : u.w;
+                *reinterpret_cast<uint4*>(row + (at0 ^ (tk * 16))) =
+                    make_uint4(fma2(n0 & 0x00FF00FFu, S, Z), fma2((n0 >> 8) & 0x00FF00FFu, S, Z), fma2(m0 & 0x00FF00FFu, S, Z), fma2((m0 >> 8) & 0x00FF00FFu, S, Z));
+                *reinterpret_cast<uint4*>(row + (at1 ^ (tk * 16))) =
+                    make_uint4(fma2(n1 & 0x00FF00FFu, S, Z), fma2((n1 >> 8) & 0x00FF00FFu, S, Z), fma2(m1 & 0x00FF00FFu, S, Z), fma2((m1 >> 8) & 0x00FF00FFu, S, Z));
+              }
+            }
+          }
+        } else {
+          const int perm = (2 * g + (g >> 2)) & 7;
+          uint8_t* out = v_image + b * W::V_IMAGE + perm * 128 + (((kb * 2 + (t4 >> 1)) ^ perm) << 4) + (t4 & 1) * 8;
+#pragma unroll 1
+          for (int gi = 0; gi < NG; ++gi, out += 64 * 128) {
+            const uint4 sz = *reinterpret_cast<const uint4*>(&s.pairs[w][gi * TOK + t4 * 4]);
+            const uint32_t S0 = __byte_perm(sz.x, sz.z, 0x5410), Z0 = __byte_perm(sz.x, sz.z, 0x7632);
+            const uint32_t S1 = __byte_perm(sz.y, sz.w, 0x5410), Z1 = __byte_perm(sz.y, sz.w, 0x7632);
+#pragma unroll
+            for (int h = 0; h < BITS / 4; ++h) {
+              const uint4 u = lds128(in + W::CODES + gi * (BITS * 128) + h * 512 + lane * 16);
+              const uint32_t n[4] = {u.x, u.y, u.z, u.w};
+              const uint32_t T0 = sixteenth(S0), T1 = sixteenth(S1);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {   // 4 bits: dims 2k and 2k + 1; 8 bits: dim 4h + k
+                const uint32_t x = n[k], y = n[k] >> 8;
+                if constexpr (BITS == 4) {
+                  *reinterpret_cast<uint2*>(out + 2 * k * 1024) = make_uint2(fma2(x & 0x000F000Fu, S0, Z0), fma2(y & 0x000F000Fu, S1, Z1));
+                  *reinterpret_cast<uint2*>(out + (2 * k + 1) * 1024) = make_uint2(fma2(x & 0x00F000F0u, T0, Z0), fma2(y & 0x00F000F0u, T1, Z1));
+                } else {
+                  *reinterpret_cast<uint2*>(out + (4 * h + k) * 1024) = make_uint2(fma2(x & 0x00FF00FFu, S0, Z0), fma2(y & 0x00FF00FFu, S1, Z1));
+                }
+              }
+            }
+          }
+        }
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&s.raw_empty[st]);
+          mbar_arrive(is_v ? &s.v_full[b] : &s.k_full[b]);
+        }
+        if (++st == RING) {
+          st = 0;
+          phase ^= 1;
+        }
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax
+    // After a wait that gave up these warps go on to their last piece's end (every later wait gives up at
+    // once), so that their barriers meet.
+    const int half = warp >> 2, slot = (warp & 3) * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    int i = 0;
+    while (next_piece(p)) {
+      const bool used = slot < p.count, busy = (warp & 3) * 32 < p.count;
+      const int id = p.slot0 + min(slot, p.count - 1), row = p.row + id / group;
+      const int limit = used ? plan.lens[row] : 0;
+      float fac;
+      {
+        // The slot's half of the query, brought to [2^13, 2^14) by a power of two, as pairs in the order in which
+        // the converters leave K's dims: 0 4 1 5 2 6 3 7, or 0 2 1 3 4 6 5 7.
+        const uint4* from = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + (size_t)row * a.q_row +
+                                                           (size_t)(p.head * group + id % group) * a.q_head + half * (D / 2));
+        float big = 0.f, nan = 0.f;
+        if (busy) {
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) {
+            const uint4 u = from[j];
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = two_floats(w[k], a.half);
+              big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
+              nan = fmaf(f.x, 0.f, fmaf(f.y, 0.f, nan));
+            }
+          }
+        }
+        s.top[half][slot] = nan == 0.f ? big : INFINITY;
+        soft_sync();
+        big = fmaxf(s.top[0][slot], s.top[1][slot]);
+        soft_sync();
+        const int e = 13 - min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 100);
+        const float up = big < INFINITY ? copysignf(__uint_as_float((uint32_t)(e + 127) << 23), a.sm_scale) : NAN;
+        fac = fabsf(a.sm_scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - e) << 23);
+        if (busy) {
+#pragma unroll
+          for (int c = 0; c < D / 4; c += 16) {
+            uint32_t y[16];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint4 u = from[c / 4 + j];   // from the cache
+              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+              float x[8];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float2 f = two_floats(w[k], a.half);
+                x[2 * k] = f.x * up;
+                x[2 * k + 1] = f.y * up;
+              }
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                y[4 * j + k] = BITS == 4 ? pack_f16(x[k], x[k + 4]) : pack_f16(x[(k >> 1) * 4 + (k & 1)], x[(k >> 1) * 4 + (k & 1) + 2]);
+            }
+            tmem_st_32x32b_x16(lanes + TMEM_Q + half * (D / 4) + c, y);
+          }
+          tmem_st_wait();
+        }
+        tc_fence_before();
+        mbar_arrive(&s.q_full);
+      }
+      float ref = -INFINITY, l = 0.f;
+      uint32_t bad = 0;
+      for (int t = 0; t < p.n; ++t, ++i) {
+        const int b = i & 1, valid = limit - (p.first + t) * WIDE_KEYS - half * 32;
+        wait_for(s, &s.s_full[b], (i >> 1) & 1, a.err);
+        wait_for(s, &s.unit_full[i & 3], (i >> 2) & 1, a.err);
+        tc_fence_after();
+        uint32_t r[32];
+        float most = -INFINITY;
+        const float v0 = s.v_log[i & 3][2 * half], v1 = s.v_log[i & 3][2 * half + 1];
+        const float f0 = fmaxf(fac * s.k_unit[i & 3][2 * half], 0x1p-126f), f1 = fmaxf(fac * s.k_unit[i & 3][2 * half + 1], 0x1p-126f);
+        if (busy) {
+          tmem_ld_32x32b_x32(lanes + b * 64 + half * 32, r);
+          tmem_ld_wait();
+          if (__any_sync(0xffffffff, valid < 32)) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j >= valid) r[j] = 0xFF800000u;
+          }
+          float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int j = 0; j < 32; ++j) x[(j >> 4) * 2 + (j & 1)] = fmaxf(x[(j >> 4) * 2 + (j & 1)], __uint_as_float(r[j]));
+          most = fmaxf(fmaf(fmaxf(x[0], x[1]), f0, v0), fmaf(fmaxf(x[2], x[3]), f1, v1));
+        }
+        tc_fence_before();
+        // All of S is read (P takes its place); does a slot's reference have to move?
+        if (soft_any(used && most > ref + SLACK)) {
+          s.top[half][slot] = most;
+          soft_sync();
+          most = fmaxf(most, s.top[half ^ 1][slot]);
+          const bool grow = used && most > ref + SLACK;
+          const float f = grow ? ex2(ref - most) : 1.f;
+          if (grow) {
+            l *= f;
+            ref = most;
+          }
+          if (t > 0 && __any_sync(0xffffffff, grow)) {
+            wait_for(s, &s.o_full[b ^ 1], ((i - 1) >> 1) & 1, a.err);   // O holds every tile before this one
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D / 2; c += 16) {
+              uint32_t o[16];
+              const uint32_t at = lanes + TMEM_O + half * (D / 2) + c;
+              tmem_ld_32x32b_x16(at, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              tmem_st_32x32b_x16(at, o);
+            }
+            tmem_st_wait();
+          }
+          soft_sync();   // the maxima have been read
+        }
+        tc_fence_after();
+        if (busy) {
+          const float off = ref == -INFINITY ? 0.f : LIFT - ref, o0 = off + v0, o1 = off + v1;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float w = ex2(fmaf(__uint_as_float(r[j]), j < 16 ? f0 : f1, j < 16 ? o0 : o1));
+            r[j] = __float_as_uint(w);
+            sum[(j >> 4) * 2 + (j & 1)] += w;
+          }
+          l += (sum[0] + sum[1]) * ex2(-v0) + (sum[2] + sum[3]) * ex2(-v1);
+          // Tokens of a four lie in the order 0 2 1 3 in V's image.
+          uint32_t pk[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int k = (j >> 1) * 4 + (j & 1);
+            pk[j] = pack_f16(__uint_as_float(r[k]), __uint_as_float(r[k + 2]));
+          }
+          tmem_st_32x32b_x16(lanes + b * 64 + half * 16, pk);
+          if (a.half) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const int k = (j >> 1) * 4 + (j & 1);
+              const float2 cut = __half22float2(*reinterpret_cast<const __half2*>(&pk[j]));
+              pk[j] = pack_f16(__uint_as_float(r[k]) - cut.x, __uint_as_float(r[k + 2]) - cut.y);
+            }
+            tmem_st_32x32b_x16(lanes + b * 64 + 32 + half * 16, pk);
+          }
+          tmem_st_wait();
+          const uint32_t* poison = s.v_bad[i & 3][2 * half];
+          if (poison[0] | poison[1] | poison[2] | poison[3]) {
+            constexpr int PAIRS = (TOK * NG + 31) / 32;
+            for (int j = 0; j < min(valid, 32); ++j)
+              for (int gi = 0; gi < NG; ++gi) {
+                const int x = (j & 15) * NG + gi;
+                bad |= (poison[(j >> 4) * 2 + x % PAIRS] >> (x / PAIRS) & 1) << gi;
+              }
+          }
+        }
+        tc_fence_before();
+        mbar_arrive(&s.p_full[b]);
+      }
+      // ---- the slots' records
+      wait_for(s, &s.o_full[(i - 1) & 1], ((i - 1) >> 1) & 1, a.err);
+      tc_fence_after();
+      s.top[half][slot] = l;
+      soft_sync();
+      l += s.top[half ^ 1][slot];
+      soft_sync();
+      s.top[half][slot] = __uint_as_float(bad);
+      soft_sync();
+      bad |= __float_as_uint(s.top[half ^ 1][slot]);
+      soft_sync();
+      const size_t rec = (size_t)p.chunk * a.num_kv_heads + p.head + cta;
+      float* to = a.partial + rec * WIDE_SLOTS * (D + 2);
+      if (busy) {
+#pragma unroll 1
+        for (int x = 0; x < D / 64; ++x) {   // 32 columns: four dims of each of a group's octets
+          const int c = half * (D / 2) + x * 32, gi = c >> 6;
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(lanes + TMEM_O + c, o);
+          tmem_ld_wait();
+          const bool nan = bad >> gi & 1;
+          float* at = to + (size_t)slot * D + gi * 64 + (c >> 3 & 7);
+          if (used) {
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {   // column 8 j + perm(g) is dim 8 g + j
+              const int perm = (2 * g + (g >> 2)) & 7;
+              float v[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) v[j] = nan ? NAN : __uint_as_float(o[j * 8 + perm]);
+              *reinterpret_cast<float4*>(at + g * 8) = make_float4(v[0], v[1], v[2], v[3]);
+            }
+          }
+        }
+        if (used && half == 0) *reinterpret_cast<float2*>(to + (size_t)WIDE_SLOTS * D + 2 * slot) = make_float2(ref, l);
+      }
+      tc_fence_before();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == MMA_WARP) tmem_dealloc(tmem, TMEM_COLS);
+}
+
+template <int D, int BITS>
+int launch(const QuantAttnArgs& a, cudaStream_t stream) {
+  using W = Wide<D, BITS>;
+  const auto kernel = wide_kernel<W>;
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, W::BYTES);
+  zs_launch(kernel, a.grid, THREADS, W::BYTES, stream, a);
+  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+}
+
+}  // namespace
+
+int launch_wide(QuantAttnArgs a, cudaStream_t stream) {
+  if (a.chunk != WIDE_SLOTS || a.stage != WIDE_KEYS || a.grid > 148) return -1;
+  if (a.head_dim == 64) return a.bits == 4 ? launch<64, 4>(a, stream) : launch<64, 8>(a, stream);
+  if (a.head_dim == 128) return a.bits == 4 ? launch<128, 4>(a, stream) : launch<128, 8>(a, stream);
+  return a.bits == 4 ? launch<256, 4>(a, stream) : launch<256, 8>(a, stream);
+}
+
+}  // namespace qc
+}  // namespace zs
