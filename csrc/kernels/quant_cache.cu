@@ -1003,7 +1003,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
 // first for its weight, then four at a time.
 constexpr int JOIN_WARPS = 8;
 
-template <int D, int PARTS>
+template <int D, int PARTS, bool WIDE>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const QuantAttnArgs a) {
   constexpr int PER = D / 32;
   pdl_wait();
@@ -1057,7 +1057,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const QuantAttnAr
 #pragma unroll
     for (int j = 0; j < PER; ++j) o[j] *= f;
     const int cnt = min(32, mine - i0);
-    const float* from = rec + i0 * step + at * D + lane * PER;
+    const float* from = rec + i0 * step + at * D;
     for (int i = 0; i < cnt; i += 4) {
       float x[4][PER];
 #pragma unroll
@@ -1065,9 +1065,15 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const QuantAttnAr
         if (i + k < cnt) {
 #pragma unroll
           for (int j = 0; j < PER; j += 2) {
-            const float2 y = *reinterpret_cast<const float2*>(from + (i + k) * step + j);
-            x[k][j] = y.x;
-            x[k][j + 1] = y.y;
+            if (WIDE) {   // dim 8 g + j of a group is at 8 j + perm(g) there
+              const int d = lane * PER + j, g = (d & 63) >> 3, to = (d & ~63) + (d & 7) * 8 + ((2 * g + (g >> 2)) & 7);
+              x[k][j] = from[(i + k) * step + to];
+              x[k][j + 1] = from[(i + k) * step + to + 8];
+            } else {
+              const float2 y = *reinterpret_cast<const float2*>(from + (i + k) * step + lane * PER + j);
+              x[k][j] = y.x;
+              x[k][j + 1] = y.y;
+            }
           }
         }
 #pragma unroll
@@ -1170,13 +1176,13 @@ constexpr Variant variant_of(int d, int bits, int slots) {
   return {4, 8, d == 64 ? 2 : 1, 1};
 }
 
-template <int D>
+template <int D, bool WIDE>
 int launch_join(const QuantAttnArgs& a, cudaStream_t stream) {
   // Warps that share a pair's records: with few pairs a long sequence leaves a record in every CTA.
   const long long items = (long long)a.rows * a.num_q_heads;
   int parts = JOIN_WARPS;
   while (parts > 1 && items * parts > 4096) parts /= 2;
-  const auto join = parts == 8 ? join_kernel<D, 8> : parts == 4 ? join_kernel<D, 4> : parts == 2 ? join_kernel<D, 2> : join_kernel<D, 1>;
+  const auto join = parts == 8 ? join_kernel<D, 8, WIDE> : parts == 4 ? join_kernel<D, 4, WIDE> : parts == 2 ? join_kernel<D, 2, WIDE> : join_kernel<D, 1, WIDE>;
   zs_launch(join, (int)((items * parts + JOIN_WARPS - 1) / JOIN_WARPS), JOIN_WARPS * 32, 0, stream, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
@@ -1193,7 +1199,7 @@ int launch_attend(QuantAttnArgs a, cudaStream_t stream) {
   const auto kernel = attend_kernel<S>;
   cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   zs_launch(kernel, a.grid, S::WARPS * 32, bytes, stream, a);
-  return launch_join<S::D>(a, stream);
+  return launch_join<S::D, false>(a, stream);
 }
 
 template <int D, int BITS, int SLOTS, bool FINE>
@@ -1214,7 +1220,7 @@ template <int D>
 int launch_bits(const QuantAttnArgs& a, cudaStream_t stream) {
   if (a.chunk == WIDE_SLOTS) {
     const int e = launch_wide(a, stream);
-    return e ? e : launch_join<D>(a, stream);
+    return e ? e : launch_join<D, true>(a, stream);
   }
   if (a.bits == 4) return a.half ? launch_tiles<D, 4, true>(a, stream) : launch_tiles<D, 4, false>(a, stream);
   return a.half ? launch_tiles<D, 8, true>(a, stream) : launch_tiles<D, 8, false>(a, stream);

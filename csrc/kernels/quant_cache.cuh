@@ -40,8 +40,9 @@ __device__ __forceinline__ float ex2(float x) {   // 2^x, results below 2^-126 a
   return y;
 }
 
-constexpr float LIFT = 11.f;    // log2 of what a weight times its scale is held at: below 2^(11 + 1 + SLACK)
-constexpr float SLACK = 3.f;    // the reference moves when a score goes this far above it
+// The weights of a row are held as f16 numbers against a reference that bounds its scores (with the scales of V):
+// at most 2^LIFT where it is exact, 2^(LIFT + SLACK) before it is moved, and twice that with a scale's mantissa.
+constexpr float LIFT = 6.f, SLACK = 8.f;
 
 struct Chunk {          // 32 bytes
   long long before;     // stages of the chunks before, all kv heads

@@ -25,7 +25,11 @@ namespace zs {
 namespace qc {
 namespace {
 
-constexpr int SOFT = 256, CONV = 256;               // threads; then the MMA and the copy warp
+constexpr int SOFT = 256, CONV = 512;               // threads; then the MMA and the copy warp
+constexpr int TEAM = CONV / 64;                     // converter warps of a tile: of K and of V of each block
+// Registers of a thread at launch (65536 / 832 threads, in eights), of the softmax and of the converter warps: 256 x 104 +
+// 512 x 56 + 64 x 72 = 832 x 72.
+constexpr int REGS = 72, SOFT_REGS = 104, CONV_REGS = 56;
 constexpr int THREADS = SOFT + CONV + 64;
 constexpr int MMA_WARP = (SOFT + CONV) / 32, COPY_WARP = MMA_WARP + 1;
 constexpr int TBLOCKS = WIDE_KEYS / TOK;
@@ -40,8 +44,9 @@ struct Smem {
   float k_unit[4][TBLOCKS];          // what the blocks of K of a tile are multiples of
   float v_log[4][TBLOCKS];           // log2 of the same of V
   uint32_t v_bad[4][TBLOCKS][2];     // poisoned (token, group) pairs: pair x is bit x / n of word x % n (n words are used)
-  alignas(16) uint32_t pairs[CONV / 32][16 * 4];   // of a converter's block: per group and token, scale and offset in f16
+  alignas(16) uint32_t pairs[CONV / 32][TOK * 4];   // of a converter's block: per group and token, scale and offset in f16
   float top[2][WIDE_SLOTS];
+  alignas(16) float stage[SOFT / 32][32][20];   // 16 columns of a warp's 32 slots, on their way to the record
 };
 
 template <int D_, int BITS_>
@@ -159,7 +164,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
   if (tid == 0) {
     for (int i = 0; i < RING; ++i) {
       mbar_init(&s.raw_full[i], 1);
-      mbar_init(&s.raw_empty[i], CONV / 32);
+      mbar_init(&s.raw_empty[i], TEAM);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.k_full[i], TBLOCKS);
@@ -277,11 +282,11 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
       if (leader) {
 #pragma unroll
         for (int k = 0; k < WIDE_KEYS / 16; ++k)
-          mma_step(tmem + TMEM_O, tmem + b * 64 + k * 8, v_lo + b * W::V_IMAGE / 16 + k * 2, idesc_o, !fresh || k > 0);
+          mma_step(tmem + TMEM_O, tmem + b * 64 + (k >> 1) * 32 + (k & 1) * 8, v_lo + b * W::V_IMAGE / 16 + k * 2, idesc_o, !fresh || k > 0);
         if (a.half) {
 #pragma unroll
           for (int k = 0; k < WIDE_KEYS / 16; ++k)   // what the rounding of P left
-            mma_step(tmem + TMEM_O, tmem + b * 64 + 32 + k * 8, v_lo + b * W::V_IMAGE / 16 + k * 2, idesc_o, true);
+            mma_step(tmem + TMEM_O, tmem + b * 64 + (k >> 1) * 32 + 16 + (k & 1) * 8, v_lo + b * W::V_IMAGE / 16 + k * 2, idesc_o, true);
         }
         tc_commit(&s.v_empty[b]);
         tc_commit(&s.o_full[b]);
@@ -305,18 +310,20 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
     __syncwarp();
   } else if (warp >= SOFT / 32) {
     // -------------------------------------------------------------- converters
-    const int w = warp - SOFT / 32, kb = w & (TBLOCKS - 1), g = lane >> 2, t4 = lane & 3;
-    const bool is_v = w >= TBLOCKS;
+    // Two teams of eight warps take turns, so that a tile has the time of two; a team's image is its own.
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CONV_REGS));
+    const int w = warp - SOFT / 32, b = w / TEAM, kb = w & (TBLOCKS - 1), g = lane >> 2, t4 = lane & 3;
+    const bool is_v = w % TEAM >= TBLOCKS;
     constexpr float TOP = (1 << BITS) - 1;
     constexpr int PAIRS = (TOK * NG + 31) / 32;
-    int i = 0, st = 0;
-    uint32_t phase = 0;
+    int i = 0;
     bool ok = true;
     while (ok && next_piece(p)) {
       for (int t = 0; ok && t < p.n; ++t, ++i) {
-        const int b = i & 1, left = p.len - (p.first + t) * WIDE_KEYS - kb * TOK;   // keys of the block from here on
+        if ((i & 1) != b) continue;
+        const int st = i % RING, left = p.len - (p.first + t) * WIDE_KEYS - kb * TOK;   // keys of the block from here on
         const uint8_t* in = ring + st * W::RAW + kb * BLOCK;
-        ok = __all_sync(0xffffffff, wait_for(s, &s.raw_full[st], phase, a.err));
+        ok = __all_sync(0xffffffff, wait_for(s, &s.raw_full[st], (i / RING) & 1, a.err));
         if (!ok) break;
         // The block's unit from its scales and offsets (a lane has one or two of the 16 NG pairs), and those as multiples
         // of it: s 2^24 and z.  What is behind the sequence does not count, and is 0 in V, as poisoned groups are.
@@ -420,16 +427,13 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
           mbar_arrive(&s.raw_empty[st]);
           mbar_arrive(is_v ? &s.v_full[b] : &s.k_full[b]);
         }
-        if (++st == RING) {
-          st = 0;
-          phase ^= 1;
-        }
       }
     }
   } else {
     // ---------------------------------------------------------------- softmax
     // After a wait that gave up these warps go on to their last piece's end (every later wait gives up at
     // once), so that their barriers meet.
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFT_REGS));
     const int half = warp >> 2, slot = (warp & 3) * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     int i = 0;
@@ -443,18 +447,18 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
         // the converters leave K's dims: 0 4 1 5 2 6 3 7, or 0 2 1 3 4 6 5 7.
         const uint4* from = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + (size_t)row * a.q_row +
                                                            (size_t)(p.head * group + id % group) * a.q_head + half * (D / 2));
+        uint4 u[D / 16];
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) u[j] = busy ? from[j] : make_uint4(0, 0, 0, 0);
         float big = 0.f, nan = 0.f;
-        if (busy) {
 #pragma unroll
-          for (int j = 0; j < D / 16; ++j) {
-            const uint4 u = from[j];
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        for (int j = 0; j < D / 16; ++j) {
+          const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float2 f = two_floats(w[k], a.half);
-              big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
-              nan = fmaf(f.x, 0.f, fmaf(f.y, 0.f, nan));
-            }
+          for (int k = 0; k < 4; ++k) {
+            const float2 f = two_floats(w[k], a.half);
+            big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
+            nan = fmaf(f.x, 0.f, fmaf(f.y, 0.f, nan));
           }
         }
         s.top[half][slot] = nan == 0.f ? big : INFINITY;
@@ -470,8 +474,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
             uint32_t y[16];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const uint4 u = from[c / 4 + j];   // from the cache
-              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+              const uint32_t w[4] = {u[c / 4 + j].x, u[c / 4 + j].y, u[c / 4 + j].z, u[c / 4 + j].w};
               float x[8];
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
@@ -515,7 +518,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
           most = fmaxf(fmaf(fmaxf(x[0], x[1]), f0, v0), fmaf(fmaxf(x[2], x[3]), f1, v1));
         }
         tc_fence_before();
-        // All of S is read (P takes its place); does a slot's reference have to move?
+        // Does a slot's reference have to move?
         if (soft_any(used && most > ref + SLACK)) {
           s.top[half][slot] = most;
           soft_sync();
@@ -561,7 +564,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
             const int k = (j >> 1) * 4 + (j & 1);
             pk[j] = pack_f16(__uint_as_float(r[k]), __uint_as_float(r[k + 2]));
           }
-          tmem_st_32x32b_x16(lanes + b * 64 + half * 16, pk);
+          tmem_st_32x32b_x16(lanes + b * 64 + half * 32, pk);   // in the place of its own scores
           if (a.half) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
@@ -569,7 +572,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
               const float2 cut = __half22float2(*reinterpret_cast<const __half2*>(&pk[j]));
               pk[j] = pack_f16(__uint_as_float(r[k]) - cut.x, __uint_as_float(r[k + 2]) - cut.y);
             }
-            tmem_st_32x32b_x16(lanes + b * 64 + 32 + half * 16, pk);
+            tmem_st_32x32b_x16(lanes + b * 64 + half * 32 + 16, pk);
           }
           tmem_st_wait();
           const uint32_t* poison = s.v_bad[i & 3][2 * half];
@@ -599,24 +602,26 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
       const size_t rec = (size_t)p.chunk * a.num_kv_heads + p.head + cta;
       float* to = a.partial + rec * WIDE_SLOTS * (D + 2);
       if (busy) {
+        // Column gi 64 + 8 j + perm(g) is dim gi 64 + 8 g + j; the join puts them in order.  16 columns at a time go
+        // through shared memory, so that an instruction stores 64 bytes of 8 slots.
 #pragma unroll 1
-        for (int x = 0; x < D / 64; ++x) {   // 32 columns: four dims of each of a group's octets
-          const int c = half * (D / 2) + x * 32, gi = c >> 6;
-          uint32_t o[32];
-          tmem_ld_32x32b_x32(lanes + TMEM_O + c, o);
+        for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 16) {
+          uint32_t o[16];
+          tmem_ld_32x32b_x16(lanes + TMEM_O + c, o);
           tmem_ld_wait();
-          const bool nan = bad >> gi & 1;
-          float* at = to + (size_t)slot * D + gi * 64 + (c >> 3 & 7);
-          if (used) {
+          const bool nan = bad >> (c >> 6) & 1;
 #pragma unroll
-            for (int g = 0; g < 8; ++g) {   // column 8 j + perm(g) is dim 8 g + j
-              const int perm = (2 * g + (g >> 2)) & 7;
-              float v[4];
+          for (int j = 0; j < 16; j += 4)
+            *reinterpret_cast<uint4*>(&s.stage[warp][lane][j]) = nan ? make_uint4(0x7FC00000u, 0x7FC00000u, 0x7FC00000u, 0x7FC00000u)
+                                                                      : make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+          __syncwarp();
 #pragma unroll
-              for (int j = 0; j < 4; ++j) v[j] = nan ? NAN : __uint_as_float(o[j * 8 + perm]);
-              *reinterpret_cast<float4*>(at + g * 8) = make_float4(v[0], v[1], v[2], v[3]);
-            }
+          for (int j = 0; j < 4; ++j) {
+            const int x = 8 * j + (lane >> 2), sl = (warp & 3) * 32 + x;
+            if (sl < p.count)
+              *reinterpret_cast<uint4*>(to + (size_t)sl * D + c + (lane & 3) * 4) = *reinterpret_cast<const uint4*>(&s.stage[warp][x][(lane & 3) * 4]);
           }
+          __syncwarp();
         }
         if (used && half == 0) *reinterpret_cast<float2*>(to + (size_t)WIDE_SLOTS * D + 2 * slot) = make_float2(ref, l);
       }
@@ -633,6 +638,8 @@ template <int D, int BITS>
 int launch(const QuantAttnArgs& a, cudaStream_t stream) {
   using W = Wide<D, BITS>;
   const auto kernel = wide_kernel<W>;
+  cudaFuncAttributes at;   // the warps' shares of the registers count on what the kernel is launched with
+  if (cudaFuncGetAttributes(&at, kernel) != cudaSuccess || at.numRegs != REGS) return -2;
   cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, W::BYTES);
   zs_launch(kernel, a.grid, THREADS, W::BYTES, stream, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
