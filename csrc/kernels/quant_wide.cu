@@ -6,14 +6,14 @@
 // keys) and O += P V (N = the dims) run on tcgen05 with Q and P in TMEM, so that a tile is turned into f16
 // once for all slots and shared memory is read once for it:
 //  * copy warp: page ids, then one bulk copy per 16-token block into a ring of tiles;
-//  * 8 converter warps, one for K or V of a block: s n + z as one f16 fused multiply-add of two numbers,
+//  * 14 converter warps, one at K or V of a block: s n + z as one f16 fused multiply-add of two numbers,
 //    rounded once (2^-12 of a value).  (w & 0x000F000F) is two subnormals n 2^-24 and the factor s 2^24, so a
 //    pair costs an integer instruction, a part of a shift and the multiply-add.  A power of two per block
 //    brings its largest value to [2^-8, 2^-7), which keeps s 2^24 and every value in f16's range whatever
 //    their size; the scores and the weights take it back.  K goes to a swizzled image of keys x dims, V to one
 //    of dims x keys (as it is stored), both K-major operands;
 //  * MMA warp: S of the next tile goes before O of this one;
-//  * softmax warps: a thread has half of a tile's keys for a slot.  The weights 2^(x - reference) are held
+//  * 16 softmax warps: a thread has a block of a tile for a slot.  The weights 2^(x - reference) are held
 //    below 2^14 times the block's power of two, as f16 (2^-11; for f16 outputs the rest goes through a second
 //    product); the reference follows the largest score only when that outgrew it by 2^3, and O in TMEM is
 //    rescaled then.
@@ -25,28 +25,27 @@ namespace zs {
 namespace qc {
 namespace {
 
-constexpr int SOFT = 256, CONV = 512;               // threads; then the MMA and the copy warp
-constexpr int TEAM = CONV / 64;                     // converter warps of a tile: of K and of V of each block
-// Registers of a thread at launch (65536 / 832 threads, in eights), of the softmax and of the converter warps: 256 x 104 +
-// 512 x 56 + 64 x 72 = 832 x 72.
-constexpr int REGS = 72, SOFT_REGS = 104, CONV_REGS = 56;
+constexpr int SOFT = 512, CONV = 448;               // threads; then the MMA and the copy warp
 constexpr int THREADS = SOFT + CONV + 64;
 constexpr int MMA_WARP = (SOFT + CONV) / 32, COPY_WARP = MMA_WARP + 1;
-constexpr int TBLOCKS = WIDE_KEYS / TOK;
+constexpr int TBLOCKS = WIDE_KEYS / TOK, PARTS = 2 * TBLOCKS;   // blocks of a tile, their K and V
 constexpr uint32_t TMEM_Q = 128, TMEM_O = 256, TMEM_COLS = 512;   // two S of 64 columns, Q as pairs, O
 constexpr int MAX_RAW = 4;
+// Tiles whose units are kept.  A tile's raw blocks are overwritten by the MAX_RAW-th after it at the earliest, whose V is
+// converted once O of the tile two before that is done: no unit is overwritten that a softmax still needs.
+constexpr int UNITS = 2 * MAX_RAW;
 
 struct Smem {
-  uint64_t raw_full[MAX_RAW], raw_empty[MAX_RAW];
-  uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], o_full[2], q_full, unit_full[4];
+  uint64_t raw_full[4], raw_empty[MAX_RAW];
+  uint64_t k_full[2], v_full[2], k_empty[4], v_empty[4], s_full[2], p_full[2], o_full[2], q_full, unit_full[UNITS];
   uint32_t tmem;
   int abort;
-  float k_unit[4][TBLOCKS];          // what the blocks of K of a tile are multiples of
-  float v_log[4][TBLOCKS];           // log2 of the same of V
-  uint32_t v_bad[4][TBLOCKS][2];     // poisoned (token, group) pairs: pair x is bit x / n of word x % n (n words are used)
+  float k_unit[UNITS][TBLOCKS];          // what the blocks of K of a tile are multiples of
+  float v_log[UNITS][TBLOCKS];           // log2 of the same of V
+  uint32_t v_bad[UNITS][TBLOCKS][2];     // poisoned (token, group) pairs: pair x is bit x / n of word x % n (n words are used)
   alignas(16) uint32_t pairs[CONV / 32][TOK * 4];   // of a converter's block: per group and token, scale and offset in f16
-  float top[2][WIDE_SLOTS];
-  alignas(16) float stage[SOFT / 32][32][20];   // 16 columns of a warp's 32 slots, on their way to the record
+  float top[TBLOCKS][WIDE_SLOTS];
+  uint4 stage[SOFT / 32][32][2];     // 8 columns of a warp's 32 slots, on their way to the record
 };
 
 template <int D_, int BITS_>
@@ -79,13 +78,13 @@ __device__ __forceinline__ bool wait_for(Smem& s, uint64_t* bar, uint32_t phase,
   *reinterpret_cast<volatile int*>(&s.abort) = 1;
   return false;
 }
-__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
 __device__ __forceinline__ bool soft_any(bool x) {
   int r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %1, 0;\n\t"
-      "bar.red.or.pred q, 1, 256, p;\n\t"
+      "bar.red.or.pred q, 1, 512, p;\n\t"
       "selp.b32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
       : "r"((int)x)
@@ -106,22 +105,15 @@ __device__ __forceinline__ uint32_t sixteenth(uint32_t a) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(0x2C002C00u));
   return d;
 }
-template <int N>
-__device__ __forceinline__ void lds(uint32_t (&r)[N], const uint8_t* p) {
-  if constexpr (N == 2) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
-    r[0] = u.x;
-    r[1] = u.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) {
-      const uint4 u = reinterpret_cast<const uint4*>(p)[i];
-      r[4 * i] = u.x;
-      r[4 * i + 1] = u.y;
-      r[4 * i + 2] = u.z;
-      r[4 * i + 3] = u.w;
-    }
-  }
+__device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+               "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld_x8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
 }
 __device__ __forceinline__ uint4 lds128(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 
@@ -162,21 +154,21 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
     tmem_relinquish();
   }
   if (tid == 0) {
-    for (int i = 0; i < RING; ++i) {
-      mbar_init(&s.raw_full[i], 1);
-      mbar_init(&s.raw_empty[i], TEAM);
-    }
+    for (int i = 0; i < RING; ++i) mbar_init(&s.raw_empty[i], PARTS);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.k_full[i], TBLOCKS);
       mbar_init(&s.v_full[i], TBLOCKS);
-      mbar_init(&s.k_empty[i], 1);
-      mbar_init(&s.v_empty[i], 1);
       mbar_init(&s.s_full[i], 1);
       mbar_init(&s.p_full[i], SOFT);
       mbar_init(&s.o_full[i], 1);
     }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&s.raw_full[i], 1);
+      mbar_init(&s.k_empty[i], 1);
+      mbar_init(&s.v_empty[i], 1);
+    }
     mbar_init(&s.q_full, SOFT);
-    for (int i = 0; i < 4; ++i) mbar_init(&s.unit_full[i], TBLOCKS);
+    for (int i = 0; i < UNITS; ++i) mbar_init(&s.unit_full[i], TBLOCKS);
     s.abort = 0;
     fence_barrier_init();
   }
@@ -237,11 +229,11 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
         }
         ok = __all_sync(0xffffffff, wait_for(s, &s.raw_empty[st], phase, a.err));
         if (!ok) break;
-        if (lane == 0) mbar_expect_tx(&s.raw_full[st], count * BLOCK);
+        if (lane == 0) mbar_expect_tx(&s.raw_full[i & 3], count * BLOCK);
         __syncwarp();
         if (lane < count)
           bulk_load(ring + st * W::RAW + lane * BLOCK,
-                    a.data + ((((size_t)page * a.num_kv_heads + p.head) << bshift) + (blk & ((1 << bshift) - 1))) * BLOCK, BLOCK, &s.raw_full[st]);
+                    a.data + ((((size_t)page * a.num_kv_heads + p.head) << bshift) + (blk & ((1 << bshift) - 1))) * BLOCK, BLOCK, &s.raw_full[i & 3]);
         page = after;
         if (++st == RING) {
           st = 0;
@@ -251,7 +243,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
     }
     // Copies in flight land before the CTA gives its shared memory back.
     if (lane == 0)
-      for (int m = max(0, i - RING); m < i; ++m) mbar_wait(&s.raw_full[m % RING], (m / RING) & 1, nullptr);
+      for (int m = max(0, i - RING); m < i; ++m) mbar_wait(&s.raw_full[m & 3], (m >> 2) & 1, nullptr);
   } else if (warp == MMA_WARP) {
     // -------------------------------------------------------------------- MMA
     const bool leader = elect_one();
@@ -268,7 +260,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
 #pragma unroll
         for (int x = 0; x < D / 16; ++x)
           mma_step(tmem + b * 64, tmem + TMEM_Q + x * 8, k_lo + (b * W::K_IMAGE + (x >> 2) * WIDE_KEYS * 128) / 16 + (x & 3) * 2, idesc_s, x > 0);
-        tc_commit(&s.k_empty[b]);
+        tc_commit(&s.k_empty[i & 3]);
         tc_commit(&s.s_full[b]);
       }
       ++ns;
@@ -282,13 +274,13 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
       if (leader) {
 #pragma unroll
         for (int k = 0; k < WIDE_KEYS / 16; ++k)
-          mma_step(tmem + TMEM_O, tmem + b * 64 + (k >> 1) * 32 + (k & 1) * 8, v_lo + b * W::V_IMAGE / 16 + k * 2, idesc_o, !fresh || k > 0);
+          mma_step(tmem + TMEM_O, tmem + b * 64 + k * 16, v_lo + b * W::V_IMAGE / 16 + k * 2, idesc_o, !fresh || k > 0);
         if (a.half) {
 #pragma unroll
           for (int k = 0; k < WIDE_KEYS / 16; ++k)   // what the rounding of P left
-            mma_step(tmem + TMEM_O, tmem + b * 64 + (k >> 1) * 32 + 16 + (k & 1) * 8, v_lo + b * W::V_IMAGE / 16 + k * 2, idesc_o, true);
+            mma_step(tmem + TMEM_O, tmem + b * 64 + k * 16 + 8, v_lo + b * W::V_IMAGE / 16 + k * 2, idesc_o, true);
         }
-        tc_commit(&s.v_empty[b]);
+        tc_commit(&s.v_empty[i & 3]);
         tc_commit(&s.o_full[b]);
       }
       ++no;
@@ -310,20 +302,19 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
     __syncwarp();
   } else if (warp >= SOFT / 32) {
     // -------------------------------------------------------------- converters
-    // Two teams of eight warps take turns, so that a tile has the time of two; a team's image is its own.
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CONV_REGS));
-    const int w = warp - SOFT / 32, b = w / TEAM, kb = w & (TBLOCKS - 1), g = lane >> 2, t4 = lane & 3;
-    const bool is_v = w % TEAM >= TBLOCKS;
+    // The warps take the parts of the tiles (K, then V of each block) in turn.
+    const int w = warp - SOFT / 32, g = lane >> 2, t4 = lane & 3;
     constexpr float TOP = (1 << BITS) - 1;
     constexpr int PAIRS = (TOK * NG + 31) / 32;
-    int i = 0;
+    int at = w, before = 0;   // the next part, counted over the CTA's tiles; tiles of the pieces before
     bool ok = true;
     while (ok && next_piece(p)) {
-      for (int t = 0; ok && t < p.n; ++t, ++i) {
-        if ((i & 1) != b) continue;
-        const int st = i % RING, left = p.len - (p.first + t) * WIDE_KEYS - kb * TOK;   // keys of the block from here on
+      for (; ok && at / PARTS < before + p.n; at += CONV / 32) {
+        const int i = at / PARTS, b = i & 1, kb = at & (TBLOCKS - 1);
+        const bool is_v = at & TBLOCKS;
+        const int st = i % RING, left = p.len - (p.first + i - before) * WIDE_KEYS - kb * TOK;   // keys of the block from here on
         const uint8_t* in = ring + st * W::RAW + kb * BLOCK;
-        ok = __all_sync(0xffffffff, wait_for(s, &s.raw_full[st], (i / RING) & 1, a.err));
+        ok = __all_sync(0xffffffff, wait_for(s, &s.raw_full[i & 3], (i >> 2) & 1, a.err));
         if (!ok) break;
         // The block's unit from its scales and offsets (a lane has one or two of the 16 NG pairs), and those as multiples
         // of it: s 2^24 and z.  What is behind the sequence does not count, and is 0 in V, as poisoned groups are.
@@ -354,17 +345,20 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
           }
           if (lane == 0) {
             if (is_v) {
-              s.v_log[i & 3][kb] = (float)e;
-              s.v_bad[i & 3][kb][0] = bad[0];
-              s.v_bad[i & 3][kb][1] = PAIRS > 1 ? bad[PAIRS - 1] : 0;
+              s.v_log[i % UNITS][kb] = (float)e;
+              s.v_bad[i % UNITS][kb][0] = bad[0];
+              s.v_bad[i % UNITS][kb][1] = PAIRS > 1 ? bad[PAIRS - 1] : 0;
             } else {
-              s.k_unit[i & 3][kb] = __uint_as_float((uint32_t)min(e + 127, 254) << 23);
+              s.k_unit[i % UNITS][kb] = __uint_as_float((uint32_t)min(e + 127, 254) << 23);
             }
           }
           __syncwarp();
-          if (is_v && lane == 0) mbar_arrive(&s.unit_full[i & 3]);   // the softmax need not wait for the image
+          if (is_v && lane == 0) mbar_arrive(&s.unit_full[i % UNITS]);   // the softmax need not wait for the image
         }
-        if (i >= 2) ok = __all_sync(0xffffffff, wait_for(s, is_v ? &s.v_empty[b] : &s.k_empty[b], ((i >> 1) - 1) & 1, a.err));
+        // The image is free once the product of the tile two before has read it.  The warps are not in step: one may be
+        // here before the product of the tile four before is done, but not that of six before, whose blocks have left the
+        // ring.  A barrier for each of four tiles, here and for the blocks, then has one phase that can be meant.
+        if (i >= 2) ok = __all_sync(0xffffffff, wait_for(s, is_v ? &s.v_empty[(i - 2) & 3] : &s.k_empty[(i - 2) & 3], ((i - 2) >> 2) & 1, a.err));
         if (!ok) break;
         if (!is_v) {
           const int r0 = kb * 16 + 2 * g;
@@ -428,31 +422,37 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
           mbar_arrive(is_v ? &s.v_full[b] : &s.k_full[b]);
         }
       }
+      before += p.n;
     }
   } else {
     // ---------------------------------------------------------------- softmax
     // After a wait that gave up these warps go on to their last piece's end (every later wait gives up at
     // once), so that their barriers meet.
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFT_REGS));
-    const int half = warp >> 2, slot = (warp & 3) * 32 + lane;
+    const int part = warp >> 2, slot = (warp & 3) * 32 + lane;   // the block of a tile, and the quarter of O's columns
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const auto row_of = [&](const Piece& x) { return x.row + (x.slot0 + min(slot, x.count - 1)) / group; };
+    const auto query_of = [&](const Piece& x) {
+      const int id = x.slot0 + min(slot, x.count - 1);
+      return reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + (size_t)(x.row + id / group) * a.q_row +
+                                            (size_t)(x.head * group + id % group) * a.q_head + part * (D / 4));
+    };
     int i = 0;
-    while (next_piece(p)) {
+    bool more = next_piece(p);
+    int limit = more ? plan.lens[row_of(p)] : 0;
+    while (more) {
       const bool used = slot < p.count, busy = (warp & 3) * 32 < p.count;
-      const int id = p.slot0 + min(slot, p.count - 1), row = p.row + id / group;
-      const int limit = used ? plan.lens[row] : 0;
+      if (!used) limit = 0;
       float fac;
       {
-        // The slot's half of the query, brought to [2^13, 2^14) by a power of two, as pairs in the order in which
+        // The slot's quarter of the query, brought to [2^13, 2^14) by a power of two, as pairs in the order in which
         // the converters leave K's dims: 0 4 1 5 2 6 3 7, or 0 2 1 3 4 6 5 7.
-        const uint4* from = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + (size_t)row * a.q_row +
-                                                           (size_t)(p.head * group + id % group) * a.q_head + half * (D / 2));
-        uint4 u[D / 16];
+        const uint4* from = query_of(p);
+        uint4 u[D / 32];
 #pragma unroll
-        for (int j = 0; j < D / 16; ++j) u[j] = busy ? from[j] : make_uint4(0, 0, 0, 0);
+        for (int j = 0; j < D / 32; ++j) u[j] = busy ? from[j] : make_uint4(0, 0, 0, 0);
         float big = 0.f, nan = 0.f;
 #pragma unroll
-        for (int j = 0; j < D / 16; ++j) {
+        for (int j = 0; j < D / 32; ++j) {
           const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -461,20 +461,20 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
             nan = fmaf(f.x, 0.f, fmaf(f.y, 0.f, nan));
           }
         }
-        s.top[half][slot] = nan == 0.f ? big : INFINITY;
+        s.top[part][slot] = nan == 0.f ? big : INFINITY;
         soft_sync();
-        big = fmaxf(s.top[0][slot], s.top[1][slot]);
+        big = fmaxf(fmaxf(s.top[0][slot], s.top[1][slot]), fmaxf(s.top[2][slot], s.top[3][slot]));
         soft_sync();
         const int e = 13 - min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 100);
         const float up = big < INFINITY ? copysignf(__uint_as_float((uint32_t)(e + 127) << 23), a.sm_scale) : NAN;
         fac = fabsf(a.sm_scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - e) << 23);
         if (busy) {
 #pragma unroll
-          for (int c = 0; c < D / 4; c += 16) {
-            uint32_t y[16];
+          for (int c = 0; c < D / 32; c += 2) {
+            uint32_t y[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint32_t w[4] = {u[c / 4 + j].x, u[c / 4 + j].y, u[c / 4 + j].z, u[c / 4 + j].w};
+            for (int j = 0; j < 2; ++j) {
+              const uint32_t w[4] = {u[c + j].x, u[c + j].y, u[c + j].z, u[c + j].w};
               float x[8];
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
@@ -486,102 +486,108 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
               for (int k = 0; k < 4; ++k)
                 y[4 * j + k] = BITS == 4 ? pack_f16(x[k], x[k + 4]) : pack_f16(x[(k >> 1) * 4 + (k & 1)], x[(k >> 1) * 4 + (k & 1) + 2]);
             }
-            tmem_st_32x32b_x16(lanes + TMEM_Q + half * (D / 4) + c, y);
+            tmem_st_x8(lanes + TMEM_Q + part * (D / 8) + c * 4, y);
           }
           tmem_st_wait();
         }
         tc_fence_before();
         mbar_arrive(&s.q_full);
       }
+      // The next piece is looked up, and its queries are brought into L2, while this one's tiles are on their way.
+      Piece next;
+      more = next_piece(next);
+      int next_limit = 0;
+      if (more) {
+        next_limit = plan.lens[row_of(next)];
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(query_of(next)));
+      }
       float ref = -INFINITY, l = 0.f;
       uint32_t bad = 0;
       for (int t = 0; t < p.n; ++t, ++i) {
-        const int b = i & 1, valid = limit - (p.first + t) * WIDE_KEYS - half * 32;
+        const int b = i & 1, valid = limit - (p.first + t) * WIDE_KEYS - part * TOK;
+        wait_for(s, &s.unit_full[i % UNITS], (i / UNITS) & 1, a.err);
+        const float v = s.v_log[i % UNITS][part];
         wait_for(s, &s.s_full[b], (i >> 1) & 1, a.err);
-        wait_for(s, &s.unit_full[i & 3], (i >> 2) & 1, a.err);
         tc_fence_after();
-        uint32_t r[32];
+        const float f = fmaxf(fac * s.k_unit[i % UNITS][part], 0x1p-126f);
+        uint32_t r[16];
         float most = -INFINITY;
-        const float v0 = s.v_log[i & 3][2 * half], v1 = s.v_log[i & 3][2 * half + 1];
-        const float f0 = fmaxf(fac * s.k_unit[i & 3][2 * half], 0x1p-126f), f1 = fmaxf(fac * s.k_unit[i & 3][2 * half + 1], 0x1p-126f);
         if (busy) {
-          tmem_ld_32x32b_x32(lanes + b * 64 + half * 32, r);
+          tmem_ld_32x32b_x16(lanes + b * 64 + part * 16, r);
           tmem_ld_wait();
-          if (__any_sync(0xffffffff, valid < 32)) {
+          if (__any_sync(0xffffffff, valid < 16)) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
+            for (int j = 0; j < 16; ++j)
               if (j >= valid) r[j] = 0xFF800000u;
           }
-          float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float x[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-          for (int j = 0; j < 32; ++j) x[(j >> 4) * 2 + (j & 1)] = fmaxf(x[(j >> 4) * 2 + (j & 1)], __uint_as_float(r[j]));
-          most = fmaxf(fmaf(fmaxf(x[0], x[1]), f0, v0), fmaf(fmaxf(x[2], x[3]), f1, v1));
+          for (int j = 0; j < 16; ++j) x[j & 1] = fmaxf(x[j & 1], __uint_as_float(r[j]));
+          most = fmaf(fmaxf(x[0], x[1]), f, v);
         }
-        tc_fence_before();
         // Does a slot's reference have to move?
         if (soft_any(used && most > ref + SLACK)) {
-          s.top[half][slot] = most;
+          s.top[part][slot] = most;
           soft_sync();
-          most = fmaxf(most, s.top[half ^ 1][slot]);
+          most = fmaxf(fmaxf(s.top[0][slot], s.top[1][slot]), fmaxf(s.top[2][slot], s.top[3][slot]));
           const bool grow = used && most > ref + SLACK;
-          const float f = grow ? ex2(ref - most) : 1.f;
+          const float shrink = grow ? ex2(ref - most) : 1.f;
           if (grow) {
-            l *= f;
+            l *= shrink;
             ref = most;
           }
           if (t > 0 && __any_sync(0xffffffff, grow)) {
             wait_for(s, &s.o_full[b ^ 1], ((i - 1) >> 1) & 1, a.err);   // O holds every tile before this one
             tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < D / 2; c += 16) {
-              uint32_t o[16];
-              const uint32_t at = lanes + TMEM_O + half * (D / 2) + c;
-              tmem_ld_32x32b_x16(at, o);
+            for (int c = 0; c < D / 4; c += 8) {
+              uint32_t o[8];
+              const uint32_t at = lanes + TMEM_O + part * (D / 4) + c;
+              tmem_ld_x8(at, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-              tmem_st_32x32b_x16(at, o);
+              for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * shrink);
+              tmem_st_x8(at, o);
             }
             tmem_st_wait();
           }
           soft_sync();   // the maxima have been read
         }
-        tc_fence_after();
         if (busy) {
-          const float off = ref == -INFINITY ? 0.f : LIFT - ref, o0 = off + v0, o1 = off + v1;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float w = ex2(fmaf(__uint_as_float(r[j]), j < 16 ? f0 : f1, j < 16 ? o0 : o1));
-            r[j] = __float_as_uint(w);
-            sum[(j >> 4) * 2 + (j & 1)] += w;
-          }
-          l += (sum[0] + sum[1]) * ex2(-v0) + (sum[2] + sum[3]) * ex2(-v1);
-          // Tokens of a four lie in the order 0 2 1 3 in V's image.
-          uint32_t pk[16];
+          const float off = (ref == -INFINITY ? 0.f : LIFT - ref) + v;
+          float sum[2] = {0.f, 0.f};
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
+            const float w = ex2(fmaf(__uint_as_float(r[j]), f, off));
+            r[j] = __float_as_uint(w);
+            sum[j & 1] += w;
+          }
+          l += (sum[0] + sum[1]) * ex2(-v);
+          // Tokens of a four lie in the order 0 2 1 3 in V's image; the weights take the place of their own scores.
+          uint32_t pk[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
             const int k = (j >> 1) * 4 + (j & 1);
             pk[j] = pack_f16(__uint_as_float(r[k]), __uint_as_float(r[k + 2]));
           }
-          tmem_st_32x32b_x16(lanes + b * 64 + half * 32, pk);   // in the place of its own scores
+          tmem_st_x8(lanes + b * 64 + part * 16, pk);
           if (a.half) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
+            for (int j = 0; j < 8; ++j) {
               const int k = (j >> 1) * 4 + (j & 1);
               const float2 cut = __half22float2(*reinterpret_cast<const __half2*>(&pk[j]));
               pk[j] = pack_f16(__uint_as_float(r[k]) - cut.x, __uint_as_float(r[k + 2]) - cut.y);
             }
-            tmem_st_32x32b_x16(lanes + b * 64 + half * 32 + 16, pk);
+            tmem_st_x8(lanes + b * 64 + part * 16 + 8, pk);
           }
           tmem_st_wait();
-          const uint32_t* poison = s.v_bad[i & 3][2 * half];
-          if (poison[0] | poison[1] | poison[2] | poison[3]) {
+          const uint32_t* poison = s.v_bad[i % UNITS][part];
+          if (poison[0] | poison[1]) {
             constexpr int PAIRS = (TOK * NG + 31) / 32;
-            for (int j = 0; j < min(valid, 32); ++j)
+            for (int j = 0; j < min(valid, TOK); ++j)
               for (int gi = 0; gi < NG; ++gi) {
-                const int x = (j & 15) * NG + gi;
-                bad |= (poison[(j >> 4) * 2 + x % PAIRS] >> (x / PAIRS) & 1) << gi;
+                const int x = j * NG + gi;
+                bad |= (poison[x % PAIRS] >> (x / PAIRS) & 1) << gi;
               }
           }
         }
@@ -589,43 +595,45 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
         mbar_arrive(&s.p_full[b]);
       }
       // ---- the slots' records
+      s.top[part][slot] = l;
+      soft_sync();
+      l = (s.top[0][slot] + s.top[1][slot]) + (s.top[2][slot] + s.top[3][slot]);
+      soft_sync();
+      s.top[part][slot] = __uint_as_float(bad);
+      soft_sync();
+      bad = (__float_as_uint(s.top[0][slot]) | __float_as_uint(s.top[1][slot])) | (__float_as_uint(s.top[2][slot]) | __float_as_uint(s.top[3][slot]));
       wait_for(s, &s.o_full[(i - 1) & 1], ((i - 1) >> 1) & 1, a.err);
       tc_fence_after();
-      s.top[half][slot] = l;
-      soft_sync();
-      l += s.top[half ^ 1][slot];
-      soft_sync();
-      s.top[half][slot] = __uint_as_float(bad);
-      soft_sync();
-      bad |= __float_as_uint(s.top[half ^ 1][slot]);
-      soft_sync();
       const size_t rec = (size_t)p.chunk * a.num_kv_heads + p.head + cta;
       float* to = a.partial + rec * WIDE_SLOTS * (D + 2);
       if (busy) {
-        // Column gi 64 + 8 j + perm(g) is dim gi 64 + 8 g + j; the join puts them in order.  16 columns at a time go
-        // through shared memory, so that an instruction stores 64 bytes of 8 slots.
+        // Column gi 64 + 8 j + perm(g) is dim gi 64 + 8 g + j; the join puts them in order.  8 columns at a time go
+        // through shared memory, so that an instruction stores whole sectors.
+        float* mine = to + (size_t)((warp & 3) * 32 + (lane >> 1)) * D + part * (D / 4) + (lane & 1) * 4;
+        const int left = p.count - (warp & 3) * 32 - (lane >> 1);
 #pragma unroll 1
-        for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 16) {
-          uint32_t o[16];
-          tmem_ld_32x32b_x16(lanes + TMEM_O + c, o);
+        for (int c = 0; c < D / 4; c += 8) {
+          uint32_t o[8];
+          tmem_ld_x8(lanes + TMEM_O + part * (D / 4) + c, o);
           tmem_ld_wait();
-          const bool nan = bad >> (c >> 6) & 1;
-#pragma unroll
-          for (int j = 0; j < 16; j += 4)
-            *reinterpret_cast<uint4*>(&s.stage[warp][lane][j]) = nan ? make_uint4(0x7FC00000u, 0x7FC00000u, 0x7FC00000u, 0x7FC00000u)
-                                                                      : make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+          const bool nan = bad >> ((part * (D / 4) + c) >> 6) & 1;
+          uint4* st = s.stage[warp][lane];   // its halves change places in every second four of slots
+          const int turn = lane >> 2 & 1;
+          st[turn] = nan ? make_uint4(0x7FC00000u, 0x7FC00000u, 0x7FC00000u, 0x7FC00000u) : make_uint4(o[0], o[1], o[2], o[3]);
+          st[turn ^ 1] = nan ? make_uint4(0x7FC00000u, 0x7FC00000u, 0x7FC00000u, 0x7FC00000u) : make_uint4(o[4], o[5], o[6], o[7]);
           __syncwarp();
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int x = 8 * j + (lane >> 2), sl = (warp & 3) * 32 + x;
-            if (sl < p.count)
-              *reinterpret_cast<uint4*>(to + (size_t)sl * D + c + (lane & 3) * 4) = *reinterpret_cast<const uint4*>(&s.stage[warp][x][(lane & 3) * 4]);
-          }
+          const uint4 x0 = s.stage[warp][lane >> 1][(lane ^ lane >> 3) & 1];
+          const uint4 x1 = s.stage[warp][16 + (lane >> 1)][(lane ^ lane >> 3) & 1];
+          if (left > 0) *reinterpret_cast<uint4*>(mine + c) = x0;
+          if (left > 16) *reinterpret_cast<uint4*>(mine + 16 * D + c) = x1;
           __syncwarp();
         }
-        if (used && half == 0) *reinterpret_cast<float2*>(to + (size_t)WIDE_SLOTS * D + 2 * slot) = make_float2(ref, l);
+        if (used && part == 0) *reinterpret_cast<float2*>(to + (size_t)WIDE_SLOTS * D + 2 * slot) = make_float2(ref, l);
       }
+      soft_sync();   // the poisoned groups have been read
       tc_fence_before();
+      p = next;
+      limit = next_limit;
     }
   }
   tc_fence_before();
@@ -638,8 +646,6 @@ template <int D, int BITS>
 int launch(const QuantAttnArgs& a, cudaStream_t stream) {
   using W = Wide<D, BITS>;
   const auto kernel = wide_kernel<W>;
-  cudaFuncAttributes at;   // the warps' shares of the registers count on what the kernel is launched with
-  if (cudaFuncGetAttributes(&at, kernel) != cudaSuccess || at.numRegs != REGS) return -2;
   cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, W::BYTES);
   zs_launch(kernel, a.grid, THREADS, W::BYTES, stream, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;

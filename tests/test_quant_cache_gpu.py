@@ -425,6 +425,26 @@ def test_long_sequence_is_split_and_repeats_exactly():
         assert torch.equal(check_attention(cache, table, 2, [0], [n - 3], seed=3), first)
 
 
+@pytest.mark.parametrize("dim,bits,dtype", [(64, 4, torch.bfloat16), (128, 8, torch.float16), (256, 4, torch.bfloat16), (256, 8, torch.bfloat16)])
+def test_long_sequences_of_many_rows(dim, bits, dtype):
+    """Five rows of eight heads over sequences long enough that every SM has dozens of tiles and several sequences."""
+    lens, hkv, per = [30000, 24001, 17000], 4, 5
+    cache, table = filled(lens, hkv, dim, bits, page=64, dtype=dtype, seed=dim)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    q = torch.randn(len(lens) * per, 8 * hkv, dim, generator=g, device=DEV).to(dtype)
+    slots = [s for s in range(3) for _ in range(per)]
+    seen = [n - per + 1 + i for n in lens for i in range(per)]
+    plan = QuantAttention(cache, 8 * hkv, max_rows=15, max_seqs=3, max_seq_rows=per)
+    plan.update(_i32(slots), _i32(seen), _i32([0, 5, 10, 15]))
+    got = plan.attend(0, q, table, dim ** -0.5)
+    plan.check()
+    rows = [0, 7, 14]
+    want, tol = reference(cache, table, q[rows], [slots[r] for r in rows], [seen[r] for r in rows], dim ** -0.5)
+    assert np.all(np.abs(got[rows].double().cpu().numpy() - want) <= tol)
+    for _ in range(3):
+        assert torch.equal(plan.attend(0, q, table, dim ** -0.5), got)
+
+
 def test_many_short_sequences():
     rng = np.random.default_rng(3)
     lens = rng.integers(0, 60, 700).tolist()
