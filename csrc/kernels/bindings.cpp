@@ -1222,8 +1222,8 @@ struct QuantPlanState {
     const int64_t group = q_heads / c.heads;
     TORCH_CHECK_VALUE(max_rows * q_heads < (1ll << 28) && max_seqs < (1ll << 24), "too many rows or sequences for a plan");
     QuantAttnArgs& a = base;
-    zs_quant_attn_shape(c.dim, c.bits, (int)std::min<int64_t>(group * max_seq_rows, 1 << 20), &a.tiles, &a.slot_warps, &a.stage);
-    a.chunk = 8 * a.tiles * a.slot_warps;
+    zs_quant_attn_shape(c.dim, c.bits, (int)std::min<int64_t>(group * max_seq_rows, 1 << 20), &a.tiles, &a.stage);
+    a.chunk = 8 * a.tiles;
     const int64_t of_seq = (group * std::min(max_seq_rows, max_rows) + a.chunk - 1) / a.chunk;
     a.max_chunks = (int)std::min(max_seqs + max_rows * group / a.chunk, max_seqs * of_seq);
     a.num_q_heads = (int)q_heads;

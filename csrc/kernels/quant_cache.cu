@@ -430,13 +430,15 @@ struct Shape {
   static constexpr int BLOCK = block_bytes(D, BITS);
   static constexpr int KEYS = KB * TOK;             // of a stage
   static constexpr int STAGE_BYTES = KB * BLOCK;
-  static constexpr int MERGE_REGS = KS * NT * 4 + NG * NT * 2 + 4 * NT;   // O, its offset part, l and reference
-  static constexpr int MERGE = WARPS / 2 * MERGE_REGS * 128;
-  static constexpr int HEAD = 2 * WARPS * MAX_RING * 8;
-  __host__ __device__ static constexpr int slots(int sw) { return 8 * NT * sw; }
-  __host__ __device__ static constexpr int fixed(int sw) {
-    return HEAD + slots(sw) * (NG + 2) * 4 + KS * NT * sw * 256 + (sw < WARPS ? MERGE : 0);
-  }
+  static constexpr int SLOTS = 8 * NT;
+  // Queries: a lane has 8 dims of a slot, so a warp has 1, 2 or 4 slots at a time.
+  static constexpr int Q_LANES = D / 8, Q_EACH = 32 / Q_LANES, Q_PASSES = (SLOTS + WARPS * Q_EACH - 1) / (WARPS * Q_EACH);
+  // The join of the warps, a tile of 8 slots at a time: its items are (group, column), of 8 sums of V and one of the offsets
+  // a lane, and every warp but an item's owner leaves its own.
+  static constexpr int ITEMS = 2 * NG, ITEM = 9;
+  static constexpr int JOIN = ITEMS * (WARPS - 1) * ITEM * 128;
+  static constexpr int BARS = WARPS * MAX_RING * 8;
+  static constexpr int FIXED = BARS + SLOTS * (NG + 2) * 4 + KS * NT * 256 + 2 * WARPS * SLOTS * 4 + JOIN;
 };
 
 struct Piece {
@@ -456,8 +458,8 @@ struct State {
 // One stage: the scores of its keys, their weights, and what they add to the sums.  With MASK a key at or
 // behind a slot's length is left out whatever the cache holds there.
 template <class S, bool MASK>
-__device__ __forceinline__ void stage_step(State<S>& st, const uint8_t* in, const uint8_t* qf, int q_step, const float* qsum,
-                                           int slots, int key0, int g, int t) {
+__device__ __forceinline__ void stage_step(State<S>& st, const uint8_t* in, const uint8_t* qf, const float* qsum, int key0, int g,
+                                           int t) {
   constexpr int NT = S::NT, NG = S::NG, KS = S::KS, KB = S::KB, BITS = S::BITS;
   float sc[KB][NT][4];
   uint32_t sz[KB][2 * NG];   // of tokens 2g and 2g + 1, which are rows g and g + 8 of a fragment
@@ -486,7 +488,7 @@ __device__ __forceinline__ void stage_step(State<S>& st, const uint8_t* in, cons
       for (int gi = 0; gi < GB; ++gi) {
         uint32_t bq[NT][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) lds(bq[n], qf + ((g0 + gi) * 4 + k) * q_step + n * 256);
+        for (int n = 0; n < NT; ++n) lds(bq[n], qf + (((g0 + gi) * 4 + k) * NT + n) * 256);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
           uint32_t a0, a1, a2, a3;   // rows g and g + 8
@@ -514,7 +516,7 @@ __device__ __forceinline__ void stage_step(State<S>& st, const uint8_t* in, cons
     for (int gi = 0; gi < GB; ++gi)
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const float2 qs = *reinterpret_cast<const float2*>(qsum + (g0 + gi) * slots + n * 8 + 2 * t);
+        const float2 qs = *reinterpret_cast<const float2*>(qsum + (g0 + gi) * S::SLOTS + n * 8 + 2 * t);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -673,72 +675,66 @@ __device__ __forceinline__ void stage_step(State<S>& st, const uint8_t* in, cons
 
 template <class S>
 __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const QuantAttnArgs a) {
-  constexpr int KS = S::KS, NG = S::NG, NT = S::NT, D = S::D, BITS = S::BITS, BLOCK = S::BLOCK, WARPS = S::WARPS, KB = S::KB;
+  constexpr int KS = S::KS, NG = S::NG, NT = S::NT, D = S::D, BITS = S::BITS, BLOCK = S::BLOCK, WARPS = S::WARPS, KB = S::KB, SLOTS = S::SLOTS;
   extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ Piece pieces[2];
   pdl_wait();
   pdl_trigger();
   const Plan plan = plan_of(a);
   const long long total = *plan.total;
-  const int first_chunk = plan.start[blockIdx.x];
-  const int sw_n = a.slot_warps, kw = WARPS / sw_n, ring = a.ring;
-  const int B = ctas_of(total, gridDim.x, a.least);
-  const int b = blockIdx.x;
+  int chunk = plan.start[blockIdx.x];   // of the CTA's first stage
+  const int ring = a.ring, B = ctas_of(total, gridDim.x, a.least), b = blockIdx.x;
   if (b >= B || total == 0) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kl = warp / sw_n, sw = warp % sw_n;   // key lane, slot part
-  const int g = lane >> 2, t = lane & 3;
-  const int slots = S::slots(sw_n);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int group = a.num_q_heads / a.num_kv_heads;
 
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem) + kl * ring;
-  uint64_t* empty = reinterpret_cast<uint64_t*>(smem) + WARPS * MAX_RING + kl * ring;
-  float* qsum = reinterpret_cast<float*>(smem + S::HEAD);         // [NG][slots]
-  float* qfac = qsum + NG * slots;                                // [slots]
-  int* qlen = reinterpret_cast<int*>(qfac + slots);               // [slots]
-  uint8_t* qfrag = reinterpret_cast<uint8_t*>(qlen + slots);      // [KS][NT sw][32 lanes][8 bytes]
-  float* merge = reinterpret_cast<float*>(qfrag + KS * NT * sw_n * 256);
-  uint8_t* stage0 = smem + a.ring_offset + (size_t)kl * ring * S::STAGE_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem) + warp * MAX_RING;
+  float* qsum = reinterpret_cast<float*>(smem + S::BARS);         // [NG][SLOTS]
+  float* qfac = qsum + NG * SLOTS;                                // [SLOTS]
+  int* qlen = reinterpret_cast<int*>(qfac + SLOTS);               // [SLOTS]
+  uint8_t* qfrag = reinterpret_cast<uint8_t*>(qlen + SLOTS);      // [KS][NT][32 lanes][8 bytes]
+  float* refs = reinterpret_cast<float*>(qfrag + KS * NT * 256);  // [WARPS][SLOTS] reference, then l
+  float* sums = refs + 2 * WARPS * SLOTS;                         // [ITEMS][WARPS - 1][ITEM][32]
+  uint8_t* stage0 = smem + a.ring_offset + warp * ring * S::STAGE_BYTES;
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kw; ++i)
-      for (int j = 0; j < ring; ++j) {
-        mbar_init(reinterpret_cast<uint64_t*>(smem) + i * ring + j, 1);
-        mbar_init(reinterpret_cast<uint64_t*>(smem) + WARPS * MAX_RING + i * ring + j, sw_n);
-      }
+  // The CTA's stages go piece by piece; the walker is the one thread that looks the next one up (n = 0: none).
+  const long long hi = total * (b + 1) / B;
+  long long pos = total * b / B;
+  const bool walker = threadIdx.x == 32;
+  auto walk = [&](Piece* p) {
+    Piece x = {};
+    if (pos < hi) {
+      Chunk e = plan.table[chunk];
+      while (e.before + (long long)e.stages * a.num_kv_heads <= pos) e = plan.table[++chunk];
+      const int r = (int)(pos - e.before);
+      x.chunk = chunk;
+      x.head = r / e.stages;
+      x.first = r % e.stages;
+      x.n = (int)min((long long)(e.stages - x.first), hi - pos);
+      x.row = e.row;
+      x.slot = e.slot;
+      x.slot0 = e.first;
+      x.count = e.count;
+      x.len = e.len;
+      pos += x.n;
+    }
+    *p = x;
+  };
+  if (walker) walk(&pieces[0]);
+  if (lane == 0) {
+    for (int j = 0; j < ring; ++j) mbar_init(&full[j], 1);
     fence_barrier_init();
   }
-
-  // This CTA's stages, and the chunk that the first is in.
-  const long long lo = total * b / B, hi = total * (b + 1) / B;
-  int c = first_chunk;
   __syncthreads();
 
-  auto piece_at = [&](long long pos) {   // c: a chunk at or before pos
-    Chunk e = plan.table[c];
-    while (e.before + (long long)e.stages * a.num_kv_heads <= pos) e = plan.table[++c];
-    const int r = (int)(pos - e.before);
-    Piece p;
-    p.chunk = c;
-    p.head = r / e.stages;
-    p.first = r % e.stages;
-    p.n = (int)min((long long)(e.stages - p.first), hi - pos);
-    p.row = e.row;
-    p.slot = e.slot;
-    p.slot0 = e.first;
-    p.count = e.count;
-    p.len = e.len;
-    return p;
-  };
-
-  // The producer of a key lane is its first warp.  Lane j of it holds where block j % KB of stage j / KB is.
+  // Each warp loads for itself.  Lane j holds where block j % KB of stage j / KB is.
   constexpr int AHEAD = 32 / KB;
-  int at_block = 0, at_next = 0, issued = 0, fill = 0, fill_phase = 1;   // stages of the piece issued; ring place
-  Piece src = {};      // the piece that is being loaded
-  int src_n = 0;
+  int at_block = 0, at_next = 0, issued = 0, fill = 0, src_n = 0;   // stages issued and in all of the piece that is loaded
+  Piece src;
   const int bshift = a.page_shift - 4;
   auto page_ids = [&](int i0) {   // raw, so that nothing waits for it here
     const int i = i0 + lane / KB;
-    const int blk = (src.first + kl + i * kw) * KB + lane % KB;
+    const int blk = (src.first + warp + i * WARPS) * KB + lane % KB;
     if (i >= src_n || blk * TOK >= src.len) return INT_MIN;
     const int index = blk >> bshift;
     if (src.slot < 0 || src.slot >= a.num_slots || index >= a.max_pages) return -1;
@@ -750,21 +746,11 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
       report_error(a.err, kErrBadShape);
       page = 0;
     }
-    const int blk = (src.first + kl + (i0 + lane / KB) * kw) * KB + lane % KB;
+    const int blk = (src.first + warp + (i0 + lane / KB) * WARPS) * KB + lane % KB;
     return ((page * a.num_kv_heads + src.head) << bshift) + (blk & ((1 << bshift) - 1));
   };
-  auto start_loads = [&](const Piece& p) {
-    src = p;
-    src_n = p.n > kl ? (p.n - kl + kw - 1) / kw : 0;
-    issued = 0;
-    const int now = page_ids(0);
-    at_next = src_n > AHEAD ? page_ids(AHEAD) : INT_MIN;
-    at_block = blocks_of(now, 0);
-  };
-  auto issue = [&]() {   // the next stage of the source piece into the ring
+  auto issue = [&]() {   // the next stage of the piece into the place that was read last
     if (issued >= src_n) return;
-    // A warp that is alone on its key lane has read the place itself.
-    if (sw_n > 1) mbar_wait(&empty[fill], fill_phase, a.err);
     const int k = issued % AHEAD * KB;
     const int b0 = __shfl_sync(0xffffffff, at_block, k);
     const int b1 = KB == 2 ? __shfl_sync(0xffffffff, at_block, (k + 1) & 31) : -1;
@@ -774,99 +760,90 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
       bulk_load(to, a.data + (size_t)(unsigned)b0 * BLOCK, BLOCK, &full[fill]);
       if (b1 >= 0) bulk_load(to + BLOCK, a.data + (size_t)(unsigned)b1 * BLOCK, BLOCK, &full[fill]);
     }
-    if (++fill == ring) {
-      fill = 0;
-      fill_phase ^= 1;
-    }
+    if (++fill == ring) fill = 0;
     if (++issued % AHEAD == 0 && issued < src_n) {
       at_block = blocks_of(at_next, issued);
       at_next = page_ids(issued + AHEAD);
     }
   };
 
-  int use = 0, use_phase = 0;   // the ring's place to be read
-  long long pos = lo;
-  Piece cur = piece_at(pos);
-  if (sw == 0) {
-    start_loads(cur);
+  // Queries: slot and first dim of the lane in a pass.
+  const int q_slot = warp * S::Q_EACH + lane / S::Q_LANES, q_dim = lane % S::Q_LANES * 8;
+  uint4 q_raw[S::Q_PASSES];
+  int q_len[S::Q_PASSES];
+  // The page ids, the queries and their lengths of a piece are asked for together, then its first stages.
+  auto start = [&](const Piece& p) {
+    src = p;
+    src_n = p.n > warp ? (p.n - warp + WARPS - 1) / WARPS : 0;
+    issued = 0;
+    const int now = page_ids(0);
+    at_next = src_n > AHEAD ? page_ids(AHEAD) : INT_MIN;
+#pragma unroll
+    for (int x = 0; x < S::Q_PASSES; ++x) {
+      const int s = q_slot + x * WARPS * S::Q_EACH, id = p.slot0 + s, row = p.row + id / group;
+      const bool real = s < p.count;
+      q_raw[x] = real ? *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + (size_t)row * a.q_row +
+                                                         (size_t)(p.head * group + id % group) * a.q_head + q_dim)
+                      : make_uint4(0, 0, 0, 0);
+      q_len[x] = real ? plan.lens[row] : p.len;
+    }
+    at_block = blocks_of(now, 0);
     for (int i = 0; i < ring; ++i) issue();
-  }
-  while (true) {
-    // Queries: a warp a slot.  A power of two brings a slot's numbers to [2^13, 2^14), where f16 is exact down to
-    // 2^-27 of the largest; the numbers that meet w & 0x00F000F0 are divided by 16.
-    const int slot_end = min(slots, (cur.count + 7) / 8 * 8);
-    for (int s = warp; s < slot_end; s += WARPS) {
-      constexpr int PER = D / 32;
-      float x[PER];
-      const int id = cur.slot0 + s;
-      const int row = cur.row + id / group;
-      const bool real = s < cur.count;
+  };
+
+  int use = 0, use_phase = 0;   // the ring's place to be read
+  Piece cur = pieces[0];
+  start(cur);
+  for (int k = 0;; ++k) {
+    if (walker) walk(&pieces[(k + 1) & 1]);
+    // A power of two brings a slot's numbers to [2^13, 2^14), where f16 is exact down to 2^-27 of the largest; the numbers
+    // that meet w & 0x00F000F0 are divided by 16.
 #pragma unroll
-      for (int j = 0; j < PER; ++j) x[j] = 0.f;
-      if (real) {
-        const uint16_t* from = static_cast<const uint16_t*>(a.q) + (size_t)row * a.q_row + (size_t)(cur.head * group + id % group) * a.q_head + lane * PER;
-        uint32_t w[PER / 2];
-        if constexpr (PER == 2) w[0] = *reinterpret_cast<const uint32_t*>(from);
-        if constexpr (PER == 4) {
-          const uint2 u = *reinterpret_cast<const uint2*>(from);
-          w[0] = u.x; w[1] = u.y;
-        }
-        if constexpr (PER == 8) {
-          const uint4 u = *reinterpret_cast<const uint4*>(from);
-          w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-        }
+    for (int y = 0; y < S::Q_PASSES; ++y) {
+      const int s = q_slot + y * WARPS * S::Q_EACH;
+      const uint32_t w[4] = {q_raw[y].x, q_raw[y].y, q_raw[y].z, q_raw[y].w};
+      float x[8], big = 0.f, nan = 0.f;
 #pragma unroll
-        for (int j = 0; j < PER / 2; ++j) {
-          const float2 f = two_floats(w[j], a.half);
-          x[2 * j] = f.x;
-          x[2 * j + 1] = f.y;
-        }
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = two_floats(w[j], a.half);
+        x[2 * j] = f.x;
+        x[2 * j + 1] = f.y;
+        big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
+        nan = fmaf(f.x, 0.f, fmaf(f.y, 0.f, nan));
       }
-      float big = 0.f;
-      bool fine = true;
+      if (nan != 0.f) big = INFINITY;
 #pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        big = fmaxf(big, fabsf(x[j]));
-        fine = fine && fabsf(x[j]) < INFINITY;
-      }
-      big = warp_max(big);
-      fine = __all_sync(0xffffffff, fine);
+      for (int o = 1; o < S::Q_LANES; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffff, big, o));
       const int e = 13 - min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 100);
-      const float up = __uint_as_float((uint32_t)(e + 127) << 23);
+      const float up = big < INFINITY ? __uint_as_float((uint32_t)(e + 127) << 23) : NAN;
       float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        x[j] = fine ? x[j] * up : NAN;
+      for (int j = 0; j < 8; ++j) {
+        x[j] *= up;
         sum += x[j];
       }
 #pragma unroll
-      for (int o = 1; o < GROUP / PER; o <<= 1) sum += __shfl_xor_sync(0xffffffff, sum, o);
-      if (lane % (GROUP / PER) == 0) qsum[lane / (GROUP / PER) * slots + s] = sum * 0x1p-24f;
-      if (lane == 0) {
-        qfac[s] = a.sm_scale * 1.4426950408889634f * __uint_as_float((uint32_t)(24 - e + 127) << 23);
-        qlen[s] = real ? plan.lens[row] : cur.len;
-      }
-#pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        const int d = lane * PER + j, in = d & 15, ln = (s & 7) * 4 + ((d & 63) >> 4);
-        int ks, reg, part;
-        if (BITS == 4) {   // number in & 7 of word in / 8: bits 8 .. 15 are shifted down for the second step
-          ks = (d >> 6) * 4 + (in >> 3) * 2 + ((in >> 1) & 1);
-          reg = in & 1;
-          part = (in >> 2) & 1;
-          if (reg) x[j] *= 0.0625f;
-        } else {
-          ks = (d >> 6) * 4 + (in >> 2);
-          reg = in & 1;
-          part = (in >> 1) & 1;
+      for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffff, sum, o);
+      if (s < SLOTS) {
+        const int gi = q_dim >> 6, word = q_dim >> 3 & 1, ln = (s & 7) * 4 + ((q_dim & 63) >> 4);
+        if ((q_dim & 63) == 0) qsum[gi * SLOTS + s] = sum * 0x1p-24f;
+        if (q_dim == 0) {
+          qfac[s] = a.sm_scale * 1.4426950408889634f * __uint_as_float((uint32_t)(24 - e + 127) << 23);
+          qlen[s] = q_len[y];
         }
-        reinterpret_cast<__half*>(qfrag)[(((ks * NT * sw_n + (s >> 3)) * 32 + ln) * 2 + reg) * 2 + part] = __float2half_rn(x[j]);
+        // Steps 2 word and 2 word + 1 of the group have these dims: with 4 bits numbers 0, 4 (1, 5 times 16) and 2, 6 (3, 7) of a
+        // word, with 8 bits 0, 2 (1, 3) of two words.
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          uint2 f;
+          if (BITS == 4) f = make_uint2(pack_f16(x[2 * z], x[2 * z + 4]), pack_f16(x[2 * z + 1] * 0.0625f, x[2 * z + 5] * 0.0625f));
+          else f = make_uint2(pack_f16(x[4 * z], x[4 * z + 2]), pack_f16(x[4 * z + 1], x[4 * z + 3]));
+          *reinterpret_cast<uint2*>(qfrag + (((gi * 4 + word * 2 + z) * NT + (s >> 3)) * 32 + ln) * 8) = f;
+        }
       }
     }
     __syncthreads();
 
-    // A part of the slots that the chunk does not reach has nothing to do (but it releases the stages).
-    const bool busy = sw * NT * 8 < slot_end;
     State<S> st;
     int shortest = INT_MAX;
 #pragma unroll
@@ -879,123 +856,106 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
         for (int i = 0; i < NG; ++i) st.oz[i][n][j] = 0.f;
         st.l[n][j] = 0.f;
         st.ref[n][j] = -INFINITY;
-        const int s = (sw * NT + n) * 8 + 2 * t + j;
-        const bool there = s < slot_end;
-        st.lens[n][j] = there ? qlen[s] : cur.len;
-        st.fac[n][j] = there ? qfac[s] : 0.f;
+        st.lens[n][j] = qlen[n * 8 + 2 * t + j];
+        st.fac[n][j] = qfac[n * 8 + 2 * t + j];
         shortest = min(shortest, st.lens[n][j]);
       }
     shortest = __reduce_min_sync(0xffffffff, shortest);
 
-    const int n_mine = cur.n > kl ? (cur.n - kl + kw - 1) / kw : 0;
+    const int n_mine = src_n;
     for (int it = 0; it < n_mine; ++it) {
       mbar_wait(&full[use], use_phase, a.err);
-      if (busy) {
-        const uint8_t* in = stage0 + use * S::STAGE_BYTES;
-        const uint8_t* qf = qfrag + (sw * NT * 32 + lane) * 8;
-        const int key0 = (cur.first + kl + it * kw) * S::KEYS;
-        if (key0 + S::KEYS <= shortest) stage_step<S, false>(st, in, qf, NT * sw_n * 256, qsum + sw * NT * 8, slots, key0, g, t);
-        else stage_step<S, true>(st, in, qf, NT * sw_n * 256, qsum + sw * NT * 8, slots, key0, g, t);
-      }
+      const uint8_t* in = stage0 + use * S::STAGE_BYTES;
+      const int key0 = (cur.first + warp + it * WARPS) * S::KEYS;
+      if (key0 + S::KEYS <= shortest) stage_step<S, false>(st, in, qfrag + lane * 8, qsum, key0, g, t);
+      else stage_step<S, true>(st, in, qfrag + lane * 8, qsum, key0, g, t);
       __syncwarp();
-      if (sw_n > 1 && lane == 0) mbar_arrive(&empty[use]);
       if (++use == ring) {
         use = 0;
         use_phase ^= 1;
       }
-      if (sw == 0) issue();
+      issue();
     }
 
     // The next piece's first stages are on their way while this one's warps are joined.
     const Piece done = cur;
-    pos += cur.n;
-    const bool more = pos < hi;
-    if (more) {
-      cur = piece_at(pos);
-      if (sw == 0) {
-        start_loads(cur);
-        for (int i = 0; i < ring; ++i) issue();
-      }
-    }
-    // Key lanes are joined in halves: those of the upper half leave their sums, register by register.
-    for (int half = kw / 2; half >= 1; half /= 2) {
-      float* place = merge + ((size_t)((kl % half) * sw_n + sw) * S::MERGE_REGS * 32) + lane;
-      if (kl >= half && kl < 2 * half) {
-        int r = 0;
+    cur = pieces[(k + 1) & 1];
+    if (cur.n > 0) start(cur);
+    // All warps' sums of a slot are brought to the largest reference and added by an item's owner, which also writes them.
+    const size_t rec = (size_t)done.chunk * a.num_kv_heads + done.head + b;
+    float* to = a.partial + rec * SLOTS * (D + 2);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            place[32 * r++] = st.ref[n][j];
-            place[32 * r++] = st.l[n][j];
+      for (int j = 0; j < 2; ++j) {
+        float l = st.l[n][j];
 #pragma unroll
-            for (int gi = 0; gi < NG; ++gi) place[32 * r++] = st.oz[gi][n][j];
-#pragma unroll
-            for (int i = 0; i < KS; ++i) {
-              place[32 * r++] = st.o[i][n][j];
-              place[32 * r++] = st.o[i][n][2 + j];
-            }
-          }
+        for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffff, l, x);
+        if (g == 0) {
+          refs[warp * SLOTS + n * 8 + 2 * t + j] = st.ref[n][j];
+          refs[(WARPS + warp) * SLOTS + n * 8 + 2 * t + j] = l;
         }
       }
-      __syncthreads();
-      if (kl < half) {
-        int r = 0;
+    __syncthreads();
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < NT; ++n) {
+      float f[2];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float other = place[32 * r++];
-            const float m = fmaxf(st.ref[n][j], other);
-            const float f0 = st.ref[n][j] == m ? 1.f : ex2(st.ref[n][j] - m), f1 = other == m ? 1.f : ex2(other - m);
-            st.ref[n][j] = m;
-            st.l[n][j] = st.l[n][j] * f0 + place[32 * r++] * f1;
+      for (int j = 0; j < 2; ++j) {
+        const int s = n * 8 + 2 * t + j;
+        float top = -INFINITY, l = 0.f;
 #pragma unroll
-            for (int gi = 0; gi < NG; ++gi) st.oz[gi][n][j] = st.oz[gi][n][j] * f0 + place[32 * r++] * f1;
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, refs[w * SLOTS + s]);
+        f[j] = st.ref[n][j] == top ? 1.f : ex2(st.ref[n][j] - top);
+        if (warp == 0 && g == 0 && s < done.count) {
 #pragma unroll
-            for (int i = 0; i < KS; ++i) {
-              st.o[i][n][j] = st.o[i][n][j] * f0 + place[32 * r++] * f1;
-              st.o[i][n][2 + j] = st.o[i][n][2 + j] * f0 + place[32 * r++] * f1;
-            }
-          }
+          for (int w = 0; w < WARPS; ++w) l += refs[(WARPS + w) * SLOTS + s] * (refs[w * SLOTS + s] == top ? 1.f : ex2(refs[w * SLOTS + s] - top));
+          *reinterpret_cast<float2*>(to + SLOTS * D + 2 * s) = make_float2(top, l);
         }
+      }
+      if (n > 0) __syncthreads();   // the tile before has been added up
+#pragma unroll
+      for (int item = 0; item < S::ITEMS; ++item) {
+        const int gi = item >> 1, j = item & 1, owner = item % WARPS;
+        if (owner == warp) continue;
+        float* out = sums + ((item * (WARPS - 1) + (warp < owner ? warp : warp - 1)) * S::ITEM) * 32 + lane;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          out[64 * i] = st.o[gi * 4 + i][n][j] * f[j];
+          out[64 * i + 32] = st.o[gi * 4 + i][n][2 + j] * f[j];
+        }
+        out[256] = st.oz[gi][n][j] * f[j];
       }
       __syncthreads();
-    }
-    if (kw == 1) __syncthreads();   // the queries are read no more
-    if (kl == 0 && busy) {
-      // Record: per slot D sums, then reference and l of all slots.
-      const size_t rec = (size_t)done.chunk * a.num_kv_heads + done.head + b;
-      float* to = a.partial + rec * slots * (D + 2);
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int item = 0; item < S::ITEMS; ++item) {
+        const int gi = item >> 1, j = item & 1, s = n * 8 + 2 * t + j;
+        if (item % WARPS != warp) continue;
+        float v[8], zz = st.oz[gi][n][j] * f[j];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int s = (sw * NT + n) * 8 + 2 * t + j;
-          float sum = st.l[n][j];
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffff, sum, x);
-          if (g == 0 && s < done.count) *reinterpret_cast<float2*>(to + slots * D + 2 * s) = make_float2(st.ref[n][j], sum);
-#pragma unroll
-          for (int gi = 0; gi < NG; ++gi) {
-            float zz = st.oz[gi][n][j];
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) zz += __shfl_xor_sync(0xffffffff, zz, x);
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              v[2 * i] = fmaf(st.o[gi * 4 + i][n][j], 0x1p24f, zz);
-              v[2 * i + 1] = fmaf(st.o[gi * 4 + i][n][2 + j], BITS == 4 ? 0x1p20f : 0x1p24f, zz);
-            }
-            if (s < done.count) {
-              float4* to4 = reinterpret_cast<float4*>(to + s * D + gi * GROUP + g * 8);
-              to4[0] = make_float4(v[0], v[1], v[2], v[3]);
-              to4[1] = make_float4(v[4], v[5], v[6], v[7]);
-            }
-          }
+        for (int i = 0; i < 4; ++i) {
+          v[2 * i] = st.o[gi * 4 + i][n][j] * f[j];
+          v[2 * i + 1] = st.o[gi * 4 + i][n][2 + j] * f[j];
         }
+        const float* in = sums + item * (WARPS - 1) * S::ITEM * 32 + lane;
+#pragma unroll
+        for (int w = 0; w < WARPS - 1; ++w) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] += in[(w * S::ITEM + i) * 32];
+          zz += in[(w * S::ITEM + 8) * 32];
+        }
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) zz += __shfl_xor_sync(0xffffffff, zz, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = fmaf(v[i], BITS == 4 && (i & 1) ? 0x1p20f : 0x1p24f, zz);
+        if (s < done.count) {
+          float4* to4 = reinterpret_cast<float4*>(to + s * D + gi * GROUP + g * 8);
+          to4[0] = make_float4(v[0], v[1], v[2], v[3]);
+          to4[1] = make_float4(v[4], v[5], v[6], v[7]);
+        }
+      }
     }
-    if (!more) break;
+    if (cur.n == 0) break;
   }
 }
 
@@ -1189,13 +1149,12 @@ int launch_join(const QuantAttnArgs& a, cudaStream_t stream) {
 
 template <class S>
 int launch_attend(QuantAttnArgs a, cudaStream_t stream) {
-  const int kw = S::WARPS / a.slot_warps;
-  const int room = (227 * 1024 / S::CTAS - 1024 * (S::CTAS > 1)) & ~127;
-  a.ring_offset = (S::fixed(a.slot_warps) + 127) & ~127;
-  a.ring = (room - a.ring_offset) / (kw * S::STAGE_BYTES);
+  const int room = (227 * 1024 / S::CTAS - 1024 * (S::CTAS > 1) - 128) & ~127;
+  a.ring_offset = (S::FIXED + 127) & ~127;
+  a.ring = (room - a.ring_offset) / (S::WARPS * S::STAGE_BYTES);
   if (a.ring > MAX_RING) a.ring = MAX_RING;
-  if (a.ring < 1 || a.chunk != S::slots(a.slot_warps) || a.stage != S::KEYS) return -1;
-  const int bytes = a.ring_offset + kw * a.ring * S::STAGE_BYTES;
+  if (a.ring < 1 || a.chunk != S::SLOTS || a.stage != S::KEYS) return -1;
+  const int bytes = a.ring_offset + S::WARPS * a.ring * S::STAGE_BYTES;
   const auto kernel = attend_kernel<S>;
   cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   zs_launch(kernel, a.grid, S::WARPS * 32, bytes, stream, a);
@@ -1235,14 +1194,13 @@ void set_grid(QuantAttnArgs& a) {
   }
   const Variant v = variant_of(a.head_dim, a.bits, 8 * a.tiles);
   a.grid = 148 * v.ctas;
-  a.least = v.warps / a.slot_warps;
+  a.least = v.warps;
 }
 
 int check_attn(const QuantAttnArgs& a) {
   if (a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256) return -1;
   if ((a.bits != 4 && a.bits != 8) || a.num_kv_heads < 1 || a.num_q_heads % a.num_kv_heads != 0) return -1;
   if (a.rows < 0 || a.rows > a.max_rows || a.num_seqs < 0 || a.max_seq_rows < 1 || a.work == nullptr) return -1;
-  if (a.slot_warps != 1 && a.slot_warps != 2 && a.slot_warps != 4 && a.slot_warps != 8) return -1;
   return 0;
 }
 
@@ -1269,20 +1227,16 @@ extern "C" int zs_quant_load(const QuantRowsArgs* args, cudaStream_t stream) {
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
-// The variant for sequences of `slots` query slots: tiles of 8 slots of a warp, warps that share a key lane, keys
-// of a stage.
-extern "C" void zs_quant_attn_shape(int head_dim, int bits, int slots, int* tiles, int* slot_warps, int* stage) {
+// The variant for sequences of `slots` query slots: tiles of 8 slots of a unit, keys of a stage.
+extern "C" void zs_quant_attn_shape(int head_dim, int bits, int slots, int* tiles, int* stage) {
   if (slots > zs::qc::most_narrow(head_dim)) {
     *tiles = zs::qc::WIDE_SLOTS / 8;
-    *slot_warps = 1;
     *stage = zs::qc::WIDE_KEYS;
     return;
   }
   const zs::qc::Variant v = zs::qc::variant_of(head_dim, bits, slots);
   *tiles = v.tiles;
   *stage = v.blocks * zs::qc::TOK;
-  *slot_warps = 1;
-  while (*slot_warps < v.warps && 8 * v.tiles * *slot_warps < slots) *slot_warps *= 2;
 }
 
 extern "C" long long zs_quant_attn_work(int max_chunks, int max_rows, int max_seqs) {

@@ -764,8 +764,8 @@ typedef struct QuantAttnArgs {
   long long gate_row, gate_head;
   int half;                 // f16 instead of bf16
   float sm_scale;
-  int tiles, slot_warps, stage;   // zs_quant_attn_shape
-  int chunk;                // slots of a unit: 8 * tiles * slot_warps
+  int tiles, stage;         // zs_quant_attn_shape
+  int chunk;                // slots of a unit: 8 * tiles
   int max_chunks;
   void* work;               // zs_quant_attn_work bytes, 32-byte aligned
   float* partial;           // (max_chunks * kv_heads + ZS_QUANT_CTAS) * chunk * (dim + 2)
@@ -776,7 +776,7 @@ typedef struct QuantAttnArgs {
   int* err;
 } QuantAttnArgs;
 
-void zs_quant_attn_shape(int head_dim, int bits, int slots, int* tiles, int* slot_warps, int* stage);
+void zs_quant_attn_shape(int head_dim, int bits, int slots, int* tiles, int* stage);
 long long zs_quant_attn_work(int max_chunks, int max_rows, int max_seqs);
 int zs_quant_attn_plan(const QuantAttnArgs* args, cudaStream_t stream);   // once a step
 int zs_quant_attn(const QuantAttnArgs* args, cudaStream_t stream);        // once a layer
