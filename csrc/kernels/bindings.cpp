@@ -1220,7 +1220,7 @@ struct QuantPlanState {
     TORCH_CHECK_VALUE(q_heads >= 1 && q_heads % c.heads == 0, q_heads, " q heads are not a multiple of ", c.heads, " kv heads");
     TORCH_CHECK_VALUE(max_rows >= 1 && max_seqs >= 1 && max_seq_rows >= 1, "max_rows, max_seqs and max_seq_rows must be positive");
     const int64_t group = q_heads / c.heads;
-    TORCH_CHECK_VALUE(max_rows * q_heads < (1ll << 28) && max_seqs < (1ll << 24), "too many rows or sequences for a plan");
+    TORCH_CHECK_VALUE(max_rows < (1ll << 28) && max_rows * q_heads < (1ll << 28) && max_seqs < (1ll << 24), "too many rows or sequences for a plan");
     QuantAttnArgs& a = base;
     zs_quant_attn_shape(c.dim, c.bits, (int)std::min<int64_t>(group * max_seq_rows, 1 << 20), &a.tiles, &a.stage);
     a.chunk = 8 * a.tiles;
@@ -1275,6 +1275,7 @@ struct QuantPlanState {
     TORCH_CHECK(c.dim == dim && c.bits == bits && c.heads == a.num_kv_heads && c.data.device() == work.device(),
                 "the plan was made for a cache of another form or device");
     TORCH_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf, "q must be bf16 or f16");
+    TORCH_CHECK_VALUE(std::isfinite(sm_scale) && std::isfinite((float)sm_scale), "sm_scale must be finite");
     check_heads(q, c.data, rows, a.num_q_heads, dim, "q");
     check_table(page_table, c.data, rows);
     const at::cuda::CUDAGuard guard(c.data.device());

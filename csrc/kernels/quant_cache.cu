@@ -178,7 +178,10 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) store_kernel(const QuantRowsAr
 #pragma unroll
       for (int j = 0; j < BITS; ++j) to[(j >> 2) * 512 + (j & 3) * 4] = (uint8_t)(n[j >> 2] >> (8 * (j & 3)));
     }
-    if (octet == 0 && there) *reinterpret_cast<uint32_t*>(scales + at) = fine ? __float_as_uint(s) >> 16 | __float_as_uint(z) : POISON;
+    // A constant group (s = 0) is z whatever its scale: with |z| 2^-17 no scale is below 2^-19 of its offset, and the
+    // attention sees from the scales alone how large V is.
+    const float held = s > 0.f ? s : fabsf(z) * 0x1p-17f;
+    if (octet == 0 && there) *reinterpret_cast<uint32_t*>(scales + at) = fine ? __float_as_uint(held) >> 16 | __float_as_uint(z) : POISON;
   };
   for (int h = r.first; h < heads; h += a.step) {
     const uint4 k = k_next, v = v_next;
@@ -266,7 +269,7 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) load_kernel(const QuantRowsArg
 // kv heads at once) stand in a table with the number of stages before them; CTA b of the attention
 // takes the stages [b T / B, (b + 1) T / B) of all T, so that every CTA has the same work whatever the
 // lengths.  One CTA of 1024 threads plans; a step's layers share the plan.
-constexpr int PLAN_THREADS = 1024;
+constexpr int PLAN_THREADS = 1024, MAX_LENGTH = 1 << 30;
 
 // Exclusive sum over the CTA's threads; *all gets the sum of all.
 __device__ __forceinline__ long long block_scan(long long x, long long* warps, long long* all) {
@@ -294,6 +297,15 @@ __device__ __forceinline__ long long block_scan(long long x, long long* warps, l
   return run - x + (warp > 0 ? warps[warp - 1] : 0);
 }
 
+__device__ __forceinline__ int length_of(const QuantAttnArgs& a, int row) {
+  const int n = a.seq_lens[row];
+  if (n > MAX_LENGTH) {
+    report_error(a.err, kErrBadShape);
+    return 0;
+  }
+  return max(n, 0);
+}
+
 __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const QuantAttnArgs a) {
   __shared__ long long warps[32];
   pdl_wait();
@@ -303,7 +315,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const QuantAttnArgs 
   // Rows of no sequence have no chunk.
   for (int r = threadIdx.x; r < a.rows; r += PLAN_THREADS) {
     p.rows[r] = make_int2(-1, 0);
-    p.lens[r] = max(a.seq_lens[r], 0);
+    p.lens[r] = length_of(a, r);
   }
   long long base = 0, all = 0;
   for (int s0 = 0; s0 < a.num_seqs; s0 += PLAN_THREADS) {
@@ -348,7 +360,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const QuantAttnArgs 
       e.count = min(a.chunk, (r1 - r0) * group - e.first);
       const int from = r0 + e.first / group, to = r0 + (e.first + e.count - 1) / group;
       for (int r = from; r <= to; ++r) {
-        e.len = max(e.len, a.seq_lens[r]);
+        e.len = max(e.len, p.lens[r]);
         // A row whose slots are in two chunks is entered by both, with the same numbers.
         p.rows[r] = make_int2(p.offset[lo], r0);
       }
@@ -371,7 +383,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const QuantAttnArgs 
     }
     p.start[b] = lo;
   }
-  if (threadIdx.x == 0) *p.total = base;
+  if (threadIdx.x == 0) {
+    p.total[0] = base;
+    p.total[1] = a.rows;
+  }
 }
 
 // ------------------------------------------------------------------------------- attention
@@ -591,12 +606,18 @@ __device__ __forceinline__ void stage_step(State<S>& st, const uint8_t* in, cons
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        // A masked score is -inf; where the reference still is too, the difference would be NaN.
-        float p = ex2(sc[kb][n][j] + (LIFT - st.ref[n][j & 1]));
+        // A masked score is -inf; where the reference still is too, the difference would be NaN.  The powers of two come last:
+        // beside a large reference they would be lost.
+        float p = ex2(sc[kb][n][j] - st.ref[n][j & 1] + (LIFT + ABOVE));
         if (MASK && key0 + kb * 16 + 2 * g + (j >> 1) >= st.lens[n][j & 1]) p = 0.f;
         sc[kb][n][j] = p;
         st.l[n][j & 1] += p;
       }
+    float low[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) low[n][j] = sc[kb][n][j] * BELOW;
 #pragma unroll
     for (int gi = 0; gi < NG; ++gi) {
       // V's numbers of the tokens 4t..4t+3 (columns 2t, 2t + 8, 2t + 1 and 2t + 9 of a fragment) for this lane's
@@ -616,7 +637,7 @@ __device__ __forceinline__ void stage_step(State<S>& st, const uint8_t* in, cons
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t x = sz[kb][(j >> 1) * NG + gi];
-          ps[j] = sc[kb][n][j] * scale_of(x);
+          ps[j] = low[n][j] * scale_of(x);
           float& oz = st.oz[gi][n][j & 1];
           if (MASK) {   // nothing of a masked key, NaN among it, is taken
             const bool out = key0 + kb * 16 + 2 * g + (j >> 1) >= st.lens[n][j & 1];
@@ -681,7 +702,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
   pdl_wait();
   pdl_trigger();
   const Plan plan = plan_of(a);
-  const long long total = *plan.total;
+  const long long total = stages_of(plan, a);
   int chunk = plan.start[blockIdx.x];   // of the CTA's first stage
   const int ring = a.ring, B = ctas_of(total, gridDim.x, a.least), b = blockIdx.x;
   if (b >= B || total == 0) return;
@@ -815,7 +836,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
 #pragma unroll
       for (int o = 1; o < S::Q_LANES; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffff, big, o));
       const int e = 13 - min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 100);
-      const float up = big < INFINITY ? __uint_as_float((uint32_t)(e + 127) << 23) : NAN;
+      const float up = big < MAX_QUERY ? __uint_as_float((uint32_t)(e + 127) << 23) : NAN;
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -947,7 +968,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) zz += __shfl_xor_sync(0xffffffff, zz, x);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = fmaf(v[i], BITS == 4 && (i & 1) ? 0x1p20f : 0x1p24f, zz);
+        for (int i = 0; i < 8; ++i) v[i] = fmaf(v[i], BITS == 4 && (i & 1) ? 0x1p44f : 0x1p48f, zz);
         if (s < done.count) {
           float4* to4 = reinterpret_cast<float4*>(to + s * D + gi * GROUP + g * 8);
           to4[0] = make_float4(v[0], v[1], v[2], v[3]);
@@ -975,7 +996,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const QuantAttnAr
   const int item = min(at_item, items - 1);
   const int row = item / a.num_q_heads, head = item % a.num_q_heads;
   const int group = a.num_q_heads / a.num_kv_heads, kvh = head / group;
-  const long long total = *plan.total;
+  const long long total = stages_of(plan, a);
   const int2 where = plan.rows[row];
   const int len = plan.lens[row];
   uint32_t gate[PER / 2];
@@ -986,7 +1007,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const QuantAttnAr
   }
   int n = 0, at = 0;
   const float* rec = a.partial;
-  if (where.x >= 0) {
+  if (where.x >= 0 && total > 0) {
     const int s = (row - where.y) * group + head % group;
     const int chunk = where.x + s / a.chunk;
     at = s % a.chunk;

@@ -42,7 +42,10 @@ __device__ __forceinline__ float ex2(float x) {   // 2^x, results below 2^-126 a
 
 // The weights of a row are held as f16 numbers against a reference that bounds its scores (with the scales of V):
 // at most 2^LIFT where it is exact, 2^(LIFT + SLACK) before it is moved, and twice that with a scale's mantissa.
-constexpr float LIFT = 6.f, SLACK = 8.f;
+// A row's sum of weights and its sum of weights times offsets are held 2^ABOVE larger, so that they leave 32 bits at neither
+// end of what V may be.
+constexpr float LIFT = 6.f, SLACK = 8.f, ABOVE = 24.f, BELOW = 0x1p-24f;
+constexpr float MAX_QUERY = 0x1p101f;   // a slot with a query of this size gives NaN
 
 struct Chunk {          // 32 bytes
   long long before;     // stages of the chunks before, all kv heads
@@ -52,7 +55,7 @@ struct Chunk {          // 32 bytes
 };
 
 struct Plan {           // the workspace's integers
-  long long* total;     // stages of all chunks, all kv heads
+  long long* total;     // stages of all chunks, all kv heads; then the rows that were planned
   Chunk* table;         // [max_chunks]
   int2* rows;           // [max_rows] first chunk and first row of the row's sequence (-1: none)
   int* lens;            // [max_rows] keys of the row
@@ -70,6 +73,14 @@ __host__ __device__ inline Plan plan_of(const QuantAttnArgs& a) {
   p.start = p.lens + a.max_rows;
   p.offset = p.start + ZS_QUANT_CTAS;
   return p;
+}
+
+// Stages of the plan, 0 if it is not of the rows that are asked for (a captured call whose plan was changed since).
+__device__ __forceinline__ long long stages_of(const Plan& p, const QuantAttnArgs& a) {
+  const longlong2 x = *reinterpret_cast<const longlong2*>(p.total);
+  if (x.y == a.rows) return x.x;
+  report_error(a.err, kErrBadShape);
+  return 0;
 }
 
 // Number of CTAs that share T stages.

@@ -9,8 +9,8 @@
 //  * 14 converter warps, one at K or V of a block: s n + z as one f16 fused multiply-add of two numbers,
 //    rounded once (2^-12 of a value).  (w & 0x000F000F) is two subnormals n 2^-24 and the factor s 2^24, so a
 //    pair costs an integer instruction, a part of a shift and the multiply-add.  A power of two per block
-//    brings its largest value to [2^-8, 2^-7), which keeps s 2^24 and every value in f16's range whatever
-//    their size; the scores and the weights take it back.  K goes to a swizzled image of keys x dims, V to one
+//    brings its largest scale to [2^-9, 2^-8), which keeps s 2^24 and every value in f16's range whatever
+//    their size (an offset is below 2^19 of its group's scale); the scores and the weights take it back.  K goes to a swizzled image of keys x dims, V to one
 //    of dims x keys (as it is stored), both K-major operands;
 //  * MMA warp: S of the next tile goes before O of this one;
 //  * 16 softmax warps: a thread has a block of a tile for a slot.  The weights 2^(x - reference) are held
@@ -40,7 +40,7 @@ struct Smem {
   uint64_t k_full[2], v_full[2], k_empty[4], v_empty[4], s_full[2], p_full[2], o_full[2], q_full, unit_full[UNITS];
   uint32_t tmem;
   int abort;
-  float k_unit[UNITS][TBLOCKS];          // what the blocks of K of a tile are multiples of
+  float k_unit[UNITS][TBLOCKS];          // 2^-9 of what the blocks of K of a tile are multiples of
   float v_log[UNITS][TBLOCKS];           // log2 of the same of V
   uint32_t v_bad[UNITS][TBLOCKS][2];     // poisoned (token, group) pairs: pair x is bit x / n of word x % n (n words are used)
   alignas(16) uint32_t pairs[CONV / 32][TOK * 4];   // of a converter's block: per group and token, scale and offset in f16
@@ -130,10 +130,10 @@ __device__ __forceinline__ void mma_step(uint32_t d, uint32_t a_tmem, uint32_t b
 __device__ __forceinline__ uint32_t desc_lo(const void* p) { return (smem_u32(p) >> 4) | ((16 >> 4) << 16); }
 constexpr uint32_t idesc_f16(uint32_t m, uint32_t n) { return 1u << 4 | (n >> 3) << 17 | (m >> 4) << 24; }
 
-// floor(log2 x) of the largest of a warp's numbers, at least -72 (and then the unit at least 2^-64).
+// floor(log2 x) of the largest of a warp's numbers, at least -72.
 __device__ __forceinline__ int warp_exponent(float x) {
   const uint32_t u = __reduce_max_sync(0xffffffff, __float_as_uint(x));
-  return min(max((int)(u >> 23) - 127, -72), 118);
+  return max((int)(u >> 23) - 127, -72);
 }
 
 template <class W>
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
   pdl_wait();
   pdl_trigger();
   const Plan plan = plan_of(a);
-  const long long total = *plan.total;
+  const long long total = stages_of(plan, a);
   const int B = ctas_of(total, gridDim.x, a.least), cta = blockIdx.x;
   const bool work = cta < B && total > 0;
   const int group = a.num_q_heads / a.num_kv_heads;
@@ -304,7 +304,6 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
     // -------------------------------------------------------------- converters
     // The warps take the parts of the tiles (K, then V of each block) in turn.
     const int w = warp - SOFT / 32, g = lane >> 2, t4 = lane & 3;
-    constexpr float TOP = (1 << BITS) - 1;
     constexpr int PAIRS = (TOK * NG + 31) / 32;
     int at = w, before = 0;   // the next part, counted over the CTA's tiles; tiles of the pieces before
     bool ok = true;
@@ -333,10 +332,10 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
             if (nan || out) {
               if (is_v) sf[c] = zf[c] = 0.f;
             } else {
-              top = fmaxf(top, fmaf(TOP, sf[c], fabsf(zf[c])));
+              top = fmaxf(top, fmaxf(sf[c], fabsf(zf[c]) * 0x1p-22f));
             }
           }
-          const int e = warp_exponent(top) + 8;
+          const int e = warp_exponent(top) + 9;
           const float f1 = __uint_as_float((uint32_t)(127 - (e >> 1)) << 23), f2 = __uint_as_float((uint32_t)(127 - (e - (e >> 1))) << 23);
 #pragma unroll
           for (int c = 0; c < PAIRS; ++c) {
@@ -349,7 +348,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
               s.v_bad[i % UNITS][kb][0] = bad[0];
               s.v_bad[i % UNITS][kb][1] = PAIRS > 1 ? bad[PAIRS - 1] : 0;
             } else {
-              s.k_unit[i % UNITS][kb] = __uint_as_float((uint32_t)min(e + 127, 254) << 23);
+              s.k_unit[i % UNITS][kb] = __uint_as_float((uint32_t)(e - 9 + 127) << 23);
             }
           }
           __syncwarp();
@@ -441,7 +440,6 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
     int limit = more ? plan.lens[row_of(p)] : 0;
     while (more) {
       const bool used = slot < p.count, busy = (warp & 3) * 32 < p.count;
-      if (!used) limit = 0;
       float fac;
       {
         // The slot's quarter of the query, brought to [2^13, 2^14) by a power of two, as pairs in the order in which
@@ -466,8 +464,8 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
         big = fmaxf(fmaxf(s.top[0][slot], s.top[1][slot]), fmaxf(s.top[2][slot], s.top[3][slot]));
         soft_sync();
         const int e = 13 - min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 100);
-        const float up = big < INFINITY ? copysignf(__uint_as_float((uint32_t)(e + 127) << 23), a.sm_scale) : NAN;
-        fac = fabsf(a.sm_scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - e) << 23);
+        const float up = big < MAX_QUERY ? copysignf(__uint_as_float((uint32_t)(e + 127) << 23), a.sm_scale) : NAN;
+        fac = fabsf(a.sm_scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + 9 - e) << 23);
         if (busy) {
 #pragma unroll
           for (int c = 0; c < D / 32; c += 2) {
@@ -562,7 +560,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
             r[j] = __float_as_uint(w);
             sum[j & 1] += w;
           }
-          l += (sum[0] + sum[1]) * ex2(-v);
+          l += (sum[0] + sum[1]) * ex2(ABOVE - v);
           // Tokens of a four lie in the order 0 2 1 3 in V's image; the weights take the place of their own scores.
           uint32_t pk[8];
 #pragma unroll
@@ -616,6 +614,8 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
           uint32_t o[8];
           tmem_ld_x8(lanes + TMEM_O + part * (D / 4) + c, o);
           tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * (1.f / BELOW));
           const bool nan = bad >> ((part * (D / 4) + c) >> 6) & 1;
           uint4* st = s.stage[warp][lane];   // its halves change places in every second four of slots
           const int turn = lane >> 2 & 1;

@@ -3,7 +3,7 @@
 64 consecutive dims of one token and head are a group.  With N = 15 (4 bits) or 255 (8 bits) a
 group is held as whole numbers n in 0..N, a scale s and an offset z in bf16: z is the group's
 minimum rounded down, s is (maximum - z) / N rounded up, n is (x - z) / s rounded to the nearest
-(ties to even), and the value held is s n + z.  That is 4.5 or 8.5 bits a value.  A group with a
+(ties to even; 0 where s is 0), and the value held is s n + z.  That is 4.5 or 8.5 bits a value.  A group with a
 NaN, an infinity or a magnitude above 2^126 reads back as NaN.
 
 A ``QuantCache`` is the paged cache of a model's attention layers; a ``QuantAttention`` plans a
@@ -85,7 +85,8 @@ class QuantAttention:
     def update(self, slots: torch.Tensor, seq_lens: torch.Tensor, seq_start: torch.Tensor | None = None) -> None:
         """Divide a step's keys over the GPU.  ``slots`` [rows] and ``seq_lens`` [rows] (int32): the sequence of each
         row and the keys it sees (0: none).  ``seq_start`` [sequences + 1] (int32): rows seq_start[i] to
-        seq_start[i+1] are of one sequence and read its keys together; None: every row reads its own."""
+        seq_start[i+1] are of one sequence (the first row's slot) and read its keys together; None: every row reads
+        its own."""
         self.state.update(slots, seq_lens, seq_start)
 
     def attend(self, layer: int, q: torch.Tensor, page_table: torch.Tensor, sm_scale: float, gate: torch.Tensor | None = None,
@@ -94,7 +95,7 @@ class QuantAttention:
         """sigmoid(gate) * attention of ``q`` [rows, q heads, dim] (bf16 or f16; rows and heads may be strided) for
         the rows of the last ``update``; ``gate`` None: no gate.  The result goes to ``out`` ([rows, heads * dim]
         of q's type, allocated unless the MXFP8 pair ``out_q``, ``out_sf`` is given alone).  A row without keys, or
-        of no sequence, gives 0."""
+        of no sequence, gives 0; a head of ``q`` with a NaN or a magnitude of 2^101 or more gives NaN."""
         return self.state.attend(self.cache.state, layer, q, page_table, sm_scale, gate, out, out_q, out_sf)
 
     def check(self) -> None:
