@@ -28,7 +28,7 @@ namespace {
 constexpr int SOFT = 512, CONV = 448;               // threads; then the MMA and the copy warp
 constexpr int THREADS = SOFT + CONV + 64;
 constexpr int MMA_WARP = (SOFT + CONV) / 32, COPY_WARP = MMA_WARP + 1;
-constexpr int TBLOCKS = WIDE_KEYS / TOK, PARTS = 2 * TBLOCKS;   // blocks of a tile, their K and V
+constexpr int TBLOCKS = WIDE_KEYS / TOK;   // blocks of a tile
 constexpr uint32_t TMEM_Q = 128, TMEM_O = 256, TMEM_COLS = 512;   // two S of 64 columns, Q as pairs, O
 constexpr int MAX_RAW = 4;
 // Tiles whose units are kept.  A tile's raw blocks are overwritten by the MAX_RAW-th after it at the earliest, whose V is
@@ -37,13 +37,13 @@ constexpr int UNITS = 2 * MAX_RAW;
 
 struct Smem {
   uint64_t raw_full[4], raw_empty[MAX_RAW];
-  uint64_t k_full[2], v_full[2], k_empty[4], v_empty[4], s_full[2], p_full[2], o_full[2], q_full, unit_full[UNITS];
+  uint64_t k_full[2], v_full[2], k_empty[4], v_empty[4], s_full[2], p_full[2], o_full[2], q_full;
   uint32_t tmem;
   int abort;
   float k_unit[UNITS][TBLOCKS];          // 2^-9 of what the blocks of K of a tile are multiples of
   float v_log[UNITS][TBLOCKS];           // log2 of the same of V
   uint32_t v_bad[UNITS][TBLOCKS][2];     // poisoned (token, group) pairs: pair x is bit x / n of word x % n (n words are used)
-  alignas(16) uint32_t pairs[CONV / 32][TOK * 4];   // of a converter's block: per group and token, scale and offset in f16
+  alignas(16) uint32_t pairs[CONV / 32][2][TOK * 4];   // of a converter's block, K and V: per group and token, scale and offset in f16
   float top[TBLOCKS][WIDE_SLOTS];
   uint4 stage[SOFT / 32][32][2];     // 8 columns of a warp's 32 slots, on their way to the record
 };
@@ -78,18 +78,37 @@ __device__ __forceinline__ bool wait_for(Smem& s, uint64_t* bar, uint32_t phase,
   *reinterpret_cast<volatile int*>(&s.abort) = 1;
   return false;
 }
-__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
-__device__ __forceinline__ bool soft_any(bool x) {
+// Of the four warps that have the same slots.
+__device__ __forceinline__ void slots_sync(int quarter) { asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory"); }
+__device__ __forceinline__ bool slots_any(int quarter, bool x) {
   int r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %1, 0;\n\t"
-      "bar.red.or.pred q, 1, 512, p;\n\t"
+      "bar.red.or.pred q, %2, 128, p;\n\t"
       "selp.b32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"((int)x)
+      : "r"((int)x), "r"(1 + quarter)
       : "memory");
   return r != 0;
+}
+__device__ __forceinline__ float2 fma_two(float2 a, float b, float c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmov.b64 c, {%5, %5};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float2 add_two(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -154,12 +173,12 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
     tmem_relinquish();
   }
   if (tid == 0) {
-    for (int i = 0; i < RING; ++i) mbar_init(&s.raw_empty[i], PARTS);
+    for (int i = 0; i < RING; ++i) mbar_init(&s.raw_empty[i], TBLOCKS);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.k_full[i], TBLOCKS);
       mbar_init(&s.v_full[i], TBLOCKS);
       mbar_init(&s.s_full[i], 1);
-      mbar_init(&s.p_full[i], SOFT);
+      mbar_init(&s.p_full[i], SOFT / 32);
       mbar_init(&s.o_full[i], 1);
     }
     for (int i = 0; i < 4; ++i) {
@@ -167,8 +186,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
       mbar_init(&s.k_empty[i], 1);
       mbar_init(&s.v_empty[i], 1);
     }
-    mbar_init(&s.q_full, SOFT);
-    for (int i = 0; i < UNITS; ++i) mbar_init(&s.unit_full[i], TBLOCKS);
+    mbar_init(&s.q_full, SOFT / 32);
     s.abort = 0;
     fence_barrier_init();
   }
@@ -302,23 +320,24 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
     __syncwarp();
   } else if (warp >= SOFT / 32) {
     // -------------------------------------------------------------- converters
-    // The warps take the parts of the tiles (K, then V of each block) in turn.
+    // The warps take the blocks of the tiles in turn, K and then V of each.
     const int w = warp - SOFT / 32, g = lane >> 2, t4 = lane & 3;
     constexpr int PAIRS = (TOK * NG + 31) / 32;
-    int at = w, before = 0;   // the next part, counted over the CTA's tiles; tiles of the pieces before
+    int at = w, before = 0;   // the next block, counted over the CTA's tiles; tiles of the pieces before
     bool ok = true;
     while (ok && next_piece(p)) {
-      for (; ok && at / PARTS < before + p.n; at += CONV / 32) {
-        const int i = at / PARTS, b = i & 1, kb = at & (TBLOCKS - 1);
-        const bool is_v = at & TBLOCKS;
+      for (; ok && at / TBLOCKS < before + p.n; at += CONV / 32) {
+        const int i = at / TBLOCKS, b = i & 1, kb = at & (TBLOCKS - 1);
         const int st = i % RING, left = p.len - (p.first + i - before) * WIDE_KEYS - kb * TOK;   // keys of the block from here on
         const uint8_t* in = ring + st * W::RAW + kb * BLOCK;
         ok = __all_sync(0xffffffff, wait_for(s, &s.raw_full[i & 3], (i >> 2) & 1, a.err));
         if (!ok) break;
-        // The block's unit from its scales and offsets (a lane has one or two of the 16 NG pairs), and those as multiples
+        // The block's units from its scales and offsets (a lane has one or two of the 16 NG pairs), and those as multiples
         // of it: s 2^24 and z.  What is behind the sequence does not count, and is 0 in V, as poisoned groups are.
-        {
-          const uint32_t* sz = reinterpret_cast<const uint32_t*>(in + 2 * W::CODES + (is_v ? TOK * NG * 4 : 0));
+        // The softmax reads the units once S is there, which no K is missing from.
+#pragma unroll 1
+        for (int is_v = 0; is_v < 2; ++is_v) {
+          const uint32_t* sz = reinterpret_cast<const uint32_t*>(in + 2 * W::CODES) + is_v * TOK * NG;
           float sf[PAIRS], zf[PAIRS], top = 0.f;
           uint32_t bad[PAIRS];
 #pragma unroll
@@ -340,7 +359,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
 #pragma unroll
           for (int c = 0; c < PAIRS; ++c) {
             const int x = lane * PAIRS + c;
-            if (x < TOK * NG) s.pairs[w][x % NG * TOK + x / NG] = pack_f16(sf[c] * f1 * f2 * 0x1p24f, zf[c] * f1 * f2);
+            if (x < TOK * NG) s.pairs[w][is_v][x % NG * TOK + x / NG] = pack_f16(sf[c] * f1 * f2 * 0x1p24f, zf[c] * f1 * f2);
           }
           if (lane == 0) {
             if (is_v) {
@@ -351,22 +370,21 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
               s.k_unit[i % UNITS][kb] = __uint_as_float((uint32_t)(e - 9 + 127) << 23);
             }
           }
-          __syncwarp();
-          if (is_v && lane == 0) mbar_arrive(&s.unit_full[i % UNITS]);   // the softmax need not wait for the image
         }
-        // The image is free once the product of the tile two before has read it.  The warps are not in step: one may be
+        __syncwarp();
+        // An image is free once the product of the tile two before has read it.  The warps are not in step: one may be
         // here before the product of the tile four before is done, but not that of six before, whose blocks have left the
         // ring.  A barrier for each of four tiles, here and for the blocks, then has one phase that can be meant.
-        if (i >= 2) ok = __all_sync(0xffffffff, wait_for(s, is_v ? &s.v_empty[(i - 2) & 3] : &s.k_empty[(i - 2) & 3], ((i - 2) >> 2) & 1, a.err));
+        if (i >= 2) ok = __all_sync(0xffffffff, wait_for(s, &s.k_empty[(i - 2) & 3], ((i - 2) >> 2) & 1, a.err));
         if (!ok) break;
-        if (!is_v) {
+        {
           const int r0 = kb * 16 + 2 * g;
           uint8_t* out = k_image + b * W::K_IMAGE + r0 * 128;
           // Every second row the other way round: the lanes of a phase then touch 32 banks.
           const int flip = g & 1, at0 = ((t4 * 2 + flip) ^ (r0 & 7)) << 4, at1 = at0 ^ 16;
 #pragma unroll 1
           for (int gi = 0; gi < NG; ++gi) {
-            const uint2 sz = *reinterpret_cast<const uint2*>(&s.pairs[w][gi * TOK + 2 * g]);
+            const uint2 sz = *reinterpret_cast<const uint2*>(&s.pairs[w][0][gi * TOK + 2 * g]);
 #pragma unroll
             for (int tk = 0; tk < 2; ++tk) {
               const uint32_t pair = tk ? sz.y : sz.x, S = __byte_perm(pair, pair, 0x1010), Z = __byte_perm(pair, pair, 0x3232);
@@ -388,12 +406,18 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
               }
             }
           }
-        } else {
+        }
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.k_full[b]);
+        if (i >= 2) ok = __all_sync(0xffffffff, wait_for(s, &s.v_empty[(i - 2) & 3], ((i - 2) >> 2) & 1, a.err));
+        if (!ok) break;
+        {
           const int perm = (2 * g + (g >> 2)) & 7;
           uint8_t* out = v_image + b * W::V_IMAGE + perm * 128 + (((kb * 2 + (t4 >> 1)) ^ perm) << 4) + (t4 & 1) * 8;
 #pragma unroll 1
           for (int gi = 0; gi < NG; ++gi, out += 64 * 128) {
-            const uint4 sz = *reinterpret_cast<const uint4*>(&s.pairs[w][gi * TOK + t4 * 4]);
+            const uint4 sz = *reinterpret_cast<const uint4*>(&s.pairs[w][1][gi * TOK + t4 * 4]);
             const uint32_t S0 = __byte_perm(sz.x, sz.z, 0x5410), Z0 = __byte_perm(sz.x, sz.z, 0x7632);
             const uint32_t S1 = __byte_perm(sz.y, sz.w, 0x5410), Z1 = __byte_perm(sz.y, sz.w, 0x7632);
 #pragma unroll
@@ -418,7 +442,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(&s.raw_empty[st]);
-          mbar_arrive(is_v ? &s.v_full[b] : &s.k_full[b]);
+          mbar_arrive(&s.v_full[b]);
         }
       }
       before += p.n;
@@ -427,8 +451,8 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
     // ---------------------------------------------------------------- softmax
     // After a wait that gave up these warps go on to their last piece's end (every later wait gives up at
     // once), so that their barriers meet.
-    const int part = warp >> 2, slot = (warp & 3) * 32 + lane;   // the block of a tile, and the quarter of O's columns
-    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const int part = warp >> 2, quarter = warp & 3, slot = quarter * 32 + lane;   // the block of a tile, and the quarter of O's columns
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     const auto row_of = [&](const Piece& x) { return x.row + (x.slot0 + min(slot, x.count - 1)) / group; };
     const auto query_of = [&](const Piece& x) {
       const int id = x.slot0 + min(slot, x.count - 1);
@@ -439,7 +463,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
     bool more = next_piece(p);
     int limit = more ? plan.lens[row_of(p)] : 0;
     while (more) {
-      const bool used = slot < p.count, busy = (warp & 3) * 32 < p.count;
+      const bool used = slot < p.count, busy = quarter * 32 < p.count;
       float fac;
       {
         // The slot's quarter of the query, brought to [2^13, 2^14) by a power of two, as pairs in the order in which
@@ -460,9 +484,9 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
           }
         }
         s.top[part][slot] = nan == 0.f ? big : INFINITY;
-        soft_sync();
+        slots_sync(quarter);
         big = fmaxf(fmaxf(s.top[0][slot], s.top[1][slot]), fmaxf(s.top[2][slot], s.top[3][slot]));
-        soft_sync();
+        slots_sync(quarter);
         const int e = 13 - min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 100);
         const float up = big < MAX_QUERY ? copysignf(__uint_as_float((uint32_t)(e + 127) << 23), a.sm_scale) : NAN;
         fac = fabsf(a.sm_scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + 9 - e) << 23);
@@ -489,7 +513,8 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
           tmem_st_wait();
         }
         tc_fence_before();
-        mbar_arrive(&s.q_full);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.q_full);
       }
       // The next piece is looked up, and its queries are brought into L2, while this one's tiles are on their way.
       Piece next;
@@ -503,10 +528,9 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
       uint32_t bad = 0;
       for (int t = 0; t < p.n; ++t, ++i) {
         const int b = i & 1, valid = limit - (p.first + t) * WIDE_KEYS - part * TOK;
-        wait_for(s, &s.unit_full[i % UNITS], (i / UNITS) & 1, a.err);
-        const float v = s.v_log[i % UNITS][part];
         wait_for(s, &s.s_full[b], (i >> 1) & 1, a.err);
         tc_fence_after();
+        const float v = s.v_log[i % UNITS][part];
         const float f = fmaxf(fac * s.k_unit[i % UNITS][part], 0x1p-126f);
         uint32_t r[16];
         float most = -INFINITY;
@@ -524,9 +548,9 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
           most = fmaf(fmaxf(x[0], x[1]), f, v);
         }
         // Does a slot's reference have to move?
-        if (soft_any(used && most > ref + SLACK)) {
+        if (busy && slots_any(quarter, used && most > ref + SLACK)) {
           s.top[part][slot] = most;
-          soft_sync();
+          slots_sync(quarter);
           most = fmaxf(fmaxf(s.top[0][slot], s.top[1][slot]), fmaxf(s.top[2][slot], s.top[3][slot]));
           const bool grow = used && most > ref + SLACK;
           const float shrink = grow ? ex2(ref - most) : 1.f;
@@ -549,18 +573,21 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
             }
             tmem_st_wait();
           }
-          soft_sync();   // the maxima have been read
+          slots_sync(quarter);   // the maxima have been read
         }
         if (busy) {
           const float off = (ref == -INFINITY ? 0.f : LIFT - ref) + v;
-          float sum[2] = {0.f, 0.f};
+          float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float w = ex2(fmaf(__uint_as_float(r[j]), f, off));
-            r[j] = __float_as_uint(w);
-            sum[j & 1] += w;
+          for (int j = 0; j < 16; j += 2) {
+            float2 w = fma_two(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), f, off);
+            w.x = ex2(w.x);
+            w.y = ex2(w.y);
+            r[j] = __float_as_uint(w.x);
+            r[j + 1] = __float_as_uint(w.y);
+            sum = add_two(sum, w);
           }
-          l += (sum[0] + sum[1]) * ex2(ABOVE - v);
+          l += (sum.x + sum.y) * ex2(ABOVE - v);
           // Tokens of a four lie in the order 0 2 1 3 in V's image; the weights take the place of their own scores.
           uint32_t pk[8];
 #pragma unroll
@@ -590,15 +617,16 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
           }
         }
         tc_fence_before();
-        mbar_arrive(&s.p_full[b]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.p_full[b]);
       }
       // ---- the slots' records
       s.top[part][slot] = l;
-      soft_sync();
+      slots_sync(quarter);
       l = (s.top[0][slot] + s.top[1][slot]) + (s.top[2][slot] + s.top[3][slot]);
-      soft_sync();
+      slots_sync(quarter);
       s.top[part][slot] = __uint_as_float(bad);
-      soft_sync();
+      slots_sync(quarter);
       bad = (__float_as_uint(s.top[0][slot]) | __float_as_uint(s.top[1][slot])) | (__float_as_uint(s.top[2][slot]) | __float_as_uint(s.top[3][slot]));
       wait_for(s, &s.o_full[(i - 1) & 1], ((i - 1) >> 1) & 1, a.err);
       tc_fence_after();
@@ -607,8 +635,8 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
       if (busy) {
         // Column gi 64 + 8 j + perm(g) is dim gi 64 + 8 g + j; the join puts them in order.  8 columns at a time go
         // through shared memory, so that an instruction stores whole sectors.
-        float* mine = to + (size_t)((warp & 3) * 32 + (lane >> 1)) * D + part * (D / 4) + (lane & 1) * 4;
-        const int left = p.count - (warp & 3) * 32 - (lane >> 1);
+        float* mine = to + (size_t)(quarter * 32 + (lane >> 1)) * D + part * (D / 4) + (lane & 1) * 4;
+        const int left = p.count - quarter * 32 - (lane >> 1);
 #pragma unroll 1
         for (int c = 0; c < D / 4; c += 8) {
           uint32_t o[8];
@@ -630,7 +658,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
         }
         if (used && part == 0) *reinterpret_cast<float2*>(to + (size_t)WIDE_SLOTS * D + 2 * slot) = make_float2(ref, l);
       }
-      soft_sync();   // the poisoned groups have been read
+      slots_sync(quarter);   // the poisoned groups have been read
       tc_fence_before();
       p = next;
       limit = next_limit;
