@@ -32,7 +32,7 @@ def test_bytes_of_a_value():
 
 
 @pytest.mark.parametrize("heads,rows,seqs,per", [(3, 1, 1, 1), (0, 1, 1, 1), (2, 0, 1, 1), (2, 1, 0, 1), (2, 1, 1, 0),
-                                                 (2, 1 << 28, 1, 1), (2, 1, 1 << 24, 1)])
+                                                 (2, 1 << 28, 1, 1), (2, 1, 1 << 24, 1), (2, 1 << 62, 1, 1)])
 def test_plan_forms(heads, rows, seqs, per):
     with pytest.raises(ValueError):
         QuantAttention(QuantCache(1, 4, 2, 64, device="cpu"), heads, max_rows=rows, max_seqs=seqs, max_seq_rows=per)

@@ -544,3 +544,266 @@ def test_plan_is_shared_by_layers_and_its_workspace_is_reused():
         want, tol = reference(one, table, q, [0, 1], lens, 0.1)
         assert np.all(np.abs(got[layer].double().cpu().numpy() - want) <= tol)
     assert math.isfinite(float(got[0].float().sum()))
+
+
+# ------------------------------------------------------------- many query slots, and the ends of the ranges
+def wide_tolerance(cache, table, q, slots, lens, scale):
+    """What sequences of many slots may be off by in addition: K and V go through f16 there, which is half a step
+    (2^-12) of a value, or 2^-16 of the largest scale of its block (at most 2^-3 of the largest value) where it is a
+    subnormal.  A score is then off by that share of the sum of |q| |k|, a weight by twice that, V by the share itself."""
+    rows, hq, dim = q.shape
+    kvh = cache.num_kv_heads
+    tol = np.zeros((rows, hq, dim))
+    qn = q.double().abs().sum(-1).cpu().numpy()
+    for r in range(rows):
+        if int(lens[r]) <= 0:
+            continue
+        pos = torch.arange(int(lens[r]), dtype=torch.int32, device=DEV)
+        k, v = (t.double().abs().cpu().numpy() for t in cache.read(0, table, torch.full_like(pos, int(slots[r])), pos, dtype=torch.float32))
+        for h in range(hq):
+            kk, vv = k[:, h * kvh // hq].max(), v[:, h * kvh // hq]
+            share = 2.0 ** -12 + 2.0 ** -19
+            tol[r, h] = (2 * abs(scale) * qn[r, h] * share * kk + share) * (vv.max(0) + vv.max())
+    return tol.reshape(rows, -1)
+
+
+def run_rows(cache, table, q, slots, lens, starts, scale, **kw):
+    most = max([b - a for a, b in zip(starts, starts[1:])] + [1])
+    plan = QuantAttention(cache, q.shape[1], max_rows=len(slots), max_seqs=len(starts) - 1, max_seq_rows=most)
+    plan.update(_i32(slots), _i32(lens), _i32(starts))
+    got = plan.attend(0, q, table, scale, **kw)
+    plan.check()
+    return got
+
+
+def assert_near(got, cache, table, q, slots, lens, scale, gate=None, absolute=True):
+    want, tol = reference(cache, table, q, slots, lens, scale, gate)
+    tol = tol + wide_tolerance(cache, table, q, slots, lens, scale) - (0 if absolute else 2.0 ** -25)
+    err = np.abs(got.double().cpu().numpy() - want)
+    assert np.all(err <= tol), (float(np.nanmax(err / np.maximum(tol, 1e-300))), int(np.isnan(err).sum()), np.argwhere(~(err <= tol))[:4].tolist())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim,bits", [(64, 4), (128, 4), (256, 4), (64, 8), (128, 8), (256, 8)])
+@pytest.mark.parametrize("per", [3, 5, 7, 33])
+def test_rows_of_each_size_of_unit(dim, bits, per, dtype):
+    """12, 20, 28 and 132 slots, both types, pages of 256 tokens; rows without keys and sequences of 0 and 1 keys."""
+    lens = [300, 1, 0, 65]
+    cache, table = filled(lens, 2, dim, bits, page=256, dtype=dtype, seed=per)
+    starts = [i * per for i in range(5)]
+    slots = [s for s in range(4) for _ in range(per)]
+    seen = [max(0, lens[s] - (i % 3) * (s != 1)) if i != 1 else 0 for s in range(4) for i in range(per)]
+    g = torch.Generator(device=DEV).manual_seed(per)
+    q = torch.randn(4 * per, 8, dim, generator=g, device=DEV).to(dtype)
+    scale = dim ** -0.5
+    got = run_rows(cache, table, q, slots, seen, starts, scale)
+    assert_near(got, cache, table, q, slots, seen, scale)
+    empty = [r for r, n in enumerate(seen) if n == 0]
+    assert not got[empty].any()
+
+
+@pytest.mark.parametrize("per", [1, 4, 20])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_scores_of_either_sign_and_none(bits, per):
+    lens = [100, 37]
+    cache, table = filled(lens, 1, 128, bits, seed=per)
+    starts, slots, seen = [0, per, 2 * per], [0] * per + [1] * per, [100] * per + [37] * per
+    q = torch.randn(2 * per, 8, 128, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).to(torch.bfloat16)
+    for scale in (-0.2, 0.0, 0.2):
+        assert_near(run_rows(cache, table, q, slots, seen, starts, scale), cache, table, q, slots, seen, scale)
+    plan = QuantAttention(cache, 8, 2 * per)
+    plan.update(_i32(slots), _i32(seen))
+    for scale in (float("nan"), float("inf"), 1e300):
+        with pytest.raises(ValueError, match="sm_scale"):
+            plan.attend(0, q, table, scale)
+
+
+@pytest.mark.parametrize("per", [1, 20])
+@pytest.mark.parametrize("dim,bits", [(64, 8), (128, 4), (256, 4), (256, 8)])
+def test_values_of_any_size(dim, bits, per):
+    """V from 2^-40 to 2^120, K that q makes up for, and V whose groups are constant."""
+    lens = [150, 33]
+    starts, slots, seen = [0, per, 2 * per], [0] * per + [1] * per, [150] * per + [33] * per
+    g = torch.Generator(device=DEV).manual_seed(per)
+    q = torch.randn(2 * per, 8, dim, generator=g, device=DEV).to(torch.bfloat16)
+    scale = dim ** -0.5
+    for v_scale in (2.0 ** -40, 2.0 ** 60, 2.0 ** 104, 2.0 ** 120):
+        cache, table = filled(lens, 1, dim, bits, seed=3, v_scale=v_scale)
+        got = run_rows(cache, table, q, slots, seen, starts, scale)
+        assert_near(got, cache, table, q, slots, seen, scale, absolute=False)
+    table, pages = table_of(lens, 16)
+    at, pos = places_of(lens)
+    for k_scale in (2.0 ** -60, 2.0 ** 90, 2.0 ** 120):
+        for const in (0.0, 2.0 ** -30, -2.0 ** 20, 2.0 ** 100):
+            cache = QuantCache(1, pages, 1, dim, bits=bits)
+            k = rows_of(len(at), 1, dim, torch.bfloat16, 5, k_scale)
+            v = torch.full((len(at), 1, dim), const, device=DEV, dtype=torch.bfloat16)
+            cache.write(0, k, v, table, at, pos)
+            small = (q.float() * min(max(1 / k_scale, 2.0 ** -90), 2.0 ** 90)).to(torch.bfloat16)
+            rest = scale / k_scale / min(max(1 / k_scale, 2.0 ** -90), 2.0 ** 90)
+            got = run_rows(cache, table, small, slots, seen, starts, rest)
+            # Weights that add up to 1 times a constant: the rounding of the weights, the images and the output.
+            assert np.all(np.abs(got.double().cpu().numpy() - const) <= abs(const) * (2.0 ** -9 + 2.0 ** -10))
+
+
+def test_sizes_that_differ_from_group_to_group():
+    """V whose groups are 2^12 apart, within a block of many slots too: the small one keeps its own precision."""
+    n, dim, per = 200, 128, 20
+    table, pages = table_of([n], 16)
+    at, pos = places_of([n])
+    k, v = rows_of(n, 1, dim, torch.bfloat16, 1), rows_of(n, 1, dim, torch.bfloat16, 2)
+    v[:, :, 64:] *= 2.0 ** -8
+    for bits in (4, 8):
+        cache = QuantCache(1, pages, 1, dim, bits=bits)
+        cache.write(0, k, v, table, at, pos)
+        q = torch.randn(per, 4, dim, generator=torch.Generator(device=DEV).manual_seed(2), device=DEV).to(torch.bfloat16)
+        got = run_rows(cache, table, q, [0] * per, [n] * per, [0, per], 0.09).view(per, 4, 2, 64)
+        want, tol = reference(cache, table, q, [0] * per, [n] * per, 0.09)
+        vmax = cache.read(0, table, at, pos, dtype=torch.float32)[1].abs().double().cpu().numpy().reshape(n, 2, 64).max((0, 2))
+        want = want.reshape(per, 4, 2, 64)
+        # A weight is off by 2^-12 and K's rounding, V by 2^-12 of itself and 2^-16 of the block's largest scale (2/15 of
+        # its largest value at most), the output by half a step.
+        dk = 0.09 * float(q.float().abs().sum(-1).max()) * float(k.float().abs().max()) * (2.0 ** -12 + 2.0 ** -19)
+        for gi in range(2):
+            limit = 2 * (2 * dk + 2.0 ** -11 + 2.0 ** -17) * vmax[gi] + 2.0 ** -16 * 2 / 15 * vmax.max() + 2.0 ** -8 * np.abs(want[:, :, gi])
+            assert np.all(np.abs(got[:, :, gi].double().cpu().numpy() - want[:, :, gi]) <= limit)
+
+
+@pytest.mark.parametrize("dim,bits", [(64, 8), (128, 4), (256, 4), (256, 8)])
+def test_poison_in_many_rows(dim, bits):
+    """As for few rows: a poisoned K spoils the rows that see it, a poisoned V their dims of its group."""
+    n, per = 90, 45
+    table, pages = table_of([n], 16)
+    at, pos = places_of([n])
+    k, v = rows_of(n, 1, dim, torch.bfloat16, 1), rows_of(n, 1, dim, torch.bfloat16, 2)
+    q = torch.randn(per, 4, dim, generator=torch.Generator(device=DEV).manual_seed(3), device=DEV).to(torch.bfloat16)
+    q[7, 2, 5] = float("inf")
+    q[8, 1, 9] = 2.0 ** 101
+    seen = [n - per + 1 + i for i in range(per)]
+    for which, group in (("k", 0), ("v", 0), ("v", dim // 64 - 1)):
+        a, b = k.clone(), v.clone()
+        (a if which == "k" else b)[70, 0, group * 64 + 9] = float("nan")   # seen by rows of more than 70 keys
+        cache = QuantCache(1, pages, 1, dim, bits=bits)
+        cache.write(0, a, b, table, at, pos)
+        got = run_rows(cache, table, q, [0] * per, seen, [0, per], 0.1).view(per, 4, dim)
+        bad = torch.zeros(per, 4, dim, dtype=torch.bool, device=DEV)
+        sees = torch.tensor([x > 70 for x in seen], device=DEV)
+        if which == "k":
+            bad[sees] = True
+        else:
+            bad[sees, :, group * 64:group * 64 + 64] = True
+        bad[7, 2] = bad[8, 1] = True
+        assert torch.equal(got.isnan(), bad)
+        clean = [r for r in range(per) if seen[r] <= 70 and r not in (7, 8)]
+        assert_near(got.view(per, -1)[clean], cache, table, q[clean], [0] * len(clean), [seen[r] for r in clean], 0.1)
+
+
+def test_strided_queries_and_mxfp8_of_many_rows():
+    from zstep_b200.ops import mx
+
+    per, hq, dim, n = 140, 4, 128, 260
+    cache, table = filled([n], 2, dim, 4, seed=12)
+    wide = torch.randn(per, 2 * hq + 1, dim, device=DEV).to(torch.bfloat16)
+    q, gate = wide[:, 0:2 * hq:2], wide[:, 1:2 * hq:2]
+    seen = [n - per + 1 + i for i in range(per)]
+    out = torch.empty(per, hq * dim, dtype=torch.bfloat16, device=DEV)
+    out_q = torch.empty(256, hq * dim, dtype=torch.uint8, device=DEV)
+    out_sf = torch.zeros(mx.atoms_bytes(per, hq * dim), dtype=torch.uint8, device=DEV)
+    run_rows(cache, table, q, [0] * per, seen, [0, per], 0.09, gate=gate, out=out, out_q=out_q, out_sf=out_sf)
+    assert_near(out, cache, table, q, [0] * per, seen, 0.09, gate)
+    got = mx.dequantize(out_q[:per], mx.codes_from_atoms(out_sf, per, hq * dim))
+    block = out.float().abs().view(per, -1, 32).amax(-1, keepdim=True).expand(-1, -1, 32).reshape(per, -1)
+    assert bool(((got - out.float()).abs() <= out.float().abs() * (2.0 ** -4 + 2.0 ** -8) + block * 2.0 ** -10).all())
+
+
+def test_one_row_of_many_heads_and_results_that_repeat():
+    """80 heads of a kv head; the same call twice, and on another stream, gives the same bits."""
+    lens = [500, 3, 64, 65]
+    cache, table = filled(lens, 1, 128, 4, seed=2)
+    q = torch.randn(4, 80, 128, generator=torch.Generator(device=DEV).manual_seed(4), device=DEV).to(torch.bfloat16)
+    plan = QuantAttention(cache, 80, 4)
+    plan.update(_i32([0, 1, 2, 3]), _i32(lens))
+    got = plan.attend(0, q, table, 0.09)
+    assert_near(got, cache, table, q, [0, 1, 2, 3], lens, 0.09)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        x = rows_of(4, 1, 128, torch.bfloat16, 6)
+        cache.write(0, x, x, table, _i32([0, 1, 2, 3]), _i32([499, 2, 63, 64]))
+        plan.update(_i32([0, 1, 2, 3]), _i32(lens))
+        other = plan.attend(0, q, table, 0.09)
+        assert_near(other, cache, table, q, [0, 1, 2, 3], lens, 0.09)
+        assert torch.equal(plan.attend(0, q, table, 0.09), other)
+    torch.cuda.current_stream().wait_stream(side)
+
+
+def test_graphs_that_share_a_plan():
+    """Each captured step plans and attends: replayed in any order they do not disturb one another.  A captured attend
+    alone, whose plan was made for other rows since, reports that and gives zeros."""
+    lens = [150, 80]
+    cache, table = filled(lens, 1, 64, 4, seed=2)
+    plan = QuantAttention(cache, 4, 24, 2, 12)
+    g = torch.Generator(device=DEV).manual_seed(4)
+    steps = []
+    for per in (1, 12, 3):
+        q = torch.randn(2 * per, 4, 64, generator=g, device=DEV).to(torch.bfloat16)
+        s, n, at = _i32([0] * per + [1] * per), _i32([150] * per + [80] * per), _i32([0, per, 2 * per])
+        out = torch.empty(2 * per, 256, dtype=torch.bfloat16, device=DEV)
+        plan.update(s, n, at)
+        plan.attend(0, q, table, 0.125, out=out)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            plan.update(s, n, at)
+            plan.attend(0, q, table, 0.125, out=out)
+        steps.append((graph, q, s, n, at, out))
+    for i in (2, 0, 1, 1, 0):
+        graph, q, s, n, _, out = steps[i]
+        out.zero_()
+        graph.replay()
+        assert_near(out, cache, table, q, s.tolist(), n.tolist(), 0.125)
+    plan.check()
+    _, q, s, n, at, out = steps[2]
+    plan.update(s, n, at)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan.attend(0, q, table, 0.125, out=out)
+    graph.replay()
+    assert_near(out, cache, table, q, s.tolist(), n.tolist(), 0.125)
+    plan.check()
+    steps[1][0].replay()
+    graph.replay()
+    assert not out.any()
+    with pytest.raises(RuntimeError, match="error status"):
+        plan.check()
+
+
+def test_lengths_beyond_any_cache_are_reported():
+    cache, table = filled([40], 1, 64, 4)
+    q = torch.randn(1, 2, 64, device=DEV).to(torch.bfloat16)
+    plan = QuantAttention(cache, 2, 4)
+    plan.update(_i32([0]), _i32([2 ** 31 - 1]))
+    assert not plan.attend(0, q, table, 0.1).any()
+    with pytest.raises(RuntimeError, match="error status"):
+        plan.check()
+    plan.update(_i32([0]), _i32([-5]))
+    assert not plan.attend(0, q, table, 0.1).any()
+    plan.check()
+
+
+def test_places_beyond_32_bits():
+    """Pages whose bytes lie more than 2^32 into a layer."""
+    dim, heads, page = 256, 2, 256
+    cache = QuantCache(1, 20000, heads, dim, bits=8, page_size=page)
+    assert cache.page_bytes * 15500 > 2 ** 32
+    n = 300
+    table = _i32([[19999, 15500], [3, 19998]])
+    slots, pos = places_of([n, n])
+    k, v = rows_of(2 * n, heads, dim, torch.bfloat16, 1), rows_of(2 * n, heads, dim, torch.bfloat16, 2)
+    cache.write(0, k, v, table, slots, pos)
+    for x, y in zip((k, v), cache.read(0, table, slots, pos, dtype=torch.float32)):
+        want = quantised(x, 8)[0]
+        assert np.all(np.abs(y.double().cpu().numpy() - want) <= 2.0 ** -24 * np.abs(want))
+    check_attention(cache, table, 8, [0, 1], [n, n])
+    q = torch.randn(20, 8, dim, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).to(torch.bfloat16)
+    got = run_rows(cache, table, q, [0] * 10 + [1] * 10, [n] * 20, [0, 10, 20], 0.06)
+    assert_near(got, cache, table, q, [0] * 10 + [1] * 10, [n] * 20, 0.06)
