@@ -93,6 +93,8 @@ def interleave_gate_up(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
 class Qwen35Runner:
     """Single-process model runner for one GPU (tp_rank of tp_size)."""
 
+    kv_bits = 16   # of the attention layers' K and V
+
     def __init__(self, cfg: Qwen35Config, *, device="cuda", weights=None, max_seqs: int = 256,
                  max_prefill_tokens: int = 4096, num_pages: int = 4096, page_size: int = 16,
                  max_model_len: int = 4096, num_ckpt_slots: int = 0, tp_rank: int = 0, tp_size: int = 1,
