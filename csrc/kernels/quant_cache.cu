@@ -443,6 +443,7 @@ template <int D_, int BITS_, int NT_, int WARPS_, int KB_, int CTAS_, bool FINE_
 struct Shape {
   static constexpr int D = D_, BITS = BITS_, NT = NT_, WARPS = WARPS_, KB = KB_, CTAS = CTAS_;
   static constexpr bool FINE = FINE_;
+  static constexpr int FOLD = FINE ? 2 : 8;         // stages between additions of the offsets' sums
   static constexpr int KS = D / 16;                 // tiles of 16 dims of V
   static constexpr int NG = D / GROUP;
   static constexpr int CODES = code_bytes(D, BITS);
@@ -477,8 +478,8 @@ struct State {
 // Sequences with few slots.  S^T = K Q^T and O^T += V^T P^T on m16n8k16 (a tile of 8 slots is the narrow side, so
 // that 8 slots waste nothing), every warp at its own stages of its own ring of bulk copies: no warp waits for
 // another before the end of a piece.  Measured with the join: 256 sequences of up to 1280 keys, 16 q heads on 2 kv heads
-// of 256 dims, 4 bits 48 us (3.1 TB/s); 61 sequences of up to 4001 keys, 8 heads of 128 dims, 8 bits 72 us (5.6 TB/s); 7
-// sequences of up to 65 535 keys, 32 on 4 heads of 128 dims, 4 bits, f16 55 us (3.9 TB/s).  With 4 bits it is bound by
+// of 256 dims, 4 bits 49 us (3.0 TB/s); 61 sequences of up to 4001 keys, 8 heads of 128 dims, 8 bits 72 us (5.6 TB/s); 7
+// sequences of up to 65 535 keys, 32 on 4 heads of 128 dims, 4 bits, f16 59 us (3.6 TB/s; 55 with offsets added every 8 stages, see FOLD).  With 4 bits it is bound by
 // the instructions that open the codes and feed the products, with 8 bits by memory.  e4m3 products for K are emulated here and took 61 -> 70 us; smaller CTAs, and
 // warps of their own for the copies, were no faster.
 //
@@ -706,6 +707,32 @@ __device__ __forceinline__ void stage_step(State<S>& st, const uint8_t* in, cons
   }
 }
 
+// The numbers of V are not negative, so that their sums grow with the keys, and the offsets' sums take most of that away
+// again in the end.  The products cut what they add to a sum behind its 24th bit, always towards zero: over
+// sequences of 65 535 keys, dozens of stages a warp, f16 outputs were off by 0.00047 of their norm instead of the 0.00021
+// of their own rounding.  The offsets' sums are
+// therefore added every FOLD stages, while both are small: 0.00032 every 8 stages, 0.00027 every 2.  For bf16 outputs,
+// whose rounding is 0.0017, 8 are enough (48 -> 49 us for 256 sequences).
+template <class S>
+__device__ __forceinline__ void fold_offsets(State<S>& st) {
+#pragma unroll
+  for (int gi = 0; gi < S::NG; ++gi)
+#pragma unroll
+    for (int n = 0; n < S::NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float zz = st.oz[gi][n][j];
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) zz += __shfl_xor_sync(0xffffffff, zz, x);
+        st.oz[gi][n][j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          st.o[gi * 4 + i][n][j] = fmaf(zz, 0x1p-48f, st.o[gi * 4 + i][n][j]);
+          st.o[gi * 4 + i][n][2 + j] = fmaf(zz, S::BITS == 4 ? 0x1p-44f : 0x1p-48f, st.o[gi * 4 + i][n][2 + j]);
+        }
+      }
+}
+
 template <class S>
 __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const QuantAttnArgs a) {
   constexpr int KS = S::KS, NG = S::NG, NT = S::NT, D = S::D, BITS = S::BITS, BLOCK = S::BLOCK, WARPS = S::WARPS, KB = S::KB, SLOTS = S::SLOTS;
@@ -908,6 +935,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
         use_phase ^= 1;
       }
       issue();
+      if (it % S::FOLD == S::FOLD - 1) fold_offsets(st);
     }
 
     // The next piece's first stages are on their way while this one's warps are joined.

@@ -807,3 +807,26 @@ def test_places_beyond_32_bits():
     q = torch.randn(20, 8, dim, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).to(torch.bfloat16)
     got = run_rows(cache, table, q, [0] * 10 + [1] * 10, [n] * 20, [0, 10, 20], 0.06)
     assert_near(got, cache, table, q, [0] * 10 + [1] * 10, [n] * 20, 0.06)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_outputs_near_zero_of_long_sequences(bits):
+    """V around zero: what is left of a long sum of numbers that are not negative has the precision of an f16 output.
+
+    320 rows of one sequence give a warp some 90 stages.  The 32-bit sums may take a quarter of the rounding's norm:
+    16 additions of 2^-23 each between two sums near zero, times the 2^7 by which 20 000 keys' numbers exceed what is
+    left, are 2^-12, a third of them in the root mean square, spread over ten such stretches of either sign."""
+    n, dim, rows = 20000, 64, 320
+    table, pages = table_of([n], 16)
+    at, pos = places_of([n])
+    g = torch.Generator(device=DEV).manual_seed(7)
+    cache = QuantCache(1, pages, 1, dim, bits=bits)
+    cache.write(0, torch.randn(n, 1, dim, generator=g, device=DEV).half(), torch.randn(n, 1, dim, generator=g, device=DEV).half(), table, at, pos)
+    q = torch.randn(rows, 8, dim, generator=g, device=DEV).half()
+    plan = QuantAttention(cache, 8, rows)
+    plan.update(_i32([0] * rows), _i32([n] * rows))
+    got = plan.attend(0, q, table, 0.125).view(rows, 8, dim).double()
+    plan.check()
+    k, v = (x[:, 0].double() for x in cache.read(0, table, at, pos, dtype=torch.float32))
+    want = torch.softmax(q.double() @ k.T * 0.125, -1) @ v
+    assert float((got - want).norm()) <= 1.25 * float((want.half().double() - want).norm())
