@@ -8,20 +8,21 @@
 //  * copy warp: page ids, then one bulk copy per 16-token block into a ring of tiles;
 //  * 14 converter warps, each at a block, its K and then its V: s n + z as one f16 fused multiply-add of two
 //    numbers, rounded once (2^-12 of a value).  (w & 0x000F000F) is two subnormals n 2^-24 and the factor s 2^24,
-//    so a pair costs an integer instruction, a part of a shift and the multiply-add.  A power of two per block
-//    brings its largest scale to [2^-9, 2^-8), which keeps s 2^24 and every value in f16's range whatever their
-//    size (an offset is below 2^19 of its group's scale); the scores and the weights take it back.  K goes to a
+//    so a pair costs an integer instruction, a part of a shift and the multiply-add.  A power of two per token
+//    (its unit) brings its largest scale to [2^-9, 2^-8), which keeps s 2^24 and every value in f16's range whatever their
+//    size (an offset is below 2^19 of its group's scale), and no token's precision depends on another; K's unit goes to
+//    the token's scores and V's to its weights, in 32 bits.  K goes to a
 //    swizzled image of keys x dims, V to one of dims x keys (as it is stored), both K-major operands;
 //  * MMA warp: S of the next tile goes before O of this one;
 //  * 16 softmax warps: a thread has a block of a tile for a slot.  The weights 2^(x - reference) are held
-//    below 2^14 times the block's power of two, as f16 (2^-11; for f16 outputs the rest goes through a second
+//    below 2^14 with the token's unit of V, as f16 (2^-11; for f16 outputs the rest goes through a second
 //    product); the reference follows the largest score only when that outgrew it by 2^8, and O in TMEM is
 //    rescaled then.
 // A poisoned group of V (NaN) is 0 in the image; the slots that see its key note it, and their dims of the
-// group become NaN in the record.  So nothing of a masked key reaches a slot.
+// group become NaN in the record.  So nothing of a masked key reaches a slot: its bits are the same whatever stands there.
 //
-// Measured (us, 16 q heads, 2 kv heads of 256 dims, 4 bits): 128 sequences of up to 2300 keys with 4 rows 99, three
-// chunks of up to 700 rows that see up to 4500 keys 195 (0.57 PFLOP/s of products).  A tile takes some 2900 cycles with 256 dims
+// Measured (us, 16 q heads, 2 kv heads of 256 dims, 4 bits): 128 sequences of up to 2300 keys with 4 rows 107, three
+// chunks of up to 700 rows that see up to 4500 keys 211 (0.52 PFLOP/s of products).  A tile takes some 2900 cycles with 256 dims
 // and 1900 with 64, of which the products are 1000 and 260.  With 256 dims the converters (16384 pairs of numbers
 // a tile) and the softmax share the issue slots; with 64 it is the softmax's chain: scores 360, agreement of the four warps 190, weights 840 (four warps of a scheduler take their 64
 // exponentials there), handing over 150.  Tried and slower or no faster: tiles taken in turn by two sets of softmax
@@ -39,17 +40,21 @@ constexpr int MMA_WARP = (SOFT + CONV) / 32, COPY_WARP = MMA_WARP + 1;
 constexpr int TBLOCKS = WIDE_KEYS / TOK;   // blocks of a tile
 constexpr uint32_t TMEM_Q = 128, TMEM_O = 256, TMEM_COLS = 512;   // two S of 64 columns, Q as pairs, O
 constexpr int MAX_RAW = 4;
-// Tiles whose units are kept.  A tile's raw blocks are overwritten by the MAX_RAW-th after it at the earliest, whose V is
-// converted once O of the tile two before that is done: no unit is overwritten that a softmax still needs.
-constexpr int UNITS = 2 * MAX_RAW;
+// Tiles whose units are kept.  The raw blocks of tile i come into the place of tile i - MAX_RAW's at the earliest, whose V was
+// converted once O of tile i - MAX_RAW - 2 was done: no unit is overwritten that a softmax still needs.
+constexpr int UNITS = MAX_RAW + 2;
+
+// What a unit of K is held as: a unit is at most 2^132, and scores of the largest K and q still stay below 2^116.
+constexpr int K_SMALL_LOG = -33;
 
 struct Smem {
   uint64_t raw_full[4], raw_empty[MAX_RAW];
   uint64_t k_full[2], v_full[2], k_empty[4], v_empty[4], s_full[2], p_full[2], o_full[2], q_full;
   uint32_t tmem;
   int abort;
-  float k_unit[UNITS][TBLOCKS];          // 2^-9 of what the blocks of K of a tile are multiples of
-  float v_log[UNITS][TBLOCKS];           // log2 of the same of V
+  alignas(16) float k_unit[UNITS][WIDE_KEYS];   // a token's unit of K, times 2^K_SMALL_LOG
+  float v_log[UNITS][WIDE_KEYS];         // log2 of a token's unit of V
+  float v_inv[UNITS][WIDE_KEYS];         // 2^ABOVE over the same unit
   uint32_t v_bad[UNITS][TBLOCKS][2];     // poisoned (token, group) pairs: pair x is bit x / n of word x % n (n words are used)
   alignas(16) uint32_t pairs[CONV / 32][2][TOK * 4];   // of a converter's block, K and V: per group and token, scale and offset in f16
   float top[TBLOCKS][WIDE_SLOTS];
@@ -100,13 +105,22 @@ __device__ __forceinline__ bool slots_any(int quarter, bool x) {
       : "memory");
   return r != 0;
 }
-__device__ __forceinline__ float2 fma_two(float2 a, float b, float c) {
+__device__ __forceinline__ float2 fma_two(float2 a, float2 b, float2 c) {
   float2 d;
   asm("{\n\t.reg .b64 a, b, c, d;\n\t"
-      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmov.b64 c, {%5, %5};\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
       "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
       : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b), "f"(c));
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul_two(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
 __device__ __forceinline__ float2 add_two(float2 a, float2 b) {
@@ -157,11 +171,6 @@ __device__ __forceinline__ void mma_step(uint32_t d, uint32_t a_tmem, uint32_t b
 __device__ __forceinline__ uint32_t desc_lo(const void* p) { return (smem_u32(p) >> 4) | ((16 >> 4) << 16); }
 constexpr uint32_t idesc_f16(uint32_t m, uint32_t n) { return 1u << 4 | (n >> 3) << 17 | (m >> 4) << 24; }
 
-// floor(log2 x) of the largest of a warp's numbers, at least -72.
-__device__ __forceinline__ int warp_exponent(float x) {
-  const uint32_t u = __reduce_max_sync(0xffffffff, __float_as_uint(x));
-  return max((int)(u >> 23) - 127, -72);
-}
 
 template <class W>
 __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a) {
@@ -340,9 +349,9 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
         const uint8_t* in = ring + st * W::RAW + kb * BLOCK;
         ok = __all_sync(0xffffffff, wait_for(s, &s.raw_full[i & 3], (i >> 2) & 1, a.err));
         if (!ok) break;
-        // The block's units from its scales and offsets (a lane has one or two of the 16 NG pairs), and those as multiples
-        // of it: s 2^24 and z.  What is behind the sequence does not count, and is 0 in V, as poisoned groups are.
-        // The softmax reads the units once S is there, which no K is missing from.
+        // The tokens' units from their scales and offsets (a lane has one or two of the 16 NG pairs, two lanes a token where
+        // there are more than one), and those as multiples of it: s 2^24 and z.  What is behind the sequence is 0 in V, as
+        // poisoned groups are.  The softmax reads the units once S is there, which no K is missing from.
 #pragma unroll 1
         for (int is_v = 0; is_v < 2; ++is_v) {
           const uint32_t* sz = reinterpret_cast<const uint32_t*>(in + 2 * W::CODES) + is_v * TOK * NG;
@@ -362,21 +371,26 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
               top = fmaxf(top, fmaxf(sf[c], fabsf(zf[c]) * 0x1p-22f));
             }
           }
-          const int e = warp_exponent(top) + 9;
+          if (NG > 1) top = fmaxf(top, __shfl_xor_sync(0xffffffff, top, 1));
+          const int e = max((int)(__float_as_uint(top) >> 23) - 127, -72) + 9;
           const float f1 = __uint_as_float((uint32_t)(127 - (e >> 1)) << 23), f2 = __uint_as_float((uint32_t)(127 - (e - (e >> 1))) << 23);
 #pragma unroll
           for (int c = 0; c < PAIRS; ++c) {
             const int x = lane * PAIRS + c;
             if (x < TOK * NG) s.pairs[w][is_v][x % NG * TOK + x / NG] = pack_f16(sf[c] * f1 * f2 * 0x1p24f, zf[c] * f1 * f2);
           }
-          if (lane == 0) {
+          if (lane * PAIRS < TOK * NG && lane * PAIRS % NG == 0) {
+            const int key = kb * TOK + lane * PAIRS / NG;
             if (is_v) {
-              s.v_log[i % UNITS][kb] = (float)e;
-              s.v_bad[i % UNITS][kb][0] = bad[0];
-              s.v_bad[i % UNITS][kb][1] = PAIRS > 1 ? bad[PAIRS - 1] : 0;
+              s.v_log[i % UNITS][key] = (float)e;
+              s.v_inv[i % UNITS][key] = __uint_as_float((uint32_t)((int)ABOVE - e + 127) << 23);
             } else {
-              s.k_unit[i % UNITS][kb] = __uint_as_float((uint32_t)(e - 9 + 127) << 23);
+              s.k_unit[i % UNITS][key] = __uint_as_float((uint32_t)(e + K_SMALL_LOG + 127) << 23);
             }
+          }
+          if (is_v && lane == 0) {
+            s.v_bad[i % UNITS][kb][0] = bad[0];
+            s.v_bad[i % UNITS][kb][1] = PAIRS > 1 ? bad[PAIRS - 1] : 0;
           }
         }
         __syncwarp();
@@ -497,7 +511,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
         slots_sync(quarter);
         const int e = 13 - min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 100);
         const float up = big < MAX_QUERY ? copysignf(__uint_as_float((uint32_t)(e + 127) << 23), a.sm_scale) : NAN;
-        fac = fabsf(a.sm_scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + 9 - e) << 23);
+        fac = fminf(fabsf(a.sm_scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - K_SMALL_LOG - e) << 23), 0x1p126f);
         if (busy) {
 #pragma unroll
           for (int c = 0; c < D / 32; c += 2) {
@@ -538,13 +552,25 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
         const int b = i & 1, valid = limit - (p.first + t) * WIDE_KEYS - part * TOK;
         wait_for(s, &s.s_full[b], (i >> 1) & 1, a.err);
         tc_fence_after();
-        const float v = s.v_log[i % UNITS][part];
-        const float f = fmaxf(fac * s.k_unit[i % UNITS][part], 0x1p-126f);
-        uint32_t r[16];
+        const float4* k_unit = reinterpret_cast<const float4*>(s.k_unit[i % UNITS] + part * TOK);
+        const float4* v_log = reinterpret_cast<const float4*>(s.v_log[i % UNITS] + part * TOK);
+        const float4* v_inv = reinterpret_cast<const float4*>(s.v_inv[i % UNITS] + part * TOK);
+        uint32_t r[16];   // scores and log2 of V's units
         float most = -INFINITY;
         if (busy) {
           tmem_ld_32x32b_x16(lanes + b * 64 + part * 16, r);
           tmem_ld_wait();
+          const float2 fac2 = make_float2(fac, fac);
+#pragma unroll
+          for (int j = 0; j < 16; j += 4) {
+            const float4 k = k_unit[j / 4], v = v_log[j / 4];
+            const float2 lo = fma_two(mul_two(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), make_float2(k.x, k.y)), fac2, make_float2(v.x, v.y));
+            const float2 hi = fma_two(mul_two(make_float2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])), make_float2(k.z, k.w)), fac2, make_float2(v.z, v.w));
+            r[j] = __float_as_uint(lo.x);
+            r[j + 1] = __float_as_uint(lo.y);
+            r[j + 2] = __float_as_uint(hi.x);
+            r[j + 3] = __float_as_uint(hi.y);
+          }
           if (__any_sync(0xffffffff, valid < 16)) {
 #pragma unroll
             for (int j = 0; j < 16; ++j)
@@ -553,7 +579,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
           float x[2] = {-INFINITY, -INFINITY};
 #pragma unroll
           for (int j = 0; j < 16; ++j) x[j & 1] = fmaxf(x[j & 1], __uint_as_float(r[j]));
-          most = fmaf(fmaxf(x[0], x[1]), f, v);
+          most = fmaxf(x[0], x[1]);
         }
         // Does a slot's reference have to move?
         if (busy && slots_any(quarter, used && most > ref + SLACK)) {
@@ -584,18 +610,19 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
           slots_sync(quarter);   // the maxima have been read
         }
         if (busy) {
-          const float off = (ref == -INFINITY ? 0.f : LIFT - ref) + v;
+          const float off = ref == -INFINITY ? 0.f : LIFT - ref;
           float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
           for (int j = 0; j < 16; j += 2) {
-            float2 w = fma_two(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), f, off);
+            float2 w = add_two(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), make_float2(off, off));
             w.x = ex2(w.x);
             w.y = ex2(w.y);
             r[j] = __float_as_uint(w.x);
             r[j + 1] = __float_as_uint(w.y);
-            sum = add_two(sum, w);
+            const float4 inv = v_inv[j / 4];
+            sum = fma_two(w, j & 2 ? make_float2(inv.z, inv.w) : make_float2(inv.x, inv.y), sum);
           }
-          l += (sum.x + sum.y) * ex2(ABOVE - v);
+          l += sum.x + sum.y;
           // Tokens of a four lie in the order 0 2 1 3 in V's image; the weights take the place of their own scores.
           uint32_t pk[8];
 #pragma unroll

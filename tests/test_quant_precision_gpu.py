@@ -1,0 +1,147 @@
+"""How near the quantised attention is to the 64-bit result, and what a row may depend on: limits that a dropped key or a
+score 2 % off do not pass (tests/test_quant_oracle.py), for every grouping of rows."""
+
+import numpy as np
+import pytest
+import torch
+
+from tests.quant_oracle import LIMIT, attention, distance, held
+from zstep_b200.ops.quant_cache import QuantAttention, QuantCache
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+FORMS = [(64, 4), (128, 4), (256, 4), (64, 8), (128, 8), (256, 8)]
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def keys_of(n, heads, dim, dtype, seed):
+    """Keys and values whose channels have offsets and sizes of their own."""
+    g = gen(seed)
+    size = torch.exp(0.5 * torch.randn(heads, dim, generator=g, device=DEV))
+    k = size * (torch.randn(n, heads, dim, generator=g, device=DEV) + torch.randn(heads, dim, generator=g, device=DEV))
+    return k.to(dtype), (0.7 * torch.randn(n, heads, dim, generator=g, device=DEV)).to(dtype)
+
+
+class Held:
+    """Sequences of these keys and values in a cache, their pages in any order."""
+
+    def __init__(self, ks, vs, bits, page=16):
+        n = [len(k) for k in ks]
+        need = [-(-x // page) for x in n]
+        ids = torch.randperm(sum(need), generator=torch.Generator().manual_seed(1)) + 1
+        table = torch.zeros(len(ks), max(need) + 1, dtype=torch.int32)
+        for i, part in enumerate(ids.split(need)):
+            table[i, :need[i]] = part
+        self.table, self.ks, self.vs, self.bits = table.to(DEV), ks, vs, bits
+        self.cache = QuantCache(1, sum(need) + 1, ks[0].shape[1], ks[0].shape[2], bits=bits, page_size=page)
+        at = i32(np.repeat(np.arange(len(n)), n).tolist()), i32([p for x in n for p in range(x)])
+        self.cache.write(0, torch.cat(ks), torch.cat(vs), self.table, *at)
+        self.cache.check()
+
+    def attend(self, q, counts, lens, scale, gate=None):
+        """counts[s] rows of sequence s, each with its length; alone where counts is None (row r of sequence r)."""
+        each = [1] * len(self.ks) if counts is None else counts
+        slots = i32([s for s, c in enumerate(each) for _ in range(c)])
+        starts = None if counts is None else i32([0] + list(np.cumsum(counts)))
+        plan = QuantAttention(self.cache, q.shape[1], max_rows=len(q), max_seqs=len(each), max_seq_rows=max(each))
+        plan.update(slots, i32(lens), starts)
+        out = plan.attend(0, q, self.table, scale, gate=gate)
+        plan.check()
+        return out.view(q.shape)
+
+    def exact(self, q, counts, lens, scale, gate=None):
+        out, r = [], 0
+        for s, c in enumerate([1] * len(self.ks) if counts is None else counts):
+            part = slice(r, r + c)
+            out.append(attention(q[part], held(self.ks[s], self.bits), held(self.vs[s], self.bits), lens[part], scale,
+                                 None if gate is None else gate[part]))
+            r += c
+        return torch.cat(out)
+
+
+# ------------------------------------------------------------------------------------ precision
+@pytest.mark.parametrize("dtype", [torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 2, 5, 9, 40, 150])
+@pytest.mark.parametrize("dim,bits", FORMS)
+def test_precision_of_every_grouping(dim, bits, rows, dtype):
+    """8 to 1200 query slots of a sequence, on all variants, with a gate: the rounding of the output's type decides."""
+    seqs = [rows + 3, 301, 160]
+    kv = [keys_of(n, 2, dim, dtype, 7 * i + dim) for i, n in enumerate(seqs)]
+    c = Held([k for k, _ in kv], [v for _, v in kv], bits)
+    counts = [rows, max(1, rows - 1), rows]
+    lens = [n - m + 1 + i for n, m in zip(seqs, counts) for i in range(m)]
+    lens[1::7] = [max(1, n - 60) for n in lens[1::7]]   # not all of them causal
+    q = torch.randn(sum(counts), 16, dim, generator=gen(rows), device=DEV).to(dtype)
+    gate = torch.randn(q.shape, generator=gen(rows + 1), device=DEV).to(dtype)
+    got = c.attend(q, counts, lens, dim ** -0.5, gate)
+    assert distance(got, c.exact(q, counts, lens, dim ** -0.5, gate)) < LIMIT
+
+
+@pytest.mark.parametrize("per", [1, 6])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_precision_of_small_groups_of_v(bits, per):
+    """V whose second group is 2^8 smaller: each group's error is its own."""
+    dim, n = 128, 200
+    k, v = keys_of(n, 1, dim, torch.bfloat16, 5)
+    v[..., 64:] *= 2.0 ** -8
+    c = Held([k], [v], bits)
+    q = torch.randn(per, 16, dim, generator=gen(2), device=DEV).to(torch.bfloat16)
+    got, want = c.attend(q, [per], [n] * per, 0.09), c.exact(q, [per], [n] * per, 0.09)
+    for part in (slice(0, 64), slice(64, 128)):
+        assert distance(got[..., part], want[..., part]) < LIMIT
+
+
+# ------------------------------------------------------------------- what rows may depend on
+def larger(x, at, size):
+    """The same rows, but the one at `at` is `size` times as large."""
+    y = x.clone()
+    y[at] = y[at] * size
+    return y
+
+
+def unseen_keys_change_nothing(which, dim, bits, rows):
+    """A key inside the sequence that only its last row sees, ever larger: every other row's bits stay."""
+    n = 120
+    k, v = keys_of(n, 1, dim, torch.bfloat16, dim + rows)
+    q = torch.randn(rows, 8, dim, generator=gen(rows), device=DEV).to(torch.bfloat16)
+    lens = [n - rows + 1 + i for i in range(rows)]
+    lens[0] = 20   # and one row far from the others
+    plain = Held([k], [v], bits).attend(q, [rows], lens, 0.08)
+    for size in (2.0 ** 8, 2.0 ** 14, 2.0 ** 20, 2.0 ** 60):
+        c = Held([larger(k, n - 1, size) if which == "k" else k], [larger(v, n - 1, size) if which == "v" else v], bits)
+        assert torch.equal(c.attend(q, [rows], lens, 0.08)[:-1], plain[:-1]), size
+    c = Held([larger(k, 30, 2.0 ** 20)], [larger(v, 30, 2.0 ** 20)], bits)
+    assert torch.equal(c.attend(q, [rows], lens, 0.08)[0], plain[0])
+
+
+def large_keys_of_no_weight_change_little(size, dim, bits, rows):
+    """Keys that all rows see with a weight of 0, K and V far larger: the others keep their precision."""
+    n = 120
+    k, v = keys_of(n, 1, dim, torch.bfloat16, dim + rows)
+    q = torch.randn(rows, 8, dim, generator=gen(rows), device=DEV).abs().to(torch.bfloat16)
+    for at in (3, 70, 71):
+        k[at] = -size * (1 + k[at].float().abs()).to(torch.bfloat16)   # a score far below every other
+        v[at] = v[at] * size
+    c = Held([k], [v], bits)
+    assert distance(c.attend(q, [rows], [n] * rows, 0.08), c.exact(q, [rows], [n] * rows, 0.08)) < LIMIT
+
+
+@pytest.mark.parametrize("rows", [6, 40])
+@pytest.mark.parametrize("dim,bits", FORMS)
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_unseen_keys_of_many_rows(which, dim, bits, rows):
+    unseen_keys_change_nothing(which, dim, bits, rows)
+
+
+@pytest.mark.parametrize("rows", [6, 40])
+@pytest.mark.parametrize("dim,bits", FORMS)
+@pytest.mark.parametrize("size", [2.0 ** 12, 2.0 ** 20, 2.0 ** 40])
+def test_large_keys_of_many_rows(size, dim, bits, rows):
+    large_keys_of_no_weight_change_little(size, dim, bits, rows)
