@@ -555,9 +555,11 @@ __device__ __forceinline__ void stage_step(State<S>& st, const uint8_t* in, cons
           }
       }
   }
-  // V's scales: the largest exponent among this lane's keys bounds them all.  The bits of a scale grow with it;
-  // a poisoned one is negative.
-  int top = 0x1F800000;   // 2^-64
+  // V's scales: the largest exponent among this lane's keys bounds them all, and tells whether a reference may have to
+  // move.  The bits of a scale grow with it; a poisoned one is negative.
+  constexpr int FLOOR = 0x1F800000;   // 2^-64
+  const auto exponent = [](int bits) { return __uint_as_float(0x4B000000u | (uint32_t)(bits >> 23)) - (8388608.f + 127.f); };
+  int top = FLOOR;
   int longest = 0;
   if (MASK) {   // what stands behind the sequence may be anything
 #pragma unroll
@@ -572,8 +574,7 @@ __device__ __forceinline__ void stage_step(State<S>& st, const uint8_t* in, cons
       for (int gi = 0; gi < NG; ++gi)
         if (!MASK || key0 + kb * 16 + 2 * g + r < longest) top = max(top, (int)(sz[kb][r * NG + gi] << 16));
   }
-  const float ex = __uint_as_float(0x4B000000u | (uint32_t)(top >> 23)) - (8388608.f + 127.f);
-  float most[NT][2];
+  const float ex = exponent(top);
   bool move = false;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -589,20 +590,35 @@ __device__ __forceinline__ void stage_step(State<S>& st, const uint8_t* in, cons
           sc[kb][n][2 * r + j] = x;
           m = fmaxf(m, x);
         }
-      most[n][j] = m + ex;
-      move = move || most[n][j] > st.ref[n][j] + SLACK;
+      move = move || m + ex > st.ref[n][j] + SLACK;
     }
   if (__any_sync(0xffffffff, move)) {
+    // A slot's reference moves for what the slot sees, every key with its own exponent: a large value that it does not see,
+    // or that has no weight, leaves the others their bits.
+    float own[KB][2];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        int x = FLOOR;
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi) x = max(x, (int)(sz[kb][r * NG + gi] << 16));
+        own[kb][r] = exponent(x);
+      }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float m = most[n][j];
+        float m = -INFINITY;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) m = fmaxf(m, sc[kb][n][2 * r + j] + own[kb][r]);
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, x));
-        m = fmaxf(m, st.ref[n][j]);
-        const float f = m == st.ref[n][j] ? 1.f : ex2(st.ref[n][j] - m);
-        st.ref[n][j] = m;
+        const bool grow = m > st.ref[n][j] + SLACK;
+        const float f = grow ? ex2(st.ref[n][j] - m) : 1.f;
+        if (grow) st.ref[n][j] = m;
         st.l[n][j] *= f;
 #pragma unroll
         for (int gi = 0; gi < NG; ++gi) st.oz[gi][n][j] *= f;

@@ -145,3 +145,17 @@ def test_unseen_keys_of_many_rows(which, dim, bits, rows):
 @pytest.mark.parametrize("size", [2.0 ** 12, 2.0 ** 20, 2.0 ** 40])
 def test_large_keys_of_many_rows(size, dim, bits, rows):
     large_keys_of_no_weight_change_little(size, dim, bits, rows)
+
+
+@pytest.mark.parametrize("rows", [2, 3])
+@pytest.mark.parametrize("dim,bits", FORMS)
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_unseen_keys_of_few_rows(which, dim, bits, rows):
+    unseen_keys_change_nothing(which, dim, bits, rows)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3])
+@pytest.mark.parametrize("dim,bits", FORMS)
+@pytest.mark.parametrize("size", [2.0 ** 12, 2.0 ** 20, 2.0 ** 40])
+def test_large_keys_of_few_rows(size, dim, bits, rows):
+    large_keys_of_no_weight_change_little(size, dim, bits, rows)
