@@ -458,7 +458,7 @@ struct Shape {
   static constexpr int ITEMS = 2 * NG, ITEM = 9;
   static constexpr int JOIN = ITEMS * (WARPS - 1) * ITEM * 128;
   static constexpr int BARS = WARPS * MAX_RING * 8;
-  static constexpr int FIXED = BARS + SLOTS * (NG + 2) * 4 + KS * NT * 256 + 2 * WARPS * SLOTS * 4 + JOIN;
+  static constexpr int FIXED = BARS + SLOTS * (NG + 2) * 4 + KS * NT * 256 + 3 * WARPS * SLOTS * 4 + JOIN;
 };
 
 struct Piece {
@@ -470,7 +470,8 @@ struct Piece {
 // one of its dims (g's).
 template <class S>
 struct State {
-  float o[S::KS][S::NT][4], oz[S::NG][S::NT][2], l[S::NT][2], ref[S::NT][2];
+  float o[S::KS][S::NT][4], oz[S::NG][S::NT][2], l[S::NT][2];
+  float ref[S::NT][2], lift[S::NT][2];   // the reference's score, and LIFT + ABOVE minus its rest
   float fac[S::NT][2];
   int lens[S::NT][2];
 };
@@ -590,7 +591,7 @@ __device__ __forceinline__ void stage_step(State<S>& st, const uint8_t* in, cons
           sc[kb][n][2 * r + j] = x;
           m = fmaxf(m, x);
         }
-      move = move || m + ex > st.ref[n][j] + SLACK;
+      move = move || (m - st.ref[n][j]) + (ex + st.lift[n][j]) > LIFT + ABOVE + SLACK;
     }
   if (__any_sync(0xffffffff, move)) {
     // A slot's reference moves for what the slot sees, every key with its own exponent: a large value that it does not see,
@@ -609,16 +610,26 @@ __device__ __forceinline__ void stage_step(State<S>& st, const uint8_t* in, cons
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float m = -INFINITY;
+        // fmaxf takes no NaN: -inf - -inf, where neither a key nor a reference is there.
+        const auto most = [&](float from, bool with_own) {
+          float m = -INFINITY;
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
+          for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int r = 0; r < 2; ++r) m = fmaxf(m, sc[kb][n][2 * r + j] + own[kb][r]);
+            for (int r = 0; r < 2; ++r) m = fmaxf(m, (sc[kb][n][2 * r + j] - from) + (with_own ? own[kb][r] : 0.f));
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, x));
-        const bool grow = m > st.ref[n][j] + SLACK;
-        const float f = grow ? ex2(st.ref[n][j] - m) : 1.f;
-        if (grow) st.ref[n][j] = m;
+          for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffff, m, x));
+          return m;
+        };
+        const float at = st.ref[n][j], lift = st.lift[n][j];
+        const float to = fmaxf(at, most(0.f, false)), rest = most(to, true);
+        const bool grow = (to - at) + (rest + lift) > LIFT + ABOVE + SLACK;
+        const float to_lift = fminf(lift + (to - at), LIFT + ABOVE - rest);
+        const float f = grow ? ex2((at - to) + (to_lift - lift)) : 1.f;
+        if (grow) {
+          st.ref[n][j] = to;
+          st.lift[n][j] = to_lift;
+        }
         st.l[n][j] *= f;
 #pragma unroll
         for (int gi = 0; gi < NG; ++gi) st.oz[gi][n][j] *= f;
@@ -635,9 +646,8 @@ __device__ __forceinline__ void stage_step(State<S>& st, const uint8_t* in, cons
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        // A masked score is -inf; where the reference still is too, the difference would be NaN.  The powers of two come last:
-        // beside a large reference they would be lost.
-        float p = ex2(sc[kb][n][j] - st.ref[n][j & 1] + (LIFT + ABOVE));
+        // A masked score is -inf; where the reference still is too, the difference would be NaN.
+        float p = ex2((sc[kb][n][j] - st.ref[n][j & 1]) + st.lift[n][j & 1]);
         if (MASK && key0 + kb * 16 + 2 * g + (j >> 1) >= st.lens[n][j & 1]) p = 0.f;
         sc[kb][n][j] = p;
         st.l[n][j & 1] += p;
@@ -769,8 +779,8 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
   float* qfac = qsum + NG * SLOTS;                                // [SLOTS]
   int* qlen = reinterpret_cast<int*>(qfac + SLOTS);               // [SLOTS]
   uint8_t* qfrag = reinterpret_cast<uint8_t*>(qlen + SLOTS);      // [KS][NT][32 lanes][8 bytes]
-  float* refs = reinterpret_cast<float*>(qfrag + KS * NT * 256);  // [WARPS][SLOTS] reference, then l
-  float* sums = refs + 2 * WARPS * SLOTS;                         // [ITEMS][WARPS - 1][ITEM][32]
+  float* refs = reinterpret_cast<float*>(qfrag + KS * NT * 256);  // [WARPS][SLOTS] score of the reference, its rest, l
+  float* sums = refs + 3 * WARPS * SLOTS;                         // [ITEMS][WARPS - 1][ITEM][32]
   uint8_t* stage0 = smem + a.ring_offset + warp * ring * S::STAGE_BYTES;
 
   // The CTA's stages go piece by piece; the walker is the one thread that looks the next one up (n = 0: none).
@@ -932,6 +942,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
         for (int i = 0; i < NG; ++i) st.oz[i][n][j] = 0.f;
         st.l[n][j] = 0.f;
         st.ref[n][j] = -INFINITY;
+        st.lift[n][j] = LIFT + ABOVE;
         st.lens[n][j] = qlen[n * 8 + 2 * t + j];
         st.fac[n][j] = qfac[n * 8 + 2 * t + j];
         shortest = min(shortest, st.lens[n][j]);
@@ -960,7 +971,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
     if (cur.n > 0) start(cur);
     // All warps' sums of a slot are brought to the largest reference and added by an item's owner, which also writes them.
     const size_t rec = (size_t)done.chunk * a.num_kv_heads + done.head + b;
-    float* to = a.partial + rec * SLOTS * (D + 2);
+    float* to = a.partial + rec * SLOTS * (D + RECORD_REST);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -969,8 +980,10 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffff, l, x);
         if (g == 0) {
-          refs[warp * SLOTS + n * 8 + 2 * t + j] = st.ref[n][j];
-          refs[(WARPS + warp) * SLOTS + n * 8 + 2 * t + j] = l;
+          float* mine = refs + warp * SLOTS + n * 8 + 2 * t + j;
+          mine[0] = st.ref[n][j];
+          mine[WARPS * SLOTS] = -st.lift[n][j];
+          mine[2 * WARPS * SLOTS] = l;
         }
       }
     __syncthreads();
@@ -980,14 +993,18 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int s = n * 8 + 2 * t + j;
-        float top = -INFINITY, l = 0.f;
+        const auto of_warp = [&](int w) { return Reference{refs[w * SLOTS + s], refs[(WARPS + w) * SLOTS + s]}; };
+        Reference top{LOWEST, LOWEST};
+        float l = 0.f;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, refs[w * SLOTS + s]);
-        f[j] = st.ref[n][j] == top ? 1.f : ex2(st.ref[n][j] - top);
+        for (int w = 0; w < WARPS; ++w) top.score = fmaxf(top.score, of_warp(w).score);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) top.rest = fmaxf(top.rest, (of_warp(w).score - top.score) + of_warp(w).rest);
+        f[j] = factor_to(Reference{st.ref[n][j], -st.lift[n][j]}, top);
         if (warp == 0 && g == 0 && s < done.count) {
 #pragma unroll
-          for (int w = 0; w < WARPS; ++w) l += refs[(WARPS + w) * SLOTS + s] * (refs[w * SLOTS + s] == top ? 1.f : ex2(refs[w * SLOTS + s] - top));
-          *reinterpret_cast<float2*>(to + SLOTS * D + 2 * s) = make_float2(top, l);
+          for (int w = 0; w < WARPS; ++w) l += refs[(2 * WARPS + w) * SLOTS + s] * factor_to(of_warp(w), top);
+          *reinterpret_cast<float4*>(to + SLOTS * D + RECORD_REST * s) = make_float4(top.score, top.rest, l, 0.f);
         }
       }
       if (n > 0) __syncthreads();   // the tile before has been added up
@@ -1074,23 +1091,26 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const QuantAttnAr
       const long long p0 = e.before + (long long)kvh * e.stages, p1 = p0 + e.stages - 1;
       const int first = (int)(((p0 + 1) * B - 1) / total);
       n = (int)(((p1 + 1) * B - 1) / total) - first + 1;
-      rec += ((size_t)chunk * a.num_kv_heads + kvh + first) * a.chunk * (D + 2);
+      rec += ((size_t)chunk * a.num_kv_heads + kvh + first) * a.chunk * (D + RECORD_REST);
     }
   }
-  const size_t step = (size_t)PARTS * a.chunk * (D + 2);
-  rec += part * (size_t)a.chunk * (D + 2);
+  const size_t step = (size_t)PARTS * a.chunk * (D + RECORD_REST);
+  rec += part * (size_t)a.chunk * (D + RECORD_REST);
   const int mine = n > part ? (n - part + PARTS - 1) / PARTS : 0;
-  float m = -INFINITY, l = 0.f, o[PER];
+  Reference m{LOWEST, LOWEST};
+  float l = 0.f, o[PER];
 #pragma unroll
   for (int j = 0; j < PER; ++j) o[j] = 0.f;
   for (int i0 = 0; i0 < mine; i0 += 32) {
-    float2 ml = make_float2(-INFINITY, 0.f);
-    if (i0 + lane < mine) ml = *reinterpret_cast<const float2*>(rec + (i0 + lane) * step + a.chunk * D + 2 * at);
-    const float top = fmaxf(m, warp_max(ml.x));
-    const float f = m == top ? 1.f : ex2(m - top);
-    const float w = ml.x == top ? 1.f : ex2(ml.x - top);
+    float4 ml = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    if (i0 + lane < mine) ml = *reinterpret_cast<const float4*>(rec + (i0 + lane) * step + a.chunk * D + RECORD_REST * at);
+    const Reference own{ml.x, ml.y};
+    Reference top;
+    top.score = fmaxf(m.score, warp_max(own.score));
+    top.rest = fmaxf(fmaxf(LOWEST, (m.score - top.score) + m.rest), warp_max((own.score - top.score) + own.rest));
+    const float f = factor_to(m, top), w = factor_to(own, top);
     m = top;
-    l = l * f + warp_sum(i0 + lane < mine ? w * ml.y : 0.f);
+    l = l * f + warp_sum(w * ml.z);
 #pragma unroll
     for (int j = 0; j < PER; ++j) o[j] *= f;
     const int cnt = min(32, mine - i0);
@@ -1124,26 +1144,29 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const QuantAttnAr
     }
   }
   if (PARTS > 1) {
-    __shared__ float all[JOIN_WARPS][D + 2];
-    float(*parts)[D + 2] = all + warp / PARTS * PARTS;
+    __shared__ float all[JOIN_WARPS][D + 3];
+    float(*parts)[D + 3] = all + warp / PARTS * PARTS;
 #pragma unroll
     for (int j = 0; j < PER; ++j) parts[part][j * 32 + lane] = o[j];
     if (lane == 0) {
-      parts[part][D] = m;
-      parts[part][D + 1] = l;
+      parts[part][D] = m.score;
+      parts[part][D + 1] = m.rest;
+      parts[part][D + 2] = l;
     }
     __syncthreads();
     if (part != 0) return;
-    m = -INFINITY;
+    m = Reference{LOWEST, LOWEST};
 #pragma unroll
-    for (int x = 0; x < PARTS; ++x) m = fmaxf(m, parts[x][D]);
+    for (int x = 0; x < PARTS; ++x) m.score = fmaxf(m.score, parts[x][D]);
+#pragma unroll
+    for (int x = 0; x < PARTS; ++x) m.rest = fmaxf(m.rest, (parts[x][D] - m.score) + parts[x][D + 1]);
     l = 0.f;
 #pragma unroll
     for (int j = 0; j < PER; ++j) o[j] = 0.f;
 #pragma unroll
     for (int x = 0; x < PARTS; ++x) {
-      const float w = parts[x][D] == m ? 1.f : ex2(parts[x][D] - m);
-      l += w * parts[x][D + 1];
+      const float w = factor_to(Reference{parts[x][D], parts[x][D + 1]}, m);
+      l += w * parts[x][D + 2];
 #pragma unroll
       for (int j = 0; j < PER; ++j) o[j] = fmaf(w, parts[x][j * 32 + lane], o[j]);
     }

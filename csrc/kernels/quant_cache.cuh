@@ -45,6 +45,17 @@ __device__ __forceinline__ float ex2(float x) {   // 2^x, results below 2^-126 a
 // A row's sum of weights and its sum of weights times offsets are held 2^ABOVE larger, so that they leave 32 bits at neither
 // end of what V may be.
 constexpr float LIFT = 6.f, SLACK = 8.f, ABOVE = 24.f, BELOW = 0x1p-24f;
+// The reference is in two parts, a score and what V's scales add to it, both in log2: beside a score of 2^25 the other would be
+// lost, and with it the bound.  A weight is 2^((score - reference's score) + (rest)), whose first difference is exact where
+// it counts.
+struct Reference {
+  float score, rest;   // score -inf: no key yet
+};
+constexpr float LOWEST = -0x1p126f;   // below every reference's parts, and finite: its distance to -inf is a number
+// What sums held against `a` are multiplied by to be held against `top`, which is not below it and not below LOWEST.
+__device__ __forceinline__ float factor_to(const Reference& a, const Reference& top) { return ex2((a.score - top.score) + (a.rest - top.rest)); }
+// A record: a slot's sums of V's dims for all slots of a unit, then for each slot its reference, its sum of weights and nothing.
+constexpr int RECORD_REST = 4;
 constexpr float MAX_QUERY = 0x1p101f;   // a slot with a query of this size gives NaN
 
 struct Chunk {          // 32 bytes

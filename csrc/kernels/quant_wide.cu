@@ -21,7 +21,7 @@
 // A poisoned group of V (NaN) is 0 in the image; the slots that see its key note it, and their dims of the
 // group become NaN in the record.  So nothing of a masked key reaches a slot: its bits are the same whatever stands there.
 //
-// Measured (us, 16 q heads, 2 kv heads of 256 dims, 4 bits): 128 sequences of up to 2300 keys with 4 rows 107, three
+// Measured (us, 16 q heads, 2 kv heads of 256 dims, 4 bits): 128 sequences of up to 2300 keys with 4 rows 109, three
 // chunks of up to 700 rows that see up to 4500 keys 211 (0.52 PFLOP/s of products).  A tile takes some 2900 cycles with 256 dims
 // and 1900 with 64, of which the products are 1000 and 260.  With 256 dims the converters (16384 pairs of numbers
 // a tile) and the softmax share the issue slots; with 64 it is the softmax's chain: scores 360, agreement of the four warps 190, weights 840 (four warps of a scheduler take their 64
@@ -510,8 +510,10 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
         big = fmaxf(fmaxf(s.top[0][slot], s.top[1][slot]), fmaxf(s.top[2][slot], s.top[3][slot]));
         slots_sync(quarter);
         const int e = 13 - min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 100);
-        const float up = big < MAX_QUERY ? copysignf(__uint_as_float((uint32_t)(e + 127) << 23), a.sm_scale) : NAN;
-        fac = fminf(fabsf(a.sm_scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - K_SMALL_LOG - e) << 23), 0x1p126f);
+        const float size = a.sm_scale == 0.f ? 0.f : copysignf(__uint_as_float((uint32_t)(e + 127) << 23), a.sm_scale);
+        const float up = big < MAX_QUERY ? size : NAN;
+        fac = fabsf(a.sm_scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - K_SMALL_LOG - e) << 23);
+        fac = fminf(fmaxf(fac, 0x1p-126f), 0x1p126f);   // its product with the distance to no reference is infinite
         if (busy) {
 #pragma unroll
           for (int c = 0; c < D / 32; c += 2) {
@@ -546,7 +548,8 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
         next_limit = plan.lens[row_of(next)];
         asm volatile("prefetch.global.L2 [%0];" ::"l"(query_of(next)));
       }
-      float ref = -INFINITY, l = 0.f;
+      // The reference's score is kept as it stands before `fac`, so that the largest one's difference to it is exactly 0.
+      float ref = -INFINITY, rest = 0.f, l = 0.f;
       uint32_t bad = 0;
       for (int t = 0; t < p.n; ++t, ++i) {
         const int b = i & 1, valid = limit - (p.first + t) * WIDE_KEYS - part * TOK;
@@ -555,62 +558,97 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
         const float4* k_unit = reinterpret_cast<const float4*>(s.k_unit[i % UNITS] + part * TOK);
         const float4* v_log = reinterpret_cast<const float4*>(s.v_log[i % UNITS] + part * TOK);
         const float4* v_inv = reinterpret_cast<const float4*>(s.v_inv[i % UNITS] + part * TOK);
-        uint32_t r[16];   // scores and log2 of V's units
-        float most = -INFINITY;
+        uint32_t r[16];
         if (busy) {
-          tmem_ld_32x32b_x16(lanes + b * 64 + part * 16, r);
-          tmem_ld_wait();
-          const float2 fac2 = make_float2(fac, fac);
-#pragma unroll
-          for (int j = 0; j < 16; j += 4) {
-            const float4 k = k_unit[j / 4], v = v_log[j / 4];
-            const float2 lo = fma_two(mul_two(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), make_float2(k.x, k.y)), fac2, make_float2(v.x, v.y));
-            const float2 hi = fma_two(mul_two(make_float2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])), make_float2(k.z, k.w)), fac2, make_float2(v.z, v.w));
-            r[j] = __float_as_uint(lo.x);
-            r[j + 1] = __float_as_uint(lo.y);
-            r[j + 2] = __float_as_uint(hi.x);
-            r[j + 3] = __float_as_uint(hi.y);
-          }
-          if (__any_sync(0xffffffff, valid < 16)) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (j >= valid) r[j] = 0xFF800000u;
-          }
-          float x[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-          for (int j = 0; j < 16; ++j) x[j & 1] = fmaxf(x[j & 1], __uint_as_float(r[j]));
-          most = fmaxf(x[0], x[1]);
-        }
-        // Does a slot's reference have to move?
-        if (busy && slots_any(quarter, used && most > ref + SLACK)) {
-          s.top[part][slot] = most;
-          slots_sync(quarter);
-          most = fmaxf(fmaxf(s.top[0][slot], s.top[1][slot]), fmaxf(s.top[2][slot], s.top[3][slot]));
-          const bool grow = used && most > ref + SLACK;
-          const float shrink = grow ? ex2(ref - most) : 1.f;
-          if (grow) {
-            l *= shrink;
-            ref = most;
-          }
-          if (t > 0 && __any_sync(0xffffffff, grow)) {
-            wait_for(s, &s.o_full[b ^ 1], ((i - 1) >> 1) & 1, a.err);   // O holds every tile before this one
-            tc_fence_after();
-#pragma unroll 1
-            for (int c = 0; c < D / 4; c += 8) {
-              uint32_t o[8];
-              const uint32_t at = lanes + TMEM_O + part * (D / 4) + c;
-              tmem_ld_x8(at, o);
+          // A reference that has to move takes the largest score first, then what V's units add to the scores against it.  It is
+          // set at a piece's first tile and looked at again at each other: two turns there where one has to move.
+          bool raise = t == 0, grow = used && raise;
+          for (;;) {
+            const auto key_scores = [&]() {
+              tmem_ld_32x32b_x16(lanes + b * 64 + part * 16, r);
               tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * shrink);
-              tmem_st_x8(at, o);
+              for (int j = 0; j < 16; j += 4) {
+                const float4 k = k_unit[j / 4];
+                const float2 lo = mul_two(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), make_float2(k.x, k.y));
+                const float2 hi = mul_two(make_float2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])), make_float2(k.z, k.w));
+                r[j] = __float_as_uint(lo.x);
+                r[j + 1] = __float_as_uint(lo.y);
+                r[j + 2] = __float_as_uint(hi.x);
+                r[j + 3] = __float_as_uint(hi.y);
+              }
+            };
+            const auto largest = [&]() {   // of the keys that the slot sees
+              if (__any_sync(0xffffffff, valid < 16)) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                  if (j >= valid) r[j] = 0xFF800000u;
+              }
+              float x[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+              for (int j = 0; j < 16; ++j) x[j & 1] = fmaxf(x[j & 1], __uint_as_float(r[j]));
+              return fmaxf(x[0], x[1]);
+            };
+            const auto of_all = [&](float x) {   // the largest of the four blocks'
+              s.top[part][slot] = x;
+              slots_sync(quarter);
+              x = fmaxf(fmaxf(s.top[0][slot], s.top[1][slot]), fmaxf(s.top[2][slot], s.top[3][slot]));
+              slots_sync(quarter);
+              return x;
+            };
+            const float was = rest;
+            float moved = 0.f;
+            if (raise) {
+              key_scores();
+              const float score = of_all(largest());
+              if (grow && score > ref) {   // the same reference from another score
+                moved = (score - ref) * fac;
+                ref = score;
+              }
             }
-            tmem_st_wait();
+            key_scores();
+            const float2 fac2 = make_float2(fac, fac), from = make_float2(-ref, -ref);
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+              const float4 v = v_log[j / 4];
+              const float2 x = fma_two(add_two(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), from), fac2,
+                                       j & 2 ? make_float2(v.z, v.w) : make_float2(v.x, v.y));
+              r[j] = __float_as_uint(x.x);
+              r[j + 1] = __float_as_uint(x.y);
+            }
+            float most = largest();
+            if (!raise) {
+              if (!slots_any(quarter, used && most > rest + SLACK)) break;
+              most = of_all(most);   // by every thread: it has barriers
+              grow = used && most > rest + SLACK;
+              raise = true;
+              continue;
+            }
+            most = of_all(most);
+            float shrink = 1.f;
+            if (grow) {
+              rest = fmaxf(was - moved, most);
+              shrink = ex2((was - moved) - rest);
+              l *= shrink;
+            }
+            if (t > 0 && __any_sync(0xffffffff, grow)) {
+              wait_for(s, &s.o_full[b ^ 1], ((i - 1) >> 1) & 1, a.err);   // O holds every tile before this one
+              tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < D / 4; c += 8) {
+                uint32_t o[8];
+                const uint32_t at = lanes + TMEM_O + part * (D / 4) + c;
+                tmem_ld_x8(at, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * shrink);
+                tmem_st_x8(at, o);
+              }
+              tmem_st_wait();
+            }
+            break;
           }
-          slots_sync(quarter);   // the maxima have been read
-        }
-        if (busy) {
-          const float off = ref == -INFINITY ? 0.f : LIFT - ref;
+          const float off = LIFT - rest;
           float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
           for (int j = 0; j < 16; j += 2) {
@@ -666,7 +704,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
       wait_for(s, &s.o_full[(i - 1) & 1], ((i - 1) >> 1) & 1, a.err);
       tc_fence_after();
       const size_t rec = (size_t)p.chunk * a.num_kv_heads + p.head + cta;
-      float* to = a.partial + rec * WIDE_SLOTS * (D + 2);
+      float* to = a.partial + rec * WIDE_SLOTS * (D + RECORD_REST);
       if (busy) {
         // Column gi 64 + 8 j + perm(g) is dim gi 64 + 8 g + j; the join puts them in order.  8 columns at a time go
         // through shared memory, so that an instruction stores whole sectors.
@@ -691,7 +729,9 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
           if (left > 16) *reinterpret_cast<uint4*>(mine + 16 * D + c) = x1;
           __syncwarp();
         }
-        if (used && part == 0) *reinterpret_cast<float2*>(to + (size_t)WIDE_SLOTS * D + 2 * slot) = make_float2(ref, l);
+        if (used && part == 0)
+          *reinterpret_cast<float4*>(to + (size_t)WIDE_SLOTS * D + RECORD_REST * slot) =
+              make_float4(ref * fac, rest, l, 0.f);
       }
       slots_sync(quarter);   // the poisoned groups have been read
       tc_fence_before();

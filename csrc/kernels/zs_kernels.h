@@ -768,7 +768,7 @@ typedef struct QuantAttnArgs {
   int chunk;                // slots of a unit: 8 * tiles
   int max_chunks;
   void* work;               // zs_quant_attn_work bytes, 32-byte aligned
-  float* partial;           // (max_chunks * kv_heads + ZS_QUANT_CTAS) * chunk * (dim + 2)
+  float* partial;           // (max_chunks * kv_heads + ZS_QUANT_CTAS) * chunk * (dim + 4)
   void* out;                // [rows, heads * dim] like q, or NULL
   uint8_t* out_q;           // MXFP8 of the same, or NULL
   uint8_t* out_sf;

@@ -159,3 +159,26 @@ def test_unseen_keys_of_few_rows(which, dim, bits, rows):
 @pytest.mark.parametrize("size", [2.0 ** 12, 2.0 ** 20, 2.0 ** 40])
 def test_large_keys_of_few_rows(size, dim, bits, rows):
     large_keys_of_no_weight_change_little(size, dim, bits, rows)
+
+
+@pytest.mark.parametrize("rows", [1, 20])
+@pytest.mark.parametrize("dim,bits", FORMS)
+@pytest.mark.parametrize("v_size", [2.0 ** -30, 1.0, 2.0 ** 30, 2.0 ** 90])
+def test_scores_of_any_size(dim, bits, rows, v_size):
+    """Scores of about 2^26, 2^40 and 2^80: one key of each row leads by far more than its score's error, and its V is the
+    result, whatever V's size: half a step of bf16 (2^-8), and half a step of f16 (2^-11) each for a weight and a value, or 2^-16
+    of the largest scale of its token, which is below 2^-2 of the largest value."""
+    n = 150
+    k, v = keys_of(n, 1, dim, torch.bfloat16, dim)
+    v = (v.float() * v_size).to(torch.bfloat16)
+    c = Held([k], [v], bits)
+    for size in (2.0 ** 24, 2.0 ** 38, 2.0 ** 78):
+        q = (size * torch.randn(rows, 8, dim, generator=gen(rows), device=DEV)).to(torch.bfloat16)
+        x = torch.einsum("rhd,nd->rhn", q.double(), held(k, bits)[:, 0])
+        lead = x.topk(2, -1).values
+        sure = (lead[..., 0] - lead[..., 1]) > 2.0 ** -10 * x.abs().amax(-1)
+        assert sure.float().mean() > 0.8
+        got, want = c.attend(q, [rows], [n] * rows, 0.08), c.exact(q, [rows], [n] * rows, 0.08)
+        err = (got.double() - want).abs()
+        top = want.abs().amax(-1, keepdim=True)
+        assert bool((err <= (2.0 ** -8 + 2.0 ** -10) * want.abs() + 2.0 ** -18 * top)[sure].all())
