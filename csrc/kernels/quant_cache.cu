@@ -787,22 +787,25 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
   const long long hi = total * (b + 1) / B;
   long long pos = total * b / B;
   const bool walker = threadIdx.x == 32;
+  // A plan for units of more slots, in longer stages, is walked by a row of CTAs for each SLOTS of a unit.
+  const int part = blockIdx.y * SLOTS, per_stage = a.stage / S::KEYS;
   auto walk = [&](Piece* p) {
     Piece x = {};
-    if (pos < hi) {
+    while (pos < hi && x.n == 0) {
       Chunk e = plan.table[chunk];
       while (e.before + (long long)e.stages * a.num_kv_heads <= pos) e = plan.table[++chunk];
-      const int r = (int)(pos - e.before);
+      const int r = (int)(pos - e.before), first = r % e.stages, n = (int)min((long long)(e.stages - first), hi - pos);
+      pos += n;
+      if (e.count <= part) continue;
       x.chunk = chunk;
       x.head = r / e.stages;
-      x.first = r % e.stages;
-      x.n = (int)min((long long)(e.stages - x.first), hi - pos);
+      x.first = first * per_stage;
+      x.n = min((first + n) * per_stage, (e.len + S::KEYS - 1) / S::KEYS) - x.first;
       x.row = e.row;
       x.slot = e.slot;
-      x.slot0 = e.first;
-      x.count = e.count;
+      x.slot0 = e.first + part;
+      x.count = min(SLOTS, e.count - part);
       x.len = e.len;
-      pos += x.n;
     }
     *p = x;
   };
@@ -879,6 +882,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
 
   int use = 0, use_phase = 0;   // the ring's place to be read
   Piece cur = pieces[0];
+  if (cur.n == 0) return;   // none of the CTA's units has so many slots
   start(cur);
   for (int k = 0;; ++k) {
     if (walker) walk(&pieces[(k + 1) & 1]);
@@ -971,7 +975,8 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
     if (cur.n > 0) start(cur);
     // All warps' sums of a slot are brought to the largest reference and added by an item's owner, which also writes them.
     const size_t rec = (size_t)done.chunk * a.num_kv_heads + done.head + b;
-    float* to = a.partial + rec * SLOTS * (D + RECORD_REST);
+    float* to = a.partial + rec * a.chunk * (D + RECORD_REST) + part * D;
+    float* to_rest = a.partial + rec * a.chunk * (D + RECORD_REST) + a.chunk * D + part * RECORD_REST;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -1004,7 +1009,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
         if (warp == 0 && g == 0 && s < done.count) {
 #pragma unroll
           for (int w = 0; w < WARPS; ++w) l += refs[(2 * WARPS + w) * SLOTS + s] * factor_to(of_warp(w), top);
-          *reinterpret_cast<float4*>(to + SLOTS * D + RECORD_REST * s) = make_float4(top.score, top.rest, l, 0.f);
+          *reinterpret_cast<float4*>(to_rest + RECORD_REST * s) = make_float4(top.score, top.rest, l, 0.f);
         }
       }
       if (n > 0) __syncthreads();   // the tile before has been added up
@@ -1222,9 +1227,13 @@ int row_blocks(QuantRowsArgs& a) {
   return (int)((some * a.step + ROW_WARPS - 1) / ROW_WARPS);
 }
 
-// More slots of a sequence than this go to quant_wide.cu.  Measured with 64 sequences of 4096 keys, 2 kv heads, 4 bits,
-// bf16, in us, here : there.  256 dims: 16 slots 67 : 87, 24 slots 111 : 87.  128 dims: 32 slots 65 : 68, 40 slots 114 : 69.
-// 64 dims: 32 slots 39 : 63, 40 slots 64 : 63.
+// More slots of a sequence than this go to quant_wide.cu.  Measured with 64 sequences of 4096 keys and 2 kv heads, in us: here
+// with the most slots of one unit : there with 40 slots (nearly the same from 17 to 64) : here with two units.
+//             4 bits, bf16        8 bits, bf16        4 bits, f16
+//   64 dims   40 :  74 :  79      42 :  71 :  84      46 :  80 :  93
+//   128 dims  74 :  79 : 148      83 :  79 : 166      94 :  88 : 187
+//   256 dims  72 : 101 : 143      76 : 124 : 153      88 : 109 : 176
+// (two units are twice one).  f16 over 8 bits stays here however many slots there are: launch_bits.
 constexpr int most_narrow(int d) { return d == 256 ? 16 : 32; }
 
 // The variant for sequences of so many query slots.
@@ -1255,11 +1264,11 @@ int launch_attend(QuantAttnArgs a, cudaStream_t stream) {
   a.ring_offset = (S::FIXED + 127) & ~127;
   a.ring = (room - a.ring_offset) / (S::WARPS * S::STAGE_BYTES);
   if (a.ring > MAX_RING) a.ring = MAX_RING;
-  if (a.ring < 1 || a.chunk != S::SLOTS || a.stage != S::KEYS) return -1;
+  if (a.ring < 1 || a.chunk % S::SLOTS != 0 || a.stage % S::KEYS != 0) return -1;
   const int bytes = a.ring_offset + S::WARPS * a.ring * S::STAGE_BYTES;
   const auto kernel = attend_kernel<S>;
   cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  zs_launch(kernel, a.grid, S::WARPS * 32, bytes, stream, a);
+  zs_launch(kernel, dim3(a.grid, a.chunk / S::SLOTS), S::WARPS * 32, bytes, stream, a);
   return launch_join<S::D, false>(a, stream);
 }
 
@@ -1280,6 +1289,10 @@ int launch_tiles(const QuantAttnArgs& a, cudaStream_t stream) {
 template <int D>
 int launch_bits(const QuantAttnArgs& a, cudaStream_t stream) {
   if (a.chunk == WIDE_SLOTS) {
+    // f16 outputs over 8 bits: quant_wide.cu rounds K and V to f16, which costs more there than the outputs' own rounding (1.6
+    // to 1.8 of it altogether; 1.25 with 4 bits, whose values need fewer bits).  Every unit of 128 slots is then walked by parts:
+    // 64 sequences of 4096 keys, 2 heads of 256 dims, 128 slots 629 us (155 there), of 64 dims 179 (81 there).
+    if (a.half && a.bits == 8) return launch_variant<D, 8, most_narrow(D), true>(a, stream);
     const int e = launch_wide(a, stream);
     return e ? e : launch_join<D, true>(a, stream);
   }

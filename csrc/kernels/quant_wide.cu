@@ -7,7 +7,8 @@
 // once for all slots and shared memory is read once for it:
 //  * copy warp: page ids, then one bulk copy per 16-token block into a ring of tiles;
 //  * 14 converter warps, each at a block, its K and then its V: s n + z as one f16 fused multiply-add of two
-//    numbers, rounded once (2^-12 of a value).  (w & 0x000F000F) is two subnormals n 2^-24 and the factor s 2^24,
+//    numbers, rounded once (by up to 2^-11 of a value: less than what bf16 outputs are rounded by; of 4 bits it leaves
+//    f16 outputs within 1.25 of their own rounding, and those over 8 bits do not come here).  (w & 0x000F000F) is two subnormals n 2^-24 and the factor s 2^24,
 //    so a pair costs an integer instruction, a part of a shift and the multiply-add.  A power of two per token
 //    (its unit) brings its largest scale to [2^-9, 2^-8), which keeps s 2^24 and every value in f16's range whatever their
 //    size (an offset is below 2^19 of its group's scale), and no token's precision depends on another; K's unit goes to
@@ -218,6 +219,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
   const int B = ctas_of(total, gridDim.x, a.least), cta = blockIdx.x;
   const bool work = cta < B && total > 0;
   const int group = a.num_q_heads / a.num_kv_heads;
+  const bool half = BITS == 4 && a.half;
   // Every role walks the CTA's pieces by itself.
   long long pos = work ? total * cta / B : 0;
   const long long hi = work ? total * (cta + 1) / B : 0;
@@ -310,7 +312,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
 #pragma unroll
         for (int k = 0; k < WIDE_KEYS / 16; ++k)
           mma_step(tmem + TMEM_O, tmem + b * 64 + k * 16, v_lo + b * W::V_IMAGE / 16 + k * 2, idesc_o, !fresh || k > 0);
-        if (a.half) {
+        if (half) {
 #pragma unroll
           for (int k = 0; k < WIDE_KEYS / 16; ++k)   // what the rounding of P left
             mma_step(tmem + TMEM_O, tmem + b * 64 + k * 16 + 8, v_lo + b * W::V_IMAGE / 16 + k * 2, idesc_o, true);
@@ -500,7 +502,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
           const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const float2 f = two_floats(w[k], a.half);
+            const float2 f = two_floats(w[k], half);
             big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
             nan = fmaf(f.x, 0.f, fmaf(f.y, 0.f, nan));
           }
@@ -524,7 +526,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
               float x[8];
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                const float2 f = two_floats(w[k], a.half);
+                const float2 f = two_floats(w[k], half);
                 x[2 * k] = f.x * up;
                 x[2 * k + 1] = f.y * up;
               }
@@ -669,7 +671,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
             pk[j] = pack_f16(__uint_as_float(r[k]), __uint_as_float(r[k + 2]));
           }
           tmem_st_x8(lanes + b * 64 + part * 16, pk);
-          if (a.half) {
+          if (half) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const int k = (j >> 1) * 4 + (j & 1);
@@ -757,7 +759,7 @@ int launch(const QuantAttnArgs& a, cudaStream_t stream) {
 }  // namespace
 
 int launch_wide(QuantAttnArgs a, cudaStream_t stream) {
-  if (a.chunk != WIDE_SLOTS || a.stage != WIDE_KEYS || a.grid > 148) return -1;
+  if (a.chunk != WIDE_SLOTS || a.stage != WIDE_KEYS || a.grid > 148 || (a.half && a.bits == 8)) return -1;
   if (a.head_dim == 64) return a.bits == 4 ? launch<64, 4>(a, stream) : launch<64, 8>(a, stream);
   if (a.head_dim == 128) return a.bits == 4 ? launch<128, 4>(a, stream) : launch<128, 8>(a, stream);
   return a.bits == 4 ? launch<256, 4>(a, stream) : launch<256, 8>(a, stream);

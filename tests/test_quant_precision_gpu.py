@@ -67,7 +67,7 @@ class Held:
 
 
 # ------------------------------------------------------------------------------------ precision
-@pytest.mark.parametrize("dtype", [torch.bfloat16])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("rows", [1, 2, 5, 9, 40, 150])
 @pytest.mark.parametrize("dim,bits", FORMS)
 def test_precision_of_every_grouping(dim, bits, rows, dtype):
