@@ -35,6 +35,9 @@ def prompt_lookup(tokens: list[int], k: int, window: int = 3) -> list[int]:
 
 
 class ParallelSampler:
+    """``runner``: one of an attention-only model.  Over a quantised cache (``kv_bits`` 8 or 4) samples share their
+    prompt's pages too, but every sample's rows read them for themselves."""
+
     def __init__(self, runner: Qwen35Runner, num_drafts: int = 3):
         if runner.cfg.gdn_layers:
             raise ValueError("forks copy pages, not recurrent state: the model must have attention layers only")
@@ -49,7 +52,7 @@ class ParallelSampler:
         self.tokens: dict[int, list[int]] = {}   # sample slot -> prompt and generated tokens
         self.prompt_of: dict[int, int] = {}      # sample slot -> its prompt's slot
         self.prompt_pages: dict[int, int] = {}   # prompt slot -> pages that its samples share
-        self.plan = self.verifier = self._plan_key = None   # of the first step on
+        self.plan = self.verifier = self._plan_key = None   # of the first step on (no plan over a quantised cache)
 
     def _ints(self, x) -> torch.Tensor:
         return torch.tensor(x, dtype=torch.int32, device=self.r.dev)
@@ -113,23 +116,30 @@ class ParallelSampler:
             self.prompt_of[s] = p
         return kids
 
-    def _plan(self, slots: list[int]) -> SharedPrefixPlan:
-        """Who shares what: changes only when samples end or start."""
+    def _plan(self, slots: list[int]) -> SharedPrefixPlan | None:
+        """Who shares what: changes only when samples end or start.  None where the cache is quantised."""
         key = tuple((s, self.prompt_of[s], self.prompt_pages[self.prompt_of[s]]) for s in slots)
         if self._plan_key != key:
-            rows = [s for s in slots for _ in range(self.k + 1)]
-            groups: dict[int, list[int]] = {}
-            for i, s in enumerate(rows):
-                groups.setdefault(self.prompt_of[s], []).append(i)
-            prefixes = [(members, self.prompt_pages[p]) for p, members in groups.items()]
-            self.plan = SharedPrefixPlan.from_prefixes(rows, prefixes, self.r.hq, self.r.hkv, device=self.r.dev)
+            if self.r.kv_bits == 16:
+                rows = [s for s in slots for _ in range(self.k + 1)]
+                groups: dict[int, list[int]] = {}
+                for i, s in enumerate(rows):
+                    groups.setdefault(self.prompt_of[s], []).append(i)
+                prefixes = [(members, self.prompt_pages[p]) for p, members in groups.items()]
+                self.plan = SharedPrefixPlan.from_prefixes(rows, prefixes, self.r.hq, self.r.hkv, device=self.r.dev)
             self.verifier = DraftVerifier(len(slots), self.k, self.r.cfg.vocab_size, device=self.r.dev)
             self._plan_key = key
         return self.plan
 
+    def _check_attention(self) -> None:
+        parts = [self.plan] if self.plan is not None else [] if self.r.quant is None else [self.r.quant, *self.r.quant_plans.values()]
+        for x in parts:
+            x.check()
+
     def logits(self, slots: list[int], drafts: list[list[int]], shared: bool = True) -> torch.Tensor:
         """f32 logits [len(slots), k + 1, vocab] after the newest token of each sample and after each of its
-        drafts (missing drafts are padded with token 0)."""
+        drafts (missing drafts are padded with token 0).  ``shared`` False: every sample's rows read the prompt's
+        pages for themselves."""
         r, k1, n = self.r, self.k + 1, len(slots)
         self._current()
         if len(drafts) != n or any(len(d) > self.k for d in drafts):
@@ -172,7 +182,7 @@ class ParallelSampler:
                                       torch.rand(n, k1, generator=generator, device=dev),
                                       counts=self._ints([len(d) for d in drafts])).tolist()
         self.verifier.check()
-        self.plan.check()
+        self._check_attention()
         new = [rec[1:1 + rec[0]] for rec in record]
         for s, t in zip(slots, new):
             self.tokens[s] += t
@@ -184,9 +194,9 @@ class ParallelSampler:
         """End samples: their pages go back and the live ones move together.  Returns their tokens."""
         if len(set(slots)) != len(slots) or any(s not in self.tokens for s in slots):
             raise ValueError(f"not all of {slots} are samples, each once")
-        for x in (self.plan, self.verifier):
-            if x is not None:
-                x.check()
+        self._check_attention()
+        if self.verifier is not None:
+            self.verifier.check()
         self.pool.free(self._ints(slots))
         self.pool.compact()
         self.pool.check()
