@@ -1177,12 +1177,13 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const QuantAttnAr
     }
   }
   if (at_item != item) return;
-  // A row without keys gives 0; one whose weights are all 0 (scores of -inf) or NaN gives NaN.
+  // A row without keys gives 0, whatever its gate; one whose weights are all 0 (scores of -inf) or NaN gives NaN.
   const float inv = 1.f / l;
+  const bool some = n > 0 && len > 0;
   float y[PER];
 #pragma unroll
-  for (int j = 0; j < PER; ++j) y[j] = n > 0 && len > 0 ? o[j] * inv : 0.f;
-  if (a.gate != nullptr) {
+  for (int j = 0; j < PER; ++j) y[j] = some ? o[j] * inv : 0.f;
+  if (a.gate != nullptr && some) {
 #pragma unroll
     for (int j = 0; j < PER / 2; ++j) {
       const float2 f = two_floats(gate[j], a.half);

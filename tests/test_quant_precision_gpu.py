@@ -182,3 +182,31 @@ def test_scores_of_any_size(dim, bits, rows, v_size):
         err = (got.double() - want).abs()
         top = want.abs().amax(-1, keepdim=True)
         assert bool((err <= (2.0 ** -8 + 2.0 ** -10) * want.abs() + 2.0 ** -18 * top)[sure].all())
+
+
+# ------------------------------------------------------------------------------ rows without keys
+@pytest.mark.parametrize("rows", [1, 9, 40])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_rows_without_keys_are_0_whatever_their_gate(bits, rows):
+    """Rows of no keys and of no sequence, as padding leaves them: queries and gates of any kind, MXFP8 output too."""
+    from zstep_b200.ops import mx
+
+    dim, n = 128, 50
+    k, v = keys_of(n, 2, dim, torch.bfloat16, 3)
+    c = Held([k], [v], bits)
+    q = torch.randn(rows + 2, 16, dim, generator=gen(rows), device=DEV).to(torch.bfloat16)
+    gate = torch.randn(q.shape, generator=gen(rows + 1), device=DEV).to(torch.bfloat16)
+    for r, bad in ((0, float("nan")), (rows, float("inf")), (rows + 1, float("nan"))):
+        q[r], gate[r] = bad, bad
+    lens = [0] + [n] * rows + [n]
+    plan = QuantAttention(c.cache, 16, max_rows=rows + 2, max_seqs=1, max_seq_rows=rows + 1)
+    plan.update(i32([0] * (rows + 2)), i32(lens), i32([0, rows]))   # the last two rows are of no sequence
+    out = torch.full((rows + 2, 16 * dim), 7.0, dtype=torch.bfloat16, device=DEV)
+    out_q = torch.full((128, 16 * dim), 9, dtype=torch.uint8, device=DEV)
+    out_sf = torch.zeros(mx.atoms_bytes(rows + 2, 16 * dim), dtype=torch.uint8, device=DEV)
+    plan.attend(0, q, c.table, 0.09, gate=gate, out=out, out_q=out_q, out_sf=out_sf)
+    plan.check()
+    got = mx.dequantize(out_q[:rows + 2], mx.codes_from_atoms(out_sf, rows + 2, 16 * dim))
+    for r in (0, rows, rows + 1):
+        assert not out[r].any() and not got[r].any()
+    assert bool(out.isfinite().all()) and bool(got.isfinite().all())
