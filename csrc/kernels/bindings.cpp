@@ -3,6 +3,7 @@
 // Each binding validates devices/dtypes/contiguity, converts tensors to raw pointers
 // and calls the C ABI in zs_kernels.h on the current CUDA stream.  Any non-zero return
 // code raises, so a missing or rejected kernel is never silently replaced.
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -1174,6 +1175,9 @@ void quant_rows(bool store, const QuantCacheState& c, int64_t layer, const Tenso
   const auto type = k.scalar_type();
   TORCH_CHECK(type == v.scalar_type() && (type == at::kBFloat16 || type == at::kHalf || (!store && type == at::kFloat)),
               "k and v must both be bf16 or both f16", store ? "" : " or both f32");
+  if (!store) {   // rows written, each to a place of its own
+    for (const Tensor* t : {&k, &v}) TORCH_CHECK(at::has_internal_overlap(*t) != at::MemOverlap::Yes, "rows to read into must not share memory");
+  }
   if (rows == 0) return;
   const at::cuda::CUDAGuard guard(c.data.device());
   a.num_pages = (int)c.data.size(1);
@@ -1222,7 +1226,7 @@ struct QuantPlanState {
     const int64_t group = q_heads / c.heads;
     TORCH_CHECK_VALUE(max_rows < (1ll << 28) && max_rows * q_heads < (1ll << 28) && max_seqs < (1ll << 24), "too many rows or sequences for a plan");
     QuantAttnArgs& a = base;
-    zs_quant_attn_shape(c.dim, c.bits, (int)std::min<int64_t>(group * max_seq_rows, 1 << 20), &a.tiles, &a.stage);
+    zs_quant_attn_shape(c.dim, c.bits, (int)std::min<int64_t>(group * std::min<int64_t>(max_seq_rows, 1 << 20), 1 << 20), &a.tiles, &a.stage);
     a.chunk = 8 * a.tiles;
     const int64_t of_seq = (group * std::min(max_seq_rows, max_rows) + a.chunk - 1) / a.chunk;
     a.max_chunks = (int)std::min(max_seqs + max_rows * group / a.chunk, max_seqs * of_seq);

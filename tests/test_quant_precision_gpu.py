@@ -210,3 +210,19 @@ def test_rows_without_keys_are_0_whatever_their_gate(bits, rows):
     for r in (0, rows, rows + 1):
         assert not out[r].any() and not got[r].any()
     assert bool(out.isfinite().all()) and bool(got.isfinite().all())
+
+
+def test_reads_into_rows_that_share_memory_are_refused():
+    k, v = keys_of(20, 2, 64, torch.bfloat16, 3)
+    c = Held([k], [v], 4)
+    at = i32([0] * 4), i32([1, 2, 3, 4])
+    one, own = torch.zeros(1, 2, 64, dtype=torch.bfloat16, device=DEV), torch.zeros(4, 2, 64, dtype=torch.bfloat16, device=DEV)
+    for shared in (one.expand(4, 2, 64), own[:, :1].expand(4, 2, 64)):
+        for kw in (dict(k=shared, v=own), dict(k=own, v=shared)):
+            with pytest.raises(RuntimeError, match="share memory"):
+                c.cache.read(0, c.table, *at, **kw)
+    # Rows to write from may be one row: a constant prefix, say.
+    c.cache.write(0, one.expand(4, 2, 64), one.expand(4, 2, 64), c.table, *at)
+    assert not c.cache.read(0, c.table, *at)[0].any()
+    c.cache.read(0, c.table, at[0][:1], at[1][:1], k=one, v=own[:1])
+    c.cache.check()
