@@ -1228,13 +1228,13 @@ int row_blocks(QuantRowsArgs& a) {
   return (int)((some * a.step + ROW_WARPS - 1) / ROW_WARPS);
 }
 
-// More slots of a sequence than this go to quant_wide.cu.  Measured with 64 sequences of 4096 keys and 2 kv heads, in us: here
-// with the most slots of one unit : there with 40 slots (nearly the same from 17 to 64) : here with two units.
-//             4 bits, bf16        8 bits, bf16        4 bits, f16
-//   64 dims   40 :  74 :  79      42 :  71 :  84      46 :  80 :  93
-//   128 dims  74 :  79 : 148      83 :  79 : 166      94 :  88 : 187
-//   256 dims  72 : 101 : 143      76 : 124 : 153      88 : 109 : 176
-// (two units are twice one).  f16 over 8 bits stays here however many slots there are: launch_bits.
+// More slots of a sequence than this go to quant_wide.cu (bf16; f16 stays here, in parts: launch_bits).  Measured with 64
+// sequences of 4096 keys and 2 kv heads, in us: here with the most slots of one unit : there with 40 slots (nearly the same from
+// 17 to 64) : here with two units, twice one.
+//             4 bits           8 bits
+//   64 dims   40 :  72 :  80   42 :  71 :  84
+//   128 dims  75 :  77 : 150   83 :  80 : 165
+//   256 dims  72 : 100 : 144   77 : 124 : 154
 constexpr int most_narrow(int d) { return d == 256 ? 16 : 32; }
 
 // The variant for sequences of so many query slots.
@@ -1290,10 +1290,11 @@ int launch_tiles(const QuantAttnArgs& a, cudaStream_t stream) {
 template <int D>
 int launch_bits(const QuantAttnArgs& a, cudaStream_t stream) {
   if (a.chunk == WIDE_SLOTS) {
-    // f16 outputs over 8 bits: quant_wide.cu rounds K and V to f16, which costs more there than the outputs' own rounding (1.6
-    // to 1.8 of it altogether; 1.25 with 4 bits, whose values need fewer bits).  Every unit of 128 slots is then walked by parts:
-    // 64 sequences of 4096 keys, 2 heads of 256 dims, 128 slots 629 us (155 there), of 64 dims 179 (81 there).
-    if (a.half && a.bits == 8) return launch_variant<D, 8, most_narrow(D), true>(a, stream);
+    // f16 outputs: quant_wide.cu rounds K and V to f16, which with the outputs' own rounding gives up to 1.8 times the latter
+    // (for bf16 outputs 1.03).  Every unit of 128 slots is then walked by parts, as exactly as few slots are, and the keys are
+    // opened for each: 64 sequences of 4096 keys, 2 heads, 128 slots take 175, 353 and 620 us with 64, 128 and 256 dims (81, 92
+    // and 129 in bf16).
+    if (a.half) return a.bits == 4 ? launch_variant<D, 4, most_narrow(D), true>(a, stream) : launch_variant<D, 8, most_narrow(D), true>(a, stream);
     const int e = launch_wide(a, stream);
     return e ? e : launch_join<D, true>(a, stream);
   }

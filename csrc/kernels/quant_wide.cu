@@ -7,23 +7,23 @@
 // once for all slots and shared memory is read once for it:
 //  * copy warp: page ids, then one bulk copy per 16-token block into a ring of tiles;
 //  * 14 converter warps, each at a block, its K and then its V: s n + z as one f16 fused multiply-add of two
-//    numbers, rounded once (by up to 2^-11 of a value: less than what bf16 outputs are rounded by; of 4 bits it leaves
-//    f16 outputs within 1.25 of their own rounding, and those over 8 bits do not come here).  (w & 0x000F000F) is two subnormals n 2^-24 and the factor s 2^24,
-//    so a pair costs an integer instruction, a part of a shift and the multiply-add.  A power of two per token
+//    numbers, rounded once (by up to 2^-11 of a value, an eighth of what a bf16 output is).  (w & 0x000F000F) is two
+//    subnormals n 2^-24 and the factor s 2^24, so a pair costs an integer instruction, a part of a shift and the
+//    multiply-add.  A power of two per token
 //    (its unit) brings its largest scale to [2^-9, 2^-8), which keeps s 2^24 and every value in f16's range whatever their
 //    size (an offset is below 2^19 of its group's scale), and no token's precision depends on another; K's unit goes to
 //    the token's scores and V's to its weights, in 32 bits.  K goes to a
 //    swizzled image of keys x dims, V to one of dims x keys (as it is stored), both K-major operands;
 //  * MMA warp: S of the next tile goes before O of this one;
 //  * 16 softmax warps: a thread has a block of a tile for a slot.  The weights 2^(x - reference) are held
-//    below 2^14 with the token's unit of V, as f16 (2^-11; for f16 outputs the rest goes through a second
-//    product); the reference follows the largest score only when that outgrew it by 2^8, and O in TMEM is
-//    rescaled then.
+//    below 2^14 with the token's unit of V, as f16 (2^-11); the reference follows the largest score only when that
+//    outgrew it by 2^8, and O in TMEM is rescaled then.
+// f16 outputs, which all this would cost bits, are left to quant_cache.cu.
 // A poisoned group of V (NaN) is 0 in the image; the slots that see its key note it, and their dims of the
 // group become NaN in the record.  So nothing of a masked key reaches a slot: its bits are the same whatever stands there.
 //
-// Measured (us, 16 q heads, 2 kv heads of 256 dims, 4 bits): 128 sequences of up to 2300 keys with 4 rows 109, three
-// chunks of up to 700 rows that see up to 4500 keys 211 (0.52 PFLOP/s of products).  A tile takes some 2900 cycles with 256 dims
+// Measured (us, 16 q heads, 2 kv heads of 256 dims, 4 bits): 128 sequences of up to 2300 keys with 4 rows 107, three
+// chunks of up to 700 rows that see up to 4500 keys 210 (0.52 PFLOP/s of products).  A tile takes some 2900 cycles with 256 dims
 // and 1900 with 64, of which the products are 1000 and 260.  With 256 dims the converters (16384 pairs of numbers
 // a tile) and the softmax share the issue slots; with 64 it is the softmax's chain: scores 360, agreement of the four warps 190, weights 840 (four warps of a scheduler take their 64
 // exponentials there), handing over 150.  Tried and slower or no faster: tiles taken in turn by two sets of softmax
@@ -219,7 +219,6 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
   const int B = ctas_of(total, gridDim.x, a.least), cta = blockIdx.x;
   const bool work = cta < B && total > 0;
   const int group = a.num_q_heads / a.num_kv_heads;
-  const bool half = BITS == 4 && a.half;
   // Every role walks the CTA's pieces by itself.
   long long pos = work ? total * cta / B : 0;
   const long long hi = work ? total * (cta + 1) / B : 0;
@@ -312,11 +311,6 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
 #pragma unroll
         for (int k = 0; k < WIDE_KEYS / 16; ++k)
           mma_step(tmem + TMEM_O, tmem + b * 64 + k * 16, v_lo + b * W::V_IMAGE / 16 + k * 2, idesc_o, !fresh || k > 0);
-        if (half) {
-#pragma unroll
-          for (int k = 0; k < WIDE_KEYS / 16; ++k)   // what the rounding of P left
-            mma_step(tmem + TMEM_O, tmem + b * 64 + k * 16 + 8, v_lo + b * W::V_IMAGE / 16 + k * 2, idesc_o, true);
-        }
         tc_commit(&s.v_empty[i & 3]);
         tc_commit(&s.o_full[b]);
       }
@@ -496,22 +490,21 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
         uint4 u[D / 32];
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) u[j] = busy ? from[j] : make_uint4(0, 0, 0, 0);
-        float big = 0.f, nan = 0.f;
+        uint32_t bits = 0;   // of the largest magnitudes, which grow with them, infinities and NaN last
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) {
           const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 f = two_floats(w[k], half);
-            big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
-            nan = fmaf(f.x, 0.f, fmaf(f.y, 0.f, nan));
-          }
+          for (int k = 0; k < 4; ++k) bits = __vmaxu2(bits, w[k] & 0x7FFF7FFFu);
         }
-        s.top[part][slot] = nan == 0.f ? big : INFINITY;
+        s.top[part][slot] = __uint_as_float(max(bits << 16, bits & 0xFFFF0000u));
         slots_sync(quarter);
-        big = fmaxf(fmaxf(s.top[0][slot], s.top[1][slot]), fmaxf(s.top[2][slot], s.top[3][slot]));
+        bits = 0;
+#pragma unroll
+        for (int j = 0; j < TBLOCKS; ++j) bits = max(bits, __float_as_uint(s.top[j][slot]));
+        const float big = __uint_as_float(bits);
         slots_sync(quarter);
-        const int e = 13 - min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 100);
+        const int e = 13 - min(max((int)(bits >> 23) - 127, -100), 100);
         const float size = a.sm_scale == 0.f ? 0.f : copysignf(__uint_as_float((uint32_t)(e + 127) << 23), a.sm_scale);
         const float up = big < MAX_QUERY ? size : NAN;
         fac = fabsf(a.sm_scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - K_SMALL_LOG - e) << 23);
@@ -526,7 +519,7 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
               float x[8];
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                const float2 f = two_floats(w[k], half);
+                const float2 f = two_floats(w[k], false);
                 x[2 * k] = f.x * up;
                 x[2 * k + 1] = f.y * up;
               }
@@ -671,15 +664,6 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
             pk[j] = pack_f16(__uint_as_float(r[k]), __uint_as_float(r[k + 2]));
           }
           tmem_st_x8(lanes + b * 64 + part * 16, pk);
-          if (half) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int k = (j >> 1) * 4 + (j & 1);
-              const float2 cut = __half22float2(*reinterpret_cast<const __half2*>(&pk[j]));
-              pk[j] = pack_f16(__uint_as_float(r[k]) - cut.x, __uint_as_float(r[k + 2]) - cut.y);
-            }
-            tmem_st_x8(lanes + b * 64 + part * 16 + 8, pk);
-          }
           tmem_st_wait();
           const uint32_t* poison = s.v_bad[i % UNITS][part];
           if (poison[0] | poison[1]) {
@@ -759,7 +743,7 @@ int launch(const QuantAttnArgs& a, cudaStream_t stream) {
 }  // namespace
 
 int launch_wide(QuantAttnArgs a, cudaStream_t stream) {
-  if (a.chunk != WIDE_SLOTS || a.stage != WIDE_KEYS || a.grid > 148 || (a.half && a.bits == 8)) return -1;
+  if (a.chunk != WIDE_SLOTS || a.stage != WIDE_KEYS || a.grid > 148 || a.half) return -1;
   if (a.head_dim == 64) return a.bits == 4 ? launch<64, 4>(a, stream) : launch<64, 8>(a, stream);
   if (a.head_dim == 128) return a.bits == 4 ? launch<128, 4>(a, stream) : launch<128, 8>(a, stream);
   return a.bits == 4 ? launch<256, 4>(a, stream) : launch<256, 8>(a, stream);

@@ -47,7 +47,7 @@ def attention(q, k, v, lens, scale, gate=None):
 
 
 def distance(got, want):
-    """|got - want| over |want rounded to got's type - want|."""
+    """|got - want| over |want rounded to got's type - want|; 0 where got is want."""
     want = want.reshape(got.shape)
-    alone = (want.to(got.dtype).double() - want).norm()
-    return float((got.double() - want).norm() / alone)
+    off, alone = (got.double() - want).norm(), (want.to(got.dtype).double() - want).norm()
+    return float(off / alone) if off != 0 else 0.0

@@ -84,6 +84,27 @@ def test_precision_of_every_grouping(dim, bits, rows, dtype):
     assert distance(got, c.exact(q, counts, lens, dim ** -0.5, gate)) < LIMIT
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim,bits", FORMS)
+def test_precision_of_mixed_steps(dim, bits, dtype):
+    """Single tokens, sequences without rows or keys, verify rows and chunks in one step; the rest of the cache is poisoned."""
+    seqs, counts = [1200, 40, 16, 333, 200, 1, 64], [1, 37, 0, 2, 130, 1, 1]
+    kv = [keys_of(n, 2, dim, dtype, 11 * i + dim) for i, n in enumerate(seqs)]
+    c = Held([k for k, _ in kv], [v for _, v in kv], bits, page=64)
+    behind = [(s, p) for s, n in enumerate(seqs) for p in range(n, -(-n // 64) * 64)]
+    nan = torch.full((len(behind), 2, dim), float("nan"), dtype=dtype, device=DEV)
+    c.cache.write(0, nan, nan, c.table, i32([s for s, _ in behind]), i32([p for _, p in behind]))
+    lens = [n - m + 1 + i for n, m in zip(seqs, counts) for i in range(m)]
+    lens[-1] = 0
+    q = torch.randn(sum(counts), 16, dim, generator=gen(dim), device=DEV).to(dtype)
+    got, want = c.attend(q, counts, lens, dim ** -0.5), c.exact(q, counts, lens, dim ** -0.5)
+    at = 0
+    for m in counts[:-1]:
+        assert m == 0 or distance(got[at:at + m], want[at:at + m]) < LIMIT
+        at += m
+    assert not got[-1].any()
+
+
 @pytest.mark.parametrize("per", [1, 6])
 @pytest.mark.parametrize("bits", [4, 8])
 def test_precision_of_small_groups_of_v(bits, per):
