@@ -443,7 +443,10 @@ template <int D_, int BITS_, int NT_, int WARPS_, int KB_, int CTAS_, bool FINE_
 struct Shape {
   static constexpr int D = D_, BITS = BITS_, NT = NT_, WARPS = WARPS_, KB = KB_, CTAS = CTAS_;
   static constexpr bool FINE = FINE_;
-  static constexpr int FOLD = FINE ? 2 : 8;         // stages between additions of the offsets' sums
+  // V's numbers all times 16 (see fold_offsets); elsewhere every second one of 4 bits.  What a sum is then multiplied by.
+  static constexpr bool HIGH = FINE && BITS == 4;
+  static constexpr float EVEN = HIGH ? 0x1p44f : 0x1p48f, ODD = BITS == 4 ? 0x1p44f : 0x1p48f;
+  static constexpr int FOLD = FINE ? 1 : 8;         // stages between additions of the offsets' sums
   static constexpr int KS = D / 16;                 // tiles of 16 dims of V
   static constexpr int NG = D / GROUP;
   static constexpr int CODES = code_bytes(D, BITS);
@@ -699,7 +702,13 @@ __device__ __forceinline__ void stage_step(State<S>& st, const uint8_t* in, cons
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint32_t a0, a1, a2, a3;
-        if (BITS == 4) {
+        if (S::HIGH) {
+          const uint32_t x = u[i];
+          a0 = (x << 4) & 0x00F000F0u;
+          a1 = x & 0x00F000F0u;
+          a2 = (x >> 4) & 0x00F000F0u;
+          a3 = (x >> 8) & 0x00F000F0u;
+        } else if (BITS == 4) {
           const uint32_t x = u[i], y = u[i] >> 8;
           a0 = x & 0x000F000Fu;
           a1 = x & 0x00F000F0u;
@@ -734,11 +743,14 @@ __device__ __forceinline__ void stage_step(State<S>& st, const uint8_t* in, cons
 }
 
 // The numbers of V are not negative, so that their sums grow with the keys, and the offsets' sums take most of that away
-// again in the end.  The products cut what they add to a sum behind its 24th bit, always towards zero: over
-// sequences of 65 535 keys, dozens of stages a warp, f16 outputs were off by 0.00047 of their norm instead of the 0.00021
-// of their own rounding.  The offsets' sums are
-// therefore added every FOLD stages, while both are small: 0.00032 every 8 stages, 0.00027 every 2.  For bf16 outputs,
-// whose rounding is 0.0017, 8 are enough (48 -> 49 us for 256 sequences).
+// again in the end.  The products cut what they add to a sum behind some 24 bits, always towards zero, which leaves a bias that
+// the keys add up.  It has two parts, measured for f16 outputs over 65 535 keys as multiples of the outputs' own rounding:
+// how large the sums are when they are added to, so the offsets' sums are added every FOLD stages, while both are small (2.2
+// without, 1.5 every 8 stages, 1.17 every 2, 1.11 every one); and how the products are lined up, by their operands' exponent
+// fields, which for 4-bit numbers as subnormals n 2^-24 are up to 10 bits above them: the low bits of a sum were lost for every
+// dim whose numbers are taken as they are (1.9 for these, 1.004 for those times 16).  f16 outputs take all of V's numbers times 16
+// (1.007 altogether; 64.6 -> 66.5 us for 7 sequences).  For bf16 outputs, whose rounding is eight times as large, FOLD 8 and the
+// cheaper form are enough (1.01).
 template <class S>
 __device__ __forceinline__ void fold_offsets(State<S>& st) {
 #pragma unroll
@@ -753,8 +765,8 @@ __device__ __forceinline__ void fold_offsets(State<S>& st) {
         st.oz[gi][n][j] = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          st.o[gi * 4 + i][n][j] = fmaf(zz, 0x1p-48f, st.o[gi * 4 + i][n][j]);
-          st.o[gi * 4 + i][n][2 + j] = fmaf(zz, S::BITS == 4 ? 0x1p-44f : 0x1p-48f, st.o[gi * 4 + i][n][2 + j]);
+          st.o[gi * 4 + i][n][j] = fmaf(zz, 1.f / S::EVEN, st.o[gi * 4 + i][n][j]);
+          st.o[gi * 4 + i][n][2 + j] = fmaf(zz, 1.f / S::ODD, st.o[gi * 4 + i][n][2 + j]);
         }
       }
 }
@@ -1046,7 +1058,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, S::CTAS) attend_kernel(const Qu
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) zz += __shfl_xor_sync(0xffffffff, zz, x);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = fmaf(v[i], BITS == 4 && (i & 1) ? 0x1p44f : 0x1p48f, zz);
+        for (int i = 0; i < 8; ++i) v[i] = fmaf(v[i], i & 1 ? S::ODD : S::EVEN, zz);
         if (s < done.count) {
           float4* to4 = reinterpret_cast<float4*>(to + s * D + gi * GROUP + g * 8);
           to4[0] = make_float4(v[0], v[1], v[2], v[3]);
@@ -1292,7 +1304,7 @@ int launch_bits(const QuantAttnArgs& a, cudaStream_t stream) {
   if (a.chunk == WIDE_SLOTS) {
     // f16 outputs: quant_wide.cu rounds K and V to f16, which with the outputs' own rounding gives up to 1.8 times the latter
     // (for bf16 outputs 1.03).  Every unit of 128 slots is then walked by parts, as exactly as few slots are, and the keys are
-    // opened for each: 64 sequences of 4096 keys, 2 heads, 128 slots take 175, 353 and 620 us with 64, 128 and 256 dims (81, 92
+    // opened for each: 64 sequences of 4096 keys, 2 heads, 128 slots take 179, 363 and 645 us with 64, 128 and 256 dims (81, 92
     // and 129 in bf16).
     if (a.half) return a.bits == 4 ? launch_variant<D, 4, most_narrow(D), true>(a, stream) : launch_variant<D, 8, most_narrow(D), true>(a, stream);
     const int e = launch_wide(a, stream);

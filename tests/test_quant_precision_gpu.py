@@ -105,6 +105,23 @@ def test_precision_of_mixed_steps(dim, bits, dtype):
     assert not got[-1].any()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_precision_of_long_sequences(dim, bits, dtype):
+    """60 000 keys whose channels have large offsets: what every product cuts from a sum adds up with the keys, and must not
+    show beside the output's rounding, in the dims of either half of a byte."""
+    n = 60000
+    g = gen(dim)
+    k = torch.randn(n, 2, dim, generator=g, device=DEV) + 4 * torch.randn(2, dim, generator=g, device=DEV)
+    v = 0.7 * torch.randn(n, 2, dim, generator=g, device=DEV)
+    c = Held([k.to(dtype)], [v.to(dtype)], bits)
+    q = torch.randn(4, 16, dim, generator=g, device=DEV).to(dtype)
+    got, want = c.attend(q, [4], [n] * 4, dim ** -0.5), c.exact(q, [4], [n] * 4, dim ** -0.5)
+    for half in (slice(0, None, 2), slice(1, None, 2)):
+        assert distance(got[..., half], want[..., half]) < LIMIT
+
+
 @pytest.mark.parametrize("per", [1, 6])
 @pytest.mark.parametrize("bits", [4, 8])
 def test_precision_of_small_groups_of_v(bits, per):
