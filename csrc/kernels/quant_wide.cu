@@ -9,10 +9,11 @@
 //  * 14 converter warps, each at a block, its K and then its V: s n + z as one f16 fused multiply-add of two
 //    numbers, rounded once (by up to 2^-11 of a value, an eighth of what a bf16 output is).  (w & 0x000F000F) is two
 //    subnormals n 2^-24 and the factor s 2^24, so a pair costs an integer instruction, a part of a shift and the
-//    multiply-add.  A power of two per token
-//    (its unit) brings its largest scale to [2^-9, 2^-8), which keeps s 2^24 and every value in f16's range whatever their
-//    size (an offset is below 2^19 of its group's scale), and no token's precision depends on another; K's unit goes to
-//    the token's scores and V's to its weights, in 32 bits.  K goes to a
+//    multiply-add.  A power of two per token (its unit) brings its largest scale to [2^-9, 2^-8), which keeps s 2^24 and
+//    every value in f16's range whatever their size (an offset is below 2^19 of its group's scale), and no token's
+//    precision depends on another; K's unit goes to the token's scores and V's to its weights, in 32 bits.  V's numbers of 4 bits
+//    are all taken times 16 and its scales brought to [2^-5, 2^-4), so that a group 2^12 smaller than the token's largest still has
+//    a step of 2^7 times f16's smallest (two shifts more for four tokens' numbers: verify requests 112 -> 113 us).  K goes to a
 //    swizzled image of keys x dims, V to one of dims x keys (as it is stored), both K-major operands;
 //  * MMA warp: S of the next tile goes before O of this one;
 //  * 16 softmax warps: a thread has a block of a tile for a slot.  The weights 2^(x - reference) are held
@@ -22,8 +23,8 @@
 // A poisoned group of V (NaN) is 0 in the image; the slots that see its key note it, and their dims of the
 // group become NaN in the record.  So nothing of a masked key reaches a slot: its bits are the same whatever stands there.
 //
-// Measured (us, 16 q heads, 2 kv heads of 256 dims, 4 bits): 128 sequences of up to 2300 keys with 4 rows 107, three
-// chunks of up to 700 rows that see up to 4500 keys 210 (0.52 PFLOP/s of products).  A tile takes some 2900 cycles with 256 dims
+// Measured (us, 16 q heads, 2 kv heads of 256 dims, 4 bits): 128 sequences of up to 2300 keys with 4 rows 108, three
+// chunks of up to 700 rows that see up to 4500 keys 211 (0.52 PFLOP/s of products).  A tile takes some 2900 cycles with 256 dims
 // and 1900 with 64, of which the products are 1000 and 260.  With 256 dims the converters (16384 pairs of numbers
 // a tile) and the softmax share the issue slots; with 64 it is the softmax's chain: scores 360, agreement of the four warps 190, weights 840 (four warps of a scheduler take their 64
 // exponentials there), handing over 150.  Tried and slower or no faster: tiles taken in turn by two sets of softmax
@@ -350,6 +351,9 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
         // poisoned groups are.  The softmax reads the units once S is there, which no K is missing from.
 #pragma unroll 1
         for (int is_v = 0; is_v < 2; ++is_v) {
+          // Bits below which the largest scale comes, and what its numbers are f16 subnormals of.
+          const int below = BITS == 4 && is_v ? 4 : 8;
+          const float number = BITS == 4 && is_v ? 0x1p20f : 0x1p24f, most_z = BITS == 4 && is_v ? 0x1p-18f : 0x1p-22f;
           const uint32_t* sz = reinterpret_cast<const uint32_t*>(in + 2 * W::CODES) + is_v * TOK * NG;
           float sf[PAIRS], zf[PAIRS], top = 0.f;
           uint32_t bad[PAIRS];
@@ -364,16 +368,16 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
             if (nan || out) {
               if (is_v) sf[c] = zf[c] = 0.f;
             } else {
-              top = fmaxf(top, fmaxf(sf[c], fabsf(zf[c]) * 0x1p-22f));
+              top = fmaxf(top, fmaxf(sf[c], fabsf(zf[c]) * most_z));
             }
           }
           if (NG > 1) top = fmaxf(top, __shfl_xor_sync(0xffffffff, top, 1));
-          const int e = max((int)(__float_as_uint(top) >> 23) - 127, -72) + 9;
+          const int e = max((int)(__float_as_uint(top) >> 23) - 127, -72) + below + 1;
           const float f1 = __uint_as_float((uint32_t)(127 - (e >> 1)) << 23), f2 = __uint_as_float((uint32_t)(127 - (e - (e >> 1))) << 23);
 #pragma unroll
           for (int c = 0; c < PAIRS; ++c) {
             const int x = lane * PAIRS + c;
-            if (x < TOK * NG) s.pairs[w][is_v][x % NG * TOK + x / NG] = pack_f16(sf[c] * f1 * f2 * 0x1p24f, zf[c] * f1 * f2);
+            if (x < TOK * NG) s.pairs[w][is_v][x % NG * TOK + x / NG] = pack_f16(sf[c] * f1 * f2 * number, zf[c] * f1 * f2);
           }
           if (lane * PAIRS < TOK * NG && lane * PAIRS % NG == 0) {
             const int key = kb * TOK + lane * PAIRS / NG;
@@ -442,15 +446,14 @@ __global__ void __launch_bounds__(THREADS, 1) wide_kernel(const QuantAttnArgs a)
             for (int h = 0; h < BITS / 4; ++h) {
               const uint4 u = lds128(in + W::CODES + gi * (BITS * 128) + h * 512 + lane * 16);
               const uint32_t n[4] = {u.x, u.y, u.z, u.w};
-              const uint32_t T0 = sixteenth(S0), T1 = sixteenth(S1);
 #pragma unroll
               for (int k = 0; k < 4; ++k) {   // 4 bits: dims 2k and 2k + 1; 8 bits: dim 4h + k
-                const uint32_t x = n[k], y = n[k] >> 8;
+                const uint32_t x = n[k];
                 if constexpr (BITS == 4) {
-                  *reinterpret_cast<uint2*>(out + 2 * k * 1024) = make_uint2(fma2(x & 0x000F000Fu, S0, Z0), fma2(y & 0x000F000Fu, S1, Z1));
-                  *reinterpret_cast<uint2*>(out + (2 * k + 1) * 1024) = make_uint2(fma2(x & 0x00F000F0u, T0, Z0), fma2(y & 0x00F000F0u, T1, Z1));
+                  *reinterpret_cast<uint2*>(out + 2 * k * 1024) = make_uint2(fma2((x << 4) & 0x00F000F0u, S0, Z0), fma2((x >> 4) & 0x00F000F0u, S1, Z1));
+                  *reinterpret_cast<uint2*>(out + (2 * k + 1) * 1024) = make_uint2(fma2(x & 0x00F000F0u, S0, Z0), fma2((x >> 8) & 0x00F000F0u, S1, Z1));
                 } else {
-                  *reinterpret_cast<uint2*>(out + (4 * h + k) * 1024) = make_uint2(fma2(x & 0x00FF00FFu, S0, Z0), fma2(y & 0x00FF00FFu, S1, Z1));
+                  *reinterpret_cast<uint2*>(out + (4 * h + k) * 1024) = make_uint2(fma2(x & 0x00FF00FFu, S0, Z0), fma2((x >> 8) & 0x00FF00FFu, S1, Z1));
                 }
               }
             }

@@ -136,6 +136,22 @@ def test_precision_of_small_groups_of_v(bits, per):
         assert distance(got[..., part], want[..., part]) < LIMIT
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("per", [1, 2, 6, 40])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_precision_of_groups_of_many_sizes(bits, per, dtype):
+    """V whose four groups are 1, 2^-4, 2^-8 and 2^-12 times as large: each one's error is its own.  (f16 outputs of the
+    last would be subnormal: V is larger there.)"""
+    dim, n = 256, 200
+    k, v = keys_of(n, 1, dim, dtype, 5)
+    v = v.float() * torch.tensor([1, 2.0 ** -4, 2.0 ** -8, 2.0 ** -12], device=DEV).repeat_interleave(64)
+    c = Held([k], [(v * 2.0 ** 12).to(dtype)], bits)
+    q = torch.randn(per, 16, dim, generator=gen(2), device=DEV).to(dtype)
+    got, want = c.attend(q, [per], [n] * per, 0.06), c.exact(q, [per], [n] * per, 0.06)
+    for part in range(0, dim, 64):
+        assert distance(got[..., part:part + 64], want[..., part:part + 64]) < LIMIT, part
+
+
 # ------------------------------------------------------------------- what rows may depend on
 def larger(x, at, size):
     """The same rows, but the one at `at` is `size` times as large."""
