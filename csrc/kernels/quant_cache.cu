@@ -482,10 +482,12 @@ struct State {
 // Sequences with few slots.  S^T = K Q^T and O^T += V^T P^T on m16n8k16 (a tile of 8 slots is the narrow side, so
 // that 8 slots waste nothing), every warp at its own stages of its own ring of bulk copies: no warp waits for
 // another before the end of a piece.  Measured with the join: 256 sequences of up to 1280 keys, 16 q heads on 2 kv heads
-// of 256 dims, 4 bits 49 us (3.0 TB/s); 61 sequences of up to 4001 keys, 8 heads of 128 dims, 8 bits 72 us (5.6 TB/s); 7
-// sequences of up to 65 535 keys, 32 on 4 heads of 128 dims, 4 bits, f16 59 us (3.6 TB/s; 55 with offsets added every 8 stages, see FOLD).  With 4 bits it is bound by
-// the instructions that open the codes and feed the products, with 8 bits by memory.  e4m3 products for K are emulated here and took 61 -> 70 us; smaller CTAs, and
-// warps of their own for the copies, were no faster.
+// of 256 dims, 4 bits 52 us (2.8 TB/s); 61 sequences of up to 4001 keys, 8 heads of 128 dims, 8 bits 72 us (5.6 TB/s); 7
+// sequences of up to 65 535 keys, 32 on 4 heads of 128 dims, 4 bits, f16 61.5 us (3.5 TB/s).  With 8 bits it is bound by memory.
+// With 4 bits no unit is full (issue slots 50 %, tensor pipe 20 %, DRAM 38 %): the 11 warps that an SM has room for, at 164
+// registers, issue an instruction every 5.5 cycles each, of which 1.4 wait for the one before, 0.6 for another warp's turn, 0.5
+// for shared memory and 0.4 each for the math pipes, the join's barriers and the instructions themselves.  e4m3 products for K
+// are emulated here and took 61 -> 70 us; smaller CTAs, and warps of their own for the copies, were no faster.
 //
 // One stage: the scores of its keys, their weights, and what they add to the sums.  With MASK a key at or
 // behind a slot's length is left out whatever the cache holds there.

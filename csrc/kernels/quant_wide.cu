@@ -24,10 +24,11 @@
 // group become NaN in the record.  So nothing of a masked key reaches a slot: its bits are the same whatever stands there.
 //
 // Measured (us, 16 q heads, 2 kv heads of 256 dims, 4 bits): 128 sequences of up to 2300 keys with 4 rows 108, three
-// chunks of up to 700 rows that see up to 4500 keys 211 (0.52 PFLOP/s of products).  A tile takes some 2900 cycles with 256 dims
-// and 1900 with 64, of which the products are 1000 and 260.  With 256 dims the converters (16384 pairs of numbers
-// a tile) and the softmax share the issue slots; with 64 it is the softmax's chain: scores 360, agreement of the four warps 190, weights 840 (four warps of a scheduler take their 64
-// exponentials there), handing over 150.  Tried and slower or no faster: tiles taken in turn by two sets of softmax
+// chunks of up to 700 rows that see up to 4500 keys 211 (0.52 PFLOP/s of products).  A tile takes some 3000
+// cycles with 256 dims and 1900 with 64, of which the products are 1000 and 260.  No unit is full with 256 dims (issue slots 46 %,
+// tensor pipe 33 %, DRAM 18 %): a tile goes through converters, products, softmax and products again, two at a time.  The four
+// softmax warps of the same 32 slots are on one scheduler, which has all of a verify step's.  With 64 dims it is the softmax's
+// chain: scores 360 cycles, agreement of the four warps 190, weights 840 (64 exponentials of four warps), handing over 150.  Tried and slower or no faster: tiles taken in turn by two sets of softmax
 // warps, blocks given to whichever converter is free, one barrier of all softmax warps, more registers for fewer
 // converters, unrolled conversion loops (they leave the instruction cache: 224 -> 296 us).
 #include "quant_cache.cuh"

@@ -6,6 +6,12 @@ minimum rounded down, s is (maximum - z) / N rounded up, n is (x - z) / s rounde
 (ties to even; 0 where s is 0), and the value held is s n + z.  That is 4.5 or 8.5 bits a value.  A group with a
 NaN, an infinity or a magnitude above 2^126 reads back as NaN.
 
+The attention is that of the values held, in 32 bits, and its output's own rounding decides its error, with two
+exceptions for bf16 queries: weights are rounded to f16 (2^-11), and in steps with many query slots of a sequence
+(rows x q heads of a kv head: more than 32, or 16 with 256 dims) K and V are too, down to 2^-16 (V of 4 bits: 2^-20)
+of their token's largest scale.  What a row does not see changes none of its bits.  Scores may have any size that 32
+bits hold; K or V below 2^-64 in magnitude lose precision.
+
 A ``QuantCache`` is the paged cache of a model's attention layers; a ``QuantAttention`` plans a
 step's attention over it (``update``, once a step) and runs it (``attend``, once a layer).  All
 calls run on the current stream with no host round trip, so a step can be captured in a CUDA
