@@ -1238,7 +1238,7 @@ struct QuantPlanState {
     a.max_seq_rows = (int)std::min<int64_t>(max_seq_rows, 1 << 30);
     const auto bytes = c.data.options();
     work = at::zeros({zs_quant_attn_work(a.max_chunks, a.max_rows, (int)max_seqs)}, bytes);
-    partial = at::empty({((int64_t)a.max_chunks * c.heads + ZS_QUANT_CTAS) * a.chunk * (c.dim + 4)}, bytes.dtype(at::kFloat));
+    partial = at::empty({((int64_t)a.max_chunks * c.heads + ZS_QUANT_CTAS) * a.chunk * (c.dim + ZS_QUANT_REST)}, bytes.dtype(at::kFloat));
     TORCH_CHECK(err.scalar_type() == at::kInt && err.numel() == 1 && err.device() == c.data.device(), "err: int32 [1]");
     a.work = ptr(work);
     a.partial = ptr<float>(partial);

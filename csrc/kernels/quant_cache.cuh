@@ -55,7 +55,7 @@ constexpr float LOWEST = -0x1p126f;   // below every reference's parts, and fini
 // What sums held against `a` are multiplied by to be held against `top`, which is not below it and not below LOWEST.
 __device__ __forceinline__ float factor_to(const Reference& a, const Reference& top) { return ex2((a.score - top.score) + (a.rest - top.rest)); }
 // A record: a slot's sums of V's dims for all slots of a unit, then for each slot its reference, its sum of weights and nothing.
-constexpr int RECORD_REST = 4;
+constexpr int RECORD_REST = ZS_QUANT_REST;
 constexpr float MAX_QUERY = 0x1p101f;   // a slot with a query of this size gives NaN
 
 struct Chunk {          // 32 bytes

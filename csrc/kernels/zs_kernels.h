@@ -723,6 +723,7 @@ int zs_ipc_close(void* ptr);
 // K/V cache held in 4 or 8 bits (quant_cache.cu).  One layer: [pages][kv_heads][page / 16 blocks].
 // ----------------------------------------------------------------------------------
 #define ZS_QUANT_CTAS 592   // most CTAs of zs_quant_attn
+#define ZS_QUANT_REST 4     // numbers of a slot's record beside its dims
 
 typedef struct QuantRowsArgs {
   uint8_t* data;            // the layer
@@ -768,7 +769,7 @@ typedef struct QuantAttnArgs {
   int chunk;                // slots of a unit: 8 * tiles
   int max_chunks;
   void* work;               // zs_quant_attn_work bytes, 32-byte aligned
-  float* partial;           // (max_chunks * kv_heads + ZS_QUANT_CTAS) * chunk * (dim + 4)
+  float* partial;           // (max_chunks * kv_heads + ZS_QUANT_CTAS) * chunk * (dim + ZS_QUANT_REST)
   void* out;                // [rows, heads * dim] like q, or NULL
   uint8_t* out_q;           // MXFP8 of the same, or NULL
   uint8_t* out_sf;
